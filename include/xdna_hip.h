@@ -803,6 +803,75 @@ size_t xdna_colsum_workspace_bytes(const uint16_t* x, int64_t R, int64_t N);
 int xdna_colsum_bf16(const uint16_t* x, uint16_t* out, int64_t R, int64_t N, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Token models: embedding, gated feed-forward, distillation, token log      */
+/* probabilities.  The reference reaches such work only through its          */
+/* zero-copy CPU fallback (torch_xdna_device.cpp:5124-5260).                 */
+/* dtype: 1 fp32, 2 bf16.  index_bytes: 4 or 8 (int32 / int64 indices).      */
+/* Rows may have any stride (ld, in elements) and any element alignment;     */
+/* outputs are dense.  Workspaces are 16-byte aligned.                       */
+/* ------------------------------------------------------------------------ */
+
+/* out[t] = scale * weight[ids[t]], each element rounded once (scale 1: a copy).  weight: vocab
+ * rows of dim, row stride ld.  An id outside the table gives a row of NaN. */
+int xdna_embed(const void* ids, int index_bytes, int64_t tokens, const void* weight, int dtype, int64_t vocab,
+               int64_t dim, int64_t ld, float scale, void* out, void* stream);
+
+/* d_weight[v] = scale * (sum of grad[t] over the tokens with ids[t] == v), every row written,
+ * fp32 sums in token order (equal inputs give equal bits), one rounding.  Ids equal to
+ * `padding` (negative: none) or outside the table are left out.  d_weight is 16-byte aligned. */
+size_t xdna_embed_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim);
+int xdna_embed_bwd(const void* ids, int index_bytes, int64_t tokens, const void* grad, int dtype, int64_t ld,
+                   int64_t vocab, int64_t dim, int64_t padding, float scale, void* d_weight, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* h = act(x Wg^T) * (x Wu^T), M x F, with w = [Wg; Wu] (2F rows of K): both projections (fp32
+ * sums), the activation (0 silu, 1 gelu with erf, 2 relu) and the product in one launch, h
+ * rounded once.  gu (M x 2F, or NULL) keeps [g u] as bf16 for the backward. */
+int xdna_gated_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t M, int64_t K, int64_t F,
+                    int act, uint16_t* h, uint16_t* gu, void* stream);
+
+/* dgu = [dh * u * act'(g), dh * act(g)] (M x 2F) from dh (M x F, row stride ld) and the kept
+ * gu: the gradients of x and w are the products dgu * w and dgu^T * x. */
+int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const uint16_t* gu, int64_t M, int64_t F, int act,
+                        uint16_t* dgu, void* stream);
+
+/* Per row of logits z (row stride ld), x = z / tau, q = softmax(x): log_probs = ln q[target]
+ * (0 for a negative target, NaN past the vocabulary), entropy = -sum q ln q, the `top` (up to
+ * 64) largest logits in order (ties to the lowest index) as ln q and index, and stats = (max z,
+ * 1 / sum exp(x - max x)), two floats a row (8-byte aligned), which the gradient takes.  A row
+ * of -inf only: log probabilities -inf, entropy 0.  vocab up to 2^22. */
+size_t xdna_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top);
+int xdna_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* targets,
+                        int index_bytes, float tau, int top, float* log_probs, float* entropy, float* stats,
+                        float* top_log_probs, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream);
+
+/* d_logits (rows x vocab, dense, of the logits' dtype) from the incoming gradients of
+ * log_probs and entropy (either may be NULL): 0 for a row without incoming gradients, a row of
+ * -inf, and an element of -inf. */
+int xdna_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* targets,
+                            int index_bytes, float tau, const float* stats, const float* entropy,
+                            const float* d_log_probs, const float* d_entropy, void* d_logits, void* stream);
+
+/* Distillation from a teacher's top logits.  Per row: p = softmax(teacher / tau) over its valid
+ * entries (ids >= 0 and a logit above -inf; an id named twice counts as the sum of its
+ * entries), loss = tau^2 sum p (ln p - ln q[id]), q = softmax(logits / tau).  row_share = the
+ * row's weight (weight NULL: 1), 0 where it has no valid entry; row_loss = row_share * loss
+ * (an id past the vocabulary: NaN).  reduction 0: that is all; 1 (mean): loss = sum row_loss /
+ * sum row_share (0 without weights), inv_weight = 1 / that sum; 2: the sum, inv_weight = 1.
+ * stats as above; p: rows x k.  k up to 1024. */
+size_t xdna_distill_workspace_bytes(int64_t rows, int64_t vocab);
+int xdna_distill(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* ids,
+                 int index_bytes, const void* teacher, int teacher_dtype, int k, float tau, const float* weight,
+                 int reduction, float* row_loss, float* row_share, float* stats, float* p, float* loss,
+                 float* inv_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* d_logits = go * row_share * inv_weight (NULL: 1) * tau * (q - p at the entries' tokens); go: a
+ * scalar, or one value per row (go_rows 1), of go_dtype. */
+int xdna_distill_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* ids,
+                     int index_bytes, int k, float tau, const float* row_share, const float* stats, const float* p,
+                     const float* inv_weight, const void* go, int go_dtype, int go_rows, void* d_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

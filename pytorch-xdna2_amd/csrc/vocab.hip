@@ -1,0 +1,887 @@
+// Rows over a vocabulary on gfx950: log probabilities of given tokens with entropy and top
+// alternatives, distillation from a teacher's top logits, and the gradients of both.  The
+// reference reaches such rows only through its zero-copy CPU fallback
+// (torch_xdna_device.cpp:5124-5260).
+//
+// Mathematics, per row of logits z with temperature tau, x = z / tau:
+//   m = max z, s = sum exp((z - m) / tau), q = exp((z - m) / tau) / s;
+//   log probability of token y: (z_y - m) / tau - ln s;
+//   entropy: ln s - u / (tau s), u = sum exp((z - m) / tau) (z - m);
+//   pieces of a row join by m = max m_i, w_i = exp((m_i - m) / tau), s = sum w_i s_i,
+//   u = sum w_i (u_i + (m_i - m) s_i).
+// The gradients take m and 1 / s from the forward: both hold q to a few fp32 roundings,
+// where m / tau + ln s in one number would lose its last bits to the size of m.
+// A row of -inf only has s = 0: log probabilities -inf, entropy 0, gradient 0; an element of
+// -inf adds nothing anywhere (its e (z - m) would be 0 * inf).  NaN and +inf make the row's
+// results NaN.
+//
+// Layout: a workgroup holds a piece of one row in registers (32 elements a thread: all its
+// loads are in flight together, the maximum is known before the first exp and no sum is ever
+// rescaled), so the row is read once also where the largest entries are selected.  Rows
+// longer than a piece, or too few to fill the chip, are cut into pieces whose partial
+// results a second launch joins in piece order; every sum has a fixed order, so equal
+// inputs give equal bits.  The gradient kernels stream: read z, write dz.
+#include "common.h"
+
+#include "../../include/xdna_hip.h"
+
+namespace xdna {
+namespace {
+
+constexpr int kPer = 32;              // elements of a piece per thread
+constexpr int kMaxTop = 64;           // alternatives: one group maximum per lane bounds them
+constexpr int kMaxTeacher = 1024;     // teacher entries per row (held in LDS by the gradient)
+constexpr int64_t kMaxVocab = int64_t(1) << 22;
+constexpr int kCandidates = 1024;     // LDS list of elements that may be among the largest
+constexpr float kLog2e = 1.4426950408889634f;
+
+// VW elements of a 16-byte window (any element-aligned address: global accesses of gfx950
+// take one), as fp32
+template <typename T>
+struct Win;
+template <>
+struct Win<float> {
+  static constexpr int VW = 4;
+};
+template <>
+struct Win<uint16_t> {
+  static constexpr int VW = 8;
+};
+
+struct Raw {
+  uint32_t w[4];
+};
+
+template <typename T>
+__device__ inline float raw_get(const Raw& r, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[e]);
+  return __uint_as_float((e & 1) ? (r.w[e >> 1] & 0xFFFF0000u) : (r.w[e >> 1] << 16));
+}
+
+template <typename T>
+__device__ inline void raw_set(Raw& r, int e, float v) {
+  if constexpr (sizeof(T) == 4) {
+    r.w[e] = __float_as_uint(v);
+  } else {
+    const uint32_t h = f32_to_bf16(v);
+    if (e & 1) r.w[e >> 1] = (r.w[e >> 1] & 0xFFFFu) | (h << 16);
+    else r.w[e >> 1] = (r.w[e >> 1] & 0xFFFF0000u) | h;
+  }
+}
+
+template <typename T>
+__device__ inline float load_one(const T* p) {
+  if constexpr (sizeof(T) == 4) return *p;
+  else return bf16_to_f32(*p);
+}
+
+template <typename T>
+__device__ inline void store_one(T* p, float v) {
+  if constexpr (sizeof(T) == 4) *p = v;
+  else *p = f32_to_bf16(v);
+}
+
+// The window of p: whole, or its first n elements and -inf after them.
+template <typename T>
+__device__ inline Raw load_win(const T* p, int n) {
+  Raw r;
+  if (n >= Win<T>::VW) {
+    const Pix8 q = *reinterpret_cast<const Pix8*>(p);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r.w[k] = q.v[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r.w[k] = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+#pragma unroll
+    for (int e = 0; e < Win<T>::VW; ++e)
+      if (e < n) raw_set<T>(r, e, load_one<T>(p + e));
+  }
+  return r;
+}
+
+template <typename T>
+__device__ inline void store_win(T* p, const Raw& r, int n) {
+  if (n >= Win<T>::VW) {
+    Pix8 q;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q.v[k] = r.w[k];
+    *reinterpret_cast<Pix8*>(p) = q;
+  } else {
+#pragma unroll
+    for (int e = 0; e < Win<T>::VW; ++e)
+      if (e < n) store_one<T>(p + e, raw_get<T>(r, e));
+  }
+}
+
+__device__ inline float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// ---- order of the alternatives: value descending, index ascending ------------------------
+// An unsigned key that grows with the value (-0 as +0, NaN above all, as sorting puts it)
+// over the inverted index: unique per element, and never 0.
+__device__ inline uint32_t order_key(float v) {
+  v = v != v ? __uint_as_float(0x7FC00000u) : v + 0.0f;
+  const uint32_t b = __float_as_uint(v);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ inline float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+__device__ inline uint64_t entry_of(uint32_t key, int idx) { return (uint64_t(key) << 32) | uint32_t(~idx); }
+__device__ inline int entry_index(uint64_t e) { return int(~uint32_t(e)); }
+
+__device__ inline uint64_t shfl64(uint64_t v, int lane) {
+  return (uint64_t(uint32_t(__shfl(int(v >> 32), lane, 64))) << 32) | uint32_t(__shfl(int(uint32_t(v)), lane, 64));
+}
+
+// ---- reductions over a workgroup of NT threads -----------------------------------------------
+template <int NT>
+__device__ inline float block_max(float v, float* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  if constexpr (NT > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, red[w]);
+  }
+  return v;
+}
+
+template <int NT>
+__device__ inline float2 block_sum2(float a, float b, float* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o, 64), b += __shfl_xor(b, o, 64);
+  if constexpr (NT > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[2 * (threadIdx.x >> 6)] = a, red[2 * (threadIdx.x >> 6) + 1] = b;
+    __syncthreads();
+    a = red[0], b = red[1];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) a += red[2 * w], b += red[2 * w + 1];
+  }
+  return make_float2(a, b);
+}
+
+struct RowStat {
+  float m, s, u;
+};
+
+struct LogprobOut {
+  const void* targets;  // [rows] token indices, negative: not scored
+  int index_bytes;
+  float* log_probs;
+  float* entropy;
+  float2* stats;  // [rows] m and 1 / s (0 for a row of -inf)
+  float* top_log_probs;  // [rows][top]
+  int64_t* top_ids;
+  int top;
+};
+
+struct DistillOut {
+  const void* ids;  // [rows][k] token indices, negative: absent
+  int index_bytes;
+  const void* teacher;  // [rows][k] logits, -inf: absent
+  int teacher_dtype;
+  const float* weight;  // [rows] or null: all 1
+  int k;
+  float tau;
+  float2* stats;  // [rows] m and 1 / s
+  float* p;       // [rows][k]
+  float* loss;    // [rows] the row's weighted loss
+  float* share;   // [rows] the row's weight, 0 where it has no valid entry
+};
+
+struct RowArgs {
+  const void* z;
+  int64_t ld;
+  int64_t rows;
+  int V;
+  int piece, pieces;  // elements per piece (a multiple of 8), pieces per row
+  float inv_tau;
+  RowStat* stat;   // [rows][pieces] where pieces > 1
+  uint64_t* list;  // [rows][pieces][top] where pieces > 1
+  LogprobOut lp;
+  DistillOut ds;
+};
+
+enum RowMode { kLogprob = 0, kDistill = 1 };
+
+__device__ inline int64_t index_at(const void* p, int bytes, int64_t i) {
+  return bytes == 8 ? static_cast<const int64_t*>(p)[i] : int64_t(static_cast<const int32_t*>(p)[i]);
+}
+
+// ln q of a logit: (z - m) / tau - ln s, -inf throughout a row of -inf (log_s = ln 0)
+__device__ inline float log_q(const RowStat& st, float log_s, float z, float inv_tau) {
+  return st.s == 0.0f ? -INFINITY : (z - st.m) * inv_tau - log_s;
+}
+
+__device__ inline float2 kept_stats(const RowStat& st) {
+  return st.s == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(st.m, 1.0f / st.s);
+}
+
+// A row's log probability, entropy and kept statistics (one thread).
+template <typename T>
+__device__ inline void logprob_row(const RowArgs& a, int64_t row, const RowStat& st) {
+  const float log_s = logf(st.s);
+  a.lp.stats[row] = kept_stats(st);
+  a.lp.entropy[row] = st.s == 0.0f ? 0.0f : log_s - st.u * a.inv_tau / st.s;
+  const int64_t y = index_at(a.lp.targets, a.lp.index_bytes, row);
+  float v = 0.0f;
+  if (y >= a.V) v = NAN;
+  else if (y >= 0) v = log_q(st, log_s, load_one<T>(static_cast<const T*>(a.z) + row * a.ld + y), a.inv_tau);
+  a.lp.log_probs[row] = v;
+}
+
+__device__ inline void top_store(const RowArgs& a, int64_t row, int rank, uint64_t e, const RowStat& st, float log_s) {
+  a.lp.top_log_probs[row * a.lp.top + rank] = log_q(st, log_s, key_value(uint32_t(e >> 32)), a.inv_tau);
+  a.lp.top_ids[row * a.lp.top + rank] = entry_index(e);
+}
+
+__device__ inline float teacher_at(const DistillOut& d, int64_t i) {
+  return d.teacher_dtype == 1 ? static_cast<const float*>(d.teacher)[i]
+                              : bf16_to_f32(static_cast<const uint16_t*>(d.teacher)[i]);
+}
+
+// A row's distillation loss from its statistics (one wave).
+template <typename T>
+__device__ inline void distill_row(const RowArgs& a, int64_t row, const RowStat& st) {
+  const DistillOut& d = a.ds;
+  const int lane = threadIdx.x & 63;
+  const float log_s = logf(st.s);
+  const int64_t at = row * d.k;
+  float tm = -INFINITY;
+  bool bad = false;
+  for (int j = lane; j < d.k; j += 64) {
+    const int64_t id = index_at(d.ids, d.index_bytes, at + j);
+    bad |= id >= a.V;
+    if (id >= 0 && id < a.V) tm = fmaxf(tm, teacher_at(d, at + j));
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor(tm, o, 64));
+  const float c = a.inv_tau * kLog2e;
+  float ts = 0.0f;
+  bool some = false;
+  for (int j = lane; j < d.k; j += 64) {
+    const int64_t id = index_at(d.ids, d.index_bytes, at + j);
+    const float t = teacher_at(d, at + j);
+    if (id >= 0 && id < a.V && t != -INFINITY) ts += exp2_hw((t - tm) * c), some = true;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) ts += __shfl_xor(ts, o, 64);
+  const float inv = 1.0f / ts, log_ts = logf(ts);
+  float sum = 0.0f;
+  for (int j = lane; j < d.k; j += 64) {
+    const int64_t id = index_at(d.ids, d.index_bytes, at + j);
+    const float t = teacher_at(d, at + j);
+    float p = 0.0f;
+    if (id >= 0 && id < a.V && t != -INFINITY) {
+      p = exp2_hw((t - tm) * c) * inv;
+      const float z = load_one<T>(static_cast<const T*>(a.z) + row * a.ld + id);
+      // p ln(p / q) is 0 where p underflows, also against q = 0
+      if (p != 0.0f) sum += p * (((t - tm) * a.inv_tau - log_ts) - log_q(st, log_s, z, a.inv_tau));
+    }
+    d.p[at + j] = p;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  const bool any_bad = __any(bad), any_some = __any(some);
+  if (lane == 0) {
+    const float w = any_some ? (d.weight ? d.weight[row] : 1.0f) : 0.0f;
+    d.stats[row] = kept_stats(st);
+    d.share[row] = w;
+    d.loss[row] = any_bad ? NAN : w == 0.0f ? 0.0f : w * (d.tau * d.tau) * sum;
+  }
+}
+
+template <int NT>
+struct TopShared {
+  uint64_t best[NT > 64 ? NT / 64 : 1][64];
+  uint64_t cand[kCandidates];
+  uint64_t bound;
+  int count;
+};
+
+// The `top` largest entries of the piece in registers, through `put(rank, entry)`; ranks past
+// the piece's elements get entry 0 where `fill`.
+//   Bound: the top-th largest of 64 group maxima (a group = the threads of equal lane): at
+// least `top` elements reach it, and in rows without special order hardly more.
+//   The elements that reach it go to an LDS list, each candidate's rank is the count of
+// greater ones (entries are unique: no order of arrival matters).
+//   More candidates than the list holds (rows whose largest entries sit in few groups): the
+// exact bound is found by bisection over the entries' 64 bits, counted over the workgroup.
+template <typename T, int NT, typename Put>
+__device__ inline void select_top(const Raw (&r)[kPer / Win<T>::VW], int lo, int len, int top, bool fill,
+                                  TopShared<NT>& sh, float* red, Put put) {
+  constexpr int VW = Win<T>::VW, NW = kPer / VW;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint64_t best = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const int base = (tid + i * NT) * VW;
+    uint32_t bk = 0;
+    int bi = 0;
+#pragma unroll
+    for (int e = 0; e < VW; ++e) {
+      const uint32_t key = base + e < len ? order_key(raw_get<T>(r[i], e)) : 0u;
+      if (key > bk) bk = key, bi = e;
+    }
+    const uint64_t en = bk ? entry_of(bk, lo + base + bi) : 0;
+    best = en > best ? en : best;
+  }
+  if (NT > 64) {
+    sh.best[wave][lane] = best;
+    __syncthreads();
+  }
+  if (wave == 0) {
+    if (NT > 64) {
+#pragma unroll
+      for (int w = 1; w < NT / 64; ++w) best = sh.best[w][lane] > best ? sh.best[w][lane] : best;
+    }
+    int rank = 0;
+    for (int l = 0; l < 64; ++l) {
+      const uint64_t o = shfl64(best, l);
+      rank += o > best ? 1 : 0;
+    }
+    // groups without an element all hold 0: then every element is a candidate
+    const uint64_t hit = __ballot(rank == top - 1 && best != 0);
+    const uint64_t bound = hit ? shfl64(best, __ffsll(static_cast<unsigned long long>(hit)) - 1) : 1;
+    if (lane == 0) sh.bound = bound, sh.count = 0;
+  }
+  __syncthreads();
+  uint64_t bound = sh.bound;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const int base = (tid + i * NT) * VW;
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        if (base + e >= len) continue;
+        const uint64_t en = entry_of(order_key(raw_get<T>(r[i], e)), lo + base + e);
+        if (en >= bound) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kCandidates) sh.cand[at] = en;
+        }
+      }
+    }
+    __syncthreads();
+    if (sh.count <= kCandidates) break;
+    // the largest bound that at least `top` elements reach
+    uint64_t exact = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t trial = exact | (uint64_t(1) << bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        const int base = (tid + i * NT) * VW;
+#pragma unroll
+        for (int e = 0; e < VW; ++e)
+          n += base + e < len && entry_of(order_key(raw_get<T>(r[i], e)), lo + base + e) >= trial ? 1 : 0;
+      }
+      const float2 total = block_sum2<NT>(float(n), 0.0f, red);  // counts below 2^24: exact
+      if (total.x >= float(top)) exact = trial;
+    }
+    bound = exact;
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+  }
+  const int n = min(sh.count, kCandidates);
+  for (int c = tid; c < n; c += NT) {
+    const uint64_t en = sh.cand[c];
+    int rank = 0;
+    for (int o = 0; o < n; ++o) rank += sh.cand[o] > en ? 1 : 0;
+    if (rank < top) put(rank, en);
+  }
+  if (fill)
+    for (int c = n + tid; c < top; c += NT) put(c, uint64_t(0));
+}
+
+// One piece of a row: statistics, and for log probabilities its largest entries; rows of one
+// piece are finished here.
+// Measured: see the launchers' rule below.
+template <typename T, int NT, int MODE, bool TOP>
+__global__ __launch_bounds__(NT) void row_kernel(RowArgs a) {
+  constexpr int VW = Win<T>::VW, NW = kPer / VW;
+  __shared__ float red[2 * (NT / 64)];
+  __shared__ TopShared<TOP ? NT : 64> sh;
+  const int tid = threadIdx.x;
+  const int64_t items = a.rows * a.pieces;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t row = a.pieces == 1 ? item : item / a.pieces;
+    const int pi = a.pieces == 1 ? 0 : int(item - row * a.pieces);
+    const int lo = pi * a.piece;
+    const int len = min(a.piece, a.V - lo);
+    const T* z = static_cast<const T*>(a.z) + row * a.ld + lo;
+    Raw r[NW];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const int at = (tid + i * NT) * VW;
+      r[i] = load_win<T>(z + min(at, len), len - at);
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) m = fmaxf(m, raw_get<T>(r[i], e));
+    m = block_max<NT>(m, red);
+    const float c = a.inv_tau * kLog2e;
+    const float m0 = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        const float d = raw_get<T>(r[i], e) - m0;
+        const float x = exp2_hw(d * c);
+        s += x;
+        // -inf: 0 * a finite number
+        if (MODE == kLogprob) u += x * fmaxf(d, -1.0e30f);
+      }
+    }
+    const float2 su = block_sum2<NT>(s, u, red);
+    const RowStat st = {m, su.x, su.y};
+    if (a.pieces > 1) {
+      if (tid == 0) a.stat[item] = st;
+      if constexpr (TOP) {
+        uint64_t* list = a.list + item * a.lp.top;
+        select_top<T, NT>(r, lo, len, a.lp.top, true, sh, red, [&](int rank, uint64_t e) { list[rank] = e; });
+      }
+    } else if constexpr (MODE == kLogprob) {
+      if (tid == 0) logprob_row<T>(a, row, st);
+      if constexpr (TOP) {
+        const float log_s = logf(st.s);
+        select_top<T, NT>(r, lo, len, a.lp.top, false, sh, red,
+                          [&](int rank, uint64_t e) { top_store(a, row, rank, e, st, log_s); });
+      }
+    } else {
+      if (tid < 64) distill_row<T>(a, row, st);
+    }
+    if (TOP) __syncthreads();  // the next piece reuses the LDS lists
+  }
+}
+
+// Joins the pieces of a row, in piece order: one workgroup of 256 per row.
+constexpr int kJoinEntries = 8192;
+
+template <typename T, int MODE, bool TOP>
+__global__ __launch_bounds__(256) void join_kernel(RowArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint64_t lists[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const float c = a.inv_tau * kLog2e;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const RowStat* stat = a.stat + row * a.pieces;
+    float m = -INFINITY;
+    for (int p = lane; p < a.pieces; p += 64) m = fmaxf(m, stat[p].m);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    float s = 0.0f, u = 0.0f;
+    for (int p = lane; p < a.pieces; p += 64) {
+      const RowStat q = stat[p];
+      if (q.s == 0.0f) continue;  // nothing but -inf
+      const float w = exp2_hw((q.m - m) * c);
+      s += w * q.s;
+      u += w * (q.u + (q.m - m) * q.s);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64), u += __shfl_xor(u, o, 64);
+    const RowStat st = {m, s, u};
+    if constexpr (MODE == kDistill) {
+      if (tid < 64) distill_row<T>(a, row, st);
+    } else {
+      if (tid == 0) logprob_row<T>(a, row, st);
+      if constexpr (TOP) {
+        const int top = a.lp.top, n = a.pieces * top;
+        __syncthreads();
+        for (int i = tid; i < n; i += 256) lists[i] = a.list[row * n + i];
+        __syncthreads();
+        const float log_s = logf(st.s);
+        for (int i = tid; i < n; i += 256) {
+          const uint64_t e = lists[i];
+          if (e == 0) continue;
+          const int mine = i / top;
+          int rank = i - mine * top;
+          // entries greater than e in each other list (sorted descending)
+          for (int p = 0; p < a.pieces && rank < top; ++p) {
+            if (p == mine) continue;
+            const uint64_t* l = lists + p * top;
+            int b = 0, t = top;
+            while (b < t) {
+              const int h = (b + t) >> 1;
+              if (l[h] > e) b = h + 1;
+              else t = h;
+            }
+            rank += b;
+          }
+          if (rank < top) top_store(a, row, rank, e, st, log_s);
+        }
+      }
+    }
+  }
+}
+
+// ---- gradients: one pass, read z, write dz ---------------------------------------------------
+
+struct LogprobBwdArgs {
+  const void* z;
+  int64_t ld;
+  void* dz;  // [rows][V]
+  int64_t rows;
+  int V, piece, pieces;
+  float inv_tau;
+  const void* targets;
+  int index_bytes;
+  const float2* stats;
+  const float* entropy;
+  const float* d_log_probs;  // [rows] or null
+  const float* d_entropy;    // [rows] or null
+};
+
+constexpr int kBwdThreads = 256;
+
+// dz_v = (g (1[v = y] - q_v) - h q_v (ln q_v + H)) / tau, g and h the row's incoming
+// gradients.  Rows without either are written as zeros and not read.
+template <typename T>
+__global__ __launch_bounds__(kBwdThreads) void logprob_bwd_kernel(LogprobBwdArgs a) {
+  constexpr int VW = Win<T>::VW;
+  const int64_t items = a.rows * a.pieces;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t row = a.pieces == 1 ? item : item / a.pieces;
+    const int lo = a.pieces == 1 ? 0 : int(item - row * a.pieces) * a.piece;
+    const int len = min(a.piece, a.V - lo);
+    const T* z = static_cast<const T*>(a.z) + row * a.ld + lo;
+    T* dz = static_cast<T*>(a.dz) + row * a.V + lo;
+    const float2 ms = a.stats[row];
+    const int64_t y64 = index_at(a.targets, a.index_bytes, row);
+    const bool scored = y64 >= 0 && y64 < a.V;
+    const int y = scored ? int(y64) - lo : -1;
+    float g = a.d_log_probs && scored ? a.d_log_probs[row] * a.inv_tau : 0.0f;
+    const float h = a.d_entropy ? a.d_entropy[row] * a.inv_tau : 0.0f;
+    const bool none = (g == 0.0f && h == 0.0f) || ms.y == 0.0f;
+    const float c = a.inv_tau * kLog2e;
+    const float H = a.entropy[row] + logf(ms.y);
+#pragma unroll 4
+    for (int at = int(threadIdx.x) * VW; at < len; at += kBwdThreads * VW) {
+      const int n = len - at;
+      Raw o = {{0u, 0u, 0u, 0u}};
+      if (!none) {
+        const Raw r = load_win<T>(z + at, n);
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          const float d = raw_get<T>(r, e) - ms.x;
+          const float q = exp2_hw(d * c) * ms.y;
+          // q ln q stays 0 at -inf
+          float v = -q * (g + h * (fmaxf(d, -1.0e30f) * a.inv_tau + H));
+          if (at + e == y) v += g;
+          raw_set<T>(o, e, v);
+        }
+      }
+      store_win<T>(dz + at, o, n);
+    }
+  }
+}
+
+struct DistillBwdArgs {
+  const void* z;
+  int64_t ld;
+  void* dz;
+  int64_t rows;
+  int V, piece, pieces;
+  float inv_tau, tau;
+  const void* ids;
+  int index_bytes;
+  int k;
+  const float* p;
+  const float2* stats;
+  const float* share;
+  const float* inv_weight;  // [1]: 1 / sum of the rows' weights, or null: 1
+  const void* go;           // a scalar, or [rows]
+  int go_dtype, go_rows;
+};
+
+// dz_v = coef (q_v - sum over the entries of token v of p), coef = go * share * tau [/ sum of
+// weights].  The piece is written without its teacher entries first; behind the barrier the
+// (few) entries' tokens are written again, each with the sum of all its entries' p, which
+// every one of them computes alike (a row may name a token twice).
+template <typename T>
+__global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(DistillBwdArgs a) {
+  constexpr int VW = Win<T>::VW;
+  __shared__ int ids[kMaxTeacher];
+  __shared__ float ps[kMaxTeacher];
+  const int64_t items = a.rows * a.pieces;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t row = a.pieces == 1 ? item : item / a.pieces;
+    const int lo = a.pieces == 1 ? 0 : int(item - row * a.pieces) * a.piece;
+    const int len = min(a.piece, a.V - lo);
+    const T* z = static_cast<const T*>(a.z) + row * a.ld + lo;
+    T* dz = static_cast<T*>(a.dz) + row * a.V + lo;
+    const int64_t gi = a.go_rows ? row : 0;
+    const float go = a.go_dtype == 1 ? static_cast<const float*>(a.go)[gi]
+                                     : bf16_to_f32(static_cast<const uint16_t*>(a.go)[gi]);
+    const float share = a.share[row];
+    const float2 ms = a.stats[row];
+    const bool none = share == 0.0f || ms.y == 0.0f;
+    const float coef = none ? 0.0f : go * (a.inv_weight ? share * *a.inv_weight : share) * a.tau;
+    for (int j = threadIdx.x; j < a.k; j += kBwdThreads) {
+      const int64_t id = index_at(a.ids, a.index_bytes, row * a.k + j) - lo;
+      ids[j] = id >= 0 && id < len ? int(id) : -1;
+      ps[j] = a.p[row * a.k + j];
+    }
+    const float c = a.inv_tau * kLog2e, cq = coef * ms.y;
+#pragma unroll 4
+    for (int at = int(threadIdx.x) * VW; at < len; at += kBwdThreads * VW) {
+      const int n = len - at;
+      Raw o = {{0u, 0u, 0u, 0u}};
+      if (!none) {
+        const Raw r = load_win<T>(z + at, n);
+#pragma unroll
+        for (int e = 0; e < VW; ++e) raw_set<T>(o, e, cq * exp2_hw((raw_get<T>(r, e) - ms.x) * c));
+      }
+      store_win<T>(dz + at, o, n);
+    }
+    __syncthreads();
+    if (!none)
+      for (int j = threadIdx.x; j < a.k; j += kBwdThreads) {
+        const int id = ids[j];
+        if (id < 0) continue;
+        float p = 0.0f;
+        for (int i = 0; i < a.k; ++i) p += ids[i] == id ? ps[i] : 0.0f;
+        store_one<T>(dz + id, cq * exp2_hw((load_one<T>(z + id) - ms.x) * c) - coef * p);
+      }
+    __syncthreads();
+  }
+}
+
+// loss = sum of the rows' losses [/ sum of their weights], in fixed order (fp64)
+template <bool MEAN>
+__global__ __launch_bounds__(1024) void distill_total_kernel(const float* __restrict__ loss,
+                                                             const float* __restrict__ share, int64_t rows,
+                                                             float* __restrict__ out, float* __restrict__ inv_weight) {
+  __shared__ double red[2][16];
+  double l = 0.0, w = 0.0;
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) l += double(loss[i]), w += double(share[i]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64), w += __shfl_xor(w, o, 64);
+  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = l, red[1][threadIdx.x >> 6] = w;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) l += red[0][i], w += red[1][i];
+    const double inv = !MEAN ? 1.0 : w != 0.0 ? 1.0 / w : 0.0;
+    out[0] = float(MEAN && w == 0.0 && l == l ? 0.0 : l * inv);
+    inv_weight[0] = float(inv);
+  }
+}
+
+// ---- launch plans --------------------------------------------------------------------------------
+
+struct Plan {
+  int threads, piece, pieces;
+};
+
+// Pieces of one row: one piece where a workgroup can hold the row, else pieces of equal
+// length.  Few rows take small workgroups, so that more of them share the work.
+Plan row_plan(int64_t rows, int64_t V, int top) {
+  Plan p;
+  const auto cap = [](int nt) { return int64_t(nt) * kPer; };
+  if (V <= cap(64)) p.threads = 64;
+  else if (V <= cap(256) || rows * ceil_div(V, cap(1024)) < 256) p.threads = 256;
+  else p.threads = 1024;
+  // the join holds every piece's list
+  if (top > 0 && ceil_div(V, cap(p.threads)) * top > kJoinEntries) p.threads = 1024;
+  p.pieces = int(ceil_div(V, cap(p.threads)));
+  p.piece = int(ceil_div(ceil_div(V, int64_t(p.pieces)), int64_t(8)) * 8);
+  p.pieces = int(ceil_div(V, int64_t(p.piece)));
+  return p;
+}
+
+Plan bwd_plan(int64_t V) {
+  Plan p;
+  p.threads = kBwdThreads;
+  p.pieces = int(ceil_div(V, int64_t(16384)));
+  p.piece = int(ceil_div(ceil_div(V, int64_t(p.pieces)), int64_t(8)) * 8);
+  p.pieces = int(ceil_div(V, int64_t(p.piece)));
+  return p;
+}
+
+// A grid's workgroups: its threads stay under 2^32, the kernels stride over the rest.
+unsigned grid_of(int64_t items, int threads) {
+  return unsigned(std::min<int64_t>(items, (int64_t(1) << 31) / threads));
+}
+
+size_t list_offset(int64_t rows, const Plan& p) {
+  return size_t(ceil_div(rows * p.pieces * int64_t(sizeof(RowStat)), int64_t(16))) * 16;
+}
+
+size_t row_workspace(int64_t rows, int64_t V, int top) {
+  const Plan p = row_plan(rows, V, top);
+  if (p.pieces == 1) return 0;
+  return list_offset(rows, p) + size_t(rows) * p.pieces * top * sizeof(uint64_t);
+}
+
+template <typename T, int MODE, bool TOP>
+bool launch_row(const Plan& p, const RowArgs& a, hipStream_t st) {
+  const int64_t items = a.rows * a.pieces;
+  if (p.threads == 64) row_kernel<T, 64, MODE, TOP><<<grid_of(items, 64), 64, 0, st>>>(a);
+  else if (p.threads == 256) row_kernel<T, 256, MODE, TOP><<<grid_of(items, 256), 256, 0, st>>>(a);
+  else row_kernel<T, 1024, MODE, TOP><<<grid_of(items, 1024), 1024, 0, st>>>(a);
+  if (a.pieces > 1) {
+    const size_t lds = TOP ? size_t(a.pieces) * a.lp.top * sizeof(uint64_t) : 0;
+    join_kernel<T, MODE, TOP><<<grid_of(a.rows, 256), 256, lds, st>>>(a);
+  }
+  return true;
+}
+
+bool rows_ok(const char* what, const void* z, int dtype, int64_t rows, int64_t V, int64_t ld, float tau) {
+  std::string why;
+  if (dtype != 1 && dtype != 2) why = "dtype must be 1 (fp32) or 2 (bf16)";
+  else if (rows < 0) why = "negative row count";
+  else if (V < 1 || V > kMaxVocab) why = "vocabulary outside 1 .. 2^22";
+  else if (ld < V) why = "rows overlap";
+  else if (!(tau > 0.0f) || !(tau < INFINITY)) why = "temperature must be positive and finite";
+  else if (rows > (int64_t(1) << 40) / V) why = "too many logits";
+  else if (rows > 0 && !z) why = "null logits";
+  else if (reinterpret_cast<uintptr_t>(z) % (dtype == 1 ? 4 : 2)) why = "misaligned logits";
+  if (why.empty()) return true;
+  set_error(std::string(what) + ": " + why);
+  return false;
+}
+
+int refuse(const char* what, const char* why) {
+  set_error(std::string(what) + ": " + why);
+  return -1;
+}
+
+bool off(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
+bool workspace_ok(const char* what, const void* ws, size_t have, size_t need) {
+  if (!need || (ws && have >= need && (reinterpret_cast<uintptr_t>(ws) & 15) == 0)) return true;
+  refuse(what, "workspace missing, misaligned or too small");
+  return false;
+}
+
+}  // namespace
+}  // namespace xdna
+
+using namespace xdna;
+
+extern "C" {
+
+size_t xdna_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top) {
+  if (rows < 1 || vocab < 1 || vocab > kMaxVocab || top < 0 || top > kMaxTop || rows > (int64_t(1) << 40) / vocab) return 0;
+  return row_workspace(rows, vocab, top);
+}
+
+int xdna_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* targets,
+                        int index_bytes, float tau, int top, float* log_probs, float* entropy, float* stats,
+                        float* top_log_probs, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "xdna_token_logprobs";
+  if (!rows_ok(what, logits, dtype, rows, vocab, ld, tau)) return -1;
+  if (top < 0 || top > kMaxTop || top > vocab) return refuse(what, "top outside 0 .. min(64, vocabulary)");
+  if (index_bytes != 4 && index_bytes != 8) return refuse(what, "indices of 4 or 8 bytes");
+  if (rows == 0) return 0;
+  if (!targets || !log_probs || !entropy || !stats || (top && (!top_log_probs || !top_ids)))
+    return refuse(what, "null operand");
+  if (off(stats, 8)) return refuse(what, "misaligned stats");
+  if (!workspace_ok(what, workspace, workspace_bytes, row_workspace(rows, vocab, top))) return -1;
+  if (!admit_launch(what)) return -1;
+  const Plan p = row_plan(rows, vocab, top);
+  RowArgs a = {};
+  a.z = logits;
+  a.ld = ld;
+  a.rows = rows;
+  a.V = int(vocab);
+  a.piece = p.piece;
+  a.pieces = p.pieces;
+  a.inv_tau = 1.0f / tau;
+  a.stat = static_cast<RowStat*>(workspace);
+  a.list = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + (p.pieces > 1 ? list_offset(rows, p) : 0));
+  a.lp = {targets, index_bytes, log_probs, entropy, reinterpret_cast<float2*>(stats), top_log_probs, top_ids, top};
+  hipStream_t st = as_stream(stream);
+  if (dtype == 1) top ? launch_row<float, kLogprob, true>(p, a, st) : launch_row<float, kLogprob, false>(p, a, st);
+  else top ? launch_row<uint16_t, kLogprob, true>(p, a, st) : launch_row<uint16_t, kLogprob, false>(p, a, st);
+  return check_launch(what);
+}
+
+int xdna_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* targets,
+                            int index_bytes, float tau, const float* stats, const float* entropy,
+                            const float* d_log_probs, const float* d_entropy, void* d_logits, void* stream) {
+  const char* what = "xdna_token_logprobs_bwd";
+  if (!rows_ok(what, logits, dtype, rows, vocab, ld, tau)) return -1;
+  if (index_bytes != 4 && index_bytes != 8) return refuse(what, "indices of 4 or 8 bytes");
+  if (rows == 0) return 0;
+  if (!targets || !stats || !entropy || !d_logits) return refuse(what, "null operand");
+  if (off(stats, 8) || off(d_logits, dtype == 1 ? 4 : 2)) return refuse(what, "misaligned operand");
+  if (!admit_launch(what)) return -1;
+  const Plan p = bwd_plan(vocab);
+  const LogprobBwdArgs a = {logits, ld, d_logits, rows, int(vocab), p.piece, p.pieces, 1.0f / tau, targets, index_bytes,
+                            reinterpret_cast<const float2*>(stats), entropy, d_log_probs, d_entropy};
+  hipStream_t st = as_stream(stream);
+  const unsigned grid = grid_of(rows * p.pieces, kBwdThreads);
+  if (dtype == 1) logprob_bwd_kernel<float><<<grid, kBwdThreads, 0, st>>>(a);
+  else logprob_bwd_kernel<uint16_t><<<grid, kBwdThreads, 0, st>>>(a);
+  return check_launch(what);
+}
+
+size_t xdna_distill_workspace_bytes(int64_t rows, int64_t vocab) {
+  if (rows < 1 || vocab < 1 || vocab > kMaxVocab || rows > (int64_t(1) << 40) / vocab) return 0;
+  return row_workspace(rows, vocab, 0);
+}
+
+int xdna_distill(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* ids,
+                 int index_bytes, const void* teacher, int teacher_dtype, int k, float tau, const float* weight,
+                 int reduction, float* row_loss, float* row_share, float* stats, float* p, float* loss, float* inv_weight,
+                 void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "xdna_distill";
+  if (!rows_ok(what, logits, dtype, rows, vocab, ld, tau)) return -1;
+  if (k < 1 || k > kMaxTeacher) return refuse(what, "teacher entries outside 1 .. 1024");
+  if (index_bytes != 4 && index_bytes != 8) return refuse(what, "indices of 4 or 8 bytes");
+  if (teacher_dtype != 1 && teacher_dtype != 2) return refuse(what, "teacher logits are fp32 or bf16");
+  if (reduction < 0 || reduction > 2) return refuse(what, "reduction must be 0 (none), 1 (mean) or 2 (sum)");
+  if (reduction != 0 && (!loss || !inv_weight)) return refuse(what, "null operand");
+  if (rows > 0 && (!ids || !teacher || !row_loss || !row_share || !stats || !p)) return refuse(what, "null operand");
+  if (off(stats, 8)) return refuse(what, "misaligned stats");
+  if (!workspace_ok(what, workspace, workspace_bytes, rows > 0 ? row_workspace(rows, vocab, 0) : 0)) return -1;
+  if (!admit_launch(what)) return -1;
+  hipStream_t st = as_stream(stream);
+  if (rows > 0) {
+    const Plan pl = row_plan(rows, vocab, 0);
+    RowArgs a = {};
+    a.z = logits;
+    a.ld = ld;
+    a.rows = rows;
+    a.V = int(vocab);
+    a.piece = pl.piece;
+    a.pieces = pl.pieces;
+    a.inv_tau = 1.0f / tau;
+    a.stat = static_cast<RowStat*>(workspace);
+    a.ds = {ids, index_bytes, teacher, teacher_dtype, weight, k, tau, reinterpret_cast<float2*>(stats), p, row_loss, row_share};
+    if (dtype == 1) launch_row<float, kDistill, false>(pl, a, st);
+    else launch_row<uint16_t, kDistill, false>(pl, a, st);
+  }
+  if (reduction == 1) distill_total_kernel<true><<<1, 1024, 0, st>>>(row_loss, row_share, rows, loss, inv_weight);
+  else if (reduction == 2) distill_total_kernel<false><<<1, 1024, 0, st>>>(row_loss, row_share, rows, loss, inv_weight);
+  return check_launch(what);
+}
+
+int xdna_distill_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* ids,
+                     int index_bytes, int k, float tau, const float* row_share, const float* stats, const float* p,
+                     const float* inv_weight, const void* go, int go_dtype, int go_rows, void* d_logits, void* stream) {
+  const char* what = "xdna_distill_bwd";
+  if (!rows_ok(what, logits, dtype, rows, vocab, ld, tau)) return -1;
+  if (k < 1 || k > kMaxTeacher) return refuse(what, "teacher entries outside 1 .. 1024");
+  if (index_bytes != 4 && index_bytes != 8) return refuse(what, "indices of 4 or 8 bytes");
+  if (go_dtype != 1 && go_dtype != 2) return refuse(what, "the incoming gradient is fp32 or bf16");
+  if (rows == 0) return 0;
+  if (!ids || !row_share || !stats || !p || !go || !d_logits) return refuse(what, "null operand");
+  if (off(stats, 8) || off(d_logits, dtype == 1 ? 4 : 2)) return refuse(what, "misaligned operand");
+  if (!admit_launch(what)) return -1;
+  const Plan pl = bwd_plan(vocab);
+  const DistillBwdArgs a = {logits, ld, d_logits, rows, int(vocab), pl.piece, pl.pieces, 1.0f / tau, tau, ids,
+                            index_bytes, k, p, reinterpret_cast<const float2*>(stats), row_share, inv_weight, go, go_dtype, go_rows ? 1 : 0};
+  hipStream_t st = as_stream(stream);
+  const unsigned grid = grid_of(rows * pl.pieces, kBwdThreads);
+  if (dtype == 1) distill_bwd_kernel<float><<<grid, kBwdThreads, 0, st>>>(a);
+  else distill_bwd_kernel<uint16_t><<<grid, kBwdThreads, 0, st>>>(a);
+  return check_launch(what);
+}
+
+}  // extern "C"

@@ -791,4 +791,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   });
   mod.def("region_loss_finish", &region_loss_finish);
   mod.def("region_gram_grad", &region_gram_grad);
+  // token-model operators (xdna_train/tokens.py)
+  mod.def("token_embed", &token_embed);
+  mod.def("token_gated_linear", &token_gated_linear);
+  mod.def("token_gated_mlp", &token_gated_mlp);
+  mod.def("token_distill", &token_distill);
+  mod.def("token_log_probs", &token_log_probs);
 }

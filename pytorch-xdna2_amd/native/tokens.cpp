@@ -1,0 +1,429 @@
+// Host side of the token-model operators (xdna_train/tokens.py): checks, workspaces, C-ABI
+// calls and autograd nodes of the embedding, the gated feed-forward, the distillation loss
+// and the token log probabilities (csrc/embed.hip, gated.hip, vocab.hip).  No call reads
+// device data on the host, so all of them can be captured in a graph.
+#include "xdna.h"
+
+#include <torch/csrc/autograd/custom_function.h>
+
+namespace xdna_backend {
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool on_xdna(const at::Tensor& t) { return t.defined() && t.device().type() == kXdna; }
+
+int float_code(const at::Tensor& t, const char* op, const char* what) {
+  TORCH_CHECK(on_xdna(t), op, ": ", what, " must be an xdna tensor");
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, op, ": ", what,
+              " must be float32 or bfloat16, got ", t.scalar_type());
+  return t.scalar_type() == at::kFloat ? 1 : 2;
+}
+
+int index_bytes(const at::Tensor& t, const char* op, const char* what) {
+  TORCH_CHECK(on_xdna(t), op, ": ", what, " must be an xdna tensor");
+  TORCH_CHECK(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, op, ": ", what,
+              " must be int64 or int32, got ", t.scalar_type());
+  return t.scalar_type() == at::kLong ? 8 : 4;
+}
+
+void check_bf16(const at::Tensor& t, const char* op, const char* what) {
+  TORCH_CHECK(on_xdna(t) && t.scalar_type() == at::kBFloat16, op, ": ", what, " must be a bfloat16 xdna tensor");
+}
+
+// [..., n] as [rows][n] with unit stride along n and a row stride of at least n (a copy only
+// where the strides do not allow a view)
+at::Tensor as_rows(const at::Tensor& t) {
+  const int64_t n = t.size(-1);
+  at::Tensor r = t.dim() == 2 ? t : t.reshape({n ? t.numel() / n : 0, n});
+  if ((n > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < n)) r = r.contiguous();
+  return r;
+}
+
+int64_t row_stride(const at::Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+at::Tensor workspace(size_t bytes) { return empty_xdna({int64_t(bytes)}, at::kByte); }
+
+void* ptr_or_null(const at::Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
+const void* cptr(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+const uint16_t* p16(const at::Tensor& t) { return static_cast<const uint16_t*>(t.const_data_ptr()); }
+uint16_t* m16(at::Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); }
+float* f32(at::Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
+const float* cf32(const at::Tensor& t) { return t.defined() ? static_cast<const float*>(t.const_data_ptr()) : nullptr; }
+
+bool tracked(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->requires_grad()) return true;
+  return false;
+}
+
+void once_only(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the gradient itself cannot be differentiated");
+}
+
+// a product of two bf16 matrices of any strides
+at::Tensor product(const at::Tensor& a, const at::Tensor& b) {
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
+  at::Tensor c = empty_xdna({M, N}, at::kBFloat16);
+  check_abi(xdna_gemm_bf16(p16(a), p16(b), m16(c), nullptr, 1, int(M), int(N), int(K), a.stride(0), a.stride(1), 0,
+                           b.stride(0), b.stride(1), 0, N, 1, 0, 0, 0, 0, 1.0f, 0.0f, current_stream()),
+            "gemm");
+  return c;
+}
+
+// ---- embedding -------------------------------------------------------------------------------
+
+at::Tensor embed_forward(const at::Tensor& ids, const at::Tensor& weight, double scale) {
+  ScopedCount sc("hip_tokens.embed.fwd.run");
+  const int ib = index_bytes(ids, "embed", "ids"), dt = float_code(weight, "embed", "weight");
+  const at::Tensor i = ids.contiguous(), w = as_rows(weight);
+  auto shape = ids.sizes().vec();
+  shape.push_back(w.size(1));
+  at::Tensor y = empty_xdna(shape, w.scalar_type());
+  check_abi(xdna_embed(cptr(i), ib, i.numel(), cptr(w), dt, w.size(0), w.size(1), row_stride(w), float(scale),
+                       ptr_or_null(y), current_stream()),
+            "embed");
+  return y;
+}
+
+struct EmbedFn : public torch::autograd::Function<EmbedFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& ids, const at::Tensor& weight, double scale,
+                            int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["dim"] = weight.size(1);
+    return embed_forward(ids, weight, scale);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("embed");
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    ScopedCount sc("hip_tokens.embed.bwd.run");
+    const at::Tensor ids = ctx->get_saved_variables()[0].contiguous();
+    const int64_t V = ctx->saved_data["vocab"].toInt(), D = ctx->saved_data["dim"].toInt();
+    const at::Tensor dy = as_rows(grads[0]);
+    const size_t bytes = xdna_embed_bwd_workspace_bytes(ids.numel(), V, D);
+    at::Tensor ws = workspace(bytes), dw = empty_xdna({V, D}, dy.scalar_type());
+    check_abi(xdna_embed_bwd(cptr(ids), ids.scalar_type() == at::kLong ? 8 : 4, ids.numel(), cptr(dy),
+                             float_code(dy, "embed", "the gradient"), row_stride(dy), V, D,
+                             ctx->saved_data["padding"].toInt(), float(ctx->saved_data["scale"].toDouble()),
+                             dw.data_ptr(), ptr_or_null(ws), bytes, current_stream()),
+              "embed backward");
+    return {at::Tensor(), dw, at::Tensor(), at::Tensor()};
+  }
+};
+
+// ---- gated feed-forward --------------------------------------------------------------------------
+
+struct GatedForward {
+  at::Tensor x, w, h, gu;  // x and w as rows
+};
+
+GatedForward gated_forward(const at::Tensor& x, const at::Tensor& w_in, int64_t act, bool keep) {
+  GatedForward r;
+  r.x = as_rows(x);
+  r.w = as_rows(w_in);
+  const int64_t M = r.x.size(0), K = r.x.size(1), F = r.w.size(0) / 2;
+  r.h = empty_xdna({M, F}, at::kBFloat16);
+  if (keep) r.gu = empty_xdna({M, 2 * F}, at::kBFloat16);
+  check_abi(xdna_gated_bf16(p16(r.x), row_stride(r.x), p16(r.w), row_stride(r.w), M, K, F, int(act), m16(r.h),
+                            keep ? m16(r.gu) : nullptr, current_stream()),
+            "gated");
+  return r;
+}
+
+at::Tensor gated_dgu(const at::Tensor& dh, const at::Tensor& gu, int64_t act) {
+  const at::Tensor d = as_rows(dh);
+  at::Tensor dgu = empty_xdna(gu.sizes(), at::kBFloat16);
+  check_abi(xdna_gated_bwd_bf16(p16(d), row_stride(d), p16(gu), gu.size(0), gu.size(1) / 2, int(act), m16(dgu),
+                                current_stream()),
+            "gated backward");
+  return dgu;
+}
+
+std::vector<int64_t> with_last(const at::Tensor& x, int64_t n) {
+  auto s = x.sizes().vec();
+  s.back() = n;
+  return s;
+}
+
+struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w_in, int64_t act) {
+    ScopedCount sc("hip_tokens.gated.fwd.run");
+    const GatedForward f = gated_forward(x, w_in, act, true);
+    ctx->save_for_backward({x, w_in, f.gu});
+    ctx->saved_data["act"] = act;
+    return f.h.view(with_last(x, f.h.size(1)));
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("gated_linear");
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
+    ScopedCount sc("hip_tokens.gated.bwd.run");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor dgu = gated_dgu(grads[0], saved[2], ctx->saved_data["act"].toInt());
+    at::Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = product(dgu, saved[1]).view(saved[0].sizes());
+    if (ctx->needs_input_grad(1)) dw = product(dgu.t(), as_rows(saved[0]));
+    return {dx, dw, at::Tensor()};
+  }
+};
+
+struct GatedMlpFn : public torch::autograd::Function<GatedMlpFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w_in,
+                            const at::Tensor& w_out, int64_t act) {
+    ScopedCount sc("hip_tokens.gated.fwd.run");
+    const GatedForward f = gated_forward(x, w_in, act, true);
+    ctx->save_for_backward({x, w_in, w_out, f.gu, f.h});
+    ctx->saved_data["act"] = act;
+    return product(f.h, w_out.t()).view(with_last(x, w_out.size(0)));
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("gated_mlp");
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    ScopedCount sc("hip_tokens.gated.bwd.run");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &w_in = saved[1], &w_out = saved[2], &gu = saved[3], &h = saved[4];
+    const at::Tensor dy = as_rows(grads[0]);
+    at::Tensor dx, dw_in, dw_out;
+    if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) {
+      const at::Tensor dgu = gated_dgu(product(dy, w_out), gu, ctx->saved_data["act"].toInt());
+      if (ctx->needs_input_grad(0)) dx = product(dgu, w_in).view(x.sizes());
+      if (ctx->needs_input_grad(1)) dw_in = product(dgu.t(), as_rows(x));
+    }
+    if (ctx->needs_input_grad(2)) dw_out = product(dy.t(), h);
+    return {dx, dw_in, dw_out, at::Tensor()};
+  }
+};
+
+void check_gated(const char* op, const at::Tensor& x, const at::Tensor& w_in) {
+  check_bf16(x, op, "x");
+  check_bf16(w_in, op, "w_in");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, op, ": x needs a last dimension");
+  TORCH_CHECK(w_in.dim() == 2 && w_in.size(0) >= 2 && w_in.size(0) % 2 == 0 && w_in.size(1) == x.size(-1), op,
+              ": w_in must hold the gate rows and then the up rows, [2 F, ", x.size(-1), "], got ", w_in.sizes());
+  TORCH_CHECK(x.numel() / x.size(-1) < (int64_t(1) << 22) && w_in.size(0) <= (int64_t(1) << 30) &&
+                  w_in.size(1) <= (int64_t(1) << 30),
+              op, ": too many rows");
+}
+
+// ---- distillation --------------------------------------------------------------------------------
+
+struct DistillForward {
+  at::Tensor loss, z, ids, share, stats, p, inv_weight;
+};
+
+DistillForward distill_forward(const at::Tensor& logits, const at::Tensor& teacher_ids, const at::Tensor& teacher,
+                               double tau, const std::optional<at::Tensor>& weight, int64_t reduction) {
+  ScopedCount sc("hip_tokens.distill.fwd.run");
+  DistillForward r;
+  r.z = as_rows(logits);
+  r.ids = as_rows(teacher_ids).contiguous();
+  const at::Tensor t = as_rows(teacher).contiguous();
+  at::Tensor w;
+  if (weight.has_value()) w = weight->to(at::kFloat).contiguous();
+  const int64_t T = r.z.size(0), V = r.z.size(1), k = r.ids.size(1);
+  at::Tensor row = empty_xdna({T}, at::kFloat), out;
+  r.share = empty_xdna({T}, at::kFloat);
+  r.stats = empty_xdna({T, 2}, at::kFloat);
+  r.p = empty_xdna({T, k}, at::kFloat);
+  if (reduction != 0) {
+    out = empty_xdna({}, at::kFloat);
+    r.inv_weight = empty_xdna({}, at::kFloat);
+  }
+  const size_t bytes = xdna_distill_workspace_bytes(T, V);
+  at::Tensor ws;
+  if (bytes) ws = workspace(bytes);
+  check_abi(xdna_distill(cptr(r.z), r.z.scalar_type() == at::kFloat ? 1 : 2, T, V, row_stride(r.z), cptr(r.ids),
+                         r.ids.scalar_type() == at::kLong ? 8 : 4, cptr(t), t.scalar_type() == at::kFloat ? 1 : 2,
+                         int(k), float(tau), cf32(w), int(reduction), f32(row), f32(r.share), f32(r.stats), f32(r.p),
+                         f32(out), f32(r.inv_weight), ptr_or_null(ws), bytes, current_stream()),
+            "distill_loss");
+  r.loss = reduction == 0 ? row.view(logits.sizes().slice(0, logits.dim() - 1)) : out;
+  return r;
+}
+
+struct DistillFn : public torch::autograd::Function<DistillFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& ids,
+                            const at::Tensor& teacher, double tau, const std::optional<at::Tensor>& weight,
+                            int64_t reduction) {
+    const DistillForward f = distill_forward(logits, ids, teacher, tau, weight, reduction);
+    ctx->save_for_backward({logits, f.ids, f.share, f.stats, f.p, f.inv_weight});
+    ctx->saved_data["tau"] = tau;
+    ctx->saved_data["rows"] = reduction == 0;
+    return f.loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("distill_loss");
+    variable_list none(6);
+    if (!grads[0].defined()) return none;
+    ScopedCount sc("hip_tokens.distill.bwd.run");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor z = as_rows(saved[0]), go = grads[0].contiguous();
+    const at::Tensor &ids = saved[1], &inv = saved[5];
+    at::Tensor dz = empty_xdna(saved[0].sizes(), z.scalar_type());
+    check_abi(xdna_distill_bwd(cptr(z), z.scalar_type() == at::kFloat ? 1 : 2, z.size(0), z.size(1), row_stride(z),
+                               cptr(ids), ids.scalar_type() == at::kLong ? 8 : 4, int(ids.size(1)),
+                               float(ctx->saved_data["tau"].toDouble()), cf32(saved[2]), cf32(saved[3]),
+                               cf32(saved[4]), cf32(inv), cptr(go), float_code(go, "distill_loss", "the gradient"),
+                               ctx->saved_data["rows"].toBool() ? 1 : 0, ptr_or_null(dz), current_stream()),
+              "distill_loss backward");
+    none[0] = dz;
+    return none;
+  }
+};
+
+// ---- token log probabilities -----------------------------------------------------------------------
+
+struct LogprobForward {
+  at::Tensor log_probs, entropy, top_log_probs, top_ids, targets, stats;
+};
+
+LogprobForward logprob_forward(const at::Tensor& logits, const at::Tensor& targets, int64_t top, double tau) {
+  ScopedCount sc("hip_tokens.logprobs.fwd.run");
+  LogprobForward r;
+  const at::Tensor z = as_rows(logits);
+  r.targets = targets.contiguous();
+  const int64_t T = z.size(0), V = z.size(1);
+  auto shape = targets.sizes().vec();
+  r.log_probs = empty_xdna(shape, at::kFloat);
+  r.entropy = empty_xdna(shape, at::kFloat);
+  r.stats = empty_xdna({T, 2}, at::kFloat);
+  shape.push_back(top);
+  r.top_log_probs = empty_xdna(shape, at::kFloat);
+  r.top_ids = empty_xdna(shape, at::kLong);
+  const size_t bytes = xdna_token_logprobs_workspace_bytes(T, V, int(top));
+  at::Tensor ws;
+  if (bytes) ws = workspace(bytes);
+  check_abi(xdna_token_logprobs(cptr(z), z.scalar_type() == at::kFloat ? 1 : 2, T, V, row_stride(z), cptr(r.targets),
+                                r.targets.scalar_type() == at::kLong ? 8 : 4, float(tau), int(top), f32(r.log_probs),
+                                f32(r.entropy), f32(r.stats), f32(r.top_log_probs),
+                                static_cast<int64_t*>(ptr_or_null(r.top_ids)), ptr_or_null(ws), bytes, current_stream()),
+            "token_log_probs");
+  return r;
+}
+
+struct LogprobFn : public torch::autograd::Function<LogprobFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& targets, int64_t top,
+                               double tau) {
+    const LogprobForward f = logprob_forward(logits, targets, top, tau);
+    // entropy goes through a detached alias: as an output it carries this node
+    ctx->save_for_backward({logits, f.targets, f.stats, f.entropy.detach()});
+    ctx->saved_data["tau"] = tau;
+    ctx->mark_non_differentiable({f.top_log_probs, f.top_ids});
+    ctx->set_materialize_grads(false);
+    return {f.log_probs, f.entropy, f.top_log_probs, f.top_ids};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("token_log_probs");
+    variable_list none(4);
+    if (!grads[0].defined() && !grads[1].defined()) return none;
+    ScopedCount sc("hip_tokens.logprobs.bwd.run");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor z = as_rows(saved[0]);
+    const at::Tensor gl = grads[0].defined() ? grads[0].to(at::kFloat).contiguous() : grads[0];
+    const at::Tensor gh = grads[1].defined() ? grads[1].to(at::kFloat).contiguous() : grads[1];
+    at::Tensor dz = empty_xdna(saved[0].sizes(), z.scalar_type());
+    check_abi(xdna_token_logprobs_bwd(cptr(z), z.scalar_type() == at::kFloat ? 1 : 2, z.size(0), z.size(1),
+                                      row_stride(z), cptr(saved[1]), saved[1].scalar_type() == at::kLong ? 8 : 4,
+                                      float(ctx->saved_data["tau"].toDouble()), cf32(saved[2]), cf32(saved[3]),
+                                      cf32(gl), cf32(gh), ptr_or_null(dz), current_stream()),
+              "token_log_probs backward");
+    none[0] = dz;
+    return none;
+  }
+};
+
+void check_tau(const char* op, double tau) {
+  TORCH_CHECK(tau > 0.0 && float(tau) > 0.0f && float(1.0 / tau) > 0.0f && std::isfinite(float(1.0 / tau)), op,
+              ": temperature must be positive and finite, got ", tau);
+}
+
+void check_logits(const char* op, const at::Tensor& logits) {
+  float_code(logits, op, "logits");
+  TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) >= 1 && logits.size(-1) <= (int64_t(1) << 22), op,
+              ": logits need a last dimension of 1 .. 2^22 tokens, got ", logits.sizes());
+}
+
+}  // namespace
+
+at::Tensor token_embed(const at::Tensor& ids, const at::Tensor& weight, double scale, std::optional<int64_t> padding) {
+  index_bytes(ids, "embed", "ids");
+  float_code(weight, "embed", "weight");
+  TORCH_CHECK(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(1) >= 1, "embed: weight must be [tokens, width], got ",
+              weight.sizes());
+  TORCH_CHECK(std::isfinite(scale), "embed: scale must be finite");
+  const int64_t V = weight.size(0);
+  int64_t pad = -1;
+  if (padding.has_value()) {
+    pad = *padding < 0 ? *padding + V : *padding;
+    TORCH_CHECK(pad >= 0 && pad < V, "embed: padding_idx ", *padding, " outside a table of ", V, " rows");
+  }
+  if (tracked({&weight})) return EmbedFn::apply(ids, weight, scale, pad);
+  return embed_forward(ids, weight, scale);
+}
+
+at::Tensor token_gated_linear(const at::Tensor& x, const at::Tensor& w_in, int64_t act) {
+  check_gated("gated_linear", x, w_in);
+  if (tracked({&x, &w_in})) return GatedLinearFn::apply(x, w_in, act);
+  ScopedCount sc("hip_tokens.gated.fwd.run");
+  const GatedForward f = gated_forward(x, w_in, act, false);
+  return f.h.view(with_last(x, f.h.size(1)));
+}
+
+at::Tensor token_gated_mlp(const at::Tensor& x, const at::Tensor& w_in, const at::Tensor& w_out, int64_t act) {
+  check_gated("gated_mlp", x, w_in);
+  check_bf16(w_out, "gated_mlp", "w_out");
+  TORCH_CHECK(w_out.dim() == 2 && w_out.size(0) >= 1 && w_out.size(0) <= (int64_t(1) << 30) &&
+                  w_out.size(1) == w_in.size(0) / 2,
+              "gated_mlp: w_out must be [N, ", w_in.size(0) / 2, "], got ", w_out.sizes());
+  if (tracked({&x, &w_in, &w_out})) return GatedMlpFn::apply(x, w_in, w_out, act);
+  ScopedCount sc("hip_tokens.gated.fwd.run");
+  const GatedForward f = gated_forward(x, w_in, act, false);
+  return product(f.h, w_out.t()).view(with_last(x, w_out.size(0)));
+}
+
+at::Tensor token_distill(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher, double tau,
+                         const std::optional<at::Tensor>& weight, int64_t reduction) {
+  const char* op = "distill_loss";
+  check_logits(op, logits);
+  index_bytes(ids, op, "teacher_ids");
+  float_code(teacher, op, "teacher_logits");
+  check_tau(op, tau);
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  TORCH_CHECK(ids.dim() == logits.dim() && ids.sizes().slice(0, ids.dim() - 1) == lead && ids.sizes() == teacher.sizes(),
+              op, ": teacher_ids and teacher_logits must be [..., k] beside logits ", logits.sizes(), ", got ", ids.sizes(),
+              " and ", teacher.sizes());
+  TORCH_CHECK(ids.size(-1) >= 1 && ids.size(-1) <= 1024, op, ": 1 to 1024 teacher entries a row, got ", ids.size(-1));
+  if (weight.has_value())
+    TORCH_CHECK(on_xdna(*weight) && weight->sizes() == lead, op, ": weight must be an xdna tensor of shape ", lead);
+  if (tracked({&logits})) return DistillFn::apply(logits, ids, teacher, tau, weight, reduction);
+  return distill_forward(logits, ids, teacher, tau, weight, reduction).loss;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_log_probs(const at::Tensor& logits,
+                                                                           const at::Tensor& targets, int64_t top,
+                                                                           double tau) {
+  const char* op = "token_log_probs";
+  check_logits(op, logits);
+  index_bytes(targets, op, "targets");
+  check_tau(op, tau);
+  TORCH_CHECK(targets.sizes() == logits.sizes().slice(0, logits.dim() - 1), op, ": targets must be ",
+              logits.sizes().slice(0, logits.dim() - 1), ", got ", targets.sizes());
+  TORCH_CHECK(top >= 0 && top <= 64 && top <= logits.size(-1), op, ": top_k must be 0 .. min(64, vocabulary), got ", top);
+  if (tracked({&logits})) {
+    const variable_list v = LogprobFn::apply(logits, targets, top, tau);
+    return {v[0], v[1], v[2], v[3]};
+  }
+  const LogprobForward f = logprob_forward(logits, targets, top, tau);
+  return {f.log_probs, f.entropy, f.top_log_probs, f.top_ids};
+}
+
+}  // namespace xdna_backend

@@ -136,6 +136,16 @@ std::tuple<at::Tensor, at::Tensor> region_loss_finish(const at::Tensor& part);
 at::Tensor region_gram_grad(const at::Tensor& G, const at::Tensor& t, double chw, double coef,
                             const std::optional<at::Tensor>& go);
 
+// Token-model operators with their autograd nodes (tokens.cpp, xdna_train/tokens.py).
+at::Tensor token_embed(const at::Tensor& ids, const at::Tensor& weight, double scale, std::optional<int64_t> padding);
+at::Tensor token_gated_linear(const at::Tensor& x, const at::Tensor& w_in, int64_t act);
+at::Tensor token_gated_mlp(const at::Tensor& x, const at::Tensor& w_in, const at::Tensor& w_out, int64_t act);
+at::Tensor token_distill(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher, double tau,
+                         const std::optional<at::Tensor>& weight, int64_t reduction);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_log_probs(const at::Tensor& logits,
+                                                                           const at::Tensor& targets, int64_t top,
+                                                                           double tau);
+
 // Live kernel timing: HIP events around hot-kernel launches on the launch stream,
 // with the algorithmic work (FLOP or bytes) of each launch.
 struct KernelTimer {

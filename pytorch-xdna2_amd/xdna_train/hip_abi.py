@@ -140,6 +140,17 @@ SIGNATURES = {
     "xdna_mse_loss_bwd": (I, [P, I, P, P, I, L, L, I, P, P]),
     "xdna_colsum_workspace_bytes": (Z, [P, L, L]),
     "xdna_colsum_bf16": (I, [P, P, L, L, P, Z, P]),
+    "xdna_embed": (I, [P, I, L, P, I, L, L, L, F, P, P]),
+    "xdna_embed_bwd_workspace_bytes": (Z, [L, L, L]),
+    "xdna_embed_bwd": (I, [P, I, L, P, I, L, L, L, L, F, P, P, Z, P]),
+    "xdna_gated_bf16": (I, [P, L, P, L, L, L, L, I, P, P, P]),
+    "xdna_gated_bwd_bf16": (I, [P, L, P, L, L, I, P, P]),
+    "xdna_token_logprobs_workspace_bytes": (Z, [L, L, I]),
+    "xdna_token_logprobs": (I, [P, I, L, L, L, P, I, F, I, P, P, P, P, P, P, Z, P]),
+    "xdna_token_logprobs_bwd": (I, [P, I, L, L, L, P, I, F, P, P, P, P, P, P]),
+    "xdna_distill_workspace_bytes": (Z, [L, L]),
+    "xdna_distill": (I, [P, I, L, L, L, P, I, P, I, I, F, P, I, P, P, P, P, P, P, P, Z, P]),
+    "xdna_distill_bwd": (I, [P, I, L, L, L, P, I, I, F, P, P, P, P, P, I, I, P, P]),
     "xdna_conv3x3_wgrad_pack_bf16": (I, [P, P, I, I, I, I, I, P, Z, P]),
     "xdna_conv3x3_wgrad_packed_bf16": (I, [P, P, I, I, I, I, I, P, Z, P]),
     "xdna_gemm_set_variant": (I, [I]),

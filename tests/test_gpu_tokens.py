@@ -1,0 +1,597 @@
+"""Token-model operators (xdna_train.tokens) against plain 64-bit implementations on the CPU,
+at the sizes, masks and strides where they can go wrong.
+
+Tolerances, per element.  u = 2^-24 (half an fp32 ulp at 1), b = 2^-8 (half a bf16 ulp at 1, the
+one rounding of a bf16 result):
+* lookups: bit-exact (one fp32 product, one rounding);
+* embedding gradient: n u sum |scale dy| for a row of n tokens (any order of fp32 sums), plus
+  the result's rounding;
+* log probabilities: (64 + 8 |value|) u: the sum over the vocabulary goes through 32 terms a
+  thread and under 32 more levels, each hardware exp is within 2 u and its argument, a
+  difference times a constant, within 2 u of itself; entropy: 4 times that on 1 + H + |ln s|;
+* gradients of rows: (64 + 4 |ln q|) u on every term's magnitude (exp turns the two roundings of
+  its argument into |ln q| u each), plus the result's rounding;
+* gated products: see gated_reference, which carries each rounding's bound through the products.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U, B = 2.0 ** -24, 2.0 ** -8
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+TINY = 1e-37  # the hardware exp flushes results below the normal range
+
+
+@pytest.fixture(scope="module")
+def T(hip):
+    from xdna_train import tokens
+    return tokens
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rounding(dtype):
+    return B if dtype == BF16 else U
+
+
+def close(got, ref, tol, what):
+    got = got.detach().cpu().to(F64)
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    same = (got == ref) | (torch.isnan(got) & torch.isnan(ref))
+    bad = ~same & ~((got - ref).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), got[bad][:4], ref[bad][:4],
+                           (tol[bad][:4] if torch.is_tensor(tol) and tol.shape == ref.shape else tol))
+
+
+def padded(t, extra, offset=0):
+    """t's values in a larger allocation: rows `extra` elements apart, `offset` elements in."""
+    rows, n = t.shape
+    buf = torch.full((rows * (n + extra) + offset + 8,), 7.0, dtype=t.dtype, device="xdna")
+    v = torch.as_strided(buf, (rows, n), (n + extra, 1), offset)
+    v.copy_(t)
+    return v
+
+
+# ---- embedding --------------------------------------------------------------------------------
+
+EMBED = [  # tokens, vocabulary, width
+    (1, 1, 1), (1, 5, 8), (3, 2, 7), (31, 9, 33), (32, 300, 64), (33, 1, 40), (65, 70000, 17), (257, 511, 512),
+    (300, 512, 520), (1000, 513, 129), (8191, 40, 24), (8192, 1024, 8), (8193, 1000, 16), (20000, 300000, 9), (17000, 3, 72),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("n,V,D", EMBED)
+def test_embedding(T, n, V, D, dtype):
+    print("embedding", n, V, D, dtype, flush=True)
+    g = gen(n + V + D)
+    scale = 1.0 if D % 2 else math.sqrt(D)
+    w = torch.randn(V, D, generator=g).to(dtype)
+    ids = (torch.rand(n, generator=g, dtype=F64) ** 3 * V).long().clamp_(max=V - 1)  # crowded low ids
+    dy = torch.randn(n, D, generator=g).to(dtype)
+    wx = w.to("xdna").requires_grad_()
+    y = T.embed(ids.to("xdna"), wx, scale=scale)
+    assert torch.equal(y.detach().cpu(), (w[ids].float() * torch.tensor(scale, dtype=F32)).to(dtype))
+    y.backward(dy.to("xdna"))
+    ref = torch.zeros(V, D, dtype=F64).index_add_(0, ids, dy.to(F64)) * scale
+    mag = torch.zeros(V, D, dtype=F64).index_add_(0, ids, dy.to(F64).abs()) * scale
+    count = torch.bincount(ids, minlength=V).to(F64)[:, None]
+    close(wx.grad, ref, (count + 2) * U * mag + rounding(dtype) * ref.abs(), "embedding gradient")
+    again = torch.autograd.grad(T.embed(ids.to("xdna"), wx, scale=scale), [wx], dy.to("xdna"))[0]
+    assert torch.equal(again.cpu(), wx.grad.cpu()), "equal inputs, different bits"
+
+
+@pytest.mark.parametrize("n", [200, 9000])
+def test_embedding_padding_outside_ids_strides_and_int32(T, n):
+    print("embedding edges", n, flush=True)
+    V, D, pad = 50, 37, 7
+    g = gen(n)
+    ids = torch.randint(-3, V + 3, (n,), generator=g)
+    ids[::5] = pad
+    w, dy = torch.randn(V, D, generator=g).bfloat16(), torch.randn(n, D, generator=g).bfloat16()
+    wx = padded(w, 3, 1).requires_grad_()
+    y = T.embed(ids.int().to("xdna"), wx, scale=0.5, padding_idx=pad - V)
+    inside = (ids >= 0) & (ids < V)
+    got = y.detach().cpu()
+    assert torch.equal(got[inside], (w[ids[inside]].float() * 0.5).bfloat16())
+    assert torch.isnan(got[~inside].float()).all()
+    dyx = padded(dy, 11, 3)
+    (dw,) = torch.autograd.grad(y, [wx], dyx)
+    keep = inside & (ids != pad)
+    ref = torch.zeros(V, D, dtype=F64).index_add_(0, ids[keep], dy[keep].to(F64)) * 0.5
+    mag = torch.zeros(V, D, dtype=F64).index_add_(0, ids[keep], dy[keep].to(F64).abs())
+    close(dw, ref, n * U * mag + B * ref.abs(), "gradient with padding")
+    assert not dw[pad].cpu().any()
+
+
+def test_embedding_without_tokens_and_of_any_shape(T):
+    w = torch.randn(6, 5, generator=gen(0)).to("xdna").requires_grad_()
+    y = T.embed(torch.zeros(0, 3, dtype=torch.long, device="xdna"), w)
+    assert y.shape == (0, 3, 5)
+    (dw,) = torch.autograd.grad(y, [w], torch.zeros(0, 3, 5, device="xdna"))
+    assert not dw.cpu().any() and dw.shape == w.shape
+    ids = torch.tensor([[0, 5], [2, 2]], device="xdna")
+    assert torch.equal(T.embed(ids, w).detach().cpu(), w.detach().cpu()[ids.cpu()])
+    broadcast = torch.ones(1, 1, 5, device="xdna").expand(2, 2, 5)  # a gradient of stride 0
+    (dw,) = torch.autograd.grad(T.embed(ids, w), [w], broadcast)
+    assert dw.cpu()[:, 0].tolist() == [1, 0, 2, 0, 0, 1]
+
+
+# ---- gated feed-forward -----------------------------------------------------------------------
+
+def act64(name, g):
+    if name == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    if name == "gelu":
+        c = 0.5 * torch.erfc(-g / math.sqrt(2))
+        return g * c, c + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    return g.clamp(min=0), (g > 0).to(F64)
+
+
+def gated_reference(x, w, wo, dy, act, fused):
+    """Values and bounds: {name: (value, tolerance)}.  Each stored bf16 value is off by b of itself,
+    each fp32 sum of n products by (n + 8) u of the sum of magnitudes; act' is at most 1.13 and act''
+    at most 0.8 in size (relu: a rounded gate keeps its sign).  fused: dh is not stored."""
+    x, w, wo, dy = (t.to(F64) for t in (x, w, wo, dy))
+    F = w.shape[0] // 2
+    K, N, M = x.shape[1], wo.shape[0], x.shape[0]
+    g, u = x @ w[:F].t(), x @ w[F:].t()
+    eg = (K + 8) * U * (x.abs() @ w[:F].abs().t())
+    eu = (K + 8) * U * (x.abs() @ w[F:].abs().t())
+    a, da = act64(act, g)
+    ea = 1.13 * eg + 16 * U * (a.abs() + g.abs())
+    h = a * u
+    eh = ea * u.abs() + (a.abs() + ea) * eu + B * h.abs()
+    y = h @ wo.t()
+    ey = (eh + (F + 8) * U * h.abs()) @ wo.abs().t() + B * y.abs()
+    dh = dy @ wo
+    edh = (N + 8) * U * (dy.abs() @ wo.abs()) + (0 if fused else B) * dh.abs()
+    kg, ku = eg + B * g.abs(), eu + B * u.abs()  # the kept projections
+    eda = (0.8 * kg if act != "relu" else torch.where(g.abs() <= 4 * eg, 1.0, 0.0)) + 32 * U * (1 + g.abs())
+    eka = 1.13 * kg + 16 * U * (a.abs() + g.abs())
+    dg, du = dh * u * da, dh * a
+    edg = edh * (u.abs() + ku) * (da.abs() + eda) + dh.abs() * (ku * (da.abs() + eda) + u.abs() * eda)
+    edu = edh * (a.abs() + eka) + dh.abs() * eka
+    d = torch.cat([dg, du], 1)
+    ed = torch.cat([edg + B * dg.abs(), edu + B * du.abs()], 1)
+    dx = d @ w
+    edx = (ed + (2 * F + 8) * U * d.abs()) @ w.abs() + B * dx.abs()
+    dw = d.t() @ x
+    edw = (ed + (M + 8) * U * d.abs()).t() @ x.abs() + B * dw.abs()
+    dwo = dy.t() @ h
+    edwo = dy.abs().t() @ (eh + (M + 8) * U * h.abs()) + B * dwo.abs()
+    out = {"h": (h, eh), "y": (y, ey), "dx": (dx, edx), "dw_in": (dw, edw), "dw_out": (dwo, edwo)}
+    return {k: (v, e + 1e-30) for k, (v, e) in out.items()}
+
+
+GATED = [  # rows, K, F, N
+    (1, 1, 1, 1), (1, 64, 32, 16), (1, 1000, 520, 1000), (2, 7, 5, 3), (5, 72, 100, 33), (16, 256, 128, 64), (17, 130, 63, 65),
+    (33, 8, 65, 8), (63, 200, 64, 17), (64, 64, 64, 64), (65, 65, 129, 100), (130, 512, 384, 512), (333, 1000, 217, 1000),
+]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("M,K,F,N", GATED)
+def test_gated_mlp(T, M, K, F, N, act):
+    print("gated", M, K, F, N, act, flush=True)
+    g = gen(M * 7 + K + F)
+    x, dy = torch.randn(M, K, generator=g).bfloat16(), torch.randn(M, N, generator=g).bfloat16()
+    w = (torch.randn(2 * F, K, generator=g) / math.sqrt(K)).bfloat16()
+    wo = (torch.randn(N, F, generator=g) / math.sqrt(F)).bfloat16()
+    ref = gated_reference(x, w, wo, dy, act, True)
+    leaves = [t.to("xdna").requires_grad_() for t in (x, w, wo)]
+    y = T.gated_mlp(*leaves, activation=act)
+    got = torch.autograd.grad(y, leaves, dy.to("xdna"))
+    close(y, *ref["y"], "y")
+    for name, t in zip(("dx", "dw_in", "dw_out"), got):
+        close(t, *ref[name], name)
+    with torch.no_grad():
+        h = T.gated_linear(leaves[0], leaves[1], activation=act)
+        close(h, *ref["h"], "h")
+        close(T.gated_mlp(*leaves, activation=act), *ref["y"], "y without gradients")
+
+
+@pytest.mark.parametrize("M,K,F", [(1, 24, 40), (70, 130, 96), (300, 256, 131)])
+def test_gated_linear_gradient_and_strides(T, M, K, F):
+    print("gated strides", M, K, F, flush=True)
+    g = gen(M + F)
+    x, dh = torch.randn(M, K, generator=g).bfloat16(), torch.randn(M, F, generator=g).bfloat16()
+    w = (torch.randn(2 * F, K, generator=g) / math.sqrt(K)).bfloat16()
+    xs, ws = padded(x, 5, 1).requires_grad_(), padded(w, 3, 5).requires_grad_()
+    h = T.gated_linear(xs, ws, activation="silu")
+    # with the identity as w_out, dy is dh itself, exactly
+    ref = gated_reference(x, w, torch.eye(F), dh, "silu", True)
+    close(h, *ref["h"], "h")
+    got = torch.autograd.grad(h, [xs, ws], padded(dh, 9, 3))
+    close(got[0], *ref["dx"], "dx")
+    close(got[1], *ref["dw_in"], "dw_in")
+    # x transposed in memory, w's columns a slice of a wider matrix: the same values
+    xt = x.t().contiguous().to("xdna").t()
+    assert torch.equal(T.gated_linear(xt, ws).cpu(), h.detach().cpu())
+    x3 = x.view(1, M, K).to("xdna")
+    assert torch.equal(T.gated_linear(x3, ws).cpu()[0], h.detach().cpu())
+
+
+def test_gated_without_rows(T):
+    w = torch.randn(8, 6, generator=gen(1)).bfloat16().to("xdna").requires_grad_()
+    wo = torch.randn(5, 4, generator=gen(2)).bfloat16().to("xdna").requires_grad_()
+    x = torch.zeros(0, 6, dtype=BF16, device="xdna").requires_grad_()
+    y = T.gated_mlp(x, w, wo)
+    assert y.shape == (0, 5)
+    dx, dw, dwo = torch.autograd.grad(y, [x, w, wo], torch.zeros(0, 5, dtype=BF16, device="xdna"))
+    assert dx.shape == (0, 6) and not dw.float().cpu().any() and not dwo.float().cpu().any()
+
+
+# ---- rows over a vocabulary -------------------------------------------------------------------
+
+VOCABS = [1, 2, 7, 64, 100, 1003, 2047, 2048, 2049, 4097, 8192, 8193, 32768, 32769, 50001, 131072]
+
+
+def make_logits(rows, V, dtype, seed, masked=0.0, extra=0):
+    g = gen(seed)
+    z = 3 * torch.randn(rows, V, generator=g)
+    if masked:
+        z[torch.rand(rows, V, generator=g) < masked] = -math.inf
+    z = z.to(dtype)
+    return z, padded(z, extra, extra % 5).requires_grad_()
+
+
+def logprob_reference(z, y, tau, k):
+    x = z.to(F64) / tau
+    m = x.amax(1, keepdim=True)
+    empty = (m == -math.inf)[:, 0]
+    m0 = torch.where(torch.isinf(m), torch.zeros_like(m), m)
+    e = torch.exp(x - m0)
+    s = e.sum(1, keepdim=True)
+    lq = torch.where(empty[:, None], torch.full_like(x, -math.inf), x - m0 - torch.log(s))
+    q = torch.where(empty[:, None], torch.zeros_like(x), e / s)
+    h = -torch.where(q > 0, q * lq, torch.zeros_like(q)).sum(1)
+    lp = lq.gather(1, y.clamp(min=0)[:, None])[:, 0]
+    lp = torch.where(y >= 0, lp, torch.zeros_like(lp))
+    ids = torch.argsort(z.to(F64), dim=1, descending=True, stable=True)[:, :k]
+    return lp, h, lq.gather(1, ids), ids, q, lq
+
+
+def tol_log(v):
+    return (64 + 8 * torch.where(torch.isfinite(v), v.abs(), torch.zeros_like(v))) * U
+
+
+def grad_tol(terms, ref, dtype, lq):
+    return (64 + 4 * lq.abs()) * U * terms + rounding(dtype) * ref.abs() + TINY
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("V", VOCABS)
+@pytest.mark.parametrize("rows,k,tau,masked", [(3, 20, 1.0, 0.0), (5, 64, 0.7, 0.6), (2, 1, 2.0, 0.0)])
+def test_token_log_probs(T, rows, V, k, tau, masked, dtype):
+    print("log probabilities", rows, V, k, tau, masked, dtype, flush=True)
+    k = min(k, V)
+    z, zx = make_logits(rows, V, dtype, V + rows, masked, extra=V % 9)
+    y = torch.randint(0, V, (rows,), generator=gen(V))
+    y[-1] = -100
+    r = T.token_log_probs(zx, y.to("xdna"), top_k=k, temperature=tau)
+    lp, h, tlp, tid, q, lq = logprob_reference(z, y, tau, k)
+    close(r.log_probs, lp, tol_log(lp), "log_probs")
+    etol = 4 * U * (64 + 8 * 30 / tau) * (1 + h)
+    close(r.entropy, h, etol, "entropy")
+    assert torch.equal(r.top_ids.cpu(), tid), "top ids"
+    close(r.top_log_probs, tlp, tol_log(tlp), "top log_probs")
+    gl, gh = torch.randn(rows, generator=gen(1)), torch.randn(rows, generator=gen(2))
+    (dz,) = torch.autograd.grad([r.log_probs, r.entropy], [zx], [gl.to("xdna"), gh.to("xdna")])
+    gl64, gh64 = torch.where(y >= 0, gl, torch.zeros(rows)).to(F64)[:, None], gh.to(F64)[:, None]
+    hot = torch.zeros(rows, V, dtype=F64).scatter_(1, y.clamp(min=0)[:, None], 1.0)
+    some = (q.sum(1, keepdim=True) > 0).to(F64)
+    lqf = torch.where(q > 0, lq, torch.zeros_like(lq))
+    ref = (gl64 * (hot - q) * some - gh64 * q * (lqf + h[:, None])) / tau
+    terms = (gl64.abs() * (hot + q) + gh64.abs() * q * (1 + lqf.abs() + h[:, None])) / tau
+    close(dz, ref, grad_tol(terms, ref, dtype, lqf), "gradient")
+
+
+def test_log_probs_of_many_rows_take_the_wide_workgroups(T):
+    """256 rows of 40000: two pieces of a wide workgroup each, joined."""
+    rows, V, k = 256, 40000, 8
+    print("wide rows", flush=True)
+    z, zx = make_logits(rows, V, BF16, 5)
+    y = torch.randint(0, V, (rows,), generator=gen(6))
+    r = T.token_log_probs(zx.detach(), y.to("xdna"), top_k=k)
+    lp, h, tlp, tid, _, _ = logprob_reference(z, y, 1.0, k)
+    close(r.log_probs, lp, tol_log(lp), "log_probs")
+    close(r.entropy, h, 4 * U * 304 * (1 + h), "entropy")
+    assert torch.equal(r.top_ids.cpu(), tid)
+    close(r.top_log_probs, tlp, tol_log(tlp), "top")
+
+
+def order_rows(V, kind, g):
+    i = torch.arange(V, dtype=F32)
+    if kind == "equal":
+        return torch.zeros(V)
+    if kind == "falling":
+        return -i / 16
+    if kind == "rising":
+        return i / 16
+    if kind == "stride":      # the largest all at one lane's places
+        return torch.where(i % 512 < 8, 40 + i / V, torch.randn(V, generator=g))
+    if kind == "few":         # fewer tokens allowed than asked for
+        z = torch.full((V,), -math.inf)
+        z[torch.randperm(V, generator=g)[:3]] = torch.tensor([1.0, 1.0, 2.0])
+        return z
+    if kind == "zeros":       # -0 and +0 are equal: the lower index comes first
+        return torch.where(i % 3 == 0, torch.tensor(-0.0), torch.tensor(0.0))
+    z = torch.full((V,), -math.inf)
+    return z                  # "barred": nothing allowed
+
+
+@pytest.mark.parametrize("kind", ["equal", "falling", "rising", "stride", "few", "zeros", "barred"])
+@pytest.mark.parametrize("V", [70, 2048, 8192, 20000, 70000])
+def test_top_alternatives_of_special_orders(T, V, kind):
+    print("order", V, kind, flush=True)
+    k = 40
+    z = torch.stack([order_rows(V, kind, gen(V + i)) for i in range(2)])
+    y = torch.tensor([0, V - 1])
+    for dtype in (BF16, F32):
+        zd = z.to(dtype)
+        r = T.token_log_probs(zd.to("xdna"), y.to("xdna"), top_k=k)
+        lp, h, tlp, tid, _, _ = logprob_reference(zd, y, 1.0, k)
+        assert torch.equal(r.top_ids.cpu(), tid), dtype
+        close(r.top_log_probs, tlp, tol_log(tlp), "top")
+        close(r.log_probs, lp, tol_log(lp), "log_probs")
+        close(r.entropy, h, 4 * U * 304 * (1 + h), "entropy")
+
+
+def test_log_probs_of_nan_infinite_and_lowest_logits(T):
+    V = 3000
+    z = torch.randn(5, V, generator=gen(3))
+    z[0, 17] = math.nan
+    z[1, 2999] = math.inf
+    z[2] = torch.finfo(F32).min          # a mask of the type's lowest value: an even row
+    z[3, 5:] = torch.finfo(F32).min
+    y = torch.tensor([3, 4, 5, 2, V])    # the last is past the vocabulary
+    zx = z.to("xdna").requires_grad_()
+    r = T.token_log_probs(zx, y.to("xdna"), top_k=2)
+    lp = r.log_probs.detach().cpu()
+    assert torch.isnan(lp[0]) and torch.isnan(lp[1]) and torch.isnan(lp[4])
+    assert r.top_ids.cpu()[0, 0] == 17 and r.top_ids.cpu()[1, 0] == 2999 and r.top_ids.cpu()[2].tolist() == [0, 1]
+    ref = logprob_reference(z[2:4], y[2:4], 1.0, 2)
+    close(r.log_probs[2:4], ref[0], tol_log(ref[0]), "log_probs")
+    close(r.entropy[2:4], ref[1], 4 * U * 304 * (1 + ref[1]), "entropy")
+    (dz,) = torch.autograd.grad(r.log_probs[2:4].sum(), [zx])
+    dz = dz.cpu()
+    assert not dz[0].any() and not dz[1].any() and not dz[4].any()  # no incoming gradient: not even NaN
+    close(dz[3], torch.nn.functional.one_hot(torch.tensor(2), V).to(F64) - ref[4][1], 128 * U * torch.ones(V, dtype=F64), "gradient")
+
+
+def test_log_probs_shapes_and_one_gradient(T):
+    z = torch.randn(2, 3, 11, generator=gen(9))
+    y = torch.randint(0, 11, (2, 3), generator=gen(10))
+    zx = z.to("xdna").requires_grad_()
+    r = T.token_log_probs(zx, y.int().to("xdna"), top_k=4)
+    assert r.log_probs.shape == (2, 3) and r.top_ids.shape == (2, 3, 4) and r.top_log_probs.shape == (2, 3, 4)
+    assert not r.top_log_probs.requires_grad
+    lp, h, _, _, q, lq = logprob_reference(z.view(6, 11), y.view(6), 1.0, 4)
+    (dz,) = torch.autograd.grad(r.entropy.sum(), [zx])
+    ref = -q * (lq + h[:, None])
+    close(dz.view(6, 11), ref, grad_tol(q * (1 + lq.abs() + h[:, None]), ref, F32, lq), "entropy's gradient")
+    empty = T.token_log_probs(torch.zeros(0, 5, device="xdna"), torch.zeros(0, dtype=torch.long, device="xdna"), top_k=2)
+    assert empty.log_probs.shape == (0,) and empty.top_ids.shape == (0, 2)
+
+
+def test_log_probs_gradient_against_differences(T):
+    """Central differences of the forward: the step's third-order term and the forward's rounding
+    over the step are both under 1e-3 of the slope's scale here."""
+    V, eps = 301, 2.0 ** -5
+    z = torch.randn(4, V, generator=gen(20))
+    d = torch.randn(4, V, generator=gen(21))
+    y = torch.randint(0, V, (4,), generator=gen(22)).to("xdna")
+
+    def value(t):
+        r = T.token_log_probs(t, y, temperature=0.9)
+        return r.log_probs.sum() + 0.5 * r.entropy.sum()
+
+    zx = z.to("xdna").requires_grad_()
+    (dz,) = torch.autograd.grad(value(zx), [zx])
+    slope = (value((z + eps * d).to("xdna")) - value((z - eps * d).to("xdna"))).item() / (2 * eps)
+    assert abs(slope - float((dz.cpu() * d).sum())) <= 1e-3 * float((dz.cpu() * d).abs().sum())
+
+
+# ---- distillation -----------------------------------------------------------------------------
+
+def distill_reference(z, ids, t, tau, w, reduction):
+    x = z.to(F64) / tau
+    lq = torch.log_softmax(x, 1)
+    q = torch.exp(lq)
+    valid = (ids >= 0) & (t > -math.inf)
+    has = valid.any(1)
+    tt = torch.where(valid, t.to(F64) / tau, torch.full(t.shape, -math.inf, dtype=F64))
+    p = torch.where(has[:, None], torch.softmax(tt, 1), torch.zeros_like(tt))
+    p = torch.nan_to_num(p)
+    lp = torch.where(p > 0, torch.log(p), torch.zeros_like(p))
+    lqi = lq.gather(1, ids.clamp(min=0))
+    rows = tau * tau * torch.where(p > 0, p * (lp - lqi), torch.zeros_like(p)).sum(1)
+    mag = tau * tau * torch.where(p > 0, p * (lp.abs() + lqi.abs() + 1), torch.zeros_like(p)).sum(1)
+    share = torch.where(has, w.to(F64), torch.zeros(len(w), dtype=F64))
+    total = share.sum() if reduction == "mean" else 1.0
+    share = torch.where(share != 0, share / (total if total else 1.0), torch.zeros_like(share))
+    rows = torch.where(share != 0, share * rows, torch.zeros_like(rows))
+    dz = (q.scatter_add(1, ids.clamp(min=0), -p)) * (share * tau)[:, None]
+    terms = (q.scatter_add(1, ids.clamp(min=0), p)) * (share.abs() * tau)[:, None]
+    return rows, share.abs() * mag, dz, terms
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,V,k,tau,reduction", [
+    (1, 2, 1, 1.0, "mean"), (3, 7, 3, 2.0, "sum"), (61, 1003, 8, 1.0, "mean"), (5, 2049, 64, 0.7, "none"), (4, 8192, 65, 1.0, "mean"),
+    (7, 40001, 128, 3.0, "mean"), (2, 131072, 1000, 1.0, "sum"), (300, 33000, 5, 1.0, "mean")])
+def test_distillation(T, rows, V, k, tau, reduction, dtype):
+    print("distillation", rows, V, k, tau, reduction, dtype, flush=True)
+    g = gen(rows + V + k)
+    z, zx = make_logits(rows, V, dtype, V + 1, extra=V % 7)
+    ids = torch.randint(0, V, (rows, k), generator=g)   # names a token twice now and then
+    t = 4 * torch.randn(rows, k, generator=g)
+    ids[torch.rand(rows, k, generator=g) < 0.2] = -1
+    t[torch.rand(rows, k, generator=g) < 0.1] = -math.inf
+    w = torch.rand(rows, generator=g)
+    if rows > 2:
+        w[1] = 0.0
+        ids[2] = -1  # a row without entries
+    loss = T.distill_loss(zx, ids.to("xdna"), t.to("xdna"), temperature=tau, weight=w.to("xdna"), reduction=reduction)
+    per_row, mag, dz, terms = distill_reference(z, ids, t, tau, w, reduction)
+    if reduction == "none":
+        close(loss, per_row, 128 * U * mag, "row losses")
+        go = torch.randn(rows, generator=g)
+        (got,) = torch.autograd.grad(loss, [zx], go.to("xdna"))
+        dz, terms = dz * go.to(F64)[:, None], terms * go.abs().to(F64)[:, None]
+    else:
+        close(loss, per_row.sum(), 128 * U * mag.sum(), "loss")
+        (got,) = torch.autograd.grad(loss, [zx], torch.tensor(-1.5, device="xdna"))
+        dz, terms = -1.5 * dz, 1.5 * terms
+    close(got, dz, grad_tol(2 * terms, dz, dtype, torch.log_softmax(z.to(F64) / tau, 1)), "gradient")
+    again = T.distill_loss(zx, ids.to("xdna"), t.to("xdna"), temperature=tau, weight=w.to("xdna"), reduction=reduction)
+    assert torch.equal(again.detach().cpu(), loss.detach().cpu())
+
+
+def test_distillation_without_weight_in_bf16_teacher_and_empty(T):
+    z, t = torch.randn(2, 3, 50, generator=gen(1)), torch.randn(2, 3, 4, generator=gen(2)).bfloat16()
+    ids = torch.randint(0, 50, (2, 3, 4), generator=gen(3))
+    loss = T.distill_loss(z.to("xdna"), ids.int().to("xdna"), t.to("xdna"))
+    rows, mag, _, _ = distill_reference(z.view(6, 50), ids.view(6, 4), t.view(6, 4).float(), 1.0, torch.ones(6), "mean")
+    close(loss, rows.sum(), 128 * U * mag.sum(), "loss")
+    none = T.distill_loss(z.to("xdna"), torch.full_like(ids, -1).to("xdna"), t.to("xdna"))
+    assert none.item() == 0.0
+    zx = torch.zeros(0, 50, device="xdna", requires_grad=True)
+    empty = T.distill_loss(zx, torch.zeros(0, 2, dtype=torch.long, device="xdna"), torch.zeros(0, 2, device="xdna"))
+    (dz,) = torch.autograd.grad(empty, [zx])
+    assert empty.item() == 0.0 and dz.shape == (0, 50)
+
+
+def test_distillation_of_masked_and_invalid_rows(T):
+    """Weight 0 leaves a row out whatever it holds; -inf student logits outside the entries add
+    nothing; a barred entry's loss is infinite; an id past the vocabulary makes the loss NaN."""
+    V = 100
+    z = torch.randn(4, V, generator=gen(4))
+    ids = torch.tensor([[1, 2], [3, 4], [5, 6], [7, 8]])
+    t = torch.zeros(4, 2)
+    z[0] = math.nan
+    z[1, 50:] = -math.inf
+    w = torch.tensor([0.0, 1.0, 1.0, 0.0])
+    zx = z.to("xdna").requires_grad_()
+    loss = T.distill_loss(zx, ids.to("xdna"), t.to("xdna"), weight=w.to("xdna"))
+    ref = distill_reference(z[1:3], ids[1:3], t[1:3], 1.0, w[1:3], "mean")
+    close(loss, ref[0].sum(), 128 * U * ref[1].sum(), "loss")
+    (dz,) = torch.autograd.grad(loss, [zx])
+    assert not dz[0].cpu().any() and not dz[3].cpu().any() and not dz[1, 50:].cpu().any()
+    close(dz[1:3], ref[2], 128 * U * ref[3] + U * ref[2].abs() + TINY, "gradient")
+    z[1, 3] = -math.inf
+    each = T.distill_loss(z.to("xdna"), ids.to("xdna"), t.to("xdna"), weight=w.to("xdna"), reduction="none").cpu()
+    assert each[0] == 0 and each[1] == math.inf and each[3] == 0
+    ids[2, 0] = V
+    assert torch.isnan(T.distill_loss(z.to("xdna"), ids.to("xdna"), t.to("xdna"), weight=w.to("xdna"))).item()
+
+
+def test_distillation_gradient_against_differences(T):
+    V, eps = 200, 2.0 ** -5
+    z, d = torch.randn(3, V, generator=gen(30)), torch.randn(3, V, generator=gen(31))
+    ids = torch.randint(0, V, (3, 9), generator=gen(32)).to("xdna")
+    t = torch.randn(3, 9, generator=gen(33)).to("xdna")
+
+    def value(a):
+        return T.distill_loss(a, ids, t, temperature=1.5, reduction="sum")
+
+    zx = z.to("xdna").requires_grad_()
+    (dz,) = torch.autograd.grad(value(zx), [zx])
+    slope = (value((z + eps * d).to("xdna")) - value((z - eps * d).to("xdna"))).item() / (2 * eps)
+    assert abs(slope - float((dz.cpu() * d).sum())) <= 1e-3 * float((dz.cpu() * d).abs().sum())
+
+
+def test_gated_gradient_against_differences(T):
+    """In bf16 the differences are noisy: the forward's rounding, b of the terms of y, over the step."""
+    M, K, F = 8, 64, 48
+    g = gen(40)
+    x = torch.randn(M, K, generator=g).bfloat16()
+    w = (torch.randn(2 * F, K, generator=g) / 8).bfloat16()
+    wo = (torch.randn(K, F, generator=g) / 7).bfloat16()
+    c, d = torch.randn(M, K, generator=g).bfloat16(), torch.randn(M, K, generator=g)
+    leaves = [t.to("xdna").requires_grad_() for t in (x, w, wo)]
+    (dx,) = torch.autograd.grad(T.gated_mlp(*leaves), [leaves[0]], c.to("xdna"))
+    eps = 2.0 ** -4
+    hi, lo = (x.float() + eps * d).bfloat16(), (x.float() - eps * d).bfloat16()
+    with torch.no_grad():
+        f = [(T.gated_mlp(t.to("xdna"), leaves[1], leaves[2]).cpu().to(F64) * c.to(F64)) for t in (hi, lo)]
+    step = hi.to(F64) - lo.to(F64)
+    noise = 2 * B * float((f[0].abs() + f[1].abs()).sum()) + 0.02 * float((dx.cpu().to(F64) * step).abs().sum())
+    assert abs(float(f[0].sum() - f[1].sum()) - float((dx.cpu().to(F64) * step).sum())) <= noise
+
+
+# ---- use --------------------------------------------------------------------------------------
+
+def test_captured_step_replays_like_the_eager_one(T):
+    """A whole token step as a graph, replayed with eager work between: the same bits each time."""
+    import xdna_train  # noqa: F401
+    V, D, F, n = 500, 64, 96, 70
+    g = gen(50)
+    table = torch.randn(V, D, generator=g).bfloat16().to("xdna").requires_grad_()
+    w_in = (torch.randn(2 * F, D, generator=g) / 8).bfloat16().to("xdna").requires_grad_()
+    w_out = (torch.randn(D, F, generator=g) / 10).bfloat16().to("xdna").requires_grad_()
+    ids = torch.randint(0, V, (n,), generator=g).to("xdna")
+    t_ids = torch.randint(0, V, (n, 6), generator=g).to("xdna")
+    t = torch.randn(n, 6, generator=g).to("xdna")
+    params = [table, w_in, w_out]
+
+    def step():
+        x = T.embed(ids, table, scale=8.0)
+        logits = torch.mm(x + T.gated_mlp(x, w_in, w_out), table.t())
+        loss = T.distill_loss(logits, t_ids, t)
+        r = T.token_log_probs(logits, ids, top_k=3)
+        return [loss.detach(), r.log_probs.detach(), r.top_ids, *torch.autograd.grad(loss - r.log_probs.mean(), params)]
+
+    def fresh(seed):
+        return torch.randint(0, V, (n,), generator=gen(seed))
+
+    for _ in range(2):
+        step()
+    graph = torch.xdna.Graph()
+    with torch.xdna.graph(graph):
+        out = step()
+    for seed in (60, 61, 62):
+        ids.copy_(fresh(seed))
+        graph.replay()
+        torch.xdna.synchronize()
+        got = [o.cpu() for o in out]
+        torch.zeros(1000, device="xdna").add_(1).sum().item()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b.cpu())
+
+
+def test_refusals_on_the_device(T):
+    z = torch.zeros(2, 5, device="xdna")
+    y = torch.zeros(2, dtype=torch.long, device="xdna")
+    w = torch.zeros(4, 3, device="xdna")
+    x16 = torch.zeros(2, 6, dtype=BF16, device="xdna")
+    w16, wo16 = torch.zeros(8, 6, dtype=BF16, device="xdna"), torch.zeros(6, 4, dtype=BF16, device="xdna")
+    two = torch.zeros(2, 2, device="xdna")
+    bad = [
+        lambda: T.embed(y.float(), w), lambda: T.embed(y, w.half()), lambda: T.embed(y, w.view(2, 2, 3)),
+        lambda: T.embed(y, w, padding_idx=4), lambda: T.embed(y, w, scale=math.inf), lambda: T.embed(y.cpu(), w),
+        lambda: T.gated_linear(x16.float(), w16), lambda: T.gated_linear(x16, w16[:7]), lambda: T.gated_linear(x16, w16[:, :5]),
+        lambda: T.gated_linear(x16, w16, activation="tanh"), lambda: T.gated_mlp(x16, w16, wo16[:, :3]),
+        lambda: T.gated_mlp(x16, w16, wo16.float()), lambda: T.token_log_probs(z, y, top_k=6), lambda: T.token_log_probs(z, y, top_k=-1),
+        lambda: T.token_log_probs(z, y, temperature=0.0), lambda: T.token_log_probs(z, y, temperature=math.nan),
+        lambda: T.token_log_probs(z, y[:1]), lambda: T.token_log_probs(z.double(), y), lambda: T.token_log_probs(z, y.float()),
+        lambda: T.distill_loss(z, two.long(), two[:1]), lambda: T.distill_loss(z, two, two), lambda: T.distill_loss(z, two.long(), two.half()),
+        lambda: T.distill_loss(z, two.long(), two, temperature=-1.0), lambda: T.distill_loss(z, two.long(), two, reduction="max"),
+        lambda: T.distill_loss(z, two.long(), two, weight=torch.ones(3, device="xdna")), lambda: T.distill_loss(z, two.long(), two, weight=torch.ones(2)),
+        lambda: T.distill_loss(z, torch.zeros(2, 1025, dtype=torch.long, device="xdna"), torch.zeros(2, 1025, device="xdna")),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises((RuntimeError, ValueError)):
+            call()
+            pytest.fail(f"call {i} was taken")
+    zx = z.clone().requires_grad_()
+    (dz,) = torch.autograd.grad(T.token_log_probs(zx, y).entropy.sum(), [zx], retain_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        torch.autograd.grad(T.token_log_probs(zx, y).entropy.sum(), [zx], create_graph=True)

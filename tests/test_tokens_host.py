@@ -1,0 +1,108 @@
+"""Token-model operators on the host: the C ABI's argument checks (every call is refused before
+any launch, or has nothing to do) and the Python functions' refusals of CPU tensors."""
+import math
+
+import pytest
+import torch
+
+from xdna_train import hip_abi, tokens
+
+A = 0x1000  # an aligned address that no call dereferences
+
+
+def refused(rc, why):
+    return rc == -1 and why in hip_abi.last_error()
+
+
+def test_embedding_refuses_bad_arguments():
+    lib = hip_abi.load()
+
+    def fwd(ids=A, ib=8, n=4, w=A, dt=2, V=10, D=8, ld=8, out=A):
+        return lib.xdna_embed(ids, ib, n, w, dt, V, D, ld, 1.0, out, None)
+
+    for kw, why in [({"ids": None}, "null"), ({"w": None}, "null"), ({"out": None}, "null"), ({"ib": 2}, "4 or 8"), ({"dt": 3}, "dtype"),
+                    ({"n": -1}, "token count"), ({"n": (1 << 30) + 1}, "token count"), ({"V": 0}, "rows"), ({"V": (1 << 30) + 1}, "rows"),
+                    ({"D": 0}, "length"), ({"ld": 7}, "overlap"), ({"w": A + 1}, "misaligned"), ({"out": A + 2, "dt": 1}, "misaligned")]:
+        assert refused(fwd(**kw), why), (kw, hip_abi.last_error())
+    assert fwd(n=0, ids=None, w=None, out=None) == 0
+    need = lib.xdna_embed_bwd_workspace_bytes(4, 10, 8)
+    assert need > 0 and lib.xdna_embed_bwd_workspace_bytes(0, 10, 8) == 0
+
+    def bwd(ids=A, ib=8, n=4, g=A, dt=2, V=10, D=8, dw=A, ws=A, have=need):
+        return lib.xdna_embed_bwd(ids, ib, n, g, dt, 8, V, D, -1, 1.0, dw, ws, have, None)
+
+    for kw, why in [({"ids": None}, "null"), ({"g": None}, "null"), ({"dw": None}, "null"), ({"dw": A + 8}, "misaligned"),
+                    ({"ws": None}, "workspace"), ({"ws": A + 8}, "workspace"), ({"have": need - 1}, "workspace"), ({"ib": 1}, "4 or 8"),
+                    ({"dt": 0}, "dtype"), ({"V": 0}, "rows")]:
+        assert refused(bwd(**kw), why), (kw, hip_abi.last_error())
+
+
+def test_gated_refuses_bad_arguments():
+    lib = hip_abi.load()
+
+    def fwd(x=A, ldx=8, w=A, ldw=8, M=2, K=8, F=4, act=0, h=A, gu=A):
+        return lib.xdna_gated_bf16(x, ldx, w, ldw, M, K, F, act, h, gu, None)
+
+    for kw, why in [({"x": None}, "null"), ({"w": None}, "null"), ({"h": None}, "null"), ({"act": 3}, "activation"), ({"act": -1}, "activation"),
+                    ({"M": -1}, "sizes"), ({"K": 0}, "sizes"), ({"F": 0}, "sizes"), ({"ldx": 7}, "overlap"), ({"ldw": 7}, "overlap"),
+                    ({"M": 1 << 29}, "rows"), ({"x": A + 1}, "misaligned"), ({"gu": A + 1}, "misaligned")]:
+        assert refused(fwd(**kw), why), (kw, hip_abi.last_error())
+    assert fwd(M=0, x=None, h=None) == 0
+
+    def bwd(dh=A, gu=A, M=2, F=4, act=0, dgu=A):
+        return lib.xdna_gated_bwd_bf16(dh, 4, gu, M, F, act, dgu, None)
+
+    for kw, why in [({"dh": None}, "null"), ({"gu": None}, "null"), ({"dgu": None}, "null"), ({"act": 9}, "activation"), ({"F": -1}, "sizes"),
+                    ({"dgu": A + 1}, "misaligned")]:
+        assert refused(bwd(**kw), why), (kw, hip_abi.last_error())
+
+
+def test_rows_over_a_vocabulary_refuse_bad_arguments():
+    lib = hip_abi.load()
+    assert lib.xdna_token_logprobs_workspace_bytes(2, 100, 0) == 0
+    need = lib.xdna_token_logprobs_workspace_bytes(2, 100000, 5)
+    assert need > 0 and lib.xdna_token_logprobs_workspace_bytes(2, 1 << 23, 5) == 0
+
+    def fwd(z=A, dt=2, n=2, V=100000, ld=100000, y=A, ib=8, tau=1.0, top=5, lp=A, h=A, st=A, tl=A, ti=A, ws=A, have=need):
+        return lib.xdna_token_logprobs(z, dt, n, V, ld, y, ib, tau, top, lp, h, st, tl, ti, ws, have, None)
+
+    for kw, why in [({"z": None}, "null"), ({"y": None}, "null"), ({"lp": None}, "null"), ({"h": None}, "null"), ({"st": None}, "null"),
+                    ({"ti": None}, "null"), ({"dt": 3}, "dtype"), ({"n": -1}, "row count"), ({"V": 0}, "vocabulary"), ({"V": (1 << 22) + 1}, "vocabulary"),
+                    ({"ld": 99999}, "overlap"), ({"tau": 0.0}, "temperature"), ({"tau": math.inf}, "temperature"), ({"tau": math.nan}, "temperature"),
+                    ({"top": 65}, "top"), ({"top": -1}, "top"), ({"V": 4, "ld": 4}, "top"), ({"ib": 2}, "4 or 8"), ({"z": A + 1}, "misaligned"),
+                    ({"ws": None}, "workspace"), ({"have": need - 1}, "workspace"), ({"ws": A + 4}, "workspace"), ({"st": A + 4}, "misaligned")]:
+        assert refused(fwd(**kw), why), (kw, hip_abi.last_error())
+    assert fwd(n=0, z=None, y=None) == 0
+
+    def bwd(z=A, dt=2, n=2, V=100, ld=100, y=A, st=A, h=A, dz=A):
+        return lib.xdna_token_logprobs_bwd(z, dt, n, V, ld, y, 8, 1.0, st, h, None, None, dz, None)
+
+    for kw, why in [({"z": None}, "null"), ({"st": None}, "null"), ({"dz": None}, "null"), ({"dz": A + 1}, "misaligned"), ({"ld": 10}, "overlap")]:
+        assert refused(bwd(**kw), why), (kw, hip_abi.last_error())
+
+    def dis(z=A, n=2, V=100, ld=100, ids=A, ib=8, t=A, td=1, k=4, tau=1.0, red=1, rl=A, sh=A, st=A, p=A, loss=A, inv=A):
+        return lib.xdna_distill(z, 2, n, V, ld, ids, ib, t, td, k, tau, None, red, rl, sh, st, p, loss, inv, None, 0, None)
+
+    for kw, why in [({"z": None}, "null"), ({"ids": None}, "null"), ({"t": None}, "null"), ({"p": None}, "null"), ({"loss": None}, "null"),
+                    ({"inv": None, "red": 2}, "null"), ({"k": 0}, "entries"), ({"k": 1025}, "entries"), ({"td": 3}, "teacher"), ({"red": 3}, "reduction"),
+                    ({"tau": -1.0}, "temperature"), ({"V": 100000, "ld": 100000}, "workspace"), ({"st": A + 4}, "misaligned")]:
+        assert refused(dis(**kw), why), (kw, hip_abi.last_error())
+
+    def dbwd(z=A, k=4, go=A, gd=1, dz=A, st=A):
+        return lib.xdna_distill_bwd(z, 2, 2, 100, 100, A, 8, k, 1.0, A, st, A, None, go, gd, 0, dz, None)
+
+    for kw, why in [({"z": None}, "null"), ({"go": None}, "null"), ({"dz": None}, "null"), ({"gd": 0}, "incoming"), ({"k": 2000}, "entries"),
+                    ({"dz": A + 1}, "misaligned")]:
+        assert refused(dbwd(**kw), why), (kw, hip_abi.last_error())
+
+
+def test_cpu_tensors_and_unknown_names_are_refused():
+    y, z = torch.zeros(2, dtype=torch.long), torch.zeros(2, 5)
+    x16, w16 = torch.zeros(2, 6, dtype=torch.bfloat16), torch.zeros(8, 6, dtype=torch.bfloat16)
+    for call in (lambda: tokens.embed(y, z), lambda: tokens.gated_linear(x16, w16), lambda: tokens.gated_mlp(x16, w16, w16[:6, :4]),
+                 lambda: tokens.token_log_probs(z, y), lambda: tokens.distill_loss(z, y[:, None], z[:, :1])):
+        with pytest.raises(RuntimeError, match="xdna tensor"):
+            call()
+    for call in (lambda: tokens.gated_linear(x16, w16, activation="tanh"), lambda: tokens.distill_loss(z, y[:, None], z[:, :1], reduction="max")):
+        with pytest.raises(ValueError, match="must be one of"):
+            call()
