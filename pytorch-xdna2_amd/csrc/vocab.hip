@@ -15,12 +15,13 @@
 // -inf adds nothing anywhere (its e (z - m) would be 0 * inf).  NaN and +inf make the row's
 // results NaN.
 //
-// Layout: a workgroup holds a piece of one row in registers (32 elements a thread: all its
-// loads are in flight together, the maximum is known before the first exp and no sum is ever
-// rescaled), so the row is read once also where the largest entries are selected.  Rows
-// longer than a piece, or too few to fill the chip, are cut into pieces whose partial
-// results a second launch joins in piece order; every sum has a fixed order, so equal
-// inputs give equal bits.  The gradient kernels stream: read z, write dz.
+// Layout: a workgroup streams a row (or, where there are few rows, a piece of one: a second
+// launch joins the pieces in order), each thread with a running maximum and sums of its own
+// that are rescaled once per 4 loaded windows; the workgroup joins its threads once at the end.
+// Every sum has a fixed order, so equal inputs give equal bits.  The largest entries need no
+// second read of the row either: the threads' own maxima bound the top-th largest element, and
+// only the threads whose maximum reaches the bound look at their elements again.  The gradient
+// kernels stream: read z, write dz.
 #include "common.h"
 
 #include "../../include/xdna_hip.h"
@@ -28,8 +29,9 @@
 namespace xdna {
 namespace {
 
-constexpr int kPer = 32;              // elements of a piece per thread
+constexpr int kWin = 4;               // 16-byte windows of a thread per step
 constexpr int kMaxTop = 64;           // alternatives: one group maximum per lane bounds them
+constexpr int kMaxPieces = 64;        // pieces of a row: their lists fit the join's LDS
 constexpr int kMaxTeacher = 1024;     // teacher entries per row (held in LDS by the gradient)
 constexpr int64_t kMaxVocab = int64_t(1) << 22;
 constexpr int kCandidates = 1024;     // LDS list of elements that may be among the largest
@@ -127,39 +129,21 @@ __device__ inline float key_value(uint32_t k) { return __uint_as_float(k & 0x800
 __device__ inline uint64_t entry_of(uint32_t key, int idx) { return (uint64_t(key) << 32) | uint32_t(~idx); }
 __device__ inline int entry_index(uint64_t e) { return int(~uint32_t(e)); }
 
-__device__ inline uint64_t shfl64(uint64_t v, int lane) {
-  return (uint64_t(uint32_t(__shfl(int(v >> 32), lane, 64))) << 32) | uint32_t(__shfl(int(uint32_t(v)), lane, 64));
+__device__ inline uint64_t lane64(uint64_t v, int lane) {
+  return (uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), lane))) << 32) |
+         uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), lane));
 }
 
-// ---- reductions over a workgroup of NT threads -----------------------------------------------
-template <int NT>
-__device__ inline float block_max(float v, float* red) {
+__device__ inline float wave_max(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  if constexpr (NT > 64) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, red[w]);
-  }
   return v;
 }
 
-template <int NT>
-__device__ inline float2 block_sum2(float a, float b, float* red) {
+__device__ inline float wave_sum(float v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o, 64), b += __shfl_xor(b, o, 64);
-  if constexpr (NT > 64) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[2 * (threadIdx.x >> 6)] = a, red[2 * (threadIdx.x >> 6) + 1] = b;
-    __syncthreads();
-    a = red[0], b = red[1];
-#pragma unroll
-    for (int w = 1; w < NT / 64; ++w) a += red[2 * w], b += red[2 * w + 1];
-  }
-  return make_float2(a, b);
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
 }
 
 struct RowStat {
@@ -219,17 +203,41 @@ __device__ inline float2 kept_stats(const RowStat& st) {
   return st.s == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(st.m, 1.0f / st.s);
 }
 
+__device__ inline float teacher_at(const DistillOut& d, int64_t i) {
+  return d.teacher_dtype == 1 ? static_cast<const float*>(d.teacher)[i]
+                              : bf16_to_f32(static_cast<const uint16_t*>(d.teacher)[i]);
+}
+
+// What the end of a row needs from memory, loaded before the row's logits are (a chain of two
+// or three loads there would wait a memory latency each).  One entry per thread: the target, or
+// the lane's first teacher entry.
+struct Early {
+  int64_t id = -1;
+  float z = 0.0f, t = 0.0f, weight = 1.0f;
+};
+
+template <typename T, int MODE>
+__device__ inline Early early_loads(const RowArgs& a, int64_t row) {
+  Early r;
+  if (MODE == kLogprob) {
+    if (threadIdx.x == 0) r.id = index_at(a.lp.targets, a.lp.index_bytes, row);
+  } else if (threadIdx.x < 64) {
+    if (int(threadIdx.x) < a.ds.k) {
+      r.id = index_at(a.ds.ids, a.ds.index_bytes, row * a.ds.k + threadIdx.x);
+      r.t = teacher_at(a.ds, row * a.ds.k + threadIdx.x);
+    }
+    if (a.ds.weight) r.weight = a.ds.weight[row];
+  }
+  if (r.id >= 0 && r.id < a.V) r.z = load_one<T>(static_cast<const T*>(a.z) + row * a.ld + r.id);
+  return r;
+}
+
 // A row's log probability, entropy and kept statistics (one thread).
-template <typename T>
-__device__ inline void logprob_row(const RowArgs& a, int64_t row, const RowStat& st) {
+__device__ inline void logprob_row(const RowArgs& a, int64_t row, const RowStat& st, const Early& early) {
   const float log_s = logf(st.s);
   a.lp.stats[row] = kept_stats(st);
   a.lp.entropy[row] = st.s == 0.0f ? 0.0f : log_s - st.u * a.inv_tau / st.s;
-  const int64_t y = index_at(a.lp.targets, a.lp.index_bytes, row);
-  float v = 0.0f;
-  if (y >= a.V) v = NAN;
-  else if (y >= 0) v = log_q(st, log_s, load_one<T>(static_cast<const T*>(a.z) + row * a.ld + y), a.inv_tau);
-  a.lp.log_probs[row] = v;
+  a.lp.log_probs[row] = early.id >= a.V ? NAN : early.id >= 0 ? log_q(st, log_s, early.z, a.inv_tau) : 0.0f;
 }
 
 __device__ inline void top_store(const RowArgs& a, int64_t row, int rank, uint64_t e, const RowStat& st, float log_s) {
@@ -237,283 +245,427 @@ __device__ inline void top_store(const RowArgs& a, int64_t row, int rank, uint64
   a.lp.top_ids[row * a.lp.top + rank] = entry_index(e);
 }
 
-__device__ inline float teacher_at(const DistillOut& d, int64_t i) {
-  return d.teacher_dtype == 1 ? static_cast<const float*>(d.teacher)[i]
-                              : bf16_to_f32(static_cast<const uint16_t*>(d.teacher)[i]);
-}
-
-// A row's distillation loss from its statistics (one wave).
+// A row's distillation loss from its statistics (one wave): its first 64 entries are in `early`.
 template <typename T>
-__device__ inline void distill_row(const RowArgs& a, int64_t row, const RowStat& st) {
+__device__ inline void distill_row(const RowArgs& a, int64_t row, const RowStat& st, const Early& early) {
   const DistillOut& d = a.ds;
   const int lane = threadIdx.x & 63;
   const float log_s = logf(st.s);
   const int64_t at = row * d.k;
+  const auto entry = [&](int j) {
+    Early r = early;
+    if (j >= 64) {
+      r.id = index_at(d.ids, d.index_bytes, at + j);
+      r.t = teacher_at(d, at + j);
+    }
+    if (r.id < 0 || r.id >= a.V) r.t = -INFINITY;  // absent
+    return r;
+  };
   float tm = -INFINITY;
   bool bad = false;
   for (int j = lane; j < d.k; j += 64) {
-    const int64_t id = index_at(d.ids, d.index_bytes, at + j);
-    bad |= id >= a.V;
-    if (id >= 0 && id < a.V) tm = fmaxf(tm, teacher_at(d, at + j));
+    const Early r = entry(j);
+    bad |= r.id >= a.V;
+    tm = fmaxf(tm, r.t);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor(tm, o, 64));
+  tm = wave_max(tm);
   const float c = a.inv_tau * kLog2e;
   float ts = 0.0f;
   bool some = false;
   for (int j = lane; j < d.k; j += 64) {
-    const int64_t id = index_at(d.ids, d.index_bytes, at + j);
-    const float t = teacher_at(d, at + j);
-    if (id >= 0 && id < a.V && t != -INFINITY) ts += exp2_hw((t - tm) * c), some = true;
+    const float t = entry(j).t;
+    if (t != -INFINITY) ts += exp2_hw((t - tm) * c), some = true;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) ts += __shfl_xor(ts, o, 64);
+  ts = wave_sum(ts);
   const float inv = 1.0f / ts, log_ts = logf(ts);
   float sum = 0.0f;
   for (int j = lane; j < d.k; j += 64) {
-    const int64_t id = index_at(d.ids, d.index_bytes, at + j);
-    const float t = teacher_at(d, at + j);
+    const Early r = entry(j);
     float p = 0.0f;
-    if (id >= 0 && id < a.V && t != -INFINITY) {
-      p = exp2_hw((t - tm) * c) * inv;
-      const float z = load_one<T>(static_cast<const T*>(a.z) + row * a.ld + id);
+    if (r.t != -INFINITY) {
+      p = exp2_hw((r.t - tm) * c) * inv;
+      const float z = j < 64 ? r.z : load_one<T>(static_cast<const T*>(a.z) + row * a.ld + r.id);
       // p ln(p / q) is 0 where p underflows, also against q = 0
-      if (p != 0.0f) sum += p * (((t - tm) * a.inv_tau - log_ts) - log_q(st, log_s, z, a.inv_tau));
+      if (p != 0.0f) sum += p * (((r.t - tm) * a.inv_tau - log_ts) - log_q(st, log_s, z, a.inv_tau));
     }
     d.p[at + j] = p;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  sum = wave_sum(sum);
   const bool any_bad = __any(bad), any_some = __any(some);
   if (lane == 0) {
-    const float w = any_some ? (d.weight ? d.weight[row] : 1.0f) : 0.0f;
+    const float w = any_some ? early.weight : 0.0f;
     d.stats[row] = kept_stats(st);
     d.share[row] = w;
     d.loss[row] = any_bad ? NAN : w == 0.0f ? 0.0f : w * (d.tau * d.tau) * sum;
   }
 }
 
+// ---- selection of the largest entries ----------------------------------------------------------
+
 template <int NT>
 struct TopShared {
-  uint64_t best[NT > 64 ? NT / 64 : 1][64];
-  uint64_t cand[kCandidates];
+  uint64_t best[NT > 64 ? NT : 1];  // the threads' largest, by group
+  uint64_t cand[kCandidates + kMaxTop];
   uint64_t bound;
-  int count;
+  int count, ties, total[NT / 64];
 };
 
-// The `top` largest entries of the piece in registers, through `put(rank, entry)`; ranks past
-// the piece's elements get entry 0 where `fill`.
-//   Bound: the top-th largest of 64 group maxima (a group = the threads of equal lane): at
-// least `top` elements reach it, and in rows without special order hardly more.
-//   The elements that reach it go to an LDS list, each candidate's rank is the count of
-// greater ones (entries are unique: no order of arrival matters).
-//   More candidates than the list holds (rows whose largest entries sit in few groups): the
-// exact bound is found by bisection over the entries' 64 bits, counted over the workgroup.
-template <typename T, int NT, typename Put>
-__device__ inline void select_top(const Raw (&r)[kPer / Win<T>::VW], int lo, int len, int top, bool fill,
-                                  TopShared<NT>& sh, float* red, Put put) {
-  constexpr int VW = Win<T>::VW, NW = kPer / VW;
+// The top-th largest of 64 groups' largest entries (a group: threads of one lane, skewed by
+// wave), 0 where fewer groups hold one: at least `top` entries reach it, and in rows without
+// special order hardly more.
+template <int NT>
+__device__ inline uint64_t group_bound(uint64_t best, int top, TopShared<NT>& sh) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint64_t best = 0;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    const int base = (tid + i * NT) * VW;
-    uint32_t bk = 0;
-    int bi = 0;
-#pragma unroll
-    for (int e = 0; e < VW; ++e) {
-      const uint32_t key = base + e < len ? order_key(raw_get<T>(r[i], e)) : 0u;
-      if (key > bk) bk = key, bi = e;
-    }
-    const uint64_t en = bk ? entry_of(bk, lo + base + bi) : 0;
-    best = en > best ? en : best;
-  }
-  if (NT > 64) {
-    sh.best[wave][lane] = best;
+  if constexpr (NT > 64) {
+    sh.best[wave * 64 + ((lane + 17 * wave) & 63)] = best;
     __syncthreads();
   }
   if (wave == 0) {
-    if (NT > 64) {
 #pragma unroll
-      for (int w = 1; w < NT / 64; ++w) best = sh.best[w][lane] > best ? sh.best[w][lane] : best;
-    }
+    for (int w = 1; w < NT / 64; ++w) best = sh.best[w * 64 + lane] > best ? sh.best[w * 64 + lane] : best;
     int rank = 0;
-    for (int l = 0; l < 64; ++l) {
-      const uint64_t o = shfl64(best, l);
-      rank += o > best ? 1 : 0;
-    }
-    // groups without an element all hold 0: then every element is a candidate
+#pragma unroll 16
+    for (int l = 0; l < 64; ++l) rank += lane64(best, l) > best ? 1 : 0;
     const uint64_t hit = __ballot(rank == top - 1 && best != 0);
-    const uint64_t bound = hit ? shfl64(best, __ffsll(static_cast<unsigned long long>(hit)) - 1) : 1;
+    const uint64_t bound = hit ? lane64(best, __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1)) : 0;
     if (lane == 0) sh.bound = bound, sh.count = 0;
   }
   __syncthreads();
-  uint64_t bound = sh.bound;
-  for (int attempt = 0; attempt < 2; ++attempt) {
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const int base = (tid + i * NT) * VW;
-#pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        if (base + e >= len) continue;
-        const uint64_t en = entry_of(order_key(raw_get<T>(r[i], e)), lo + base + e);
-        if (en >= bound) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kCandidates) sh.cand[at] = en;
-        }
-      }
-    }
-    __syncthreads();
-    if (sh.count <= kCandidates) break;
-    // the largest bound that at least `top` elements reach
-    uint64_t exact = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t trial = exact | (uint64_t(1) << bit);
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) {
-        const int base = (tid + i * NT) * VW;
-#pragma unroll
-        for (int e = 0; e < VW; ++e)
-          n += base + e < len && entry_of(order_key(raw_get<T>(r[i], e)), lo + base + e) >= trial ? 1 : 0;
-      }
-      const float2 total = block_sum2<NT>(float(n), 0.0f, red);  // counts below 2^24: exact
-      if (total.x >= float(top)) exact = trial;
-    }
-    bound = exact;
-    __syncthreads();
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-  }
-  const int n = min(sh.count, kCandidates);
-  for (int c = tid; c < n; c += NT) {
+  return sh.bound;
+}
+
+// Ranks the n candidates (entries are unique: their order of arrival does not matter) and
+// hands the first `top` to put(rank, entry); `fill`: entry 0 for ranks past them.
+template <int NT, typename Put>
+__device__ inline void rank_candidates(const TopShared<NT>& sh, int n, int top, bool fill, Put put) {
+  for (int c = threadIdx.x; c < n; c += NT) {
     const uint64_t en = sh.cand[c];
     int rank = 0;
+#pragma unroll 4
     for (int o = 0; o < n; ++o) rank += sh.cand[o] > en ? 1 : 0;
     if (rank < top) put(rank, en);
   }
   if (fill)
-    for (int c = n + tid; c < top; c += NT) put(c, uint64_t(0));
+    for (int c = n + int(threadIdx.x); c < top; c += NT) put(c, uint64_t(0));
 }
 
-// One piece of a row: statistics, and for log probabilities its largest entries; rows of one
-// piece are finished here.
-// Measured: see the launchers' rule below.
+template <int NT>
+__device__ inline int block_count(int n, TopShared<NT>& sh) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  if constexpr (NT > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.total[threadIdx.x >> 6] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) n += sh.total[w];
+  }
+  return n;
+}
+
+// The `top` largest of the piece z[0, len) (element 0 has index lo in its row), through
+// put(rank, entry).  m: the thread's maximum over its windows tid, tid + NT, ...
+//   Usual rows: the elements of value at least the bound go to an LDS list, found by the threads
+// whose maximum reaches it.
+//   Rows where that list overflows, or where the bound is -inf (fewer allowed tokens than asked
+// for): the elements above the bound only, and as many equal ones as are still wanted in index
+// order, by a scan that ends when it has them.
+//   Rows where even those overflow (the largest elements sit in few groups) or that hold NaN:
+// the exact top-th largest key by bisection, then the same.
+template <typename T, int NT, typename Put>
+__device__ inline void select_top(const T* z, int lo, int len, int top, bool fill, float m, bool nan,
+                                  TopShared<NT>& sh, Put put) {
+  constexpr int VW = Win<T>::VW;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const bool mine = tid * VW < len;
+  uint32_t bound = uint32_t(group_bound<NT>(mine ? uint64_t(order_key(m)) << 32 | uint32_t(~tid) : 0, top, sh) >> 32);
+  const uint32_t lowest = order_key(-INFINITY);
+  if (bound == 0) bound = lowest;
+  const auto scan = [&](uint32_t from, bool all) {  // entries of key >= from to the list
+    const float fb = key_value(from);
+    if (all || m >= fb) {
+#pragma unroll 2
+      for (int at = tid * VW; at < len; at += NT * VW) {
+        const Raw r = load_win<T>(z + at, len - at);
+        float wm = raw_get<T>(r, 0);
+#pragma unroll
+        for (int e = 1; e < VW; ++e) wm = fmaxf(wm, raw_get<T>(r, e));
+        if (!all && !(wm >= fb)) continue;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          const uint32_t key = order_key(raw_get<T>(r, e));
+          if (at + e < len && key >= from) {
+            const int c = atomicAdd(&sh.count, 1);
+            if (c < kCandidates) sh.cand[c] = entry_of(key, lo + at + e);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    return sh.count;
+  };
+  if (!nan && bound > lowest) {
+    const int n = scan(bound, false);
+    if (n <= kCandidates) {
+      rank_candidates<NT>(sh, n, top, fill, put);
+      return;
+    }
+  }
+  int n = kCandidates + 1;
+  if (!nan) {
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    n = scan(bound + 1, false);
+  }
+  if (n > kCandidates) {
+    bound = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t trial = bound | (1u << bit);
+      int c = 0;
+      for (int at = tid * VW; at < len; at += NT * VW) {
+        const Raw r = load_win<T>(z + at, len - at);
+#pragma unroll
+        for (int e = 0; e < VW; ++e) c += at + e < len && order_key(raw_get<T>(r, e)) >= trial ? 1 : 0;
+      }
+      if (block_count<NT>(c, sh) >= top) bound = trial;
+    }
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    n = scan(bound + 1, true);  // fewer than top
+  }
+  // elements equal to the bound, in index order
+  int want = top - n;
+  for (int base = 0; base < len && want > 0; base += NT * VW) {
+    const int at = base + tid * VW;
+    int hits = 0;
+    if (at < len) {
+      const Raw r = load_win<T>(z + at, len - at);
+#pragma unroll
+      for (int e = 0; e < VW; ++e) hits |= (at + e < len && order_key(raw_get<T>(r, e)) == bound ? 1 : 0) << e;
+    }
+    int before = __popc(hits);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(before, o, 64);
+      if (lane >= o) before += t;
+    }
+    int all = __shfl(before, 63, 64);
+    before -= __popc(hits);
+    if constexpr (NT > 64) {
+      __syncthreads();
+      if (lane == 0) sh.total[wave] = all;
+      __syncthreads();
+      all = 0;
+#pragma unroll
+      for (int w = 0; w < NT / 64; ++w) {
+        before += w < wave ? sh.total[w] : 0;
+        all += sh.total[w];
+      }
+    }
+    for (; hits && before < want; hits &= hits - 1, ++before)
+      sh.cand[n + before] = entry_of(bound, lo + at + __ffs(hits) - 1);
+    n += min(want, all);
+    want -= min(want, all);
+  }
+  __syncthreads();
+  rank_candidates<NT>(sh, n, top, fill, put);
+}
+
+// ---- forward ----------------------------------------------------------------------------------
+
+template <typename T>
+struct Steps {  // kWin windows of a thread
+  Raw r[kWin];
+};
+
+// One thread's running statistics over another kWin windows: the new maximum first, then the
+// old sums rescaled to it (by 0 while there were none) and the windows' terms.
+template <typename T, bool ENT>
+__device__ inline void accumulate(const Steps<T>& w, float c, float& m, float& s, float& u) {
+  constexpr int VW = Win<T>::VW;
+  float top = m;
+#pragma unroll
+  for (int i = 0; i < kWin; ++i)
+#pragma unroll
+    for (int e = 0; e < VW; ++e) top = fmaxf(top, raw_get<T>(w.r[i], e));
+  const float m0 = top == -INFINITY ? 0.0f : top;
+  if (top > m) {
+    const float d = m == -INFINITY ? -INFINITY : m - m0;
+    const float k = exp2_hw(d * c);
+    if (ENT) u = k * (u + fmaxf(d, -1.0e30f) * s);
+    s *= k;
+    m = top;
+  }
+#pragma unroll
+  for (int i = 0; i < kWin; ++i)
+#pragma unroll
+    for (int e = 0; e < VW; ++e) {
+      const float d = raw_get<T>(w.r[i], e) - m0;
+      const float x = exp2_hw(d * c);
+      s += x;
+      if (ENT) u = fmaf(x, fmaxf(d, -1.0e30f), u);  // -inf: 0 * a finite number
+    }
+}
+
+// (m, s, u) of several threads or pieces, joined at the overall maximum M
+template <bool ENT>
+__device__ inline void rescale(float M, float c, float m, float& s, float& u) {
+  const float d = m == M ? 0.0f : m - M;
+  const float k = s == 0.0f ? 0.0f : exp2_hw(d * c);  // s == 0: nothing but -inf (or nothing at all)
+  if (ENT) u = s == 0.0f ? 0.0f : k * (u + fmaxf(d, -1.0e30f) * s);  // (k is 0 long before the bound)
+  s *= k;
+}
+
+// A row (or a piece of one): statistics, and for log probabilities its largest entries.
 template <typename T, int NT, int MODE, bool TOP>
 __global__ __launch_bounds__(NT) void row_kernel(RowArgs a) {
-  constexpr int VW = Win<T>::VW, NW = kPer / VW;
-  __shared__ float red[2 * (NT / 64)];
+  constexpr int VW = Win<T>::VW, kStep = NT * VW * kWin;
+  constexpr bool ENT = MODE == kLogprob;
+  __shared__ float red[3][NT / 64];
   __shared__ TopShared<TOP ? NT : 64> sh;
   const int tid = threadIdx.x;
   const int64_t items = a.rows * a.pieces;
+  const float c = a.inv_tau * kLog2e;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t row = a.pieces == 1 ? item : item / a.pieces;
-    const int pi = a.pieces == 1 ? 0 : int(item - row * a.pieces);
-    const int lo = pi * a.piece;
+    const int lo = a.pieces == 1 ? 0 : int(item - row * a.pieces) * a.piece;
     const int len = min(a.piece, a.V - lo);
     const T* z = static_cast<const T*>(a.z) + row * a.ld + lo;
-    Raw r[NW];
+    Early early;
+    if (a.pieces == 1) early = early_loads<T, MODE>(a, row);
+    float m = -INFINITY, s = 0.0f, u = 0.0f;
+    const int whole = len / kStep * kStep;  // elements in whole steps of the workgroup
+    const auto load = [&](int at) {
+      Steps<T> w;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const int at = (tid + i * NT) * VW;
-      r[i] = load_win<T>(z + min(at, len), len - at);
-    }
-    float m = -INFINITY;
+      for (int i = 0; i < kWin; ++i) {
+        const Pix8 q = *reinterpret_cast<const Pix8*>(z + at + (tid + i * NT) * VW);
 #pragma unroll
-    for (int i = 0; i < NW; ++i)
-#pragma unroll
-      for (int e = 0; e < VW; ++e) m = fmaxf(m, raw_get<T>(r[i], e));
-    m = block_max<NT>(m, red);
-    const float c = a.inv_tau * kLog2e;
-    const float m0 = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f, u = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-#pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        const float d = raw_get<T>(r[i], e) - m0;
-        const float x = exp2_hw(d * c);
-        s += x;
-        // -inf: 0 * a finite number
-        if (MODE == kLogprob) u += x * fmaxf(d, -1.0e30f);
+        for (int k = 0; k < 4; ++k) w.r[i].w[k] = q.v[k];
       }
+      return w;
+    };
+    if (whole > 0) {
+      Steps<T> next = load(0);
+      for (int at = kStep; at < whole; at += kStep) {
+        const Steps<T> w = next;
+        next = load(at);
+        accumulate<T, ENT>(w, c, m, s, u);
+      }
+      accumulate<T, ENT>(next, c, m, s, u);
     }
-    const float2 su = block_sum2<NT>(s, u, red);
-    const RowStat st = {m, su.x, su.y};
+    if (whole < len) {
+      Steps<T> w;
+#pragma unroll
+      for (int i = 0; i < kWin; ++i) {
+        const int at = whole + (tid + i * NT) * VW;
+        w.r[i] = load_win<T>(z + min(at, len), len - at);
+      }
+      accumulate<T, ENT>(w, c, m, s, u);
+    }
+    float M = wave_max(m);
+    if constexpr (NT > 64) {
+      __syncthreads();
+      if ((tid & 63) == 0) red[0][tid >> 6] = M;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < NT / 64; ++w) M = fmaxf(M, red[0][w]);
+    }
+    rescale<ENT>(M, c, m, s, u);
+    s = wave_sum(s);
+    if (ENT) u = wave_sum(u);
+    if constexpr (NT > 64) {
+      if ((tid & 63) == 0) red[1][tid >> 6] = s, red[2][tid >> 6] = u;
+      __syncthreads();
+      s = red[1][0], u = red[2][0];
+#pragma unroll
+      for (int w = 1; w < NT / 64; ++w) s += red[1][w], u += red[2][w];
+    }
+    const RowStat st = {M, s, u};
     if (a.pieces > 1) {
       if (tid == 0) a.stat[item] = st;
       if constexpr (TOP) {
         uint64_t* list = a.list + item * a.lp.top;
-        select_top<T, NT>(r, lo, len, a.lp.top, true, sh, red, [&](int rank, uint64_t e) { list[rank] = e; });
+        select_top<T, NT>(z, lo, len, a.lp.top, true, m, s != s, sh, [&](int rank, uint64_t e) { list[rank] = e; });
       }
     } else if constexpr (MODE == kLogprob) {
-      if (tid == 0) logprob_row<T>(a, row, st);
+      if (tid == 0) logprob_row(a, row, st, early);
       if constexpr (TOP) {
         const float log_s = logf(st.s);
-        select_top<T, NT>(r, lo, len, a.lp.top, false, sh, red,
+        select_top<T, NT>(z, lo, len, a.lp.top, false, m, s != s, sh,
                           [&](int rank, uint64_t e) { top_store(a, row, rank, e, st, log_s); });
       }
     } else {
-      if (tid < 64) distill_row<T>(a, row, st);
+      if (tid < 64) distill_row<T>(a, row, st, early);
     }
-    if (TOP) __syncthreads();  // the next piece reuses the LDS lists
+    if (TOP) __syncthreads();  // the next item reuses the LDS lists
   }
 }
 
-// Joins the pieces of a row, in piece order: one workgroup of 256 per row.
-constexpr int kJoinEntries = 8192;
+// Joins the pieces of a row, in piece order: one workgroup per row.
+constexpr int kJoinThreads = 256;
 
 template <typename T, int MODE, bool TOP>
-__global__ __launch_bounds__(256) void join_kernel(RowArgs a) {
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(RowArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint64_t lists[];
+  __shared__ TopShared<TOP ? kJoinThreads : 64> sh;
+  constexpr bool ENT = MODE == kLogprob;
   const int tid = threadIdx.x, lane = tid & 63;
   const float c = a.inv_tau * kLog2e;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const RowStat* stat = a.stat + row * a.pieces;
-    float m = -INFINITY;
-    for (int p = lane; p < a.pieces; p += 64) m = fmaxf(m, stat[p].m);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    float s = 0.0f, u = 0.0f;
-    for (int p = lane; p < a.pieces; p += 64) {
-      const RowStat q = stat[p];
-      if (q.s == 0.0f) continue;  // nothing but -inf
-      const float w = exp2_hw((q.m - m) * c);
-      s += w * q.s;
-      u += w * (q.u + (q.m - m) * q.s);
+    if (MODE == kDistill && tid >= 64) continue;
+    const Early early = early_loads<T, MODE>(a, row);
+    const int n = a.pieces * a.lp.top;
+    uint64_t best = 0;
+    if constexpr (TOP) {
+      for (int i = tid; i < n; i += kJoinThreads) {
+        const uint64_t e = a.list[row * n + i];
+        lists[i] = e;
+        best = e > best ? e : best;
+      }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64), u += __shfl_xor(u, o, 64);
-    const RowStat st = {m, s, u};
+    RowStat q = {-INFINITY, 0.0f, 0.0f};  // (a row has at most 64 pieces)
+    if (lane < a.pieces) q = a.stat[row * a.pieces + lane];
+    const float m = wave_max(q.m);
+    rescale<ENT>(m, c, q.m, q.s, q.u);
+    const RowStat st = {m, wave_sum(q.s), wave_sum(q.u)};
     if constexpr (MODE == kDistill) {
-      if (tid < 64) distill_row<T>(a, row, st);
+      distill_row<T>(a, row, st, early);
     } else {
-      if (tid == 0) logprob_row<T>(a, row, st);
+      if (tid == 0) logprob_row(a, row, st, early);
       if constexpr (TOP) {
-        const int top = a.lp.top, n = a.pieces * top;
-        __syncthreads();
-        for (int i = tid; i < n; i += 256) lists[i] = a.list[row * n + i];
-        __syncthreads();
         const float log_s = logf(st.s);
-        for (int i = tid; i < n; i += 256) {
-          const uint64_t e = lists[i];
-          if (e == 0) continue;
-          const int mine = i / top;
-          int rank = i - mine * top;
-          // entries greater than e in each other list (sorted descending)
-          for (int p = 0; p < a.pieces && rank < top; ++p) {
-            if (p == mine) continue;
-            const uint64_t* l = lists + p * top;
-            int b = 0, t = top;
-            while (b < t) {
-              const int h = (b + t) >> 1;
-              if (l[h] > e) b = h + 1;
-              else t = h;
+        uint64_t bound = group_bound<kJoinThreads>(best, a.lp.top, sh);
+        bound = bound ? bound : 1;
+        const auto collect = [&] {
+          for (int i = tid; i < n; i += kJoinThreads)
+            if (lists[i] >= bound) {
+              const int at = atomicAdd(&sh.count, 1);
+              if (at < kCandidates) sh.cand[at] = lists[i];
             }
-            rank += b;
+          __syncthreads();
+          return sh.count;
+        };
+        int count = collect();
+        if (count > kCandidates) {  // the exact top-th largest entry, by bisection
+          bound = 0;
+          for (int bit = 63; bit >= 0; --bit) {
+            const uint64_t trial = bound | (uint64_t(1) << bit);
+            int k = 0;
+            for (int i = tid; i < n; i += kJoinThreads) k += lists[i] >= trial ? 1 : 0;
+            if (block_count<kJoinThreads>(k, sh) >= a.lp.top) bound = trial;
           }
-          if (rank < top) top_store(a, row, rank, e, st, log_s);
+          __syncthreads();
+          if (tid == 0) sh.count = 0;
+          __syncthreads();
+          count = collect();
         }
+        rank_candidates<kJoinThreads>(sh, count, a.lp.top, false,
+                                      [&](int rank, uint64_t e) { top_store(a, row, rank, e, st, log_s); });
+        __syncthreads();
       }
     }
   }
@@ -677,17 +829,12 @@ struct Plan {
   int threads, piece, pieces;
 };
 
-// Pieces of one row: one piece where a workgroup can hold the row, else pieces of equal
-// length.  Few rows take small workgroups, so that more of them share the work.
-Plan row_plan(int64_t rows, int64_t V, int top) {
+// Whole rows where they fill the chip (two workgroups a CU), else pieces of equal length, of
+// at least one step of the workgroup.
+Plan row_plan(int64_t rows, int64_t V) {
   Plan p;
-  const auto cap = [](int nt) { return int64_t(nt) * kPer; };
-  if (V <= cap(64)) p.threads = 64;
-  else if (V <= cap(256) || rows * ceil_div(V, cap(1024)) < 256) p.threads = 256;
-  else p.threads = 1024;
-  // the join holds every piece's list
-  if (top > 0 && ceil_div(V, cap(p.threads)) * top > kJoinEntries) p.threads = 1024;
-  p.pieces = int(ceil_div(V, cap(p.threads)));
+  p.threads = V <= 2048 ? 64 : 256;
+  p.pieces = rows >= 512 ? 1 : int(std::min<int64_t>({ceil_div(V, int64_t(4096)), ceil_div(int64_t(1024), rows), kMaxPieces}));
   p.piece = int(ceil_div(ceil_div(V, int64_t(p.pieces)), int64_t(8)) * 8);
   p.pieces = int(ceil_div(V, int64_t(p.piece)));
   return p;
@@ -712,22 +859,20 @@ size_t list_offset(int64_t rows, const Plan& p) {
 }
 
 size_t row_workspace(int64_t rows, int64_t V, int top) {
-  const Plan p = row_plan(rows, V, top);
+  const Plan p = row_plan(rows, V);
   if (p.pieces == 1) return 0;
   return list_offset(rows, p) + size_t(rows) * p.pieces * top * sizeof(uint64_t);
 }
 
 template <typename T, int MODE, bool TOP>
-bool launch_row(const Plan& p, const RowArgs& a, hipStream_t st) {
+void launch_row(const Plan& p, const RowArgs& a, hipStream_t st) {
   const int64_t items = a.rows * a.pieces;
   if (p.threads == 64) row_kernel<T, 64, MODE, TOP><<<grid_of(items, 64), 64, 0, st>>>(a);
-  else if (p.threads == 256) row_kernel<T, 256, MODE, TOP><<<grid_of(items, 256), 256, 0, st>>>(a);
-  else row_kernel<T, 1024, MODE, TOP><<<grid_of(items, 1024), 1024, 0, st>>>(a);
+  else row_kernel<T, 256, MODE, TOP><<<grid_of(items, 256), 256, 0, st>>>(a);
   if (a.pieces > 1) {
     const size_t lds = TOP ? size_t(a.pieces) * a.lp.top * sizeof(uint64_t) : 0;
-    join_kernel<T, MODE, TOP><<<grid_of(a.rows, 256), 256, lds, st>>>(a);
+    join_kernel<T, MODE, TOP><<<grid_of(a.rows, kJoinThreads), kJoinThreads, lds, st>>>(a);
   }
-  return true;
 }
 
 bool rows_ok(const char* what, const void* z, int dtype, int64_t rows, int64_t V, int64_t ld, float tau) {
@@ -783,7 +928,7 @@ int xdna_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t voc
   if (off(stats, 8)) return refuse(what, "misaligned stats");
   if (!workspace_ok(what, workspace, workspace_bytes, row_workspace(rows, vocab, top))) return -1;
   if (!admit_launch(what)) return -1;
-  const Plan p = row_plan(rows, vocab, top);
+  const Plan p = row_plan(rows, vocab);
   RowArgs a = {};
   a.z = logits;
   a.ld = ld;
@@ -843,7 +988,7 @@ int xdna_distill(const void* logits, int dtype, int64_t rows, int64_t vocab, int
   if (!admit_launch(what)) return -1;
   hipStream_t st = as_stream(stream);
   if (rows > 0) {
-    const Plan pl = row_plan(rows, vocab, 0);
+    const Plan pl = row_plan(rows, vocab);
     RowArgs a = {};
     a.z = logits;
     a.ld = ld;
