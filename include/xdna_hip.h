@@ -836,6 +836,18 @@ int xdna_gated_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t l
 int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const uint16_t* gu, int64_t M, int64_t F, int act,
                         uint16_t* dgu, void* stream);
 
+/* The same from the block's output: dh = dy w_out (w_out: N rows of F) stays in fp32 between the
+ * product and the activation's gradient, in one launch. */
+int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_out, int64_t ldw, const uint16_t* gu,
+                            int64_t M, int64_t N, int64_t F, int act, uint16_t* dgu, void* stream);
+
+/* out[q * ldc + p] = sum over k of P[p][k] Q[q][k], for operands of any alignment and row stride:
+ * contiguous along k (p_rows / q_rows 0: element (r, k) at r * ld + k) or along the rows (1: at
+ * k * ld + r; q only where p is too).  The products of the gated block whose sizes the large
+ * tiles of xdna_gemm_bf16 cannot load as vectors. */
+int xdna_tile_mm_bf16(const uint16_t* p, int64_t ldp, int p_rows, const uint16_t* q, int64_t ldq, int q_rows, int64_t P,
+                      int64_t Q, int64_t K, uint16_t* out, int64_t ldc, void* stream);
+
 /* Per row of logits z (row stride ld), x = z / tau, q = softmax(x): log_probs = ln q[target]
  * (0 for a negative target, NaN past the vocabulary), entropy = -sum q ln q, the `top` (up to
  * 64) largest logits in order (ties to the lowest index) as ln q and index, and stats = (max z,

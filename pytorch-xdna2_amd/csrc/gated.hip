@@ -9,6 +9,7 @@
 //   dg = dh u act'(g), du = dh act(g), as [dg du] (M x 2F), so that dx = [dg du] w and
 //   dw = [dg du]^T x are one product each.
 #include "common.h"
+#include "gemm_dma.h"
 #include "mfma.h"
 
 #include "../../include/xdna_hip.h"
@@ -20,7 +21,7 @@ enum Act { kSilu = 0, kGelu = 1, kRelu = 2 };
 
 template <int ACT>
 __device__ inline float act_of(float g) {
-  if constexpr (ACT == kSilu) return g / (1.0f + __expf(-g));
+  if constexpr (ACT == kSilu) return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g));
   if constexpr (ACT == kGelu) return g * 0.5f * (1.0f + erff(g * 0.70710678118654752f));
   return g > 0.0f ? g : (g != g ? g : 0.0f);
 }
@@ -29,7 +30,7 @@ __device__ inline float act_of(float g) {
 template <int ACT>
 __device__ inline float2 act_pair(float g) {
   if constexpr (ACT == kSilu) {
-    const float s = 1.0f / (1.0f + __expf(-g));
+    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
     return make_float2(g * s, s * (1.0f + g * (1.0f - s)));
   }
   if constexpr (ACT == kGelu) {
@@ -39,20 +40,36 @@ __device__ inline float2 act_pair(float g) {
   return g > 0.0f ? make_float2(g, 1.0f) : make_float2(g != g ? g : 0.0f, 0.0f);
 }
 
-struct GatedArgs {
-  const uint16_t* x;  // [M][K], row stride ldx
-  const uint16_t* w;  // [2F][K], row stride ldw: gate rows, then up rows
-  uint16_t* h;        // [M][F]
-  uint16_t* gu;       // [M][2F] or null
-  int M, K, F;
-  int64_t ldx, ldw;
+// ---- products in tiles, any sizes, alignments and row strides --------------------------------
+// D[p][q] = sum over k of P[p][k] Q[q][k], written at out[q * ldc + p]: the p index is the one
+// that is contiguous in memory, so that the 4 consecutive rows an MFMA accumulator quad holds
+// are 4 consecutive elements of the output (and of [g u] beside it).  Each operand is contiguous
+// along k, or along its rows (then staged [k][row] and transposed by the LDS reads).  Loads are
+// 16 bytes at any element-aligned address (gfx950 takes them); out-of-range elements are zeros.
+//
+// Every wave multiplies a 64 x 64 block (2 x 2 MFMAs of 32x32x16: as many LDS reads as MFMAs):
+//   wide tiles, 128 x 128: four waves side by side, k-tiles of 64;
+//   narrow tiles, 64 x 64, where wide ones would leave CUs without work: eight waves on the
+// same block, each with its own k-step of a k-tile of 128 (an eighth of the k-tiles' memory
+// latencies of one wave), their accumulators added in wave order through LDS.
+// The next k-tile's loads fly in registers during a k-tile's MFMAs; one barrier per k-tile.
+enum TileEpi { kPlain = 0, kGated = 1, kGatedKeep = 2, kGatedGrad = 3 };
+
+struct TileOperand {
+  const uint16_t* src;
+  int64_t ld;  // between rows (k-contiguous), or between k (row-contiguous)
+  int rows;
 };
 
-// ---- tiles of 64 rows x 64 hidden units ---------------------------------------------------
-// Four waves of 32 x 32, each with a gate and an up accumulator; k-tiles of 64 in LDS ([row][k],
-// pitch 72) with the next one's loads in registers meanwhile.  Loads are 16 bytes at any
-// element-aligned address (gfx950 takes them), elements past K are zeros.
-constexpr int kT = 64, kKT = 64, kP = 72;
+struct TileArgs {
+  TileOperand p, q;
+  int K;
+  uint16_t* out;   // kPlain: D; kGated*: h; kGatedGrad: [dg du]
+  int64_t ldc;
+  uint16_t* gu;    // kGatedKeep: written; kGatedGrad: read
+  int F;           // kGated*: p.src holds F gate rows, then F up rows (p.rows = F)
+  int vec;         // 8-byte accesses of out and gu: their addresses and strides are multiples of 4
+};
 
 __device__ inline Pix8 row_vec(const uint16_t* p, int n) {  // n elements, zeros after them
   if (n >= 8) return *reinterpret_cast<const Pix8*>(p);
@@ -63,67 +80,389 @@ __device__ inline Pix8 row_vec(const uint16_t* p, int n) {  // n elements, zeros
   return q;
 }
 
-template <int ACT, bool KEEP>
-__global__ __launch_bounds__(256) void gated_tile_kernel(GatedArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t xs[2][kT * kP];
-  __shared__ __attribute__((aligned(16))) uint16_t ws[2][2 * kT * kP];
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+
+template <bool WIDE>
+struct Tile {
+  static constexpr int T = WIDE ? 128 : 64;        // rows of each operand
+  static constexpr int KT = WIDE ? 64 : 128;       // k per k-tile
+  static constexpr int NT = WIDE ? 256 : 512;      // threads
+  static constexpr int V = T * KT / 8 / NT;        // 16-byte vectors per thread and operand
+  static constexpr int PITCH = KT + 8;             // elements of a k-contiguous LDS row
+  static constexpr int ELEMS = T * PITCH;          // (a [k][row] tile is smaller)
+  static constexpr size_t LDS = size_t(2) * 2 * ELEMS * 2;
+};
+
+// Row of the operand that tile row r holds: itself, or (gated) 32 gate rows and the same 32
+// units' up rows in turn, so that one wave has both.  -1 past the operand.
+template <bool GATED>
+__device__ inline int64_t tile_row(const TileArgs& a, const TileOperand& o, int r0, int r) {
+  if constexpr (GATED) {
+    const int f = r0 / 2 + (r >> 6) * 32 + (r & 31);
+    return f < a.F ? f + int64_t((r >> 5) & 1) * a.F : -1;
+  }
+  return r0 + r < o.rows ? r0 + r : -1;
+}
+
+template <bool WIDE, bool ROWS, bool GATED>
+__device__ inline void tile_load(Pix8 (&v)[Tile<WIDE>::V], const TileArgs& a, const TileOperand& o, int r0, int k0,
+                                 int tid) {
+  using C = Tile<WIDE>;
+#pragma unroll
+  for (int j = 0; j < C::V; ++j) {
+    const int i = tid + j * C::NT;
+    if constexpr (!ROWS) {
+      constexpr int kVecs = C::KT / 8;
+      const int64_t r = tile_row<GATED>(a, o, r0, i / kVecs);
+      const int k = k0 + (i % kVecs) * 8;
+      v[j] = row_vec(o.src + (r < 0 ? 0 : r) * o.ld + min(k, a.K), r < 0 ? 0 : a.K - k);
+    } else {
+      constexpr int rVecs = C::T / 8;
+      const int r = r0 + (i % rVecs) * 8, k = k0 + i / rVecs;
+      v[j] = row_vec(o.src + int64_t(min(k, a.K - 1)) * o.ld + min(r, o.rows), k < a.K ? o.rows - r : 0);
+    }
+  }
+}
+
+// [k][row] tiles: 16-byte pieces of 8 rows, permuted by the k row so that the transposing reads'
+// 4 k rows fall on distinct banks
+template <bool WIDE>
+__device__ inline int piece_at(int kr, int q) {
+  return WIDE ? kr * 16 + (q ^ (4 * (kr & 3))) : kr * 8 + (q ^ (4 * ((kr >> 1) & 1)));
+}
+
+template <bool WIDE, bool ROWS>
+__device__ inline void tile_store(uint16_t* lds, const Pix8 (&v)[Tile<WIDE>::V], int tid) {
+  using C = Tile<WIDE>;
+#pragma unroll
+  for (int j = 0; j < C::V; ++j) {
+    const int i = tid + j * C::NT;
+    int at;
+    if constexpr (!ROWS) at = i / (C::KT / 8) * C::PITCH + i % (C::KT / 8) * 8;
+    else at = piece_at<WIDE>(i / (C::T / 8), i % (C::T / 8)) * 8;
+    *reinterpret_cast<uint4*>(lds + at) = make_uint4(v[j].v[0], v[j].v[1], v[j].v[2], v[j].v[3]);
+  }
+}
+
+// MFMA fragment: rows rb + lane % 32, k = 16 ks + 8 (lane / 32) .. +7
+template <bool WIDE, bool ROWS>
+__device__ inline bf16x8_t tile_frag(const uint16_t* lds, int rb, int ks, int lane) {
+  if constexpr (!ROWS) {
+    return as_bf16x8(*reinterpret_cast<const uint4*>(lds + (rb + (lane & 31)) * Tile<WIDE>::PITCH + ks * 16 + (lane >> 5) * 8));
+  } else {
+    const int g = lane >> 4, j = lane & 15;
+    const int kr = 16 * ks + 8 * (g >> 1) + (j >> 2), r = rb + 16 * (g & 1) + 4 * (j & 3);
+    const uint16_t* lo = lds + piece_at<WIDE>(kr, r >> 3) * 8 + (r & 7);
+    const uint16_t* hi = lds + piece_at<WIDE>(kr + 4, r >> 3) * 8 + (r & 7);
+    const u32x2_t a = __builtin_bit_cast(
+        u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(lo)));
+    const u32x2_t b = __builtin_bit_cast(
+        u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(hi)));
+    return as_bf16x8(u32x4_t{a[0], a[1], b[0], b[1]});
+  }
+}
+
+__device__ inline uint32_t pack2(float a, float b) {  // (NaN stays NaN: no canonical form is asked for here)
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
+// n (up to 4) consecutive bf16 at p, as one 8-byte access where `vec`
+__device__ inline void put4(uint16_t* p, const float (&v)[4], int n, int vec) {
+  if (vec && n >= 4) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) p[e] = f32_to_bf16(v[e]);
+}
+
+__device__ inline void get4(float (&v)[4], const uint16_t* p, int n, int vec) {
+  if (vec && n >= 4) {
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(q.x << 16), v[1] = __uint_as_float(q.x & 0xFFFF0000u);
+    v[2] = __uint_as_float(q.y << 16), v[3] = __uint_as_float(q.y & 0xFFFF0000u);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = e < n ? bf16_to_f32(p[e]) : 0.0f;
+}
+
+// 4 consecutive outputs: d0 (and for the gated forward the up projection d1) of row q, from
+// column `at` on
+template <int EPI, int ACT>
+__device__ inline void put_quad(const TileArgs& a, int q, int at, const float (&d0)[4], const float (&d1)[4]) {
+  if constexpr (EPI == kPlain) {
+    put4(a.out + int64_t(q) * a.ldc + at, d0, a.p.rows - at, a.vec);
+  } else if constexpr (EPI == kGatedGrad) {
+    const int n = a.F - at;
+    if (n <= 0) return;
+    const int64_t row = int64_t(q) * 2 * a.F + at;
+    float g[4], u[4], og[4], ou[4];
+    get4(g, a.gu + row, n, a.vec);
+    get4(u, a.gu + row + a.F, n, a.vec);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 t = act_pair<ACT>(g[e]);
+      og[e] = d0[e] * u[e] * t.y;
+      ou[e] = d0[e] * t.x;
+    }
+    put4(a.out + row, og, n, a.vec);
+    put4(a.out + row + a.F, ou, n, a.vec);
+  } else {
+    const int n = a.F - at;
+    float h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = act_of<ACT>(d0[e]) * d1[e];
+    put4(a.out + int64_t(q) * a.F + at, h, n, a.vec);
+    if constexpr (EPI == kGatedKeep) {
+      put4(a.gu + int64_t(q) * 2 * a.F + at, d0, n, a.vec);
+      put4(a.gu + int64_t(q) * 2 * a.F + a.F + at, d1, n, a.vec);
+    }
+  }
+}
+
+template <bool WIDE, bool PROWS, bool QROWS, int EPI, int ACT>
+__global__ __launch_bounds__(Tile<WIDE>::NT) void tile_kernel(TileArgs a) {
+  using C = Tile<WIDE>;
+  constexpr bool GATED = EPI == kGated || EPI == kGatedKeep;
+  extern __shared__ __attribute__((aligned(16))) uint16_t smem[];  // [2 buffers][P, Q]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wm = wave & 1, wn = wave >> 1;
-  const int m0 = blockIdx.y * kT, f0 = blockIdx.x * kT;
-  const int lr = lane & 31, lk = (lane >> 5) * 8;
-  f32x16_t g = zero_acc(), u = zero_acc();
-  Pix8 rx[2], rw[4];
-  const auto load = [&](int k0) {
-    const int kv = k0 + (tid & 7) * 8;
+  const int wp = WIDE ? wave & 1 : 0, wq = WIDE ? wave >> 1 : 0;
+  const int p0 = blockIdx.x * C::T, q0 = blockIdx.y * C::T;
+  f32x16_t acc[2][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int m = m0 + (tid >> 3) + j * 32;
-      rx[j] = row_vec(a.x + int64_t(min(m, a.M - 1)) * a.ldx + min(kv, a.K), m < a.M ? a.K - kv : 0);
-    }
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int f = f0 + (tid >> 3) + (j & 1) * 32;
-      rw[j] = row_vec(a.w + (int64_t(min(f, a.F - 1)) + (j >> 1) * int64_t(a.F)) * a.ldw + min(kv, a.K), f < a.F ? a.K - kv : 0);
-    }
-  };
-  const auto store = [&](int b) {
-    const int at = (tid >> 3) * kP + (tid & 7) * 8;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      *reinterpret_cast<uint4*>(xs[b] + at + j * 32 * kP) = make_uint4(rx[j].v[0], rx[j].v[1], rx[j].v[2], rx[j].v[3]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<uint4*>(ws[b] + at + j * 32 * kP) = make_uint4(rw[j].v[0], rw[j].v[1], rw[j].v[2], rw[j].v[3]);
-  };
-  load(0);
-  store(0);
+    for (int j = 0; j < 2; ++j) acc[i][j] = zero_acc();
+  Pix8 rp[C::V], rq[C::V];
+  tile_load<WIDE, PROWS, GATED>(rp, a, a.p, p0, 0, tid);
+  tile_load<WIDE, QROWS, false>(rq, a, a.q, q0, 0, tid);
+  tile_store<WIDE, PROWS>(smem, rp, tid);
+  tile_store<WIDE, QROWS>(smem + C::ELEMS, rq, tid);
   __syncthreads();
   int b = 0;
-  for (int k0 = 0; k0 < a.K; k0 += kKT) {
-    const bool more = k0 + kKT < a.K;
-    if (more) load(k0 + kKT);
-#pragma unroll
-    for (int ks = 0; ks < kKT / 16; ++ks) {
-      const bf16x8_t fx = as_bf16x8(*reinterpret_cast<const uint4*>(xs[b] + (wm * 32 + lr) * kP + ks * 16 + lk));
-      const bf16x8_t fg = as_bf16x8(*reinterpret_cast<const uint4*>(ws[b] + (wn * 32 + lr) * kP + ks * 16 + lk));
-      const bf16x8_t fu = as_bf16x8(*reinterpret_cast<const uint4*>(ws[b] + (kT + wn * 32 + lr) * kP + ks * 16 + lk));
-      g = mfma_32x32x16(fx, fg, g);
-      u = mfma_32x32x16(fx, fu, u);
+  for (int k0 = 0; k0 < a.K; k0 += C::KT) {
+    const bool more = k0 + C::KT < a.K;
+    if (more) {
+      tile_load<WIDE, PROWS, GATED>(rp, a, a.p, p0, k0 + C::KT, tid);
+      tile_load<WIDE, QROWS, false>(rq, a, a.q, q0, k0 + C::KT, tid);
     }
-    if (more) store(b ^ 1);  // its last reads ended before the previous barrier
+    const uint16_t* ps = smem + b * 2 * C::ELEMS;
+    const uint16_t* qs = ps + C::ELEMS;
+#pragma unroll
+    for (int s = 0; s < (WIDE ? 4 : 1); ++s) {
+      const int ks = WIDE ? s : wave;
+      bf16x8_t fp[2], fq[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fp[i] = tile_frag<WIDE, PROWS>(ps, wp * 64 + i * 32, ks, lane);
+        fq[i] = tile_frag<WIDE, QROWS>(qs, wq * 64 + i * 32, ks, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma_32x32x16(fp[i], fq[j], acc[i][j]);
+    }
+    if (more) {  // the other buffer's last reads ended before the previous barrier
+      uint16_t* to = smem + (b ^ 1) * 2 * C::ELEMS;
+      tile_store<WIDE, PROWS>(to, rp, tid);
+      tile_store<WIDE, QROWS>(to + C::ELEMS, rq, tid);
+    }
     __syncthreads();
     b ^= 1;
   }
-  const int f = f0 + wn * 32 + lr;
-  if (f >= a.F) return;
+  // accumulator quads: (i, j) block, rows 8 g + 4 (lane / 32) .. +3 of it, column lane % 32
+  const auto column = [&](int i, int g, int l) {  // of the output's contiguous index
+    return GATED ? p0 / 2 + wp * 32 + 8 * g + 4 * (l >> 5) : p0 + wp * 64 + i * 32 + 8 * g + 4 * (l >> 5);
+  };
+  if constexpr (WIDE) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int m = m0 + wm * 32 + mfma_row(r, lane);
-    if (m >= a.M) continue;
-    a.h[int64_t(m) * a.F + f] = f32_to_bf16(act_of<ACT>(g[r]) * u[r]);
-    if constexpr (KEEP) {
-      a.gu[int64_t(m) * 2 * a.F + f] = f32_to_bf16(g[r]);
-      a.gu[int64_t(m) * 2 * a.F + a.F + f] = f32_to_bf16(u[r]);
+    for (int j = 0; j < 2; ++j) {
+      const int q = q0 + wq * 64 + j * 32 + (lane & 31);
+      if (q >= a.q.rows) continue;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+#pragma unroll
+        for (int i = 0; i < (GATED ? 1 : 2); ++i) {
+          float d0[4], d1[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d0[e] = acc[i][j][4 * g + e], d1[e] = GATED ? acc[1][j][4 * g + e] : 0.0f;
+          if (column(i, g, lane) < (GATED ? a.F : a.p.rows)) put_quad<EPI, ACT>(a, q, column(i, g, lane), d0, d1);
+        }
+      }
+    }
+  } else {
+    // two rounds (j): the eight waves' quads [wave][i][g][lane] in 64 KB, a thread per (g, lane)
+    // pair and, of plain results, per i
+    float4* red = reinterpret_cast<float4*>(smem);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          red[((wave * 2 + i) * 4 + g) * 64 + lane] =
+              make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+      __syncthreads();
+      const int g = (tid >> 6) & 3, half = tid >> 8;
+      const auto sum = [&](int i, float (&d)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          const float4 v = red[((w * 2 + i) * 4 + g) * 64 + lane];
+          d[0] += v.x, d[1] += v.y, d[2] += v.z, d[3] += v.w;
+        }
+      };
+      const int q = q0 + j * 32 + (lane & 31);
+      if (q < a.q.rows && (!GATED || half == 0)) {
+        const int at = column(half, g, lane);
+        if (at < (GATED ? a.F : a.p.rows)) {
+          float d0[4], d1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          sum(GATED ? 0 : half, d0);
+          if (GATED) sum(1, d1);
+          put_quad<EPI, ACT>(a, q, at, d0, d1);
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ---- large tiles --------------------------------------------------------------------------------
+// The 256 x 256 tile of the library's large products (gemm_dma.h): operands that can be loaded as
+// whole 16-byte vectors by the LDS DMA.  Rows of P (the hidden units) run along the MFMA's rows:
+// a lane's accumulator quad is 4 consecutive units of one row of x.  For the projections P's tile
+// rows hold 16 gate rows and the same 16 units' up rows in turn, so that one tile has both
+// projections of 128 units.
+template <bool ROWS>
+constexpr int kDmaMode = ROWS ? kAlongRow : kAlongK;
+
+// DMA plan of P = w for the projections: tile row r is unit f0 + 16 (r / 32) + r % 16, its gate
+// row for even r / 16 and its up row for odd.
+__device__ inline G5Operand gated_operand(const TileArgs& a, int f0, int tid) {
+  G5Operand o = g5_operand<kAlongK, true>(a.p.src, a.p.ld, 1, 0, 2 * a.F, a.K, tid);
+  const int lane = tid & 63, w = tid >> 6;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = 4 * w + i;  // tile rows 16 j .. 16 j + 15, lane L at row 16 j + L / 4
+    const int f = f0 + 16 * (j >> 1) + (lane >> 2);
+    o.roff[i] = f < a.F ? int((f + int64_t(j & 1) * a.F) * a.p.ld) : -1;
+  }
+  return o;
+}
+
+__device__ inline uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+}
+
+__device__ inline void unpack8(float (&v)[8], const uint4& q) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[2 * e] = __uint_as_float(w[e] << 16);
+    v[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+  }
+}
+
+// The epilogue passes the accumulators through LDS, 128 rows of x at a time ([row][256 tile rows of
+// P] in fp32, pitch 260: quads of 16 rows on distinct banks), so that every global access is 16
+// bytes of a 256- or 512-byte run and the code is a short loop: stored straight from the
+// accumulators (8-byte quads, straight-line code) the forward's epilogue took as long as the k-loop
+// at K = 1024.
+constexpr int kEpiRows = 128, kEpiPitch = kT4 + 4;
+constexpr size_t kLargeLds = std::max(kGemm5Lds, size_t(kEpiRows) * kEpiPitch * 4);
+
+template <bool PROWS, int EPI, int ACT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void gated_large_kernel(TileArgs a, int xcd_group) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
+  constexpr bool GATED = EPI != kGatedGrad;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = wave & 1, wn = wave >> 1;
+  int tp, tq;
+  xcd_tile_xy(xcd_group, tp, tq);
+  const int f0 = tp * (GATED ? kT4 / 2 : kT4), q0 = tq * kT4;
+  f32x4_t acc[8][8];
+  {
+    G5Operand op;
+    if constexpr (GATED) op = gated_operand(a, f0, tid);
+    else op = g5_operand<kAlongRow, true>(a.p.src, 1, a.p.ld, f0, a.F, a.K, tid);
+    const G5Operand oq = g5_operand<kAlongK, true>(a.q.src, a.q.ld, 1, q0, a.q.rows, a.K, tid);
+    gemm6_loop<kDmaMode<PROWS>, kAlongK>(acc, op, oq, smem, 0, a.K, tid);
+  }
+  mfma16_fence(acc);
+  float* epi = reinterpret_cast<float*>(smem);
+  // threads of a row, 8 units each; rows per round
+  constexpr int kAcross = (GATED ? kT4 / 2 : kT4) / 8, kRound = 256 / kAcross;
+  const int o = tid % kAcross, rr = tid / kAcross;
+  const int f = f0 + 8 * o;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    __syncthreads();  // the k-loop's (or the last half's) LDS reads are done
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<f32x4_t*>(epi + (wn * 64 + j * 16 + (lane & 15)) * kEpiPitch + wm * 128 + i * 16 + 4 * (lane >> 4)) =
+            acc[i][half * 4 + j];
+    __syncthreads();
+    // LDS row r is row 128 (r / 64) + 64 half + r % 64 of the tile
+    const auto row = [&](int r) { return q0 + 128 * (r >> 6) + 64 * half + (r & 63); };
+    if constexpr (GATED) {
+      const float* at = epi + (o >> 1) * 32 + (o & 1) * 8;
+#pragma unroll 2
+      for (int r = rr; r < kEpiRows; r += kRound) {
+        const int q = row(r);
+        float g[8], u[8], h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = at[r * kEpiPitch + e], u[e] = at[r * kEpiPitch + 16 + e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = act_of<ACT>(g[e]) * u[e];
+        if (q < a.q.rows && f < a.F) {
+          *reinterpret_cast<uint4*>(a.out + int64_t(q) * a.F + f) = pack8(h);
+          if constexpr (EPI == kGatedKeep) {
+            uint16_t* gu = a.gu + int64_t(q) * 2 * a.F + f;
+            *reinterpret_cast<uint4*>(gu) = pack8(g);
+            *reinterpret_cast<uint4*>(gu + a.F) = pack8(u);
+          }
+        }
+      }
+    } else {
+      // four rows' [g u] in flight: clamped addresses, no branch around the loads
+#pragma unroll 1
+      for (int r = rr; r < kEpiRows; r += 4 * kRound) {
+        uint4 kg[4], ku[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint16_t* p = a.gu + int64_t(min(row(r + n * kRound), a.q.rows - 1)) * 2 * a.F + min(f, a.F - 8);
+          kg[n] = *reinterpret_cast<const uint4*>(p);
+          ku[n] = *reinterpret_cast<const uint4*>(p + a.F);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int q = row(r + n * kRound);
+          float g[8], u[8], og[8], ou[8];
+          unpack8(g, kg[n]);
+          unpack8(u, ku[n]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float d = epi[(r + n * kRound) * kEpiPitch + 8 * o + e];
+            const float2 t = act_pair<ACT>(g[e]);
+            og[e] = d * u[e] * t.y;
+            ou[e] = d * t.x;
+          }
+          if (q < a.q.rows && f < a.F) {
+            uint16_t* to = a.out + int64_t(q) * 2 * a.F + f;
+            *reinterpret_cast<uint4*>(to) = pack8(og);
+            *reinterpret_cast<uint4*>(to + a.F) = pack8(ou);
+          }
+        }
+      }
     }
   }
 }
@@ -190,11 +529,66 @@ const char* gated_fault(int64_t M, int64_t K, int64_t F, int act) {
 
 bool odd(const void* p) { return reinterpret_cast<uintptr_t>(p) & 1; }
 
-template <int ACT>
-void launch_tile(const GatedArgs& a, hipStream_t st) {
-  const dim3 grid(unsigned(ceil_div(a.F, kT)), unsigned(ceil_div(a.M, kT)));
-  if (a.gu) gated_tile_kernel<ACT, true><<<grid, 256, 0, st>>>(a);
-  else gated_tile_kernel<ACT, false><<<grid, 256, 0, st>>>(a);
+template <bool WIDE, bool PROWS, bool QROWS, int EPI, int ACT>
+bool launch_tile(const TileArgs& a, dim3 grid, hipStream_t st) {
+  using C = Tile<WIDE>;
+  void (*f)(TileArgs) = tile_kernel<WIDE, PROWS, QROWS, EPI, ACT>;
+  static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             int(C::LDS)) == hipSuccess;
+  if (!ok) return false;
+  f<<<grid, C::NT, C::LDS, st>>>(a);
+  return true;
+}
+
+// Wide tiles where they give every CU one: below that the narrow ones share a block's k.
+template <bool PROWS, bool QROWS, int EPI, int ACT>
+bool launch_tiles(const TileArgs& a, hipStream_t st) {
+  constexpr int side = EPI == kGated || EPI == kGatedKeep ? 2 : 1;  // tile rows per unit of p
+  const auto tiles = [&](int t) { return dim3(unsigned(ceil_div(int64_t(a.p.rows) * side, t)), unsigned(ceil_div(a.q.rows, t))); };
+  const dim3 wide = tiles(128), narrow = tiles(64);
+  if (int64_t(wide.x) * wide.y >= 256 || narrow.y > 65535) return launch_tile<true, PROWS, QROWS, EPI, ACT>(a, wide, st);
+  return launch_tile<false, PROWS, QROWS, EPI, ACT>(a, narrow, st);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
+
+// Operands the LDS DMA can load: 16-byte aligned rows, whole vectors of k (and of units where
+// they are contiguous), 32-bit byte offsets.
+bool dma_ok(const TileOperand& o, int64_t rows, int64_t K, bool along_rows) {
+  const int64_t extent = along_rows ? (K - 1) * o.ld + rows : (rows - 1) * o.ld + K;
+  return aligned16(o.src) && o.ld % 8 == 0 && extent * 2 < (int64_t(1) << 31);
+}
+
+template <bool PROWS, int EPI, int ACT>
+bool launch_large(const TileArgs& a, dim3 grid, hipStream_t st) {
+  void (*f)(TileArgs, int) = gated_large_kernel<PROWS, EPI, ACT>;
+  static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             int(kLargeLds)) == hipSuccess;
+  if (!ok) return false;
+  const int group = int64_t(grid.x) * grid.y % kGemmXcds == 0 ? int(std::min(grid.y, 8u)) : 0;
+  f<<<grid, 256, kLargeLds, st>>>(a, group);
+  return true;
+}
+
+template <int EPI, bool PROWS, int ACT>
+bool launch_sized(const TileArgs& a, hipStream_t st) {
+  constexpr bool GATED = EPI != kGatedGrad;
+  const dim3 grid(unsigned(ceil_div(a.F, GATED ? kT4 / 2 : kT4)), unsigned(ceil_div(a.q.rows, kT4)));
+  const bool large = int64_t(grid.x) * grid.y >= 128 && a.K % 8 == 0 && a.F % 8 == 0 && aligned16(a.out) && aligned16(a.gu) &&
+                     dma_ok(a.p, GATED ? 2 * int64_t(a.F) : a.F, a.K, PROWS) && dma_ok(a.q, a.q.rows, a.K, false);
+  return large ? launch_large<PROWS, EPI, ACT>(a, grid, st) : launch_tiles<PROWS, false, EPI, ACT>(a, st);
+}
+
+template <int EPI, bool PROWS>
+bool launch_gated(int act, const TileArgs& a, hipStream_t st) {
+  if (act == kSilu) return launch_sized<EPI, PROWS, kSilu>(a, st);
+  if (act == kGelu) return launch_sized<EPI, PROWS, kGelu>(a, st);
+  return launch_sized<EPI, PROWS, kRelu>(a, st);
+}
+
+int launched(const char* what, bool ok) {
+  return ok ? check_launch(what) : refuse(what, "cannot enable a tile kernel's LDS size");
 }
 
 }  // namespace
@@ -209,17 +603,66 @@ int xdna_gated_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t l
   const char* what = "xdna_gated_bf16";
   if (const char* why = gated_fault(M, K, F, act)) return refuse(what, why);
   if ((ldx < K && M > 1) || ldw < K) return refuse(what, "rows overlap");
-  if (ceil_div(M, int64_t(kT)) > 65535) return refuse(what, "too many rows");
+  if (ceil_div(M, int64_t(64)) > 65535) return refuse(what, "too many rows");
   if (M == 0) return 0;
   if (!x || !w || !h) return refuse(what, "null operand");
   if (odd(x) || odd(w) || odd(h) || odd(gu)) return refuse(what, "misaligned operand");
   if (!admit_launch(what)) return -1;
-  const GatedArgs a = {x, w, h, gu, int(M), int(K), int(F), ldx, ldw};
+  TileArgs a = {};
+  a.p = {w, ldw, int(F)};
+  a.q = {x, M > 1 ? ldx : K, int(M)};
+  a.K = int(K);
+  a.out = h;
+  a.gu = gu;
+  a.F = int(F);
+  a.vec = F % 4 == 0 && aligned8(h) && aligned8(gu) ? 1 : 0;
   hipStream_t st = as_stream(stream);
-  if (act == kSilu) launch_tile<kSilu>(a, st);
-  else if (act == kGelu) launch_tile<kGelu>(a, st);
-  else launch_tile<kRelu>(a, st);
-  return check_launch(what);
+  return launched(what, gu ? launch_gated<kGatedKeep, false>(act, a, st) : launch_gated<kGated, false>(act, a, st));
+}
+
+int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_out, int64_t ldw, const uint16_t* gu,
+                            int64_t M, int64_t N, int64_t F, int act, uint16_t* dgu, void* stream) {
+  const char* what = "xdna_gated_mlp_bwd_bf16";
+  if (const char* why = gated_fault(M, N, F, act)) return refuse(what, why);
+  if ((lddy < N && M > 1) || (ldw < F && N > 1)) return refuse(what, "rows overlap");
+  if (ceil_div(M, int64_t(64)) > 65535) return refuse(what, "too many rows");
+  if (M == 0) return 0;
+  if (!dy || !w_out || !gu || !dgu) return refuse(what, "null operand");
+  if (odd(dy) || odd(w_out) || odd(gu) || odd(dgu)) return refuse(what, "misaligned operand");
+  if (!admit_launch(what)) return -1;
+  TileArgs a = {};
+  a.p = {w_out, ldw, int(F)};
+  a.q = {dy, M > 1 ? lddy : N, int(M)};
+  a.K = int(N);
+  a.out = dgu;
+  a.gu = const_cast<uint16_t*>(gu);
+  a.F = int(F);
+  a.vec = F % 4 == 0 && aligned8(dgu) && aligned8(gu) ? 1 : 0;
+  return launched(what, launch_gated<kGatedGrad, true>(act, a, as_stream(stream)));
+}
+
+int xdna_tile_mm_bf16(const uint16_t* p, int64_t ldp, int p_rows, const uint16_t* q, int64_t ldq, int q_rows, int64_t P,
+                      int64_t Q, int64_t K, uint16_t* out, int64_t ldc, void* stream) {
+  const char* what = "xdna_tile_mm_bf16";
+  if (P < 0 || P > kMaxSide || Q < 0 || Q > int64_t(65535) * 64 || K < 1 || K > kMaxSide) return refuse(what, "sizes out of range");
+  if ((p_rows != 0 && p_rows != 1) || (q_rows != 0 && q_rows != 1) || (q_rows && !p_rows))
+    return refuse(what, "operands are k-contiguous (0) or row-contiguous (1), q only beside such a p");
+  if (ldp < (p_rows ? P : K) || ldq < (q_rows ? Q : K) || ldc < P) return refuse(what, "rows overlap");
+  if (P == 0 || Q == 0) return 0;
+  if (!p || !q || !out) return refuse(what, "null operand");
+  if (odd(p) || odd(q) || odd(out)) return refuse(what, "misaligned operand");
+  if (!admit_launch(what)) return -1;
+  TileArgs a = {};
+  a.p = {p, ldp, int(P)};
+  a.q = {q, ldq, int(Q)};
+  a.K = int(K);
+  a.out = out;
+  a.ldc = ldc;
+  a.vec = ldc % 4 == 0 && aligned8(out) ? 1 : 0;
+  hipStream_t st = as_stream(stream);
+  return launched(what, q_rows   ? launch_tiles<true, true, kPlain, kSilu>(a, st)
+                        : p_rows ? launch_tiles<true, false, kPlain, kSilu>(a, st)
+                                 : launch_tiles<false, false, kPlain, kSilu>(a, st));
 }
 
 int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const uint16_t* gu, int64_t M, int64_t F, int act, uint16_t* dgu,

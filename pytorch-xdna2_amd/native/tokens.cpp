@@ -63,10 +63,26 @@ void once_only(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the gradient itself cannot be differentiated");
 }
 
-// a product of two bf16 matrices of any strides
+// whether the library's products load a matrix as whole vectors
+bool vector_rows(const at::Tensor& t) {
+  const int64_t ld = t.stride(1) == 1 ? t.stride(0) : t.stride(0) == 1 ? t.stride(1) : 1;
+  return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 && ld % 8 == 0;
+}
+
+// a b of two bf16 matrices, each contiguous along one dimension.  Operands that xdna_gemm_bf16
+// would load element by element take the tiles that load at any alignment.
 at::Tensor product(const at::Tensor& a, const at::Tensor& b) {
   const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
   at::Tensor c = empty_xdna({M, N}, at::kBFloat16);
+  const bool b_rows = b.stride(1) == 1 && K > 1, a_rows = a.stride(0) == 1 && M > 1 && a.stride(1) != 1;
+  const bool a_ok = a_rows ? b_rows : a.stride(1) == 1 || K == 1, b_ok = b_rows || b.stride(0) == 1 || K == 1;
+  if (K > 0 && !(vector_rows(a) && vector_rows(b)) && a_ok && b_ok) {
+    const int64_t lda = a_rows ? a.stride(1) : M > 1 ? a.stride(0) : K, ldb = b_rows ? b.stride(0) : N > 1 ? b.stride(1) : K;
+    check_abi(xdna_tile_mm_bf16(p16(b), ldb, b_rows ? 1 : 0, p16(a), lda, a_rows ? 1 : 0, N, M, K, m16(c), N,
+                                current_stream()),
+              "tile product");
+    return c;
+  }
   check_abi(xdna_gemm_bf16(p16(a), p16(b), m16(c), nullptr, 1, int(M), int(N), int(K), a.stride(0), a.stride(1), 0,
                            b.stride(0), b.stride(1), 0, N, 1, 0, 0, 0, 0, 1.0f, 0.0f, current_stream()),
             "gemm");
@@ -167,7 +183,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor dgu = gated_dgu(grads[0], saved[2], ctx->saved_data["act"].toInt());
     at::Tensor dx, dw;
-    if (ctx->needs_input_grad(0)) dx = product(dgu, saved[1]).view(saved[0].sizes());
+    if (ctx->needs_input_grad(0)) dx = product(dgu, as_rows(saved[1])).view(saved[0].sizes());
     if (ctx->needs_input_grad(1)) dw = product(dgu.t(), as_rows(saved[0]));
     return {dx, dw, at::Tensor()};
   }
@@ -180,7 +196,7 @@ struct GatedMlpFn : public torch::autograd::Function<GatedMlpFn> {
     const GatedForward f = gated_forward(x, w_in, act, true);
     ctx->save_for_backward({x, w_in, w_out, f.gu, f.h});
     ctx->saved_data["act"] = act;
-    return product(f.h, w_out.t()).view(with_last(x, w_out.size(0)));
+    return product(f.h, as_rows(w_out).t()).view(with_last(x, w_out.size(0)));
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -192,8 +208,12 @@ struct GatedMlpFn : public torch::autograd::Function<GatedMlpFn> {
     const at::Tensor dy = as_rows(grads[0]);
     at::Tensor dx, dw_in, dw_out;
     if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) {
-      const at::Tensor dgu = gated_dgu(product(dy, w_out), gu, ctx->saved_data["act"].toInt());
-      if (ctx->needs_input_grad(0)) dx = product(dgu, w_in).view(x.sizes());
+      const at::Tensor wo = as_rows(w_out);
+      at::Tensor dgu = empty_xdna(gu.sizes(), at::kBFloat16);
+      check_abi(xdna_gated_mlp_bwd_bf16(p16(dy), row_stride(dy), p16(wo), row_stride(wo), p16(gu), dy.size(0), dy.size(1),
+                                        h.size(1), int(ctx->saved_data["act"].toInt()), m16(dgu), current_stream()),
+                "gated_mlp backward");
+      if (ctx->needs_input_grad(0)) dx = product(dgu, as_rows(w_in)).view(x.sizes());
       if (ctx->needs_input_grad(1)) dw_in = product(dgu.t(), as_rows(x));
     }
     if (ctx->needs_input_grad(2)) dw_out = product(dy.t(), h);
@@ -387,7 +407,7 @@ at::Tensor token_gated_mlp(const at::Tensor& x, const at::Tensor& w_in, const at
   if (tracked({&x, &w_in, &w_out})) return GatedMlpFn::apply(x, w_in, w_out, act);
   ScopedCount sc("hip_tokens.gated.fwd.run");
   const GatedForward f = gated_forward(x, w_in, act, false);
-  return product(f.h, w_out.t()).view(with_last(x, w_out.size(0)));
+  return product(f.h, as_rows(w_out).t()).view(with_last(x, w_out.size(0)));
 }
 
 at::Tensor token_distill(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher, double tau,

@@ -595,3 +595,35 @@ def test_refusals_on_the_device(T):
     (dz,) = torch.autograd.grad(T.token_log_probs(zx, y).entropy.sum(), [zx], retain_graph=True)
     with pytest.raises(RuntimeError, match="cannot be differentiated"):
         torch.autograd.grad(T.token_log_probs(zx, y).entropy.sum(), [zx], create_graph=True)
+
+
+LARGE = [  # rows, K, F, N: at least 128 tiles of 256 x 256, ragged at the edges
+    (4000, 264, 1000, 264), (2049, 72, 4104, 40), (300, 1024, 16384, 64), (8200, 512, 512, 1024),
+]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("M,K,F,N", LARGE)
+def test_gated_mlp_large(T, M, K, F, N, act):
+    """The large tiles: sampled rows and units against the 64-bit block (each row of y, h and dx
+    depends on its own row of x and dy only), the weight gradients against the products of the
+    kernels' own bf16 operands."""
+    print("gated large", M, K, F, N, act, flush=True)
+    g = gen(M + K + F)
+    x, dy = torch.randn(M, K, generator=g).bfloat16(), torch.randn(M, N, generator=g).bfloat16()
+    w = (torch.randn(2 * F, K, generator=g) / math.sqrt(K)).bfloat16()
+    wo = (torch.randn(N, F, generator=g) / math.sqrt(F)).bfloat16()
+    rows = torch.unique(torch.cat([torch.arange(0, M, 97), torch.arange(max(0, M - 20), M)]))
+    ref = gated_reference(x[rows], w, wo, dy[rows], act, True)
+    leaves = [t.to("xdna").requires_grad_() for t in (x, w, wo)]
+    y = T.gated_mlp(*leaves, activation=act)
+    dx, dw, dwo = torch.autograd.grad(y, leaves, dy.to("xdna"))
+    close(y.detach().cpu()[rows], *ref["y"], "y")
+    close(dx.cpu()[rows], *ref["dx"], "dx")
+    with torch.no_grad():
+        h = T.gated_linear(leaves[0], leaves[1], activation=act)
+    close(h.cpu()[rows], *ref["h"], "h")
+    units = torch.unique(torch.cat([torch.arange(0, F, 131), torch.arange(F - 9, F)]))
+    some = gated_reference(x, torch.cat([w[units], w[F + units]]), wo[:, units], dy, act, True)
+    close(dw.cpu()[torch.cat([units, F + units])], *some["dw_in"], "dw_in")
+    close(dwo.cpu()[:, units], *some["dw_out"], "dw_out")
