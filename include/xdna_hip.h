@@ -827,18 +827,20 @@ int xdna_embed_bwd(const void* ids, int index_bytes, int64_t tokens, const void*
 
 /* h = act(x Wg^T) * (x Wu^T), M x F, with w = [Wg; Wu] (2F rows of K): both projections (fp32
  * sums), the activation (0 silu, 1 gelu with erf, 2 relu) and the product in one launch, h
- * rounded once.  gu (M x 2F, or NULL) keeps [g u] as bf16 for the backward. */
+ * rounded once.  gu (xdna_gated_kept_bytes, or NULL) keeps g and u for the backward: [g u] (M x 2F)
+ * as bf16, then M x F bytes with 4 more mantissa bits of both. */
+size_t xdna_gated_kept_bytes(int64_t M, int64_t F);
 int xdna_gated_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t M, int64_t K, int64_t F,
-                    int act, uint16_t* h, uint16_t* gu, void* stream);
+                    int act, uint16_t* h, void* gu, void* stream);
 
 /* dgu = [dh * u * act'(g), dh * act(g)] (M x 2F) from dh (M x F, row stride ld) and the kept
  * gu: the gradients of x and w are the products dgu * w and dgu^T * x. */
-int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const uint16_t* gu, int64_t M, int64_t F, int act,
+int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const void* gu, int64_t M, int64_t F, int act,
                         uint16_t* dgu, void* stream);
 
 /* The same from the block's output: dh = dy w_out (w_out: N rows of F) stays in fp32 between the
  * product and the activation's gradient, in one launch. */
-int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_out, int64_t ldw, const uint16_t* gu,
+int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_out, int64_t ldw, const void* gu,
                             int64_t M, int64_t N, int64_t F, int act, uint16_t* dgu, void* stream);
 
 /* out[q * ldc + p] = sum over k of P[p][k] Q[q][k], for operands of any alignment and row stride:

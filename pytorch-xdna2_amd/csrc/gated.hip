@@ -3,9 +3,12 @@
 // these as separate mm / activation / mul ops (torch_xdna_device.cpp:4360-4417, 5124-5260).
 //
 // w holds [Wg; Wu], 2F rows of K.  The projections are summed in fp32 and stay there through
-// the activation and the product; h is rounded once.  For training g and u are kept as bf16
-// (the form the framework keeps every activation in): the backward reads them instead of
-// multiplying again.
+// the activation and the product; h is rounded once.  For training g and u are kept, in 20 bits
+// each: a bf16 and 4 more bits of the mantissa, the two units' in one byte (M x 2F bf16, then
+// M x F bytes).  The backward's products take [dg du] as bf16; with g and u in bf16 as well their
+// rounding is the third of equal size in dx and dw (error of dx against 64 bits 1.75 times that of
+// its own rounding, 1.4 times with the 4 bits), and the 4 bits cost a quarter of their traffic,
+// where multiplying again would cost two more products.
 //   dg = dh u act'(g), du = dh act(g), as [dg du] (M x 2F), so that dx = [dg du] w and
 //   dw = [dg du]^T x are one product each.
 #include "common.h"
@@ -66,7 +69,8 @@ struct TileArgs {
   int K;
   uint16_t* out;   // kPlain: D; kGated*: h; kGatedGrad: [dg du]
   int64_t ldc;
-  uint16_t* gu;    // kGatedKeep: written; kGatedGrad: read
+  uint16_t* gu;    // kGatedKeep: written; kGatedGrad: read.  The high parts, [q][2F] ...
+  uint8_t* low;    // ... and the low ones, [q][F]: g's in bits 0-3, u's in bits 4-7
   int F;           // kGated*: p.src holds F gate rows, then F up rows (p.rows = F)
   int vec;         // 8-byte accesses of out and gu: their addresses and strides are multiples of 4
 };
@@ -169,6 +173,25 @@ __device__ inline uint32_t pack2(float a, float b) {  // (NaN stays NaN: no cano
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
+// An fp32 value rounded to 20 bits (to nearest, ties away), in the high bits.  The sum cannot
+// leave a NaN's or an infinity's class: a product of bf16 operands makes NaN with nothing in the
+// low half.
+__device__ inline uint32_t round20(float v) { return __float_as_uint(v) + 0x800u; }
+
+// g's and u's low 4 bits of 4 units as 4 bytes
+__device__ inline uint32_t low_bits(const uint32_t (&g)[4], const uint32_t (&u)[4]) {
+  uint32_t b[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b[e] = ((g[e] >> 12) & 15u) | ((u[e] >> 8) & 0xF0u);
+  return (b[0] | b[1] << 8) | (b[2] | b[3] << 8) << 16;
+}
+
+// value e of 4 from its bf16 part (of a pair) and the units' low bytes; shift 0 for g, 4 for u
+__device__ inline float kept(uint32_t pair, uint32_t low, int e, int shift) {
+  const uint32_t hi = e & 1 ? pair & 0xFFFF0000u : pair << 16;
+  return __uint_as_float(hi | (((low >> (8 * e + shift)) & 15u) << 12));
+}
+
 // n (up to 4) consecutive bf16 at p, as one 8-byte access where `vec`
 __device__ inline void put4(uint16_t* p, const float (&v)[4], int n, int vec) {
   if (vec && n >= 4) {
@@ -180,15 +203,49 @@ __device__ inline void put4(uint16_t* p, const float (&v)[4], int n, int vec) {
     if (e < n) p[e] = f32_to_bf16(v[e]);
 }
 
-__device__ inline void get4(float (&v)[4], const uint16_t* p, int n, int vec) {
-  if (vec && n >= 4) {
-    const uint2 q = *reinterpret_cast<const uint2*>(p);
-    v[0] = __uint_as_float(q.x << 16), v[1] = __uint_as_float(q.x & 0xFFFF0000u);
-    v[2] = __uint_as_float(q.y << 16), v[3] = __uint_as_float(q.y & 0xFFFF0000u);
-    return;
+// g and u of 4 units (n of them in range) from the kept parts, and to them
+__device__ inline void load_kept(const TileArgs& a, int q, int at, int n, float (&g)[4], float (&u)[4]) {
+  const uint16_t* hi = a.gu + int64_t(q) * 2 * a.F + at;
+  const uint8_t* lo = a.low + int64_t(q) * a.F + at;
+  uint32_t gp[2] = {0, 0}, up[2] = {0, 0}, w = 0;
+  if (a.vec && n >= 4) {
+    const uint2 g2 = *reinterpret_cast<const uint2*>(hi), u2 = *reinterpret_cast<const uint2*>(hi + a.F);
+    gp[0] = g2.x, gp[1] = g2.y, up[0] = u2.x, up[1] = u2.y;
+    w = *reinterpret_cast<const uint32_t*>(lo);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) {
+        gp[e >> 1] |= uint32_t(hi[e]) << (16 * (e & 1));
+        up[e >> 1] |= uint32_t(hi[a.F + e]) << (16 * (e & 1));
+        w |= uint32_t(lo[e]) << (8 * e);
+      }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = e < n ? bf16_to_f32(p[e]) : 0.0f;
+  for (int e = 0; e < 4; ++e) g[e] = kept(gp[e >> 1], w, e, 0), u[e] = kept(up[e >> 1], w, e, 4);
+}
+
+__device__ inline void store_kept(const TileArgs& a, int q, int at, int n, const float (&g)[4], const float (&u)[4]) {
+  uint16_t* hi = a.gu + int64_t(q) * 2 * a.F + at;
+  uint8_t* lo = a.low + int64_t(q) * a.F + at;
+  uint32_t gb[4], ub[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) gb[e] = round20(g[e]), ub[e] = round20(u[e]);
+  if (a.vec && n >= 4) {
+    const auto pair = [](uint32_t x, uint32_t y) { return (x >> 16) | (y & 0xFFFF0000u); };
+    *reinterpret_cast<uint2*>(hi) = make_uint2(pair(gb[0], gb[1]), pair(gb[2], gb[3]));
+    *reinterpret_cast<uint2*>(hi + a.F) = make_uint2(pair(ub[0], ub[1]), pair(ub[2], ub[3]));
+    *reinterpret_cast<uint32_t*>(lo) = low_bits(gb, ub);
+    return;
+  }
+  const uint32_t w = low_bits(gb, ub);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) {
+      hi[e] = uint16_t(gb[e] >> 16);
+      hi[a.F + e] = uint16_t(ub[e] >> 16);
+      lo[e] = uint8_t(w >> (8 * e));
+    }
 }
 
 // 4 consecutive outputs: d0 (and for the gated forward the up projection d1) of row q, from
@@ -202,8 +259,7 @@ __device__ inline void put_quad(const TileArgs& a, int q, int at, const float (&
     if (n <= 0) return;
     const int64_t row = int64_t(q) * 2 * a.F + at;
     float g[4], u[4], og[4], ou[4];
-    get4(g, a.gu + row, n, a.vec);
-    get4(u, a.gu + row + a.F, n, a.vec);
+    load_kept(a, q, at, n, g, u);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 t = act_pair<ACT>(g[e]);
@@ -218,10 +274,7 @@ __device__ inline void put_quad(const TileArgs& a, int q, int at, const float (&
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = act_of<ACT>(d0[e]) * d1[e];
     put4(a.out + int64_t(q) * a.F + at, h, n, a.vec);
-    if constexpr (EPI == kGatedKeep) {
-      put4(a.gu + int64_t(q) * 2 * a.F + at, d0, n, a.vec);
-      put4(a.gu + int64_t(q) * 2 * a.F + a.F + at, d1, n, a.vec);
-    }
+    if constexpr (EPI == kGatedKeep) store_kept(a, q, at, n, d0, d1);
   }
 }
 
@@ -360,15 +413,6 @@ __device__ inline uint4 pack8(const float (&v)[8]) {
   return make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
 }
 
-__device__ inline void unpack8(float (&v)[8], const uint4& q) {
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[2 * e] = __uint_as_float(w[e] << 16);
-    v[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
-  }
-}
-
 // The epilogue passes the accumulators through LDS, 128 rows of x at a time ([row][256 tile rows of
 // P] in fp32, pitch 260: quads of 16 rows on distinct banks), so that every global access is 16
 // bytes of a 256- or 512-byte run and the code is a short loop: stored straight from the
@@ -426,9 +470,23 @@ void gated_large_kernel(TileArgs a, int xcd_group) {
         if (q < a.q.rows && f < a.F) {
           *reinterpret_cast<uint4*>(a.out + int64_t(q) * a.F + f) = pack8(h);
           if constexpr (EPI == kGatedKeep) {
+            uint32_t gp[4], up[4], lo[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              uint32_t gb[4], ub[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) gb[e] = round20(g[4 * x + e]), ub[e] = round20(u[4 * x + e]);
+              lo[x] = low_bits(gb, ub);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                gp[2 * x + e] = (gb[2 * e] >> 16) | (gb[2 * e + 1] & 0xFFFF0000u);
+                up[2 * x + e] = (ub[2 * e] >> 16) | (ub[2 * e + 1] & 0xFFFF0000u);
+              }
+            }
             uint16_t* gu = a.gu + int64_t(q) * 2 * a.F + f;
-            *reinterpret_cast<uint4*>(gu) = pack8(g);
-            *reinterpret_cast<uint4*>(gu + a.F) = pack8(u);
+            *reinterpret_cast<uint4*>(gu) = make_uint4(gp[0], gp[1], gp[2], gp[3]);
+            *reinterpret_cast<uint4*>(gu + a.F) = make_uint4(up[0], up[1], up[2], up[3]);
+            *reinterpret_cast<uint2*>(a.low + int64_t(q) * a.F + f) = make_uint2(lo[0], lo[1]);
           }
         }
       }
@@ -437,23 +495,26 @@ void gated_large_kernel(TileArgs a, int xcd_group) {
 #pragma unroll 1
       for (int r = rr; r < kEpiRows; r += 4 * kRound) {
         uint4 kg[4], ku[4];
+        uint2 kl[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          const uint16_t* p = a.gu + int64_t(min(row(r + n * kRound), a.q.rows - 1)) * 2 * a.F + min(f, a.F - 8);
-          kg[n] = *reinterpret_cast<const uint4*>(p);
-          ku[n] = *reinterpret_cast<const uint4*>(p + a.F);
+          const int64_t q = min(row(r + n * kRound), a.q.rows - 1);
+          const int at = min(f, a.F - 8);
+          kg[n] = *reinterpret_cast<const uint4*>(a.gu + q * 2 * a.F + at);
+          ku[n] = *reinterpret_cast<const uint4*>(a.gu + q * 2 * a.F + a.F + at);
+          kl[n] = *reinterpret_cast<const uint2*>(a.low + q * a.F + at);
         }
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           const int q = row(r + n * kRound);
-          float g[8], u[8], og[8], ou[8];
-          unpack8(g, kg[n]);
-          unpack8(u, ku[n]);
+          const uint32_t gp[4] = {kg[n].x, kg[n].y, kg[n].z, kg[n].w}, up[4] = {ku[n].x, ku[n].y, ku[n].z, ku[n].w};
+          const uint32_t lo[2] = {kl[n].x, kl[n].y};
+          float og[8], ou[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float d = epi[(r + n * kRound) * kEpiPitch + 8 * o + e];
-            const float2 t = act_pair<ACT>(g[e]);
-            og[e] = d * u[e] * t.y;
+            const float2 t = act_pair<ACT>(kept(gp[e >> 1], lo[e >> 2], e & 3, 0));
+            og[e] = d * kept(up[e >> 1], lo[e >> 2], e & 3, 4) * t.y;
             ou[e] = d * t.x;
           }
           if (q < a.q.rows && f < a.F) {
@@ -470,47 +531,29 @@ void gated_large_kernel(TileArgs a, int xcd_group) {
 // ---- backward, elementwise: [dg du] from dh and the kept [g u] ------------------------------
 struct GatedBwdArgs {
   const uint16_t* dh;  // [M][F], row stride ld
-  const uint16_t* gu;  // [M][2F]
-  uint16_t* dgu;       // [M][2F]
-  int64_t M, ld;
-  int F, windows;      // windows of 8 per row
+  int64_t ld;
+  TileArgs t;          // out: [dg du], gu, low, F, vec; q.rows: M
+  int windows;         // windows of 4 per row
 };
 
 template <int ACT>
 __global__ __launch_bounds__(256) void gated_bwd_kernel(GatedBwdArgs a) {
-  const int64_t total = a.M * a.windows;
+  const int64_t total = int64_t(a.t.q.rows) * a.windows;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-    const int64_t m = i / a.windows;
-    const int f = int(i - m * a.windows) * 8, n = a.F - f;
-    const uint16_t* gp = a.gu + m * 2 * a.F + f;
-    uint16_t* dp = a.dgu + m * 2 * a.F + f;
-    const Pix8 qd = row_vec(a.dh + m * a.ld + f, n), qg = row_vec(gp, n), qu = row_vec(gp + a.F, n);
-    Pix8 og, ou;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      uint32_t pg = 0, pu = 0;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const auto half = [&](uint32_t w) { return __uint_as_float(s ? w & 0xFFFF0000u : w << 16); };
-        const float d = half(qd.v[e]), u = half(qu.v[e]);
-        const float2 t = act_pair<ACT>(half(qg.v[e]));
-        pg |= uint32_t(f32_to_bf16(d * u * t.y)) << (16 * s);
-        pu |= uint32_t(f32_to_bf16(d * t.x)) << (16 * s);
-      }
-      og.v[e] = pg;
-      ou.v[e] = pu;
-    }
-    if (n >= 8) {
-      *reinterpret_cast<Pix8*>(dp) = og;
-      *reinterpret_cast<Pix8*>(dp + a.F) = ou;
+    const int q = int(i / a.windows);
+    const int f = int(i - int64_t(q) * a.windows) * 4;
+    const uint16_t* p = a.dh + q * a.ld + f;
+    float d[4], none[4];
+    const int n = min(4, a.t.F - f);
+    if (n == 4) {
+      const Pix4 v = *reinterpret_cast<const Pix4*>(p);
+      d[0] = __uint_as_float(v.lo << 16), d[1] = __uint_as_float(v.lo & 0xFFFF0000u);
+      d[2] = __uint_as_float(v.hi << 16), d[3] = __uint_as_float(v.hi & 0xFFFF0000u);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < n) {
-          dp[e] = uint16_t(og.v[e >> 1] >> (16 * (e & 1)));
-          dp[a.F + e] = uint16_t(ou.v[e >> 1] >> (16 * (e & 1)));
-        }
+      for (int e = 0; e < 4; ++e) d[e] = e < n ? bf16_to_f32(p[e]) : 0.0f;
     }
+    put_quad<kGatedGrad, ACT>(a.t, q, f, d, none);
   }
 }
 
@@ -587,6 +630,18 @@ bool launch_gated(int act, const TileArgs& a, hipStream_t st) {
   return launch_sized<EPI, PROWS, kRelu>(a, st);
 }
 
+// out, the kept projections and the sizes the epilogues go by (gu: one block of xdna_gated_kept_bytes)
+TileArgs kept_args(int64_t M, int64_t F, const void* gu, uint16_t* out) {
+  TileArgs a = {};
+  a.q.rows = int(M);
+  a.F = int(F);
+  a.out = out;
+  a.gu = static_cast<uint16_t*>(const_cast<void*>(gu));
+  a.low = reinterpret_cast<uint8_t*>(a.gu) + M * F * 4;
+  a.vec = F % 4 == 0 && aligned8(out) && aligned8(gu) ? 1 : 0;
+  return a;
+}
+
 int launched(const char* what, bool ok) {
   return ok ? check_launch(what) : refuse(what, "cannot enable a tile kernel's LDS size");
 }
@@ -598,8 +653,12 @@ using namespace xdna;
 
 extern "C" {
 
+size_t xdna_gated_kept_bytes(int64_t M, int64_t F) {
+  return M < 1 || F < 1 || M > kMaxSide || F > kMaxSide / 2 ? 0 : size_t(M) * size_t(F) * 5;
+}
+
 int xdna_gated_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t M, int64_t K, int64_t F,
-                    int act, uint16_t* h, uint16_t* gu, void* stream) {
+                    int act, uint16_t* h, void* gu, void* stream) {
   const char* what = "xdna_gated_bf16";
   if (const char* why = gated_fault(M, K, F, act)) return refuse(what, why);
   if ((ldx < K && M > 1) || ldw < K) return refuse(what, "rows overlap");
@@ -608,19 +667,16 @@ int xdna_gated_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t l
   if (!x || !w || !h) return refuse(what, "null operand");
   if (odd(x) || odd(w) || odd(h) || odd(gu)) return refuse(what, "misaligned operand");
   if (!admit_launch(what)) return -1;
-  TileArgs a = {};
+  TileArgs a = kept_args(M, F, gu, h);
   a.p = {w, ldw, int(F)};
-  a.q = {x, M > 1 ? ldx : K, int(M)};
+  a.q.src = x;
+  a.q.ld = M > 1 ? ldx : K;
   a.K = int(K);
-  a.out = h;
-  a.gu = gu;
-  a.F = int(F);
-  a.vec = F % 4 == 0 && aligned8(h) && aligned8(gu) ? 1 : 0;
   hipStream_t st = as_stream(stream);
   return launched(what, gu ? launch_gated<kGatedKeep, false>(act, a, st) : launch_gated<kGated, false>(act, a, st));
 }
 
-int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_out, int64_t ldw, const uint16_t* gu,
+int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_out, int64_t ldw, const void* gu,
                             int64_t M, int64_t N, int64_t F, int act, uint16_t* dgu, void* stream) {
   const char* what = "xdna_gated_mlp_bwd_bf16";
   if (const char* why = gated_fault(M, N, F, act)) return refuse(what, why);
@@ -630,14 +686,11 @@ int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_
   if (!dy || !w_out || !gu || !dgu) return refuse(what, "null operand");
   if (odd(dy) || odd(w_out) || odd(gu) || odd(dgu)) return refuse(what, "misaligned operand");
   if (!admit_launch(what)) return -1;
-  TileArgs a = {};
+  TileArgs a = kept_args(M, F, gu, dgu);
   a.p = {w_out, ldw, int(F)};
-  a.q = {dy, M > 1 ? lddy : N, int(M)};
+  a.q.src = dy;
+  a.q.ld = M > 1 ? lddy : N;
   a.K = int(N);
-  a.out = dgu;
-  a.gu = const_cast<uint16_t*>(gu);
-  a.F = int(F);
-  a.vec = F % 4 == 0 && aligned8(dgu) && aligned8(gu) ? 1 : 0;
   return launched(what, launch_gated<kGatedGrad, true>(act, a, as_stream(stream)));
 }
 
@@ -665,7 +718,7 @@ int xdna_tile_mm_bf16(const uint16_t* p, int64_t ldp, int p_rows, const uint16_t
                                  : launch_tiles<false, false, kPlain, kSilu>(a, st));
 }
 
-int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const uint16_t* gu, int64_t M, int64_t F, int act, uint16_t* dgu,
+int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const void* gu, int64_t M, int64_t F, int act, uint16_t* dgu,
                         void* stream) {
   const char* what = "xdna_gated_bwd_bf16";
   if (const char* why = gated_fault(M, 1, F, act)) return refuse(what, why);
@@ -673,8 +726,12 @@ int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const uint16_t* gu, int6
   if (!dh || !gu || !dgu) return refuse(what, "null operand");
   if (odd(dh) || odd(gu) || odd(dgu)) return refuse(what, "misaligned operand");
   if (!admit_launch(what)) return -1;
-  const GatedBwdArgs a = {dh, gu, dgu, M, ld, int(F), int(ceil_div(F, int64_t(8)))};
-  const unsigned grid = unsigned(std::min<int64_t>(ceil_div(a.M * a.windows, int64_t(256)), 16384));
+  GatedBwdArgs a = {};
+  a.dh = dh;
+  a.ld = M > 1 ? ld : F;
+  a.t = kept_args(M, F, gu, dgu);
+  a.windows = int(ceil_div(F, int64_t(4)));
+  const unsigned grid = unsigned(std::min<int64_t>(ceil_div(M * a.windows, int64_t(256)), 16384));
   hipStream_t st = as_stream(stream);
   if (act == kSilu) gated_bwd_kernel<kSilu><<<grid, 256, 0, st>>>(a);
   else if (act == kGelu) gated_bwd_kernel<kGelu><<<grid, 256, 0, st>>>(a);

@@ -145,18 +145,18 @@ GatedForward gated_forward(const at::Tensor& x, const at::Tensor& w_in, int64_t 
   r.w = as_rows(w_in);
   const int64_t M = r.x.size(0), K = r.x.size(1), F = r.w.size(0) / 2;
   r.h = empty_xdna({M, F}, at::kBFloat16);
-  if (keep) r.gu = empty_xdna({M, 2 * F}, at::kBFloat16);
+  if (keep) r.gu = empty_xdna({int64_t(xdna_gated_kept_bytes(M, F))}, at::kByte);
   check_abi(xdna_gated_bf16(p16(r.x), row_stride(r.x), p16(r.w), row_stride(r.w), M, K, F, int(act), m16(r.h),
-                            keep ? m16(r.gu) : nullptr, current_stream()),
+                            keep ? ptr_or_null(r.gu) : nullptr, current_stream()),
             "gated");
   return r;
 }
 
 at::Tensor gated_dgu(const at::Tensor& dh, const at::Tensor& gu, int64_t act) {
   const at::Tensor d = as_rows(dh);
-  at::Tensor dgu = empty_xdna(gu.sizes(), at::kBFloat16);
-  check_abi(xdna_gated_bwd_bf16(p16(d), row_stride(d), p16(gu), gu.size(0), gu.size(1) / 2, int(act), m16(dgu),
-                                current_stream()),
+  const int64_t M = d.size(0), F = d.size(1);
+  at::Tensor dgu = empty_xdna({M, 2 * F}, at::kBFloat16);
+  check_abi(xdna_gated_bwd_bf16(p16(d), row_stride(d), cptr(gu), M, F, int(act), m16(dgu), current_stream()),
             "gated backward");
   return dgu;
 }
@@ -209,8 +209,8 @@ struct GatedMlpFn : public torch::autograd::Function<GatedMlpFn> {
     at::Tensor dx, dw_in, dw_out;
     if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) {
       const at::Tensor wo = as_rows(w_out);
-      at::Tensor dgu = empty_xdna(gu.sizes(), at::kBFloat16);
-      check_abi(xdna_gated_mlp_bwd_bf16(p16(dy), row_stride(dy), p16(wo), row_stride(wo), p16(gu), dy.size(0), dy.size(1),
+      at::Tensor dgu = empty_xdna({h.size(0), 2 * h.size(1)}, at::kBFloat16);
+      check_abi(xdna_gated_mlp_bwd_bf16(p16(dy), row_stride(dy), p16(wo), row_stride(wo), cptr(gu), dy.size(0), dy.size(1),
                                         h.size(1), int(ctx->saved_data["act"].toInt()), m16(dgu), current_stream()),
                 "gated_mlp backward");
       if (ctx->needs_input_grad(0)) dx = product(dgu, as_rows(w_in)).view(x.sizes());

@@ -143,6 +143,7 @@ SIGNATURES = {
     "xdna_embed": (I, [P, I, L, P, I, L, L, L, F, P, P]),
     "xdna_embed_bwd_workspace_bytes": (Z, [L, L, L]),
     "xdna_embed_bwd": (I, [P, I, L, P, I, L, L, L, L, F, P, P, Z, P]),
+    "xdna_gated_kept_bytes": (Z, [L, L]),
     "xdna_gated_bf16": (I, [P, L, P, L, L, L, L, I, P, P, P]),
     "xdna_gated_bwd_bf16": (I, [P, L, P, L, L, I, P, P]),
     "xdna_gated_mlp_bwd_bf16": (I, [P, L, P, L, P, L, L, L, I, P, P]),

@@ -45,7 +45,7 @@ def gated_linear(x: torch.Tensor, w_in: torch.Tensor, activation: str = "silu") 
     """``act(x @ w_in[:F].T) * (x @ w_in[F:].T)`` in one kernel: ``x`` [..., K], ``w_in``
     [2 F, K] (gate rows, then up rows), both bf16; ``activation`` "silu", "gelu" (with erf) or
     "relu".  The projections stay in fp32 through the activation and the product; for the
-    backward they are kept as bf16."""
+    backward they are kept in 20 bits each."""
     return _dev.native().token_gated_linear(x, w_in, _choice(_ACTIVATIONS, activation, "activation"))
 
 
