@@ -3,15 +3,16 @@
 //
 //   y[t] = scale W[id_t];   dW[v] = scale sum over {t: id_t = v} of dy[t], 0 for other rows.
 //
-// The gradient sorts the token positions by id (stable, least significant digit first) and
-// sums each id's rows in that order in fp32, rounded once: the same inputs give the same
-// bits, and no token, however common, makes others wait for its row.
-//   Sort: up to kSortItems positions in one workgroup's LDS, all digits in one launch; more
-// in blocks, a histogram and a scatter launch per digit.  Digits have up to 9 bits: two
-// passes serve every vocabulary below 2^18.
-//   The rows of dW that no token names have to be written too: the sort's first launch,
-// which fills a few CUs only, writes all of dW with zeros in its other workgroups.
-//   Sum: a wave takes kChunk sorted positions and 64 windows of 16 bytes of the columns.  A
+// The gradient sorts the token positions by id (stable) and sums each id's rows in that order
+// in fp32, rounded once: the same inputs give the same bits, and no token, however common,
+// makes others wait for its row.
+//   Order of up to kRankItems positions: by counting.  A workgroup holds all ids in LDS and
+// counts, for 64 positions, the ids that come before: one launch and no passes.  The count
+// grows with the square of the positions; above, a radix sort in blocks, a histogram and a
+// scatter launch per digit of up to 9 bits (two digits serve every vocabulary below 2^18).
+//   The rows of dW that no token names have to be written too: the ordering launches, which are
+// bound by latency, share the writing of zeros to all of dW among their other workgroups.
+//   Sum: a wave takes a chunk of sorted positions and 64 windows of 16 bytes of the columns.  A
 // run of one id inside the chunk is written straight to dW; the parts of a run that crosses
 // chunks go to fp32 partials (one slot for the run that came in, one for the run that goes
 // on), which a last launch joins in chunk order.
@@ -24,10 +25,12 @@
 namespace xdna {
 namespace {
 
-constexpr int kChunk = 32;           // sorted positions per wave
+constexpr int kMinChunk = 8, kMaxChunk = 64;  // sorted positions per wave (a group of loads; its lanes)
 constexpr int kSortPer = 8;          // positions per thread of a sorting workgroup
 constexpr int kSortThreads = 1024;
 constexpr int kSortItems = kSortPer * kSortThreads;
+constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kRankItems = 16384;    // 64 KB of ids in LDS
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
 
 template <typename T>
@@ -142,15 +145,14 @@ struct SortArgs {
   int index_bytes;
   int n, vocab;
   int64_t padding;
-  int shift, bits;         // this pass's digit (block form)
-  int passes, pass_bits;   // all passes (one-workgroup form)
+  int shift, bits;         // this pass's digit
   const uint32_t* key_in;  // null: from ids
   const uint32_t* pos_in;
   uint32_t* key;
   uint32_t* pos;
   uint32_t* hist;          // [blocks][kDigits]
   int blocks;
-  uint4* fill;             // zeros for fill_bytes bytes, by the workgroups past the sorting ones
+  char* fill;              // zeros for fill_bytes bytes, by the workgroups past the sorting ones
   int64_t fill_bytes;
 };
 
@@ -160,12 +162,72 @@ __device__ inline uint32_t sort_key(const SortArgs& a, int64_t i) {
   return id < 0 || id >= a.vocab || id == a.padding ? uint32_t(a.vocab) : uint32_t(id);
 }
 
+// fill_bytes are whole 16-byte vectors but for the last launch's end
 __device__ inline void zero_fill(const SortArgs& a, int block, int blocks, int threads) {
   const int64_t whole = a.fill_bytes >> 4;
   const int64_t step = int64_t(blocks) * threads;
-  for (int64_t i = int64_t(block) * threads + threadIdx.x; i < whole; i += step) a.fill[i] = make_uint4(0, 0, 0, 0);
+  uint4* to = reinterpret_cast<uint4*>(a.fill);
+  for (int64_t i = int64_t(block) * threads + threadIdx.x; i < whole; i += step) to[i] = make_uint4(0, 0, 0, 0);
   if (block == 0 && threadIdx.x < ((a.fill_bytes & 15) >> 1))
-    reinterpret_cast<uint16_t*>(a.fill + whole)[threadIdx.x] = 0;
+    reinterpret_cast<uint16_t*>(to + whole)[threadIdx.x] = 0;
+}
+
+// Order by counting: workgroup b finds the places of positions 64 b .. 64 b + 63 (lane l: 64 b +
+// l), each of its 16 waves against a sixteenth of all keys, read from LDS four at a time.  A key
+// comes before an equal one at a later position.
+__global__ __launch_bounds__(kSortThreads) void rank_kernel(SortArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t keys[];  // [n rounded up to 64]
+  __shared__ uint32_t part[kSortThreads];
+  if (int(blockIdx.x) >= a.blocks) {
+    zero_fill(a, int(blockIdx.x) - a.blocks, int(gridDim.x) - a.blocks, kSortThreads);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int groups = a.blocks;
+  // (clamped positions: the loads of a round are issued together)
+  for (int base = 0; base < groups * 64; base += 8 * kSortThreads) {
+    uint32_t k[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) k[j] = sort_key(a, min(base + j * kSortThreads + tid, a.n - 1));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = base + j * kSortThreads + tid;
+      if (i < groups * 64) keys[i] = i < a.n ? k[j] : 0xFFFFFFFFu;
+    }
+  }
+  __syncthreads();
+  const int own = blockIdx.x;
+  const uint32_t mine = keys[own * 64 + lane];
+  uint32_t count = 0;
+  for (int g = wave; g < groups; g += kSortWaves) {
+    const uint4* q = reinterpret_cast<const uint4*>(keys + g * 64);
+    if (g == own) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint4 v = q[i];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) count += w[e] < mine || (w[e] == mine && 4 * i + e < lane) ? 1u : 0u;
+      }
+    } else {
+      // keys below `least` come before: mine itself, or one more where equal ones do (keys of
+      // real positions are below 2^31)
+      const uint32_t least = mine + (g < own ? 1u : 0u);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint4 v = q[i];
+        count += (v.x < least ? 1u : 0u) + (v.y < least ? 1u : 0u) + (v.z < least ? 1u : 0u) + (v.w < least ? 1u : 0u);
+      }
+    }
+  }
+  part[tid] = count;
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int w = 1; w < kSortWaves; ++w) count += part[w * 64 + lane];
+    const int i = own * 64 + lane;
+    if (i < a.n) a.key[count] = mine, a.pos[count] = uint32_t(i);
+  }
 }
 
 // Ranks of this thread's items within the workgroup's items of equal digit, in item order
@@ -209,72 +271,6 @@ __device__ inline uint32_t digit_prefix(uint32_t v, uint32_t* red) {
   return base + s - v;
 }
 
-constexpr int kSortWaves = kSortThreads / 64;
-constexpr size_t kSortLds = size_t(2) * kSortItems * 4 + size_t(kSortWaves) * kDigits * 4;
-
-// All passes over up to kSortItems positions in LDS (workgroup 0; the others fill dW).
-__global__ __launch_bounds__(kSortThreads) void sort_small_kernel(SortArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
-  if (blockIdx.x > 0) {
-    zero_fill(a, int(blockIdx.x) - 1, int(gridDim.x) - 1, kSortThreads);
-    return;
-  }
-  __shared__ uint32_t red[kDigits / 64];
-  uint32_t* keys = lds;
-  uint32_t* poss = lds + kSortItems;
-  uint32_t* count = lds + 2 * kSortItems;  // [waves][kDigits]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int first = wave * (64 * kSortPer) + lane;
-  uint32_t key[kSortPer], pos[kSortPer], rank[kSortPer], digit[kSortPer];
-#pragma unroll
-  for (int j = 0; j < kSortPer; ++j) {
-    const int i = first + j * 64;
-    // places past the end hold the greatest key and the last positions: they stay last
-    key[j] = i < a.n ? sort_key(a, i) : 0xFFFFFFFFu;
-    pos[j] = uint32_t(i);
-  }
-  for (int p = 0; p < a.passes; ++p) {
-    const int shift = p * a.pass_bits;
-    const uint32_t mask = (1u << a.pass_bits) - 1;
-    uint32_t* mine = count + wave * kDigits;
-#pragma unroll
-    for (int d = 0; d < kDigits / 64; ++d) mine[d * 64 + lane] = 0;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int j = 0; j < kSortPer; ++j) digit[j] = (key[j] >> shift) & mask;
-    wave_rank(digit, a.pass_bits, mine, lane, rank);
-    __syncthreads();
-    // counts -> first places: digits in order, waves in order within a digit
-    uint32_t total = 0;
-    if (tid < kDigits)
-      for (int w = 0; w < kSortWaves; ++w) total += count[w * kDigits + tid];
-    uint32_t place = digit_prefix(total, red);
-    if (tid < kDigits)
-      for (int w = 0; w < kSortWaves; ++w) {
-        const uint32_t c = count[w * kDigits + tid];
-        count[w * kDigits + tid] = place;
-        place += c;
-      }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kSortPer; ++j) {
-      const uint32_t at = mine[digit[j]] + rank[j];
-      keys[at] = key[j];
-      poss[at] = pos[j];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kSortPer; ++j) key[j] = keys[first + j * 64], pos[j] = poss[first + j * 64];
-    __syncthreads();
-  }
-#pragma unroll
-  for (int j = 0; j < kSortPer; ++j) {
-    const int i = first + j * 64;
-    if (i < a.n) a.key[i] = key[j], a.pos[i] = pos[j];
-  }
-}
-
 // One pass in blocks of kSortItems: digit counts of each block ...
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
   __shared__ uint32_t count[kDigits];
@@ -300,6 +296,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) {
   __shared__ uint32_t count[kSortWaves * kDigits];
   __shared__ uint32_t red[kDigits / 64];
+  if (int(blockIdx.x) >= a.blocks) {
+    zero_fill(a, int(blockIdx.x) - a.blocks, int(gridDim.x) - a.blocks, kSortThreads);
+    return;
+  }
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t first = int64_t(blockIdx.x) * kSortItems + wave * (64 * kSortPer) + lane;
   const uint32_t mask = (1u << a.bits) - 1;
@@ -350,49 +350,70 @@ struct SumArgs {
   const uint32_t* key;
   const uint32_t* pos;
   int n, vocab, dim, slices;  // slices of 64 windows along dim
-  int chunks;
+  int chunk, chunks;
   const void* dy;
   int64_t ld;
   void* dw;      // [vocab][dim]
-  float* part;   // [chunks][2][dim]
+  float* part;   // [chunks][2][pitch]
+  int pitch;     // dim rounded up to windows
   float scale;
 };
 
+template <int W>
+__device__ inline void put_part(float* p, const float (&v)[W]) {
+#pragma unroll
+  for (int e = 0; e < W; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+}
+
+template <int W>
+__device__ inline void add_part(float (&v)[W], const float* p) {
+#pragma unroll
+  for (int e = 0; e < W; e += 4) {
+    const float4 q = *reinterpret_cast<const float4*>(p + e);
+    v[e] += q.x, v[e + 1] += q.y, v[e + 2] += q.z, v[e + 3] += q.w;
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
-  constexpr int W = EW<T>::n;
+  constexpr int W = EW<T>::n, G = 8;  // rows in flight
   const int lane = threadIdx.x & 63;
   const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (item >= int64_t(a.chunks) * a.slices) return;
   const int chunk = __builtin_amdgcn_readfirstlane(int(item / a.slices));
   const int slice = __builtin_amdgcn_readfirstlane(int(item - int64_t(chunk) * a.slices));
-  const int first = chunk * kChunk;
-  const int count = min(kChunk, a.n - first);
+  const int first = chunk * a.chunk;
+  const int count = min(a.chunk, a.n - first);
   const int col = (slice * 64 + lane) * W;
   const int width = a.dim - col;  // below 1: this lane has no column
-  // the chunk's keys in lanes 0 .. 31, the neighbours' in lanes 32 and 33
+  // the chunk's keys and positions by lane; the neighbours' keys
   uint32_t k = 0xFFFFFFFFu, ps = 0;
   if (lane < count) k = a.key[first + lane], ps = a.pos[first + lane];
-  if (lane == 32 && first > 0) k = a.key[first - 1];
-  if (lane == 33 && first + count < a.n) k = a.key[first + count];
-  const uint32_t prev = __builtin_amdgcn_readlane(k, 32), next = __builtin_amdgcn_readlane(k, 33);
+  const uint32_t prev = first > 0 ? a.key[first - 1] : 0xFFFFFFFFu;
+  const uint32_t next = first + count >= a.n ? 0xFFFFFFFFu : a.key[first + count];
   const T* dy = static_cast<const T*>(a.dy);
+  const auto load = [&](int base, Pix8 (&q)[G]) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int at = min(base + i, count - 1);
+      q[i] = {{0u, 0u, 0u, 0u}};
+      if (uint32_t(__builtin_amdgcn_readlane(k, at)) < uint32_t(a.vocab) && width > 0)
+        q[i] = window<T>(dy + int64_t(uint32_t(__builtin_amdgcn_readlane(ps, at))) * a.ld + col, width);
+    }
+  };
   float acc[W];
 #pragma unroll
   for (int e = 0; e < W; ++e) acc[e] = 0.0f;
-  bool came_in = __builtin_amdgcn_readlane(k, 0) == prev;
-  for (int base = 0; base < count; base += 8) {
-    Pix8 q[8];
+  bool came_in = uint32_t(__builtin_amdgcn_readlane(k, 0)) == prev;
+  Pix8 nq[G];
+  load(0, nq);
+  for (int base = 0; base < count; base += G) {
+    Pix8 q[G];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = base + i;
-      const uint32_t id = at < count ? __builtin_amdgcn_readlane(k, at) : 0xFFFFFFFFu;
-      q[i] = {{0u, 0u, 0u, 0u}};
-      if (id < uint32_t(a.vocab) && width > 0)
-        q[i] = window<T>(dy + int64_t(__builtin_amdgcn_readlane(ps, at)) * a.ld + col, width);
-    }
+    for (int i = 0; i < G; ++i) q[i] = nq[i];
+    if (base + G < count) load(base + G, nq);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < G; ++i) {
       const int at = base + i;
       if (at >= count) break;
       const uint32_t id = __builtin_amdgcn_readlane(k, at);
@@ -401,19 +422,16 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
       unpack<T>(q[i], v);
 #pragma unroll
       for (int e = 0; e < W; ++e) acc[e] += v[e];
-      const uint32_t after = at + 1 < count ? __builtin_amdgcn_readlane(k, at + 1) : next;
-      const bool ends = at + 1 < count || first + count < a.n ? after != id : true;
-      if (!ends && at + 1 < count) continue;
+      const bool edge = at + 1 == count;
+      const bool ends = (edge ? next : uint32_t(__builtin_amdgcn_readlane(k, min(at + 1, 63)))) != id;
+      if (!ends && !edge) continue;
       if (width > 0) {
         if (ends && !came_in) {
 #pragma unroll
           for (int e = 0; e < W; ++e) v[e] = acc[e] * a.scale;
           put_window<T>(static_cast<T*>(a.dw) + int64_t(id) * a.dim + col, v, width);
         } else {
-          float* to = a.part + (int64_t(chunk) * 2 + (came_in ? 0 : 1)) * a.dim + col;
-#pragma unroll
-          for (int e = 0; e < W; ++e)
-            if (e < width) to[e] = acc[e];
+          put_part<W>(a.part + (int64_t(chunk) * 2 + (came_in ? 0 : 1)) * a.pitch + col, acc);
         }
       }
 #pragma unroll
@@ -423,26 +441,24 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
   }
 }
 
-// Joins the runs that cross chunks: the wave of the chunk where a run begins.
+// Joins the runs that cross chunks: a workgroup for the chunk where a run begins and a slice of
+// the columns; of a long run each of its four waves adds a quarter, in order.
 template <typename T>
 __global__ __launch_bounds__(256) void sum_join_kernel(SumArgs a) {
   constexpr int W = EW<T>::n;
-  const int lane = threadIdx.x & 63;
-  const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (item >= int64_t(a.chunks - 1) * a.slices) return;
-  const int chunk = __builtin_amdgcn_readfirstlane(int(item / a.slices));
-  const int slice = __builtin_amdgcn_readfirstlane(int(item - int64_t(chunk) * a.slices));
-  const int last = (chunk + 1) * kChunk - 1;  // chunk + 1 exists: position last + 1 does
-  const uint32_t id = a.key[last];
-  if (id >= uint32_t(a.vocab) || a.key[last + 1] != id) return;
-  const int first = chunk * kChunk;
+  __shared__ __attribute__((aligned(16))) float quarter[3][64 * W];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunk = int(blockIdx.x) / a.slices, slice = int(blockIdx.x) - chunk * a.slices;
+  const int first = chunk * a.chunk;
+  const int64_t after = int64_t(first) + a.chunk;  // chunk + 1 exists: position `after` does
+  const uint32_t id = a.key[after - 1];
+  if (id >= uint32_t(a.vocab) || a.key[after] != id) return;
   if (a.key[first] == id && first > 0 && a.key[first - 1] == id) return;  // it began earlier
-  // chunks after this one that the run reaches: chunk + 1, and further while the last position
-  // of a chunk and the first of the next still hold id
+  // chunks after this one that the run reaches: chunk + 1, and further while the first position
+  // of a next one still holds id
   int reach = 1;
   for (;;) {
-    const int64_t c = int64_t(chunk) + reach + lane;  // does the run go on past chunk c?
-    const int64_t at = (c + 1) * kChunk;
+    const int64_t at = (int64_t(chunk) + reach + lane + 1) * a.chunk;
     const bool on = at < a.n && a.key[at] == id;
     const uint64_t stop = ~__ballot(on);
     if (stop) {
@@ -451,19 +467,30 @@ __global__ __launch_bounds__(256) void sum_join_kernel(SumArgs a) {
     }
     reach += 64;
   }
+  const bool shared = reach > 16;
+  if (!shared && wave > 0) return;
   const int col = (slice * 64 + lane) * W;
   const int width = a.dim - col;
-  if (width <= 0) return;
   float acc[W];
-  const float* from = a.part + (int64_t(chunk) * 2 + 1) * a.dim + col;
 #pragma unroll
-  for (int e = 0; e < W; ++e) acc[e] = e < width ? from[e] : 0.0f;
+  for (int e = 0; e < W; ++e) acc[e] = 0.0f;
+  if (width > 0) {
+    const int64_t step = 2 * int64_t(a.pitch);
+    const float* from = a.part + int64_t(chunk) * step + col;
+    if (wave == 0) add_part<W>(acc, from + a.pitch);
+    const int share = (reach + 3) / 4;
+    const int lo = shared ? 1 + wave * share : 1, hi = shared ? min(reach, lo + share - 1) : reach;
 #pragma unroll 8
-  for (int j = 1; j <= reach; ++j) {
-    const float* p = a.part + int64_t(chunk + j) * 2 * a.dim + col;
-#pragma unroll
-    for (int e = 0; e < W; ++e) acc[e] += e < width ? p[e] : 0.0f;
+    for (int j = lo; j <= hi; ++j) add_part<W>(acc, from + j * step);
   }
+  if (shared) {
+    if (wave > 0) put_part<W>(&quarter[wave - 1][lane * W], acc);
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) add_part<W>(acc, &quarter[w][lane * W]);
+  }
+  if (width <= 0) return;
 #pragma unroll
   for (int e = 0; e < W; ++e) acc[e] *= a.scale;
   put_window<T>(static_cast<T*>(a.dw) + int64_t(id) * a.dim + col, acc, width);
@@ -475,7 +502,8 @@ __global__ __launch_bounds__(256) void sum_join_kernel(SumArgs a) {
 int64_t up16(int64_t b) { return (b + 15) & ~int64_t(15); }
 
 struct GradPlan {
-  int bits, passes, pass_bits, blocks, chunks;
+  int bits, passes, pass_bits, blocks, chunk, chunks, pitch;
+  bool rank;
   int64_t keys, hist, part, total;  // byte sizes and the total
 };
 
@@ -485,12 +513,17 @@ GradPlan grad_plan(int64_t tokens, int64_t vocab, int64_t dim) {
   while ((int64_t(1) << p.bits) <= vocab) ++p.bits;  // keys 0 .. vocab
   p.passes = int(ceil_div(p.bits, kDigitBits));
   p.pass_bits = int(ceil_div(p.bits, p.passes));
-  p.blocks = int(ceil_div(tokens, int64_t(kSortItems)));
-  p.chunks = int(ceil_div(tokens, int64_t(kChunk)));
+  p.rank = tokens <= kRankItems;
+  p.blocks = int(ceil_div(tokens, int64_t(p.rank ? 64 : kSortItems)));
+  p.pitch = int(ceil_div(dim, int64_t(8)) * 8);
+  // chunks that give 4096 waves (four a SIMD)
+  p.chunk = kMinChunk;
+  while (p.chunk < kMaxChunk && ceil_div(tokens, int64_t(2 * p.chunk)) * ceil_div(dim, int64_t(512)) >= 4096) p.chunk *= 2;
+  p.chunks = int(ceil_div(tokens, int64_t(p.chunk)));
   p.keys = up16(tokens * 4);
-  p.hist = p.blocks > 1 ? up16(int64_t(p.blocks) * kDigits * 4) : 0;
-  p.part = up16(int64_t(p.chunks) * 2 * dim * 4);
-  p.total = p.keys * (p.blocks > 1 ? 4 : 2) + p.hist + p.part;
+  p.hist = p.rank ? 0 : up16(int64_t(p.blocks) * kDigits * 4);
+  p.part = int64_t(p.chunks) * 2 * p.pitch * 4;
+  p.total = p.keys * (p.rank ? 2 : 4) + p.hist + p.part;
   return p;
 }
 
@@ -516,8 +549,12 @@ template <typename T>
 void launch_sums(const SumArgs& s, hipStream_t st) {
   const int64_t items = int64_t(s.chunks) * s.slices;
   sum_kernel<T><<<unsigned(ceil_div(items, int64_t(4))), 256, 0, st>>>(s);
-  if (s.chunks > 1)
-    sum_join_kernel<T><<<unsigned(ceil_div(int64_t(s.chunks - 1) * s.slices, int64_t(4))), 256, 0, st>>>(s);
+  if (s.chunks > 1) sum_join_kernel<T><<<unsigned(int64_t(s.chunks - 1) * s.slices), 256, 0, st>>>(s);
+}
+
+// Workgroups for a share of the zeros: 64 KB each, up to four a CU.
+unsigned fillers(int64_t bytes) {
+  return unsigned(std::max<int64_t>(bytes > 0 ? 1 : 0, std::min<int64_t>(ceil_div(bytes, int64_t(65536)), 1024)));
 }
 
 }  // namespace
@@ -561,9 +598,8 @@ int xdna_embed_bwd(const void* ids, int index_bytes, int64_t tokens, const void*
   const GradPlan p = grad_plan(std::max<int64_t>(tokens, 1), vocab, dim);
   if (tokens > 0 && (!workspace || workspace_bytes < size_t(p.total) || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return refuse(what, "workspace missing, misaligned or too small");
-  static const bool lds_ok = hipFuncSetAttribute(reinterpret_cast<const void*>(&sort_small_kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, int(kSortLds)) == hipSuccess;
-  if (!lds_ok) return refuse(what, "cannot enable the sort's LDS size");
+  if (int64_t(p.chunks) * ceil_div(dim, int64_t(64) * (dtype == 1 ? 4 : 8)) > kMaxGridX256)
+    return refuse(what, "too many rows and columns");
   if (!admit_launch(what)) return -1;
   hipStream_t st = as_stream(stream);
   SortArgs s = {};
@@ -572,28 +608,34 @@ int xdna_embed_bwd(const void* ids, int index_bytes, int64_t tokens, const void*
   s.n = int(tokens);
   s.vocab = int(vocab);
   s.padding = padding;
-  s.fill = static_cast<uint4*>(d_weight);
+  s.fill = static_cast<char*>(d_weight);
   s.fill_bytes = vocab * dim * (dtype == 1 ? 4 : 2);
-  // 32 KB of zeros per filling workgroup and round
-  const unsigned fillers = unsigned(std::max<int64_t>(1, std::min<int64_t>(ceil_div(s.fill_bytes, int64_t(32768)), 1024)));
-  if (tokens == 0) {  // nothing to sort: workgroup 0 of the counting kernel fills as well
-    sort_count_kernel<<<fillers, kSortThreads, 0, st>>>(s);
+  if (tokens == 0) {  // nothing to order
+    sort_count_kernel<<<fillers(s.fill_bytes), kSortThreads, 0, st>>>(s);
     return check_launch(what);
   }
   char* ws = static_cast<char*>(workspace);
   uint32_t* buf[4];  // key, position, and the other side of the passes
-  for (int i = 0; i < (p.blocks > 1 ? 4 : 2); ++i, ws += p.keys) buf[i] = reinterpret_cast<uint32_t*>(ws);
+  for (int i = 0; i < (p.rank ? 2 : 4); ++i, ws += p.keys) buf[i] = reinterpret_cast<uint32_t*>(ws);
   s.hist = reinterpret_cast<uint32_t*>(ws);
   ws += p.hist;
   int side = 0;
-  if (p.blocks == 1) {
-    s.passes = p.passes;
-    s.pass_bits = p.pass_bits;
+  s.blocks = p.blocks;
+  if (p.rank) {
+    static const bool lds_ok = hipFuncSetAttribute(reinterpret_cast<const void*>(&rank_kernel),
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, kRankItems * 4) == hipSuccess;
+    if (!lds_ok) return refuse(what, "cannot enable the ordering kernel's LDS size");
     s.key = buf[0];
     s.pos = buf[1];
-    sort_small_kernel<<<1 + fillers, kSortThreads, kSortLds, st>>>(s);
+    rank_kernel<<<unsigned(p.blocks) + fillers(s.fill_bytes), kSortThreads, size_t(p.blocks) * 256, st>>>(s);
   } else {
-    s.blocks = p.blocks;
+    const int64_t all = s.fill_bytes, share = ceil_div(all, int64_t(2 * p.passes) * 16) * 16;
+    const auto next_share = [&](int i) {  // of the i-th launch
+      const int64_t lo = std::min(all, i * share), hi = std::min(all, lo + share);
+      s.fill = static_cast<char*>(d_weight) + lo;
+      s.fill_bytes = hi - lo;
+      return unsigned(p.blocks) + fillers(s.fill_bytes);
+    };
     for (int i = 0; i < p.passes; ++i) {
       s.shift = i * p.pass_bits;
       s.bits = p.pass_bits;
@@ -602,8 +644,10 @@ int xdna_embed_bwd(const void* ids, int index_bytes, int64_t tokens, const void*
       side = i ? 2 - side : 0;
       s.key = buf[side];
       s.pos = buf[side + 1];
-      sort_count_kernel<<<unsigned(p.blocks) + (i ? 0 : fillers), kSortThreads, 0, st>>>(s);
-      sort_scatter_kernel<<<unsigned(p.blocks), kSortThreads, 0, st>>>(s);
+      const unsigned count_grid = next_share(2 * i);
+      sort_count_kernel<<<count_grid, kSortThreads, 0, st>>>(s);
+      const unsigned scatter_grid = next_share(2 * i + 1);
+      sort_scatter_kernel<<<scatter_grid, kSortThreads, 0, st>>>(s);
     }
   }
   SumArgs m = {};
@@ -613,7 +657,9 @@ int xdna_embed_bwd(const void* ids, int index_bytes, int64_t tokens, const void*
   m.vocab = int(vocab);
   m.dim = int(dim);
   m.slices = int(ceil_div(dim, int64_t(64) * (dtype == 1 ? 4 : 8)));
+  m.chunk = p.chunk;
   m.chunks = p.chunks;
+  m.pitch = p.pitch;
   m.dy = grad;
   m.ld = ld;
   m.dw = d_weight;

@@ -627,3 +627,19 @@ def test_gated_mlp_large(T, M, K, F, N, act):
     some = gated_reference(x, torch.cat([w[units], w[F + units]]), wo[:, units], dy, act, True)
     close(dw.cpu()[torch.cat([units, F + units])], *some["dw_in"], "dw_in")
     close(dwo.cpu()[:, units], *some["dw_out"], "dw_out")
+
+
+@pytest.mark.parametrize("n,V,D", [(16384, 90, 200), (16385, 90, 200), (40000, 5, 70), (70000, 1 << 18, 12), (3000, 1, 600), (100, 100000, 2)])
+def test_embedding_gradient_of_long_runs_and_both_orders(T, n, V, D):
+    """Around the size where the order's kernels change, few ids (runs over many chunks), many ids."""
+    print("embedding runs", n, V, D, flush=True)
+    g = gen(n + V)
+    ids = torch.randint(0, V, (n,), generator=g)
+    ids[: n // 2] = V // 2
+    dy = torch.randn(n, D, generator=g).bfloat16()
+    w = torch.zeros(V, D, dtype=BF16, device="xdna", requires_grad=True)
+    (dw,) = torch.autograd.grad(T.embed(ids.to("xdna"), w), [w], dy.to("xdna"))
+    ref = torch.zeros(V, D, dtype=F64).index_add_(0, ids, dy.to(F64))
+    mag = torch.zeros(V, D, dtype=F64).index_add_(0, ids, dy.to(F64).abs())
+    count = torch.bincount(ids, minlength=V).to(F64)[:, None]
+    close(dw, ref, (count + 2) * U * mag + B * ref.abs(), "gradient")
