@@ -386,6 +386,111 @@ __global__ __launch_bounds__(Tile<WIDE>::NT) void tile_kernel(TileArgs a) {
   }
 }
 
+// ---- few rows -------------------------------------------------------------------------------------
+// A step of decoding: bound by the weights' bytes, which pass once from memory to registers.  A
+// workgroup takes 16 units (their gate and up rows) or `span` plain rows as the rows of 16x16x32
+// MFMAs, its eight waves every eighth k-step, with the loads of up to 8 steps in flight; x's
+// fragments come from L2.  The waves' sums are added in wave order through LDS.  (Sixteen waves
+// were slower: 6.7 -> 7.3 us for 1 x 4096 -> 1024, 4.1 -> 4.6 for 1 x 1024 -> 4096.)
+//   Fewer than 16 plain rows a workgroup (the MFMA's other rows repeat them) put every CU to work
+// where there are few.  With up to 4 rows of x the repeats become useful: MFMA row (c, i) holds
+// weight row i and column (c', m) row m of x, both at the c-th or c'-th of 4 chunks of 32 k, so
+// that a load reads 1 KB of weights instead of 256 bytes; the products with c == c' are the sum's
+// terms, the others are dropped.
+constexpr int kFewGated = 64, kFewPlain = 16;  // most rows of x
+
+template <int MT, int CH, int EPI, int ACT>
+__global__ __launch_bounds__(512) void few_kernel(TileArgs a) {
+  constexpr bool GATED = EPI == kGated || EPI == kGatedKeep;
+  constexpr int PT = GATED ? 2 : 1, WAVES = 8, STEP = 32 * CH;
+  extern __shared__ __attribute__((aligned(16))) float4 red[];  // [wave][PT][MT][lane]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int span = GATED ? 16 : CH > 1 ? 4 : a.F;  // units of the workgroup: 16, 8 or 4
+  const int p0 = blockIdx.x * span, r = lane & 15;
+  const int kq = (lane >> 4) * 8 + (CH > 1 ? (r >> 2) * 32 : 0);
+  const uint16_t* wp[PT];
+  const uint16_t* xp[MT];
+  const int units = GATED ? a.F : a.p.rows;
+#pragma unroll
+  for (int p = 0; p < PT; ++p) wp[p] = a.p.src + (int64_t(min(p0 + (r & (span - 1)), units - 1)) + int64_t(p) * a.F) * a.p.ld + kq;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) xp[t] = a.q.src + int64_t(min(t * 16 + (CH > 1 ? r & 3 : r), a.q.rows - 1)) * a.q.ld + kq;
+  f32x4_t acc[PT][MT];
+#pragma unroll
+  for (int p = 0; p < PT; ++p)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[p][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const auto frag = [](const Pix8& v) { return as_bf16x8(u32x4_t{v.v[0], v.v[1], v.v[2], v.v[3]}); };
+  const auto multiply = [&](const Pix8 (&w)[PT], const Pix8 (&x)[MT]) {
+#pragma unroll
+    for (int p = 0; p < PT; ++p)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+        acc[p][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(w[p]), frag(x[t]), acc[p][t], 0, 0, 0);
+  };
+  const int whole = a.K / STEP;  // steps without a ragged end
+  const auto batch = [&](int s0, auto steps) {
+    constexpr int U = decltype(steps)::value;
+    Pix8 w[U][PT], x[U][MT];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {  // (steps past the end load the last one again, unused)
+      const int k = min(s0 + i * WAVES, whole - 1) * STEP;
+#pragma unroll
+      for (int p = 0; p < PT; ++p) w[i][p] = *reinterpret_cast<const Pix8*>(wp[p] + k);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) x[i][t] = *reinterpret_cast<const Pix8*>(xp[t] + k);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (s0 + i * WAVES < whole) multiply(w[i], x[i]);
+  };
+  int s0 = wave;
+  if constexpr (MT == 1)
+    for (; s0 + 7 * WAVES < whole; s0 += 8 * WAVES) batch(s0, std::integral_constant<int, 8>{});
+  for (; s0 < whole; s0 += 4 * WAVES) batch(s0, std::integral_constant<int, 4>{});
+  if (whole * STEP < a.K && whole % WAVES == wave) {
+    const int n = a.K - whole * STEP - kq;
+    Pix8 w[PT], x[MT];
+#pragma unroll
+    for (int p = 0; p < PT; ++p) w[p] = row_vec(wp[p] - kq + min(whole * STEP + kq, a.K), max(n, 0));
+#pragma unroll
+    for (int t = 0; t < MT; ++t) x[t] = row_vec(xp[t] - kq + min(whole * STEP + kq, a.K), max(n, 0));
+    multiply(w, x);
+  }
+#pragma unroll
+  for (int p = 0; p < PT; ++p)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+      red[((wave * PT + p) * MT + t) * 64 + lane] = make_float4(acc[p][t][0], acc[p][t][1], acc[p][t][2], acc[p][t][3]);
+  __syncthreads();
+  if constexpr (CH > 1) {
+    // rows m of x by thread; chunk c's terms are with lanes 16 c + 4 c + m
+    if (tid >= 4 || tid >= a.q.rows || p0 >= units) return;
+    float d[4] = {}, none[4] = {};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const float4 v = red[w * 64 + 20 * c + tid];
+        d[0] += v.x, d[1] += v.y, d[2] += v.z, d[3] += v.w;
+      }
+    put_quad<EPI, ACT>(a, tid, p0, d, none);
+    return;
+  }
+  if (tid >= MT * 64) return;
+  const int t = tid >> 6, q = t * 16 + r, at = p0 + 4 * (lane >> 4);
+  if (q >= a.q.rows || at >= units || 4 * (lane >> 4) >= span) return;
+  float d[2][4] = {};
+#pragma unroll
+  for (int p = 0; p < PT; ++p)
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float4 v = red[((w * PT + p) * MT + t) * 64 + lane];
+      d[p][0] += v.x, d[p][1] += v.y, d[p][2] += v.z, d[p][3] += v.w;
+    }
+  put_quad<EPI, ACT>(a, q, at, d[0], d[1]);
+}
+
 // ---- large tiles --------------------------------------------------------------------------------
 // The 256 x 256 tile of the library's large products (gemm_dma.h): operands that can be loaded as
 // whole 16-byte vectors by the LDS DMA.  Rows of P (the hidden units) run along the MFMA's rows:
@@ -583,11 +688,37 @@ bool launch_tile(const TileArgs& a, dim3 grid, hipStream_t st) {
   return true;
 }
 
+template <int MT, int CH, int EPI, int ACT>
+bool launch_few(TileArgs a, hipStream_t st) {
+  constexpr bool GATED = EPI == kGated || EPI == kGatedKeep;
+  constexpr size_t lds = size_t(8) * (GATED ? 2 : 1) * MT * 1024;
+  static_assert(lds <= 65536, "the waves' sums fit the LDS a launch has without asking");
+  int span = CH > 1 ? 4 : 16;
+  if (!GATED) {
+    while (span > 4 && ceil_div(a.p.rows, span) < 256) span /= 2;
+    a.F = span;
+  }
+  few_kernel<MT, CH, EPI, ACT><<<unsigned(ceil_div(GATED ? a.F : a.p.rows, span)), 512, lds, st>>>(a);
+  return true;
+}
+
 // Wide tiles where they give every CU one: below that the narrow ones share a block's k.
 template <bool PROWS, bool QROWS, int EPI, int ACT>
 bool launch_tiles(const TileArgs& a, hipStream_t st) {
   constexpr int side = EPI == kGated || EPI == kGatedKeep ? 2 : 1;  // tile rows per unit of p
   const auto tiles = [&](int t) { return dim3(unsigned(ceil_div(int64_t(a.p.rows) * side, t)), unsigned(ceil_div(a.q.rows, t))); };
+  if constexpr (!PROWS && !QROWS) {
+    if constexpr (EPI == kPlain) {
+      // chunks of k where k is long or the weight's rows are few: 4096 rows of 1024 take 4.1 us
+      // without them and 6.0 with (a step per wave), 1024 rows of 4096 6.7 and 4.2
+      if (a.q.rows <= 4 && (a.K >= 2048 || a.p.rows <= 2048)) return launch_few<1, 4, EPI, ACT>(a, st);
+      if (a.q.rows <= kFewPlain) return launch_few<1, 1, EPI, ACT>(a, st);
+    } else {
+      if (a.q.rows <= 16) return launch_few<1, 1, EPI, ACT>(a, st);
+      if (a.q.rows <= 32) return launch_few<2, 1, EPI, ACT>(a, st);
+      if (a.q.rows <= kFewGated) return launch_few<4, 1, EPI, ACT>(a, st);
+    }
+  }
   const dim3 wide = tiles(128), narrow = tiles(64);
   if (int64_t(wide.x) * wide.y >= 256 || narrow.y > 65535) return launch_tile<true, PROWS, QROWS, EPI, ACT>(a, wide, st);
   return launch_tile<false, PROWS, QROWS, EPI, ACT>(a, narrow, st);

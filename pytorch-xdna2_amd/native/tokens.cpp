@@ -70,13 +70,15 @@ bool vector_rows(const at::Tensor& t) {
 }
 
 // a b of two bf16 matrices, each contiguous along one dimension.  Operands that xdna_gemm_bf16
-// would load element by element take the tiles that load at any alignment.
+// would load element by element, and few rows against a weight's rows, take the gated block's
+// own tiles.
 at::Tensor product(const at::Tensor& a, const at::Tensor& b) {
   const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
   at::Tensor c = empty_xdna({M, N}, at::kBFloat16);
   const bool b_rows = b.stride(1) == 1 && K > 1, a_rows = a.stride(0) == 1 && M > 1 && a.stride(1) != 1;
   const bool a_ok = a_rows ? b_rows : a.stride(1) == 1 || K == 1, b_ok = b_rows || b.stride(0) == 1 || K == 1;
-  if (K > 0 && !(vector_rows(a) && vector_rows(b)) && a_ok && b_ok) {
+  const bool few = M <= 16 && !a_rows && !b_rows;
+  if (K > 0 && (few || !(vector_rows(a) && vector_rows(b))) && a_ok && b_ok) {
     const int64_t lda = a_rows ? a.stride(1) : M > 1 ? a.stride(0) : K, ldb = b_rows ? b.stride(0) : N > 1 ? b.stride(1) : K;
     check_abi(xdna_tile_mm_bf16(p16(b), ldb, b_rows ? 1 : 0, p16(a), lda, a_rows ? 1 : 0, N, M, K, m16(c), N,
                                 current_stream()),
