@@ -46,7 +46,10 @@ __device__ inline float2 act_pair(float g) {
 // ---- products in tiles, any sizes, alignments and row strides --------------------------------
 // D[p][q] = sum over k of P[p][k] Q[q][k], written at out[q * ldc + p]: the p index is the one
 // that is contiguous in memory, so that the 4 consecutive rows an MFMA accumulator quad holds
-// are 4 consecutive elements of the output (and of [g u] beside it).  Each operand is contiguous
+// are 4 consecutive elements of the output (and of [g u] beside it); the block's results go through
+// LDS, so that 8 consecutive outputs are one access and consecutive threads continue the row
+// (stored straight from the accumulators, each wave's store touched 32 rows: the epilogue of the
+// projections of 3972 x 692 -> 998 units took most of its 64 us).  Each operand is contiguous
 // along k, or along its rows (then staged [k][row] and transposed by the LDS reads).  Loads are
 // 16 bytes at any element-aligned address (gfx950 takes them); out-of-range elements are zeros.
 //
@@ -54,8 +57,14 @@ __device__ inline float2 act_pair(float g) {
 //   wide tiles, 128 x 128: four waves side by side, k-tiles of 64;
 //   narrow tiles, 64 x 64, where wide ones would leave CUs without work: eight waves on the
 // same block, each with its own k-step of a k-tile of 128 (an eighth of the k-tiles' memory
-// latencies of one wave), their accumulators added in wave order through LDS.
+// latencies of one wave), their accumulators added in wave order through LDS.  Where even they
+// leave CUs without work (weight gradients: short outputs, k as long as the batch), plain
+// products split k over the grid too, into fp32 partials that a second launch adds in order.
 // The next k-tile's loads fly in registers during a k-tile's MFMAs; one barrier per k-tile.
+// Addresses are formed once, per vector and not per k-tile; a row past the operand reads the last
+// one (its results are not stored), so that only the last k-tile and the vectors across a
+// row-contiguous operand's end are masked.  (Addresses and masks formed in every k-tile took more
+// VALU time than the MFMAs: 445 us for the block at 4895 x 448 x 1506, forward and backward.)
 enum TileEpi { kPlain = 0, kGated = 1, kGatedKeep = 2, kGatedGrad = 3 };
 
 struct TileOperand {
@@ -73,6 +82,8 @@ struct TileArgs {
   uint8_t* low;    // ... and the low ones, [q][F]: g's in bits 0-3, u's in bits 4-7
   int F;           // kGated*: p.src holds F gate rows, then F up rows (p.rows = F)
   int vec;         // 8-byte accesses of out and gu: their addresses and strides are multiples of 4
+  float* part;     // kPlain with k split over blockIdx.z: [split][q][p] partials, else null
+  int k_split;     // k per split (whole k-tiles)
 };
 
 __device__ inline Pix8 row_vec(const uint16_t* p, int n) {  // n elements, zeros after them
@@ -82,6 +93,26 @@ __device__ inline Pix8 row_vec(const uint16_t* p, int n) {  // n elements, zeros
   for (int e = 0; e < 8; ++e)
     if (e < n) q.v[e >> 1] |= uint32_t(p[e]) << ((e & 1) * 16);
   return q;
+}
+
+// v without its first s (0 .. 7) elements, zeros after the others
+__device__ inline Pix8 shifted(Pix8 q, int s) {
+  if (s & 4) q.v[0] = q.v[2], q.v[1] = q.v[3], q.v[2] = 0u, q.v[3] = 0u;
+  if (s & 2) q.v[0] = q.v[1], q.v[1] = q.v[2], q.v[2] = q.v[3], q.v[3] = 0u;
+  if (s & 1) {
+    q.v[0] = q.v[0] >> 16 | q.v[1] << 16;
+    q.v[1] = q.v[1] >> 16 | q.v[2] << 16;
+    q.v[2] = q.v[2] >> 16 | q.v[3] << 16;
+    q.v[3] = q.v[3] >> 16;
+  }
+  return q;
+}
+
+// row_vec where the 8 - n elements before p can be read: the 16 bytes that end with element n - 1
+__device__ inline Pix8 end_vec(const uint16_t* p, int n) {
+  if (n <= 0) return {{0u, 0u, 0u, 0u}};
+  const int s = 8 - min(n, 8);
+  return shifted(*reinterpret_cast<const Pix8*>(p - s), s);
 }
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
@@ -99,35 +130,77 @@ struct Tile {
 };
 
 // Row of the operand that tile row r holds: itself, or (gated) 32 gate rows and the same 32
-// units' up rows in turn, so that one wave has both.  -1 past the operand.
+// units' up rows in turn, so that one wave has both.  Past the operand: its last row.
 template <bool GATED>
 __device__ inline int64_t tile_row(const TileArgs& a, const TileOperand& o, int r0, int r) {
-  if constexpr (GATED) {
-    const int f = r0 / 2 + (r >> 6) * 32 + (r & 31);
-    return f < a.F ? f + int64_t((r >> 5) & 1) * a.F : -1;
-  }
-  return r0 + r < o.rows ? r0 + r : -1;
+  if constexpr (GATED) return min(r0 / 2 + (r >> 6) * 32 + (r & 31), a.F - 1) + int64_t((r >> 5) & 1) * a.F;
+  return min(r0 + r, o.rows - 1);
 }
 
+// One operand's loads: per thread V vectors of 16 bytes of a k-tile, vector j at from[j] + t step,
+// its k offset in the k-tile kq[j].  A row-contiguous vector across the operand's end is read from
+// 8 elements before the end and shifted when it is stored (a shift, or a masked load, where it is
+// read would wait for it there, and the ragged tiles would take several times the others' time).
 template <bool WIDE, bool ROWS, bool GATED>
-__device__ inline void tile_load(Pix8 (&v)[Tile<WIDE>::V], const TileArgs& a, const TileOperand& o, int r0, int k0,
-                                 int tid) {
+struct TileLoads {
   using C = Tile<WIDE>;
+  const uint16_t* from[C::V];
+  int64_t step;  // elements between k-tiles
+  int kq[C::V];
+  int shift;     // row-contiguous: elements before the first one
+  bool inside;   // all the tile's rows are the operand's
+  bool run;      // 8 elements along the contiguous direction exist
+  int n;         // row-contiguous: rows from the vector's first on (below 1: none)
+
+  __device__ inline void plan(const TileArgs& a, const TileOperand& o, int r0, int kbeg, int tid) {
+    step = ROWS ? C::KT * o.ld : C::KT;
+    inside = !ROWS || r0 + C::T <= o.rows;
+    run = (ROWS ? o.rows : a.K) >= 8;
+    shift = 0;
+    n = 8;
 #pragma unroll
-  for (int j = 0; j < C::V; ++j) {
-    const int i = tid + j * C::NT;
-    if constexpr (!ROWS) {
-      constexpr int kVecs = C::KT / 8;
-      const int64_t r = tile_row<GATED>(a, o, r0, i / kVecs);
-      const int k = k0 + (i % kVecs) * 8;
-      v[j] = row_vec(o.src + (r < 0 ? 0 : r) * o.ld + min(k, a.K), r < 0 ? 0 : a.K - k);
-    } else {
-      constexpr int rVecs = C::T / 8;
-      const int r = r0 + (i % rVecs) * 8, k = k0 + i / rVecs;
-      v[j] = row_vec(o.src + int64_t(min(k, a.K - 1)) * o.ld + min(r, o.rows), k < a.K ? o.rows - r : 0);
+    for (int j = 0; j < C::V; ++j) {
+      const int i = tid + j * C::NT;
+      if constexpr (!ROWS) {
+        kq[j] = i % (C::KT / 8) * 8;
+        from[j] = o.src + tile_row<GATED>(a, o, r0, i / (C::KT / 8)) * o.ld + kbeg + kq[j];
+      } else {  // (NT is a multiple of the vectors along the rows: the same rows for every j)
+        const int r = r0 + i % (C::T / 8) * 8, first = max(min(r, o.rows - 8), 0);
+        kq[j] = i / (C::T / 8);
+        n = o.rows - r;
+        shift = run ? min(r - first, 7) : 0;  // (rows past the end: anything)
+        from[j] = o.src + int64_t(kbeg + kq[j]) * o.ld + first;
+      }
     }
   }
-}
+
+  // the k-tile `t`: `left` is what k has from its start on
+  __device__ inline void load(Pix8 (&v)[C::V], int t, int left) const {
+    if (left >= C::KT && run) {
+#pragma unroll
+      for (int j = 0; j < C::V; ++j) v[j] = *reinterpret_cast<const Pix8*>(from[j] + t * step);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < C::V; ++j) {
+      // (from[j] + t step is not formed for a vector that is not read)
+      if constexpr (ROWS) {
+        const bool in = kq[j] < left;
+        v[j] = row_vec(in ? from[j] + t * step : from[j], in ? (run ? 8 : n) : 0);
+      } else {
+        const int got = left - kq[j];
+        const uint16_t* p = got > 0 ? from[j] + t * step : from[j];
+        v[j] = run ? end_vec(p, got) : row_vec(p, got);
+      }
+    }
+  }
+
+  __device__ inline void align(Pix8 (&v)[C::V]) const {
+    if (!ROWS || inside) return;
+#pragma unroll
+    for (int j = 0; j < C::V; ++j) v[j] = shifted(v[j], shift);
+  }
+};
 
 // [k][row] tiles: 16-byte pieces of 8 rows, permuted by the k row so that the transposing reads'
 // 4 k rows fall on distinct banks
@@ -278,8 +351,123 @@ __device__ inline void put_quad(const TileArgs& a, int q, int at, const float (&
   }
 }
 
+struct __attribute__((packed, aligned(4))) Floats4 {  // 16 bytes at any fp32 element
+  float v[4];
+};
+
+struct __attribute__((packed, aligned(1))) Bytes8 {
+  uint32_t v[2];
+};
+
+// n (at most 8) elements at p
+__device__ inline void put_vec(uint16_t* p, const Pix8& v, int n) {
+  if (n >= 8) {
+    *reinterpret_cast<Pix8*>(p) = v;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n) p[e] = uint16_t(v.v[e >> 1] >> (16 * (e & 1)));
+}
+
+__device__ inline Pix8 pack_vec(const float (&v)[8]) {
+  return {{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])}};
+}
+
+// 8 units' kept projections (n in range), high parts and low bits
+__device__ inline void load_kept8(const TileArgs& a, int q, int at, int n, Pix8& g, Pix8& u, Bytes8& low) {
+  const uint16_t* hi = a.gu + int64_t(q) * 2 * a.F + at;
+  const uint8_t* lo = a.low + int64_t(q) * a.F + at;
+  g = row_vec(hi, n);
+  u = row_vec(hi + a.F, n);
+  if (n >= 8) {
+    low = *reinterpret_cast<const Bytes8*>(lo);
+    return;
+  }
+  low = {{0u, 0u}};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n) low.v[e >> 2] |= uint32_t(lo[e]) << (8 * (e & 3));
+}
+
+__device__ inline void store_kept8(const TileArgs& a, int q, int at, int n, const float (&g)[8], const float (&u)[8]) {
+  Pix8 gp, up;
+  Bytes8 low;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    uint32_t gb[4], ub[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) gb[e] = round20(g[4 * x + e]), ub[e] = round20(u[4 * x + e]);
+    low.v[x] = low_bits(gb, ub);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      gp.v[2 * x + e] = (gb[2 * e] >> 16) | (gb[2 * e + 1] & 0xFFFF0000u);
+      up.v[2 * x + e] = (ub[2 * e] >> 16) | (ub[2 * e + 1] & 0xFFFF0000u);
+    }
+  }
+  uint16_t* hi = a.gu + int64_t(q) * 2 * a.F + at;
+  uint8_t* lo = a.low + int64_t(q) * a.F + at;
+  put_vec(hi, gp, n);
+  put_vec(hi + a.F, up, n);
+  if (n >= 8) {
+    *reinterpret_cast<Bytes8*>(lo) = low;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n) lo[e] = uint8_t(low.v[e >> 2] >> (8 * (e & 3)));
+}
+
+// [dg du] of 8 units from dh and the kept projections
+template <int ACT>
+__device__ inline void grad8(const float (&d)[8], const Pix8& g, const Pix8& u, const Bytes8& low, float (&dg)[8],
+                             float (&du)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float2 t = act_pair<ACT>(kept(g.v[e >> 1], low.v[e >> 2], e & 3, 0));
+    dg[e] = d[e] * kept(u.v[e >> 1], low.v[e >> 2], e & 3, 4) * t.y;
+    du[e] = d[e] * t.x;
+  }
+}
+
+// 8 consecutive outputs of row q from column `at` on (n of them in range): d0, and for the gated
+// forward the up projection d1
+template <int EPI, int ACT>
+__device__ inline void put_row8(const TileArgs& a, int q, int at, int n, const float (&d0)[8], const float (&d1)[8]) {
+  if constexpr (EPI == kPlain) {
+    if (a.part) {
+      float* to = a.part + (int64_t(blockIdx.z) * a.q.rows + q) * a.p.rows + at;
+      if (n >= 8) {
+        *reinterpret_cast<Floats4*>(to) = {{d0[0], d0[1], d0[2], d0[3]}};
+        *reinterpret_cast<Floats4*>(to + 4) = {{d0[4], d0[5], d0[6], d0[7]}};
+        return;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n) to[e] = d0[e];
+      return;
+    }
+    put_vec(a.out + int64_t(q) * a.ldc + at, pack_vec(d0), n);
+  } else if constexpr (EPI == kGatedGrad) {
+    Pix8 g, u;
+    Bytes8 low;
+    load_kept8(a, q, at, n, g, u, low);
+    float dg[8], du[8];
+    grad8<ACT>(d0, g, u, low, dg, du);
+    uint16_t* to = a.out + int64_t(q) * 2 * a.F + at;
+    put_vec(to, pack_vec(dg), n);
+    put_vec(to + a.F, pack_vec(du), n);
+  } else {
+    float h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = act_of<ACT>(d0[e]) * d1[e];
+    put_vec(a.out + int64_t(q) * a.F + at, pack_vec(h), n);
+    if constexpr (EPI == kGatedKeep) store_kept8(a, q, at, n, d0, d1);
+  }
+}
+
 template <bool WIDE, bool PROWS, bool QROWS, int EPI, int ACT>
-__global__ __launch_bounds__(Tile<WIDE>::NT) void tile_kernel(TileArgs a) {
+__global__ __launch_bounds__(Tile<WIDE>::NT, WIDE ? 2 : 4) void tile_kernel(TileArgs a) {
   using C = Tile<WIDE>;
   constexpr bool GATED = EPI == kGated || EPI == kGatedKeep;
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];  // [2 buffers][P, Q]
@@ -291,18 +479,27 @@ __global__ __launch_bounds__(Tile<WIDE>::NT) void tile_kernel(TileArgs a) {
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc[i][j] = zero_acc();
+  const int kbeg = EPI == kPlain && a.part ? int(blockIdx.z) * a.k_split : 0;
+  const int kend = EPI == kPlain && a.part ? min(a.K, kbeg + a.k_split) : a.K;
+  TileLoads<WIDE, PROWS, GATED> lp;
+  TileLoads<WIDE, QROWS, false> lq;
+  lp.plan(a, a.p, p0, kbeg, tid);
+  lq.plan(a, a.q, q0, kbeg, tid);
   Pix8 rp[C::V], rq[C::V];
-  tile_load<WIDE, PROWS, GATED>(rp, a, a.p, p0, 0, tid);
-  tile_load<WIDE, QROWS, false>(rq, a, a.q, q0, 0, tid);
+  lp.load(rp, 0, kend - kbeg);
+  lq.load(rq, 0, kend - kbeg);
+  lp.align(rp);
+  lq.align(rq);
   tile_store<WIDE, PROWS>(smem, rp, tid);
   tile_store<WIDE, QROWS>(smem + C::ELEMS, rq, tid);
   __syncthreads();
-  int b = 0;
-  for (int k0 = 0; k0 < a.K; k0 += C::KT) {
-    const bool more = k0 + C::KT < a.K;
+  const int tiles = (kend - kbeg + C::KT - 1) / C::KT;
+  for (int t = 0; t < tiles; ++t) {
+    const bool more = t + 1 < tiles;
+    const int b = t & 1;
     if (more) {
-      tile_load<WIDE, PROWS, GATED>(rp, a, a.p, p0, k0 + C::KT, tid);
-      tile_load<WIDE, QROWS, false>(rq, a, a.q, q0, k0 + C::KT, tid);
+      lp.load(rp, t + 1, kend - kbeg - (t + 1) * C::KT);
+      lq.load(rq, t + 1, kend - kbeg - (t + 1) * C::KT);
     }
     const uint16_t* ps = smem + b * 2 * C::ELEMS;
     const uint16_t* qs = ps + C::ELEMS;
@@ -322,66 +519,102 @@ __global__ __launch_bounds__(Tile<WIDE>::NT) void tile_kernel(TileArgs a) {
     }
     if (more) {  // the other buffer's last reads ended before the previous barrier
       uint16_t* to = smem + (b ^ 1) * 2 * C::ELEMS;
+      lp.align(rp);
+      lq.align(rq);
       tile_store<WIDE, PROWS>(to, rp, tid);
       tile_store<WIDE, QROWS>(to + C::ELEMS, rq, tid);
     }
     __syncthreads();
-    b ^= 1;
   }
-  // accumulator quads: (i, j) block, rows 8 g + 4 (lane / 32) .. +3 of it, column lane % 32
-  const auto column = [&](int i, int g, int l) {  // of the output's contiguous index
-    return GATED ? p0 / 2 + wp * 32 + 8 * g + 4 * (l >> 5) : p0 + wp * 64 + i * 32 + 8 * g + 4 * (l >> 5);
-  };
+  // the block as [q][p] in fp32.  Accumulator quad (i, j, g): p 32 i + 8 g + 4 (lane / 32) .. +3,
+  // q 32 j + lane % 32 of the wave's block.
+  constexpr int EP = C::T + 4;  // (a quad's 16 rows on distinct banks)
+  float* block = reinterpret_cast<float*>(smem);
   if constexpr (WIDE) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int q = q0 + wq * 64 + j * 32 + (lane & 31);
-      if (q >= a.q.rows) continue;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-#pragma unroll
-        for (int i = 0; i < (GATED ? 1 : 2); ++i) {
-          float d0[4], d1[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) d0[e] = acc[i][j][4 * g + e], d1[e] = GATED ? acc[1][j][4 * g + e] : 0.0f;
-          if (column(i, g, lane) < (GATED ? a.F : a.p.rows)) put_quad<EPI, ACT>(a, q, column(i, g, lane), d0, d1);
-        }
-      }
-    }
-  } else {
-    // two rounds (j): the eight waves' quads [wave][i][g][lane] in 64 KB, a thread per (g, lane)
-    // pair and, of plain results, per i
-    float4* red = reinterpret_cast<float4*>(smem);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          red[((wave * 2 + i) * 4 + g) * 64 + lane] =
+          *reinterpret_cast<float4*>(block + (wq * 64 + j * 32 + (lane & 31)) * EP + wp * 64 + i * 32 + 8 * g + 4 * (lane >> 5)) =
               make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+  } else {
+    // two rounds (j): the eight waves' quads [wave][i][g][lane] in 64 KB, summed by a thread per
+    // (i, g, lane)
+    float4* red = reinterpret_cast<float4*>(smem);
+    const int g = wave & 3, i = wave >> 2;
+    float4 sum[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          red[((wave * 2 + x) * 4 + y) * 64 + lane] =
+              make_float4(acc[x][j][4 * y], acc[x][j][4 * y + 1], acc[x][j][4 * y + 2], acc[x][j][4 * y + 3]);
       __syncthreads();
-      const int g = (tid >> 6) & 3, half = tid >> 8;
-      const auto sum = [&](int i, float (&d)[4]) {
+      sum[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d[e] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          const float4 v = red[((w * 2 + i) * 4 + g) * 64 + lane];
-          d[0] += v.x, d[1] += v.y, d[2] += v.z, d[3] += v.w;
-        }
-      };
-      const int q = q0 + j * 32 + (lane & 31);
-      if (q < a.q.rows && (!GATED || half == 0)) {
-        const int at = column(half, g, lane);
-        if (at < (GATED ? a.F : a.p.rows)) {
-          float d0[4], d1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          sum(GATED ? 0 : half, d0);
-          if (GATED) sum(1, d1);
-          put_quad<EPI, ACT>(a, q, at, d0, d1);
-        }
+      for (int w = 0; w < 8; ++w) {
+        const float4 v = red[((w * 2 + i) * 4 + g) * 64 + lane];
+        sum[j].x += v.x, sum[j].y += v.y, sum[j].z += v.z, sum[j].w += v.w;
       }
       __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      *reinterpret_cast<float4*>(block + (j * 32 + (lane & 31)) * EP + i * 32 + 8 * g + 4 * (lane >> 5)) = sum[j];
+  }
+  __syncthreads();
+  // rows in windows of 8 outputs, consecutive threads along a row
+  constexpr int kAcross = (GATED ? C::T / 2 : C::T) / 8;
+  const int o = tid % kAcross;
+  const int at = (GATED ? p0 / 2 : p0) + 8 * o, n = (EPI == kPlain ? a.p.rows : a.F) - at;
+  const float* from = block + (GATED ? (o >> 2) * 64 + (o & 3) * 8 : 8 * o);
+  if (n <= 0) return;
+#pragma unroll 2
+  for (int r = tid / kAcross; r < C::T; r += C::NT / kAcross) {
+    if (q0 + r >= a.q.rows) break;
+    float d0[8], d1[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d0[e] = from[r * EP + e], d1[e] = GATED ? from[r * EP + 32 + e] : 0.0f;
+    put_row8<EPI, ACT>(a, q0 + r, at, n, d0, d1);
+  }
+}
+
+// out[q][p] = the partials of the k splits, added in order, four outputs a thread (eight splits'
+// loads in flight)
+__global__ __launch_bounds__(256) void tile_join_kernel(TileArgs a, int splits) {
+  const int64_t n = int64_t(a.q.rows) * a.p.rows;
+  for (int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4; i < n; i += int64_t(gridDim.x) * 1024) {
+    float d[4] = {};
+    const int m = int(n - i < 4 ? n - i : 4);
+    for (int z = 0; z < splits; z += 8) {
+      Floats4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float* p = a.part + int64_t(min(z + u, splits - 1)) * n + i;
+        if (m == 4) {
+          v[u] = *reinterpret_cast<const Floats4*>(p);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[u].v[e] = e < m ? p[e] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (z + u < splits) d[0] += v[u].v[0], d[1] += v[u].v[1], d[2] += v[u].v[2], d[3] += v[u].v[3];
+    }
+    if (a.ldc == a.p.rows && m == 4) {
+      *reinterpret_cast<Pix4*>(a.out + i) = {pack2(d[0], d[1]), pack2(d[2], d[3])};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < m) {
+          const int64_t q = (i + e) / a.p.rows;
+          a.out[q * a.ldc + (i + e - q * a.p.rows)] = f32_to_bf16(d[e]);
+        }
     }
   }
 }
@@ -514,10 +747,6 @@ __device__ inline G5Operand gated_operand(const TileArgs& a, int f0, int tid) {
   return o;
 }
 
-__device__ inline uint4 pack8(const float (&v)[8]) {
-  return make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
-}
-
 // The epilogue passes the accumulators through LDS, 128 rows of x at a time ([row][256 tile rows of
 // P] in fp32, pitch 260: quads of 16 rows on distinct banks), so that every global access is 16
 // bytes of a 256- or 512-byte run and the code is a short loop: stored straight from the
@@ -566,66 +795,31 @@ void gated_large_kernel(TileArgs a, int xcd_group) {
       const float* at = epi + (o >> 1) * 32 + (o & 1) * 8;
 #pragma unroll 2
       for (int r = rr; r < kEpiRows; r += kRound) {
-        const int q = row(r);
-        float g[8], u[8], h[8];
+        float g[8], u[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[e] = at[r * kEpiPitch + e], u[e] = at[r * kEpiPitch + 16 + e];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = act_of<ACT>(g[e]) * u[e];
-        if (q < a.q.rows && f < a.F) {
-          *reinterpret_cast<uint4*>(a.out + int64_t(q) * a.F + f) = pack8(h);
-          if constexpr (EPI == kGatedKeep) {
-            uint32_t gp[4], up[4], lo[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              uint32_t gb[4], ub[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) gb[e] = round20(g[4 * x + e]), ub[e] = round20(u[4 * x + e]);
-              lo[x] = low_bits(gb, ub);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                gp[2 * x + e] = (gb[2 * e] >> 16) | (gb[2 * e + 1] & 0xFFFF0000u);
-                up[2 * x + e] = (ub[2 * e] >> 16) | (ub[2 * e + 1] & 0xFFFF0000u);
-              }
-            }
-            uint16_t* gu = a.gu + int64_t(q) * 2 * a.F + f;
-            *reinterpret_cast<uint4*>(gu) = make_uint4(gp[0], gp[1], gp[2], gp[3]);
-            *reinterpret_cast<uint4*>(gu + a.F) = make_uint4(up[0], up[1], up[2], up[3]);
-            *reinterpret_cast<uint2*>(a.low + int64_t(q) * a.F + f) = make_uint2(lo[0], lo[1]);
-          }
-        }
+        if (row(r) < a.q.rows && f < a.F) put_row8<EPI, ACT>(a, row(r), f, 8, g, u);
       }
     } else {
       // four rows' [g u] in flight: clamped addresses, no branch around the loads
 #pragma unroll 1
       for (int r = rr; r < kEpiRows; r += 4 * kRound) {
-        uint4 kg[4], ku[4];
-        uint2 kl[4];
+        Pix8 kg[4], ku[4];
+        Bytes8 kl[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int64_t q = min(row(r + n * kRound), a.q.rows - 1);
-          const int at = min(f, a.F - 8);
-          kg[n] = *reinterpret_cast<const uint4*>(a.gu + q * 2 * a.F + at);
-          ku[n] = *reinterpret_cast<const uint4*>(a.gu + q * 2 * a.F + a.F + at);
-          kl[n] = *reinterpret_cast<const uint2*>(a.low + q * a.F + at);
-        }
+        for (int n = 0; n < 4; ++n)
+          load_kept8(a, min(row(r + n * kRound), a.q.rows - 1), min(f, a.F - 8), 8, kg[n], ku[n], kl[n]);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           const int q = row(r + n * kRound);
-          const uint32_t gp[4] = {kg[n].x, kg[n].y, kg[n].z, kg[n].w}, up[4] = {ku[n].x, ku[n].y, ku[n].z, ku[n].w};
-          const uint32_t lo[2] = {kl[n].x, kl[n].y};
-          float og[8], ou[8];
+          float d[8], og[8], ou[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float d = epi[(r + n * kRound) * kEpiPitch + 8 * o + e];
-            const float2 t = act_pair<ACT>(kept(gp[e >> 1], lo[e >> 2], e & 3, 0));
-            og[e] = d * kept(up[e >> 1], lo[e >> 2], e & 3, 4) * t.y;
-            ou[e] = d * t.x;
-          }
+          for (int e = 0; e < 8; ++e) d[e] = epi[(r + n * kRound) * kEpiPitch + 8 * o + e];
+          grad8<ACT>(d, kg[n], ku[n], kl[n], og, ou);
           if (q < a.q.rows && f < a.F) {
             uint16_t* to = a.out + int64_t(q) * 2 * a.F + f;
-            *reinterpret_cast<uint4*>(to) = pack8(og);
-            *reinterpret_cast<uint4*>(to + a.F) = pack8(ou);
+            put_vec(to, pack_vec(og), 8);
+            put_vec(to + a.F, pack_vec(ou), 8);
           }
         }
       }
@@ -702,7 +896,26 @@ bool launch_few(TileArgs a, hipStream_t st) {
   return true;
 }
 
-// Wide tiles where they give every CU one: below that the narrow ones share a block's k.
+// k split over the grid into `splits` parts, joined by a second launch
+template <bool WIDE, bool PROWS, bool QROWS>
+bool launch_split(TileArgs a, dim3 grid, int64_t splits, hipStream_t st) {
+  constexpr int kt = Tile<WIDE>::KT;
+  a.k_split = int(ceil_div(ceil_div(a.K, kt), splits)) * kt;
+  grid.z = unsigned(ceil_div(a.K, a.k_split));
+  const int64_t n = int64_t(a.p.rows) * a.q.rows;
+  a.part = static_cast<float*>(xdna_hip_cache_alloc(size_t(grid.z) * size_t(n) * sizeof(float)));
+  if (!a.part) return false;
+  const bool ok = launch_tile<WIDE, PROWS, QROWS, kPlain, kSilu>(a, grid, st);
+  if (ok) tile_join_kernel<<<unsigned(std::min<int64_t>(ceil_div(n, int64_t(1024)), 4096)), 256, 0, st>>>(a, int(grid.z));
+  xdna_hip_cache_free(a.part);  // stream-ordered reuse: the block's next user runs after the join
+  return ok;
+}
+
+// Wide tiles where they give every CU one, with k split over the grid (plain products: towards
+// two a CU, six k-tiles a split or more, twelve where the tiles alone come near) where that gives
+// half the CUs one; else narrow tiles, split towards two a CU with two k-tiles a split or more.
+// Measured, p x q x k: 218 x 5893 x 5632 wide and split 47 us, narrow 74; 960 x 495 x 2832 21.6
+// and 27.0; 692 x 3972 x 998 36.1 and 28.5 (16 k-tiles, 192 wide tiles).
 template <bool PROWS, bool QROWS, int EPI, int ACT>
 bool launch_tiles(const TileArgs& a, hipStream_t st) {
   constexpr int side = EPI == kGated || EPI == kGatedKeep ? 2 : 1;  // tile rows per unit of p
@@ -720,7 +933,16 @@ bool launch_tiles(const TileArgs& a, hipStream_t st) {
     }
   }
   const dim3 wide = tiles(128), narrow = tiles(64);
-  if (int64_t(wide.x) * wide.y >= 256 || narrow.y > 65535) return launch_tile<true, PROWS, QROWS, EPI, ACT>(a, wide, st);
+  const int64_t wides = int64_t(wide.x) * wide.y, narrows = int64_t(narrow.x) * narrow.y;
+  if constexpr (EPI == kPlain) {
+    const int64_t split = std::min(512 / wides, ceil_div(a.K, Tile<true>::KT) / (wides < 160 ? 6 : 12));
+    if (split > 1 && wides * split >= 128) return launch_split<true, PROWS, QROWS>(a, wide, split, st);
+  }
+  if (wides >= 256 || narrow.y > 65535) return launch_tile<true, PROWS, QROWS, EPI, ACT>(a, wide, st);
+  if constexpr (EPI == kPlain) {
+    const int64_t split = std::min(ceil_div(512, narrows), ceil_div(a.K, Tile<false>::KT) / 2);
+    if (split > 1) return launch_split<false, PROWS, QROWS>(a, narrow, split, st);
+  }
   return launch_tile<false, PROWS, QROWS, EPI, ACT>(a, narrow, st);
 }
 
@@ -745,11 +967,13 @@ bool launch_large(const TileArgs& a, dim3 grid, hipStream_t st) {
   return true;
 }
 
+// Large tiles where they give every CU one (8192 x 512 -> 1024 units: 256 tiles 27 us, against 38
+// in wide tiles; with 128 tiles the wide ones are ahead: 28 against 37 for the gradient there).
 template <int EPI, bool PROWS, int ACT>
 bool launch_sized(const TileArgs& a, hipStream_t st) {
   constexpr bool GATED = EPI != kGatedGrad;
   const dim3 grid(unsigned(ceil_div(a.F, GATED ? kT4 / 2 : kT4)), unsigned(ceil_div(a.q.rows, kT4)));
-  const bool large = int64_t(grid.x) * grid.y >= 128 && a.K % 8 == 0 && a.F % 8 == 0 && aligned16(a.out) && aligned16(a.gu) &&
+  const bool large = int64_t(grid.x) * grid.y >= 256 && a.K % 8 == 0 && a.F % 8 == 0 && aligned16(a.out) && aligned16(a.gu) &&
                      dma_ok(a.p, GATED ? 2 * int64_t(a.F) : a.F, a.K, PROWS) && dma_ok(a.q, a.q.rows, a.K, false);
   return large ? launch_large<PROWS, EPI, ACT>(a, grid, st) : launch_tiles<PROWS, false, EPI, ACT>(a, st);
 }
@@ -774,7 +998,7 @@ TileArgs kept_args(int64_t M, int64_t F, const void* gu, uint16_t* out) {
 }
 
 int launched(const char* what, bool ok) {
-  return ok ? check_launch(what) : refuse(what, "cannot enable a tile kernel's LDS size");
+  return ok ? check_launch(what) : refuse(what, "no memory for partial sums, or a tile kernel's LDS size cannot be had");
 }
 
 }  // namespace

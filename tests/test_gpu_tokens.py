@@ -597,8 +597,8 @@ def test_refusals_on_the_device(T):
         torch.autograd.grad(T.token_log_probs(zx, y).entropy.sum(), [zx], create_graph=True)
 
 
-LARGE = [  # rows, K, F, N: at least 128 tiles of 256 x 256, ragged at the edges
-    (4000, 264, 1000, 264), (2049, 72, 4104, 40), (300, 1024, 16384, 64), (8200, 512, 512, 1024),
+LARGE = [  # rows, K, F, N: up to the largest tiles' sizes (both kernels of the last), ragged at the edges
+    (4000, 264, 1000, 264), (2049, 72, 4104, 40), (300, 1024, 16384, 64), (8200, 512, 512, 1024), (4104, 200, 4000, 520),
 ]
 
 
@@ -643,3 +643,30 @@ def test_embedding_gradient_of_long_runs_and_both_orders(T, n, V, D):
     mag = torch.zeros(V, D, dtype=F64).index_add_(0, ids, dy.to(F64).abs())
     count = torch.bincount(ids, minlength=V).to(F64)[:, None]
     close(dw, ref, (count + 2) * U * mag + B * ref.abs(), "gradient")
+
+
+@pytest.mark.parametrize("P,Q,K", [(692, 400, 1999), (131, 77, 700), (64, 300, 2600), (7, 5, 900), (200, 140, 9), (1030, 520, 130), (130, 3000, 5)])
+@pytest.mark.parametrize("modes", [(0, 0), (1, 0), (1, 1)])
+def test_tile_product(hip, stream, P, Q, K, modes):
+    """The gated block's plain products in every layout: odd strides and addresses, k split over the
+    grid or not, ragged ends of each direction."""
+    from xdna_train import hip_abi
+    print("tile product", P, Q, K, modes, flush=True)
+    g = gen(P + Q + K)
+    p, q = torch.randn(P, K, generator=g).bfloat16(), torch.randn(Q, K, generator=g).bfloat16()
+
+    def laid(t, rows, pad, offset):
+        m = t.t() if rows else t
+        buf = torch.full((m.shape[0] * (m.shape[1] + pad) + offset + 8,), 9.0, device="cuda", dtype=BF16)
+        v = torch.as_strided(buf, m.shape, (m.shape[1] + pad, 1), offset)
+        v.copy_(m)
+        return v, m.shape[1] + pad
+
+    pv, ldp = laid(p, modes[0], 3, 1)
+    qv, ldq = laid(q, modes[1], 2, 3)
+    out = torch.full((Q, P + 1), 5.0, device="cuda", dtype=BF16)
+    rc = hip.xdna_tile_mm_bf16(pv.data_ptr(), ldp, modes[0], qv.data_ptr(), ldq, modes[1], P, Q, K, out.data_ptr(), P + 1, stream)
+    assert rc == 0, hip_abi.last_error()
+    ref = q.to(F64) @ p.to(F64).t()
+    close(out[:, :P], ref, (K + 8) * U * (q.to(F64).abs() @ p.to(F64).abs().t()) + B * ref.abs() + 1e-30, "product")
+    assert (out[:, P].cpu() == 5.0).all(), "stored past a row's end"

@@ -106,3 +106,24 @@ def test_cpu_tensors_and_unknown_names_are_refused():
     for call in (lambda: tokens.gated_linear(x16, w16, activation="tanh"), lambda: tokens.distill_loss(z, y[:, None], z[:, :1], reduction="max")):
         with pytest.raises(ValueError, match="must be one of"):
             call()
+
+
+def test_gated_products_refuse_bad_arguments():
+    lib = hip_abi.load()
+
+    def mm(p=A, ldp=8, pr=0, q=A, ldq=8, qr=0, P=4, Q=4, K=8, out=A, ldc=4):
+        return lib.xdna_tile_mm_bf16(p, ldp, pr, q, ldq, qr, P, Q, K, out, ldc, None)
+
+    for kw, why in [({"p": None}, "null"), ({"q": None}, "null"), ({"out": None}, "null"), ({"K": 0}, "sizes"), ({"P": -1}, "sizes"),
+                    ({"Q": 1 << 23}, "sizes"), ({"pr": 2}, "contiguous"), ({"qr": 1}, "contiguous"), ({"ldp": 7}, "overlap"), ({"ldq": 7}, "overlap"),
+                    ({"ldc": 3}, "overlap"), ({"pr": 1, "ldp": 3}, "overlap"), ({"p": A + 1}, "misaligned")]:
+        assert refused(mm(**kw), why), (kw, hip_abi.last_error())
+    assert mm(P=0, p=None) == 0
+
+    def bwd(dy=A, ld=8, wo=A, ldw=4, gu=A, M=2, N=8, F=4, act=0, dgu=A):
+        return lib.xdna_gated_mlp_bwd_bf16(dy, ld, wo, ldw, gu, M, N, F, act, dgu, None)
+
+    for kw, why in [({"dy": None}, "null"), ({"wo": None}, "null"), ({"gu": None}, "null"), ({"dgu": None}, "null"), ({"ld": 7}, "overlap"),
+                    ({"ldw": 3}, "overlap"), ({"act": 4}, "activation"), ({"N": 0}, "sizes"), ({"dgu": A + 1}, "misaligned")]:
+        assert refused(bwd(**kw), why), (kw, hip_abi.last_error())
+    assert lib.xdna_gated_kept_bytes(3, 4) == 60 and lib.xdna_gated_kept_bytes(0, 4) == 0
