@@ -56,15 +56,17 @@ __device__ inline float2 act_pair(float g) {
 // Every wave multiplies a 64 x 64 block (2 x 2 MFMAs of 32x32x16: as many LDS reads as MFMAs):
 //   wide tiles, 128 x 128: four waves side by side, k-tiles of 64;
 //   narrow tiles, 64 x 64, where wide ones would leave CUs without work: eight waves on the
-// same block, each with its own k-step of a k-tile of 128 (an eighth of the k-tiles' memory
-// latencies of one wave), their accumulators added in wave order through LDS.  Where even they
-// leave CUs without work (weight gradients: short outputs, k as long as the batch), plain
-// products split k over the grid too, into fp32 partials that a second launch adds in order.
-// The next k-tile's loads fly in registers during a k-tile's MFMAs; one barrier per k-tile.
-// Addresses are formed once, per vector and not per k-tile; a row past the operand reads the last
-// one (its results are not stored), so that only the last k-tile and the vectors across a
-// row-contiguous operand's end are masked.  (Addresses and masks formed in every k-tile took more
-// VALU time than the MFMAs: 445 us for the block at 4895 x 448 x 1506, forward and backward.)
+// same block, each with half its columns and two k-steps of a k-tile of 128 (few k-tiles: each
+// costs a barrier), the four k parts added in wave order through LDS.  Where even they leave CUs
+// without work (weight gradients: short outputs, k as long as the batch), plain products split k
+// over the grid too, into fp32 partials that a second launch adds in order.
+// What bounds small products is the latency of the k-tiles' loads: two k-tiles fly in registers
+// while one is multiplied (one, with a k-step per wave and 64 more accumulators: 333 x 4096 -> 1367
+// units 38 us, now 26; three do not fit the registers of two workgroups a CU).  Large ones are
+// bounded by the LDS reads beside the MFMAs: 8192 x 512 x 2048 in wide tiles 27 us, 640 TFLOP/s.
+// One barrier per k-tile.  Addresses are formed once, per vector and not per k-tile, and only the
+// last k-tile is masked.  (Addresses and masks formed in every k-tile took more VALU time than the
+// MFMAs: 445 us for the block at 4895 x 448 x 1506, forward and backward.)
 enum TileEpi { kPlain = 0, kGated = 1, kGatedKeep = 2, kGatedGrad = 3 };
 
 struct TileOperand {
@@ -84,7 +86,36 @@ struct TileArgs {
   int vec;         // 8-byte accesses of out and gu: their addresses and strides are multiples of 4
   float* part;     // kPlain with k split over blockIdx.z: [split][q][p] partials, else null
   int k_split;     // k per split (whole k-tiles)
+  int nx, ny, group;  // the grid's tiles along p and along q, and the band of tile_at
 };
+
+// A workgroup's tile.  Workgroups go to the XCDs (each with its own L2) in turn: XCD c takes the
+// c-th eighth of the tiles in an order of splits, then bands of `group` tiles along q, within a
+// band q fastest.  The tiles an XCD works on together so form a near-square block of one split,
+// whose operands its L2 reads once; in launch order (p fastest) every XCD read all of both:
+// 333 x 1000 -> 1367 units 15.0 us and so 12.3, 333 x 2048 -> 1367 23.9 and 18.5.
+struct TileAt {
+  int x, y, z;
+};
+__device__ inline TileAt tile_at(const TileArgs& a) {
+  const int n = int(gridDim.x), c = int(blockIdx.x) % kGemmXcds, i = int(blockIdx.x) / kGemmXcds;
+  const int t = c * (n / kGemmXcds) + min(c, n % kGemmXcds) + i;
+  const int plane = a.nx * a.ny, z = t / plane, r = t - z * plane;
+  const int band = r / (a.group * a.nx), in = r - band * a.group * a.nx;
+  const int high = min(a.group, a.ny - band * a.group);
+  return {in / high, band * a.group + in % high, z};
+}
+
+// nx x ny tiles in `splits` splits as a grid of tile_at, `together` tiles at work on an XCD
+int64_t plan_tiles(TileArgs& a, int64_t nx, int64_t ny, int64_t splits, int together) {
+  a.nx = int(nx);
+  a.ny = int(ny);
+  const int64_t n = std::min({ceil_div(nx * ny * splits, int64_t(kGemmXcds)), nx * ny, int64_t(together)});
+  int g = 1;
+  while (g < ny && int64_t(g) * g < n) ++g;
+  a.group = g;
+  return nx * ny * splits;
+}
 
 __device__ inline Pix8 row_vec(const uint16_t* p, int n) {  // n elements, zeros after them
   if (n >= 8) return *reinterpret_cast<const Pix8*>(p);
@@ -108,13 +139,6 @@ __device__ inline Pix8 shifted(Pix8 q, int s) {
   return q;
 }
 
-// row_vec where the 8 - n elements before p can be read: the 16 bytes that end with element n - 1
-__device__ inline Pix8 end_vec(const uint16_t* p, int n) {
-  if (n <= 0) return {{0u, 0u, 0u, 0u}};
-  const int s = 8 - min(n, 8);
-  return shifted(*reinterpret_cast<const Pix8*>(p - s), s);
-}
-
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 
@@ -124,6 +148,8 @@ struct Tile {
   static constexpr int KT = WIDE ? 64 : 128;       // k per k-tile
   static constexpr int NT = WIDE ? 256 : 512;      // threads
   static constexpr int V = T * KT / 8 / NT;        // 16-byte vectors per thread and operand
+  static constexpr int NJ = WIDE ? 2 : 1;          // a wave's block: 64 x 32 NJ
+  static constexpr int KS = WIDE ? 4 : 2;          // k-steps of a wave per k-tile
   static constexpr int PITCH = KT + 8;             // elements of a k-contiguous LDS row
   static constexpr int ELEMS = T * PITCH;          // (a [k][row] tile is smaller)
   static constexpr size_t LDS = size_t(2) * 2 * ELEMS * 2;
@@ -138,26 +164,25 @@ __device__ inline int64_t tile_row(const TileArgs& a, const TileOperand& o, int 
 }
 
 // One operand's loads: per thread V vectors of 16 bytes of a k-tile, vector j at from[j] + t step,
-// its k offset in the k-tile kq[j].  A row-contiguous vector across the operand's end is read from
-// 8 elements before the end and shifted when it is stored (a shift, or a masked load, where it is
-// read would wait for it there, and the ragged tiles would take several times the others' time).
+// its k offset in the k-tile kq[j].  Every load is whole and none hangs on a branch, so that waiting
+// for one k-tile leaves the younger ones in flight.  Results of rows past the operand are not
+// stored, so what they multiply does not matter: a vector across a row-contiguous operand's end
+// reads on into the next k row.  Only the last k-tile (LAST) needs care: vectors past the end of k
+// read the last elements (the last k row) instead and are shifted (cleared) before they are stored,
+// and so is a vector across the end of the last k row.
 template <bool WIDE, bool ROWS, bool GATED>
 struct TileLoads {
   using C = Tile<WIDE>;
   const uint16_t* from[C::V];
-  int64_t step;  // elements between k-tiles
+  int64_t ld;
   int kq[C::V];
-  int shift;     // row-contiguous: elements before the first one
-  bool inside;   // all the tile's rows are the operand's
-  bool run;      // 8 elements along the contiguous direction exist
-  int n;         // row-contiguous: rows from the vector's first on (below 1: none)
+  int over;  // row-contiguous: elements of the vectors past the operand's rows
+  bool run;  // 8 elements along the contiguous direction exist
 
   __device__ inline void plan(const TileArgs& a, const TileOperand& o, int r0, int kbeg, int tid) {
-    step = ROWS ? C::KT * o.ld : C::KT;
-    inside = !ROWS || r0 + C::T <= o.rows;
+    ld = o.ld;
     run = (ROWS ? o.rows : a.K) >= 8;
-    shift = 0;
-    n = 8;
+    over = 0;
 #pragma unroll
     for (int j = 0; j < C::V; ++j) {
       const int i = tid + j * C::NT;
@@ -165,40 +190,47 @@ struct TileLoads {
         kq[j] = i % (C::KT / 8) * 8;
         from[j] = o.src + tile_row<GATED>(a, o, r0, i / (C::KT / 8)) * o.ld + kbeg + kq[j];
       } else {  // (NT is a multiple of the vectors along the rows: the same rows for every j)
-        const int r = r0 + i % (C::T / 8) * 8, first = max(min(r, o.rows - 8), 0);
+        int r = r0 + i % (C::T / 8) * 8;
         kq[j] = i / (C::T / 8);
-        n = o.rows - r;
-        shift = run ? min(r - first, 7) : 0;  // (rows past the end: anything)
-        from[j] = o.src + int64_t(kbeg + kq[j]) * o.ld + first;
+        over = max(r + 8 - o.rows, 0);
+        if (r >= o.rows) r = run ? o.rows - 8 : 0, over = run ? 0 : 8;
+        from[j] = o.src + int64_t(kbeg + kq[j]) * o.ld + r;
       }
     }
   }
 
-  // the k-tile `t`: `left` is what k has from its start on
+  // The k-tile `t`: `left` is what k has from its start on.
+  template <bool LAST>
   __device__ inline void load(Pix8 (&v)[C::V], int t, int left) const {
-    if (left >= C::KT && run) {
-#pragma unroll
-      for (int j = 0; j < C::V; ++j) v[j] = *reinterpret_cast<const Pix8*>(from[j] + t * step);
-      return;
-    }
 #pragma unroll
     for (int j = 0; j < C::V; ++j) {
-      // (from[j] + t step is not formed for a vector that is not read)
-      if constexpr (ROWS) {
-        const bool in = kq[j] < left;
-        v[j] = row_vec(in ? from[j] + t * step : from[j], in ? (run ? 8 : n) : 0);
-      } else {
-        const int got = left - kq[j];
-        const uint16_t* p = got > 0 ? from[j] + t * step : from[j];
-        v[j] = run ? end_vec(p, got) : row_vec(p, got);
+      const uint16_t* p = from[j] + t * (ROWS ? C::KT * ld : int64_t(C::KT));
+      if (LAST && left <= C::KT) {
+        if (!ROWS) p -= max(kq[j] + 8 - left, 0);
+        else if (kq[j] >= left - 1) p -= int64_t(kq[j] - left + 1) * ld + over;
       }
+      v[j] = *reinterpret_cast<const Pix8*>(p);
     }
   }
 
-  __device__ inline void align(Pix8 (&v)[C::V]) const {
-    if (!ROWS || inside) return;
+  __device__ inline void align(Pix8 (&v)[C::V], int left) const {
+    if (left > C::KT) return;
 #pragma unroll
-    for (int j = 0; j < C::V; ++j) v[j] = shifted(v[j], shift);
+    for (int j = 0; j < C::V; ++j) {
+      const int past = kq[j] + (ROWS ? 1 : 8) - left;
+      if (past >= (ROWS ? 1 : 8)) v[j] = {{0u, 0u, 0u, 0u}};
+      else if (past >= 0) v[j] = shifted(v[j], ROWS ? over : past);
+    }
+  }
+
+  // load() and align() where an operand has fewer than 8 elements along its contiguous direction
+  __device__ inline void load_short(Pix8 (&v)[C::V], int t, int left) const {
+#pragma unroll
+    for (int j = 0; j < C::V; ++j) {
+      const bool in = kq[j] < left;  // (no address is formed for a vector that is not read)
+      const uint16_t* p = in ? from[j] + t * (ROWS ? C::KT * ld : int64_t(C::KT)) : from[j];
+      v[j] = row_vec(p, !in ? 0 : ROWS ? 8 - over : left - kq[j]);
+    }
   }
 };
 
@@ -433,10 +465,10 @@ __device__ inline void grad8(const float (&d)[8], const Pix8& g, const Pix8& u, 
 // 8 consecutive outputs of row q from column `at` on (n of them in range): d0, and for the gated
 // forward the up projection d1
 template <int EPI, int ACT>
-__device__ inline void put_row8(const TileArgs& a, int q, int at, int n, const float (&d0)[8], const float (&d1)[8]) {
+__device__ inline void put_row8(const TileArgs& a, int q, int at, int n, const float (&d0)[8], const float (&d1)[8], int split) {
   if constexpr (EPI == kPlain) {
     if (a.part) {
-      float* to = a.part + (int64_t(blockIdx.z) * a.q.rows + q) * a.p.rows + at;
+      float* to = a.part + (int64_t(split) * a.q.rows + q) * a.p.rows + at;
       if (n >= 8) {
         *reinterpret_cast<Floats4*>(to) = {{d0[0], d0[1], d0[2], d0[3]}};
         *reinterpret_cast<Floats4*>(to + 4) = {{d0[4], d0[5], d0[6], d0[7]}};
@@ -472,57 +504,89 @@ __global__ __launch_bounds__(Tile<WIDE>::NT, WIDE ? 2 : 4) void tile_kernel(Tile
   constexpr bool GATED = EPI == kGated || EPI == kGatedKeep;
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];  // [2 buffers][P, Q]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wp = WIDE ? wave & 1 : 0, wq = WIDE ? wave >> 1 : 0;
-  const int p0 = blockIdx.x * C::T, q0 = blockIdx.y * C::T;
-  f32x16_t acc[2][2];
+  const int wp = WIDE ? wave & 1 : 0, wq = WIDE ? wave >> 1 : wave & 1, wk = WIDE ? 0 : wave >> 1;
+  const TileAt tile = tile_at(a);
+  const int p0 = tile.x * C::T, q0 = tile.y * C::T;
+  f32x16_t acc[2][C::NJ];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = zero_acc();
-  const int kbeg = EPI == kPlain && a.part ? int(blockIdx.z) * a.k_split : 0;
-  const int kend = EPI == kPlain && a.part ? min(a.K, kbeg + a.k_split) : a.K;
+    for (int j = 0; j < C::NJ; ++j) acc[i][j] = zero_acc();
+  const int kbeg = EPI == kPlain && a.part ? tile.z * a.k_split : 0;
+  const int klen = (EPI == kPlain && a.part ? min(a.K, kbeg + a.k_split) : a.K) - kbeg;
   TileLoads<WIDE, PROWS, GATED> lp;
   TileLoads<WIDE, QROWS, false> lq;
   lp.plan(a, a.p, p0, kbeg, tid);
   lq.plan(a, a.q, q0, kbeg, tid);
-  Pix8 rp[C::V], rq[C::V];
-  lp.load(rp, 0, kend - kbeg);
-  lq.load(rq, 0, kend - kbeg);
-  lp.align(rp);
-  lq.align(rq);
-  tile_store<WIDE, PROWS>(smem, rp, tid);
-  tile_store<WIDE, QROWS>(smem + C::ELEMS, rq, tid);
-  __syncthreads();
-  const int tiles = (kend - kbeg + C::KT - 1) / C::KT;
-  for (int t = 0; t < tiles; ++t) {
-    const bool more = t + 1 < tiles;
-    const int b = t & 1;
-    if (more) {
-      lp.load(rp, t + 1, kend - kbeg - (t + 1) * C::KT);
-      lq.load(rq, t + 1, kend - kbeg - (t + 1) * C::KT);
-    }
+  const int tiles = (klen + C::KT - 1) / C::KT;
+  const auto put = [&](const Pix8 (&rp)[C::V], const Pix8 (&rq)[C::V], int b) {
+    uint16_t* to = smem + b * 2 * C::ELEMS;
+    tile_store<WIDE, PROWS>(to, rp, tid);
+    tile_store<WIDE, QROWS>(to + C::ELEMS, rq, tid);
+  };
+  const auto multiply = [&](int b) {
     const uint16_t* ps = smem + b * 2 * C::ELEMS;
     const uint16_t* qs = ps + C::ELEMS;
 #pragma unroll
-    for (int s = 0; s < (WIDE ? 4 : 1); ++s) {
-      const int ks = WIDE ? s : wave;
-      bf16x8_t fp[2], fq[2];
+    for (int s = 0; s < C::KS; ++s) {
+      const int ks = wk * C::KS + s;
+      bf16x8_t fp[2], fq[C::NJ];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fp[i] = tile_frag<WIDE, PROWS>(ps, wp * 64 + i * 32, ks, lane);
-        fq[i] = tile_frag<WIDE, QROWS>(qs, wq * 64 + i * 32, ks, lane);
-      }
+      for (int i = 0; i < 2; ++i) fp[i] = tile_frag<WIDE, PROWS>(ps, wp * 64 + i * 32, ks, lane);
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j) fq[j] = tile_frag<WIDE, QROWS>(qs, (wq * C::NJ + j) * 32, ks, lane);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma_32x32x16(fp[i], fq[j], acc[i][j]);
+        for (int j = 0; j < C::NJ; ++j) acc[i][j] = mfma_32x32x16(fp[i], fq[j], acc[i][j]);
     }
-    if (more) {  // the other buffer's last reads ended before the previous barrier
-      uint16_t* to = smem + (b ^ 1) * 2 * C::ELEMS;
-      lp.align(rp);
-      lq.align(rq);
-      tile_store<WIDE, PROWS>(to, rp, tid);
-      tile_store<WIDE, QROWS>(to + C::ELEMS, rq, tid);
+  };
+  if (lp.run && lq.run) {
+    Pix8 rp[2][C::V], rq[2][C::V];  // k-tile t's loads in set t % 2, its LDS buffer too
+    const auto load = [&](int set, int t) {
+      lp.template load<false>(rp[set], t, 0);
+      lq.template load<false>(rq[set], t, 0);
+    };
+    const auto load_end = [&](int set, int t) {
+      lp.template load<true>(rp[set], t, a.K - kbeg - t * C::KT);
+      lq.template load<true>(rq[set], t, a.K - kbeg - t * C::KT);
+    };
+    const auto put_end = [&](int set, int t) {
+      lp.align(rp[set], a.K - kbeg - t * C::KT);
+      lq.align(rq[set], a.K - kbeg - t * C::KT);
+      put(rp[set], rq[set], set);
+    };
+    load_end(0, 0);
+    if (tiles > 1) load_end(1, 1);
+    put_end(0, 0);
+    __syncthreads();
+    int t = 0;
+    for (; t + 4 < tiles; t += 2) {  // (neither loads nor stores the last k-tile)
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        load(d, t + d + 2);
+        multiply(d);
+        put(rp[d ^ 1], rq[d ^ 1], d ^ 1);  // that buffer's last reads ended before the previous barrier
+        __syncthreads();
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      if (t + d < tiles) {
+        if (d < 2 && t + d + 2 < tiles) load_end(d, t + d + 2);
+        multiply(d & 1);
+        if (t + d + 1 < tiles) put_end((d + 1) & 1, t + d + 1);
+        __syncthreads();
+      }
+    }
+  } else {
+    for (int t = 0; t < tiles; ++t) {
+      Pix8 rp[C::V], rq[C::V];
+      lp.load_short(rp, t, a.K - kbeg - t * C::KT);
+      lq.load_short(rq, t, a.K - kbeg - t * C::KT);
+      put(rp, rq, t & 1);
+      __syncthreads();
+      multiply(t & 1);
     }
     __syncthreads();
   }
@@ -540,31 +604,31 @@ __global__ __launch_bounds__(Tile<WIDE>::NT, WIDE ? 2 : 4) void tile_kernel(Tile
           *reinterpret_cast<float4*>(block + (wq * 64 + j * 32 + (lane & 31)) * EP + wp * 64 + i * 32 + 8 * g + 4 * (lane >> 5)) =
               make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
   } else {
-    // two rounds (j): the eight waves' quads [wave][i][g][lane] in 64 KB, summed by a thread per
-    // (i, g, lane)
+    // the eight waves' quads [wave][i][g][lane] in 64 KB, the four k parts of each summed by a
+    // thread per (q half, g, lane) of both i
     float4* red = reinterpret_cast<float4*>(smem);
-    const int g = wave & 3, i = wave >> 2;
+    const int g = wave & 3, half = wave >> 2;
     float4 sum[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int y = 0; y < 4; ++y)
+        red[((wave * 2 + x) * 4 + y) * 64 + lane] =
+            make_float4(acc[x][0][4 * y], acc[x][0][4 * y + 1], acc[x][0][4 * y + 2], acc[x][0][4 * y + 3]);
+    __syncthreads();
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-          red[((wave * 2 + x) * 4 + y) * 64 + lane] =
-              make_float4(acc[x][j][4 * y], acc[x][j][4 * y + 1], acc[x][j][4 * y + 2], acc[x][j][4 * y + 3]);
-      __syncthreads();
-      sum[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < 2; ++i) {
+      sum[i] = red[((half * 2 + i) * 4 + g) * 64 + lane];
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const float4 v = red[((w * 2 + i) * 4 + g) * 64 + lane];
-        sum[j].x += v.x, sum[j].y += v.y, sum[j].z += v.z, sum[j].w += v.w;
+      for (int w = 1; w < 4; ++w) {
+        const float4 v = red[(((w * 2 + half) * 2 + i) * 4 + g) * 64 + lane];
+        sum[i].x += v.x, sum[i].y += v.y, sum[i].z += v.z, sum[i].w += v.w;
       }
-      __syncthreads();
     }
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      *reinterpret_cast<float4*>(block + (j * 32 + (lane & 31)) * EP + i * 32 + 8 * g + 4 * (lane >> 5)) = sum[j];
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<float4*>(block + (half * 32 + (lane & 31)) * EP + i * 32 + 8 * g + 4 * (lane >> 5)) = sum[i];
   }
   __syncthreads();
   // rows in windows of 8 outputs, consecutive threads along a row
@@ -579,7 +643,7 @@ __global__ __launch_bounds__(Tile<WIDE>::NT, WIDE ? 2 : 4) void tile_kernel(Tile
     float d0[8], d1[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) d0[e] = from[r * EP + e], d1[e] = GATED ? from[r * EP + 32 + e] : 0.0f;
-    put_row8<EPI, ACT>(a, q0 + r, at, n, d0, d1);
+    put_row8<EPI, ACT>(a, q0 + r, at, n, d0, d1, tile.z);
   }
 }
 
@@ -757,14 +821,13 @@ constexpr size_t kLargeLds = std::max(kGemm5Lds, size_t(kEpiRows) * kEpiPitch * 
 
 template <bool PROWS, int EPI, int ACT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void gated_large_kernel(TileArgs a, int xcd_group) {
+void gated_large_kernel(TileArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   constexpr bool GATED = EPI != kGatedGrad;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave & 1, wn = wave >> 1;
-  int tp, tq;
-  xcd_tile_xy(xcd_group, tp, tq);
-  const int f0 = tp * (GATED ? kT4 / 2 : kT4), q0 = tq * kT4;
+  const TileAt tile = tile_at(a);
+  const int f0 = tile.x * (GATED ? kT4 / 2 : kT4), q0 = tile.y * kT4;
   f32x4_t acc[8][8];
   {
     G5Operand op;
@@ -798,7 +861,7 @@ void gated_large_kernel(TileArgs a, int xcd_group) {
         float g[8], u[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[e] = at[r * kEpiPitch + e], u[e] = at[r * kEpiPitch + 16 + e];
-        if (row(r) < a.q.rows && f < a.F) put_row8<EPI, ACT>(a, row(r), f, 8, g, u);
+        if (row(r) < a.q.rows && f < a.F) put_row8<EPI, ACT>(a, row(r), f, 8, g, u, 0);
       }
     } else {
       // four rows' [g u] in flight: clamped addresses, no branch around the loads
@@ -862,23 +925,27 @@ int refuse(const char* what, const char* why) {
 }
 
 constexpr int64_t kMaxSide = int64_t(1) << 30;
+constexpr int64_t kMaxRows = int64_t(1) << 22;  // of x
+constexpr int64_t kMaxOutputs = int64_t(1) << 42;  // (2^28 wide tiles: a grid has under 2^31)
 
 const char* gated_fault(int64_t M, int64_t K, int64_t F, int act) {
   if (act < 0 || act > 2) return "activation must be 0 (silu), 1 (gelu) or 2 (relu)";
   if (M < 0 || M > kMaxSide || K < 1 || K > kMaxSide || F < 1 || F > kMaxSide / 2) return "sizes outside 1 .. 2^30";
+  if (M > kMaxRows) return "too many rows";
+  if (M * F > kMaxOutputs) return "too many outputs";
   return nullptr;
 }
 
 bool odd(const void* p) { return reinterpret_cast<uintptr_t>(p) & 1; }
 
 template <bool WIDE, bool PROWS, bool QROWS, int EPI, int ACT>
-bool launch_tile(const TileArgs& a, dim3 grid, hipStream_t st) {
+bool launch_tile(TileArgs a, dim3 tiles, hipStream_t st) {
   using C = Tile<WIDE>;
   void (*f)(TileArgs) = tile_kernel<WIDE, PROWS, QROWS, EPI, ACT>;
   static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize,
                                              int(C::LDS)) == hipSuccess;
   if (!ok) return false;
-  f<<<grid, C::NT, C::LDS, st>>>(a);
+  f<<<unsigned(plan_tiles(a, tiles.x, tiles.y, tiles.z, 64)), C::NT, C::LDS, st>>>(a);
   return true;
 }
 
@@ -898,24 +965,37 @@ bool launch_few(TileArgs a, hipStream_t st) {
 
 // k split over the grid into `splits` parts, joined by a second launch
 template <bool WIDE, bool PROWS, bool QROWS>
-bool launch_split(TileArgs a, dim3 grid, int64_t splits, hipStream_t st) {
+bool launch_split(TileArgs a, dim3 tiles, int64_t splits, hipStream_t st) {
   constexpr int kt = Tile<WIDE>::KT;
   a.k_split = int(ceil_div(ceil_div(a.K, kt), splits)) * kt;
-  grid.z = unsigned(ceil_div(a.K, a.k_split));
+  tiles.z = unsigned(ceil_div(a.K, a.k_split));
   const int64_t n = int64_t(a.p.rows) * a.q.rows;
-  a.part = static_cast<float*>(xdna_hip_cache_alloc(size_t(grid.z) * size_t(n) * sizeof(float)));
+  a.part = static_cast<float*>(xdna_hip_cache_alloc(size_t(tiles.z) * size_t(n) * sizeof(float)));
   if (!a.part) return false;
-  const bool ok = launch_tile<WIDE, PROWS, QROWS, kPlain, kSilu>(a, grid, st);
-  if (ok) tile_join_kernel<<<unsigned(std::min<int64_t>(ceil_div(n, int64_t(1024)), 4096)), 256, 0, st>>>(a, int(grid.z));
+  const bool ok = launch_tile<WIDE, PROWS, QROWS, kPlain, kSilu>(a, tiles, st);
+  if (ok) tile_join_kernel<<<unsigned(std::min<int64_t>(ceil_div(n, int64_t(1024)), 4096)), 256, 0, st>>>(a, int(tiles.z));
   xdna_hip_cache_free(a.part);  // stream-ordered reuse: the block's next user runs after the join
   return ok;
 }
 
-// Wide tiles where they give every CU one, with k split over the grid (plain products: towards
-// two a CU, six k-tiles a split or more, twelve where the tiles alone come near) where that gives
-// half the CUs one; else narrow tiles, split towards two a CU with two k-tiles a split or more.
-// Measured, p x q x k: 218 x 5893 x 5632 wide and split 47 us, narrow 74; 960 x 495 x 2832 21.6
-// and 27.0; 692 x 3972 x 998 36.1 and 28.5 (16 k-tiles, 192 wide tiles).
+// What a product in tiles takes in us, `kt` k-tiles each: the grid in rounds of two tiles a CU,
+// its last round alone on the CUs if it has no more tiles than they are.  Fitted to 100 products
+// (64 .. 6000 x 64 .. 6000, k 100 .. 8000, all three layouts, either tile, k in 1 to 16 splits):
+// 9 % off in the mean, and the choice by it 0.6 % off the best of each.
+float tile_cost(bool wide, int64_t tiles, int64_t kt) {
+  const float alone = wide ? 0.65f : 0.54f, paired = wide ? 1.2f : 1.1f;
+  const int64_t full = (tiles - 1) / 512, rest = tiles - full * 512;
+  return float(full) * (paired * float(kt) + (wide ? 1.1f : 2.75f)) + (rest <= 256 ? alone : paired) * float(kt) + (wide ? 6.5f : 4.6f);
+}
+
+// The same with k split: fp32 partials written and read, and the join's launch.
+float split_cost(bool wide, int64_t tiles, int64_t kt, int64_t splits, int64_t outputs) {
+  return tile_cost(wide, tiles * splits, ceil_div(kt, splits)) + 3.3f + float(outputs) * (float(splits) * 1.8e-6f + 0.4e-6f);
+}
+
+// Tiles and splits by the costs above.  Measured, p x q x k, one of each outcome: 500 x 4001 x 700
+// narrow 10.0 us (wide 12.8, wide in two splits 25.0); 500 x 6002 x 700 wide 16.3 (narrow 20.1);
+// 1024 x 512 x 8192 narrow in four splits 26.1 (whole 36.6).
 template <bool PROWS, bool QROWS, int EPI, int ACT>
 bool launch_tiles(const TileArgs& a, hipStream_t st) {
   constexpr int side = EPI == kGated || EPI == kGatedKeep ? 2 : 1;  // tile rows per unit of p
@@ -932,18 +1012,29 @@ bool launch_tiles(const TileArgs& a, hipStream_t st) {
       if (a.q.rows <= kFewGated) return launch_few<4, 1, EPI, ACT>(a, st);
     }
   }
-  const dim3 wide = tiles(128), narrow = tiles(64);
-  const int64_t wides = int64_t(wide.x) * wide.y, narrows = int64_t(narrow.x) * narrow.y;
-  if constexpr (EPI == kPlain) {
-    const int64_t split = std::min(512 / wides, ceil_div(a.K, Tile<true>::KT) / (wides < 160 ? 6 : 12));
-    if (split > 1 && wides * split >= 128) return launch_split<true, PROWS, QROWS>(a, wide, split, st);
+  bool use_wide = false;
+  int64_t use_splits = 1;
+  float best = INFINITY;
+  for (const bool wide : {false, true}) {
+    const dim3 t = tiles(wide ? 128 : 64);
+    const int64_t n = int64_t(t.x) * t.y, kt = ceil_div(a.K, wide ? Tile<true>::KT : Tile<false>::KT);
+    const float whole = tile_cost(wide, n, kt);
+    if (whole < best) best = whole, use_wide = wide, use_splits = 1;
+    if constexpr (EPI == kPlain) {
+      const int64_t outputs = int64_t(a.p.rows) * a.q.rows;
+      for (const int64_t s : {2, 3, 4, 6, 8, 12, 16}) {
+        if (2 * s > kt || n * s > 1024) break;
+        const float cost = split_cost(wide, n, kt, s, outputs);
+        if (cost < best) best = cost, use_wide = wide, use_splits = s;
+      }
+    }
   }
-  if (wides >= 256 || narrow.y > 65535) return launch_tile<true, PROWS, QROWS, EPI, ACT>(a, wide, st);
+  const dim3 t = tiles(use_wide ? 128 : 64);
   if constexpr (EPI == kPlain) {
-    const int64_t split = std::min(ceil_div(512, narrows), ceil_div(a.K, Tile<false>::KT) / 2);
-    if (split > 1) return launch_split<false, PROWS, QROWS>(a, narrow, split, st);
+    if (use_splits > 1)
+      return use_wide ? launch_split<true, PROWS, QROWS>(a, t, use_splits, st) : launch_split<false, PROWS, QROWS>(a, t, use_splits, st);
   }
-  return launch_tile<false, PROWS, QROWS, EPI, ACT>(a, narrow, st);
+  return use_wide ? launch_tile<true, PROWS, QROWS, EPI, ACT>(a, t, st) : launch_tile<false, PROWS, QROWS, EPI, ACT>(a, t, st);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -957,23 +1048,25 @@ bool dma_ok(const TileOperand& o, int64_t rows, int64_t K, bool along_rows) {
 }
 
 template <bool PROWS, int EPI, int ACT>
-bool launch_large(const TileArgs& a, dim3 grid, hipStream_t st) {
-  void (*f)(TileArgs, int) = gated_large_kernel<PROWS, EPI, ACT>;
+bool launch_large(TileArgs a, dim3 tiles, hipStream_t st) {
+  void (*f)(TileArgs) = gated_large_kernel<PROWS, EPI, ACT>;
   static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize,
                                              int(kLargeLds)) == hipSuccess;
   if (!ok) return false;
-  const int group = int64_t(grid.x) * grid.y % kGemmXcds == 0 ? int(std::min(grid.y, 8u)) : 0;
-  f<<<grid, 256, kLargeLds, st>>>(a, group);
+  f<<<unsigned(plan_tiles(a, tiles.x, tiles.y, 1, 32)), 256, kLargeLds, st>>>(a);
   return true;
 }
 
-// Large tiles where they give every CU one (8192 x 512 -> 1024 units: 256 tiles 27 us, against 38
-// in wide tiles; with 128 tiles the wide ones are ahead: 28 against 37 for the gradient there).
+// Large tiles where they give every CU one and fill the rounds that they take.  Measured, large
+// and wide tiles in us: 8192 x 512 -> 1024 units (256 tiles) 27 and 34, 8192 x 1024 -> 4096 158 and
+// 192; but 8192 x 512 -> 1024's gradient (128 tiles) 37 and 27, 4800 x 1024 -> 2048 (1.2 rounds) 64
+// and 57.
 template <int EPI, bool PROWS, int ACT>
 bool launch_sized(const TileArgs& a, hipStream_t st) {
   constexpr bool GATED = EPI != kGatedGrad;
   const dim3 grid(unsigned(ceil_div(a.F, GATED ? kT4 / 2 : kT4)), unsigned(ceil_div(a.q.rows, kT4)));
-  const bool large = int64_t(grid.x) * grid.y >= 256 && a.K % 8 == 0 && a.F % 8 == 0 && aligned16(a.out) && aligned16(a.gu) &&
+  const int64_t n = int64_t(grid.x) * grid.y;
+  const bool large = n >= 256 && 100 * n >= 65 * 256 * ceil_div(n, int64_t(256)) && a.K % 8 == 0 && a.F % 8 == 0 && aligned16(a.out) && aligned16(a.gu) &&
                      dma_ok(a.p, GATED ? 2 * int64_t(a.F) : a.F, a.K, PROWS) && dma_ok(a.q, a.q.rows, a.K, false);
   return large ? launch_large<PROWS, EPI, ACT>(a, grid, st) : launch_tiles<PROWS, false, EPI, ACT>(a, st);
 }
@@ -1017,7 +1110,6 @@ int xdna_gated_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t l
   const char* what = "xdna_gated_bf16";
   if (const char* why = gated_fault(M, K, F, act)) return refuse(what, why);
   if ((ldx < K && M > 1) || ldw < K) return refuse(what, "rows overlap");
-  if (ceil_div(M, int64_t(64)) > 65535) return refuse(what, "too many rows");
   if (M == 0) return 0;
   if (!x || !w || !h) return refuse(what, "null operand");
   if (odd(x) || odd(w) || odd(h) || odd(gu)) return refuse(what, "misaligned operand");
@@ -1036,7 +1128,6 @@ int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_
   const char* what = "xdna_gated_mlp_bwd_bf16";
   if (const char* why = gated_fault(M, N, F, act)) return refuse(what, why);
   if ((lddy < N && M > 1) || (ldw < F && N > 1)) return refuse(what, "rows overlap");
-  if (ceil_div(M, int64_t(64)) > 65535) return refuse(what, "too many rows");
   if (M == 0) return 0;
   if (!dy || !w_out || !gu || !dgu) return refuse(what, "null operand");
   if (odd(dy) || odd(w_out) || odd(gu) || odd(dgu)) return refuse(what, "misaligned operand");
@@ -1052,7 +1143,8 @@ int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_
 int xdna_tile_mm_bf16(const uint16_t* p, int64_t ldp, int p_rows, const uint16_t* q, int64_t ldq, int q_rows, int64_t P,
                       int64_t Q, int64_t K, uint16_t* out, int64_t ldc, void* stream) {
   const char* what = "xdna_tile_mm_bf16";
-  if (P < 0 || P > kMaxSide || Q < 0 || Q > int64_t(65535) * 64 || K < 1 || K > kMaxSide) return refuse(what, "sizes out of range");
+  if (P < 0 || P > kMaxSide || Q < 0 || Q > kMaxSide || K < 1 || K > kMaxSide || P * Q > kMaxOutputs)
+    return refuse(what, "sizes out of range");
   if ((p_rows != 0 && p_rows != 1) || (q_rows != 0 && q_rows != 1) || (q_rows && !p_rows))
     return refuse(what, "operands are k-contiguous (0) or row-contiguous (1), q only beside such a p");
   if (ldp < (p_rows ? P : K) || ldq < (q_rows ? Q : K) || ldc < P) return refuse(what, "rows overlap");

@@ -69,17 +69,22 @@ bool vector_rows(const at::Tensor& t) {
   return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 && ld % 8 == 0;
 }
 
-// a b of two bf16 matrices, each contiguous along one dimension: large products of operands that
-// the library's 256 x 256 tiles can load take those, others the gated block's own tiles (512 x
-// 8192 x 2048: 41 and 51 us; 1024 x 4096 x 1024: 35 and 28; 960 x 2832 x 495: 43 and 14).
+// a b of two bf16 matrices, each contiguous along one dimension: on the framework's GEMM where its
+// 256 x 256 tiles can load them and fill the CUs (or do with k split evenly) for long enough, else
+// on the gated block's own tiles.  Measured (rows x columns x k, GEMM and own tiles in us): 8192 x
+// 2048 x 4096 110 and 147, 4096 x 4096 x 1024 36 and 44, 8192 x 1024 x 8192 132 and 174; but 4800 x
+// 4096 x 2048 (1.2 rounds of the CUs) 100 and 95, 8192 x 768 x 6144 (96 tiles) 121 and 105, 4096 x
+// 1024 x 4096 55 and 46, 8192 x 1024 x 2048 51 and 42, 6424 x 896 x 1024 44 and 23.
 at::Tensor product(const at::Tensor& a, const at::Tensor& b) {
   const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
   at::Tensor c = empty_xdna({M, N}, at::kBFloat16);
   const bool b_rows = b.stride(1) == 1 && K > 1, a_rows = a.stride(0) == 1 && M > 1 && a.stride(1) != 1;
   const bool a_ok = a_rows ? b_rows : a.stride(1) == 1 || K == 1, b_ok = b_rows || b.stride(0) == 1 || K == 1;
   const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
-  const bool large = vector_rows(a) && vector_rows(b) && K % 8 == 0 && K >= 1024 && tiles >= 64 && K * tiles >= 131072;
-  if (K > 0 && !large && a_ok && b_ok && M <= int64_t(65535) * 64) {
+  const bool fills = tiles >= 192 && 100 * tiles >= 65 * 256 * ((tiles + 255) / 256) && K * tiles >= 262144;
+  const bool splits = (tiles == 64 || tiles == 128) && K * tiles >= 524288;
+  const bool large = vector_rows(a) && vector_rows(b) && K % 8 == 0 && K >= 1024 && (fills || splits);
+  if (K > 0 && !large && a_ok && b_ok) {
     const int64_t lda = a_rows ? a.stride(1) : M > 1 ? a.stride(0) : K, ldb = b_rows ? b.stride(0) : N > 1 ? b.stride(1) : K;
     check_abi(xdna_tile_mm_bf16(p16(b), ldb, b_rows ? 1 : 0, p16(a), lda, a_rows ? 1 : 0, N, M, K, m16(c), N,
                                 current_stream()),
