@@ -845,8 +845,9 @@ int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_
 
 /* out[q * ldc + p] = sum over k of P[p][k] Q[q][k], for operands of any alignment and row stride:
  * contiguous along k (p_rows / q_rows 0: element (r, k) at r * ld + k) or along the rows (1: at
- * k * ld + r; q only where p is too).  The products of the gated block whose sizes the large
- * tiles of xdna_gemm_bf16 cannot load as vectors. */
+ * k * ld + r; q only where p is too).  The gated block's products that xdna_gemm_bf16's large
+ * tiles cannot load as vectors or do not fill the chip with.  Q up to 2^22.  Where k is split, the
+ * fp32 partials come from the library's caching allocator (-1 if it has no memory). */
 int xdna_tile_mm_bf16(const uint16_t* p, int64_t ldp, int p_rows, const uint16_t* q, int64_t ldq, int q_rows, int64_t P,
                       int64_t Q, int64_t K, uint16_t* out, int64_t ldc, void* stream);
 

@@ -925,7 +925,7 @@ int refuse(const char* what, const char* why) {
 }
 
 constexpr int64_t kMaxSide = int64_t(1) << 30;
-constexpr int64_t kMaxRows = int64_t(1) << 22;  // of x
+constexpr int64_t kMaxRows = int64_t(1) << 22;  // of x; of a plain product's second operand
 constexpr int64_t kMaxOutputs = int64_t(1) << 42;  // (2^28 wide tiles: a grid has under 2^31)
 
 const char* gated_fault(int64_t M, int64_t K, int64_t F, int act) {
@@ -1143,7 +1143,7 @@ int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_
 int xdna_tile_mm_bf16(const uint16_t* p, int64_t ldp, int p_rows, const uint16_t* q, int64_t ldq, int q_rows, int64_t P,
                       int64_t Q, int64_t K, uint16_t* out, int64_t ldc, void* stream) {
   const char* what = "xdna_tile_mm_bf16";
-  if (P < 0 || P > kMaxSide || Q < 0 || Q > kMaxSide || K < 1 || K > kMaxSide || P * Q > kMaxOutputs)
+  if (P < 0 || P > kMaxSide || Q < 0 || Q > kMaxRows || K < 1 || K > kMaxSide || P * Q > kMaxOutputs)
     return refuse(what, "sizes out of range");
   if ((p_rows != 0 && p_rows != 1) || (q_rows != 0 && q_rows != 1) || (q_rows && !p_rows))
     return refuse(what, "operands are k-contiguous (0) or row-contiguous (1), q only beside such a p");

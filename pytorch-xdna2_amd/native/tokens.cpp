@@ -84,7 +84,7 @@ at::Tensor product(const at::Tensor& a, const at::Tensor& b) {
   const bool fills = tiles >= 192 && 100 * tiles >= 65 * 256 * ((tiles + 255) / 256) && K * tiles >= 262144;
   const bool splits = (tiles == 64 || tiles == 128) && K * tiles >= 524288;
   const bool large = vector_rows(a) && vector_rows(b) && K % 8 == 0 && K >= 1024 && (fills || splits);
-  if (K > 0 && !large && a_ok && b_ok) {
+  if (K > 0 && !large && a_ok && b_ok && M <= int64_t(1) << 22) {
     const int64_t lda = a_rows ? a.stride(1) : M > 1 ? a.stride(0) : K, ldb = b_rows ? b.stride(0) : N > 1 ? b.stride(1) : K;
     check_abi(xdna_tile_mm_bf16(p16(b), ldb, b_rows ? 1 : 0, p16(a), lda, a_rows ? 1 : 0, N, M, K, m16(c), N,
                                 current_stream()),
