@@ -296,7 +296,7 @@ __device__ inline void distill_row(const RowArgs& a, int64_t row, const RowStat&
     const float w = any_some ? early.weight : 0.0f;
     d.stats[row] = kept_stats(st);
     d.share[row] = w;
-    d.loss[row] = any_bad ? NAN : w == 0.0f ? 0.0f : w * (d.tau * d.tau) * sum;
+    d.loss[row] = early.weight == 0.0f ? 0.0f : any_bad ? NAN : w == 0.0f ? 0.0f : w * (d.tau * d.tau) * sum;
   }
 }
 

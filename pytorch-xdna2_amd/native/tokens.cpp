@@ -242,37 +242,45 @@ void check_gated(const char* op, const at::Tensor& x, const at::Tensor& w_in) {
 
 // ---- distillation --------------------------------------------------------------------------------
 
+// What a call's kernels write beside the loss, in one buffer (an allocation each would cost a short
+// call as much as its kernels): the pieces' workspace, [T] (m, 1 / s), [T][k] p, [T] shares,
+// [T] row losses (where the loss itself is one number) and 1 / sum of the weights.
+struct DistillAux {
+  size_t workspace;  // bytes, a multiple of 16
+  int64_t T, k;
+  DistillAux(int64_t rows, int64_t V, int64_t entries)
+      : workspace((xdna_distill_workspace_bytes(rows, V) + 15) / 16 * 16), T(rows), k(entries) {}
+  int64_t bytes() const { return int64_t(workspace) + (T * (k + 4) + 1) * int64_t(sizeof(float)); }
+  float* stats(void* p) const { return reinterpret_cast<float*>(static_cast<char*>(p) + workspace); }
+  float* p(void* b) const { return stats(b) + 2 * T; }
+  float* share(void* b) const { return p(b) + T * k; }
+  float* row(void* b) const { return share(b) + T; }
+  float* inv_weight(void* b) const { return row(b) + T; }
+};
+
 struct DistillForward {
-  at::Tensor loss, z, ids, share, stats, p, inv_weight;
+  at::Tensor loss, ids, aux;
 };
 
 DistillForward distill_forward(const at::Tensor& logits, const at::Tensor& teacher_ids, const at::Tensor& teacher,
                                double tau, const std::optional<at::Tensor>& weight, int64_t reduction) {
   ScopedCount sc("hip_tokens.distill.fwd.run");
   DistillForward r;
-  r.z = as_rows(logits);
+  const at::Tensor z = as_rows(logits), t = as_rows(teacher).contiguous();
   r.ids = as_rows(teacher_ids).contiguous();
-  const at::Tensor t = as_rows(teacher).contiguous();
   at::Tensor w;
   if (weight.has_value()) w = weight->to(at::kFloat).contiguous();
-  const int64_t T = r.z.size(0), V = r.z.size(1), k = r.ids.size(1);
-  at::Tensor row = empty_xdna({T}, at::kFloat), out;
-  r.share = empty_xdna({T}, at::kFloat);
-  r.stats = empty_xdna({T, 2}, at::kFloat);
-  r.p = empty_xdna({T, k}, at::kFloat);
-  if (reduction != 0) {
-    out = empty_xdna({}, at::kFloat);
-    r.inv_weight = empty_xdna({}, at::kFloat);
-  }
-  const size_t bytes = xdna_distill_workspace_bytes(T, V);
-  at::Tensor ws;
-  if (bytes) ws = workspace(bytes);
-  check_abi(xdna_distill(cptr(r.z), r.z.scalar_type() == at::kFloat ? 1 : 2, T, V, row_stride(r.z), cptr(r.ids),
+  const DistillAux aux(z.size(0), z.size(1), r.ids.size(1));
+  r.loss = reduction == 0 ? empty_xdna(logits.sizes().slice(0, logits.dim() - 1), at::kFloat) : empty_xdna({}, at::kFloat);
+  r.aux = workspace(size_t(aux.bytes()));
+  void* b = r.aux.data_ptr();
+  float* loss = static_cast<float*>(ptr_or_null(r.loss));
+  check_abi(xdna_distill(cptr(z), z.scalar_type() == at::kFloat ? 1 : 2, aux.T, z.size(1), row_stride(z), cptr(r.ids),
                          r.ids.scalar_type() == at::kLong ? 8 : 4, cptr(t), t.scalar_type() == at::kFloat ? 1 : 2,
-                         int(k), float(tau), cf32(w), int(reduction), f32(row), f32(r.share), f32(r.stats), f32(r.p),
-                         f32(out), f32(r.inv_weight), ptr_or_null(ws), bytes, current_stream()),
+                         int(aux.k), float(tau), cf32(w), int(reduction), reduction == 0 ? loss : aux.row(b), aux.share(b),
+                         aux.stats(b), aux.p(b), reduction == 0 ? nullptr : loss, aux.inv_weight(b), b, aux.workspace,
+                         current_stream()),
             "distill_loss");
-  r.loss = reduction == 0 ? row.view(logits.sizes().slice(0, logits.dim() - 1)) : out;
   return r;
 }
 
@@ -281,7 +289,7 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
                             const at::Tensor& teacher, double tau, const std::optional<at::Tensor>& weight,
                             int64_t reduction) {
     const DistillForward f = distill_forward(logits, ids, teacher, tau, weight, reduction);
-    ctx->save_for_backward({logits, f.ids, f.share, f.stats, f.p, f.inv_weight});
+    ctx->save_for_backward({logits, f.ids, f.aux});
     ctx->saved_data["tau"] = tau;
     ctx->saved_data["rows"] = reduction == 0;
     return f.loss;
@@ -294,13 +302,17 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
     ScopedCount sc("hip_tokens.distill.bwd.run");
     const auto saved = ctx->get_saved_variables();
     const at::Tensor z = as_rows(saved[0]), go = grads[0].contiguous();
-    const at::Tensor &ids = saved[1], &inv = saved[5];
+    const at::Tensor& ids = saved[1];
+    const bool rows = ctx->saved_data["rows"].toBool();
+    const DistillAux aux(z.size(0), z.size(1), ids.size(1));
+    void* b = saved[2].data_ptr();
     at::Tensor dz = empty_xdna(saved[0].sizes(), z.scalar_type());
     check_abi(xdna_distill_bwd(cptr(z), z.scalar_type() == at::kFloat ? 1 : 2, z.size(0), z.size(1), row_stride(z),
                                cptr(ids), ids.scalar_type() == at::kLong ? 8 : 4, int(ids.size(1)),
-                               float(ctx->saved_data["tau"].toDouble()), cf32(saved[2]), cf32(saved[3]),
-                               cf32(saved[4]), cf32(inv), cptr(go), float_code(go, "distill_loss", "the gradient"),
-                               ctx->saved_data["rows"].toBool() ? 1 : 0, ptr_or_null(dz), current_stream()),
+                               float(ctx->saved_data["tau"].toDouble()), aux.share(b), aux.stats(b), aux.p(b),
+                               rows ? nullptr : aux.inv_weight(b), cptr(go),
+                               float_code(go, "distill_loss", "the gradient"), rows ? 1 : 0, ptr_or_null(dz),
+                               current_stream()),
               "distill_loss backward");
     none[0] = dz;
     return none;
@@ -313,6 +325,14 @@ struct LogprobForward {
   at::Tensor log_probs, entropy, top_log_probs, top_ids, targets, stats;
 };
 
+size_t logprob_workspace(int64_t T, int64_t V, int64_t top) {
+  return (xdna_token_logprobs_workspace_bytes(T, V, int(top)) + 15) / 16 * 16;
+}
+
+float* stats_in(void* b, size_t workspace) {
+  return b ? reinterpret_cast<float*>(static_cast<char*>(b) + workspace) : nullptr;
+}
+
 LogprobForward logprob_forward(const at::Tensor& logits, const at::Tensor& targets, int64_t top, double tau) {
   ScopedCount sc("hip_tokens.logprobs.fwd.run");
   LogprobForward r;
@@ -322,17 +342,17 @@ LogprobForward logprob_forward(const at::Tensor& logits, const at::Tensor& targe
   auto shape = targets.sizes().vec();
   r.log_probs = empty_xdna(shape, at::kFloat);
   r.entropy = empty_xdna(shape, at::kFloat);
-  r.stats = empty_xdna({T, 2}, at::kFloat);
+  // the pieces' workspace, then [T] (m, 1 / s)
+  const size_t bytes = logprob_workspace(T, V, top);
+  r.stats = workspace(bytes + size_t(T) * 2 * sizeof(float));
   shape.push_back(top);
   r.top_log_probs = empty_xdna(shape, at::kFloat);
   r.top_ids = empty_xdna(shape, at::kLong);
-  const size_t bytes = xdna_token_logprobs_workspace_bytes(T, V, int(top));
-  at::Tensor ws;
-  if (bytes) ws = workspace(bytes);
+  void* b = ptr_or_null(r.stats);
   check_abi(xdna_token_logprobs(cptr(z), z.scalar_type() == at::kFloat ? 1 : 2, T, V, row_stride(z), cptr(r.targets),
                                 r.targets.scalar_type() == at::kLong ? 8 : 4, float(tau), int(top), f32(r.log_probs),
-                                f32(r.entropy), f32(r.stats), f32(r.top_log_probs),
-                                static_cast<int64_t*>(ptr_or_null(r.top_ids)), ptr_or_null(ws), bytes, current_stream()),
+                                f32(r.entropy), stats_in(b, bytes), f32(r.top_log_probs),
+                                static_cast<int64_t*>(ptr_or_null(r.top_ids)), b, bytes, current_stream()),
             "token_log_probs");
   return r;
 }
@@ -344,6 +364,7 @@ struct LogprobFn : public torch::autograd::Function<LogprobFn> {
     // entropy goes through a detached alias: as an output it carries this node
     ctx->save_for_backward({logits, f.targets, f.stats, f.entropy.detach()});
     ctx->saved_data["tau"] = tau;
+    ctx->saved_data["top"] = top;
     ctx->mark_non_differentiable({f.top_log_probs, f.top_ids});
     ctx->set_materialize_grads(false);
     return {f.log_probs, f.entropy, f.top_log_probs, f.top_ids};
@@ -361,8 +382,9 @@ struct LogprobFn : public torch::autograd::Function<LogprobFn> {
     at::Tensor dz = empty_xdna(saved[0].sizes(), z.scalar_type());
     check_abi(xdna_token_logprobs_bwd(cptr(z), z.scalar_type() == at::kFloat ? 1 : 2, z.size(0), z.size(1),
                                       row_stride(z), cptr(saved[1]), saved[1].scalar_type() == at::kLong ? 8 : 4,
-                                      float(ctx->saved_data["tau"].toDouble()), cf32(saved[2]), cf32(saved[3]),
-                                      cf32(gl), cf32(gh), ptr_or_null(dz), current_stream()),
+                                      float(ctx->saved_data["tau"].toDouble()),
+                                      stats_in(ptr_or_null(saved[2]), logprob_workspace(z.size(0), z.size(1), ctx->saved_data["top"].toInt())),
+                                      cf32(saved[3]), cf32(gl), cf32(gh), ptr_or_null(dz), current_stream()),
               "token_log_probs backward");
     none[0] = dz;
     return none;

@@ -493,6 +493,20 @@ def test_distillation_of_masked_and_invalid_rows(T):
     assert torch.isnan(T.distill_loss(z.to("xdna"), ids.to("xdna"), t.to("xdna"), weight=w.to("xdna"))).item()
 
 
+@pytest.mark.parametrize("rows, V", [(2, 100), (2, 20000)])
+def test_distillation_leaves_out_rows_of_weight_zero_with_invalid_ids(T, rows, V):
+    z = torch.randn(rows, V, generator=gen(5))
+    ids = torch.tensor([[V + 3, 1], [2, 3]])
+    t = torch.zeros(rows, 2)
+    zx = z.to("xdna").requires_grad_()
+    each = T.distill_loss(zx, ids.to("xdna"), t.to("xdna"), weight=torch.tensor([0.0, 1.0]).to("xdna"), reduction="none")
+    ref = distill_reference(z[1:], ids[1:], t[1:], 1.0, torch.ones(1), "none")
+    assert each[0].item() == 0.0
+    close(each[1:], ref[0], 128 * U * ref[1], "loss")
+    (dz,) = torch.autograd.grad(each.sum(), [zx])
+    assert not dz[0].cpu().any() and torch.isfinite(dz).all().item()
+
+
 def test_distillation_gradient_against_differences(T):
     V, eps = 200, 2.0 ** -5
     z, d = torch.randn(3, V, generator=gen(30)), torch.randn(3, V, generator=gen(31))
