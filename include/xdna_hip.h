@@ -843,6 +843,14 @@ int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const void* gu, int64_t 
 int xdna_gated_mlp_bwd_bf16(const uint16_t* dy, int64_t lddy, const uint16_t* w_out, int64_t ldw, const void* gu,
                             int64_t M, int64_t N, int64_t F, int act, uint16_t* dgu, void* stream);
 
+/* The gradients that follow dgu in one launch: dx = dgu w_in (M x K), dw_in = dgu^T x (2F x K), and,
+ * where N > 0, dw_out = dy^T h (N x F); dgu and h are dense.  _pick: 1 where that is modelled faster
+ * than the products one by one (a few hundred rows). */
+int xdna_gated_grads_pick(int64_t M, int64_t K, int64_t F, int64_t N);
+int xdna_gated_grads_bf16(const uint16_t* dgu, const uint16_t* x, int64_t ldx, const uint16_t* w_in, int64_t ldw,
+                          const uint16_t* dy, int64_t lddy, const uint16_t* h, int64_t M, int64_t K, int64_t F,
+                          int64_t N, uint16_t* dx, uint16_t* dw_in, uint16_t* dw_out, void* stream);
+
 /* out[q * ldc + p] = sum over k of P[p][k] Q[q][k], for operands of any alignment and row stride:
  * contiguous along k (p_rows / q_rows 0: element (r, k) at r * ld + k) or along the rows (1: at
  * k * ld + r; q only where p is too).  The gated block's products that xdna_gemm_bf16's large

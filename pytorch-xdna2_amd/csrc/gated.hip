@@ -97,9 +97,9 @@ struct TileArgs {
 struct TileAt {
   int x, y, z;
 };
-__device__ inline TileAt tile_at(const TileArgs& a) {
-  const int n = int(gridDim.x), c = int(blockIdx.x) % kGemmXcds, i = int(blockIdx.x) / kGemmXcds;
-  const int t = c * (n / kGemmXcds) + min(c, n % kGemmXcds) + i;
+__device__ inline TileAt tile_at(const TileArgs& a, int block, int n) {
+  const int c = block % kGemmXcds;
+  const int t = c * (n / kGemmXcds) + min(c, n % kGemmXcds) + block / kGemmXcds;
   const int plane = a.nx * a.ny, z = t / plane, r = t - z * plane;
   const int band = r / (a.group * a.nx), in = r - band * a.group * a.nx;
   const int high = min(a.group, a.ny - band * a.group);
@@ -498,14 +498,14 @@ __device__ inline void put_row8(const TileArgs& a, int q, int at, int n, const f
   }
 }
 
+// One tile, by a workgroup.
 template <bool WIDE, bool PROWS, bool QROWS, int EPI, int ACT>
-__global__ __launch_bounds__(Tile<WIDE>::NT, WIDE ? 2 : 4) void tile_kernel(TileArgs a) {
+__device__ inline void tile_block(const TileArgs& a, const TileAt tile) {
   using C = Tile<WIDE>;
   constexpr bool GATED = EPI == kGated || EPI == kGatedKeep;
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];  // [2 buffers][P, Q]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wp = WIDE ? wave & 1 : 0, wq = WIDE ? wave >> 1 : wave & 1, wk = WIDE ? 0 : wave >> 1;
-  const TileAt tile = tile_at(a);
   const int p0 = tile.x * C::T, q0 = tile.y * C::T;
   f32x16_t acc[2][C::NJ];
 #pragma unroll
@@ -644,6 +644,32 @@ __global__ __launch_bounds__(Tile<WIDE>::NT, WIDE ? 2 : 4) void tile_kernel(Tile
 #pragma unroll
     for (int e = 0; e < 8; ++e) d0[e] = from[r * EP + e], d1[e] = GATED ? from[r * EP + 32 + e] : 0.0f;
     put_row8<EPI, ACT>(a, q0 + r, at, n, d0, d1, tile.z);
+  }
+}
+
+template <bool WIDE, bool PROWS, bool QROWS, int EPI, int ACT>
+__global__ __launch_bounds__(Tile<WIDE>::NT, WIDE ? 2 : 4) void tile_kernel(TileArgs a) {
+  tile_block<WIDE, PROWS, QROWS, EPI, ACT>(a, tile_at(a, int(blockIdx.x), int(gridDim.x)));
+}
+
+// The block's gradients that follow dgu, dx = dgu w_in, dw_in = dgu^T x and dw_out = dy^T h, in one
+// launch: at few hundred rows each alone has too few tiles or too few k-tiles to fill the chip, and
+// its last round and its launch cost as much as its work.  The products with the longer k go first.
+struct GradsArgs {
+  TileArgs dx, dw_in, dw_out;
+  int n_dx, n_in, n_out;  // tiles of each
+  int dx_first;
+};
+
+template <bool WIDE>
+__global__ __launch_bounds__(Tile<WIDE>::NT, WIDE ? 2 : 4) void grads_kernel(GradsArgs g) {
+  const int i = int(blockIdx.x) - (g.dx_first ? g.n_dx : 0), n_w = g.n_in + g.n_out;
+  if (i >= 0 && i < n_w) {
+    const bool in = i < g.n_in;
+    const TileArgs& a = in ? g.dw_in : g.dw_out;
+    tile_block<WIDE, true, true, kPlain, kSilu>(a, tile_at(a, in ? i : i - g.n_in, in ? g.n_in : g.n_out));
+  } else {
+    tile_block<WIDE, true, false, kPlain, kSilu>(g.dx, tile_at(g.dx, i < 0 ? int(blockIdx.x) : i - n_w, g.n_dx));
   }
 }
 
@@ -826,7 +852,7 @@ void gated_large_kernel(TileArgs a) {
   constexpr bool GATED = EPI != kGatedGrad;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave & 1, wn = wave >> 1;
-  const TileAt tile = tile_at(a);
+  const TileAt tile = tile_at(a, int(blockIdx.x), int(gridDim.x));
   const int f0 = tile.x * (GATED ? kT4 / 2 : kT4), q0 = tile.y * kT4;
   f32x4_t acc[8][8];
   {
@@ -993,9 +1019,33 @@ float split_cost(bool wide, int64_t tiles, int64_t kt, int64_t splits, int64_t o
   return tile_cost(wide, tiles * splits, ceil_div(kt, splits)) + 3.3f + float(outputs) * (float(splits) * 1.8e-6f + 0.4e-6f);
 }
 
-// Tiles and splits by the costs above.  Measured, p x q x k, one of each outcome: 500 x 4001 x 700
-// narrow 10.0 us (wide 12.8, wide in two splits 25.0); 500 x 6002 x 700 wide 16.3 (narrow 20.1);
-// 1024 x 512 x 8192 narrow in four splits 26.1 (whole 36.6).
+// Tiles and splits by the costs above, P x Q outputs (P in rows of the operand).  Measured, p x q x
+// k, one of each outcome: 500 x 4001 x 700 narrow 10.0 us (wide 12.8, wide in two splits 25.0); 500
+// x 6002 x 700 wide 16.3 (narrow 20.1); 1024 x 512 x 8192 narrow in four splits 26.1 (whole 36.6).
+struct TileChoice {
+  bool wide;
+  int64_t splits;
+  float cost;
+};
+
+int64_t tile_count(bool wide, int64_t P, int64_t Q) { return ceil_div(P, int64_t(wide ? 128 : 64)) * ceil_div(Q, int64_t(wide ? 128 : 64)); }
+int64_t k_tiles(bool wide, int64_t K) { return ceil_div(K, int64_t(wide ? Tile<true>::KT : Tile<false>::KT)); }
+
+TileChoice choose_tiles(int64_t P, int64_t Q, int64_t K, bool may_split) {
+  TileChoice best = {false, 1, INFINITY};
+  for (const bool wide : {false, true}) {
+    const int64_t n = tile_count(wide, P, Q), kt = k_tiles(wide, K);
+    const float whole = tile_cost(wide, n, kt);
+    if (whole < best.cost) best = {wide, 1, whole};
+    for (const int64_t s : {2, 3, 4, 6, 8, 12, 16}) {
+      if (!may_split || 2 * s > kt || n * s > 1024) break;
+      const float cost = split_cost(wide, n, kt, s, P * Q);
+      if (cost < best.cost) best = {wide, s, cost};
+    }
+  }
+  return best;
+}
+
 template <bool PROWS, bool QROWS, int EPI, int ACT>
 bool launch_tiles(const TileArgs& a, hipStream_t st) {
   constexpr int side = EPI == kGated || EPI == kGatedKeep ? 2 : 1;  // tile rows per unit of p
@@ -1012,29 +1062,44 @@ bool launch_tiles(const TileArgs& a, hipStream_t st) {
       if (a.q.rows <= kFewGated) return launch_few<4, 1, EPI, ACT>(a, st);
     }
   }
-  bool use_wide = false;
-  int64_t use_splits = 1;
-  float best = INFINITY;
-  for (const bool wide : {false, true}) {
-    const dim3 t = tiles(wide ? 128 : 64);
-    const int64_t n = int64_t(t.x) * t.y, kt = ceil_div(a.K, wide ? Tile<true>::KT : Tile<false>::KT);
-    const float whole = tile_cost(wide, n, kt);
-    if (whole < best) best = whole, use_wide = wide, use_splits = 1;
-    if constexpr (EPI == kPlain) {
-      const int64_t outputs = int64_t(a.p.rows) * a.q.rows;
-      for (const int64_t s : {2, 3, 4, 6, 8, 12, 16}) {
-        if (2 * s > kt || n * s > 1024) break;
-        const float cost = split_cost(wide, n, kt, s, outputs);
-        if (cost < best) best = cost, use_wide = wide, use_splits = s;
-      }
-    }
-  }
-  const dim3 t = tiles(use_wide ? 128 : 64);
+  const TileChoice c = choose_tiles(int64_t(a.p.rows) * side, a.q.rows, a.K, EPI == kPlain);
+  const dim3 t = tiles(c.wide ? 128 : 64);
   if constexpr (EPI == kPlain) {
-    if (use_splits > 1)
-      return use_wide ? launch_split<true, PROWS, QROWS>(a, t, use_splits, st) : launch_split<false, PROWS, QROWS>(a, t, use_splits, st);
+    if (c.splits > 1)
+      return c.wide ? launch_split<true, PROWS, QROWS>(a, t, c.splits, st) : launch_split<false, PROWS, QROWS>(a, t, c.splits, st);
   }
-  return use_wide ? launch_tile<true, PROWS, QROWS, EPI, ACT>(a, t, st) : launch_tile<false, PROWS, QROWS, EPI, ACT>(a, t, st);
+  return c.wide ? launch_tile<true, PROWS, QROWS, EPI, ACT>(a, t, st) : launch_tile<false, PROWS, QROWS, EPI, ACT>(a, t, st);
+}
+
+// What the gradients' three products take in one launch, in us: the tiles' work spread over the
+// chip, or the longest tile.  Fitted as above to 50 blocks (16 .. 6000 rows, widths 64 .. 1024, 64 ..
+// 4096 units; 10 % off in the mean): narrow tiles, wide tiles or apart by it, their geometric mean is
+// 13.6 us, always apart 23.6.  333 x 1000 -> 1367: 23.2 narrow, 35.7 wide, 37.5 apart; 1628 x 723 ->
+// 1767: 71.4, 61.0, 82.7; 143 x 308 -> 3370 (53 k-tiles for 15 tiles of dx): 33.0, 70.6, 27.1.
+float grads_cost(bool wide, int64_t M, int64_t K, int64_t F, int64_t N) {
+  const int64_t n_dx = tile_count(wide, K, M), n_w = tile_count(wide, K, 2 * F) + (N ? tile_count(wide, F, N) : 0);
+  const float k_dx = float(k_tiles(wide, 2 * F)), k_w = float(k_tiles(wide, M));
+  const auto tile = [&](float k) { return wide ? 1.05f * k + 1.5f : 1.48f * k + 1.3f; };
+  const float work = (float(n_dx) * tile(k_dx) + float(n_w) * tile(k_w)) / 512.0f, k = std::max(k_dx, k_w);
+  return wide ? 4.0f + std::max(work, 0.73f * k + 1.1f) : 5.3f + std::max(work, 0.56f * k - 1.0f);
+}
+
+template <bool WIDE>
+bool launch_grads(GradsArgs g, hipStream_t st) {
+  using C = Tile<WIDE>;
+  void (*f)(GradsArgs) = grads_kernel<WIDE>;
+  static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             int(C::LDS)) == hipSuccess;
+  if (!ok) return false;
+  const auto plan = [](TileArgs& a) {
+    return a.p.rows ? int(plan_tiles(a, ceil_div(a.p.rows, C::T), ceil_div(a.q.rows, C::T), 1, 64)) : 0;
+  };
+  g.n_dx = plan(g.dx);
+  g.n_in = plan(g.dw_in);
+  g.n_out = plan(g.dw_out);
+  g.dx_first = g.dx.K >= g.dw_in.K ? 1 : 0;
+  f<<<unsigned(g.n_dx + g.n_in + g.n_out), C::NT, C::LDS, st>>>(g);
+  return true;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -1163,6 +1228,50 @@ int xdna_tile_mm_bf16(const uint16_t* p, int64_t ldp, int p_rows, const uint16_t
   return launched(what, q_rows   ? launch_tiles<true, true, kPlain, kSilu>(a, st)
                         : p_rows ? launch_tiles<true, false, kPlain, kSilu>(a, st)
                                  : launch_tiles<false, false, kPlain, kSilu>(a, st));
+}
+
+int xdna_gated_grads_pick(int64_t M, int64_t K, int64_t F, int64_t N) {
+  if (gated_fault(M, K, F, 0) || M == 0 || N < 0 || N > kMaxRows || F > kMaxRows / 2) return 0;
+  const float apart = choose_tiles(K, M, 2 * F, true).cost + choose_tiles(K, 2 * F, M, true).cost +
+                      (N ? choose_tiles(F, N, M, true).cost : 0.0f);
+  return std::min(grads_cost(false, M, K, F, N), grads_cost(true, M, K, F, N)) < apart ? 1 : 0;
+}
+
+int xdna_gated_grads_bf16(const uint16_t* dgu, const uint16_t* x, int64_t ldx, const uint16_t* w_in, int64_t ldw,
+                          const uint16_t* dy, int64_t lddy, const uint16_t* h, int64_t M, int64_t K, int64_t F, int64_t N,
+                          uint16_t* dx, uint16_t* dw_in, uint16_t* dw_out, void* stream) {
+  const char* what = "xdna_gated_grads_bf16";
+  if (const char* why = gated_fault(M, K, F, 0)) return refuse(what, why);
+  if (M == 0) return refuse(what, "no rows");
+  if (N < 0 || N > kMaxRows || F > kMaxRows / 2 || 2 * F * K > kMaxOutputs || M * K > kMaxOutputs || N * F > kMaxOutputs)
+    return refuse(what, "sizes out of range");
+  if ((ldx < K && M > 1) || ldw < K || (N > 0 && lddy < N && M > 1)) return refuse(what, "rows overlap");
+  if (!dgu || !x || !w_in || !dx || !dw_in || (N > 0 && (!dy || !h || !dw_out))) return refuse(what, "null operand");
+  if (odd(dgu) || odd(x) || odd(w_in) || odd(dy) || odd(h) || odd(dx) || odd(dw_in) || odd(dw_out))
+    return refuse(what, "misaligned operand");
+  if (!admit_launch(what)) return -1;
+  GradsArgs g = {};
+  g.dx.p = {w_in, ldw, int(K)};
+  g.dx.q = {dgu, 2 * F, int(M)};
+  g.dx.K = int(2 * F);
+  g.dx.out = dx;
+  g.dx.ldc = K;
+  const int64_t lx = M > 1 ? ldx : K;
+  g.dw_in.p = {x, lx, int(K)};
+  g.dw_in.q = {dgu, 2 * F, int(2 * F)};
+  g.dw_in.K = int(M);
+  g.dw_in.out = dw_in;
+  g.dw_in.ldc = K;
+  if (N > 0) {
+    g.dw_out.p = {h, F, int(F)};
+    g.dw_out.q = {dy, M > 1 ? lddy : N, int(N)};
+    g.dw_out.K = int(M);
+    g.dw_out.out = dw_out;
+    g.dw_out.ldc = F;
+  }
+  const bool wide = grads_cost(true, M, K, F, N) < grads_cost(false, M, K, F, N);
+  hipStream_t st = as_stream(stream);
+  return launched(what, wide ? launch_grads<true>(g, st) : launch_grads<false>(g, st));
 }
 
 int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const void* gu, int64_t M, int64_t F, int act, uint16_t* dgu,

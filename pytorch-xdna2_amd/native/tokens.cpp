@@ -75,16 +75,19 @@ bool vector_rows(const at::Tensor& t) {
 // 2048 x 4096 110 and 147, 4096 x 4096 x 1024 36 and 44, 8192 x 1024 x 8192 132 and 174; but 4800 x
 // 4096 x 2048 (1.2 rounds of the CUs) 100 and 95, 8192 x 768 x 6144 (96 tiles) 121 and 105, 4096 x
 // 1024 x 4096 55 and 46, 8192 x 1024 x 2048 51 and 42, 6424 x 896 x 1024 44 and 23.
+bool on_gemm(const at::Tensor& a, const at::Tensor& b) {
+  const int64_t K = a.size(1), tiles = ((a.size(0) + 255) / 256) * ((b.size(1) + 255) / 256);
+  const bool fills = tiles >= 192 && 100 * tiles >= 65 * 256 * ((tiles + 255) / 256) && K * tiles >= 262144;
+  const bool splits = (tiles == 64 || tiles == 128) && K * tiles >= 524288;
+  return vector_rows(a) && vector_rows(b) && K % 8 == 0 && K >= 1024 && (fills || splits);
+}
+
 at::Tensor product(const at::Tensor& a, const at::Tensor& b) {
   const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
   at::Tensor c = empty_xdna({M, N}, at::kBFloat16);
   const bool b_rows = b.stride(1) == 1 && K > 1, a_rows = a.stride(0) == 1 && M > 1 && a.stride(1) != 1;
   const bool a_ok = a_rows ? b_rows : a.stride(1) == 1 || K == 1, b_ok = b_rows || b.stride(0) == 1 || K == 1;
-  const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
-  const bool fills = tiles >= 192 && 100 * tiles >= 65 * 256 * ((tiles + 255) / 256) && K * tiles >= 262144;
-  const bool splits = (tiles == 64 || tiles == 128) && K * tiles >= 524288;
-  const bool large = vector_rows(a) && vector_rows(b) && K % 8 == 0 && K >= 1024 && (fills || splits);
-  if (K > 0 && !large && a_ok && b_ok && M <= int64_t(1) << 22) {
+  if (K > 0 && !on_gemm(a, b) && a_ok && b_ok && M <= int64_t(1) << 22) {
     const int64_t lda = a_rows ? a.stride(1) : M > 1 ? a.stride(0) : K, ldb = b_rows ? b.stride(0) : N > 1 ? b.stride(1) : K;
     check_abi(xdna_tile_mm_bf16(p16(b), ldb, b_rows ? 1 : 0, p16(a), lda, a_rows ? 1 : 0, N, M, K, m16(c), N,
                                 current_stream()),
@@ -169,6 +172,32 @@ at::Tensor gated_dgu(const at::Tensor& dh, const at::Tensor& gu, int64_t act) {
   return dgu;
 }
 
+// The gradients that follow dgu, of all inputs: one launch where that is faster, else one each.
+struct GatedGrads {
+  at::Tensor dx, dw_in, dw_out;
+};
+
+GatedGrads gated_grads(const at::Tensor& dgu, const at::Tensor& x, const at::Tensor& w, const at::Tensor& dy,
+                       const at::Tensor& h) {
+  const int64_t M = x.size(0), K = x.size(1), F = dgu.size(1) / 2, N = dy.defined() ? dy.size(1) : 0;
+  GatedGrads r;
+  if (M > 0 && xdna_gated_grads_pick(M, K, F, N) && !on_gemm(dgu, w) && !on_gemm(dgu.t(), x) &&
+      !(N && on_gemm(dy.t(), h))) {
+    r.dx = empty_xdna({M, K}, at::kBFloat16);
+    r.dw_in = empty_xdna({2 * F, K}, at::kBFloat16);
+    if (N) r.dw_out = empty_xdna({N, F}, at::kBFloat16);
+    check_abi(xdna_gated_grads_bf16(p16(dgu), p16(x), row_stride(x), p16(w), row_stride(w), N ? p16(dy) : nullptr,
+                                    N ? row_stride(dy) : 0, N ? p16(h) : nullptr, M, K, F, N, m16(r.dx), m16(r.dw_in),
+                                    N ? m16(r.dw_out) : nullptr, current_stream()),
+              "gated backward");
+    return r;
+  }
+  r.dx = product(dgu, w);
+  r.dw_in = product(dgu.t(), x);
+  if (N) r.dw_out = product(dy.t(), h);
+  return r;
+}
+
 std::vector<int64_t> with_last(const at::Tensor& x, int64_t n) {
   auto s = x.sizes().vec();
   s.back() = n;
@@ -191,6 +220,10 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor dgu = gated_dgu(grads[0], saved[2], ctx->saved_data["act"].toInt());
     at::Tensor dx, dw;
+    if (ctx->needs_input_grad(0) && ctx->needs_input_grad(1)) {
+      const GatedGrads g = gated_grads(dgu, as_rows(saved[0]), as_rows(saved[1]), at::Tensor(), at::Tensor());
+      return {g.dx.view(saved[0].sizes()), g.dw_in, at::Tensor()};
+    }
     if (ctx->needs_input_grad(0)) dx = product(dgu, as_rows(saved[1])).view(saved[0].sizes());
     if (ctx->needs_input_grad(1)) dw = product(dgu.t(), as_rows(saved[0]));
     return {dx, dw, at::Tensor()};
@@ -221,6 +254,10 @@ struct GatedMlpFn : public torch::autograd::Function<GatedMlpFn> {
       check_abi(xdna_gated_mlp_bwd_bf16(p16(dy), row_stride(dy), p16(wo), row_stride(wo), cptr(gu), dy.size(0), dy.size(1),
                                         h.size(1), int(ctx->saved_data["act"].toInt()), m16(dgu), current_stream()),
                 "gated_mlp backward");
+      if (ctx->needs_input_grad(0) && ctx->needs_input_grad(1) && ctx->needs_input_grad(2)) {
+        const GatedGrads g = gated_grads(dgu, as_rows(x), as_rows(w_in), dy, h);
+        return {g.dx.view(x.sizes()), g.dw_in, g.dw_out, at::Tensor()};
+      }
       if (ctx->needs_input_grad(0)) dx = product(dgu, as_rows(w_in)).view(x.sizes());
       if (ctx->needs_input_grad(1)) dw_in = product(dgu.t(), as_rows(x));
     }

@@ -147,6 +147,8 @@ SIGNATURES = {
     "xdna_gated_bf16": (I, [P, L, P, L, L, L, L, I, P, P, P]),
     "xdna_gated_bwd_bf16": (I, [P, L, P, L, L, I, P, P]),
     "xdna_gated_mlp_bwd_bf16": (I, [P, L, P, L, P, L, L, L, I, P, P]),
+    "xdna_gated_grads_pick": (I, [L, L, L, L]),
+    "xdna_gated_grads_bf16": (I, [P, P, L, P, L, P, L, P, L, L, L, L, P, P, P, P]),
     "xdna_tile_mm_bf16": (I, [P, L, I, P, L, I, L, L, L, P, L, P]),
     "xdna_token_logprobs_workspace_bytes": (Z, [L, L, I]),
     "xdna_token_logprobs": (I, [P, I, L, L, L, P, I, F, I, P, P, P, P, P, P, Z, P]),

@@ -684,3 +684,29 @@ def test_tile_product(hip, stream, P, Q, K, modes):
     ref = q.to(F64) @ p.to(F64).t()
     close(out[:, :P], ref, (K + 8) * U * (q.to(F64).abs() @ p.to(F64).abs().t()) + B * ref.abs() + 1e-30, "product")
     assert (out[:, P].cpu() == 5.0).all(), "stored past a row's end"
+
+
+@pytest.mark.parametrize("M,K,F,N", [(1, 1, 1, 1), (3, 5, 2, 4), (7, 40, 3, 9), (9, 130, 700, 0), (129, 64, 65, 63), (333, 500, 217, 500),
+                                     (65, 200, 900, 3), (2000, 515, 260, 130), (1201, 300, 700, 301)])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_gated_gradients_in_one_launch(hip, stream, M, K, F, N, pad):
+    """dx, dw_in and dw_out from one launch, whatever the rule would choose: narrow and wide tiles,
+    operands shorter than a vector, rows with padding, without dw_out."""
+    from xdna_train import hip_abi
+    print("gated gradients", M, K, F, N, pad, flush=True)
+    g = gen(M + K + F)
+
+    def rows(r, c, p):
+        v = torch.as_strided(torch.full((r * (c + p),), 9.0, device="cuda", dtype=BF16), (r, c), (c + p, 1))
+        return v.copy_(torch.randn(r, c, generator=g).bfloat16())
+
+    dgu, h, x, w, dy = rows(M, 2 * F, 0), rows(M, F, 0), rows(M, K, pad), rows(2 * F, K, pad), rows(M, max(N, 1), pad)
+    dx, dwi, dwo = (torch.full(s, 5.0, device="cuda", dtype=BF16) for s in ((M, K), (2 * F, K), (max(N, 1), F)))
+    rc = hip.xdna_gated_grads_bf16(dgu.data_ptr(), x.data_ptr(), K + pad, w.data_ptr(), K + pad, dy.data_ptr(), max(N, 1) + pad,
+                                   h.data_ptr(), M, K, F, N, dx.data_ptr(), dwi.data_ptr(), dwo.data_ptr(), stream)
+    assert rc == 0, hip_abi.last_error()
+    d = [t.cpu().to(F64) for t in (dgu, x, w, dy, h)]
+    pairs = [(dx, d[0], d[2]), (dwi, d[0].t(), d[1])] + ([(dwo, d[3].t(), d[4])] if N else [])
+    for out, a, b in pairs:
+        close(out, a @ b, (a.shape[1] + 8) * U * (a.abs() @ b.abs()) + B * (a @ b).abs() + 1e-30, "product")
+    assert N or (dwo.cpu() == 5.0).all()

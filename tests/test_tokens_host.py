@@ -127,3 +127,21 @@ def test_gated_products_refuse_bad_arguments():
                     ({"ldw": 3}, "overlap"), ({"act": 4}, "activation"), ({"N": 0}, "sizes"), ({"dgu": A + 1}, "misaligned")]:
         assert refused(bwd(**kw), why), (kw, hip_abi.last_error())
     assert lib.xdna_gated_kept_bytes(3, 4) == 60 and lib.xdna_gated_kept_bytes(0, 4) == 0
+
+
+def test_gated_gradients_refuse_bad_arguments():
+    lib = hip_abi.load()
+
+    def grads(dgu=A, x=A, ldx=8, w=A, ldw=8, dy=A, lddy=6, h=A, M=2, K=8, F=4, N=6, dx=A, dwi=A, dwo=A):
+        return lib.xdna_gated_grads_bf16(dgu, x, ldx, w, ldw, dy, lddy, h, M, K, F, N, dx, dwi, dwo, None)
+
+    for kw, why in [({"dgu": None}, "null"), ({"x": None}, "null"), ({"w": None}, "null"), ({"dy": None}, "null"), ({"h": None}, "null"),
+                    ({"dx": None}, "null"), ({"dwi": None}, "null"), ({"dwo": None}, "null"), ({"M": 0}, "rows"), ({"K": 0}, "sizes"),
+                    ({"N": -1}, "sizes"), ({"N": 1 << 23}, "sizes"), ({"ldx": 7}, "overlap"), ({"ldw": 7}, "overlap"), ({"lddy": 5}, "overlap"),
+                    ({"x": A + 1}, "misaligned"), ({"dwo": A + 1}, "misaligned")]:
+        assert refused(grads(**kw), why), (kw, hip_abi.last_error())
+    assert lib.xdna_gated_grads_pick(0, 8, 4, 6) == 0 and lib.xdna_gated_grads_pick(2, 0, 4, 6) == 0
+    # few hundred rows at once; a long k over few tiles, and batches that fill the chip, apart
+    assert lib.xdna_gated_grads_pick(333, 1000, 1367, 1000) == 1
+    assert lib.xdna_gated_grads_pick(143, 308, 3370, 308) == 0
+    assert lib.xdna_gated_grads_pick(64, 512, 512, 0) == 1
