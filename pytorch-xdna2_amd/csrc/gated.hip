@@ -714,7 +714,10 @@ __global__ __launch_bounds__(256) void tile_join_kernel(TileArgs a, int splits) 
 // workgroup takes 16 units (their gate and up rows) or `span` plain rows as the rows of 16x16x32
 // MFMAs, its eight waves every eighth k-step, with the loads of up to 8 steps in flight; x's
 // fragments come from L2.  The waves' sums are added in wave order through LDS.  (Sixteen waves
-// were slower: 6.7 -> 7.3 us for 1 x 4096 -> 1024, 4.1 -> 4.6 for 1 x 1024 -> 4096.)
+// were slower: 6.7 -> 7.3 us for 1 x 4096 -> 1024, 4.1 -> 4.6 for 1 x 1024 -> 4096.)  1 x 1024 ->
+// 4096 units takes 5.9 us (16.8 MB, 2.8 TB/s with the launch), the product back 4.4; in narrow tiles
+// 7.3 and 9.1.  32 rows 5.9 and 7.4; at 64 the two meet: 1024 -> 4096 8.2 and 7.4, 1000 -> 300 6.2
+// and 7.5.
 //   Fewer than 16 plain rows a workgroup (the MFMA's other rows repeat them) put every CU to work
 // where there are few.  With up to 4 rows of x the repeats become useful: MFMA row (c, i) holds
 // weight row i and column (c', m) row m of x, both at the c-th or c'-th of 4 chunks of 32 k, so
@@ -819,7 +822,10 @@ __global__ __launch_bounds__(512) void few_kernel(TileArgs a) {
 // whole 16-byte vectors by the LDS DMA.  Rows of P (the hidden units) run along the MFMA's rows:
 // a lane's accumulator quad is 4 consecutive units of one row of x.  For the projections P's tile
 // rows hold 16 gate rows and the same 16 units' up rows in turn, so that one tile has both
-// projections of 128 units.
+// projections of 128 units.  One workgroup a CU (the accumulators take half the registers), so that
+// nothing runs beside an epilogue: 8192 x 1024 -> 4096 with the kept projections takes 171 us (805
+// TFLOP/s; its k-loop alone runs at about 1.1 PFLOP/s, the epilogue writes 235 MB), [dg du] from dy
+// 139 us (the same bytes read, and 134 MB written).
 template <bool ROWS>
 constexpr int kDmaMode = ROWS ? kAlongRow : kAlongK;
 
@@ -917,6 +923,7 @@ void gated_large_kernel(TileArgs a) {
 }
 
 // ---- backward, elementwise: [dg du] from dh and the kept [g u] ------------------------------
+// Bound by its bytes: 8192 x 4096 units, 370 MB, take 65 us (5.7 TB/s).
 struct GatedBwdArgs {
   const uint16_t* dh;  // [M][F], row stride ld
   int64_t ld;

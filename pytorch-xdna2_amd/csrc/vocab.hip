@@ -312,10 +312,25 @@ struct TopShared {
 
 // The top-th largest of 64 groups' largest entries (a group: threads of one lane, skewed by
 // wave), 0 where fewer groups hold one: at least `top` entries reach it, and in rows without
-// special order hardly more.
+// special order hardly more.  For nearly as many entries as groups the threads themselves are the
+// groups: the least of 64 maxima lets 4 to 5 times as many entries through as are asked for (64 of
+// 1 x 131072 took 37 us before their join, so 13; 40 of them 18 either way).
 template <int NT>
 __device__ inline uint64_t group_bound(uint64_t best, int top, TopShared<NT>& sh) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if constexpr (NT > 64) {
+    if (top > 48) {
+      sh.best[tid] = best;
+      if (tid == 0) sh.bound = 0, sh.count = 0;
+      __syncthreads();
+      int rank = 0;
+#pragma unroll 8
+      for (int t = 0; t < NT; ++t) rank += sh.best[t] > best ? 1 : 0;
+      if (rank == top - 1 && best != 0) sh.bound = best;  // (entries are unique: one thread at most)
+      __syncthreads();
+      return sh.bound;
+    }
+  }
   if constexpr (NT > 64) {
     sh.best[wave * 64 + ((lane + 17 * wave) & 63)] = best;
     __syncthreads();
@@ -519,7 +534,11 @@ __device__ inline void rescale(float M, float c, float m, float& s, float& u) {
   s *= k;
 }
 
-// A row (or a piece of one): statistics, and for log probabilities its largest entries.
+// A row (or a piece of one): statistics, and for log probabilities its largest entries.  Bound by
+// the bytes of z where the rows are long: 4096 x 131072 in bf16 229 us (4.7 TB/s) for distillation;
+// 1024 x 32768 in fp32 41 us (3.3 TB/s: four workgroups a CU, whose starts and joins show); 4096 x
+// 50001 with 5 alternatives 138 us (3.0 TB/s: odd rows, and the selection behind a barrier).  Few
+// rows are bound by latency: 4 x 131072 with 20 alternatives, in 128 pieces, 9.6 us and the join 6.3.
 template <typename T, int NT, int MODE, bool TOP>
 __global__ __launch_bounds__(NT) void row_kernel(RowArgs a) {
   constexpr int VW = Win<T>::VW, kStep = NT * VW * kWin;
@@ -621,8 +640,11 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(RowArgs a) {
     const int n = a.pieces * a.lp.top;
     uint64_t best = 0;
     if constexpr (TOP) {
+      // by rank and then piece, so that the largest (the lists are in order) are spread over the
+      // threads: one thread's bound lets few others through
       for (int i = tid; i < n; i += kJoinThreads) {
-        const uint64_t e = a.list[row * n + i];
+        const int rank = i / a.pieces, piece = i - rank * a.pieces;
+        const uint64_t e = a.list[row * n + piece * a.lp.top + rank];
         lists[i] = e;
         best = e > best ? e : best;
       }
@@ -691,7 +713,8 @@ struct LogprobBwdArgs {
 constexpr int kBwdThreads = 256;
 
 // dz_v = (g (1[v = y] - q_v) - h q_v (ln q_v + H)) / tau, g and h the row's incoming
-// gradients.  Rows without either are written as zeros and not read.
+// gradients.  Rows without either are written as zeros and not read.  Bound by its bytes: 1024 x
+// 32768 in fp32, 268 MB, take 47 us (5.7 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kBwdThreads) void logprob_bwd_kernel(LogprobBwdArgs a) {
   constexpr int VW = Win<T>::VW;
@@ -753,7 +776,8 @@ struct DistillBwdArgs {
 // dz_v = coef (q_v - sum over the entries of token v of p), coef = go * share * tau [/ sum of
 // weights].  The piece is written without its teacher entries first; behind the barrier the
 // (few) entries' tokens are written again, each with the sum of all its entries' p, which
-// every one of them computes alike (a row may name a token twice).
+// every one of them computes alike (a row may name a token twice).  Bound by its bytes: 4096 x
+// 131072 in bf16, 2.1 GB, take 363 us (5.9 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(DistillBwdArgs a) {
   constexpr int VW = Win<T>::VW;
@@ -803,7 +827,7 @@ __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(DistillBwdArgs
   }
 }
 
-// loss = sum of the rows' losses [/ sum of their weights], in fixed order (fp64)
+// loss = sum of the rows' losses [/ sum of their weights], in fixed order (fp64): 4096 rows 4.9 us
 template <bool MEAN>
 __global__ __launch_bounds__(1024) void distill_total_kernel(const float* __restrict__ loss,
                                                              const float* __restrict__ share, int64_t rows,
@@ -829,12 +853,17 @@ struct Plan {
   int threads, piece, pieces;
 };
 
-// Whole rows where they fill the chip (two workgroups a CU), else pieces of equal length, of
-// at least one step of the workgroup.
+// Whole rows where they are short or come near filling the chip, else pieces of equal length, of at
+// least half a step of the workgroup, and their join.  Measured, pieces and whole rows in us (bf16):
+// 400 x 131072 26.7 and 20.8, 300 x 131072 with 5 alternatives 38 and 45; 300 x 50001 12.8 and 12.0;
+// 1 x 32000 7.1 and 5.4, with 20 alternatives 15.0 and 16.2, 200 x 32000 with 20 23 and 19.
+// One wave a row where that is short and there are enough of them (no barriers): 3000 x 6000 9.4 and
+// 12.0 with four waves, 3000 x 4000 with 5 alternatives 17 and 27, but 200 x 4000 10.3 and 8.6.
 Plan row_plan(int64_t rows, int64_t V) {
   Plan p;
-  p.threads = V <= 2048 ? 64 : 256;
-  p.pieces = rows >= 512 ? 1 : int(std::min<int64_t>({ceil_div(V, int64_t(4096)), ceil_div(int64_t(1024), rows), kMaxPieces}));
+  p.threads = V <= 2048 || (V <= 6144 && rows >= 1024) ? 64 : 256;
+  const bool whole = V <= 32768 || rows >= 384 || (rows >= 256 && V <= 65536);
+  p.pieces = whole ? 1 : int(std::min<int64_t>({ceil_div(V, int64_t(4096)), ceil_div(int64_t(1024), rows), kMaxPieces}));
   p.piece = int(ceil_div(ceil_div(V, int64_t(p.pieces)), int64_t(8)) * 8);
   p.pieces = int(ceil_div(V, int64_t(p.piece)));
   return p;
