@@ -35,6 +35,7 @@ constexpr int kMaxPieces = 64;        // pieces of a row: their lists fit the jo
 constexpr int kMaxTeacher = 1024;     // teacher entries per row (held in LDS by the gradient)
 constexpr int64_t kMaxVocab = int64_t(1) << 22;
 constexpr int kCandidates = 1024;     // LDS list of elements that may be among the largest
+constexpr int kScan = 8;              // windows that the selection reads at once
 constexpr float kLog2e = 1.4426950408889634f;
 
 // VW elements of a 16-byte window (any element-aligned address: global accesses of gfx950
@@ -399,23 +400,37 @@ __device__ inline void select_top(const T* z, int lo, int len, int top, bool fil
   if (bound == 0) bound = lowest;
   const auto scan = [&](uint32_t from, bool all) {  // entries of key >= from to the list
     const float fb = key_value(from);
-    if (all || m >= fb) {
-#pragma unroll 2
-      for (int at = tid * VW; at < len; at += NT * VW) {
-        const Raw r = load_win<T>(z + at, len - at);
-        float wm = raw_get<T>(r, 0);
+    const auto take = [&](const Raw& r, int at) {
+      float wm = raw_get<T>(r, 0);
 #pragma unroll
-        for (int e = 1; e < VW; ++e) wm = fmaxf(wm, raw_get<T>(r, e));
-        if (!all && !(wm >= fb)) continue;
+      for (int e = 1; e < VW; ++e) wm = fmaxf(wm, raw_get<T>(r, e));
+      if (!all && !(wm >= fb)) return;
 #pragma unroll
-        for (int e = 0; e < VW; ++e) {
-          const uint32_t key = order_key(raw_get<T>(r, e));
-          if (at + e < len && key >= from) {
-            const int c = atomicAdd(&sh.count, 1);
-            if (c < kCandidates) sh.cand[c] = entry_of(key, lo + at + e);
-          }
+      for (int e = 0; e < VW; ++e) {
+        const uint32_t key = order_key(raw_get<T>(r, e));
+        if (at + e < len && key >= from) {
+          const int c = atomicAdd(&sh.count, 1);
+          if (c < kCandidates) sh.cand[c] = entry_of(key, lo + at + e);
         }
       }
+    };
+    if (all || m >= fb) {
+      // the few threads that are here wait for a round of kScan windows at once (4096 x 50001: 140
+      // us with two, 122 with eight)
+      const int whole = len / VW;
+      for (int w = tid; w < whole; w += kScan * NT) {
+        Raw r[kScan];
+#pragma unroll
+        for (int i = 0; i < kScan; ++i) {
+          const Pix8 q = *reinterpret_cast<const Pix8*>(z + min(w + i * NT, whole - 1) * VW);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) r[i].w[k] = q.v[k];
+        }
+#pragma unroll
+        for (int i = 0; i < kScan; ++i)
+          if (w + i * NT < whole) take(r[i], (w + i * NT) * VW);
+      }
+      if (whole * VW < len && whole % NT == tid) take(load_win<T>(z + whole * VW, len - whole * VW), whole * VW);
     }
     __syncthreads();
     return sh.count;
@@ -537,10 +552,11 @@ __device__ inline void rescale(float M, float c, float m, float& s, float& u) {
 // A row (or a piece of one): statistics, and for log probabilities its largest entries.  Bound by
 // the bytes of z where the rows are long: 4096 x 131072 in bf16 229 us (4.7 TB/s) for distillation;
 // 1024 x 32768 in fp32 41 us (3.3 TB/s: four workgroups a CU, whose starts and joins show); 4096 x
-// 50001 with 5 alternatives 138 us (3.0 TB/s: odd rows, and the selection behind a barrier).  Few
+// 50001 with 5 alternatives 111 us (3.7 TB/s; 94 where rows start at whole words), 88 without: five
+// waves a SIMD, so that others stream while one workgroup selects (four: 122).  Few
 // rows are bound by latency: 4 x 131072 with 20 alternatives, in 128 pieces, 9.6 us and the join 6.3.
 template <typename T, int NT, int MODE, bool TOP>
-__global__ __launch_bounds__(NT) void row_kernel(RowArgs a) {
+__global__ __launch_bounds__(NT, 5) void row_kernel(RowArgs a) {
   constexpr int VW = Win<T>::VW, kStep = NT * VW * kWin;
   constexpr bool ENT = MODE == kLogprob;
   __shared__ float red[3][NT / 64];

@@ -710,3 +710,39 @@ def test_gated_gradients_in_one_launch(hip, stream, M, K, F, N, pad):
     for out, a, b in pairs:
         close(out, a @ b, (a.shape[1] + 8) * U * (a.abs() @ b.abs()) + B * (a @ b).abs() + 1e-30, "product")
     assert N or (dwo.cpu() == 5.0).all()
+
+
+def test_offsets_past_32_bits(T):
+    """More than 2^31 elements in the logits, the table, its gradient and the block's projections: the
+    last rows against the first, which hold the same values."""
+    rows, V = 17000, 131072
+    z = torch.randn(1, V, generator=gen(1)).bfloat16().to("xdna").expand(rows, V).contiguous().requires_grad_()
+    y = torch.full((rows,), 77, device="xdna")
+    r = T.token_log_probs(z, y, top_k=3)
+    for t in (r.log_probs, r.entropy, r.top_log_probs, r.top_ids):
+        assert torch.equal(t[-1], t[0]) and torch.equal(t[rows // 2], t[0])
+    (dz,) = torch.autograd.grad([r.log_probs, r.entropy], [z], [torch.ones(rows, device="xdna")] * 2)
+    assert torch.equal(dz[-1], dz[0]) and dz[0].any().item()
+    ids = torch.tensor([[5, V - 1]], device="xdna").expand(rows, 2)
+    each = T.distill_loss(z, ids, torch.zeros(rows, 2, device="xdna"), reduction="none")
+    (dz,) = torch.autograd.grad(each.sum(), [z])
+    assert torch.equal(each[-1], each[0]) and torch.equal(dz[-1], dz[0]) and dz[0].any().item()
+    del z, r, dz
+    V, D = 1050000, 2056
+    w = torch.zeros(V, D, device="xdna", dtype=BF16)
+    w[V - 2] = torch.randn(D, generator=gen(2)).bfloat16().to("xdna")
+    w.requires_grad_()
+    x = T.embed(torch.tensor([V - 2, 3], device="xdna"), w, scale=2.0)
+    assert torch.equal(x[0], w[V - 2].detach() * 2) and not x[1].any().item()
+    dy = torch.randn(2, D, generator=gen(3)).bfloat16().to("xdna")
+    (dw,) = torch.autograd.grad(x, [w], dy)
+    assert torch.equal(dw[V - 2], dy[0] * 2) and torch.equal(dw[3], dy[1] * 2) and not dw[V - 1].any().item()
+    del w, x, dw
+    M, K, F = 270000, 8, 4096
+    x = torch.randn(1, K, generator=gen(4)).bfloat16().to("xdna").expand(M, K).contiguous().requires_grad_()
+    wi = torch.randn(2 * F, K, generator=gen(5)).bfloat16().to("xdna")
+    h = T.gated_linear(x, wi)
+    assert torch.equal(h[-1], h[0]) and h[0].any().item()
+    dh = torch.randn(1, F, generator=gen(6)).bfloat16().to("xdna").expand(M, F)
+    (dx,) = torch.autograd.grad(h, [x], dh)
+    assert torch.equal(dx[-1], dx[0]) and dx[0].any().item()
