@@ -116,6 +116,12 @@ __device__ inline void store_win(T* p, const Raw& r, int n) {
   }
 }
 
+// 1 where p starts inside a word: windows of whole words start one element before it or after it.
+template <typename T>
+__device__ inline int word_skip(const T* p) {
+  return sizeof(T) == 2 ? int(reinterpret_cast<uintptr_t>(p) >> 1) & 1 : 0;
+}
+
 __device__ inline float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // ---- order of the alternatives: value descending, index ascending ------------------------
@@ -380,7 +386,7 @@ __device__ inline int block_count(int n, TopShared<NT>& sh) {
   return n;
 }
 
-// The `top` largest of the piece z[0, len) (element 0 has index lo in its row), through
+// The `top` largest of the piece z[skip, len) (element 0 has index lo in its row), through
 // put(rank, entry).  m: the thread's maximum over its windows tid, tid + NT, ...
 //   Usual rows: the elements of value at least the bound go to an LDS list, found by the threads
 // whose maximum reaches it.
@@ -390,7 +396,7 @@ __device__ inline int block_count(int n, TopShared<NT>& sh) {
 //   Rows where even those overflow (the largest elements sit in few groups) or that hold NaN:
 // the exact top-th largest key by bisection, then the same.
 template <typename T, int NT, typename Put>
-__device__ inline void select_top(const T* z, int lo, int len, int top, bool fill, float m, bool nan,
+__device__ inline void select_top(const T* z, int skip, int lo, int len, int top, bool fill, float m, bool nan,
                                   TopShared<NT>& sh, Put put) {
   constexpr int VW = Win<T>::VW;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -408,7 +414,7 @@ __device__ inline void select_top(const T* z, int lo, int len, int top, bool fil
 #pragma unroll
       for (int e = 0; e < VW; ++e) {
         const uint32_t key = order_key(raw_get<T>(r, e));
-        if (at + e < len && key >= from) {
+        if (at + e >= skip && at + e < len && key >= from) {
           const int c = atomicAdd(&sh.count, 1);
           if (c < kCandidates) sh.cand[c] = entry_of(key, lo + at + e);
         }
@@ -457,7 +463,7 @@ __device__ inline void select_top(const T* z, int lo, int len, int top, bool fil
       for (int at = tid * VW; at < len; at += NT * VW) {
         const Raw r = load_win<T>(z + at, len - at);
 #pragma unroll
-        for (int e = 0; e < VW; ++e) c += at + e < len && order_key(raw_get<T>(r, e)) >= trial ? 1 : 0;
+        for (int e = 0; e < VW; ++e) c += at + e >= skip && at + e < len && order_key(raw_get<T>(r, e)) >= trial ? 1 : 0;
       }
       if (block_count<NT>(c, sh) >= top) bound = trial;
     }
@@ -474,7 +480,7 @@ __device__ inline void select_top(const T* z, int lo, int len, int top, bool fil
     if (at < len) {
       const Raw r = load_win<T>(z + at, len - at);
 #pragma unroll
-      for (int e = 0; e < VW; ++e) hits |= (at + e < len && order_key(raw_get<T>(r, e)) == bound ? 1 : 0) << e;
+      for (int e = 0; e < VW; ++e) hits |= (at + e >= skip && at + e < len && order_key(raw_get<T>(r, e)) == bound ? 1 : 0) << e;
     }
     int before = __popc(hits);
 #pragma unroll
@@ -552,8 +558,8 @@ __device__ inline void rescale(float M, float c, float m, float& s, float& u) {
 // A row (or a piece of one): statistics, and for log probabilities its largest entries.  Bound by
 // the bytes of z where the rows are long: 4096 x 131072 in bf16 229 us (4.7 TB/s) for distillation;
 // 1024 x 32768 in fp32 41 us (3.3 TB/s: four workgroups a CU, whose starts and joins show); 4096 x
-// 50001 with 5 alternatives 111 us (3.7 TB/s; 94 where rows start at whole words), 88 without: five
-// waves a SIMD, so that others stream while one workgroup selects (four: 122).  Few
+// 50001 with 5 alternatives 109 us (3.8 TB/s), 79 without (5.2 TB/s): five waves a SIMD, so that
+// others stream while one workgroup selects (with four a tenth more).  Few
 // rows are bound by latency: 4 x 131072 with 20 alternatives, in 128 pieces, 9.6 us and the join 6.3.
 template <typename T, int NT, int MODE, bool TOP>
 __global__ __launch_bounds__(NT, 5) void row_kernel(RowArgs a) {
@@ -566,9 +572,17 @@ __global__ __launch_bounds__(NT, 5) void row_kernel(RowArgs a) {
   const float c = a.inv_tau * kLog2e;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t row = a.pieces == 1 ? item : item / a.pieces;
-    const int lo = a.pieces == 1 ? 0 : int(item - row * a.pieces) * a.piece;
-    const int len = min(a.piece, a.V - lo);
+    int lo = a.pieces == 1 ? 0 : int(item - row * a.pieces) * a.piece;
+    int len = min(a.piece, a.V - lo);
     const T* z = static_cast<const T*>(a.z) + row * a.ld + lo;
+    // windows start at whole words: where z does not, one element earlier, which is left out (its
+    // word holds z's first element too).  4096 x 50001 takes 79 us so, with 5 alternatives 109; 91 and 123 with
+    // windows across the words.
+    const int skip = word_skip(z);
+    z -= skip, lo -= skip, len += skip;
+    const auto leave_out = [&](Steps<T>& w) {
+      if (sizeof(T) == 2 && skip && tid == 0) w.r[0].w[0] = (w.r[0].w[0] & 0xFFFF0000u) | 0xFF80u;  // -inf
+    };
     Early early;
     if (a.pieces == 1) early = early_loads<T, MODE>(a, row);
     float m = -INFINITY, s = 0.0f, u = 0.0f;
@@ -586,10 +600,12 @@ __global__ __launch_bounds__(NT, 5) void row_kernel(RowArgs a) {
     if (whole > 0) {
       Steps<T> next = load(0);
       for (int at = kStep; at < whole; at += kStep) {
-        const Steps<T> w = next;
+        Steps<T> w = next;
         next = load(at);
+        if (at == kStep) leave_out(w);
         accumulate<T, ENT>(w, c, m, s, u);
       }
+      if (whole == kStep) leave_out(next);
       accumulate<T, ENT>(next, c, m, s, u);
     }
     if (whole < len) {
@@ -599,6 +615,7 @@ __global__ __launch_bounds__(NT, 5) void row_kernel(RowArgs a) {
         const int at = whole + (tid + i * NT) * VW;
         w.r[i] = load_win<T>(z + min(at, len), len - at);
       }
+      if (whole == 0) leave_out(w);
       accumulate<T, ENT>(w, c, m, s, u);
     }
     float M = wave_max(m);
@@ -624,13 +641,13 @@ __global__ __launch_bounds__(NT, 5) void row_kernel(RowArgs a) {
       if (tid == 0) a.stat[item] = st;
       if constexpr (TOP) {
         uint64_t* list = a.list + item * a.lp.top;
-        select_top<T, NT>(z, lo, len, a.lp.top, true, m, s != s, sh, [&](int rank, uint64_t e) { list[rank] = e; });
+        select_top<T, NT>(z, skip, lo, len, a.lp.top, true, m, s != s, sh, [&](int rank, uint64_t e) { list[rank] = e; });
       }
     } else if constexpr (MODE == kLogprob) {
       if (tid == 0) logprob_row(a, row, st, early);
       if constexpr (TOP) {
         const float log_s = logf(st.s);
-        select_top<T, NT>(z, lo, len, a.lp.top, false, m, s != s, sh,
+        select_top<T, NT>(z, skip, lo, len, a.lp.top, false, m, s != s, sh,
                           [&](int rank, uint64_t e) { top_store(a, row, rank, e, st, log_s); });
       }
     } else {
@@ -750,9 +767,7 @@ __global__ __launch_bounds__(kBwdThreads) void logprob_bwd_kernel(LogprobBwdArgs
     const bool none = (g == 0.0f && h == 0.0f) || ms.y == 0.0f;
     const float c = a.inv_tau * kLog2e;
     const float H = a.entropy[row] + logf(ms.y);
-#pragma unroll 4
-    for (int at = int(threadIdx.x) * VW; at < len; at += kBwdThreads * VW) {
-      const int n = len - at;
+    const auto window = [&](int at, int n) {
       Raw o = {{0u, 0u, 0u, 0u}};
       if (!none) {
         const Raw r = load_win<T>(z + at, n);
@@ -767,6 +782,16 @@ __global__ __launch_bounds__(kBwdThreads) void logprob_bwd_kernel(LogprobBwdArgs
         }
       }
       store_win<T>(dz + at, o, n);
+    };
+    // (4096 x 50001 in bf16: 162 us; 170 with stores across the words, 195 with the last
+    // window's elements one by one too)
+    const int skip = word_skip(dz);
+    if (len >= VW) {  // the first and the last window overlap their neighbours: the same values twice
+#pragma unroll 4
+      for (int at = skip + int(threadIdx.x) * VW; at < len; at += kBwdThreads * VW) window(min(at, len - VW), VW);
+      if (skip && threadIdx.x == kBwdThreads - 1) window(0, VW);
+    } else if (threadIdx.x == 0) {
+      window(0, len);
     }
   }
 }
@@ -819,9 +844,7 @@ __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(DistillBwdArgs
       ps[j] = a.p[row * a.k + j];
     }
     const float c = a.inv_tau * kLog2e, cq = coef * ms.y;
-#pragma unroll 4
-    for (int at = int(threadIdx.x) * VW; at < len; at += kBwdThreads * VW) {
-      const int n = len - at;
+    const auto window = [&](int at, int n) {
       Raw o = {{0u, 0u, 0u, 0u}};
       if (!none) {
         const Raw r = load_win<T>(z + at, n);
@@ -829,6 +852,14 @@ __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(DistillBwdArgs
         for (int e = 0; e < VW; ++e) raw_set<T>(o, e, cq * exp2_hw((raw_get<T>(r, e) - ms.x) * c));
       }
       store_win<T>(dz + at, o, n);
+    };
+    const int skip = word_skip(dz);
+    if (len >= VW) {  // the first and the last window overlap their neighbours: the same values twice
+#pragma unroll 4
+      for (int at = skip + int(threadIdx.x) * VW; at < len; at += kBwdThreads * VW) window(min(at, len - VW), VW);
+      if (skip && threadIdx.x == kBwdThreads - 1) window(0, VW);
+    } else if (threadIdx.x == 0) {
+      window(0, len);
     }
     __syncthreads();
     if (!none)

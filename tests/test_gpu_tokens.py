@@ -746,3 +746,26 @@ def test_offsets_past_32_bits(T):
     dh = torch.randn(1, F, generator=gen(6)).bfloat16().to("xdna").expand(M, F)
     (dx,) = torch.autograd.grad(h, [x], dh)
     assert torch.equal(dx[-1], dx[0]) and dx[0].any().item()
+
+
+@pytest.mark.parametrize("kind", ["equal", "falling", "rising", "stride", "few", "zeros", "barred"])
+@pytest.mark.parametrize("V", [3, 9, 1001, 5001, 20000, 20001, 69999])
+def test_rows_at_odd_addresses_between_nan(T, V, kind):
+    """Rows that start and end inside a word, with NaN on both sides: none of it may be seen."""
+    print("odd rows", V, kind, flush=True)
+    k = min(V, 40)
+    z = torch.stack([order_rows(V, kind, gen(V + i)) for i in range(3)]).bfloat16()
+    y = torch.tensor([0, V - 1, V // 2])
+    base = torch.full((3, V + 2), math.nan, dtype=BF16)
+    base[:, 1:V + 1] = z
+    zx = base.to("xdna")[:, 1:V + 1].detach().requires_grad_()
+    assert zx.stride(0) == V + 2
+    r = T.token_log_probs(zx, y.to("xdna"), top_k=k)
+    lp, h, tlp, tid, _, _ = logprob_reference(z, y, 1.0, k)
+    assert torch.equal(r.top_ids.cpu(), tid)
+    close(r.top_log_probs, tlp, tol_log(tlp), "top")
+    close(r.log_probs, lp, tol_log(lp), "log_probs")
+    close(r.entropy, h, 4 * U * 304 * (1 + h), "entropy")
+    if kind != "barred":
+        each = T.distill_loss(zx, y[:, None].to("xdna"), torch.zeros(3, 1, device="xdna"), reduction="none")
+        close(each, -lp, tol_log(lp), "loss")
