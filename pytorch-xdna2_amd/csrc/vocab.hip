@@ -558,8 +558,8 @@ __device__ inline void rescale(float M, float c, float m, float& s, float& u) {
 // A row (or a piece of one): statistics, and for log probabilities its largest entries.  Bound by
 // the bytes of z where the rows are long: 4096 x 131072 in bf16 229 us (4.7 TB/s) for distillation;
 // 1024 x 32768 in fp32 41 us (3.3 TB/s: four workgroups a CU, whose starts and joins show); 4096 x
-// 50001 with 5 alternatives 109 us (3.8 TB/s), 79 without (5.2 TB/s): five waves a SIMD, so that
-// others stream while one workgroup selects (with four a tenth more).  Few
+// 50001 with 5 alternatives 100 to 109 us (4 TB/s), 79 without (5.2 TB/s): five waves a SIMD, so
+// that others stream while one workgroup selects (with four a tenth more).  Few
 // rows are bound by latency: 4 x 131072 with 20 alternatives, in 128 pieces, 9.6 us and the join 6.3.
 template <typename T, int NT, int MODE, bool TOP>
 __global__ __launch_bounds__(NT, 5) void row_kernel(RowArgs a) {
@@ -747,7 +747,7 @@ constexpr int kBwdThreads = 256;
 
 // dz_v = (g (1[v = y] - q_v) - h q_v (ln q_v + H)) / tau, g and h the row's incoming
 // gradients.  Rows without either are written as zeros and not read.  Bound by its bytes: 1024 x
-// 32768 in fp32, 268 MB, take 47 us (5.7 TB/s).
+// 32768 in fp32, 268 MB, take 43 us (6.2 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kBwdThreads) void logprob_bwd_kernel(LogprobBwdArgs a) {
   constexpr int VW = Win<T>::VW;
