@@ -603,6 +603,7 @@ int xdna_embed_bwd(const void* ids, int index_bytes, int64_t tokens, const void*
                    size_t workspace_bytes, void* stream) {
   const char* what = "xdna_embed_bwd";
   if (const char* why = embed_fault(index_bytes, tokens, dtype, vocab, dim)) return refuse(what, why);
+  if (ld < dim && tokens > 1) return refuse(what, "gradient rows overlap");
   if (!d_weight || (tokens > 0 && (!ids || !grad))) return refuse(what, "null operand");
   if ((reinterpret_cast<uintptr_t>(d_weight) & 15) || off_element(grad, dtype)) return refuse(what, "misaligned operand");
   const GradPlan p = grad_plan(std::max<int64_t>(tokens, 1), vocab, dim);

@@ -1285,6 +1285,7 @@ int xdna_gated_bwd_bf16(const uint16_t* dh, int64_t ld, const void* gu, int64_t 
                         void* stream) {
   const char* what = "xdna_gated_bwd_bf16";
   if (const char* why = gated_fault(M, 1, F, act)) return refuse(what, why);
+  if (ld < F && M > 1) return refuse(what, "rows overlap");
   if (M == 0) return 0;
   if (!dh || !gu || !dgu) return refuse(what, "null operand");
   if (odd(dh) || odd(gu) || odd(dgu)) return refuse(what, "misaligned operand");

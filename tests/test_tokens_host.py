@@ -145,3 +145,12 @@ def test_gated_gradients_refuse_bad_arguments():
     assert lib.xdna_gated_grads_pick(333, 1000, 1367, 1000) == 1
     assert lib.xdna_gated_grads_pick(143, 308, 3370, 308) == 0
     assert lib.xdna_gated_grads_pick(64, 512, 512, 0) == 1
+
+
+def test_backward_rows_may_not_overlap():
+    """A row stride under the row's length (a negative one would be read before the operand)."""
+    lib = hip_abi.load()
+    need = lib.xdna_embed_bwd_workspace_bytes(4, 10, 8)
+    for ld in (7, 0, -8):
+        assert refused(lib.xdna_embed_bwd(A, 8, 4, A, 2, ld, 10, 8, -1, 1.0, A, A, need, None), "overlap"), ld
+        assert refused(lib.xdna_gated_bwd_bf16(A, ld, A, 2, 8, 0, A, None), "overlap"), ld
