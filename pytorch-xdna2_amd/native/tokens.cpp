@@ -59,6 +59,14 @@ bool tracked(std::initializer_list<const at::Tensor*> ts) {
   return false;
 }
 
+// Raises where an operand carries a tangent (forward-mode differentiation, whatever the grad mode):
+// the operators have no such rule, and a plain call would hand out a result without it.  (PyTorch
+// opens one level at a time, 0.)
+void no_tangents(const char* op, std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), op, ": forward-mode differentiation is not supported");
+}
+
 void once_only(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the gradient itself cannot be differentiated");
 }
@@ -442,6 +450,7 @@ void check_logits(const char* op, const at::Tensor& logits) {
 }  // namespace
 
 at::Tensor token_embed(const at::Tensor& ids, const at::Tensor& weight, double scale, std::optional<int64_t> padding) {
+  no_tangents("embed", {&weight});
   index_bytes(ids, "embed", "ids");
   float_code(weight, "embed", "weight");
   TORCH_CHECK(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(1) >= 1, "embed: weight must be [tokens, width], got ",
@@ -458,6 +467,7 @@ at::Tensor token_embed(const at::Tensor& ids, const at::Tensor& weight, double s
 }
 
 at::Tensor token_gated_linear(const at::Tensor& x, const at::Tensor& w_in, int64_t act) {
+  no_tangents("gated_linear", {&x, &w_in});
   check_gated("gated_linear", x, w_in);
   if (tracked({&x, &w_in})) return GatedLinearFn::apply(x, w_in, act);
   ScopedCount sc("hip_tokens.gated.fwd.run");
@@ -466,6 +476,7 @@ at::Tensor token_gated_linear(const at::Tensor& x, const at::Tensor& w_in, int64
 }
 
 at::Tensor token_gated_mlp(const at::Tensor& x, const at::Tensor& w_in, const at::Tensor& w_out, int64_t act) {
+  no_tangents("gated_mlp", {&x, &w_in, &w_out});
   check_gated("gated_mlp", x, w_in);
   check_bf16(w_out, "gated_mlp", "w_out");
   TORCH_CHECK(w_out.dim() == 2 && w_out.size(0) >= 1 && w_out.size(0) <= (int64_t(1) << 30) &&
@@ -480,6 +491,8 @@ at::Tensor token_gated_mlp(const at::Tensor& x, const at::Tensor& w_in, const at
 at::Tensor token_distill(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher, double tau,
                          const std::optional<at::Tensor>& weight, int64_t reduction) {
   const char* op = "distill_loss";
+  no_tangents(op, {&logits, &teacher});
+  if (weight.has_value()) no_tangents(op, {&*weight});
   check_logits(op, logits);
   index_bytes(ids, op, "teacher_ids");
   float_code(teacher, op, "teacher_logits");
@@ -499,6 +512,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_log_probs(const
                                                                            const at::Tensor& targets, int64_t top,
                                                                            double tau) {
   const char* op = "token_log_probs";
+  no_tangents(op, {&logits});
   check_logits(op, logits);
   index_bytes(targets, op, "targets");
   check_tau(op, tau);

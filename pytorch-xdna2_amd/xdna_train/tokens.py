@@ -8,7 +8,7 @@ dtype or shape that the kernels do not take raises.  Token indices are int64 or 
 masks are data on the device and are never read by the host, so every function can be captured
 in a graph; what an invalid index does is stated with each function.  Sums and softmax
 statistics are fp32 and have a fixed order: equal inputs give equal bits.  The gradients cannot
-be differentiated again.
+be differentiated again, and an operand with a tangent (forward-mode differentiation) raises.
 
     ids -> embed -> gated_mlp -> head (mm) -> distill_loss / token_log_probs
 """

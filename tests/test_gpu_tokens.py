@@ -769,3 +769,30 @@ def test_rows_at_odd_addresses_between_nan(T, V, kind):
     if kind != "barred":
         each = T.distill_loss(zx, y[:, None].to("xdna"), torch.zeros(3, 1, device="xdna"), reduction="none")
         close(each, -lp, tol_log(lp), "loss")
+
+
+def test_forward_mode_is_refused(T):
+    """A tangent that the operators cannot carry on raises, whether or not the tensor also takes part
+    in a backward pass, and under no_grad too."""
+    import torch.autograd.forward_ad as fw
+
+    x, w, wo = (torch.randn(*s, generator=gen(1)).bfloat16().to("xdna") for s in ((3, 8), (12, 8), (5, 6)))
+    z, table = (torch.randn(*s, generator=gen(2)).to("xdna") for s in ((3, 20), (7, 4)))
+    y, ids, t = torch.tensor([1, 2, 3], device="xdna"), torch.tensor([[1], [2], [3]], device="xdna"), torch.zeros(3, 1, device="xdna")
+    calls = [
+        (table, lambda d: T.embed(y, d)), (x, lambda d: T.gated_linear(d, w)), (w, lambda d: T.gated_linear(x, d)),
+        (x, lambda d: T.gated_mlp(d, w, wo)), (wo, lambda d: T.gated_mlp(x, w, d)), (z, lambda d: T.token_log_probs(d, y, top_k=2)),
+        (z, lambda d: T.distill_loss(d, ids, t)), (t, lambda d: T.distill_loss(z, ids, d)), (t[:, 0], lambda d: T.distill_loss(z, ids, t, weight=d)),
+        (z[:0], lambda d: T.token_log_probs(d, y[:0])),
+    ]
+    for i, (leaf, call) in enumerate(calls):
+        for grad in (False, True):
+            with fw.dual_level():
+                dual = fw.make_dual(leaf.clone().requires_grad_(grad), torch.ones_like(leaf))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(dual)
+                    pytest.fail(f"call {i} lost a tangent")
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(dual)
+    with fw.dual_level():  # no tangent among the operands: nothing to lose
+        assert T.embed(y, table).shape == (3, 4)

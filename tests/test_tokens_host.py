@@ -154,3 +154,21 @@ def test_backward_rows_may_not_overlap():
     for ld in (7, 0, -8):
         assert refused(lib.xdna_embed_bwd(A, 8, 4, A, 2, ld, 10, 8, -1, 1.0, A, A, need, None), "overlap"), ld
         assert refused(lib.xdna_gated_bwd_bf16(A, ld, A, 2, 8, 0, A, None), "overlap"), ld
+
+
+def test_forward_mode_is_refused_before_anything_else():
+    import torch.autograd.forward_ad as fw
+
+    y, z = torch.zeros(2, dtype=torch.long), torch.zeros(2, 5)
+    x, w, wo = (torch.zeros(*s, dtype=torch.bfloat16) for s in ((2, 6), (8, 6), (6, 4)))
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: tokens.embed(y, dual(z)), lambda: tokens.gated_linear(dual(x), w), lambda: tokens.gated_linear(x, dual(w)),
+                     lambda: tokens.gated_mlp(dual(x), w, wo), lambda: tokens.gated_mlp(x, dual(w), wo), lambda: tokens.gated_mlp(x, w, dual(wo)),
+                     lambda: tokens.token_log_probs(dual(z), y), lambda: tokens.distill_loss(dual(z), y[:, None], z[:, :1]),
+                     lambda: tokens.distill_loss(z, y[:, None], dual(z[:, :1])),
+                     lambda: tokens.distill_loss(z, y[:, None], z[:, :1], weight=dual(z[:, 0]))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
