@@ -775,8 +775,8 @@ __global__ __launch_bounds__(kBwdThreads) void logprob_bwd_kernel(LogprobBwdArgs
         for (int e = 0; e < VW; ++e) {
           const float d = raw_get<T>(r, e) - ms.x;
           const float q = exp2_hw(d * c) * ms.y;
-          // q ln q stays 0 at -inf
-          float v = -q * (g + h * (fmaxf(d, -1.0e30f) * a.inv_tau + H));
+          // selected by q: ln q is -inf at a masked token, or h times it is (q NaN stays NaN)
+          float v = q == 0.0f ? 0.0f : -q * (g + h * (d * a.inv_tau + H));
           if (at + e == y) v += g;
           raw_set<T>(o, e, v);
         }

@@ -796,3 +796,30 @@ def test_forward_mode_is_refused(T):
                     call(dual)
     with fw.dual_level():  # no tangent among the operands: nothing to lose
         assert T.embed(y, table).shape == (3, 4)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("mask", ["inf", "lowest"])
+@pytest.mark.parametrize("tau,gh", [(1e-2, 65536.0), (1e-3, 400.0), (1e-4, 4.0), (1e-9, 1.0), (1.0, 2.0 ** 40)])
+def test_entropy_gradient_of_masked_tokens_stays_finite(T, tau, gh, mask, dtype):
+    """Masked tokens have probability 0 and gradient 0, however far below the maximum they are in units
+    of the temperature and however large the incoming gradient is.  The logits are of the temperature's
+    size, so that no other probability underflows."""
+    print("masked gradient", tau, gh, mask, dtype, flush=True)
+    rows, V = 3, 3001
+    z = tau * 3 * torch.randn(rows, V, generator=gen(70))
+    barred = torch.rand(rows, V, generator=gen(71)) < 0.5
+    barred[:, 5] = False
+    z = z.masked_fill(barred, -math.inf if mask == "inf" else torch.finfo(dtype).min).to(dtype)
+    y = torch.full((rows,), 5)
+    zx = z.to("xdna").requires_grad_()
+    r = T.token_log_probs(zx, y.to("xdna"), temperature=tau)
+    (dz,) = torch.autograd.grad([r.log_probs, r.entropy], [zx], [torch.ones(rows, device="xdna"), torch.full((rows,), gh, device="xdna")])
+    t32 = float(torch.tensor(tau, dtype=F32))
+    _, h, _, _, q, lq = logprob_reference(z, y, t32, 1)
+    assert not dz.cpu()[barred].any(), "a masked token has a gradient"
+    hot = torch.nn.functional.one_hot(y, V).to(F64)
+    lqf = torch.where(q > 0, lq, torch.zeros_like(lq))
+    ref = (hot - q - gh * q * (lqf + h[:, None])) / t32
+    terms = (hot + q + gh * q * (1 + lqf.abs() + h[:, None])) / t32
+    close(dz, ref, grad_tol(terms, ref, dtype, lqf), "gradient")
