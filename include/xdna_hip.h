@@ -879,8 +879,9 @@ int xdna_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t
 /* Distillation from a teacher's top logits.  Per row: p = softmax(teacher / tau) over its valid
  * entries (ids >= 0 and a logit above -inf; an id named twice counts as the sum of its
  * entries), loss = tau^2 sum p (ln p - ln q[id]), q = softmax(logits / tau).  row_share = the
- * row's weight (weight NULL: 1), 0 where it has no valid entry; row_loss = row_share * loss
- * (an id past the vocabulary: NaN).  reduction 0: that is all; 1 (mean): loss = sum row_loss /
+ * row's weight (weight NULL: 1), 0 where it has no valid entry; row_loss = row_share * loss.  A
+ * valid entry's id past the vocabulary makes row_loss NaN and row_share 0 (no gradient), unless the
+ * row's weight is 0.  reduction 0: that is all; 1 (mean): loss = sum row_loss /
  * sum row_share (0 without weights), inv_weight = 1 / that sum; 2: the sum, inv_weight = 1.
  * stats as above; p: rows x k.  k up to 1024. */
 size_t xdna_distill_workspace_bytes(int64_t rows, int64_t vocab);

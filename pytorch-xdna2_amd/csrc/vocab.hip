@@ -179,7 +179,7 @@ struct DistillOut {
   float2* stats;  // [rows] m and 1 / s
   float* p;       // [rows][k]
   float* loss;    // [rows] the row's weighted loss
-  float* share;   // [rows] the row's weight, 0 where it has no valid entry
+  float* share;   // [rows] the row's weight, 0 where it has no valid entry or one past the vocabulary
 };
 
 struct RowArgs {
@@ -259,22 +259,19 @@ __device__ inline void distill_row(const RowArgs& a, int64_t row, const RowStat&
   const int lane = threadIdx.x & 63;
   const float log_s = logf(st.s);
   const int64_t at = row * d.k;
+  bool bad = false;  // an entry that is present names no token of the vocabulary
   const auto entry = [&](int j) {
     Early r = early;
     if (j >= 64) {
       r.id = index_at(d.ids, d.index_bytes, at + j);
       r.t = teacher_at(d, at + j);
     }
+    bad |= r.id >= a.V && r.t != -INFINITY;
     if (r.id < 0 || r.id >= a.V) r.t = -INFINITY;  // absent
     return r;
   };
   float tm = -INFINITY;
-  bool bad = false;
-  for (int j = lane; j < d.k; j += 64) {
-    const Early r = entry(j);
-    bad |= r.id >= a.V;
-    tm = fmaxf(tm, r.t);
-  }
+  for (int j = lane; j < d.k; j += 64) tm = fmaxf(tm, entry(j).t);
   tm = wave_max(tm);
   const float c = a.inv_tau * kLog2e;
   float ts = 0.0f;
@@ -300,7 +297,7 @@ __device__ inline void distill_row(const RowArgs& a, int64_t row, const RowStat&
   sum = wave_sum(sum);
   const bool any_bad = __any(bad), any_some = __any(some);
   if (lane == 0) {
-    const float w = any_some ? early.weight : 0.0f;
+    const float w = any_some && !any_bad ? early.weight : 0.0f;  // 0: out of the gradient too
     d.stats[row] = kept_stats(st);
     d.share[row] = w;
     d.loss[row] = early.weight == 0.0f ? 0.0f : any_bad ? NAN : w == 0.0f ? 0.0f : w * (d.tau * d.tau) * sum;

@@ -63,7 +63,8 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
 
     ``logits`` [..., vocabulary] in bf16 or fp32; ``teacher_ids`` and ``teacher_logits`` [..., k],
     k up to 1024.  An entry with a negative id or a logit of -inf is absent; a token named twice
-    counts with the sum of its entries; an id past the vocabulary makes the row's loss NaN.
+    counts with the sum of its entries; the id of an entry that is present past the vocabulary
+    makes the row's loss NaN and leaves the row out of the gradient.
     ``weight`` [...] scales rows (0: the row is left out, whatever it holds); a row without
     entries has weight 0.  ``reduction`` "mean" divides by the sum of the weights (0 where that
     is 0), "sum" does not, "none" gives the weighted row losses.  The loss is fp32; the gradient

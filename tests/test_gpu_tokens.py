@@ -823,3 +823,31 @@ def test_entropy_gradient_of_masked_tokens_stays_finite(T, tau, gh, mask, dtype)
     ref = (hot - q - gh * q * (lqf + h[:, None])) / t32
     terms = (hot + q + gh * q * (1 + lqf.abs() + h[:, None])) / t32
     close(dz, ref, grad_tol(terms, ref, dtype, lqf), "gradient")
+
+
+@pytest.mark.parametrize("V", [100, 40000])  # whole rows; pieces and their join
+def test_distillation_entries_outside_the_vocabulary(T, V):
+    """An entry of logit -inf is absent whatever its id; one that is present makes its row's loss NaN
+    and takes the row out of the gradient, and of the other rows' share."""
+    z = torch.randn(3, V, generator=gen(90))
+    ids = torch.tensor([[1, V, 3], [4, V + 7, 6], [7, 8, -1]])
+    t = torch.tensor([[0.5, -math.inf, 1.0], [0.0, -math.inf, -math.inf], [1.0, 0.0, 2.0]])
+    w = torch.tensor([0.5, 1.0, 2.0])
+    zx = z.to("xdna").requires_grad_()
+    loss = T.distill_loss(zx, ids.to("xdna"), t.to("xdna"), weight=w.to("xdna"))
+    rows, mag, dz, terms = distill_reference(z, torch.where(ids < V, ids, torch.full_like(ids, -1)), t, 1.0, w, "mean")
+    close(loss, rows.sum(), 128 * U * mag.sum(), "loss with absent entries")
+    (got,) = torch.autograd.grad(loss, [zx])
+    close(got, dz, grad_tol(2 * terms, dz, F32, torch.log_softmax(z.to(F64), 1)), "gradient with absent entries")
+    t[1, 1] = 0.0  # present now
+    each = T.distill_loss(zx, ids.to("xdna"), t.to("xdna"), weight=w.to("xdna"), reduction="none")
+    assert torch.isnan(each[1]).item() and torch.isfinite(each[::2]).all().item()
+    (got,) = torch.autograd.grad(each, [zx], torch.ones(3, device="xdna"))
+    _, _, dz, terms = distill_reference(z, torch.where(ids < V, ids, torch.full_like(ids, -1)), t, 1.0, w * torch.tensor([1.0, 0.0, 1.0]), "none")
+    assert not got[1].cpu().any(), "a row of a NaN loss has a gradient"
+    close(got, dz, grad_tol(2 * terms, dz, F32, torch.log_softmax(z.to(F64), 1)), "gradient beside an invalid row")
+    mean = T.distill_loss(zx, ids.to("xdna"), t.to("xdna"), weight=w.to("xdna"))
+    assert torch.isnan(mean).item()
+    (got,) = torch.autograd.grad(mean, [zx])
+    _, _, dz, terms = distill_reference(z, torch.where(ids < V, ids, torch.full_like(ids, -1)), t, 1.0, w * torch.tensor([1.0, 0.0, 1.0]), "mean")
+    close(got, dz, grad_tol(2 * terms, dz, F32, torch.log_softmax(z.to(F64), 1)), "mean's gradient beside an invalid row")
