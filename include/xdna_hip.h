@@ -877,13 +877,14 @@ int xdna_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t
                             const float* d_log_probs, const float* d_entropy, void* d_logits, void* stream);
 
 /* Distillation from a teacher's top logits.  Per row: p = softmax(teacher / tau) over its valid
- * entries (ids >= 0 and a logit above -inf; an id named twice counts as the sum of its
- * entries), loss = tau^2 sum p (ln p - ln q[id]), q = softmax(logits / tau).  row_share = the
- * row's weight (weight NULL: 1), 0 where it has no valid entry; row_loss = row_share * loss.  A
- * valid entry's id past the vocabulary makes row_loss NaN and row_share 0 (no gradient), unless the
- * row's weight is 0.  reduction 0: that is all; 1 (mean): loss = sum row_loss /
- * sum row_share (0 without weights), inv_weight = 1 / that sum; 2: the sum, inv_weight = 1.
- * stats as above; p: rows x k.  k up to 1024. */
+ * entries (ids >= 0 and a logit above -inf), loss = tau^2 sum over the entries p (ln p - ln q[id]),
+ * q = softmax(logits / tau).  An id named twice stays two entries in the loss, each with its own
+ * ln p (below the divergence of the joined entries by a constant); the gradient's target at a token
+ * is the sum of its entries' p, either way.  row_share = the row's weight (weight NULL: 1), 0 where
+ * it has no valid entry; row_loss = row_share * loss.  A valid entry's id past the vocabulary makes
+ * row_loss NaN and row_share 0 (no gradient), unless the row's weight is 0.  reduction 0: that is
+ * all; 1 (mean): loss = sum row_loss / sum row_share (0 without weights), inv_weight = 1 / that sum;
+ * 2: the sum, inv_weight = 1.  stats as above; p: rows x k.  k up to 1024. */
 size_t xdna_distill_workspace_bytes(int64_t rows, int64_t vocab);
 int xdna_distill(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* ids,
                  int index_bytes, const void* teacher, int teacher_dtype, int k, float tau, const float* weight,

@@ -252,7 +252,9 @@ __device__ inline void top_store(const RowArgs& a, int64_t row, int rank, uint64
   a.lp.top_ids[row * a.lp.top + rank] = entry_index(e);
 }
 
-// A row's distillation loss from its statistics (one wave): its first 64 entries are in `early`.
+// A row's distillation loss from its statistics (one wave): its first 64 entries are in `early`.  A
+// sum over the entries: two of one token are two terms (joining them would change the loss by a
+// constant and take a search per entry).
 template <typename T>
 __device__ inline void distill_row(const RowArgs& a, int64_t row, const RowStat& st, const Early& early) {
   const DistillOut& d = a.ds;

@@ -62,10 +62,11 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     ``logits / temperature`` over the vocabulary, ``temperature**2 * sum p (ln p - ln q)``.
 
     ``logits`` [..., vocabulary] in bf16 or fp32; ``teacher_ids`` and ``teacher_logits`` [..., k],
-    k up to 1024.  An entry with a negative id or a logit of -inf is absent; a token named twice
-    counts with the sum of its entries; the id of an entry that is present past the vocabulary
-    makes the row's loss NaN and leaves the row out of the gradient.
-    ``weight`` [...] scales rows (0: the row is left out, whatever it holds); a row without
+    k up to 1024.  An entry with a negative id or a logit of -inf is absent.  The sum goes over the
+    entries: a token named twice is two terms with a ``p`` each, which differs from the divergence
+    of the joined entries by a constant, not in its gradient (``q`` minus their sum).  The id of an
+    entry that is present past the vocabulary makes the row's loss NaN and leaves the row out of
+    the gradient.  ``weight`` [...] scales rows (0: the row is left out, whatever it holds); a row without
     entries has weight 0.  ``reduction`` "mean" divides by the sum of the weights (0 where that
     is 0), "sum" does not, "none" gives the weighted row losses.  The loss is fp32; the gradient
     goes to ``logits`` only."""

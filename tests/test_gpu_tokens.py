@@ -851,3 +851,27 @@ def test_distillation_entries_outside_the_vocabulary(T, V):
     (got,) = torch.autograd.grad(mean, [zx])
     _, _, dz, terms = distill_reference(z, torch.where(ids < V, ids, torch.full_like(ids, -1)), t, 1.0, w * torch.tensor([1.0, 0.0, 1.0]), "mean")
     close(got, dz, grad_tol(2 * terms, dz, F32, torch.log_softmax(z.to(F64), 1)), "mean's gradient beside an invalid row")
+
+
+def test_distillation_of_a_token_named_twice(T):
+    """The loss is a sum over the entries, each with its own p; the gradient's target is the sum of a
+    token's entries, so that it is the gradient of the row with these entries as one."""
+    V = 60
+    z = torch.randn(2, V, generator=gen(80))
+    ids, t = torch.tensor([[7, 3, 7], [9, 9, 9]]), torch.tensor([[0.5, 1.0, -0.25], [0.0, 0.0, 0.0]])
+    zx = z.to("xdna").requires_grad_()
+    each = T.distill_loss(zx, ids.to("xdna"), t.to("xdna"), reduction="none")
+    lq = torch.log_softmax(z.to(F64), 1)
+    lp = torch.log_softmax(t.to(F64), 1)
+    terms = lp.exp() * (lp - lq.gather(1, ids))
+    mag = (lp.exp() * (lp.abs() + lq.gather(1, ids).abs() + 1)).sum(1)
+    close(each, terms.sum(1), 128 * U * mag, "loss by entries")
+    (dz,) = torch.autograd.grad(each.sum(), [zx])
+    target = torch.zeros(2, V, dtype=F64).scatter_add_(1, ids, lp.exp())
+    ref = lq.exp() - target
+    close(dz, ref, grad_tol(lq.exp() + target, ref, F32, lq), "gradient")
+    one_ids = torch.tensor([[7, 3, -1], [9, -1, -1]])
+    one_t = torch.where(one_ids >= 0, target.gather(1, one_ids.clamp(min=0)).log(), torch.zeros(2, 3, dtype=F64)).float()
+    one = T.distill_loss(zx, one_ids.to("xdna"), one_t.to("xdna"), reduction="none")
+    (dz1,) = torch.autograd.grad(one.sum(), [zx])
+    close(dz1, ref, grad_tol(lq.exp() + target, ref, F32, lq), "gradient of the joined entries")
