@@ -870,8 +870,9 @@ int xdna_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t voc
                         float* top_log_probs, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream);
 
 /* d_logits (rows x vocab, dense, of the logits' dtype) from the incoming gradients of
- * log_probs and entropy (either may be NULL): 0 for a row without incoming gradients, a row of
- * -inf, and an element of -inf. */
+ * log_probs and entropy (either may be NULL): 0 for a row without incoming gradients, for a row of
+ * -inf, and at an element of -inf that is not the target.  The target's own term is d_log_probs / tau
+ * at any logit, as a log-softmax has it; a target past the vocabulary has none. */
 int xdna_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* targets,
                             int index_bytes, float tau, const float* stats, const float* entropy,
                             const float* d_log_probs, const float* d_entropy, void* d_logits, void* stream);

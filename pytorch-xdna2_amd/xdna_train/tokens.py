@@ -87,6 +87,8 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
     index.  ``logits`` [..., vocabulary] in bf16 or fp32; masked tokens are -inf.
 
     ``log_probs`` and ``entropy`` have a gradient in ``logits``.  A negative target is not
-    scored (0, no gradient), one past the vocabulary gives NaN.  A row of -inf only has log
-    probabilities of -inf, entropy 0 and no gradient."""
+    scored (0, no gradient), one past the vocabulary gives NaN (and no gradient).  A masked token's
+    gradient is 0, unless it is the target: that has the derivative of its own logit, 1 /
+    ``temperature``, beside a log probability of -inf.  A row of -inf only has log probabilities of
+    -inf, entropy 0 and no gradient."""
     return TokenLogProbs(*_dev.native().token_log_probs(logits, targets, top_k, temperature))

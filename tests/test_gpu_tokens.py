@@ -875,3 +875,21 @@ def test_distillation_of_a_token_named_twice(T):
     one = T.distill_loss(zx, one_ids.to("xdna"), one_t.to("xdna"), reduction="none")
     (dz1,) = torch.autograd.grad(one.sum(), [zx])
     close(dz1, ref, grad_tol(lq.exp() + target, ref, F32, lq), "gradient of the joined entries")
+
+
+def test_gradient_of_a_barred_target(T):
+    """The target's own logit has the derivative of a log-softmax also where it is -inf; other masked
+    tokens have none, and neither has the row of a target past the vocabulary."""
+    V, tau = 300, 0.5
+    z = torch.randn(3, V, generator=gen(72))
+    z[0, ::2] = -math.inf
+    y = torch.tensor([4, 5, V])  # barred in row 0
+    zx = z.to("xdna").requires_grad_()
+    r = T.token_log_probs(zx, y.to("xdna"), temperature=tau)
+    assert r.log_probs.detach().cpu()[0] == -math.inf
+    (dz,) = torch.autograd.grad(r.log_probs, [zx], torch.tensor([3.0, 1.0, 1.0], device="xdna"))
+    dz = dz.cpu()
+    assert dz[0, 4] == 3.0 / tau
+    dz[0, 4] = 0.0
+    assert not dz[0, ::2].any() and (dz[0, 1::2] < 0).all()
+    assert torch.isnan(r.log_probs.detach().cpu()[2]) and dz[1].any() and not dz[2].any()
