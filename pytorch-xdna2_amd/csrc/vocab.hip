@@ -957,6 +957,7 @@ bool rows_ok(const char* what, const void* z, int dtype, int64_t rows, int64_t V
   else if (V < 1 || V > kMaxVocab) why = "vocabulary outside 1 .. 2^22";
   else if (ld < V) why = "rows overlap";
   else if (!(tau > 0.0f) || !(tau < INFINITY)) why = "temperature must be positive and finite";
+  else if (!(1.0f / tau * kLog2e < INFINITY)) why = "temperature too small: log2(e) / temperature is infinite";
   else if (rows > (int64_t(1) << 40) / V) why = "too many logits";
   else if (rows > 0 && !z) why = "null logits";
   else if (reinterpret_cast<uintptr_t>(z) % (dtype == 1 ? 4 : 2)) why = "misaligned logits";

@@ -437,8 +437,9 @@ struct LogprobFn : public torch::autograd::Function<LogprobFn> {
 };
 
 void check_tau(const char* op, double tau) {
-  TORCH_CHECK(tau > 0.0 && float(tau) > 0.0f && float(1.0 / tau) > 0.0f && std::isfinite(float(1.0 / tau)), op,
-              ": temperature must be positive and finite, got ", tau);
+  // the kernels divide by tau in base 2: log2(e) / tau has to be a finite fp32 number
+  TORCH_CHECK(float(tau) > 0.0f && std::isfinite(float(tau)) && std::isfinite(1.0f / float(tau) * 1.442695041f), op,
+              ": temperature must be positive and finite (in fp32, and log2(e) / temperature too), got ", tau);
 }
 
 void check_logits(const char* op, const at::Tensor& logits) {

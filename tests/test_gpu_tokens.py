@@ -893,3 +893,26 @@ def test_gradient_of_a_barred_target(T):
     dz[0, 4] = 0.0
     assert not dz[0, ::2].any() and (dz[0, 1::2] < 0).all()
     assert torch.isnan(r.log_probs.detach().cpu()[2]) and dz[1].any() and not dz[2].any()
+
+
+@pytest.mark.parametrize("tau", [4.5e-39, 1e-30, 1e-10, 1e10])
+def test_temperatures_at_the_ends_of_the_range(T, tau):
+    """Logits of the temperature's size: at any temperature the same distribution, and a loss of
+    temperature**2 times the divergence where that is an fp32 number."""
+    t32 = float(torch.tensor(tau, dtype=F32))
+    V = 40
+    z = torch.randn(2, V, generator=gen(95)) * tau
+    t = torch.randn(2, 3, generator=gen(96)) * tau
+    y, ids = torch.tensor([3, 7]), torch.tensor([[1, 2, 3], [4, 5, 6]])
+    r = T.token_log_probs(z.to("xdna"), y.to("xdna"), temperature=tau)
+    lp, h, _, _, _, _ = logprob_reference(z, y, t32, 1)
+    # the smallest ones have few bits left: an input's own grain is 2^-149, and so is 1 / tau's
+    grain = 16 * 2.0 ** -149 / t32 + (16 * 2.0 ** -149 * t32)
+    close(r.log_probs, lp, tol_log(lp) + grain, "log_probs")
+    close(r.entropy, h, 4 * U * 304 * (1 + h) + 4 * grain, "entropy")
+    if 1e-18 < tau < 1e18:
+        each = T.distill_loss(z.to("xdna"), ids.to("xdna"), t.to("xdna"), temperature=tau, reduction="none")
+        per_row, mag, _, _ = distill_reference(z, ids, t, t32, torch.ones(2), "none")
+        close(each, per_row, 128 * U * mag, "row losses")
+    with pytest.raises(RuntimeError, match="temperature"):
+        T.token_log_probs(z.to("xdna"), y.to("xdna"), temperature=4e-39)

@@ -172,3 +172,13 @@ def test_forward_mode_is_refused_before_anything_else():
                      lambda: tokens.distill_loss(z, y[:, None], z[:, :1], weight=dual(z[:, 0]))):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+def test_temperatures_whose_scale_is_infinite_are_refused():
+    """log2(e) / tau multiplies differences that may be 0, which would make NaN of the row's maximum."""
+    lib = hip_abi.load()
+    for tau in (4.0e-39, 2.0e-39, 1e-45):
+        assert refused(lib.xdna_token_logprobs(A, 2, 2, 100, 100, A, 8, tau, 0, A, A, A, None, None, None, 0, None), "temperature"), tau
+        assert refused(lib.xdna_token_logprobs_bwd(A, 2, 2, 100, 100, A, 8, tau, A, A, None, None, A, None), "temperature"), tau
+        assert refused(lib.xdna_distill(A, 2, 2, 100, 100, A, 8, A, 1, 4, tau, None, 1, A, A, A, A, A, A, None, 0, None), "temperature"), tau
+        assert refused(lib.xdna_distill_bwd(A, 2, 2, 100, 100, A, 8, 4, tau, A, A, A, None, A, 1, 0, A, None), "temperature"), tau
