@@ -37,6 +37,7 @@ constexpr int64_t kMaxVocab = int64_t(1) << 22;
 constexpr int kCandidates = 1024;     // LDS list of elements that may be among the largest
 constexpr int kScan = 8;              // windows that the selection reads at once
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.402823466e38f;  // z - m of a term of weight 0: 0 times it is 0, where 0 * -inf is NaN
 
 // VW elements of a 16-byte window (any element-aligned address: global accesses of gfx950
 // take one), as fp32
@@ -530,8 +531,8 @@ __device__ inline void accumulate(const Steps<T>& w, float c, float& m, float& s
   if (top > m) {
     const float d = m == -INFINITY ? -INFINITY : m - m0;
     const float k = exp2_hw(d * c);
-    if (ENT) u = k * (u + fmaxf(d, -1.0e30f) * s);
     s *= k;
+    if (ENT) u = fmaf(fmaxf(d, kLowest), s, k * u);
     m = top;
   }
 #pragma unroll
@@ -541,7 +542,7 @@ __device__ inline void accumulate(const Steps<T>& w, float c, float& m, float& s
       const float d = raw_get<T>(w.r[i], e) - m0;
       const float x = exp2_hw(d * c);
       s += x;
-      if (ENT) u = fmaf(x, fmaxf(d, -1.0e30f), u);  // -inf: 0 * a finite number
+      if (ENT) u = fmaf(x, fmaxf(d, kLowest), u);
     }
 }
 
@@ -550,7 +551,7 @@ template <bool ENT>
 __device__ inline void rescale(float M, float c, float m, float& s, float& u) {
   const float d = m == M ? 0.0f : m - M;
   const float k = s == 0.0f ? 0.0f : exp2_hw(d * c);  // s == 0: nothing but -inf (or nothing at all)
-  if (ENT) u = s == 0.0f ? 0.0f : k * (u + fmaxf(d, -1.0e30f) * s);  // (k is 0 long before the bound)
+  if (ENT) u = s == 0.0f ? 0.0f : fmaf(fmaxf(d, kLowest), s * k, k * u);
   s *= k;
 }
 

@@ -895,7 +895,7 @@ def test_gradient_of_a_barred_target(T):
     assert torch.isnan(r.log_probs.detach().cpu()[2]) and dz[1].any() and not dz[2].any()
 
 
-@pytest.mark.parametrize("tau", [4.5e-39, 1e-30, 1e-10, 1e10])
+@pytest.mark.parametrize("tau", [4.5e-39, 1e-30, 1e-10, 1e10, 1e30])
 def test_temperatures_at_the_ends_of_the_range(T, tau):
     """Logits of the temperature's size: at any temperature the same distribution, and a loss of
     temperature**2 times the divergence where that is an fp32 number."""
