@@ -303,7 +303,7 @@ __device__ inline void distill_row(const RowArgs& a, int64_t row, const RowStat&
     const float w = any_some && !any_bad ? early.weight : 0.0f;  // 0: out of the gradient too
     d.stats[row] = kept_stats(st);
     d.share[row] = w;
-    d.loss[row] = early.weight == 0.0f ? 0.0f : any_bad ? NAN : w == 0.0f ? 0.0f : w * (d.tau * d.tau) * sum;
+    d.loss[row] = early.weight == 0.0f ? 0.0f : any_bad ? NAN : w == 0.0f ? 0.0f : w * (d.tau * (d.tau * sum));  // (tau^2 alone may leave fp32)
   }
 }
 

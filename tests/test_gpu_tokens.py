@@ -916,3 +916,15 @@ def test_temperatures_at_the_ends_of_the_range(T, tau):
         close(each, per_row, 128 * U * mag, "row losses")
     with pytest.raises(RuntimeError, match="temperature"):
         T.token_log_probs(z.to("xdna"), y.to("xdna"), temperature=4e-39)
+
+
+def test_distillation_loss_of_a_temperature_whose_square_underflows(T):
+    tau, V = 1e-25, 12
+    t32 = float(torch.tensor(tau, dtype=F32))
+    z, t = torch.randn(2, V, generator=gen(97)), torch.randn(2, 3, generator=gen(98))
+    z[:, 0] += 10.0  # the student's token, none of the teacher's
+    ids = torch.tensor([[1, 2, 3], [4, 5, 6]])
+    each = T.distill_loss(z.to("xdna"), ids.to("xdna"), t.to("xdna"), temperature=tau, reduction="none")
+    per_row, mag, _, _ = distill_reference(z, ids, t, t32, torch.ones(2), "none")
+    close(each, per_row, 128 * U * mag, "row losses")
+    assert (each.cpu() > 0).all()
