@@ -22,10 +22,30 @@ namespace {
 
 enum Act { kSilu = 0, kGelu = 1, kRelu = 2 };
 
+// The normal distribution function Phi(g) and e = exp(-g^2 / 2).  The lower tail keeps its relative
+// accuracy (1 + erf(g / sqrt 2) loses it to the 1: 4 % off at -5, 0 from -5.5 on): Phi(-|g|) =
+// e t P(t) with t = 1 / (1 + 0.3 |g|), which turns the half line into (0, 1].  P is the polynomial of
+// degree 7 whose largest relative error on |g| <= 14 is least, 1.5e-7 (Lawson's weighted least squares
+// on 4000 Chebyshev points; e underflows past 13.2).  The derivative shares e.  The block at 8192 x
+// 1024 x 4096, forward and backward: 709 us; 767 with the library's erfc, 752 with its erf.
+__device__ inline float2 normal_cdf(float g) {
+  const float x = fabsf(g), e = __expf(-0.5f * g * g), t = __builtin_amdgcn_rcpf(fmaf(0.3f, x, 1.0f));
+  float p = 0.035674773156642914f;
+  p = fmaf(p, t, -0.1572030782699585f);
+  p = fmaf(p, t, 0.20635350048542023f);
+  p = fmaf(p, t, -0.05368364229798317f);
+  p = fmaf(p, t, 0.12856163084506989f);
+  p = fmaf(p, t, 0.09991349279880524f);
+  p = fmaf(p, t, 0.12075395882129669f);
+  p = fmaf(p, t, 0.11962930113077164f);
+  const float tail = e * (t * p);
+  return make_float2(g > 0.0f ? 1.0f - tail : tail, e);
+}
+
 template <int ACT>
 __device__ inline float act_of(float g) {
   if constexpr (ACT == kSilu) return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g));
-  if constexpr (ACT == kGelu) return g * 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+  if constexpr (ACT == kGelu) return g * normal_cdf(g).x;
   return g > 0.0f ? g : (g != g ? g : 0.0f);
 }
 
@@ -37,8 +57,8 @@ __device__ inline float2 act_pair(float g) {
     return make_float2(g * s, s * (1.0f + g * (1.0f - s)));
   }
   if constexpr (ACT == kGelu) {
-    const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-    return make_float2(g * cdf, cdf + g * 0.3989422804014327f * __expf(-0.5f * g * g));
+    const float2 n = normal_cdf(g);
+    return make_float2(g * n.x, n.x + g * 0.3989422804014327f * n.y);
   }
   return g > 0.0f ? make_float2(g, 1.0f) : make_float2(g != g ? g : 0.0f, 0.0f);
 }

@@ -928,3 +928,28 @@ def test_distillation_loss_of_a_temperature_whose_square_underflows(T):
     per_row, mag, _, _ = distill_reference(z, ids, t, t32, torch.ones(2), "none")
     close(each, per_row, 128 * U * mag, "row losses")
     assert (each.cpu() > 0).all()
+
+
+@pytest.mark.parametrize("M", [1, 70, 300])  # the kernels of few rows, and of tiles
+def test_gelu_keeps_its_lower_tail(T, M):
+    """gelu(g) = g Phi(g) relative to its own size where Phi is far below an fp32 ulp of 1.  A relative
+    error e of erfc's argument x = g / sqrt 2 is one of 2 x^2 e = g^2 e of the tail, the exponential of
+    -g^2 / 2 has the same, and each function is within 16 u of its argument's value; then the roundings:
+    h, or dg and the product that hands it out."""
+    g = -torch.linspace(2.0, 12.0, 161).bfloat16().float()
+    F = g.numel()
+    x = torch.zeros(M, 8)
+    x[:, 0] = 1.0
+    w = torch.zeros(2 * F, 8)
+    w[:F, 0], w[F:, 0] = g, 1.0
+    xd, wd = x.bfloat16().to("xdna").requires_grad_(), w.bfloat16().to("xdna").requires_grad_()
+    h = T.gated_linear(xd, wd, activation="gelu")
+    a, da = act64("gelu", g.to(F64))
+    rel = (2 * g.to(F64) ** 2 + 64) * U
+    close(h, a.expand(M, F), ((rel + B) * a.abs()).expand(M, F), "gelu")
+    dh = torch.zeros(M, F)
+    dh[M - 1] = 1.0  # one row: dw_in's first column is its dg
+    (dw,) = torch.autograd.grad(h, [wd], dh.bfloat16().to("xdna"))
+    pdf = torch.exp(-0.5 * g.to(F64) ** 2) / math.sqrt(2 * math.pi)
+    close(dw[:F, 0], da, (rel * (da.abs() + 2 * g.to(F64).abs() * pdf) + 2.1 * B * da.abs()), "gelu's derivative")
+    close(dw[F:, 0], a, (rel + 2.1 * B) * a.abs(), "du")
