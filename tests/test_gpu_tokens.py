@@ -953,3 +953,63 @@ def test_gelu_keeps_its_lower_tail(T, M):
     pdf = torch.exp(-0.5 * g.to(F64) ** 2) / math.sqrt(2 * math.pi)
     close(dw[:F, 0], da, (rel * (da.abs() + 2 * g.to(F64).abs() * pdf) + 2.1 * B * da.abs()), "gelu's derivative")
     close(dw[F:, 0], a, (rel + 2.1 * B) * a.abs(), "du")
+
+
+def kept_parts(gu, M, F):
+    """g and u from the buffer that the backward reads, in 64 bits."""
+    hi = gu[: M * F * 4].view(torch.int16).view(M, 2 * F).cpu().to(torch.int32) << 16
+    low = gu[M * F * 4:].view(M, F).cpu().to(torch.int32)
+    g = (hi[:, :F] | ((low & 15) << 12)).view(F32).to(F64)
+    u = (hi[:, F:] | ((low >> 4) << 12)).view(F32).to(F64)
+    return g, u
+
+
+@pytest.mark.parametrize("M,K,F", [(1, 8, 64), (1, 24, 37), (16, 8, 50), (33, 16, 65), (64, 40, 96), (65, 24, 64), (70, 9, 61), (130, 5, 66),
+                                   (1000, 16, 516), (1300, 24, 1031), (2048, 16, 4096), (2050, 8, 4104), (4000, 8, 4104)])
+def test_kept_projections_hold_20_bits(hip, stream, M, K, F):
+    """What the forward keeps of g and u, by itself: a bf16 and 4 more bits are half an ulp of 2^-11 from
+    the sum, which is (K + 8) u of its terms from the exact one.  Few rows, both tiles, the large tiles."""
+    from xdna_train import hip_abi
+    print("kept", M, K, F, flush=True)
+    g = gen(M + K + F)
+    x, w = torch.randn(M, K, generator=g).bfloat16(), torch.randn(2 * F, K, generator=g).bfloat16()
+    xd, wd = x.cuda(), w.cuda()
+    h = torch.zeros(M, F, device="cuda", dtype=BF16)
+    size = hip.xdna_gated_kept_bytes(M, F)
+    gu = torch.full((size + 16,), 0x5A, device="cuda", dtype=torch.uint8)
+    rc = hip.xdna_gated_bf16(xd.data_ptr(), K, wd.data_ptr(), K, M, K, F, 0, h.data_ptr(), gu.data_ptr(), stream)
+    assert rc == 0, hip_abi.last_error()
+    got = kept_parts(gu[:size], M, F)
+    assert (gu[size:].cpu() == 0x5A).all(), "stored past the end"
+    for part, rows, what in ((got[0], w[:F], "g"), (got[1], w[F:], "u")):
+        ref = x.to(F64) @ rows.to(F64).t()
+        close(part, ref, 2.0 ** -12 * ref.abs() + (K + 8) * U * (x.to(F64).abs() @ rows.to(F64).abs().t()), what)
+
+
+@pytest.mark.parametrize("form,M,F", [("linear", 5, 64), ("linear", 7, 37), ("linear", 33, 66), ("block", 5, 64), ("block", 70, 37), ("block", 300, 1031),
+                                      ("block", 2000, 2000), ("block", 4096, 4096), ("block", 4401, 4872)])
+def test_kept_projections_are_read_in_20_bits(hip, stream, form, M, F):
+    """The backward of a buffer of known bits.  With relu, dh = 1 and positive g the result is [u, g],
+    rounded once from their 20 bits: exact."""
+    from xdna_train import hip_abi
+    print("kept bits", form, M, F, flush=True)
+    g = gen(M + F)
+    bits = torch.randint(0x3F000, 0x41000, (2, M, F), generator=g, dtype=torch.int32)  # 0.5 .. 8 by 2^-11 of themselves
+    bits[1] |= torch.randint(0, 2, (M, F), generator=g, dtype=torch.int32) << 19           # u of both signs
+    hi = torch.cat([bits[0] >> 4, bits[1] >> 4], 1)
+    low = (bits[0] & 15) | ((bits[1] & 15) << 4)
+    gu = torch.cat([hi.to(torch.int64).to(torch.uint16).view(torch.uint8).flatten(), low.to(torch.uint8).flatten()]).cuda()
+    assert gu.numel() == hip.xdna_gated_kept_bytes(M, F)
+    out = torch.zeros(M, 2 * F, device="cuda", dtype=BF16)
+    if form == "linear":
+        dh = torch.ones(M, F, device="cuda", dtype=BF16)
+        rc = hip.xdna_gated_bwd_bf16(dh.data_ptr(), F, gu.data_ptr(), M, F, 2, out.data_ptr(), stream)
+    else:
+        N = 8
+        dy, wo = torch.zeros(M, N, device="cuda", dtype=BF16), torch.zeros(N, F, device="cuda", dtype=BF16)
+        dy[:, 3] = 1
+        wo[3] = 1
+        rc = hip.xdna_gated_mlp_bwd_bf16(dy.data_ptr(), N, wo.data_ptr(), F, gu.data_ptr(), M, N, F, 2, out.data_ptr(), stream)
+    assert rc == 0, hip_abi.last_error()
+    value = (bits << 12).view(F32).bfloat16()
+    assert torch.equal(out[:, :F].cpu(), value[1]) and torch.equal(out[:, F:].cpu(), value[0])
