@@ -1013,3 +1013,65 @@ def test_kept_projections_are_read_in_20_bits(hip, stream, form, M, F):
     assert rc == 0, hip_abi.last_error()
     value = (bits << 12).view(F32).bfloat16()
     assert torch.equal(out[:, :F].cpu(), value[1]) and torch.equal(out[:, F:].cpu(), value[0])
+
+
+def gpu_reference(z, y, tau, k):
+    """logprob_reference of many rows, on the GPU in 64 bits (-0 as +0: they are equal)."""
+    return [t.cpu() for t in logprob_reference(z.cuda().to(F64) + 0.0, y.cuda(), tau, k)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,V,k", [(255, 40000, 8), (300, 70001, 64), (383, 70000, 5), (130, 131071, 40)])
+def test_log_probs_of_hundreds_of_rows_in_pieces(T, rows, V, k, dtype):
+    """Just below the row counts that take whole rows: pieces and their join."""
+    print("pieces", rows, V, k, dtype, flush=True)
+    z, zx = make_logits(rows, V, dtype, rows, masked=0.2, extra=3)
+    z[3] = order_rows(V, "equal", gen(1)).to(dtype)
+    z[4] = order_rows(V, "stride", gen(2)).to(dtype)
+    z[5] = order_rows(V, "few", gen(3)).to(dtype)
+    with torch.no_grad():
+        zx.copy_(z)
+    y = torch.randint(0, V, (rows,), generator=gen(6))
+    r = T.token_log_probs(zx.detach(), y.to("xdna"), top_k=k)
+    lp, h, tlp, tid, _, _ = gpu_reference(z, y, 1.0, k)
+    close(r.log_probs, lp, tol_log(lp), "log_probs")
+    close(r.entropy, h, 4 * U * 304 * (1 + h), "entropy")
+    assert torch.equal(r.top_ids.cpu(), tid)
+    close(r.top_log_probs, tlp, tol_log(tlp), "top")
+
+
+def test_distillation_of_hundreds_of_rows_in_pieces(T):
+    rows, V, k = 255, 40000, 70
+    g = gen(7)
+    z, zx = make_logits(rows, V, BF16, 8, extra=1)
+    ids, t, w = torch.randint(0, V, (rows, k), generator=g), 4 * torch.randn(rows, k, generator=g), torch.rand(rows, generator=g)
+    ids[torch.rand(rows, k, generator=g) < 0.2] = -1
+    loss = T.distill_loss(zx, ids.to("xdna"), t.to("xdna"), weight=w.to("xdna"))
+    per_row, mag, dz, terms = distill_reference(z, ids, t, 1.0, w, "mean")
+    close(loss, per_row.sum(), 128 * U * mag.sum(), "loss")
+    (got,) = torch.autograd.grad(loss, [zx])
+    close(got, dz, grad_tol(2 * terms, dz, BF16, torch.log_softmax(z.to(F64), 1)), "gradient")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("V", [2049, 4097, 6001, 6144, 6145])
+@pytest.mark.parametrize("k", [0, 5, 64])
+def test_log_probs_of_many_short_rows(T, V, k, dtype):
+    """Rows that one wave takes (up to 6144 tokens from 1024 rows on), over a step of it and a tail, the
+    selection in more than one round; special orders among them, odd row strides."""
+    print("short rows", V, k, dtype, flush=True)
+    rows, tau = 1031, 0.9
+    z, zx = make_logits(rows, V, dtype, V, masked=0.3, extra=V % 4 + 1)
+    for i, kind in enumerate(("equal", "falling", "rising", "stride", "few", "zeros", "barred")):
+        z[i] = z[rows - 1 - i] = order_rows(V, kind, gen(i)).to(dtype)
+    with torch.no_grad():
+        zx.copy_(z)
+    y = torch.randint(0, V, (rows,), generator=gen(V))
+    y[::7] = -1
+    r = T.token_log_probs(zx, y.to("xdna"), top_k=k, temperature=tau)
+    t32 = float(torch.tensor(tau, dtype=F32))
+    lp, h, tlp, tid, q, lq = gpu_reference(z, y, t32, k)
+    close(r.log_probs, lp, tol_log(lp), "log_probs")
+    close(r.entropy, h, 4 * U * (64 + 8 * 400 / tau) * (1 + h), "entropy")
+    assert torch.equal(r.top_ids.cpu(), tid)
+    close(r.top_log_probs, tlp, tol_log(tlp), "top")
