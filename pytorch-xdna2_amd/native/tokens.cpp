@@ -82,11 +82,15 @@ bool vector_rows(const at::Tensor& t) {
 // on the gated block's own tiles.  Measured (rows x columns x k, GEMM and own tiles in us): 8192 x
 // 2048 x 4096 110 and 147, 4096 x 4096 x 1024 36 and 44, 8192 x 1024 x 8192 132 and 174; but 4800 x
 // 4096 x 2048 (1.2 rounds of the CUs) 100 and 95, 8192 x 768 x 6144 (96 tiles) 121 and 105, 4096 x
-// 1024 x 4096 55 and 46, 8192 x 1024 x 2048 51 and 42, 6424 x 896 x 1024 44 and 23.
+// 1024 x 4096 55 and 46, 8192 x 1024 x 2048 51 and 42, 6424 x 896 x 1024 44 and 23.  Even splits begin
+// where the two cross, in the mean of the three layouts (a w^T, a w, a^T b): 64 tiles 4096 x 1024 x 5120
+// 60 58 58 and 52 55 57, x 6144 66 63 66 and 61 65 67, x 7168 71 69 72 and 70 74 77 (2048 x 2048 and
+// 8192 x 512 the same); 128 tiles 8192 x 1024 x 3328 65 65 65 and 60 63 66, x 3840 71 71 71 and 69 72
+// 75, x 5120 86 86 87 and 90 93 97 (4096 x 2048 the same).
 bool on_gemm(const at::Tensor& a, const at::Tensor& b) {
   const int64_t K = a.size(1), tiles = ((a.size(0) + 255) / 256) * ((b.size(1) + 255) / 256);
   const bool fills = tiles >= 192 && 100 * tiles >= 65 * 256 * ((tiles + 255) / 256) && K * tiles >= 262144;
-  const bool splits = (tiles == 64 || tiles == 128) && K * tiles >= 524288;
+  const bool splits = (tiles == 64 && K >= 6144) || (tiles == 128 && K >= 3744);
   return vector_rows(a) && vector_rows(b) && K % 8 == 0 && K >= 1024 && (fills || splits);
 }
 
@@ -185,12 +189,23 @@ struct GatedGrads {
   at::Tensor dx, dw_in, dw_out;
 };
 
+// Whether one launch is faster than products of which some run on the GEMM: while the block is short,
+// the launch's tiles of one product fill the CUs that another leaves.  Measured, rows x K x F with N =
+// K, one launch and apart in us: 6000 x 1024 x 4096 294 and 319, 7000 344 and 335; 12288 x 1024 x 2048
+// 326 and 337, 16384 447 and 355; 16384 x 1024 x 1024 228 and 237; 10000 x 512 x 4096 281 and 301,
+// 16384 448 and 391.  Without dw_out, whose few tiles gain most: 7000 x 1024 x 2048 142 and 148, 12288
+// 241 and 237; 3500 x 1024 x 4096 143 and 166, 4096 186 and 154; 7000 x 512 x 4096 141 and 164, 10000
+// 238 and 216.
+bool short_block(int64_t M, int64_t K, int64_t F, int64_t N) {
+  return double(M) * double(F) * double(4 * K + N) <= (N ? 129e9 : 64e9);
+}
+
 GatedGrads gated_grads(const at::Tensor& dgu, const at::Tensor& x, const at::Tensor& w, const at::Tensor& dy,
                        const at::Tensor& h) {
   const int64_t M = x.size(0), K = x.size(1), F = dgu.size(1) / 2, N = dy.defined() ? dy.size(1) : 0;
   GatedGrads r;
-  if (M > 0 && xdna_gated_grads_pick(M, K, F, N) && !on_gemm(dgu, w) && !on_gemm(dgu.t(), x) &&
-      !(N && on_gemm(dy.t(), h))) {
+  const auto apart = [&] { return on_gemm(dgu, w) || on_gemm(dgu.t(), x) || (N && on_gemm(dy.t(), h)); };
+  if (M > 0 && xdna_gated_grads_pick(M, K, F, N) && (short_block(M, K, F, N) || !apart())) {
     r.dx = empty_xdna({M, K}, at::kBFloat16);
     r.dw_in = empty_xdna({2 * F, K}, at::kBFloat16);
     if (N) r.dw_out = empty_xdna({N, F}, at::kBFloat16);
