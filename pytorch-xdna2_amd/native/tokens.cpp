@@ -295,7 +295,7 @@ void check_gated(const char* op, const at::Tensor& x, const at::Tensor& w_in) {
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, op, ": x needs a last dimension");
   TORCH_CHECK(w_in.dim() == 2 && w_in.size(0) >= 2 && w_in.size(0) % 2 == 0 && w_in.size(1) == x.size(-1), op,
               ": w_in must hold the gate rows and then the up rows, [2 F, ", x.size(-1), "], got ", w_in.sizes());
-  TORCH_CHECK(x.numel() / x.size(-1) < (int64_t(1) << 22) && w_in.size(0) <= (int64_t(1) << 30) &&
+  TORCH_CHECK(x.numel() / x.size(-1) <= (int64_t(1) << 22) && w_in.size(0) <= (int64_t(1) << 30) &&
                   w_in.size(1) <= (int64_t(1) << 30),
               op, ": too many rows");
 }

@@ -1075,3 +1075,16 @@ def test_log_probs_of_many_short_rows(T, V, k, dtype):
     close(r.entropy, h, 4 * U * (64 + 8 * 400 / tau) * (1 + h), "entropy")
     assert torch.equal(r.top_ids.cpu(), tid)
     close(r.top_log_probs, tlp, tol_log(tlp), "top")
+
+
+def test_gated_block_of_the_most_rows(T):
+    """2^22 rows are taken and one more is not: the first and the last rows, which hold the same values."""
+    M, K, F = 1 << 22, 2, 3
+    x = torch.randn(64, K, generator=gen(99)).bfloat16().to("xdna").repeat(M // 64, 1).requires_grad_()
+    w, wo = torch.randn(2 * F, K, generator=gen(100)).bfloat16().to("xdna"), torch.randn(K, F, generator=gen(101)).bfloat16().to("xdna")
+    y = T.gated_mlp(x, w, wo)
+    (dx,) = torch.autograd.grad(y, [x], torch.ones(1, K, dtype=BF16, device="xdna").expand(M, K))
+    for t in (y.detach(), dx):
+        assert torch.equal(t[-64:], t[:64]) and t[:64].any().item()
+    with pytest.raises(RuntimeError, match="too many rows"):
+        T.gated_mlp(torch.zeros(M + 1, 1, dtype=BF16, device="xdna"), w[:, :1], wo)
