@@ -471,7 +471,7 @@ at::Tensor token_embed(const at::Tensor& ids, const at::Tensor& weight, double s
   float_code(weight, "embed", "weight");
   TORCH_CHECK(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(1) >= 1, "embed: weight must be [tokens, width], got ",
               weight.sizes());
-  TORCH_CHECK(std::isfinite(scale), "embed: scale must be finite");
+  TORCH_CHECK(std::isfinite(float(scale)), "embed: scale must be finite in fp32, got ", scale);
   const int64_t V = weight.size(0);
   int64_t pad = -1;
   if (padding.has_value()) {

@@ -1088,3 +1088,12 @@ def test_gated_block_of_the_most_rows(T):
         assert torch.equal(t[-64:], t[:64]) and t[:64].any().item()
     with pytest.raises(RuntimeError, match="too many rows"):
         T.gated_mlp(torch.zeros(M + 1, 1, dtype=BF16, device="xdna"), w[:, :1], wo)
+
+
+def test_embedding_refuses_a_scale_past_fp32(T):
+    """It would be infinite in the kernels, and the zeros of a row NaN."""
+    w = torch.zeros(4, 3, device="xdna")
+    for scale in (1e39, -1e300):
+        with pytest.raises(RuntimeError, match="scale"):
+            T.embed(torch.tensor([1], device="xdna"), w, scale=scale)
+    assert not T.embed(torch.tensor([1], device="xdna"), w, scale=3e38).cpu().any()
