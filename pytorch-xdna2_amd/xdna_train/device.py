@@ -305,7 +305,8 @@ def autotune_result() -> dict | None:
 @_api
 def set_npu_mode(mode: int) -> None:
     """2 every HIP path, 1 no HIP weight gradient, 0 every op through the generic
-    PyTorch-ROCm fallback (the reference's NPU modes)."""
+    PyTorch-ROCm fallback (the reference's NPU modes).  The modes choose the routes of PyTorch's
+    operators; the functions of ``xdna_train.tokens`` have one route and take no part."""
     native().set_npu_mode(int(mode))
 
 

@@ -4,11 +4,12 @@ distillation from a teacher's top logits, and log probabilities of given tokens.
 Each is one autograd node over the gfx950 kernels (csrc/embed.hip, gated.hip, vocab.hip); the
 reference has no counterpart beyond its zero-copy CPU fallback
 (torch_xdna_device.cpp:5124-5260).  Operands are xdna tensors; nothing falls back: a device,
-dtype or shape that the kernels do not take raises.  Token indices are int64 or int32.  Ids and
-masks are data on the device and are never read by the host, so every function can be captured
-in a graph; what an invalid index does is stated with each function.  Sums and softmax
-statistics are fp32 and have a fixed order: equal inputs give equal bits.  The gradients cannot
-be differentiated again, and an operand with a tangent (forward-mode differentiation) raises.
+dtype or shape that the kernels do not take raises, and ``set_npu_mode`` does not concern them.
+Token indices are int64 or int32.  Ids and masks are data on the device and are never read by the
+host, so every function can be captured in a graph; what an invalid index does is stated with each
+function.  Sums and softmax statistics are fp32 and have a fixed order: equal inputs give equal
+bits.  The gradients cannot be differentiated again, and an operand with a tangent (forward-mode
+differentiation) raises.
 
     ids -> embed -> gated_mlp -> head (mm) -> distill_loss / token_log_probs
 """

@@ -1097,3 +1097,30 @@ def test_embedding_refuses_a_scale_past_fp32(T):
         with pytest.raises(RuntimeError, match="scale"):
             T.embed(torch.tensor([1], device="xdna"), w, scale=scale)
     assert not T.embed(torch.tensor([1], device="xdna"), w, scale=3e38).cpu().any()
+
+
+def test_npu_modes_do_not_concern_the_functions(T):
+    """They have one route: the same bits in every mode, from the same kernels."""
+    import xdna_train
+
+    g = gen(110)
+    x, w, wo = (torch.randn(*s, generator=g).bfloat16().to("xdna").requires_grad_() for s in ((70, 64), (96, 64), (40, 48)))
+    ids, t = torch.randint(0, 40, (70, 4), generator=g).to("xdna"), torch.randn(70, 4, generator=g).to("xdna")
+
+    def step():
+        y = T.gated_mlp(x, w, wo)
+        loss = T.distill_loss(y, ids, t) - T.token_log_probs(y, ids[:, 0], top_k=3).log_probs.mean() + T.embed(ids, w).float().mean()
+        return [y.detach(), *torch.autograd.grad(loss, [x, w, wo])]
+
+    want = [v.cpu() for v in step()]
+    before = xdna_train.npu_mode()
+    try:
+        for mode in (0, 1, 2):
+            xdna_train.set_npu_mode(mode)
+            xdna_train.reset_mapped_cpu_stats()
+            got = [v.cpu() for v in step()]
+            stats = xdna_train.mapped_cpu_stats()
+            assert all(stats.get(f"hip_tokens.{k}.{d}.run", {}).get("calls", 0) > 0 for k in ("embed", "gated", "distill", "logprobs") for d in ("fwd", "bwd")), mode
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), mode
+    finally:
+        xdna_train.set_npu_mode(before)
