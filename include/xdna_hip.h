@@ -808,8 +808,10 @@ int xdna_colsum_bf16(const uint16_t* x, uint16_t* out, int64_t R, int64_t N, voi
 /* probabilities.  The reference reaches such work only through its          */
 /* zero-copy CPU fallback (torch_xdna_device.cpp:5124-5260).                 */
 /* dtype: 1 fp32, 2 bf16.  index_bytes: 4 or 8 (int32 / int64 indices).      */
-/* Rows may have any stride (ld, in elements) and any element alignment;     */
-/* outputs are dense.  Workspaces are 16-byte aligned.                       */
+/* Rows may have any stride from their length on (ld, in elements) and any   */
+/* element alignment; outputs are dense.  Workspaces are 16-byte aligned.    */
+/* Temperatures are positive, finite and not so small that log2(e) / tau     */
+/* overflows fp32 (4.3e-39).                                                 */
 /* ------------------------------------------------------------------------ */
 
 /* out[t] = scale * weight[ids[t]], each element rounded once (scale 1: a copy).  weight: vocab

@@ -1124,3 +1124,9 @@ def test_npu_modes_do_not_concern_the_functions(T):
             assert all(torch.equal(a, b) for a, b in zip(got, want)), mode
     finally:
         xdna_train.set_npu_mode(before)
+
+
+@pytest.mark.parametrize("M,K,F,N", [(8192, 1024, 2048, 1024), (5000, 1024, 4096, 1024), (7000, 1024, 4096, 1024)])
+def test_gated_gradients_on_both_sides_of_the_short_block(T, M, K, F, N):
+    """One launch for the three gradients although the GEMM would take some of them, and beyond it."""
+    test_gated_mlp_large(T, M, K, F, N, "silu")
