@@ -900,6 +900,83 @@ int xdna_distill_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
                      int index_bytes, int k, float tau, const float* row_share, const float* stats, const float* p,
                      const float* inv_weight, const void* go, int go_dtype, int go_rows, void* d_logits, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* A token model's block: layer norm, linear layer, linear attention with a  */
+/* decay for each head.  Conventions as above; the reference reaches them    */
+/* only through its zero-copy CPU fallback (torch_xdna_device.cpp:5124-5260). */
+/* ------------------------------------------------------------------------ */
+
+/* Layer norm of rows of dim elements: y = (s - m) / sqrt(var + eps) * weight + bias, s = x, or with a
+ * residual s = x + residual, stored (rounded once) in `sum`; the norm is that of the stored sum.
+ * weight / bias: NULL (1 / 0) or dim values of param_dtype (fp32, or the rows' dtype).  stats (NULL, or
+ * two floats a row): mean and 1 / sqrt(var + eps), for the gradient.  sum and y are dense.  dim up to
+ * 2^24.  eps >= 0. */
+int xdna_layer_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, int dtype, int64_t rows, int64_t dim,
+                    const void* weight, const void* bias, int param_dtype, float eps, void* sum, void* y, float* stats,
+                    void* stream);
+
+/* Its gradients from dy and (dsum, or NULL) the gradient of the sum itself; x: the normalised rows (the
+ * stored sum).  dx (dense, or NULL) is the gradient of x and of the residual alike; dweight and dbias
+ * (either may be NULL; of param_dtype) are sums over the rows in fp32, in a fixed order. */
+size_t xdna_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t dim);
+int xdna_layer_norm_bwd(const void* dy, int64_t lddy, const void* dsum, int64_t ldds, const void* x, int64_t ldx, int dtype,
+                        int64_t rows, int64_t dim, const void* weight, int param_dtype, const float* stats, void* dx,
+                        void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = act(x w^T + bias) + residual (M x N, dense) in one kernel, w: N rows of K; act 0 silu, 1 gelu with
+ * erf, 2 relu, 3 none; bias (N values) and residual (rows of N) may be NULL.  fp32 to the one rounding.
+ * slope (M x N 16-bit values, or NULL; not with act 3): act'(v) 2^15 as fp16, for the gradient.  Where k
+ * is split, the fp32 partials come from the library's caching allocator.  M up to 2^22. */
+int xdna_linear_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t M, int64_t K, int64_t N, int act,
+                     const uint16_t* bias, const uint16_t* residual, int64_t ldr, uint16_t* y, uint16_t* slope, void* stream);
+
+/* dp = dy act'(v) (M x N, dense, or NULL) from the kept slopes (NULL: 1), and d_bias (N, or NULL) = its
+ * column sums before that rounding, fp32 in a fixed order.  dx = dp w and dw = dp^T x are plain products,
+ * or one launch, where _pick says 1 (a few hundred rows). */
+size_t xdna_linear_bwd_workspace_bytes(int64_t M, int64_t N);
+int xdna_linear_bwd_bf16(const uint16_t* dy, int64_t ld, const uint16_t* slope, int64_t M, int64_t N, uint16_t* dp,
+                         uint16_t* d_bias, void* workspace, size_t workspace_bytes, void* stream);
+int xdna_linear_grads_pick(int64_t M, int64_t K, int64_t N);
+int xdna_linear_grads_bf16(const uint16_t* dp, int64_t lddp, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw,
+                           int64_t M, int64_t K, int64_t N, uint16_t* dx, uint16_t* dw, void* stream);
+
+/* One operand by heads: element (b, t, h, d) at data[b * batch + t * token + h * head + d], strides in
+ * elements, not negative.  The struct itself is host memory. */
+typedef struct {
+  const uint16_t* data;
+  int64_t batch, token, head;
+} xdna_heads_bf16;
+
+/* Linear attention with a decay for each head: S_t = exp(log_decay[h]) S_{t-1} + k_t^T v_t, o_t = scale
+ * q_t S_t, over B sequences of T tokens (T >= 1) and H heads of q; k and v have G heads, head h of q with
+ * head h / (H / G) of them.  Head sizes dk, dv 1 .. 128.  lengths (NULL, or B int32 / int64 values, taken
+ * into 0 .. T): tokens from there on are not read, and their outputs are 0.  state (NULL: 0): the S before
+ * the first token, [B][H][dk][dv] fp32; state_out (or NULL): the S behind the last, which may be `state`'s
+ * memory only where the workspace is empty.  out: dense [B][T][H][dv]. */
+size_t xdna_decay_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv);
+int xdna_decay_attention(const xdna_heads_bf16* q, const xdna_heads_bf16* k, const xdna_heads_bf16* v, int64_t B, int64_t T,
+                         int64_t H, int64_t G, int64_t dk, int64_t dv, const float* log_decay, const void* lengths,
+                         int index_bytes, float scale, const float* state, uint16_t* out, float* state_out, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Its gradients from those of out and (NULL: 0) of state_out: d_q, d_k, d_v dense, shared heads' summed in
+ * fp32 in head order and rounded once; d_state (or NULL).  0 behind a sequence's end.  log_decay is a
+ * constant. */
+size_t xdna_decay_bwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t G, int64_t dk, int64_t dv);
+int xdna_decay_attention_bwd(const xdna_heads_bf16* dout, const float* d_state_out, const xdna_heads_bf16* q,
+                             const xdna_heads_bf16* k, const xdna_heads_bf16* v, int64_t B, int64_t T, int64_t H, int64_t G,
+                             int64_t dk, int64_t dv, const float* log_decay, const void* lengths, int index_bytes, float scale,
+                             const float* state, uint16_t* d_q, uint16_t* d_k, uint16_t* d_v, float* d_state, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* One token of B sequences (the operands' token stride is not used): state[slot] is updated in place, out:
+ * dense [B][H][dv].  state: [slots][H][dk][dv] fp32; index (NULL: slot b) B int32 / int64 slots: a negative
+ * one is an empty place (output 0); one past the pool, or one that an earlier place of the call has, gives
+ * NaN and touches no state. */
+int xdna_decay_step(const xdna_heads_bf16* q, const xdna_heads_bf16* k, const xdna_heads_bf16* v, int64_t B, int64_t H,
+                    int64_t G, int64_t dk, int64_t dv, const float* log_decay, float* state, int64_t slots, const void* index,
+                    int index_bytes, float scale, uint16_t* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,6 +11,11 @@
 // where multiplying again would cost two more products.
 //   dg = dh u act'(g), du = dh act(g), as [dg du] (M x 2F), so that dx = [dg du] w and
 //   dw = [dg du]^T x are one product each.
+//
+// The linear layer y = act(x W^T + b) + r runs on the same tiles with an epilogue of its own.  For
+// training it keeps the slope act'(v) as an fp16 times 2^15 (2 bytes a unit, 11 bits of mantissa
+// down to 1.9e-9): what the backward multiplies dy by, without the activation again and within 2^-12,
+// where a slope in bf16 would be a second rounding as large as that of dy act'(v) itself.
 #include "common.h"
 #include "gemm_dma.h"
 #include "mfma.h"
@@ -20,7 +25,7 @@
 namespace xdna {
 namespace {
 
-enum Act { kSilu = 0, kGelu = 1, kRelu = 2 };
+enum Act { kSilu = 0, kGelu = 1, kRelu = 2, kNone = 3 };
 
 // The normal distribution function Phi(g) and e = exp(-g^2 / 2).  The lower tail keeps its relative
 // accuracy (1 + erf(g / sqrt 2) loses it to the 1: 4 % off at -5, 0 from -5.5 on): Phi(-|g|) =
@@ -87,7 +92,10 @@ __device__ inline float2 act_pair(float g) {
 // One barrier per k-tile.  Addresses are formed once, per vector and not per k-tile, and only the
 // last k-tile is masked.  (Addresses and masks formed in every k-tile took more VALU time than the
 // MFMAs: 445 us for the block at 4895 x 448 x 1506, forward and backward.)
-enum TileEpi { kPlain = 0, kGated = 1, kGatedKeep = 2, kGatedGrad = 3 };
+enum TileEpi { kPlain = 0, kGated = 1, kGatedKeep = 2, kGatedGrad = 3, kLinear = 4 };
+
+constexpr bool gated_epi(int epi) { return epi == kGated || epi == kGatedKeep; }
+constexpr bool own_rows(int epi) { return epi == kPlain || epi == kLinear; }  // an output per row of P
 
 struct TileOperand {
   const uint16_t* src;
@@ -107,6 +115,12 @@ struct TileArgs {
   float* part;     // kPlain with k split over blockIdx.z: [split][q][p] partials, else null
   int k_split;     // k per split (whole k-tiles)
   int nx, ny, group;  // the grid's tiles along p and along q, and the band of tile_at
+  // kLinear
+  int act;
+  const uint16_t* bias;  // [p] or null
+  const uint16_t* res;   // [q][p], row stride ldr, or null
+  int64_t ldr;
+  uint16_t* slope;       // [q][p], written where not null
 };
 
 // A workgroup's tile.  Workgroups go to the XCDs (each with its own L2) in turn: XCD c takes the
@@ -373,12 +387,56 @@ __device__ inline void store_kept(const TileArgs& a, int q, int at, int n, const
     }
 }
 
+constexpr float kSlopeScale = 32768.0f;  // slopes are up to 1.13 in size: 37000 of fp16's 65504
+
+// act(v) and act'(v) where the activation is a value of the launch: an epilogue's few instructions
+// are cheaper than four copies of every tile kernel
+__device__ inline float2 act_pair(int act, float v) {
+  if (act == kNone) return make_float2(v, 1.0f);
+  if (act == kSilu) return act_pair<kSilu>(v);
+  if (act == kGelu) return act_pair<kGelu>(v);
+  return act_pair<kRelu>(v);
+}
+
+// N outputs of row q from column `at` on (n of them in range): the product's sums d to the layer's
+// outputs, and their slopes
+template <int N>
+__device__ inline void linear_values(const TileArgs& a, int q, int at, int n, float (&d)[N], uint16_t (&slope)[N]) {
+  if (a.bias) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) d[e] += e < n ? bf16_to_f32(a.bias[at + e]) : 0.0f;
+  }
+  if (a.act != kNone) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float2 t = act_pair(a.act, d[e]);
+      d[e] = t.x;
+      slope[e] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(t.y * kSlopeScale));
+    }
+  }
+}
+
 // 4 consecutive outputs: d0 (and for the gated forward the up projection d1) of row q, from
 // column `at` on
 template <int EPI, int ACT>
 __device__ inline void put_quad(const TileArgs& a, int q, int at, const float (&d0)[4], const float (&d1)[4]) {
   if constexpr (EPI == kPlain) {
     put4(a.out + int64_t(q) * a.ldc + at, d0, a.p.rows - at, a.vec);
+  } else if constexpr (EPI == kLinear) {
+    const int n = min(a.p.rows - at, 4);
+    float y[4] = {d0[0], d0[1], d0[2], d0[3]};
+    uint16_t slope[4] = {};
+    linear_values(a, q, at, n, y, slope);
+    if (a.res) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += e < n ? bf16_to_f32(a.res[int64_t(q) * a.ldr + at + e]) : 0.0f;
+    }
+    put4(a.out + int64_t(q) * a.ldc + at, y, n, a.vec);
+    if (a.slope) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < n) a.slope[int64_t(q) * a.p.rows + at + e] = slope[e];
+    }
   } else if constexpr (EPI == kGatedGrad) {
     const int n = a.F - at;
     if (n <= 0) return;
@@ -482,11 +540,33 @@ __device__ inline void grad8(const float (&d)[8], const Pix8& g, const Pix8& u, 
   }
 }
 
+// 8 outputs of the linear layer
+__device__ inline void put_linear8(const TileArgs& a, int q, int at, int n, const float (&d)[8]) {
+  Pix8 r = {{0u, 0u, 0u, 0u}};
+  if (a.res) r = row_vec(a.res + int64_t(q) * a.ldr + at, n);  // (in flight beside the activation)
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = d[e];
+  uint16_t slope[8] = {};
+  linear_values(a, q, at, n, y, slope);
+  if (a.res) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] += __uint_as_float(e & 1 ? r.v[e >> 1] & 0xFFFF0000u : r.v[e >> 1] << 16);
+  }
+  put_vec(a.out + int64_t(q) * a.ldc + at, pack_vec(y), n);
+  if (a.slope) {
+    Pix8 s;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s.v[e] = uint32_t(slope[2 * e]) | uint32_t(slope[2 * e + 1]) << 16;
+    put_vec(a.slope + int64_t(q) * a.p.rows + at, s, n);
+  }
+}
+
 // 8 consecutive outputs of row q from column `at` on (n of them in range): d0, and for the gated
 // forward the up projection d1
 template <int EPI, int ACT>
 __device__ inline void put_row8(const TileArgs& a, int q, int at, int n, const float (&d0)[8], const float (&d1)[8], int split) {
-  if constexpr (EPI == kPlain) {
+  if constexpr (own_rows(EPI)) {
     if (a.part) {
       float* to = a.part + (int64_t(split) * a.q.rows + q) * a.p.rows + at;
       if (n >= 8) {
@@ -499,7 +579,8 @@ __device__ inline void put_row8(const TileArgs& a, int q, int at, int n, const f
         if (e < n) to[e] = d0[e];
       return;
     }
-    put_vec(a.out + int64_t(q) * a.ldc + at, pack_vec(d0), n);
+    if constexpr (EPI == kLinear) put_linear8(a, q, at, n, d0);
+    else put_vec(a.out + int64_t(q) * a.ldc + at, pack_vec(d0), n);
   } else if constexpr (EPI == kGatedGrad) {
     Pix8 g, u;
     Bytes8 low;
@@ -522,7 +603,7 @@ __device__ inline void put_row8(const TileArgs& a, int q, int at, int n, const f
 template <bool WIDE, bool PROWS, bool QROWS, int EPI, int ACT>
 __device__ inline void tile_block(const TileArgs& a, const TileAt tile) {
   using C = Tile<WIDE>;
-  constexpr bool GATED = EPI == kGated || EPI == kGatedKeep;
+  constexpr bool GATED = gated_epi(EPI);
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];  // [2 buffers][P, Q]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wp = WIDE ? wave & 1 : 0, wq = WIDE ? wave >> 1 : wave & 1, wk = WIDE ? 0 : wave >> 1;
@@ -532,8 +613,8 @@ __device__ inline void tile_block(const TileArgs& a, const TileAt tile) {
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) acc[i][j] = zero_acc();
-  const int kbeg = EPI == kPlain && a.part ? tile.z * a.k_split : 0;
-  const int klen = (EPI == kPlain && a.part ? min(a.K, kbeg + a.k_split) : a.K) - kbeg;
+  const int kbeg = own_rows(EPI) && a.part ? tile.z * a.k_split : 0;
+  const int klen = (own_rows(EPI) && a.part ? min(a.K, kbeg + a.k_split) : a.K) - kbeg;
   TileLoads<WIDE, PROWS, GATED> lp;
   TileLoads<WIDE, QROWS, false> lq;
   lp.plan(a, a.p, p0, kbeg, tid);
@@ -654,7 +735,7 @@ __device__ inline void tile_block(const TileArgs& a, const TileAt tile) {
   // rows in windows of 8 outputs, consecutive threads along a row
   constexpr int kAcross = (GATED ? C::T / 2 : C::T) / 8;
   const int o = tid % kAcross;
-  const int at = (GATED ? p0 / 2 : p0) + 8 * o, n = (EPI == kPlain ? a.p.rows : a.F) - at;
+  const int at = (GATED ? p0 / 2 : p0) + 8 * o, n = (own_rows(EPI) ? a.p.rows : a.F) - at;
   const float* from = block + (GATED ? (o >> 2) * 64 + (o & 3) * 8 : 8 * o);
   if (n <= 0) return;
 #pragma unroll 2
@@ -729,6 +810,106 @@ __global__ __launch_bounds__(256) void tile_join_kernel(TileArgs a, int splits) 
   }
 }
 
+// The same for the linear layer: a thread per window of 8 outputs of a row.
+__global__ __launch_bounds__(256) void linear_join_kernel(TileArgs a, int splits) {
+  const int windows = (a.p.rows + 7) / 8;
+  const int64_t total = int64_t(a.q.rows) * windows, plane = int64_t(a.q.rows) * a.p.rows;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+    const int q = int(i / windows), at = int(i - int64_t(q) * windows) * 8, n = min(a.p.rows - at, 8);
+    const float* from = a.part + int64_t(q) * a.p.rows + at;
+    float d[8] = {};
+    for (int z = 0; z < splits; z += 4) {
+      Floats4 v[4][2];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float* p = from + int64_t(min(z + u, splits - 1)) * plane;
+        if (n == 8) {
+          v[u][0] = *reinterpret_cast<const Floats4*>(p);
+          v[u][1] = *reinterpret_cast<const Floats4*>(p + 4);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[u][e >> 2].v[e & 3] = e < n ? p[e] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (z + u < splits) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] += v[u][e >> 2].v[e & 3];
+        }
+    }
+    put_linear8(a, q, at, n, d);
+  }
+}
+
+// dp = dy act'(v) from the kept slopes (null: 1), rounded once, and the column sums of the products
+// before that rounding, for the bias: a workgroup takes 256 columns of every gridDim.y-th 8 rows, 32
+// threads of 8 columns a row, and writes its sums as partials [gridDim.y][N].
+struct LinearBwdArgs {
+  const uint16_t* dy;     // [M][N], row stride ld
+  int64_t ld;
+  const uint16_t* slope;  // dense
+  uint16_t* dp;           // dense, or null
+  float* part;            // or null
+  int M, N;
+};
+
+__global__ __launch_bounds__(256) void linear_bwd_kernel(LinearBwdArgs a) {
+  __shared__ float red[8][256];
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int at = blockIdx.x * 256 + lane * 8, n = min(a.N - at, 8);
+  float sum[8] = {};
+  if (n > 0) {
+    const int step = gridDim.y * 8;
+    for (int64_t q0 = int64_t(blockIdx.y) * 8 + row; q0 < a.M; q0 += 4 * int64_t(step)) {
+      Pix8 d[4], k[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {  // (rows past the end: the last one again, unused)
+        const int64_t q = min(q0 + int64_t(u) * step, int64_t(a.M - 1));
+        d[u] = row_vec(a.dy + q * a.ld + at, n);
+        if (a.slope) k[u] = row_vec(a.slope + q * a.N + at, n);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t q = q0 + int64_t(u) * step;
+        if (q >= a.M) break;
+        float g[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          g[e] = __uint_as_float(e & 1 ? d[u].v[e >> 1] & 0xFFFF0000u : d[u].v[e >> 1] << 16);
+          if (a.slope) g[e] *= float(__builtin_bit_cast(_Float16, uint16_t(k[u].v[e >> 1] >> (16 * (e & 1))))) * (1.0f / kSlopeScale);
+          sum[e] += g[e];
+        }
+        if (a.dp) put_vec(a.dp + q * a.N + at, pack_vec(g), n);
+      }
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) red[row][lane * 8 + e] = sum[e];
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.N) return;
+  float s = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) s += red[r][threadIdx.x];
+  a.part[int64_t(blockIdx.y) * a.N + c] = s;
+}
+
+// d_bias: the partials in order, 64 columns a workgroup, 16 waves
+__global__ __launch_bounds__(1024) void linear_bias_kernel(const float* part, int parts, int N, uint16_t* d_bias) {
+  __shared__ float red[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
+  red[wave][lane] = c < N ? sum_strided8(0.0f, part + c, N, wave, 16, parts) : 0.0f;
+  __syncthreads();
+  if (wave != 0 || c >= N) return;
+  float s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) s += red[w][lane];
+  d_bias[c] = f32_to_bf16(s);
+}
+
 // ---- few rows -------------------------------------------------------------------------------------
 // A step of decoding: bound by the weights' bytes, which pass once from memory to registers.  A
 // workgroup takes 16 units (their gate and up rows) or `span` plain rows as the rows of 16x16x32
@@ -747,7 +928,7 @@ constexpr int kFewGated = 64, kFewPlain = 16;  // most rows of x
 
 template <int MT, int CH, int EPI, int ACT>
 __global__ __launch_bounds__(512) void few_kernel(TileArgs a) {
-  constexpr bool GATED = EPI == kGated || EPI == kGatedKeep;
+  constexpr bool GATED = gated_epi(EPI);
   constexpr int PT = GATED ? 2 : 1, WAVES = 8, STEP = 32 * CH;
   extern __shared__ __attribute__((aligned(16))) float4 red[];  // [wave][PT][MT][lane]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -875,7 +1056,8 @@ template <bool PROWS, int EPI, int ACT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void gated_large_kernel(TileArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
-  constexpr bool GATED = EPI != kGatedGrad;
+  constexpr bool GATED = gated_epi(EPI);
+  const int units = EPI == kLinear ? a.p.rows : a.F;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave & 1, wn = wave >> 1;
   const TileAt tile = tile_at(a, int(blockIdx.x), int(gridDim.x));
@@ -884,7 +1066,8 @@ void gated_large_kernel(TileArgs a) {
   {
     G5Operand op;
     if constexpr (GATED) op = gated_operand(a, f0, tid);
-    else op = g5_operand<kAlongRow, true>(a.p.src, 1, a.p.ld, f0, a.F, a.K, tid);
+    else if constexpr (PROWS) op = g5_operand<kAlongRow, true>(a.p.src, 1, a.p.ld, f0, units, a.K, tid);
+    else op = g5_operand<kAlongK, true>(a.p.src, a.p.ld, 1, f0, units, a.K, tid);
     const G5Operand oq = g5_operand<kAlongK, true>(a.q.src, a.q.ld, 1, q0, a.q.rows, a.K, tid);
     gemm6_loop<kDmaMode<PROWS>, kAlongK>(acc, op, oq, smem, 0, a.K, tid);
   }
@@ -914,6 +1097,14 @@ void gated_large_kernel(TileArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[e] = at[r * kEpiPitch + e], u[e] = at[r * kEpiPitch + 16 + e];
         if (row(r) < a.q.rows && f < a.F) put_row8<EPI, ACT>(a, row(r), f, 8, g, u, 0);
+      }
+    } else if constexpr (EPI == kLinear) {
+#pragma unroll 2
+      for (int r = rr; r < kEpiRows; r += kRound) {
+        float d[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = epi[r * kEpiPitch + 8 * o + e];
+        if (row(r) < a.q.rows && f < units) put_linear8(a, row(r), f, min(units - f, 8), d);
       }
     } else {
       // four rows' [g u] in flight: clamped addresses, no branch around the loads
@@ -1004,7 +1195,7 @@ bool launch_tile(TileArgs a, dim3 tiles, hipStream_t st) {
 
 template <int MT, int CH, int EPI, int ACT>
 bool launch_few(TileArgs a, hipStream_t st) {
-  constexpr bool GATED = EPI == kGated || EPI == kGatedKeep;
+  constexpr bool GATED = gated_epi(EPI);
   constexpr size_t lds = size_t(8) * (GATED ? 2 : 1) * MT * 1024;
   static_assert(lds <= 65536, "the waves' sums fit the LDS a launch has without asking");
   int span = CH > 1 ? 4 : 16;
@@ -1017,7 +1208,7 @@ bool launch_few(TileArgs a, hipStream_t st) {
 }
 
 // k split over the grid into `splits` parts, joined by a second launch
-template <bool WIDE, bool PROWS, bool QROWS>
+template <bool WIDE, bool PROWS, bool QROWS, int EPI>
 bool launch_split(TileArgs a, dim3 tiles, int64_t splits, hipStream_t st) {
   constexpr int kt = Tile<WIDE>::KT;
   a.k_split = int(ceil_div(ceil_div(a.K, kt), splits)) * kt;
@@ -1025,8 +1216,11 @@ bool launch_split(TileArgs a, dim3 tiles, int64_t splits, hipStream_t st) {
   const int64_t n = int64_t(a.p.rows) * a.q.rows;
   a.part = static_cast<float*>(xdna_hip_cache_alloc(size_t(tiles.z) * size_t(n) * sizeof(float)));
   if (!a.part) return false;
-  const bool ok = launch_tile<WIDE, PROWS, QROWS, kPlain, kSilu>(a, tiles, st);
-  if (ok) tile_join_kernel<<<unsigned(std::min<int64_t>(ceil_div(n, int64_t(1024)), 4096)), 256, 0, st>>>(a, int(tiles.z));
+  const bool ok = launch_tile<WIDE, PROWS, QROWS, EPI, kSilu>(a, tiles, st);
+  if (ok && EPI == kLinear)
+    linear_join_kernel<<<unsigned(std::min<int64_t>(ceil_div(int64_t(a.q.rows) * ceil_div(a.p.rows, 8), int64_t(256)), 4096)), 256, 0, st>>>(
+        a, int(tiles.z));
+  else if (ok) tile_join_kernel<<<unsigned(std::min<int64_t>(ceil_div(n, int64_t(1024)), 4096)), 256, 0, st>>>(a, int(tiles.z));
   xdna_hip_cache_free(a.part);  // stream-ordered reuse: the block's next user runs after the join
   return ok;
 }
@@ -1078,7 +1272,7 @@ bool launch_tiles(const TileArgs& a, hipStream_t st) {
   constexpr int side = EPI == kGated || EPI == kGatedKeep ? 2 : 1;  // tile rows per unit of p
   const auto tiles = [&](int t) { return dim3(unsigned(ceil_div(int64_t(a.p.rows) * side, t)), unsigned(ceil_div(a.q.rows, t))); };
   if constexpr (!PROWS && !QROWS) {
-    if constexpr (EPI == kPlain) {
+    if constexpr (own_rows(EPI)) {
       // chunks of k where k is long or the weight's rows are few: 4096 rows of 1024 take 4.1 us
       // without them and 6.0 with (a step per wave), 1024 rows of 4096 6.7 and 4.2
       if (a.q.rows <= 4 && (a.K >= 2048 || a.p.rows <= 2048)) return launch_few<1, 4, EPI, ACT>(a, st);
@@ -1089,11 +1283,11 @@ bool launch_tiles(const TileArgs& a, hipStream_t st) {
       if (a.q.rows <= kFewGated) return launch_few<4, 1, EPI, ACT>(a, st);
     }
   }
-  const TileChoice c = choose_tiles(int64_t(a.p.rows) * side, a.q.rows, a.K, EPI == kPlain);
+  const TileChoice c = choose_tiles(int64_t(a.p.rows) * side, a.q.rows, a.K, own_rows(EPI));
   const dim3 t = tiles(c.wide ? 128 : 64);
-  if constexpr (EPI == kPlain) {
+  if constexpr (own_rows(EPI)) {
     if (c.splits > 1)
-      return c.wide ? launch_split<true, PROWS, QROWS>(a, t, c.splits, st) : launch_split<false, PROWS, QROWS>(a, t, c.splits, st);
+      return c.wide ? launch_split<true, PROWS, QROWS, EPI>(a, t, c.splits, st) : launch_split<false, PROWS, QROWS, EPI>(a, t, c.splits, st);
   }
   return c.wide ? launch_tile<true, PROWS, QROWS, EPI, ACT>(a, t, st) : launch_tile<false, PROWS, QROWS, EPI, ACT>(a, t, st);
 }
@@ -1103,9 +1297,10 @@ bool launch_tiles(const TileArgs& a, hipStream_t st) {
 // 4096 units; 10 % off in the mean): narrow tiles, wide tiles or apart by it, their geometric mean is
 // 13.6 us, always apart 23.6.  333 x 1000 -> 1367: 23.2 narrow, 35.7 wide, 37.5 apart; 1628 x 723 ->
 // 1767: 71.4, 61.0, 82.7; 143 x 308 -> 3370 (53 k-tiles for 15 tiles of dx): 33.0, 70.6, 27.1.
-float grads_cost(bool wide, int64_t M, int64_t K, int64_t F, int64_t N) {
-  const int64_t n_dx = tile_count(wide, K, M), n_w = tile_count(wide, K, 2 * F) + (N ? tile_count(wide, F, N) : 0);
-  const float k_dx = float(k_tiles(wide, 2 * F)), k_w = float(k_tiles(wide, M));
+// `units`: rows of the input weight (2F, or the linear layer's).
+float grads_cost(bool wide, int64_t M, int64_t K, int64_t units, int64_t F, int64_t N) {
+  const int64_t n_dx = tile_count(wide, K, M), n_w = tile_count(wide, K, units) + (N ? tile_count(wide, F, N) : 0);
+  const float k_dx = float(k_tiles(wide, units)), k_w = float(k_tiles(wide, M));
   const auto tile = [&](float k) { return wide ? 1.05f * k + 1.5f : 1.48f * k + 1.3f; };
   const float work = (float(n_dx) * tile(k_dx) + float(n_w) * tile(k_w)) / 512.0f, k = std::max(k_dx, k_w);
   return wide ? 4.0f + std::max(work, 0.73f * k + 1.1f) : 5.3f + std::max(work, 0.56f * k - 1.0f);
@@ -1155,11 +1350,12 @@ bool launch_large(TileArgs a, dim3 tiles, hipStream_t st) {
 // and 57.
 template <int EPI, bool PROWS, int ACT>
 bool launch_sized(const TileArgs& a, hipStream_t st) {
-  constexpr bool GATED = EPI != kGatedGrad;
-  const dim3 grid(unsigned(ceil_div(a.F, GATED ? kT4 / 2 : kT4)), unsigned(ceil_div(a.q.rows, kT4)));
+  constexpr bool GATED = gated_epi(EPI);
+  const int64_t units = EPI == kLinear ? a.p.rows : a.F;
+  const dim3 grid(unsigned(ceil_div(units, GATED ? kT4 / 2 : kT4)), unsigned(ceil_div(a.q.rows, kT4)));
   const int64_t n = int64_t(grid.x) * grid.y;
-  const bool large = n >= 256 && 100 * n >= 65 * 256 * ceil_div(n, int64_t(256)) && a.K % 8 == 0 && a.F % 8 == 0 && aligned16(a.out) && aligned16(a.gu) &&
-                     dma_ok(a.p, GATED ? 2 * int64_t(a.F) : a.F, a.K, PROWS) && dma_ok(a.q, a.q.rows, a.K, false);
+  const bool large = n >= 256 && 100 * n >= 65 * 256 * ceil_div(n, int64_t(256)) && a.K % 8 == 0 && (EPI == kLinear || (a.F % 8 == 0 && aligned16(a.out) && aligned16(a.gu))) &&
+                     dma_ok(a.p, GATED ? 2 * units : units, a.K, PROWS) && dma_ok(a.q, a.q.rows, a.K, false);
   return large ? launch_large<PROWS, EPI, ACT>(a, grid, st) : launch_tiles<PROWS, false, EPI, ACT>(a, st);
 }
 
@@ -1180,6 +1376,34 @@ TileArgs kept_args(int64_t M, int64_t F, const void* gu, uint16_t* out) {
   a.low = reinterpret_cast<uint8_t*>(a.gu) + M * F * 4;
   a.vec = F % 4 == 0 && aligned8(out) && aligned8(gu) ? 1 : 0;
   return a;
+}
+
+// dx = d w and dw = d^T x of a product x w^T with `units` rows of w
+GradsArgs input_grads(const uint16_t* d, int64_t ldd, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw,
+                      int64_t M, int64_t K, int64_t units, uint16_t* dx, uint16_t* dw) {
+  GradsArgs g = {};
+  g.dx.p = {w, ldw, int(K)};
+  g.dx.q = {d, ldd, int(M)};
+  g.dx.K = int(units);
+  g.dx.out = dx;
+  g.dx.ldc = K;
+  g.dw_in.p = {x, M > 1 ? ldx : K, int(K)};
+  g.dw_in.q = {d, ldd, int(units)};
+  g.dw_in.K = int(M);
+  g.dw_in.out = dw;
+  g.dw_in.ldc = K;
+  return g;
+}
+
+const char* linear_fault(int64_t M, int64_t K, int64_t N) {
+  if (M < 0 || M > kMaxRows || K < 1 || K > kMaxSide || N < 1 || N > kMaxSide) return "sizes out of range";
+  return M * N > kMaxOutputs ? "too many outputs" : nullptr;
+}
+
+// Row slices of the column sums: enough workgroups for the chip (four a CU), 32 rows a slice at least.
+int64_t linear_parts(int64_t M, int64_t N) {
+  if (M <= 0) return 0;
+  return std::max<int64_t>(1, std::min(ceil_div(int64_t(1024), ceil_div(N, int64_t(256))), ceil_div(M, int64_t(32))));
 }
 
 int launched(const char* what, bool ok) {
@@ -1261,7 +1485,7 @@ int xdna_gated_grads_pick(int64_t M, int64_t K, int64_t F, int64_t N) {
   if (gated_fault(M, K, F, 0) || M == 0 || N < 0 || N > kMaxRows || F > kMaxRows / 2) return 0;
   const float apart = choose_tiles(K, M, 2 * F, true).cost + choose_tiles(K, 2 * F, M, true).cost +
                       (N ? choose_tiles(F, N, M, true).cost : 0.0f);
-  return std::min(grads_cost(false, M, K, F, N), grads_cost(true, M, K, F, N)) < apart ? 1 : 0;
+  return std::min(grads_cost(false, M, K, 2 * F, F, N), grads_cost(true, M, K, 2 * F, F, N)) < apart ? 1 : 0;
 }
 
 int xdna_gated_grads_bf16(const uint16_t* dgu, const uint16_t* x, int64_t ldx, const uint16_t* w_in, int64_t ldw,
@@ -1277,18 +1501,7 @@ int xdna_gated_grads_bf16(const uint16_t* dgu, const uint16_t* x, int64_t ldx, c
   if (odd(dgu) || odd(x) || odd(w_in) || odd(dy) || odd(h) || odd(dx) || odd(dw_in) || odd(dw_out))
     return refuse(what, "misaligned operand");
   if (!admit_launch(what)) return -1;
-  GradsArgs g = {};
-  g.dx.p = {w_in, ldw, int(K)};
-  g.dx.q = {dgu, 2 * F, int(M)};
-  g.dx.K = int(2 * F);
-  g.dx.out = dx;
-  g.dx.ldc = K;
-  const int64_t lx = M > 1 ? ldx : K;
-  g.dw_in.p = {x, lx, int(K)};
-  g.dw_in.q = {dgu, 2 * F, int(2 * F)};
-  g.dw_in.K = int(M);
-  g.dw_in.out = dw_in;
-  g.dw_in.ldc = K;
+  GradsArgs g = input_grads(dgu, 2 * F, x, ldx, w_in, ldw, M, K, 2 * F, dx, dw_in);
   if (N > 0) {
     g.dw_out.p = {h, F, int(F)};
     g.dw_out.q = {dy, M > 1 ? lddy : N, int(N)};
@@ -1296,7 +1509,78 @@ int xdna_gated_grads_bf16(const uint16_t* dgu, const uint16_t* x, int64_t ldx, c
     g.dw_out.out = dw_out;
     g.dw_out.ldc = F;
   }
-  const bool wide = grads_cost(true, M, K, F, N) < grads_cost(false, M, K, F, N);
+  const bool wide = grads_cost(true, M, K, 2 * F, F, N) < grads_cost(false, M, K, 2 * F, F, N);
+  hipStream_t st = as_stream(stream);
+  return launched(what, wide ? launch_grads<true>(g, st) : launch_grads<false>(g, st));
+}
+
+int xdna_linear_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t M, int64_t K, int64_t N, int act,
+                     const uint16_t* bias, const uint16_t* residual, int64_t ldr, uint16_t* y, uint16_t* slope, void* stream) {
+  const char* what = "xdna_linear_bf16";
+  if (const char* why = linear_fault(M, K, N)) return refuse(what, why);
+  if (act < 0 || act > 3) return refuse(what, "activation must be 0 (silu), 1 (gelu), 2 (relu) or 3 (none)");
+  if ((M > 1 && (ldx < K || (residual && ldr < N))) || (ldw < K && N > 1)) return refuse(what, "rows overlap");
+  if (M == 0) return 0;
+  if (!x || !w || !y) return refuse(what, "null operand");
+  if (slope && act == 3) return refuse(what, "no activation has no slopes");
+  if (odd(x) || odd(w) || odd(bias) || odd(residual) || odd(y) || odd(slope)) return refuse(what, "misaligned operand");
+  if (!admit_launch(what)) return -1;
+  TileArgs a = {};
+  a.p = {w, N > 1 ? ldw : K, int(N)};
+  a.q = {x, M > 1 ? ldx : K, int(M)};
+  a.K = int(K);
+  a.out = y;
+  a.ldc = N;
+  a.vec = N % 4 == 0 && aligned8(y) ? 1 : 0;
+  a.act = act;
+  a.bias = bias;
+  a.res = residual;
+  a.ldr = M > 1 ? ldr : N;
+  a.slope = slope;
+  return launched(what, launch_sized<kLinear, false, kSilu>(a, as_stream(stream)));
+}
+
+size_t xdna_linear_bwd_workspace_bytes(int64_t M, int64_t N) {
+  return linear_fault(M, 1, N) ? 0 : size_t(linear_parts(M, N)) * size_t(N) * sizeof(float);
+}
+
+int xdna_linear_bwd_bf16(const uint16_t* dy, int64_t ld, const uint16_t* slope, int64_t M, int64_t N, uint16_t* dp,
+                         uint16_t* d_bias, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "xdna_linear_bwd_bf16";
+  if (const char* why = linear_fault(M, 1, N)) return refuse(what, why);
+  if (ld < N && M > 1) return refuse(what, "rows overlap");
+  if (M > 0 && !dy) return refuse(what, "null operand");
+  if (odd(dy) || odd(slope) || odd(dp) || odd(d_bias)) return refuse(what, "misaligned operand");
+  if (d_bias && M > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < xdna_linear_bwd_workspace_bytes(M, N)))
+    return refuse(what, "workspace missing, misaligned or too small");
+  if ((M == 0 || !dp) && !d_bias) return 0;
+  if (!admit_launch(what)) return -1;
+  hipStream_t st = as_stream(stream);
+  LinearBwdArgs a = {dy, M > 1 ? ld : N, slope, dp, d_bias ? static_cast<float*>(workspace) : nullptr, int(M), int(N)};
+  const int64_t parts = linear_parts(M, N);
+  if (M > 0) linear_bwd_kernel<<<dim3(unsigned(ceil_div(N, int64_t(256))), unsigned(parts)), 256, 0, st>>>(a);
+  if (d_bias) linear_bias_kernel<<<unsigned(ceil_div(N, int64_t(64))), 1024, 0, st>>>(a.part, int(parts), int(N), d_bias);
+  return check_launch(what);
+}
+
+int xdna_linear_grads_pick(int64_t M, int64_t K, int64_t N) {
+  if (linear_fault(M, K, N) || M == 0 || N > kMaxRows) return 0;
+  const float apart = choose_tiles(K, M, N, true).cost + choose_tiles(K, N, M, true).cost;
+  return std::min(grads_cost(false, M, K, N, 0, 0), grads_cost(true, M, K, N, 0, 0)) < apart ? 1 : 0;
+}
+
+int xdna_linear_grads_bf16(const uint16_t* dp, int64_t lddp, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw,
+                           int64_t M, int64_t K, int64_t N, uint16_t* dx, uint16_t* dw, void* stream) {
+  const char* what = "xdna_linear_grads_bf16";
+  if (const char* why = linear_fault(M, K, N)) return refuse(what, why);
+  if (M == 0) return refuse(what, "no rows");
+  if (N > kMaxRows || N * K > kMaxOutputs || M * K > kMaxOutputs) return refuse(what, "sizes out of range");
+  if ((M > 1 && (lddp < N || ldx < K)) || (ldw < K && N > 1)) return refuse(what, "rows overlap");
+  if (!dp || !x || !w || !dx || !dw) return refuse(what, "null operand");
+  if (odd(dp) || odd(x) || odd(w) || odd(dx) || odd(dw)) return refuse(what, "misaligned operand");
+  if (!admit_launch(what)) return -1;
+  const GradsArgs g = input_grads(dp, M > 1 ? lddp : N, x, ldx, w, N > 1 ? ldw : K, M, K, N, dx, dw);
+  const bool wide = grads_cost(true, M, K, N, 0, 0) < grads_cost(false, M, K, N, 0, 0);
   hipStream_t st = as_stream(stream);
   return launched(what, wide ? launch_grads<true>(g, st) : launch_grads<false>(g, st));
 }

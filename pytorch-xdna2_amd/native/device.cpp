@@ -797,4 +797,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("token_gated_mlp", &token_gated_mlp);
   mod.def("token_distill", &token_distill);
   mod.def("token_log_probs", &token_log_probs);
+  mod.def("token_layer_norm", &token_layer_norm);
+  mod.def("token_linear", &token_linear);
+  mod.def("token_decay", &token_decay);
+  mod.def("token_decay_step", &token_decay_step);
 }

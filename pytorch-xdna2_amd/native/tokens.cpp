@@ -1,6 +1,7 @@
 // Host side of the token-model operators (xdna_train/tokens.py): checks, workspaces, C-ABI
-// calls and autograd nodes of the embedding, the gated feed-forward, the distillation loss
-// and the token log probabilities (csrc/embed.hip, gated.hip, vocab.hip).  No call reads
+// calls and autograd nodes of the embedding, the gated feed-forward, the distillation loss,
+// the token log probabilities, layer norm, the linear layer and decay attention
+// (csrc/embed.hip, gated.hip, vocab.hip, layer_norm.hip, decay.hip).  No call reads
 // device data on the host, so all of them can be captured in a graph.
 #include "xdna.h"
 
@@ -451,6 +452,288 @@ struct LogprobFn : public torch::autograd::Function<LogprobFn> {
   }
 };
 
+// ---- layer norm ------------------------------------------------------------------------------------
+// A tensor that a call leaves out is undefined here and an empty optional to its node, which has no
+// edge for it: whether argument `i` of those that are there gets a gradient is asked by its place among them.
+std::optional<at::Tensor> given(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
+
+struct Wanted {
+  AutogradContext* ctx;
+  size_t next = 0;
+  bool operator()(bool there) { return there && ctx->needs_input_grad(next++); }
+};
+
+int param_code(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias) {
+  const at::Tensor& p = weight.defined() ? weight : bias;
+  return (p.defined() ? p : x).scalar_type() == at::kFloat ? 1 : 2;
+}
+
+struct NormForward {
+  at::Tensor y, sum, stats;  // sum: undefined without a residual
+};
+
+NormForward norm_forward(const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight, const at::Tensor& bias,
+                         double eps, bool keep) {
+  ScopedCount sc("hip_tokens.norm.fwd.run");
+  NormForward r;
+  const at::Tensor xr = as_rows(x), rr = residual.defined() ? as_rows(residual) : residual;
+  const at::Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+  r.y = empty_xdna(x.sizes(), x.scalar_type());
+  if (residual.defined()) r.sum = empty_xdna(x.sizes(), x.scalar_type());
+  if (keep) r.stats = empty_xdna({xr.size(0), 2}, at::kFloat);
+  check_abi(xdna_layer_norm(cptr(xr), row_stride(xr), cptr(rr), rr.defined() ? row_stride(rr) : 0,
+                            xr.scalar_type() == at::kFloat ? 1 : 2, xr.size(0), xr.size(1), cptr(w), cptr(b),
+                            param_code(x, w, b), float(eps), ptr_or_null(r.sum), ptr_or_null(r.y),
+                            static_cast<float*>(ptr_or_null(r.stats)), current_stream()),
+            "layer_norm");
+  return r;
+}
+
+struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& residual_,
+                               const std::optional<at::Tensor>& weight_, const std::optional<at::Tensor>& bias_, double eps) {
+    const at::Tensor residual = residual_.value_or(at::Tensor()), weight = weight_.value_or(at::Tensor()),
+                     bias = bias_.value_or(at::Tensor());
+    const NormForward f = norm_forward(x, residual, weight, bias, eps, true);
+    // the sum goes through a detached alias: as an output it carries this node
+    ctx->save_for_backward({residual.defined() ? f.sum.detach() : x, weight, bias, f.stats});
+    ctx->saved_data["add"] = residual.defined();
+    ctx->set_materialize_grads(false);
+    if (residual.defined()) return {f.y, f.sum};
+    return {f.y};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("layer_norm");
+    variable_list none(5);
+    const at::Tensor dsum = grads.size() > 1 ? grads[1] : at::Tensor();
+    const auto saved = ctx->get_saved_variables();
+    Wanted wanted{ctx};
+    const bool want_x = wanted(true), want_r = wanted(ctx->saved_data["add"].toBool()), want_w = wanted(saved[1].defined()),
+               want_b = wanted(saved[2].defined());
+    if (!grads[0].defined()) {  // the norm has no gradient, the sum may have one
+      if (want_x) none[0] = dsum;
+      if (want_r) none[1] = dsum;
+      return none;
+    }
+    ScopedCount sc("hip_tokens.norm.bwd.run");
+    const at::Tensor x = as_rows(saved[0]), dy = as_rows(grads[0]), ds = dsum.defined() ? as_rows(dsum) : dsum;
+    const at::Tensor w = saved[1].defined() ? saved[1].contiguous() : saved[1];
+    const int64_t R = x.size(0), D = x.size(1);
+    const int pt = param_code(x, saved[1], saved[2]);
+    const at::ScalarType ptype = pt == 1 ? at::kFloat : at::kBFloat16;
+    at::Tensor dx, dw, db, ws;
+    if (want_x || want_r) dx = empty_xdna(saved[0].sizes(), x.scalar_type());
+    if (want_w) dw = empty_xdna({D}, ptype);
+    if (want_b) db = empty_xdna({D}, ptype);
+    const size_t bytes = dw.defined() || db.defined() ? xdna_layer_norm_bwd_workspace_bytes(R, D) : 0;
+    if (bytes) ws = workspace(bytes);
+    check_abi(xdna_layer_norm_bwd(cptr(dy), row_stride(dy), cptr(ds), ds.defined() ? row_stride(ds) : 0, cptr(x), row_stride(x),
+                                  x.scalar_type() == at::kFloat ? 1 : 2, R, D, cptr(w), pt, cf32(saved[3]), ptr_or_null(dx),
+                                  ptr_or_null(dw), ptr_or_null(db), ptr_or_null(ws), bytes, current_stream()),
+              "layer_norm backward");
+    if (want_x) none[0] = dx;
+    if (want_r) none[1] = dx;
+    none[2] = dw;
+    none[3] = db;
+    return none;
+  }
+};
+
+// ---- linear layer ------------------------------------------------------------------------------------
+
+constexpr int64_t kNoActivation = 3;
+
+struct LinearForward {
+  at::Tensor y, slope;  // slope: undefined where not kept
+};
+
+LinearForward linear_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, const at::Tensor& residual,
+                             int64_t act, bool keep) {
+  ScopedCount sc("hip_tokens.linear.fwd.run");
+  LinearForward r;
+  const at::Tensor xr = as_rows(x), w = as_rows(weight), b = bias.defined() ? bias.contiguous() : bias;
+  const at::Tensor rr = residual.defined() ? as_rows(residual) : residual;
+  const int64_t M = xr.size(0), K = xr.size(1), N = w.size(0);
+  r.y = empty_xdna(with_last(x, N), at::kBFloat16);
+  if (keep && act != kNoActivation) r.slope = empty_xdna({M, N}, at::kShort);
+  check_abi(xdna_linear_bf16(p16(xr), row_stride(xr), p16(w), row_stride(w), M, K, N, int(act),
+                             static_cast<const uint16_t*>(cptr(b)), static_cast<const uint16_t*>(cptr(rr)),
+                             rr.defined() ? row_stride(rr) : 0, static_cast<uint16_t*>(ptr_or_null(r.y)),
+                             static_cast<uint16_t*>(ptr_or_null(r.slope)), current_stream()),
+            "linear");
+  return r;
+}
+
+struct LinearFn : public torch::autograd::Function<LinearFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                            const std::optional<at::Tensor>& bias_, const std::optional<at::Tensor>& residual_, int64_t act) {
+    const at::Tensor bias = bias_.value_or(at::Tensor()), residual = residual_.value_or(at::Tensor());
+    // only the gradient of what comes before the activation takes its slopes
+    const auto wants = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
+    const LinearForward f = linear_forward(x, weight, bias, residual, act, wants(x) || wants(weight) || wants(bias));
+    ctx->save_for_backward({x, weight, f.slope});
+    ctx->saved_data["bias"] = bias.defined();
+    ctx->saved_data["residual"] = residual.defined();
+    return f.y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("linear");
+    variable_list out(5);
+    if (!grads[0].defined()) return out;
+    Wanted wanted{ctx};
+    const bool want_x = wanted(true), want_w = wanted(true), want_b = wanted(ctx->saved_data["bias"].toBool());
+    if (wanted(ctx->saved_data["residual"].toBool())) out[3] = grads[0];
+    if (!want_x && !want_w && !want_b) return out;
+    ScopedCount sc("hip_tokens.linear.bwd.run");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor x = as_rows(saved[0]), w = as_rows(saved[1]), dy = as_rows(grads[0]), &slope = saved[2];
+    const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+    at::Tensor dp = dy, db, ws;
+    if (slope.defined() && (want_x || want_w)) dp = empty_xdna({M, N}, at::kBFloat16);
+    if (want_b) db = empty_xdna({N}, at::kBFloat16);
+    if (slope.defined() || want_b) {
+      const size_t bytes = want_b ? xdna_linear_bwd_workspace_bytes(M, N) : 0;
+      if (bytes) ws = workspace(bytes);
+      check_abi(xdna_linear_bwd_bf16(p16(dy), row_stride(dy), static_cast<const uint16_t*>(ptr_or_null(slope)), M, N,
+                                     slope.defined() && (want_x || want_w) ? static_cast<uint16_t*>(ptr_or_null(dp)) : nullptr,
+                                     static_cast<uint16_t*>(ptr_or_null(db)), ptr_or_null(ws), bytes, current_stream()),
+                "linear backward");
+      out[2] = db;
+    }
+    if (want_x && want_w && M > 0 && xdna_linear_grads_pick(M, K, N) &&
+        (short_block(M, K, N, 0) || !(on_gemm(dp, w) || on_gemm(dp.t(), x)))) {
+      at::Tensor dx = empty_xdna({M, K}, at::kBFloat16), dw = empty_xdna({N, K}, at::kBFloat16);
+      check_abi(xdna_linear_grads_bf16(p16(dp), row_stride(dp), p16(x), row_stride(x), p16(w), row_stride(w), M, K, N, m16(dx),
+                                       m16(dw), current_stream()),
+                "linear backward");
+      out[0] = dx.view(saved[0].sizes());
+      out[1] = dw;
+      return out;
+    }
+    if (want_x) out[0] = product(dp, w).view(saved[0].sizes());
+    if (want_w) out[1] = product(dp.t(), x);
+    return out;
+  }
+};
+
+// ---- decay attention ---------------------------------------------------------------------------------
+
+// [B, T, H, D] as the C ABI takes it: unit stride along the head, no negative stride (a copy only
+// where the strides are others)
+at::Tensor as_heads(const at::Tensor& t) { return t.size(-1) > 1 && t.stride(-1) != 1 ? t.contiguous() : t; }
+
+xdna_heads_bf16 heads_of(const at::Tensor& t) { return {p16(t), t.stride(0), t.stride(1), t.stride(2)}; }
+
+struct DecaySizes {
+  int64_t B, T, H, G, dk, dv;
+  DecaySizes(const at::Tensor& q, const at::Tensor& v)
+      : B(q.size(0)), T(q.size(1)), H(q.size(2)), G(v.size(2)), dk(q.size(3)), dv(v.size(3)) {}
+  bool none() const { return B == 0 || T == 0; }
+};
+
+int index_size(const at::Tensor& t) { return t.defined() && t.scalar_type() == at::kInt ? 4 : 8; }
+
+struct DecayForward {
+  at::Tensor out, state;
+};
+
+DecayForward decay_forward(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& state_,
+                           const at::Tensor& log_decay, const at::Tensor& lengths, double scale) {
+  ScopedCount sc("hip_tokens.decay.fwd.run");
+  const DecaySizes n(q_, v_);
+  DecayForward r;
+  const at::Tensor q = as_heads(q_), k = as_heads(k_), v = as_heads(v_), state = state_.defined() ? state_.contiguous() : state_;
+  r.out = empty_xdna({n.B, n.T, n.H, n.dv}, at::kBFloat16);
+  r.state = empty_xdna({n.B, n.H, n.dk, n.dv}, at::kFloat);
+  if (n.none()) {
+    if (state.defined()) r.state.copy_(state);
+    else r.state.zero_();
+    return r;
+  }
+  const size_t bytes = xdna_decay_workspace_bytes(n.B, n.T, n.H, n.dk, n.dv);
+  at::Tensor ws;
+  if (bytes) ws = workspace(bytes);
+  const xdna_heads_bf16 hq = heads_of(q), hk = heads_of(k), hv = heads_of(v);
+  check_abi(xdna_decay_attention(&hq, &hk, &hv, n.B, n.T, n.H, n.G, n.dk, n.dv, cf32(log_decay), cptr(lengths),
+                                 index_size(lengths), float(scale), cf32(state), m16(r.out), f32(r.state), ptr_or_null(ws), bytes,
+                                 current_stream()),
+            "decay_attention");
+  return r;
+}
+
+struct DecayFn : public torch::autograd::Function<DecayFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const std::optional<at::Tensor>& state_, const at::Tensor& log_decay,
+                               const std::optional<at::Tensor>& lengths_, double scale) {
+    const at::Tensor state = state_.value_or(at::Tensor()), lengths = lengths_.value_or(at::Tensor());
+    const DecayForward f = decay_forward(q, k, v, state, log_decay, lengths, scale);
+    ctx->save_for_backward({q, k, v, state, log_decay, lengths});
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    return {f.out, f.state};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("decay_attention");
+    variable_list none(7);
+    if (!grads[0].defined() && !grads[1].defined()) return none;
+    ScopedCount sc("hip_tokens.decay.bwd.run");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor q = as_heads(saved[0]), k = as_heads(saved[1]), v = as_heads(saved[2]);
+    const at::Tensor state = saved[3].defined() ? saved[3].contiguous() : saved[3];
+    const at::Tensor &log_decay = saved[4], &lengths = saved[5];
+    const DecaySizes n(q, v);
+    at::Tensor dout = grads[0].defined() ? as_heads(grads[0]) : empty_xdna({n.B, n.T, n.H, n.dv}, at::kBFloat16).zero_();
+    const at::Tensor ds = grads[1].defined() ? grads[1].contiguous() : grads[1];
+    at::Tensor dq = empty_xdna(q.sizes(), at::kBFloat16), dk = empty_xdna(k.sizes(), at::kBFloat16),
+               dv = empty_xdna(v.sizes(), at::kBFloat16), d_state;
+    if (state.defined() && ctx->needs_input_grad(3)) d_state = empty_xdna({n.B, n.H, n.dk, n.dv}, at::kFloat);
+    if (n.none()) {
+      if (d_state.defined() && ds.defined()) d_state.copy_(ds);
+      else if (d_state.defined()) d_state.zero_();
+    } else {
+      const size_t bytes = xdna_decay_bwd_workspace_bytes(n.B, n.T, n.H, n.G, n.dk, n.dv);
+      at::Tensor ws;
+      if (bytes) ws = workspace(bytes);
+      const xdna_heads_bf16 ho = heads_of(dout), hq = heads_of(q), hk = heads_of(k), hv = heads_of(v);
+      check_abi(xdna_decay_attention_bwd(&ho, cf32(ds), &hq, &hk, &hv, n.B, n.T, n.H, n.G, n.dk, n.dv, cf32(log_decay),
+                                         cptr(lengths), index_size(lengths), float(ctx->saved_data["scale"].toDouble()),
+                                         cf32(state), m16(dq), m16(dk), m16(dv), f32(d_state), ptr_or_null(ws), bytes,
+                                         current_stream()),
+                "decay_attention backward");
+    }
+    none[0] = dq;
+    none[1] = dk;
+    none[2] = dv;
+    none[3] = d_state;
+    return none;
+  }
+};
+
+// q, k, v of heads after `lead` dimensions (2: batch, tokens; 1: batch), log_decay and scale
+void check_decay(const char* op, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+                 int64_t lead, double scale) {
+  check_bf16(q, op, "q");
+  check_bf16(k, op, "k");
+  check_bf16(v, op, "v");
+  TORCH_CHECK(q.dim() == lead + 2 && k.dim() == lead + 2 && v.dim() == lead + 2 &&
+                  q.sizes().slice(0, lead) == k.sizes().slice(0, lead) && q.sizes().slice(0, lead) == v.sizes().slice(0, lead),
+              op, ": q, k and v must be [", lead == 2 ? "batch, tokens" : "batch", ", heads, size], got ", q.sizes(), ", ", k.sizes(),
+              " and ", v.sizes());
+  const int64_t H = q.size(lead), G = k.size(lead);
+  TORCH_CHECK(q.size(-1) == k.size(-1), op, ": q and k have heads of ", q.size(-1), " and ", k.size(-1));
+  TORCH_CHECK(q.size(-1) >= 1 && q.size(-1) <= 128 && v.size(-1) >= 1 && v.size(-1) <= 128, op, ": heads of 1 to 128, got ",
+              q.size(-1), " and ", v.size(-1));
+  TORCH_CHECK(G >= 1 && v.size(lead) == G && H >= G && H % G == 0, op, ": k and v must have as many heads, a divisor of q's ", H,
+              ", got ", G, " and ", v.size(lead));
+  TORCH_CHECK(on_xdna(log_decay) && log_decay.scalar_type() == at::kFloat && log_decay.dim() == 1 && log_decay.size(0) == H, op,
+              ": log_decay must be a float32 xdna tensor of ", H, " heads");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && log_decay.requires_grad()), op, ": log_decay is a constant, it gets no gradient");
+  TORCH_CHECK(std::isfinite(float(scale)), op, ": scale must be finite in fp32, got ", scale);
+}
+
 void check_tau(const char* op, double tau) {
   // the kernels divide by tau in base 2: log2(e) / tau has to be a finite fp32 number
   TORCH_CHECK(float(tau) > 0.0f && std::isfinite(float(tau)) && std::isfinite(1.0f / float(tau) * 1.442695041f), op,
@@ -502,6 +785,115 @@ at::Tensor token_gated_mlp(const at::Tensor& x, const at::Tensor& w_in, const at
   ScopedCount sc("hip_tokens.gated.fwd.run");
   const GatedForward f = gated_forward(x, w_in, act, false);
   return product(f.h, as_rows(w_out).t()).view(with_last(x, w_out.size(0)));
+}
+
+std::tuple<at::Tensor, at::Tensor> token_layer_norm(const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                                                    const std::optional<at::Tensor>& weight,
+                                                    const std::optional<at::Tensor>& bias, double eps) {
+  const char* op = residual.has_value() ? "add_layer_norm" : "layer_norm";
+  const at::Tensor r = residual.value_or(at::Tensor()), w = weight.value_or(at::Tensor()), b = bias.value_or(at::Tensor());
+  no_tangents(op, {&x, &r, &w, &b});
+  float_code(x, op, "x");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= (int64_t(1) << 24) && x.numel() / x.size(-1) <= (int64_t(1) << 30),
+              op, ": x must be [..., width], width 1 .. 2^24 and up to 2^30 rows, got ", x.sizes());
+  if (r.defined())
+    TORCH_CHECK(on_xdna(r) && r.scalar_type() == x.scalar_type() && r.sizes() == x.sizes(), op, ": residual must be an xdna tensor like x, ",
+                x.scalar_type(), " ", x.sizes());
+  for (const at::Tensor* p : {&w, &b})
+    TORCH_CHECK(!p->defined() || (on_xdna(*p) && (p->scalar_type() == at::kFloat || p->scalar_type() == x.scalar_type()) &&
+                                  p->dim() == 1 && p->size(0) == x.size(-1)),
+                op, ": weight and bias must be xdna tensors [", x.size(-1), "] of float32 or of x's type");
+  TORCH_CHECK(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(), op, ": weight and bias must be of one type");
+  TORCH_CHECK(float(eps) >= 0.0f && std::isfinite(float(eps)), op, ": eps must be finite and not negative, got ", eps);
+  const auto wants = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
+  if (at::GradMode::is_enabled() && (wants(x) || wants(r) || wants(w) || wants(b))) {
+    const variable_list v = LayerNormFn::apply(x, given(r), given(w), given(b), eps);
+    return {v[0], v.size() > 1 ? v[1] : at::Tensor()};
+  }
+  const NormForward f = norm_forward(x, r, w, b, eps, false);
+  return {f.y, f.sum};
+}
+
+at::Tensor token_linear(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias,
+                        const std::optional<at::Tensor>& residual, int64_t act) {
+  const char* op = "linear";
+  const at::Tensor b = bias.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
+  no_tangents(op, {&x, &weight, &b, &r});
+  check_bf16(x, op, "x");
+  check_bf16(weight, op, "weight");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= (int64_t(1) << 30), op, ": x needs a last dimension");
+  TORCH_CHECK(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(0) <= (int64_t(1) << 22) && weight.size(1) == x.size(-1), op,
+              ": weight must be [units, ", x.size(-1), "], up to 2^22 units, got ", weight.sizes());
+  TORCH_CHECK(x.numel() / x.size(-1) <= (int64_t(1) << 22), op, ": more than 2^22 rows");
+  if (b.defined()) {
+    check_bf16(b, op, "bias");
+    TORCH_CHECK(b.dim() == 1 && b.size(0) == weight.size(0), op, ": bias must be [", weight.size(0), "], got ", b.sizes());
+  }
+  if (r.defined()) {
+    check_bf16(r, op, "residual");
+    const std::vector<int64_t> want = with_last(x, weight.size(0));
+    TORCH_CHECK(r.sizes() == at::IntArrayRef(want), op, ": residual must be ", at::IntArrayRef(want), ", got ", r.sizes());
+  }
+  const auto wants = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
+  if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(b) || wants(r)))
+    return LinearFn::apply(x, weight, given(b), given(r), act);
+  return linear_forward(x, weight, b, r, act, false).y;
+}
+
+std::tuple<at::Tensor, at::Tensor> token_decay(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                               const at::Tensor& log_decay, const std::optional<at::Tensor>& state,
+                                               const std::optional<at::Tensor>& lengths, double scale) {
+  const char* op = "decay_attention";
+  const at::Tensor s = state.value_or(at::Tensor()), l = lengths.has_value() ? lengths->contiguous() : at::Tensor();
+  no_tangents(op, {&q, &k, &v, &log_decay, &s});
+  check_decay(op, q, k, v, log_decay, 2, scale);
+  if (s.defined()) {
+    const std::vector<int64_t> want = {q.size(0), q.size(2), q.size(3), v.size(3)};
+    TORCH_CHECK(on_xdna(s) && s.scalar_type() == at::kFloat && s.sizes() == at::IntArrayRef(want), op,
+                ": state must be a float32 xdna tensor ", at::IntArrayRef(want));
+  }
+  if (l.defined()) {
+    index_bytes(l, op, "lengths");
+    TORCH_CHECK(l.dim() == 1 && l.size(0) == q.size(0), op, ": lengths must be [", q.size(0), "], got ", l.sizes());
+  }
+  const at::Tensor g = log_decay.contiguous();
+  if (tracked({&q, &k, &v}) || (s.defined() && tracked({&s}))) {
+    const variable_list r = DecayFn::apply(q, k, v, given(s), g, given(l), scale);
+    return {r[0], r[1]};
+  }
+  const DecayForward f = decay_forward(q, k, v, s, g, l, scale);
+  return {f.out, f.state};
+}
+
+at::Tensor token_decay_step(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& log_decay,
+                            at::Tensor state, const std::optional<at::Tensor>& slots, double scale) {
+  const char* op = "decay_attention_step";
+  const at::Tensor l = slots.has_value() ? slots->contiguous() : at::Tensor();
+  no_tangents(op, {&q_, &k_, &v_, &log_decay, &state});
+  check_decay(op, q_, k_, v_, log_decay, 1, scale);
+  TORCH_CHECK(!tracked({&q_, &k_, &v_, &state}), op, " writes the state in place and has no gradient: call it under no_grad");
+  const int64_t B = q_.size(0), H = q_.size(1), G = k_.size(1), dk = q_.size(2), dv = v_.size(2);
+  TORCH_CHECK(on_xdna(state) && state.scalar_type() == at::kFloat && state.dim() == 4 && state.is_contiguous() &&
+                  state.size(1) == H && state.size(2) == dk && state.size(3) == dv,
+              op, ": state must be a contiguous float32 xdna tensor [slots, ", H, ", ", dk, ", ", dv, "], got ", state.sizes());
+  if (l.defined()) {
+    index_bytes(l, op, "slots");
+    TORCH_CHECK(l.dim() == 1 && l.size(0) == B, op, ": slots must be [", B, "], got ", l.sizes());
+  } else {
+    TORCH_CHECK(state.size(0) == B, op, ": without slots the states must be the batch's ", B, ", got ", state.size(0));
+  }
+  ScopedCount sc("hip_tokens.decay.step.run");
+  at::Tensor out = empty_xdna({B, H, dv}, at::kBFloat16);
+  if (B == 0) return out;
+  const at::Tensor q = as_heads(q_), k = as_heads(k_), v = as_heads(v_), g = log_decay.contiguous();
+  const auto heads = [](const at::Tensor& t) { return xdna_heads_bf16{p16(t), t.stride(0), 0, t.stride(1)}; };
+  const xdna_heads_bf16 hq = heads(q), hk = heads(k), hv = heads(v);
+  check_abi(xdna_decay_step(&hq, &hk, &hv, B, H, G, dk, dv, cf32(g), static_cast<float*>(ptr_or_null(state)), state.size(0), cptr(l),
+                            index_size(l), float(scale), m16(out), current_stream()),
+            op);
+  bump_write_epoch(state);
+  state.unsafeGetTensorImpl()->bump_version();
+  return out;
 }
 
 at::Tensor token_distill(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher, double tau,

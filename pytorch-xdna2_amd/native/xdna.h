@@ -145,6 +145,17 @@ at::Tensor token_distill(const at::Tensor& logits, const at::Tensor& ids, const 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_log_probs(const at::Tensor& logits,
                                                                            const at::Tensor& targets, int64_t top,
                                                                            double tau);
+// The sum is undefined without a residual.
+std::tuple<at::Tensor, at::Tensor> token_layer_norm(const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                                                    const std::optional<at::Tensor>& weight,
+                                                    const std::optional<at::Tensor>& bias, double eps);
+at::Tensor token_linear(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias,
+                        const std::optional<at::Tensor>& residual, int64_t act);
+std::tuple<at::Tensor, at::Tensor> token_decay(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                               const at::Tensor& log_decay, const std::optional<at::Tensor>& state,
+                                               const std::optional<at::Tensor>& lengths, double scale);
+at::Tensor token_decay_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+                            at::Tensor state, const std::optional<at::Tensor>& slots, double scale);
 
 // Live kernel timing: HIP events around hot-kernel launches on the launch stream,
 // with the algorithmic work (FLOP or bytes) of each launch.

@@ -21,6 +21,16 @@ D = ctypes.c_double
 PP = ctypes.POINTER(ctypes.c_void_p)
 PL = ctypes.POINTER(ctypes.c_int64)
 
+
+
+class Heads(ctypes.Structure):
+    """``xdna_heads_bf16``: device pointer and element strides of a [B, T, H, D] operand."""
+
+    _fields_ = [("data", P), ("batch", L), ("token", L), ("head", L)]
+
+
+PH = ctypes.POINTER(Heads)
+
 # row layouts of the packed conv operands (XDNA_CONV3X3_LAYOUT_*)
 LAYOUT_REF = 0
 LAYOUT_TIGHT = 1
@@ -156,6 +166,19 @@ SIGNATURES = {
     "xdna_distill_workspace_bytes": (Z, [L, L]),
     "xdna_distill": (I, [P, I, L, L, L, P, I, P, I, I, F, P, I, P, P, P, P, P, P, P, Z, P]),
     "xdna_distill_bwd": (I, [P, I, L, L, L, P, I, I, F, P, P, P, P, P, I, I, P, P]),
+    "xdna_layer_norm": (I, [P, L, P, L, I, L, L, P, P, I, F, P, P, P, P]),
+    "xdna_layer_norm_bwd_workspace_bytes": (Z, [L, L]),
+    "xdna_layer_norm_bwd": (I, [P, L, P, L, P, L, I, L, L, P, I, P, P, P, P, P, Z, P]),
+    "xdna_linear_bf16": (I, [P, L, P, L, L, L, L, I, P, P, L, P, P, P]),
+    "xdna_linear_bwd_workspace_bytes": (Z, [L, L]),
+    "xdna_linear_bwd_bf16": (I, [P, L, P, L, L, P, P, P, Z, P]),
+    "xdna_linear_grads_pick": (I, [L, L, L]),
+    "xdna_linear_grads_bf16": (I, [P, L, P, L, P, L, L, L, L, P, P, P]),
+    "xdna_decay_workspace_bytes": (Z, [L] * 5),
+    "xdna_decay_attention": (I, [PH, PH, PH] + [L] * 6 + [P, P, I, F, P, P, P, P, Z, P]),
+    "xdna_decay_bwd_workspace_bytes": (Z, [L] * 6),
+    "xdna_decay_attention_bwd": (I, [PH, P, PH, PH, PH] + [L] * 6 + [P, P, I, F, P, P, P, P, P, P, Z, P]),
+    "xdna_decay_step": (I, [PH, PH, PH] + [L] * 5 + [P, P, L, P, I, F, P, P]),
     "xdna_conv3x3_wgrad_pack_bf16": (I, [P, P, I, I, I, I, I, P, Z, P]),
     "xdna_conv3x3_wgrad_packed_bf16": (I, [P, P, I, I, I, I, I, P, Z, P]),
     "xdna_gemm_set_variant": (I, [I]),

@@ -1,7 +1,9 @@
-"""Operators of token models on the xdna device: the embedding, the gated feed-forward block,
-distillation from a teacher's top logits, and log probabilities of given tokens.
+"""Operators of token models on the xdna device: the embedding, layer norm, the linear layer, linear
+attention with a decay for each head, the gated feed-forward block, distillation from a teacher's top
+logits, and log probabilities of given tokens.
 
-Each is one autograd node over the gfx950 kernels (csrc/embed.hip, gated.hip, vocab.hip); the
+Each is one autograd node over the gfx950 kernels (csrc/embed.hip, layer_norm.hip, gated.hip,
+decay.hip, vocab.hip); the
 reference has no counterpart beyond its zero-copy CPU fallback
 (torch_xdna_device.cpp:5124-5260).  Operands are xdna tensors; nothing falls back: a device,
 dtype or shape that the kernels do not take raises, and ``set_npu_mode`` does not concern them.
@@ -11,7 +13,8 @@ function.  Sums and softmax statistics are fp32 and have a fixed order: equal in
 bits.  The gradients cannot be differentiated again, and an operand with a tangent (forward-mode
 differentiation) raises.
 
-    ids -> embed -> gated_mlp -> head (mm) -> distill_loss / token_log_probs
+    ids -> embed -> blocks -> layer_norm -> head (mm) -> distill_loss / token_log_probs
+    block: layer_norm -> linear -> decay_attention -> linear (residual) -> add_layer_norm -> gated_mlp
 """
 from __future__ import annotations
 
@@ -22,6 +25,7 @@ import torch
 from . import device as _dev
 
 _ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
+_LINEAR_ACTIVATIONS = {**_ACTIVATIONS, "none": 3}
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
@@ -93,3 +97,73 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
     ``temperature``, beside a log probability of -inf.  A row of -inf only has log probabilities of
     -inf, entropy 0 and no gradient."""
     return TokenLogProbs(*_dev.native().token_log_probs(logits, targets, top_k, temperature))
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension (biased variance):
+    ``x`` [..., width] in bf16 or fp32 of any row stride, ``weight`` and ``bias`` [width] in fp32 or
+    ``x``'s type.  fp32 between the loads and one rounding; the gradients of ``weight`` and ``bias``
+    are fp32 sums over the rows in a fixed order."""
+    return _dev.native().token_layer_norm(x, None, weight, bias, eps)[0]
+
+
+class AddLayerNorm(NamedTuple):
+    norm: torch.Tensor  # the norm of the sum
+    sum: torch.Tensor   # x + residual
+
+
+def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                   eps: float = 1e-5) -> AddLayerNorm:
+    """The sum ``x + residual`` (rounded to their type) and its layer norm, in one pass: the bits of
+    ``s = x + residual; layer_norm(s, weight, bias, eps)``.  Both results have gradients."""
+    return AddLayerNorm(*_dev.native().token_layer_norm(x, residual, weight, bias, eps))
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` in one kernel: ``x`` [..., K], ``weight`` [N, K],
+    ``bias`` [N], ``residual`` [..., N], all bf16 (rows of any stride); ``activation`` "none",
+    "silu", "gelu" (with erf) or "relu".  fp32 from the product to the one rounding.  For the backward
+    the activation's slopes are kept in 16 bits (11 of mantissa)."""
+    return _dev.native().token_linear(x, weight, bias, residual, _choice(_LINEAR_ACTIVATIONS, activation, "activation"))
+
+
+class DecayAttention(NamedTuple):
+    out: torch.Tensor    # [batch, tokens, heads, dv] bf16
+    state: torch.Tensor  # [batch, heads, dk, dv] fp32
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor | None = None,
+                    lengths: torch.Tensor | None = None, scale: float | None = None) -> DecayAttention:
+    """Causal linear attention with a decay for each head:
+    ``S_t = exp(log_decay) S_{t-1} + k_t^T v_t``, ``out_t = scale q_t S_t``, for prompts and training.
+
+    ``q`` [batch, tokens, heads, dk], ``k`` [batch, tokens, kv heads, dk], ``v`` [batch, tokens, kv heads,
+    dv] in bf16, heads of 1 to 128, any strides (slices of one projection are not copied); kv heads
+    divide the heads, head ``h`` of ``q`` goes with head ``h // (heads / kv heads)`` of them.  ``log_decay``
+    [heads] fp32, at most 0 (``-inf``: nothing is remembered), a constant.  ``state`` [batch, heads, dk, dv]
+    fp32 is the state before the first token (default: zeros); the returned one is the state behind the
+    last, for the next part of the sequence or ``decay_attention_step``.  ``lengths`` [batch], taken into 0 ..
+    tokens: what lies behind a sequence's end is not read, its ``out`` and gradients are 0.  ``scale`` defaults
+    to ``dk ** -0.5``.
+
+    The state is fp32; the weighted scores, and the state where ``q`` multiplies it, are rounded to bf16
+    (each as large an error as that of ``out``'s own rounding).  ``q``, ``k``, ``v`` and ``state`` have
+    gradients; those of shared heads are summed in fp32 before their one rounding.  A token whose ``k`` or
+    ``v`` is not finite may make every output of its sequence NaN."""
+    return DecayAttention(*_dev.native().token_decay(q, k, v, log_decay, state, lengths, _scale(q, scale)))
+
+
+def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor,
+                         slots: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """One token of each sequence: updates ``state`` in place and returns ``out`` [batch, heads, dv].
+    ``q`` [batch, heads, dk], ``k`` and ``v`` [batch, kv heads, size] in bf16; ``state`` [slots, heads, dk,
+    dv] fp32, contiguous.  ``slots`` [batch] names each sequence's state in a pool (default: its own
+    place): a negative one is an empty place of the batch (``out`` 0), one past the pool, or one that an
+    earlier place of the batch has, gives NaN; none of these touches a state.  All arithmetic is fp32.
+    It has no gradient and raises where one would be recorded."""
+    return _dev.native().token_decay_step(q, k, v, log_decay, state, slots, _scale(q, scale))
+
+
+def _scale(q: torch.Tensor, scale: float | None) -> float:
+    return scale if scale is not None else max(1, q.shape[-1]) ** -0.5

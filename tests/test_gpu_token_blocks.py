@@ -1,0 +1,878 @@
+"""A token model's block (xdna_train.tokens: layer norm, linear layer, decay attention) against plain
+64-bit implementations on the CPU, at the sizes, lengths and strides where they can go wrong.
+
+Tolerances, per element.  u = 2^-24 (half an fp32 ulp at 1), b = 2^-8 (half a bf16 ulp at 1, the one
+rounding of a bf16 result); each function's docstring derives its own:
+* layer norm: norm_reference;  * linear layer: linear_reference;  * decay attention: walk.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U, B = 2.0 ** -24, 2.0 ** -8
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+
+
+@pytest.fixture(scope="module")
+def T(hip):
+    from xdna_train import tokens
+    return tokens
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rounding(dtype):
+    return B if dtype == BF16 else U
+
+
+def close(got, ref, tol, what):
+    got = got.detach().cpu().to(F64)
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    bad = ~((got == ref) | ((got - ref).abs() <= tol))
+    assert not bad.any(), (what, int(bad.sum()), got[bad][:4], ref[bad][:4], tol[bad][:4] if torch.is_tensor(tol) else tol)
+
+
+def padded(t, extra, offset=0):
+    """t's values in a larger allocation of NaN: rows `extra` elements apart, `offset` elements in."""
+    rows, n = t.shape
+    buf = torch.full((rows * (n + extra) + offset + 8,), math.nan, dtype=t.dtype, device="xdna")
+    v = torch.as_strided(buf, (rows, n), (n + extra, 1), offset)
+    v.copy_(t)
+    return v
+
+
+def same(a, b):
+    """equal bits (the tests' values hold no NaN)"""
+    return torch.equal(a.detach().cpu(), b.detach().cpu())
+
+
+# ---- layer norm --------------------------------------------------------------------------------
+
+def norm_reference(x, w, b, dy, ds, eps, dtype, ptype):
+    """{name: (value, tolerance)} for the stored rows x.
+
+    A row's sum goes through at most 40 terms a thread, 6 steps in a wave and 16 waves: 64 u of the sum of
+    magnitudes.  That is the mean's error; the deviations' squares add up within 66 u, and a mean that is off
+    by e adds (e / deviation)^2 to the variance; a square root and a reciprocal within 3 u: the inverse
+    deviation is off by 40 u of itself and half of that square.  h is off by (64 u mean|x| + u |x - m|) / deviation and
+    the inverse's error.  The gradients' sums over rows go through at most 128 terms in any order."""
+    x, w, b, dy, ds = (None if t is None else t.to(F64) for t in (x, w, b, dy, ds))
+    r, p = rounding(dtype), rounding(ptype)
+    one = torch.ones(x.shape[1], dtype=F64)
+    wv, bv = one if w is None else w, 0 * one if b is None else b
+    m = x.mean(1, keepdim=True)
+    d = x - m
+    inv = 1 / torch.sqrt((d * d).mean(1, keepdim=True) + eps)
+    h = d * inv
+    em = 64 * U * x.abs().mean(1, keepdim=True)
+    ei = 40 * U + (em * inv) ** 2 / 2
+    eh = inv * (em + U * d.abs()) + (ei + 2 * U) * h.abs()
+    y = h * wv + bv
+    ey = eh * wv.abs() + 4 * U * ((h * wv).abs() + bv.abs()) + r * y.abs()
+    out = {"y": (y, ey)}
+    if dy is not None:
+        g = dy * wv
+        mg, mh = g.mean(1, keepdim=True), (g * h).mean(1, keepdim=True)
+        emg = 66 * U * g.abs().mean(1, keepdim=True)
+        emh = 67 * U * (g * h).abs().mean(1, keepdim=True) + (g.abs() * eh).mean(1, keepdim=True)
+        core = g - mg - h * mh
+        dx = inv * core
+        edx = inv * (4 * U * (g.abs() + mg.abs() + (h * mh).abs()) + emg + eh * mh.abs() + (h.abs() + eh) * emh) + (ei + 2 * U) * dx.abs()
+        if ds is not None:
+            dx = dx + ds
+            edx = edx + 2 * U * (dx.abs() + ds.abs())
+        out["dx"] = (dx, edx + r * dx.abs())
+        dw, db = (dy * h).sum(0), dy.sum(0)
+        out["dw"] = (dw, (dy.abs() * eh).sum(0) + 130 * U * (dy * h).abs().sum(0) + p * dw.abs())
+        out["db"] = (db, 130 * U * dy.abs().sum(0) + p * db.abs())
+    return {k: (v, e + 1e-30) for k, (v, e) in out.items()}
+
+
+NORM = [  # rows, width
+    (1, 1), (1, 2), (3, 7), (2, 8), (5, 9), (1, 511), (4, 512), (9, 513), (33, 515), (7, 1000), (3, 1024), (6, 1025), (700, 1160), (2, 2047), (5, 2048),
+    (3, 2049), (2, 4096), (3, 4099), (2, 8192), (2, 8193), (2, 16384), (2, 16385), (3, 20011), (4200, 64), (9000, 24),
+]
+
+
+@pytest.mark.parametrize("types", [(BF16, BF16), (BF16, F32), (F32, F32)], ids=["bf16", "bf16-f32", "f32"])
+@pytest.mark.parametrize("add", [False, True], ids=["norm", "add"])
+@pytest.mark.parametrize("R,D", NORM)
+def test_layer_norm(T, R, D, add, types):
+    print("layer norm", R, D, add, types, flush=True)
+    dtype, ptype = types
+    g = gen(R * 7 + D)
+    x = (torch.randn(R, D, generator=g) + torch.randn(R, 1, generator=g)).to(dtype)
+    r = torch.randn(R, D, generator=g).to(dtype) if add else None
+    w, b = (1 + 0.2 * torch.randn(D, generator=g)).to(ptype), torch.randn(D, generator=g).to(ptype)
+    dy, ds = torch.randn(R, D, generator=g).to(dtype), torch.randn(R, D, generator=g).to(dtype) if add else None
+    leaves = [t.to("xdna").requires_grad_() for t in (x, r, w, b) if t is not None]
+    if add:
+        y, s = T.add_layer_norm(*leaves)
+        stored = (x.float() + r.float()).to(dtype)
+        assert same(s, stored)
+        grads = torch.autograd.grad([y, s], leaves, [dy.to("xdna"), ds.to("xdna")])
+        assert same(grads[0], grads[1])
+        grads = grads[1:]
+    else:
+        y, stored = T.layer_norm(*leaves), x
+        grads = torch.autograd.grad(y, leaves, dy.to("xdna"))
+    ref = norm_reference(stored, w, b, dy, ds, 1e-5, dtype, ptype)
+    for got, name in zip((y, *grads), ("y", "dx", "dw", "db")):
+        close(got, *ref[name], name)
+    with torch.no_grad():  # without a gradient: the same bits
+        again = T.add_layer_norm(*leaves) if add else (T.layer_norm(*leaves),)
+    assert same(again[0], y)
+    if add:  # the fused form is the norm of the stored sum
+        assert same(T.layer_norm(s.detach(), *[t.detach() for t in leaves[2:]]), y)
+
+
+@pytest.mark.parametrize("D", [5, 515, 520, 3001])
+def test_layer_norm_strides_and_absent_parameters(T, D):
+    print("layer norm strides", D, flush=True)
+    g = gen(D)
+    x, r, dy = (torch.randn(11, D, generator=g).to(BF16) for _ in range(3))
+    w = torch.randn(D, generator=g)
+    xx, rx, dyx = padded(x, 3, 1).requires_grad_(), padded(r, 5, 3).requires_grad_(), padded(dy, 1, 5)
+    y, s = T.add_layer_norm(xx, rx)
+    ref = norm_reference((x.float() + r.float()).to(BF16), None, None, dy, None, 1e-5, BF16, BF16)
+    close(y, *ref["y"], "without parameters")
+    (dx,) = torch.autograd.grad(y, [xx], dyx, retain_graph=True)
+    close(dx, *ref["dx"], "dx of the norm alone")
+    dr, = torch.autograd.grad(s, [rx], dyx)
+    assert same(dr, dy)  # the sum alone has no norm's gradient
+    wx = w.to("xdna").requires_grad_()
+    y = T.layer_norm(xx.detach(), wx, eps=1e-3)
+    ref = norm_reference(x, w, None, dy, None, 1e-3, BF16, F32)
+    close(y, *ref["y"], "weight alone")
+    close(torch.autograd.grad(y, [wx], dyx)[0], *ref["dw"], "dw without dx")
+    y3 = T.layer_norm(xx.detach().view(1, 11, D), wx.detach(), eps=1e-3)
+    assert y3.shape == (1, 11, D) and same(y3[0], y)
+    t = torch.randn(D, 11, generator=g).to(BF16)
+    assert same(T.layer_norm(t.to("xdna").t()), T.layer_norm(t.t().contiguous().to("xdna")))
+
+
+def test_layer_norm_of_no_rows_and_broadcast_gradients(T):
+    w, b = torch.ones(9, device="xdna").requires_grad_(), torch.zeros(9, device="xdna").requires_grad_()
+    x = torch.zeros(0, 9, device="xdna").requires_grad_()
+    y = T.layer_norm(x, w, b)
+    grads = torch.autograd.grad(y, [x, w, b], torch.zeros(0, 9, device="xdna"))
+    assert y.shape == (0, 9) and grads[0].shape == (0, 9) and not grads[1].cpu().any() and not grads[2].cpu().any()
+    x = torch.randn(4, 9, generator=gen(3))
+    xx = x.to("xdna").requires_grad_()
+    (dx, dw) = torch.autograd.grad(T.layer_norm(xx, w, b).sum(), [xx, w])  # a gradient of stride 0
+    ref = norm_reference(x, torch.ones(9), torch.zeros(9), torch.ones(4, 9), None, 1e-5, F32, F32)
+    close(dx, *ref["dx"], "dx")
+    close(dw, *ref["dw"], "dw")
+
+
+def test_layer_norm_of_special_rows(T):
+    """A constant row is exact zeros (and the bias); a row of an infinity or NaN is NaN and touches no other;
+    a row of large values with a small spread keeps it (two passes)."""
+    x = torch.zeros(6, 64)
+    x[0] = 3.0
+    x[1] = torch.randn(64, generator=gen(1))
+    x[1, 5] = math.inf
+    x[2] = math.nan
+    x[3] = 4096 + torch.randn(64, generator=gen(2))
+    x[4] = torch.randn(64, generator=gen(3))
+    x[5] = 1e-30 * torch.randn(64, generator=gen(4))
+    y = T.layer_norm(x.to("xdna"), None, torch.full((64,), 0.5, device="xdna")).cpu()
+    assert (y[0] == 0.5).all() and torch.isnan(y[1]).all() and torch.isnan(y[2]).all()
+    ref = norm_reference(x[3:], None, torch.full((64,), 0.5), None, None, 1e-5, F32, F32)["y"]
+    close(y[3:], *ref, "rows beside them")
+
+
+def test_layer_norm_gradient_against_differences(T):
+    g = gen(11)
+    x, w, dy = torch.randn(3, 40, generator=g), 1 + 0.1 * torch.randn(40, generator=g), torch.randn(3, 40, generator=g)
+
+    def f(x, w):
+        d = x.to(F64) - x.to(F64).mean(1, keepdim=True)
+        return (d / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-5) * w.to(F64) * dy.to(F64)).sum()
+
+    xx, wx = x.to("xdna").requires_grad_(), w.to("xdna").requires_grad_()
+    dx, dw = (t.cpu().to(F64) for t in torch.autograd.grad(T.layer_norm(xx, wx), [xx, wx], dy.to("xdna")))
+    for i in range(5):
+        vx, vw = torch.randn(3, 40, generator=g).to(F64), torch.randn(40, generator=g).to(F64)
+        e = 1e-5
+        slope = (f(x.to(F64) + e * vx, w.to(F64) + e * vw) - f(x.to(F64) - e * vx, w.to(F64) - e * vw)) / (2 * e)
+        assert abs(slope - ((dx * vx).sum() + (dw * vw).sum())) <= 1e-4 * (1 + abs(slope))
+
+
+# ---- linear layer --------------------------------------------------------------------------------
+
+def act64(act, g):
+    if act == "none":
+        return g, torch.ones_like(g)
+    if act == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    if act == "gelu":
+        cdf = 0.5 * torch.erfc(-g / math.sqrt(2.0))
+        return g * cdf, cdf + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    return g.clamp(min=0), (g > 0).to(F64)
+
+
+def linear_reference(x, w, b, r, dy, act):
+    """{name: (value, tolerance)}.  A fp32 sum of n products is off by (n + 8) u of the sum of magnitudes;
+    act' is at most 1.13 and act'' at most 0.8 in size; the slope is kept within 2^-12 of itself (fp16
+    times 2^15: 2^-40 where that is subnormal), and for relu it is another one where the sum's sign is in doubt."""
+    x, w, b, r, dy = (None if t is None else t.to(F64) for t in (x, w, b, r, dy))
+    K, (M, N) = x.shape[1], (x.shape[0], w.shape[0])
+    v, mag = x @ w.t(), x.abs() @ w.abs().t()
+    if b is not None:
+        v, mag = v + b, mag + b.abs()
+    ev = (K + 8) * U * mag
+    y, s = act64(act, v)
+    ey = 1.13 * ev + (0 if act == "none" else 16 * U * (y.abs() + v.abs()))
+    if r is not None:
+        y = y + r
+        ey = ey + U * (y.abs() + r.abs())
+    out = {"y": (y, ey + B * y.abs())}
+    if dy is not None:
+        if act == "none":
+            es = 0 * s
+        else:
+            es = (torch.where(v.abs() <= 2 * ev, 1.0, 0.0) if act == "relu" else 0.8 * ev + 32 * U * (1 + v.abs())) + 2.0 ** -12 * s.abs() + 2.0 ** -40
+        p = dy * s
+        ep = dy.abs() * es + 2 * U * p.abs()
+        stored = ep + (0 if act == "none" else B) * p.abs()
+        dx, dw, db = p @ w, p.t() @ x, p.sum(0)
+        out["dx"] = (dx, (stored + (N + 8) * U * p.abs()) @ w.abs() + B * dx.abs())
+        out["dw"] = (dw, (stored + (M + 8) * U * p.abs()).t() @ x.abs() + B * dw.abs())
+        out["db"] = (db, (ep + (M + 8) * U * p.abs()).sum(0) + B * db.abs())
+    return {k: (t, e + 1e-30) for k, (t, e) in out.items()}
+
+
+LINEAR = [  # rows, K, N
+    (1, 1, 1), (1, 64, 32), (1, 2048, 300), (1, 4096, 64), (2, 7, 5), (4, 3000, 100), (5, 72, 100), (16, 256, 128), (17, 130, 63), (33, 8, 65),
+    (64, 64, 64), (65, 65, 129), (130, 512, 384), (333, 1000, 217), (200, 4000, 65), (70, 3, 4), (100, 5000, 3),
+]
+
+
+@pytest.mark.parametrize("act", ["none", "silu", "gelu", "relu"])
+@pytest.mark.parametrize("M,K,N", LINEAR)
+def test_linear(T, M, K, N, act):
+    print("linear", M, K, N, act, flush=True)
+    g = gen(M + K + N)
+    x, w = torch.randn(M, K, generator=g).to(BF16), (torch.randn(N, K, generator=g) / math.sqrt(K)).to(BF16)
+    b = torch.randn(N, generator=g).to(BF16) if (M + N) % 3 else None
+    r = torch.randn(M, N, generator=g).to(BF16) if M % 2 else None
+    dy = torch.randn(M, N, generator=g).to(BF16)
+    given = {"x": x, "w": w, "b": b, "r": r}
+    lv = {n: t.to("xdna").requires_grad_() for n, t in given.items() if t is not None}
+    y = T.linear(lv["x"], lv["w"], lv.get("b"), act, lv.get("r"))
+    ref = linear_reference(x, w, b, r, dy, act)
+    close(y, *ref["y"], "y")
+    grads = dict(zip(lv, torch.autograd.grad(y, list(lv.values()), dy.to("xdna"))))
+    close(grads["x"], *ref["dx"], "dx")
+    close(grads["w"], *ref["dw"], "dw")
+    if b is not None:
+        close(grads["b"], *ref["db"], "db")
+    if r is not None:
+        assert same(grads["r"], dy)
+    with torch.no_grad():
+        assert same(T.linear(lv["x"], lv["w"], lv.get("b"), act, lv.get("r")), y)
+
+
+@pytest.mark.parametrize("M,K,N,act", [(4096, 264, 4096, "relu"), (4100, 512, 4096, "silu"), (2048, 1024, 2056, "none"), (600, 8192, 512, "gelu"),
+                                       (8200, 128, 3080, "gelu")])
+def test_linear_large(T, M, K, N, act):
+    """The 256 x 256 tiles, k in splits, gradients on the GEMM: rows of the result checked at random."""
+    print("linear large", M, K, N, act, flush=True)
+    g = gen(M)
+    x, w = torch.randn(M, K, generator=g).to(BF16), (torch.randn(N, K, generator=g) / math.sqrt(K)).to(BF16)
+    b, r, dy = torch.randn(N, generator=g).to(BF16), torch.randn(M, N, generator=g).to(BF16), torch.randn(M, N, generator=g).to(BF16)
+    lv = [t.to("xdna").requires_grad_() for t in (x, w, b)]
+    y = T.linear(*lv, act, r.to("xdna"))
+    dx, dw, db = torch.autograd.grad(y, lv, dy.to("xdna"))
+    ref = linear_reference(x, w, b, r, dy, act)
+    for got, name in ((y, "y"), (dx, "dx"), (dw, "dw"), (db, "db")):
+        close(got, *ref[name], name)
+
+
+@pytest.mark.parametrize("M,K,N", [(3, 40, 24), (70, 129, 65), (700, 264, 512)])
+def test_linear_strides_and_parts_of_the_gradient(T, M, K, N):
+    print("linear strides", M, K, N, flush=True)
+    g = gen(M)
+    x, w, r, dy = (torch.randn(*s, generator=g).to(BF16) for s in ((M, K), (N, K), (M, N), (M, N)))
+    b = torch.randn(2 * N, generator=g).to(BF16).to("xdna")[::2]
+    ref = linear_reference(x, w, b.cpu(), r, dy, "gelu")
+    xx, wx, rx, dyx = padded(x, 3, 1), padded(w, 5, 3), padded(r, 1, 1), padded(dy, 7, 5)
+    for wanted in ((0,), (1,), (2,), (0, 1), (1, 2), (3,), (0, 1, 2, 3)):
+        lv = [t.detach().requires_grad_(i in wanted) for i, t in enumerate((xx, wx, b, rx))]
+        y = T.linear(lv[0], lv[1], lv[2], "gelu", lv[3])
+        close(y, *ref["y"], "y")
+        for i, got in zip(wanted, torch.autograd.grad(y, [lv[i] for i in wanted], dyx)):
+            if i == 3:
+                assert same(got, dy)
+            else:
+                close(got, *ref[("dx", "dw", "db")[i]], i)
+    y3 = T.linear(xx.unsqueeze(0), wx, b, "gelu", rx.unsqueeze(0))
+    assert y3.shape == (1, M, N) and same(y3[0], y)
+    assert same(T.linear(x.t().contiguous().to("xdna").t(), wx, b, "gelu", rx), y)
+    one = torch.ones(1, N, device="xdna", dtype=BF16).expand(M, N)  # stride 0
+    lv = [xx.detach().requires_grad_(), wx.detach()]
+    ref = linear_reference(x, w, None, torch.ones(M, N).to(BF16), torch.ones(M, N).to(BF16), "silu")
+    y = T.linear(*lv, None, "silu", one)
+    close(y, *ref["y"], "broadcast residual")
+    close(torch.autograd.grad(y, [lv[0]], one)[0], *ref["dx"], "broadcast gradient")
+
+
+def test_linear_without_rows(T):
+    x, w, b = torch.zeros(0, 8, device="xdna", dtype=BF16), torch.ones(5, 8, device="xdna", dtype=BF16), torch.ones(5, device="xdna", dtype=BF16)
+    lv = [t.requires_grad_() for t in (x, w, b)]
+    for act in ("none", "silu"):
+        y = T.linear(*lv, act)
+        dx, dw, db = torch.autograd.grad(y, lv, torch.zeros(0, 5, device="xdna", dtype=BF16))
+        assert y.shape == (0, 5) and dx.shape == (0, 8) and not dw.cpu().any() and not db.cpu().any()
+
+
+def test_linear_slopes_keep_the_lower_tail(T):
+    """A unit far in an activation's tail still has a gradient: the kept slope's relative error is 2^-12 down
+    to 1.9e-9."""
+    M, K = 32, 16
+    for act, at in (("silu", -12.0), ("gelu", -5.0), ("silu", -19.0)):
+        x = torch.zeros(M, K)
+        x[:, 0] = at
+        x[:, 1] = 1.0
+        w, dy = torch.zeros(1, K), torch.ones(M, 1)
+        w[0, 0] = 1.0
+        lv = [t.to(BF16).to("xdna").requires_grad_() for t in (x, w)]
+        dx, dw = torch.autograd.grad(T.linear(*lv, None, act), lv, dy.to(BF16).to("xdna"))
+        s = float(act64(act, torch.tensor(at, dtype=F64))[1])
+        assert abs(float(dx[0, 0]) - s) <= (2 * B + 2.0 ** -10) * abs(s), (act, at, float(dx[0, 0]), s)
+        assert abs(float(dw[0, 1]) - M * s) <= (2 * B + 2.0 ** -10) * abs(M * s)
+
+
+def test_linear_gradient_against_differences(T):
+    g = gen(5)
+    x, w, b, dy = (torch.randn(*s, generator=g).to(BF16) for s in ((6, 24), (10, 24), (10,), (6, 10)))
+    w = (w.float() / 5).to(BF16)
+    for act in ("silu", "gelu"):
+        def f(x, w, b):
+            return (act64(act, x @ w.t() + b)[0] * dy.to(F64)).sum()
+
+        lv = [t.to("xdna").requires_grad_() for t in (x, w, b)]
+        grads = [t.cpu().to(F64) for t in torch.autograd.grad(T.linear(*lv, act), lv, dy.to("xdna"))]
+        base = [t.to(F64) for t in (x, w, b)]
+        for _ in range(5):
+            vs = [torch.randn(t.shape, generator=g).to(F64) for t in base]
+            e = 1e-5
+            slope = (f(*[t + e * v for t, v in zip(base, vs)]) - f(*[t - e * v for t, v in zip(base, vs)])) / (2 * e)
+            mine = sum((d * v).sum() for d, v in zip(grads, vs))
+            mag = sum((d * v).abs().sum() for d, v in zip(grads, vs))
+            assert abs(slope - mine) <= 2 * B * mag, (act, slope, mine)
+
+
+# ---- decay attention -------------------------------------------------------------------------------
+
+CHUNK = 128
+
+
+def walk(q, k, v, g, s0, lead, p, qs, ks):
+    """One head's walk in 64 bits: ((outputs, tolerance), (last state, tolerance)) without the outputs' own
+    rounding.  Weights are exp of a product: (2 |exponent| + 4) u, under 200 u of the largest that counts.  fp32 sums
+    over n tokens, 128 of a head and the carries: (n + 640) u of the sum of magnitudes.  The weighted scores of a
+    chunk and the state before it, as operands, are rounded to bf16 (b each); the state's own sum has its
+    weighted v in two bf16: 2^-16."""
+    n, u = q.shape[0], (q.shape[0] + 640) * U
+    at = torch.arange(n, dtype=F64)
+    apart = at[:, None] - at
+    weight = torch.where(apart >= 0, torch.exp(apart * g), 0.0) if g > -math.inf else (apart == 0).to(F64)
+    power = (lambda e: torch.exp(e * g)) if g > -math.inf else (lambda e: (e == 0).to(F64))
+    P = (q @ k.t()) * weight * p
+    mag = (q.abs() @ k.abs().t()) * weight * abs(p)
+    inner = (at[:, None] // CHUNK) == (at // CHUNK)
+    out = P @ v + qs / p * 0 * q[:, :1]
+    tol = u * (mag @ v.abs()) + B * ((P * inner).abs() @ v.abs()) + 2.0 ** -16 * (mag @ v.abs())
+    first = power(at + lead)[:, None]
+    out = out + qs * first * (q @ s0)
+    tol = tol + u * abs(qs) * first * (q.abs() @ s0.abs())
+    # the states before the chunks, for what their rounding costs
+    s, c0 = s0, 0
+    for c0 in range(0, n, CHUNK):
+        m = min(CHUNK, n - c0)
+        local = power(torch.arange(m, dtype=F64) + lead)[:, None]
+        tol[c0:c0 + m] += B * abs(qs) * local * (q[c0:c0 + m].abs() @ s.abs())
+        w = power(m - lead - torch.arange(m, dtype=F64))[:, None] * ks
+        s = power(torch.tensor(float(m), dtype=F64)) * s + (k[c0:c0 + m] * w).t() @ v[c0:c0 + m]
+    w = power(n - lead - at)[:, None] * abs(ks)
+    es = (u + 2.0 ** -16) * ((k.abs() * w).t() @ v.abs() + power(torch.tensor(float(n), dtype=F64)) * s0.abs())
+    return (out, tol), (s, es)
+
+
+def decay_reference(q, k, v, g, s0, lengths, scale, dout=None, ds=None):
+    """{name: (value, tolerance)} of every output and gradient."""
+    q, k, v, g = (t.to(F64) for t in (q, k, v, g))
+    Bn, Tn, H, dk = q.shape
+    G, dv = k.shape[2], v.shape[3]
+    zeros = lambda *s: (torch.zeros(*s, dtype=F64), torch.zeros(*s, dtype=F64))  # noqa: E731
+    out, last = zeros(Bn, Tn, H, dv), zeros(Bn, H, dk, dv)
+    dq, dkk, dvv, d0 = zeros(Bn, Tn, H, dk), zeros(Bn, Tn, G, dk), zeros(Bn, Tn, G, dv), zeros(Bn, H, dk, dv)
+    for b in range(Bn):
+        n = Tn if lengths is None else max(0, min(Tn, int(lengths[b])))
+        for h in range(H):
+            j = h // (H // G)
+            qh, kh, vh = q[b, :n, h], k[b, :n, j], v[b, :n, j]
+            s = torch.zeros(dk, dv, dtype=F64) if s0 is None else s0[b, h].to(F64)
+            o, e = walk(qh, kh, vh, g[h], s, 1, scale, scale, 1.0)
+            for at in (0, 1):
+                out[at][b, :n, h], last[at][b, h] = o[at], e[at]
+            if dout is None:
+                continue
+            do = dout[b, :n, h].to(F64)
+            r = torch.zeros(dk, dv, dtype=F64) if ds is None else ds[b, h].to(F64)
+            o, _ = walk(do, vh, kh, g[h], s.t(), 1, scale, scale, 1.0)
+            rev = lambda t: t.flip(0)  # noqa: E731
+            ov, e0 = walk(rev(kh), rev(qh), rev(do), g[h], r, 0, scale, 1.0, scale)
+            ok, _ = walk(rev(vh), rev(do), rev(qh), g[h], r.t(), 0, scale, 1.0, scale)
+            for at in (0, 1):
+                dq[at][b, :n, h] = o[at]
+                dvv[at][b, :n, j] += rev(ov[at])
+                dkk[at][b, :n, j] += rev(ok[at])
+                d0[at][b, h] = e0[at]
+    ref = {"out": out, "state": last}
+    if dout is not None:
+        ref |= {"dq": dq, "dk": dkk, "dv": dvv, "dstate": d0}
+    return {n: (t, e + (B * t.abs() if "state" not in n else 2 * U * t.abs()) + 1e-30) for n, (t, e) in ref.items()}
+
+
+def decay_values(Bn, Tn, H, G, dk, dv, seed, state=True):
+    g = gen(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    v = {"q": r(Bn, Tn, H, dk).to(BF16), "k": r(Bn, Tn, G, dk).to(BF16), "v": r(Bn, Tn, G, dv).to(BF16),
+         "g": -torch.exp2(-0.5 - 8.0 * torch.arange(H) / H), "dout": r(Bn, Tn, H, dv).to(BF16)}
+    v["state"], v["dstate"] = (2 * r(Bn, H, dk, dv), r(Bn, H, dk, dv)) if state else (None, None)
+    return v
+
+
+def run_decay(T, v, lengths=None, scale=None, grads=True):
+    """Outputs and gradients by name."""
+    names = [n for n in ("q", "k", "v", "state") if v[n] is not None]
+    lv = {n: (v[n] if v[n].device.type == "xdna" else v[n].to("xdna")).detach().requires_grad_(grads) for n in names}
+    r = T.decay_attention(lv["q"], lv["k"], lv["v"], v["g"].to("xdna"), lv.get("state"), None if lengths is None else lengths.to("xdna"), scale)
+    got = {"out": r.out, "state": r.state}
+    if grads:
+        ends = [(r.out, v["dout"])] + ([(r.state, v["dstate"])] if v["dstate"] is not None else [])
+        d = torch.autograd.grad([e for e, _ in ends], list(lv.values()), [x.to("xdna") for _, x in ends])
+        got |= {"d" + n: t for n, t in zip(names, d)}
+    return got
+
+
+def check_decay(got, ref):
+    for n, t in got.items():
+        close(t, *ref[n], n)
+
+
+DECAY = [  # batch, tokens, heads, kv heads, dk, dv
+    (1, 1, 1, 1, 1, 1), (1, 2, 1, 1, 8, 8), (2, 5, 2, 1, 16, 16), (1, 16, 1, 1, 64, 64), (1, 31, 2, 2, 64, 64), (2, 32, 1, 1, 33, 65), (1, 33, 3, 1, 64, 128),
+    (1, 64, 1, 1, 128, 64), (1, 100, 2, 1, 7, 3), (1, 127, 2, 2, 128, 128), (2, 128, 1, 1, 100, 72), (1, 129, 2, 2, 48, 80), (1, 256, 1, 1, 128, 128),
+    (1, 300, 4, 2, 64, 64), (2, 391, 2, 1, 72, 127), (1, 777, 6, 2, 48, 80),
+]
+
+
+@pytest.mark.parametrize("state", [True, False], ids=["state", "new"])
+@pytest.mark.parametrize("size", DECAY)
+def test_decay_attention(T, size, state):
+    print("decay", size, state, flush=True)
+    v = decay_values(*size, seed=sum(size), state=state)
+    scale = 0.37 if size[1] % 2 else None
+    got = run_decay(T, v, scale=scale)
+    check_decay(got, decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], None, scale or size[4] ** -0.5, v["dout"], v["dstate"]))
+    again = run_decay(T, v, scale=scale)
+    assert all(same(got[n], again[n]) for n in got), "equal inputs, different bits"
+
+
+@pytest.mark.parametrize("size", [(7, 300, 2, 1, 64, 64), (6, 200, 3, 3, 40, 100), (7, 700, 1, 1, 128, 128)])
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32], ids=["int64", "int32"])
+def test_decay_attention_of_ragged_batches(T, size, kind):
+    """Lengths of zero, one, a chunk and its neighbours, past the tensor and below zero; what lies behind a
+    sequence's end is NaN."""
+    print("decay ragged", size, kind, flush=True)
+    Bn, Tn = size[:2]
+    lengths = torch.tensor([0, 1, 128, 129, Tn - 1, Tn + 5, -3][:Bn], dtype=kind)
+    v = decay_values(*size, seed=5)
+    ref = decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], lengths, 0.2, v["dout"], v["dstate"])
+    for b in range(Bn):
+        n = max(0, min(Tn, int(lengths[b])))
+        for name in ("q", "k", "v", "dout"):
+            v[name][b, n:] = math.nan
+    got = run_decay(T, v, lengths, 0.2)
+    check_decay(got, ref)
+    for name in ("out", "dq", "dk", "dv"):
+        for b in range(Bn):
+            assert not got[name][b, max(0, min(Tn, int(lengths[b]))):].cpu().any(), (name, b)
+
+
+@pytest.mark.parametrize("size", [(1, 1500, 1, 1, 64, 64), (1, 1025, 64, 32, 8, 16), (2, 1400, 33, 33, 16, 8)])
+def test_decay_attention_of_long_sequences_in_segments(T, size):
+    """Sequences cut into segments of one chunk and of several, ragged among them."""
+    print("decay segments", size, flush=True)
+    v = decay_values(*size, seed=7)
+    lengths = None if size[0] == 1 else torch.tensor([size[1], 300])
+    got = run_decay(T, v, lengths)
+    check_decay(got, decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], lengths, size[4] ** -0.5, v["dout"], v["dstate"]))
+
+
+def test_decay_attention_of_many_heads_in_one_walk(T):
+    """As many workgroups as the chip takes: no segments, several chunks each."""
+    size = (1, 400, 260, 260, 9, 70)
+    v = decay_values(*size, seed=8)
+    check_decay(run_decay(T, v), decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], None, size[4] ** -0.5, v["dout"], v["dstate"]))
+
+
+def test_decay_attention_at_the_ends_of_the_decays(T):
+    """Nothing forgotten (0), everything (-inf), and decays that underflow within a chunk."""
+    v = decay_values(2, 200, 4, 4, 16, 24, seed=9)
+    v["g"] = torch.tensor([0.0, -math.inf, -30.0, -3.0])
+    check_decay(run_decay(T, v), decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], None, 0.25, v["dout"], v["dstate"]))
+    got = T.decay_attention(*[v[n].to("xdna") for n in ("q", "k", "v", "g")], scale=-0.25)
+    close(got.out, *decay_reference(v["q"], v["k"], v["v"], v["g"], None, None, -0.25)["out"], "negative scale")
+    got = T.decay_attention(*[v[n].to("xdna") for n in ("q", "k", "v", "g")], scale=0.0)
+    assert not got.out.cpu().any()
+
+
+def test_decay_attention_of_slices_and_broadcast_heads(T):
+    Bn, Tn, H, G, dk, dv = 2, 150, 4, 2, 24, 40
+    v = decay_values(Bn, Tn, H, G, dk, dv, seed=10)
+    ref = decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], None, dk ** -0.5, v["dout"], v["dstate"])
+    qkv = torch.cat([v["q"].flatten(2), v["k"].flatten(2), v["v"].flatten(2)], 2).to("xdna")
+    parts = torch.split(qkv, [H * dk, G * dk, G * dv], 2)
+    cut = dict(v, q=parts[0].view(Bn, Tn, H, dk), k=parts[1].view(Bn, Tn, G, dk), v=parts[2].view(Bn, Tn, G, dv))
+    check_decay(run_decay(T, cut), ref)
+    heads_first = dict(v, **{n: v[n].transpose(1, 2).contiguous().to("xdna").transpose(1, 2) for n in ("q", "k", "v", "dout")})
+    heads_first["dout"] = heads_first["dout"].to("xdna")
+    check_decay(run_decay(T, heads_first), ref)
+    size_first = dict(v, q=v["q"].permute(3, 0, 1, 2).contiguous().to("xdna").permute(1, 2, 3, 0))  # a copy is made
+    check_decay(run_decay(T, size_first), ref)
+    # one head of k and v for all, as a broadcast: the gradient of the one is the sum
+    one_k, one_v = v["k"][:, :, :1], v["v"][:, :, :1]
+    kx, vx = one_k.to("xdna").requires_grad_(), one_v.to("xdna").requires_grad_()
+    r = T.decay_attention(v["q"].to("xdna"), kx.expand(-1, -1, H, -1), vx.expand(-1, -1, H, -1), v["g"].to("xdna"))
+    ref = decay_reference(v["q"], one_k, one_v, v["g"], None, None, dk ** -0.5, v["dout"])
+    close(r.out, *ref["out"], "broadcast")
+    dkx, dvx = torch.autograd.grad(r.out, [kx, vx], v["dout"].to("xdna"))
+    for got, (t, e), single in ((dkx, ref["dk"], v["k"]), (dvx, ref["dv"], v["v"])):
+        close(got, t, 2 * e, "sum of rounded gradients")  # (a head's gradient, rounded, is off by b of terms that e holds b of)
+
+
+def test_decay_attention_continues_where_it_left_off(T):
+    """A sequence in two parts, then token by token, against the whole."""
+    Bn, Tn, H, G, dk, dv = 2, 260, 4, 2, 40, 48
+    v = decay_values(Bn, Tn, H, G, dk, dv, seed=12)
+    d = {n: t.to("xdna") for n, t in v.items()}
+    ref = decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], None, 0.3)
+    first = T.decay_attention(d["q"][:, :100], d["k"][:, :100], d["v"][:, :100], d["g"], d["state"], scale=0.3)
+    second = T.decay_attention(d["q"][:, 100:200], d["k"][:, 100:200], d["v"][:, 100:200], d["g"], first.state, scale=0.3)
+    outs, state = [first.out, second.out], second.state.clone()
+    for t in range(200, Tn):
+        outs.append(T.decay_attention_step(d["q"][:, t], d["k"][:, t], d["v"][:, t], d["g"], state, scale=0.3)[:, None])
+    (o, eo), (s, es) = ref["out"], ref["state"]
+    # (where the whole has chunks the parts have others: both within the tolerance of their own)
+    q, k, w = (v[n].to(F64) for n in ("q", "k", "v"))
+    at = torch.arange(Tn, dtype=F64)
+    apart = (at[:, None] - at).clamp(min=0)
+    for h in range(H):
+        weight = torch.where(at[:, None] >= at, torch.exp(apart * v["g"][h].to(F64)), 0.0)
+        for b in range(Bn):
+            mag = ((q[b, :, h].abs() @ k[b, :, h // 2].abs().t()) * weight) @ w[b, :, h // 2].abs()
+            mag += torch.exp((at + 1) * v["g"][h].to(F64))[:, None] * (q[b, :, h].abs() @ v["state"][b, h].to(F64).abs())
+            eo[b, :, h] = 2 * B * 0.3 * mag + B * o[b, :, h].abs()
+    close(torch.cat([x.cpu() for x in outs], 1), o, eo, "parts")
+    close(state, s, es, "state")
+
+
+@pytest.mark.parametrize("Bn,H,G,dk,dv", [(1, 1, 1, 1, 1), (1, 8, 8, 64, 64), (3, 4, 2, 33, 5), (5, 2, 1, 128, 128), (2, 3, 3, 31, 127), (4, 2, 2, 100, 36)])
+def test_decay_step(T, Bn, H, G, dk, dv):
+    print("decay step", Bn, H, G, dk, dv, flush=True)
+    v = decay_values(Bn, 1, H, G, dk, dv, seed=Bn + dk)
+    d = {n: t.to("xdna") for n, t in v.items()}
+    state = d["state"].clone()
+    version = state._version
+    out = T.decay_attention_step(d["q"][:, 0], d["k"][:, 0], d["v"][:, 0], d["g"], state)
+    assert state._version > version
+    s = v["state"].to(F64) * torch.exp(v["g"].to(F64))[:, None, None]
+    kh, vh = (v[n][:, 0].to(F64).repeat_interleave(H // G, 1) for n in ("k", "v"))
+    add = kh[..., None] * vh[..., None, :]
+    close(state, s + add, 8 * U * (s.abs() + add.abs()) + 1e-30, "state")
+    o = dk ** -0.5 * (v["q"][:, 0].to(F64)[..., None] * (s + add)).sum(2)
+    mag = dk ** -0.5 * (v["q"][:, 0].to(F64).abs()[..., None] * (s.abs() + add.abs())).sum(2)
+    close(out, o, (dk + 16) * U * mag + B * o.abs() + 1e-30, "out")
+
+
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32], ids=["int64", "int32"])
+def test_decay_step_of_a_pool(T, kind):
+    """Slots in any order; empty places, slots past the pool and slots named twice touch no state."""
+    Bn, H, dk, dv, pool = 300, 2, 16, 20, 320
+    v = decay_values(Bn, 1, H, H, dk, dv, seed=3)
+    q, k, w = (v[n][:, 0].to("xdna") for n in ("q", "k", "v"))
+    states = torch.randn(pool, H, dk, dv, generator=gen(4))
+    slots = torch.randperm(pool, generator=gen(5))[:Bn].to(kind)
+    slots[3], slots[50], slots[120], slots[299] = -1, pool, slots[7], slots[298]
+    slots[298] = slots[0]
+    pool_x = states.to("xdna")
+    out = T.decay_attention_step(q, k, w, v["g"].to("xdna"), pool_x, slots.to("xdna")).cpu()
+    seen, expect = set(), states.clone()
+    for b in range(Bn):
+        s = int(slots[b])
+        if s < 0:
+            assert not out[b].any()
+        elif s >= pool or s in seen:
+            assert torch.isnan(out[b]).all(), b
+        else:
+            one = states[s:s + 1].to("xdna")
+            alone = T.decay_attention_step(q[b:b + 1], k[b:b + 1], w[b:b + 1], v["g"].to("xdna"), one)
+            assert same(alone[0], out[b])
+            expect[s] = one[0].cpu()
+        seen.add(s)
+    assert same(pool_x, expect)
+
+
+def test_decay_attention_without_tokens_or_sequences(T):
+    g, s = torch.tensor([-0.5, -0.1], device="xdna"), torch.randn(3, 2, 4, 5, device="xdna").requires_grad_()
+    q, k, w = (torch.zeros(3, 0, 2, n, device="xdna", dtype=BF16).requires_grad_() for n in (4, 4, 5))
+    r = T.decay_attention(q, k, w, g, s)
+    assert r.out.shape == (3, 0, 2, 5) and same(r.state, s)
+    (ds, dq) = torch.autograd.grad([r.out, r.state], [s, q], [torch.zeros_like(r.out), torch.ones_like(r.state)])
+    assert (ds.cpu() == 1).all() and dq.shape == q.shape
+    assert not T.decay_attention(q.detach(), k.detach(), w.detach(), g).state.cpu().any()
+    none = T.decay_attention(*(t.detach()[:0] for t in (q, k, w)), g)
+    assert none.out.shape == (0, 0, 2, 5) and none.state.shape == (0, 2, 4, 5)
+    step = T.decay_attention_step(*(torch.zeros(0, 2, n, device="xdna", dtype=BF16) for n in (4, 4, 5)), g, torch.zeros(0, 2, 4, 5, device="xdna"))
+    assert step.shape == (0, 2, 5)
+
+
+def test_decay_gradients_of_one_result_alone(T):
+    v = decay_values(1, 150, 2, 2, 24, 32, seed=21)
+    lv = [v[n].to("xdna").requires_grad_() for n in ("q", "k", "v", "state")]
+    r = T.decay_attention(*lv[:3], v["g"].to("xdna"), lv[3])
+    grads = torch.autograd.grad(r.state, lv, v["dstate"].to("xdna"))
+    ref = decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], None, 24 ** -0.5, 0 * v["dout"], v["dstate"])
+    for got, n in zip(grads, ("dq", "dk", "dv", "dstate")):
+        close(got, *ref[n], n)
+    frozen = T.decay_attention(lv[0], lv[1].detach(), lv[2].detach(), v["g"].to("xdna"), lv[3].detach())
+    (dq,) = torch.autograd.grad(frozen.out, [lv[0]], v["dout"].to("xdna"))
+    close(dq, *decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], None, 24 ** -0.5, v["dout"])["dq"], "dq alone")
+
+
+def test_decay_gradient_against_differences(T):
+    v = decay_values(1, 140, 1, 1, 12, 10, seed=22)
+    got = run_decay(T, v)
+    base = {n: v[n].to(F64) for n in ("q", "k", "v", "state")}
+
+    def f(x):  # token by token
+        s, total, a = x["state"][0, 0], 0.0, math.exp(float(v["g"][0]))
+        for t in range(140):
+            s = a * s + x["k"][0, t, 0][:, None] * x["v"][0, t, 0]
+            total = total + 12 ** -0.5 * ((x["q"][0, t, 0] @ s) * v["dout"][0, t, 0].to(F64)).sum()
+        return float(total + (s * v["dstate"][0, 0].to(F64)).sum())
+
+    g = gen(23)
+    for _ in range(4):
+        vs = {n: torch.randn(t.shape, generator=g).to(F64) for n, t in base.items()}
+        e = 1e-4
+        slope = (f({n: t + e * vs[n] for n, t in base.items()}) - f({n: t - e * vs[n] for n, t in base.items()})) / (2 * e)
+        terms = [(got["d" + n].detach().cpu().to(F64) * vs[n]) for n in base]
+        assert abs(slope - sum(t.sum() for t in terms)) <= 4 * B * sum(t.abs().sum() for t in terms)
+
+
+def test_decay_attention_past_32_bits(T):
+    """Offsets of q, k, v and of the states past 2^31 elements."""
+    H, dk, dv, far = 1, 16, 16, (1 << 31) + 64
+    v = decay_values(1, 2, H, H, dk, dv, seed=31)
+    buf = torch.zeros(far + 1024, dtype=BF16, device="xdna")
+    cut = dict(v)
+    for i, n in enumerate(("q", "k", "v")):
+        t = torch.as_strided(buf, (1, 2, 1, 16), (far, far, 16, 1), 256 * i)
+        t.copy_(v[n])
+        cut[n] = t
+    check_decay(run_decay(T, cut), decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], None, 0.25, v["dout"], v["dstate"]))
+    del buf, cut, t
+    pool = torch.zeros((1 << 23) + 3, 1, 16, 16, dtype=F32, device="xdna")
+    pool[-1] = v["state"][0].to("xdna")
+    slots = torch.tensor([(1 << 23) + 2], device="xdna")
+    out = T.decay_attention_step(*(v[n][:, 0].to("xdna") for n in ("q", "k", "v", )), v["g"].to("xdna"), pool, slots)
+    one = v["state"].to("xdna").clone()
+    assert same(out, T.decay_attention_step(*(v[n][:, 0].to("xdna") for n in ("q", "k", "v")), v["g"].to("xdna"), one))
+    assert same(pool[-1], one[0])
+
+
+# ---- together --------------------------------------------------------------------------------------
+
+def block_weights(width, heads, head, seed):
+    g = gen(seed)
+    r = lambda *s: (torch.randn(*s, generator=g) / math.sqrt(s[-1])).to(BF16)  # noqa: E731
+    return {"n1": (1 + 0.1 * torch.randn(width, generator=g)).to(BF16), "b1": torch.zeros(width, dtype=BF16), "qkv": r(3 * heads * head, width),
+            "bq": torch.zeros(3 * heads * head, dtype=BF16), "o": r(width, heads * head), "n2": torch.ones(width, dtype=BF16), "b2": torch.zeros(width, dtype=BF16),
+            "w_in": r(4 * width, width), "w_out": r(width, 2 * width)}
+
+
+def block(T, p, x, g, heads, head, state=None, lengths=None):
+    """norm -> projection -> attention -> projection and residual -> norm -> feed-forward, and the block's residual in
+    the next norm's sum."""
+    Bn, Tn, _ = x.shape
+    q, k, v = T.linear(T.layer_norm(x, p["n1"], p["b1"]), p["qkv"], p["bq"]).view(Bn, Tn, 3, heads, head).unbind(2)
+    a = T.decay_attention(q, k, v, g, state, lengths)
+    x = T.linear(a.out.reshape(Bn, Tn, heads * head), p["o"], residual=x)
+    m = T.gated_mlp(T.layer_norm(x, p["n2"], p["b2"]), p["w_in"], p["w_out"])
+    return T.add_layer_norm(m, x, p["n1"], p["b1"]), a.state
+
+
+def block32(p, x, g, heads, head, acts=False):
+    """The same in plain fp32 operations on the CPU, token by token, differentiable."""
+    Bn, Tn, _ = x.shape
+    norm = lambda t, w, b: (t - t.mean(-1, keepdim=True)) / torch.sqrt(t.var(-1, correction=0, keepdim=True) + 1e-5) * w + b  # noqa: E731
+    q, k, v = (norm(x, p["n1"], p["b1"]) @ p["qkv"].t() + p["bq"]).view(Bn, Tn, 3, heads, head).unbind(2)
+    s, outs = torch.zeros(Bn, heads, head, head), []
+    for t in range(Tn):
+        s = s * torch.exp(g)[:, None, None] + k[:, t, :, :, None] * v[:, t, :, None, :]
+        outs.append(head ** -0.5 * (q[:, t, :, :, None] * s).sum(2))
+    x = torch.stack(outs, 1).reshape(Bn, Tn, heads * head) @ p["o"].t() + x
+    gu = norm(x, p["n2"], p["b2"]) @ p["w_in"].t()
+    f = gu.shape[-1] // 2
+    x = (torch.nn.functional.silu(gu[..., :f]) * gu[..., f:]) @ p["w_out"].t() + x
+    return norm(x, p["n1"], p["b1"]), x, s
+
+
+def test_a_block_of_them_together(T):
+    """Forward and gradients of a whole block against fp32, in the 2-norm: each of the chain's 8 roundings to bf16 is
+    under b of its tensor's norm and no step of the block enlarges a relative error by more than 4."""
+    Bn, Tn, width, heads, head = 2, 150, 64, 4, 16
+    p = block_weights(width, heads, head, 1)
+    x = torch.randn(Bn, Tn, width, generator=gen(2)).to(BF16)
+    g = -torch.exp2(-1.0 - torch.arange(heads).float())
+    dy = torch.randn(Bn, Tn, width, generator=gen(3)).to(BF16)
+    lv = {n: t.to("xdna").requires_grad_() for n, t in p.items()}
+    xx = x.to("xdna").requires_grad_()
+    (y, s), state = block(T, lv, xx, g.to("xdna"), heads, head)
+    grads = torch.autograd.grad([y, s], [xx, *lv.values()], [dy.to("xdna"), dy.to("xdna")])
+    ref = {n: t.float().requires_grad_() for n, t in p.items()}
+    xr = x.float().requires_grad_()
+    yr, sr, stater = block32(ref, xr, g, heads, head)
+    want = torch.autograd.grad([yr, sr], [xr, *ref.values()], [dy.float(), dy.float()])
+    for got, w, n in [(y, yr, "y"), (s, sr, "sum"), (state, stater, "state")] + list(zip(grads, want, ["x", *p])):
+        off = (got.detach().cpu().float() - w.detach()).norm() / w.detach().norm()
+        assert off <= 8 * 4 * B, (n, float(off))
+
+
+def test_decoding_token_by_token_is_the_prompt(T):
+    """The block's steps from the prompt's state against the prompt itself: the norms, projections and the
+    feed-forward of a token are the same rows, the attention's states the same numbers up to their rounding."""
+    Bn, Tn, width, heads, head = 3, 40, 64, 4, 16
+    p = {n: t.to("xdna") for n, t in block_weights(width, heads, head, 4).items()}
+    x = torch.randn(Bn, Tn, width, generator=gen(5)).to(BF16).to("xdna")
+    g = -torch.exp2(-1.0 - torch.arange(heads).float()).to("xdna")
+    with torch.no_grad():
+        (y, _), state = block(T, p, x, g, heads, head)
+        (_, _), s = block(T, p, x[:, :30], g, heads, head)
+        s = s.clone()
+        for t in range(30, Tn):
+            xt = x[:, t]
+            q, k, v = T.linear(T.layer_norm(xt, p["n1"], p["b1"]), p["qkv"], p["bq"]).view(Bn, 3, heads, head).unbind(1)
+            a = T.decay_attention_step(q, k, v, g, s)
+            xt = T.linear(a.reshape(Bn, heads * head), p["o"], residual=xt)
+            r = T.add_layer_norm(T.gated_mlp(T.layer_norm(xt, p["n2"], p["b2"]), p["w_in"], p["w_out"]), xt, p["n1"], p["b1"])
+            off = (r.norm.cpu().float() - y[:, t].cpu().float()).norm() / y[:, t].cpu().float().norm()
+            assert off <= 8 * 4 * B, (t, float(off))
+    off = (s - state).cpu().norm() / state.cpu().norm()
+    assert off <= 4 * 4 * B, float(off)
+
+
+def test_captured_block_replays_like_the_eager_one(T):
+    """Forward, backward and a decoding step of a block as a graph, replayed with eager work between: the same bits
+    each time."""
+    Bn, Tn, width, heads, head = 2, 300, 64, 2, 32
+    p = {n: t.to("xdna").requires_grad_() for n, t in block_weights(width, heads, head, 6).items()}
+    x = torch.randn(Bn, Tn, width, generator=gen(7)).to(BF16).to("xdna")
+    dy = torch.randn(Bn, Tn, width, generator=gen(8)).to(BF16).to("xdna")
+    g = torch.tensor([-0.3, -0.01], device="xdna")
+    lengths = torch.tensor([300, 171], device="xdna")
+    pool = torch.zeros(4, heads, head, head, device="xdna")
+    slots = torch.tensor([2, 0], device="xdna")
+
+    def step():
+        (y, s), state = block(T, p, x, g, heads, head, None, lengths)
+        grads = torch.autograd.grad([y, s], list(p.values()), [dy, dy])
+        with torch.no_grad():
+            pool[:2].copy_(state.detach())
+            qs = x[:, :3].reshape(Bn, 3, heads, head)
+            o = T.decay_attention_step(qs[:, 0], qs[:, 1], qs[:, 2], g, pool, slots)
+        return [y.detach(), s.detach(), o, *grads]
+
+    eager = [t.cpu() for t in step()]
+    pool_after = pool.cpu()
+    for _ in range(2):
+        step()
+    graph = torch.xdna.Graph()
+    with torch.xdna.graph(graph):
+        out = step()
+    for i in range(4):
+        pool[2:].zero_()
+        graph.replay()
+        torch.xdna.synchronize()
+        for j, (a, b) in enumerate(zip(out, eager)):
+            assert same(a, b), (i, j)
+        if i == 0:
+            assert pool.shape == pool_after.shape
+        between = [t.cpu() for t in step()] if i % 2 else None  # eager work between the replays
+        del between
+    graph.reset()
+
+
+def test_refusals_on_the_device(T):
+    x, w = torch.randn(3, 8, device="xdna"), torch.ones(8, device="xdna")
+    for call, why in [
+        (lambda: T.layer_norm(x.half(), w.half()), "float32 or bfloat16"), (lambda: T.layer_norm(x, w[:4]), "weight and bias"),
+        (lambda: T.layer_norm(x, w, w.bfloat16()), "weight and bias"), (lambda: T.layer_norm(x.bfloat16(), w, w.bfloat16()), "one type"),
+        (lambda: T.layer_norm(x, eps=-1.0), "eps"), (lambda: T.layer_norm(x, eps=math.inf), "eps"), (lambda: T.layer_norm(x, eps=1e39), "eps"),
+        (lambda: T.layer_norm(x.cpu()), "xdna"), (lambda: T.add_layer_norm(x, x[:2]), "residual"), (lambda: T.add_layer_norm(x, x.bfloat16()), "residual"),
+        (lambda: T.layer_norm(x, w.cpu()), "weight and bias"), (lambda: T.layer_norm(torch.zeros((), device="xdna")), "width"),
+        (lambda: T.linear(x, x), "bfloat16"), (lambda: T.linear(x.bfloat16(), x[:, :4].bfloat16()), "weight"),
+        (lambda: T.linear(x.bfloat16(), x.bfloat16(), w), "bias"), (lambda: T.linear(x.bfloat16(), x.bfloat16(), w.bfloat16()), "bias"),
+        (lambda: T.linear(x.bfloat16(), x.bfloat16(), residual=x.bfloat16()), "residual"), (lambda: T.linear(x.bfloat16(), x.bfloat16(), activation="tanh"), "one of"),
+    ]:
+        with pytest.raises((RuntimeError, ValueError), match=why):
+            call()
+    q, k, v = (torch.zeros(2, 5, h, n, device="xdna", dtype=BF16) for h, n in ((4, 8), (2, 8), (2, 6)))
+    g, s = torch.zeros(4, device="xdna"), torch.zeros(2, 4, 8, 6, device="xdna")
+    wide = torch.zeros(2, 5, 4, 129, device="xdna", dtype=BF16)
+    A, S = T.decay_attention, T.decay_attention_step
+    q1, k1, v1 = q[:, 0], k[:, 0], v[:, 0]
+    leaf = q.clone().requires_grad_()
+    for call, why in [
+        (lambda: A(q.float(), k, v, g), "bfloat16"), (lambda: A(q, k, v[:, :4], g), "tokens"), (lambda: A(q, k[..., :4], v, g), "heads of"),
+        (lambda: A(q[:, :, :3], k, v, g[:3]), "divisor"), (lambda: A(q, k, v[:, :, :1], g), "divisor"), (lambda: A(wide, wide, wide, g), "1 to 128"),
+        (lambda: A(q, k, v, g[:2]), "log_decay"), (lambda: A(q, k, v, g.bfloat16()), "log_decay"), (lambda: A(q, k, v, g.clone().requires_grad_()), "constant"),
+        (lambda: A(q, k, v, g, s[:1]), "state"), (lambda: A(q, k, v, g, s.bfloat16()), "state"), (lambda: A(q, k, v, g, lengths=torch.zeros(3, device="xdna", dtype=torch.long)), "lengths"),
+        (lambda: A(q, k, v, g, lengths=torch.zeros(2, device="xdna")), "int64 or int32"), (lambda: A(q, k, v, g, scale=math.inf), "scale"),
+        (lambda: A(q, k, v, g, scale=math.nan), "scale"), (lambda: A(q1, k1, v1, g), "batch, tokens"), (lambda: S(q, k, v, g, s), "batch, heads"),
+        (lambda: S(q1, k1, v1, g, s[:1]), "without slots"), (lambda: S(q1, k1, v1, g, s.transpose(0, 1)), "contiguous"),
+        (lambda: S(q1, k1, v1, g, s.bfloat16()), "float32"), (lambda: S(q1, k1, v1, g, s, torch.zeros(3, device="xdna", dtype=torch.long)), "slots"),
+        (lambda: S(q1, k1, v1, g, s, torch.zeros(2, device="xdna")), "int64 or int32"), (lambda: S(leaf[:, 0], k1, v1, g, s), "no gradient"),
+        (lambda: S(q1, k1, v1, g, s.clone().requires_grad_()), "no gradient"),
+    ]:
+        with pytest.raises((RuntimeError, ValueError), match=why):
+            call()
+    r = A(leaf, k, v, g)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        torch.autograd.grad(r.out.sum(), [leaf], create_graph=True)
+
+
+def test_forward_mode_is_refused(T):
+    import torch.autograd.forward_ad as fw
+
+    x = torch.randn(3, 8, device="xdna").bfloat16()
+    q = torch.zeros(1, 3, 2, 8, device="xdna", dtype=BF16)
+    g, s = torch.zeros(2, device="xdna"), torch.zeros(1, 2, 8, 8, device="xdna")
+    with fw.dual_level():
+        d, dq = fw.make_dual(x, torch.ones_like(x)), fw.make_dual(q, torch.ones_like(q))
+        for call in (lambda: T.layer_norm(d), lambda: T.add_layer_norm(x, d), lambda: T.linear(x, d), lambda: T.linear(x, x, residual=fw.make_dual(x[:, :3].contiguous(), x[:, :3].contiguous())),
+                     lambda: T.decay_attention(q, dq, q, g), lambda: T.decay_attention_step(dq[:, 0], q[:, 0], q[:, 0], g, s)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
