@@ -144,6 +144,48 @@ struct __attribute__((packed, aligned(2))) Pix8 {
   uint32_t v[4];
 };
 
+// ---- 8 elements of a bf16 row, at any alignment --------------------------------
+
+__device__ inline Pix8 row_vec(const uint16_t* p, int n) {  // n elements, zeros after them
+  if (n >= 8) return *reinterpret_cast<const Pix8*>(p);
+  Pix8 q = {{0u, 0u, 0u, 0u}};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n) q.v[e >> 1] |= uint32_t(p[e]) << ((e & 1) * 16);
+  return q;
+}
+
+// v without its first s (0 .. 7) elements, zeros after the others
+__device__ inline Pix8 shifted(Pix8 q, int s) {
+  if (s & 4) q.v[0] = q.v[2], q.v[1] = q.v[3], q.v[2] = 0u, q.v[3] = 0u;
+  if (s & 2) q.v[0] = q.v[1], q.v[1] = q.v[2], q.v[2] = q.v[3], q.v[3] = 0u;
+  if (s & 1) {
+    q.v[0] = q.v[0] >> 16 | q.v[1] << 16;
+    q.v[1] = q.v[1] >> 16 | q.v[2] << 16;
+    q.v[2] = q.v[2] >> 16 | q.v[3] << 16;
+    q.v[3] = q.v[3] >> 16;
+  }
+  return q;
+}
+
+// n (at most 8) elements at p (none for n <= 0)
+__device__ inline void put_vec(uint16_t* p, const Pix8& v, int n) {
+  if (n >= 8) {
+    *reinterpret_cast<Pix8*>(p) = v;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n) p[e] = uint16_t(v.v[e >> 1] >> (16 * (e & 1)));
+}
+
+// two bf16 (NaN stays NaN: no canonical form is asked for here)
+__device__ inline uint32_t pack2(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
 // Most workgroups of 256 threads along a grid's x (its threads stay under 2^32).
 constexpr int64_t kMaxGridX256 = (int64_t(1) << 24) - 1;
 

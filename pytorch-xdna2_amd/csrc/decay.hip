@@ -4,7 +4,7 @@
 //
 //   S_t = a S_{t-1} + k_t^T v_t,   o_t = scale q_t S_t,   a = exp(log_decay[head]),  S: Dk x Dv
 //
-// Chunks of C = 128 tokens: with S the state before a chunk and i, j places in it,
+// Chunks of C = 64 tokens: with S the state before a chunk and i, j places in it,
 //   o_i = scale (sum over j <= i of a^(i-j) (q_i k_j) v_j + a^(i+1) q_i S),
 //   S' = a^n S + sum over j of a^(n-1-j) k_j^T v_j         (n tokens in the chunk).
 // The backward pass is three more walks of the same form.  With G_t the gradient of S_t, which
@@ -18,8 +18,9 @@
 //
 // A workgroup of four waves walks one sequence, head and 64 columns of v, the state in its registers
 // in fp32.  Rounded to bf16 are the weighted scores and the state as an operand of q S (one rounding
-// each beside the result's own, error against 64 bits 1.4 times that of the result's rounding);
-// the weighted v of the state's own sum is carried in two bf16 (16 bits), since the state is fp32.
+// each beside the result's own: error against 64 bits 1.4 times that of the result's rounding);
+// the weighted v of the state's own sum is carried in three bf16 (24 bits), since the state is fp32
+// (two leave it 2.8e-6 off).
 #include "common.h"
 #include "mfma.h"
 
@@ -28,7 +29,7 @@
 namespace xdna {
 namespace {
 
-constexpr int kC = 128;       // tokens of a chunk: 32 for each wave
+constexpr int kC = 64;        // tokens of a chunk
 constexpr int kVB = 64;       // columns of v of a workgroup
 constexpr int kMaxHead = 128;
 constexpr int kThreads = 256;
@@ -45,16 +46,17 @@ struct Heads {
 struct Walk {
   Heads q, k, v;
   int dk, dv;       // head sizes of k and q, and of v
+  int dma;          // rows of k and v can be loaded by the LDS DMA
   int vb;           // workgroups along dv
   int reverse;
   float p_scale, q_scale, kv_scale;
   void* out;        // dense [B][T][H][dv], bf16 or (wide) fp32
   int wide;
   const float* s0;  // state before the first token, [B][H] x (dk, dv by these strides), or null
-  int64_t s0_k, s0_v;
+  int s0_k, s0_v;
   float* s1;        // the state behind the last token, dense, or null
   float* local;     // segments' own states [B][H][segments - 1] x (dk, dv by these strides)
-  int64_t local_k, local_v;
+  int local_k, local_v;
 };
 
 struct DecayArgs {
@@ -66,6 +68,7 @@ struct DecayArgs {
   const void* lengths;  // null: T
   int index_bytes;
   int segments, chunks;  // of a sequence, and chunks of a segment
+  int scanned;           // Walk::local holds the states before segments 1, 2, .. (else the segments' own)
 };
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
@@ -73,33 +76,103 @@ typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 
 __device__ inline float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-__device__ inline Pix8 vec_of(const uint16_t* p, int n) {  // n elements, zeros after them
-  if (n >= 8) return *reinterpret_cast<const Pix8*>(p);
-  Pix8 q = {{0u, 0u, 0u, 0u}};
+// A value that the compiler takes for a new one: comparisons with it stay where they are written (hoisted
+// out of the chunks' loop, the rare paths' lane masks took every scalar register and more).
+__device__ inline int here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+__device__ inline void put4(float* row, int c, int d, float x, float y, float z, float w) {  // columns c .. of d
+  const float v[4] = {x, y, z, w};
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < n) q.v[e >> 1] |= uint32_t(p[e]) << ((e & 1) * 16);
-  return q;
+  for (int e = 0; e < 4; ++e)
+    if (c + e < d) row[c + e] = v[e];
 }
 
-__device__ inline uint32_t pack2(float a, float b) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+// Tiles in LDS: rows of W elements (64 or 128), in pieces of 8.  Piece p of row r is at p ^ swizzle(r): row
+// reads (32 rows, one piece each) and transposing reads (4 rows, two pieces) then fall on distinct banks.
+template <int W>
+__device__ inline int swizzle(int r) {
+  return W == 128 ? 2 * (r & 3) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
+}
+template <int W>
+__device__ inline int place(int r, int p) {
+  return r * W + ((p ^ swizzle<W>(r)) * 8);
 }
 
-// MFMA operand of a [k][row] tile in LDS: rows c0 + lane % 32, four k rows from k0 (of the lane's
-// half) on and four from k1 on
-__device__ inline bf16x8_t frag_tr(const uint16_t* tile, int pitch, int k0, int k1, int c0, int lane) {
-  const int g = lane >> 4, j = lane & 15;
-  const int c = c0 + 16 * (g & 1) + 4 * (j & 3);
-  const uint16_t* lo = tile + (k0 + (j >> 2)) * pitch + c;
-  const uint16_t* hi = tile + (k1 + (j >> 2)) * pitch + c;
+// A lane's byte offsets of the MFMA operands in a tile, of which every other read differs by an XOR or an
+// addition with constants (addresses formed one by one, hoisted out of the chunks' loop, spilled a hundred registers).
+//   row: row lane % 32, piece `half`; element 16 kk on: row ^ 32 kk.  Rows 32 on: + 32 rows.
+//   tr_lo / tr_hi: columns lane % 32 of rows 8 half + 0 .. 3 and + 4 .. 7, transposed; column tile x: ^ 64 x.
+//   pairs: the same of rows 4 half + 0 .. 3; + 8 rows: the next four.
+template <int W>
+struct LaneAt {
+  static constexpr int kRow = 2 * W;  // bytes
+  uint32_t row, tr_lo, tr_hi, pairs;
+  __device__ inline LaneAt(int lane, int c0) {  // c0: first column of the transposed reads, a multiple of 32
+    const int l32 = lane & 31, half = lane >> 5, g = lane >> 4, j = lane & 15;
+    const int c = c0 + 16 * (g & 1) + 4 * (j & 3);
+    const auto at = [&](int r) { return uint32_t(place<W>(r, c >> 3) + (c & 7)) * 2u; };
+    row = uint32_t(place<W>(l32, half)) * 2u;
+    tr_lo = at(8 * half + (j >> 2));
+    tr_hi = at(8 * half + 4 + (j >> 2));
+    pairs = at(4 * half + (j >> 2));
+  }
+};
+
+template <class T>
+__device__ inline T lds_at(uint32_t at) {
+  return *reinterpret_cast<__attribute__((address_space(3))) const T*>(at);
+}
+
+__device__ inline bf16x8_t frag_row(uint32_t at) { return as_bf16x8(lds_at<u32x4_t>(at)); }
+
+__device__ inline u32x4_t frag_tr(uint32_t lo, uint32_t hi) {
   const u32x2_t a = __builtin_bit_cast(
-      u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(lo)));
+      u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) i16x4_t*>(lo)));
   const u32x2_t b = __builtin_bit_cast(
-      u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(hi)));
-  return as_bf16x8(u32x4_t{a[0], a[1], b[0], b[1]});
+      u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) i16x4_t*>(hi)));
+  return u32x4_t{a[0], a[1], b[0], b[1]};
+}
+
+// One of the two operands that go to LDS by chunks: rows of d elements, `step` from one token of the walk to
+// the next (negative backwards).
+struct Stream {
+  const uint16_t* first;  // the segment's first token
+  int64_t step;
+  int d;
+};
+
+// Rows sh .. 63 of a chunk (tokens c0 .. of the segment) into a tile, zeros in the rows before and behind d: by
+// 16-byte LDS DMA, W / 32 instructions a wave.  The caller waits.
+template <int W>
+__device__ inline void stage_dma(const Stream& x, int c0, int sh, const uint16_t* tile, int lane, int wave) {
+  constexpr int P = W / 8, ROWS = 64 / P;  // pieces of a row, rows of an instruction
+  // the base is the lowest address: the chunk's first token, or backwards its last
+  const bool down = x.step < 0;
+  const uint16_t* base = x.first + (c0 + (down ? kC - 1 - sh : 0)) * x.step;
+  const i32x4_t rs = uniform_rsrc(lds_dma_rsrc(base, 0x7FFFFFE0));
+  const uint32_t bytes = uint32_t(down ? -x.step : x.step) * 2u;
+  const uint32_t to = lds_addr(tile) + uint32_t(wave * (W / 32)) * 1024u;
+#pragma unroll
+  for (int i = 0; i < W / 32; ++i) {
+    const int r = (wave * (W / 32) + i) * ROWS + lane / P, p = (lane % P) ^ swizzle<W>(r);
+    const uint32_t at = uint32_t(down ? kC - 1 - r : r - sh) * bytes + uint32_t(p) * 16u;
+    lds_dma16_m0(rs, to + uint32_t(i) * 1024u, r >= sh && p * 8 < x.d ? int(at) : 0x7FFFFFF0);
+  }
+}
+
+// The same for rows of any length, stride and alignment, through registers.
+template <int W>
+__device__ inline void stage_any(const Stream& x, int c0, int sh, uint16_t* tile, int tid) {
+#pragma unroll 2
+  for (int i = tid; i < kC * (W / 8); i += kThreads) {
+    const int r = i / (W / 8), p = i % (W / 8);
+    Pix8 v = {{0u, 0u, 0u, 0u}};
+    if (r >= sh && p * 8 < x.d) v = row_vec(x.first + (c0 + r - sh) * x.step + p * 8, x.d - p * 8);
+    *reinterpret_cast<uint4*>(tile + place<W>(r, p)) = make_uint4(v.v[0], v.v[1], v.v[2], v.v[3]);
+  }
 }
 
 __device__ inline int64_t length_of(const DecayArgs& a, int b) {
@@ -109,23 +182,29 @@ __device__ inline int64_t length_of(const DecayArgs& a, int b) {
 }
 
 template <int KT>
-struct Lds {
-  static constexpr int kPitch = KT + 16, vPitch = kVB + 16, sPitch = KT + 8;
-  static constexpr int kElems = kC * kPitch, vElems = kC * vPitch, sElems = kVB * sPitch;
-  static constexpr size_t bytes = size_t(kElems + vElems + sElems) * 2 + kC * sizeof(float);
+struct Lds {  // two buffers each
+  static constexpr int k = kC * KT, v = kC * kVB, s = kVB * KT;
+  static constexpr size_t bytes = size_t(2) * (k + v + s) * 2;
 };
 
 // STATE: the state of a segment by itself, from zero, and no outputs.
+//
+// Wave (tt, vt) has the outputs of tokens 32 tt .. of a chunk and columns 32 vt .. of v, as [dv][token] so that a
+// lane has one token, and of the state the same columns and half of the rows.  K and V of the next chunk are
+// loaded while one is worked on, and the state before a chunk is in LDS twice, so that a chunk has one barrier.  A
+// chunk of n < 64 tokens takes the tile's last n rows, its first ones are zeros: the weights inside a chunk, which
+// go by differences and by the distance to its end, are those of every other.
 template <int KT, bool STATE>
 __global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
   using L = Lds<KT>;
-  constexpr int KV = KT / 16, VV = kVB / 16;  // 16-byte vectors a thread of a chunk of k and v
-  constexpr int NS = KT / 64;                 // a wave's 32 x 32 tiles of the state
+  constexpr int NS = KT / 64;  // a wave's 32 x 32 tiles of the state
+  constexpr int KK = KT / 16;
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
-  uint16_t* ks = smem;               // [token][dk]
-  uint16_t* vs = ks + L::kElems;     // [token][dv]
-  uint16_t* ss = vs + L::vElems;     // [dv][dk], the state before the chunk
-  float* wt = reinterpret_cast<float*>(ss + L::sElems);  // [token] weight of v in the state's sum
+  uint16_t* const ks = smem;            // [buffer][token][dk]
+  uint16_t* const vs = ks + 2 * L::k;   // [buffer][token][dv]
+  uint16_t* const ss = vs + 2 * L::v;   // [buffer][dv][dk]
+  static_assert(L::s == L::k, "a row's place in K and in the state's tile differ by a constant");
+  constexpr uint32_t kBuf = 2 * L::k, vBuf = 2 * L::v, kS = 2 * (2 * L::k + 2 * L::v);  // bytes
 
   // workgroups of one sequence and head next to each other on one XCD (each has its own L2)
   const int n_all = int(gridDim.x), xcd = int(blockIdx.x) % 8;
@@ -141,19 +220,22 @@ __global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
+  const int vt = wave & 1, tt = wave >> 1;
   const int len = int(length_of(a, batch));
   const int seg_len = a.chunks * kC, begin = seg * seg_len;
   const int todo = max(0, min(len - begin, seg_len));  // tokens of this segment
   const int lead = w.reverse ? 0 : 1;
   float g2 = a.log_decay[head] * kLog2e;
   g2 = g2 < -1e4f ? -1e4f : g2;  // (exp(-inf) as exp(-1e4): 0, and 0 times it is 0)
-  const int d0 = vb * kVB, dvn = min(w.dv - d0, kVB);  // columns of v
+  const int d0 = vb * kVB, dk = w.dk, dv = min(w.dv - d0, kVB);  // columns of k, and of v here
 
-  const uint16_t* qp = w.q.p + batch * w.q.sb + int64_t(head / w.q.share) * w.q.sh;
-  const uint16_t* kp = w.k.p + batch * w.k.sb + int64_t(head / w.k.share) * w.k.sh;
-  const uint16_t* vp = w.v.p + batch * w.v.sb + int64_t(head / w.v.share) * w.v.sh + d0;
-  // place i of the walk is this token
-  const auto token = [&](int i) { return int64_t(w.reverse ? len - 1 - i : i); };
+  // place i of the segment is token t0 + i or, backwards, t0 - i
+  const int64_t t0 = w.reverse ? len - 1 - begin : begin;
+  const auto step = [&](int64_t st) { return w.reverse ? -st : st; };
+  const uint16_t* const qp = w.q.p + batch * w.q.sb + int64_t(head / w.q.share) * w.q.sh + t0 * w.q.st;
+  const int64_t q_step = step(w.q.st), o_step = step(int64_t(a.H) * w.dv);
+  const Stream kx = {w.k.p + batch * w.k.sb + int64_t(head / w.k.share) * w.k.sh + t0 * w.k.st, step(w.k.st), dk};
+  const Stream vx = {w.v.p + batch * w.v.sb + int64_t(head / w.v.share) * w.v.sh + t0 * w.v.st + d0, step(w.v.st), dv};
 
   // ---- tokens behind the sequence: zeros
   if constexpr (!STATE) {
@@ -161,7 +243,7 @@ __global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
     for (int64_t i = tid; i < int64_t(to - from) * kVB; i += kThreads) {
       const int64_t t = from + i / kVB;
       const int c = int(i % kVB);
-      if (c < dvn) {
+      if (c < dv) {
         const int64_t at = ((int64_t(batch) * a.T + t) * a.H + head) * w.dv + d0 + c;
         if (w.wide) static_cast<float*>(w.out)[at] = 0.0f;
         else static_cast<uint16_t*>(w.out)[at] = 0;
@@ -171,26 +253,81 @@ __global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
   const bool last = !STATE && w.s1 && seg == max(0, (len + seg_len - 1) / seg_len - 1);
   if (todo == 0 && !last && !STATE) return;
 
-  // ---- the state: tile x of this wave is dk 32 kt(x) .., dv 32 (wave % 2) ..
+  // chunk c0 .. into buffer b
+  const auto stage = [&](int c0, int b) {
+    const int sh = max(0, kC - (todo - c0));
+    if (w.dma) {
+      stage_dma<KT>(kx, c0, sh, ks + b * L::k, lane, wave);
+      stage_dma<kVB>(vx, c0, sh, vs + b * L::v, lane, wave);
+    } else {
+      stage_any<KT>(kx, c0, sh, ks + b * L::k, tid);
+      stage_any<kVB>(vx, c0, sh, vs + b * L::v, tid);
+    }
+  };
+  // q of the wave's 32 tokens: lane's token, k 16 kk + 8 half .. (those of no token are not stored; columns past the
+  // head meet zeros of k and of the state)
+  Pix8 qf[KK];
+  const auto load_q = [&](int c0) {
+    const int sh = max(0, kC - (todo - c0));
+    const uint16_t* row = qp + (c0 + max(32 * tt + l32 - sh, 0)) * q_step;
+    const int d = here(dk);
+    if (dk == KT) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(row + 16 * kk + 8 * half);
+    } else if (dk % 8 == 0) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(row + min(16 * kk + 8 * half, d - 8));
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const int c = 16 * kk + 8 * half;
+        qf[kk] = row_vec(row + min(c, d), max(d - c, 0));
+      }
+    }
+  };
+  const auto frag = [](const Pix8& v) { return as_bf16x8(u32x4_t{v.v[0], v.v[1], v.v[2], v.v[3]}); };
+  if (todo > 0) {
+    stage(0, 0);
+    if constexpr (!STATE) load_q(0);
+  }
+
+  // ---- the state: tile x of this wave is dk 32 (tt NS + x) .., dv 32 vt ..
   f32x16_t S[NS];
 #pragma unroll
   for (int x = 0; x < NS; ++x) S[x] = zero_acc();
-  const int vt = wave & 1;
-  const auto dk_of = [&](int x, int i) { return 32 * ((wave >> 1) * NS + x) + mfma_row(i, lane); };
+  const auto dk_of = [&](int x, int i) { return 32 * (tt * NS + x) + mfma_row(i, lane); };
   const int dv_of = 32 * vt + l32;
+  const uint32_t smem_at = lds_addr(smem);
+  const LaneAt<KT> k_at(lane, 32 * tt * NS);
+  const LaneAt<kVB> v_at(lane, 32 * vt);
+  const uint32_t s_to = smem_at + kS + uint32_t(place<KT>(dv_of, 4 * tt * NS)) * 2u + uint32_t(half) * 8u;
+  const auto store_state = [&](int b) {
+    const uint32_t to = s_to + uint32_t(b) * kBuf;
+#pragma unroll
+    for (int x = 0; x < NS; ++x)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(to ^ uint32_t((4 * x + q) * 16)) =
+            u32x2_t{pack2(S[x][4 * q], S[x][4 * q + 1]), pack2(S[x][4 * q + 2], S[x][4 * q + 3])};
+  };
   if constexpr (!STATE) {
-    const auto add = [&](const float* s, int64_t sk, int64_t sv) {
+    const auto add = [&](const float* s, int sk, int sv) {  // (a state's places fit 32 bits: one base for all loads)
+      const int rows = here(dk);
+      const uint32_t column = uint32_t((d0 + min(dv_of, dv - 1)) * sv);
 #pragma unroll
-      for (int x = 0; x < NS; ++x)
+      for (int x = 0; x < NS; ++x) {
+        float v[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int dk = dk_of(x, i);
-          if (dk < w.dk && dv_of < dvn) S[x][i] += s[dk * sk + (d0 + dv_of) * sv];
-        }
+        for (int i = 0; i < 16; ++i) v[i] = s[column + uint32_t(min(dk_of(x, i), rows - 1) * sk)];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[x][i] += dk_of(x, i) < rows && dv_of < dv ? v[i] : 0.0f;
+      }
     };
     const int64_t per = int64_t(w.dk) * w.dv;
-    if (w.s0) add(w.s0 + bh * per, w.s0_k, w.s0_v);
-    for (int j = 0; j < seg; ++j) {  // the segments before this one
+    if (w.s0 && !(seg > 0 && a.scanned)) add(w.s0 + bh * per, w.s0_k, w.s0_v);
+    // the segments before this one: summed up by scan_kernel, or few
+    if (seg > 0 && a.scanned) add(w.local + (bh * (a.segments - 1) + seg - 1) * per, w.local_k, w.local_v);
+    for (int j = 0; j < seg && !a.scanned; ++j) {
       const float f = pow2(g2 * float(max(0, min(len - j * seg_len, seg_len))));
 #pragma unroll
       for (int x = 0; x < NS; ++x)
@@ -198,197 +335,209 @@ __global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
         for (int i = 0; i < 16; ++i) S[x][i] *= f;
       add(w.local + (bh * (a.segments - 1) + j) * per, w.local_k, w.local_v);
     }
+    if (todo > 0) store_state(0);
   }
 
-  // ---- loads of a chunk
-  Pix8 kr[KV], vr[VV];
-  const auto load_kv = [&](int c0, int n) {
+  // ---- weights.  Of this lane's token (32 tt + l32) against the 16 tokens of its score registers, in its own 32
+  // (diag) and in the 32 before them (off[i / 4] times near[i % 4]); of v in the state's sum, for token e of the lane's
+  // 8 in the last 16: tail times far[e].  The factors' exponents are not negative, near and far the same in all lanes.
+  float diag[16], off[4], near[4], far[8];
+  const auto uniform = [](float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); };
 #pragma unroll
-    for (int j = 0; j < KV; ++j) {
-      const int i = tid + j * kThreads, r = i / (KT / 8), c = i % (KT / 8) * 8;
-      kr[j] = {{0u, 0u, 0u, 0u}};
-      if (r < n && c < w.dk) kr[j] = vec_of(kp + token(begin + c0 + r) * w.k.st + c, w.dk - c);
-    }
-#pragma unroll
-    for (int j = 0; j < VV; ++j) {
-      const int i = tid + j * kThreads, r = i / (kVB / 8), c = i % (kVB / 8) * 8;
-      vr[j] = {{0u, 0u, 0u, 0u}};
-      if (r < n && c < dvn) vr[j] = vec_of(vp + token(begin + c0 + r) * w.v.st + c, dvn - c);
-    }
-  };
-  const auto store_kv = [&]() {
-#pragma unroll
-    for (int j = 0; j < KV; ++j) {
-      const int i = tid + j * kThreads, r = i / (KT / 8), c = i % (KT / 8) * 8;
-      *reinterpret_cast<uint4*>(ks + r * L::kPitch + c) = make_uint4(kr[j].v[0], kr[j].v[1], kr[j].v[2], kr[j].v[3]);
-    }
-#pragma unroll
-    for (int j = 0; j < VV; ++j) {
-      const int i = tid + j * kThreads, r = i / (kVB / 8), c = i % (kVB / 8) * 8;
-      *reinterpret_cast<uint4*>(vs + r * L::vPitch + c) = make_uint4(vr[j].v[0], vr[j].v[1], vr[j].v[2], vr[j].v[3]);
-    }
-  };
-  const auto store_weights = [&](int n) {
-    if (tid < kC) wt[tid] = tid < n ? w.kv_scale * pow2(g2 * float(n - lead - tid)) : 0.0f;
-  };
-  const auto store_state = [&]() {
-#pragma unroll
-    for (int x = 0; x < NS; ++x)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint2*>(ss + dv_of * L::sPitch + dk_of(x, 4 * q)) =
-            make_uint2(pack2(S[x][4 * q], S[x][4 * q + 1]), pack2(S[x][4 * q + 2], S[x][4 * q + 3]));
-  };
-  // q of the wave's 32 tokens: lane's token, k 16 kk + 8 half ..
-  Pix8 qf[KT / 16];
-  const auto load_q = [&](int c0, int n) {
-    const int i = 32 * wave + l32;
-#pragma unroll
-    for (int kk = 0; kk < KT / 16; ++kk) {
-      const int c = 16 * kk + 8 * half;
-      qf[kk] = {{0u, 0u, 0u, 0u}};
-      if (i < n && c < w.dk) qf[kk] = vec_of(qp + token(begin + c0 + i) * w.q.st + c, w.dk - c);
-    }
-  };
-  const auto frag = [](const Pix8& v) { return as_bf16x8(u32x4_t{v.v[0], v.v[1], v.v[2], v.v[3]}); };
-
-  // ---- weights of this lane's token (32 wave + l32) against the 16 tokens of its score registers:
-  // inside the wave's own 32, and against the 32 before them
-  float diag[16], off[16];
-  float a32 = 0.0f, row_weight = 0.0f;
-  if constexpr (!STATE) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int s = mfma_row(i, lane);
-      diag[i] = l32 >= s ? w.p_scale * pow2(g2 * float(l32 - s)) : 0.0f;
-      off[i] = w.p_scale * pow2(g2 * float(32 + l32 - s));
-    }
-    a32 = pow2(g2 * 32.0f);
-    row_weight = w.q_scale * pow2(g2 * float(32 * wave + l32 + lead));
+  for (int i = 0; i < 16; ++i) {
+    const int apart = l32 - mfma_row(i, lane);
+    diag[i] = apart >= 0 ? w.p_scale * pow2(g2 * float(apart)) : 0.0f;
   }
-
-  int n = min(todo, kC);
-  if (todo > 0) {
-    load_kv(0, n);
-    if constexpr (!STATE) load_q(0, n);
-    store_kv();
-    store_weights(n);
-    if constexpr (!STATE) store_state();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    off[i] = w.p_scale * pow2(g2 * float(32 + l32 - mfma_row(4 * i + 3, lane)));
+    near[i] = uniform(pow2(g2 * float(3 - i)));
   }
-  __syncthreads();
-  for (int c0 = 0; c0 < todo; c0 += kC) {
-    const int next = min(todo - c0 - kC, kC);  // tokens of the next chunk
-    if (next > 0) load_kv(c0 + kC, next);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) far[e] = uniform(pow2(g2 * float(8 - lead - e)));
+  const float tail = w.kv_scale * pow2(g2 * float(8 - 8 * half));
+  const float a16 = pow2(g2 * 16.0f);
+
+  const int64_t o_at = (int64_t(batch) * a.T + t0) * a.H * w.dv + int64_t(head) * w.dv + d0;
+  int b = 0;
+  for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
+    // this wave's loads and LDS writes of the chunk have landed; the barrier publishes everyone's, and everyone has
+    // left the other buffers
+    lds_dma_wait<0>();
+    __syncthreads();
+    const bool more = c0 + kC < todo;
+    if (more) stage(c0 + kC, b ^ 1);
+    const uint32_t kb = smem_at + uint32_t(b) * kBuf, vbuf = smem_at + 2 * kBuf + uint32_t(b) * vBuf;
+    const int sh = max(0, kC - (todo - c0));
     if constexpr (!STATE) {
-      const int i = 32 * wave + l32;
-      f32x16_t o[2] = {zero_acc(), zero_acc()};  // [dv][token]
-      if (32 * wave < n) {
+      const int row = 32 * tt + l32;
+      f32x16_t o = zero_acc();  // [dv][token]
+      if (32 * tt + 32 > sh) {
+        constexpr uint32_t k32 = 32 * LaneAt<KT>::kRow;  // bytes of 32 rows
+        const uint32_t k_row = here(int(k_at.row + kb)), s_row = k_row + kS + uint32_t(vt) * k32;
+        const uint32_t v_pairs = v_at.pairs + vbuf;
+        f32x16_t p = zero_acc();  // [key token][token]
+        uint32_t pw[8];
+        const auto times_v = [&](uint32_t at) {
 #pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk)
+          for (int s = 0; s < 2; ++s)
+            o = mfma_32x32x16(as_bf16x8(frag_tr(at + (16 * s) * 128, at + (16 * s + 8) * 128)),
+                              as_bf16x8(u32x4_t{pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]}), o);
+        };
+        const float row_weight = w.q_scale * pow2(g2 * float(max(row - sh, 0) + lead));
+        if (tt == 0) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-            o[t] = mfma_32x32x16(as_bf16x8(*reinterpret_cast<const u32x4_t*>(ss + (32 * t + l32) * L::sPitch + 16 * kk + 8 * half)),
-                                 frag(qf[kk]), o[t]);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) o[t][x] *= row_weight;
-        float f = 1.0f;
-        for (int j = wave; j >= 0; --j) {
-          f32x16_t p = zero_acc();  // [key token][token]
-#pragma unroll
-          for (int kk = 0; kk < KT / 16; ++kk)
-            p = mfma_32x32x16(as_bf16x8(*reinterpret_cast<const u32x4_t*>(ks + (32 * j + l32) * L::kPitch + 16 * kk + 8 * half)),
-                              frag(qf[kk]), p);
-          uint32_t pw[8];
-          if (j == wave) {
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              pw[x] = pack2(diag[2 * x] != 0.0f ? p[2 * x] * diag[2 * x] : 0.0f,
-                            diag[2 * x + 1] != 0.0f ? p[2 * x + 1] * diag[2 * x + 1] : 0.0f);
-          } else {
-#pragma unroll
-            for (int x = 0; x < 8; ++x) pw[x] = pack2(p[2 * x] * (off[2 * x] * f), p[2 * x + 1] * (off[2 * x + 1] * f));
-            f *= a32;
+          for (int kk = 0; kk < KK; ++kk) {
+            o = mfma_32x32x16(frag_row(s_row ^ (32 * kk)), frag(qf[kk]), o);
+            p = mfma_32x32x16(frag_row(k_row ^ (32 * kk)), frag(qf[kk]), p);
           }
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const bf16x8_t pf = as_bf16x8(u32x4_t{pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]});
-            const int k0 = 32 * j + 16 * s + 4 * half;
+          for (int x = 0; x < 16; ++x) o[x] *= row_weight;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) o[t] = mfma_32x32x16(frag_tr(vs, L::vPitch, k0, k0 + 8, 32 * t, lane), pf, o[t]);
+          for (int i = 0; i < 8; ++i) pw[i] = pack2(p[2 * i] * diag[2 * i], p[2 * i + 1] * diag[2 * i + 1]);
+          times_v(v_pairs);
+        } else {
+          f32x16_t before = zero_acc();
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            before = mfma_32x32x16(frag_row(k_row ^ (32 * kk)), frag(qf[kk]), before);
+            o = mfma_32x32x16(frag_row(s_row ^ (32 * kk)), frag(qf[kk]), o);
+            p = mfma_32x32x16(frag_row((k_row ^ (32 * kk)) + k32), frag(qf[kk]), p);
           }
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[x] *= row_weight;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            pw[i] = pack2(before[2 * i] * (off[i / 2] * near[2 * i % 4]), before[2 * i + 1] * (off[i / 2] * near[(2 * i + 1) % 4]));
+          times_v(v_pairs);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pw[i] = pack2(p[2 * i] * diag[2 * i], p[2 * i + 1] * diag[2 * i + 1]);
+          times_v(v_pairs + 32 * 128);
         }
       }
-      if (next > 0) load_q(c0 + kC, next);
-      if (i < n) {
-        const int64_t at = ((int64_t(batch) * a.T + token(begin + c0 + i)) * a.H + head) * w.dv + d0;
+      if (more) load_q(c0 + kC);
+      if (row >= sh) {
+        const int64_t at = o_at + (c0 + row - sh) * o_step + 32 * vt;
+        const int d = here(dv) - 32 * vt;
         if (w.wide) {
-          float* to = static_cast<float*>(w.out) + at;
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              const int c = 32 * t + mfma_row(x, lane);
-              if (c < dvn) to[c] = o[t][x];
-            }
+          for (int x = 0; x < 16; x += 4)
+            put4(static_cast<float*>(w.out) + at, mfma_row(x, lane), d, o[x], o[x + 1], o[x + 2], o[x + 3]);
         } else {
+          // quads of 4 columns to 8 a lane: the halves of a wave (of the same 32 tokens) trade their second and first quads
           uint16_t* to = static_cast<uint16_t*>(w.out) + at;
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              const int c = 32 * t + mfma_row(x, lane);
-              if (c < dvn) to[c] = f32_to_bf16(o[t][x]);
-            }
+          for (int x = 0; x < 16; x += 8) {
+            const auto lo = __builtin_amdgcn_permlane32_swap(pack2(o[x], o[x + 1]), pack2(o[x + 4], o[x + 5]), false, false);
+            const auto hi = __builtin_amdgcn_permlane32_swap(pack2(o[x + 2], o[x + 3]), pack2(o[x + 6], o[x + 7]), false, false);
+            const int c = 2 * x + 8 * half;
+            put_vec(to + c, {{lo[0], hi[0], lo[1], hi[1]}}, d - c);
+          }
         }
       }
     }
-    // ---- the state behind the chunk
-    const float f = pow2(g2 * float(n));
+    // ---- the state behind the chunk: v weighted, in three bf16
+    const float f = pow2(g2 * float(kC - sh));
 #pragma unroll
     for (int x = 0; x < NS; ++x)
 #pragma unroll
       for (int i = 0; i < 16; ++i) S[x][i] *= f;
-    for (int s = 0; 16 * s < n; ++s) {
-      const int k0 = 16 * s + 8 * half;
-      const bf16x8_t v = frag_tr(vs, L::vPitch, k0, k0 + 4, 32 * vt, lane);
-      const u32x4_t vu = __builtin_bit_cast(u32x4_t, v);
-      const float4 w0 = *reinterpret_cast<const float4*>(wt + k0), w1 = *reinterpret_cast<const float4*>(wt + k0 + 4);
-      const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-      u32x4_t hi, lo;
+    float ahead = tail;  // times a^(16 (3 - s))
+    const uint32_t k_lo = here(int(k_at.tr_lo + kb)), k_hi = here(int(k_at.tr_hi + kb));
+    const uint32_t v_lo = v_at.tr_lo + vbuf, v_hi = v_at.tr_hi + vbuf;
+#pragma unroll 2  // (four at once spill registers, whose reloads wait for the DMA in flight)
+    for (int s = 3; s >= 0; --s) {
+      const u32x4_t vu = frag_tr(v_lo + s * 16 * 128, v_hi + s * 16 * 128);
+      bf16x8_t k[NS];
+#pragma unroll
+      for (int x = 0; x < NS; ++x)
+        k[x] = as_bf16x8(frag_tr((k_lo ^ (64 * x)) + s * 16 * LaneAt<KT>::kRow, (k_hi ^ (64 * x)) + s * 16 * LaneAt<KT>::kRow));
+      u32x4_t part[3];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x0 = __uint_as_float(vu[e] << 16) * ww[2 * e], x1 = __uint_as_float(vu[e] & 0xFFFF0000u) * ww[2 * e + 1];
-        hi[e] = pack2(x0, x1);
-        lo[e] = pack2(x0 - __uint_as_float(hi[e] << 16), x1 - __uint_as_float(hi[e] & 0xFFFF0000u));
-      }
+        float x0 = __uint_as_float(vu[e] << 16) * (far[2 * e] * ahead);
+        float x1 = __uint_as_float(vu[e] & 0xFFFF0000u) * (far[2 * e + 1] * ahead);
 #pragma unroll
-      for (int x = 0; x < NS; ++x) {
-        const bf16x8_t k = frag_tr(ks, L::kPitch, k0, k0 + 4, 32 * ((wave >> 1) * NS + x), lane);
-        S[x] = mfma_32x32x16(k, as_bf16x8(lo), S[x]);
-        S[x] = mfma_32x32x16(k, as_bf16x8(hi), S[x]);
+        for (int y = 0; y < 3; ++y) {
+          part[y][e] = pack2(x0, x1);
+          x0 -= __uint_as_float(part[y][e] << 16);
+          x1 -= __uint_as_float(part[y][e] & 0xFFFF0000u);
+        }
       }
+      ahead *= a16;
+#pragma unroll
+      for (int y = 2; y >= 0; --y)
+#pragma unroll
+        for (int x = 0; x < NS; ++x) S[x] = mfma_32x32x16(k[x], as_bf16x8(part[y]), S[x]);
     }
-    if (next > 0) {
-      __syncthreads();
-      store_kv();
-      if (next < kC) store_weights(next);
-      if constexpr (!STATE) store_state();
-      __syncthreads();
-      n = next;
-    }
+    if (!STATE && more) store_state(b ^ 1);
   }
   if (STATE || last) {
     const int64_t per = int64_t(w.dk) * w.dv;
     float* to = STATE ? w.local + (bh * n_seg + seg) * per : w.s1 + bh * per;
+    const int rows = here(dk);
+    if (dv_of < dv) {
 #pragma unroll
-    for (int x = 0; x < NS; ++x)
+      for (int x = 0; x < NS; ++x)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int dk = dk_of(x, i);
-        if (dk < w.dk && dv_of < dvn) to[int64_t(dk) * w.dv + d0 + dv_of] = S[x][i];
+        for (int i = 0; i < 16; ++i)
+          if (dk_of(x, i) < rows) to[uint32_t(dk_of(x, i) * w.dv + d0 + dv_of)] = S[x][i];
+    }
+  }
+}
+
+// The segments' own states to the states before segments 1, 2, ..: in place, a thread four elements, the
+// segments' loads four ahead.  s0: the state before the first (dense [B][H][dk][dv], or null).
+struct ScanArgs {
+  float* local;
+  const float* s0;
+  int per, count;  // elements of a state, segments - 1
+};
+
+__global__ __launch_bounds__(256) void scan_kernel(ScanArgs x, ScanArgs y, DecayArgs a) {
+  const ScanArgs& s = blockIdx.z ? y : x;
+  const int i = (int(blockIdx.x) * 256 + int(threadIdx.x)) * 4, bh = blockIdx.y;
+  if (i >= s.per) return;
+  const int n = min(4, s.per - i);
+  const int len = int(length_of(a, bh / a.H)), seg_len = a.chunks * kC;
+  float g2 = a.log_decay[bh % a.H] * kLog2e;
+  g2 = g2 < -1e4f ? -1e4f : g2;
+  float* p = s.local + int64_t(bh) * s.count * s.per + i;
+  const bool vec = s.per % 4 == 0;
+  const auto get = [&](const float* from, float (&v)[4]) {
+    if (vec) {
+      const float4 q = *reinterpret_cast<const float4*>(from);
+      v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = e < n ? from[e] : 0.0f;
+    }
+  };
+  float S[4] = {};
+  if (s.s0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) S[e] = e < n ? s.s0[int64_t(bh) * s.per + i + e] : 0.0f;
+  }
+  for (int j0 = 0; j0 < s.count; j0 += 4) {
+    float v[4][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) get(p + int64_t(min(j0 + u, s.count - 1)) * s.per, v[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + u;
+      if (j >= s.count) break;
+      const float f = pow2(g2 * float(max(0, min(len - j * seg_len, seg_len))));
+      float* to = p + int64_t(j) * s.per;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[e] = S[e] * f + v[u][e];
+      if (vec) {
+        *reinterpret_cast<float4*>(to) = make_float4(S[0], S[1], S[2], S[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < n) to[e] = S[e];
       }
+    }
   }
 }
 
@@ -548,6 +697,11 @@ size_t local_floats(const Plan& p, int64_t B, int64_t H, int64_t dk, int64_t dv)
   return size_t(p.segments - 1) * size_t(B * H) * size_t(dk * dv);
 }
 
+// 16-byte aligned rows, and offsets inside a chunk that 31 bits hold
+bool dma_rows(const Heads& h) {
+  return (reinterpret_cast<uintptr_t>(h.p) & 15) == 0 && h.sb % 8 == 0 && h.st % 8 == 0 && h.sh % 8 == 0 && h.st < (int64_t(1) << 23);
+}
+
 template <int KT, bool STATE>
 bool launch_walks(DecayArgs& a, hipStream_t st) {
   void (*f)(DecayArgs) = walk_kernel<KT, STATE>;
@@ -557,8 +711,10 @@ bool launch_walks(DecayArgs& a, hipStream_t st) {
   int64_t n = 0;
   for (int i = 0; i < a.n; ++i) {
     a.first[i] = n;
-    a.walk[i].vb = blocks64(a.walk[i].dv);
-    n += int64_t(a.B) * a.H * a.walk[i].vb * (STATE ? a.segments - 1 : a.segments);
+    Walk& w = a.walk[i];
+    w.vb = blocks64(w.dv);
+    w.dma = w.dk % 8 == 0 && w.dv % 8 == 0 && dma_rows(w.k) && dma_rows(w.v) ? 1 : 0;
+    n += int64_t(a.B) * a.H * w.vb * (STATE ? a.segments - 1 : a.segments);
   }
   f<<<unsigned(n), kThreads, Lds<KT>::bytes, st>>>(a);
   return true;
@@ -574,6 +730,22 @@ bool launch(const DecayArgs& a, const Walk* walks, int n, hipStream_t st) {
       if ((walks[i].dk > 64) == big) b.walk[b.n++] = walks[i];
     if (b.n && !(big ? launch_walks<128, STATE>(b, st) : launch_walks<64, STATE>(b, st))) return false;
   }
+  return true;
+}
+
+constexpr int kScanFrom = 5;  // segments
+
+// the segments' own states, and where they are many the states before them
+template <int N>
+bool launch_segments(DecayArgs& a, const Walk (&walks)[N], const float* const (&s0)[N], hipStream_t st) {
+  if (a.segments == 1) return true;
+  if (!launch<true>(a, walks, N, st)) return false;
+  a.scanned = a.segments >= kScanFrom ? 1 : 0;
+  if (!a.scanned) return true;
+  const int per = walks[0].dk * walks[0].dv;
+  ScanArgs s[2] = {};
+  for (int i = 0; i < N; ++i) s[i] = {walks[i].local, s0[i], per, a.segments - 1};
+  scan_kernel<<<dim3(unsigned(ceil_div(per, 1024)), unsigned(a.B * a.H), N), 256, 0, st>>>(s[0], s[1], a);
   return true;
 }
 
@@ -632,12 +804,12 @@ int xdna_decay_attention(const xdna_heads_bf16* q, const xdna_heads_bf16* k, con
   w.kv_scale = 1.0f;
   w.out = out;
   w.s0 = state;
-  w.s0_k = dv, w.s0_v = 1;
+  w.s0_k = int(dv), w.s0_v = 1;
   w.s1 = state_out;
   w.local = static_cast<float*>(workspace);
-  w.local_k = dv, w.local_v = 1;
+  w.local_k = int(dv), w.local_v = 1;
   hipStream_t st = as_stream(stream);
-  const bool ok = (p.segments == 1 || launch<true>(a, &w, 1, st)) && launch<false>(a, &w, 1, st);
+  const bool ok = launch_segments<1>(a, {w}, {state}, st) && launch<false>(a, &w, 1, st);
   return ok ? check_launch(what) : refuse(what, "the kernel's LDS size cannot be had");
 }
 
@@ -686,9 +858,9 @@ int xdna_decay_attention_bwd(const xdna_heads_bf16* dout, const float* d_state_o
   w[0].kv_scale = 1.0f;
   w[0].out = d_q;
   w[0].s0 = state;
-  w[0].s0_k = 1, w[0].s0_v = dv;
+  w[0].s0_k = 1, w[0].s0_v = int(dv);
   w[0].local = local_s;
-  w[0].local_k = 1, w[0].local_v = dv;
+  w[0].local_k = 1, w[0].local_v = int(dv);
   // dv
   w[1].q = hk, w[1].k = hq, w[1].v = hd;
   w[1].dk = int(dk), w[1].dv = int(dv);
@@ -698,29 +870,24 @@ int xdna_decay_attention_bwd(const xdna_heads_bf16* dout, const float* d_state_o
   w[1].out = group > 1 ? static_cast<void*>(wide_v) : d_v;
   w[1].wide = group > 1;
   w[1].s0 = d_state_out;
-  w[1].s0_k = dv, w[1].s0_v = 1;
+  w[1].s0_k = int(dv), w[1].s0_v = 1;
   w[1].s1 = d_state;
   w[1].local = local_r;
-  w[1].local_k = dv, w[1].local_v = 1;
+  w[1].local_k = int(dv), w[1].local_v = 1;
   // dk: G transposed
   w[2] = w[1];
   w[2].q = hv, w[2].k = hd, w[2].v = hq;
   w[2].dk = int(dv), w[2].dv = int(dk);
   w[2].out = group > 1 ? static_cast<void*>(wide_k) : d_k;
-  w[2].s0_k = 1, w[2].s0_v = dv;
+  w[2].s0_k = 1, w[2].s0_v = int(dv);
   w[2].s1 = nullptr;
-  w[2].local_k = 1, w[2].local_v = dv;
+  w[2].local_k = 1, w[2].local_v = int(dv);
   hipStream_t st = as_stream(stream);
-  bool ok = true;
-  if (p.segments > 1) {
-    // the segments' own states: S from (k, v) and G from (q, do), each [dk][dv]
-    Walk s[2] = {w[0], w[1]};
-    s[0].k = hk, s[0].v = hv;
-    s[0].dk = int(dk), s[0].dv = int(dv);
-    ok = launch<true>(a, s, 2, st);
-  }
-  ok = ok && launch<false>(a, w, 3, st);
-  if (!ok) return refuse(what, "the kernel's LDS size cannot be had");
+  // the segments' own states: S from (k, v) and G from (q, do), each [dk][dv]
+  Walk s[2] = {w[0], w[1]};
+  s[0].k = hk, s[0].v = hv;
+  s[0].dk = int(dk), s[0].dv = int(dv);
+  if (!launch_segments<2>(a, s, {state, d_state_out}, st) || !launch<false>(a, w, 3, st)) return refuse(what, "the kernel's LDS size cannot be had");
   if (group > 1) {
     const auto sum = [&](const float* from, uint16_t* to, int64_t d) {
       const unsigned grid = unsigned(std::min<int64_t>(ceil_div(B * T * G * d, int64_t(256)), 16384));

@@ -151,28 +151,6 @@ int64_t plan_tiles(TileArgs& a, int64_t nx, int64_t ny, int64_t splits, int toge
   return nx * ny * splits;
 }
 
-__device__ inline Pix8 row_vec(const uint16_t* p, int n) {  // n elements, zeros after them
-  if (n >= 8) return *reinterpret_cast<const Pix8*>(p);
-  Pix8 q = {{0u, 0u, 0u, 0u}};
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < n) q.v[e >> 1] |= uint32_t(p[e]) << ((e & 1) * 16);
-  return q;
-}
-
-// v without its first s (0 .. 7) elements, zeros after the others
-__device__ inline Pix8 shifted(Pix8 q, int s) {
-  if (s & 4) q.v[0] = q.v[2], q.v[1] = q.v[3], q.v[2] = 0u, q.v[3] = 0u;
-  if (s & 2) q.v[0] = q.v[1], q.v[1] = q.v[2], q.v[2] = q.v[3], q.v[3] = 0u;
-  if (s & 1) {
-    q.v[0] = q.v[0] >> 16 | q.v[1] << 16;
-    q.v[1] = q.v[1] >> 16 | q.v[2] << 16;
-    q.v[2] = q.v[2] >> 16 | q.v[3] << 16;
-    q.v[3] = q.v[3] >> 16;
-  }
-  return q;
-}
-
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 
@@ -304,12 +282,6 @@ __device__ inline bf16x8_t tile_frag(const uint16_t* lds, int rb, int ks, int la
         u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(hi)));
     return as_bf16x8(u32x4_t{a[0], a[1], b[0], b[1]});
   }
-}
-
-__device__ inline uint32_t pack2(float a, float b) {  // (NaN stays NaN: no canonical form is asked for here)
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
 // An fp32 value rounded to 20 bits (to nearest, ties away), in the high bits.  The sum cannot
@@ -468,17 +440,6 @@ struct __attribute__((packed, aligned(4))) Floats4 {  // 16 bytes at any fp32 el
 struct __attribute__((packed, aligned(1))) Bytes8 {
   uint32_t v[2];
 };
-
-// n (at most 8) elements at p
-__device__ inline void put_vec(uint16_t* p, const Pix8& v, int n) {
-  if (n >= 8) {
-    *reinterpret_cast<Pix8*>(p) = v;
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < n) p[e] = uint16_t(v.v[e >> 1] >> (16 * (e & 1)));
-}
 
 __device__ inline Pix8 pack_vec(const float (&v)[8]) {
   return {{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])}};

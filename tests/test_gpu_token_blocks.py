@@ -372,7 +372,7 @@ def test_linear_gradient_against_differences(T):
 
 # ---- decay attention -------------------------------------------------------------------------------
 
-CHUNK = 128
+CHUNK = 64
 
 
 def walk(q, k, v, g, s0, lead, p, qs, ks):
@@ -472,7 +472,7 @@ def check_decay(got, ref):
 
 DECAY = [  # batch, tokens, heads, kv heads, dk, dv
     (1, 1, 1, 1, 1, 1), (1, 2, 1, 1, 8, 8), (2, 5, 2, 1, 16, 16), (1, 16, 1, 1, 64, 64), (1, 31, 2, 2, 64, 64), (2, 32, 1, 1, 33, 65), (1, 33, 3, 1, 64, 128),
-    (1, 64, 1, 1, 128, 64), (1, 100, 2, 1, 7, 3), (1, 127, 2, 2, 128, 128), (2, 128, 1, 1, 100, 72), (1, 129, 2, 2, 48, 80), (1, 256, 1, 1, 128, 128),
+    (1, 64, 1, 1, 128, 64), (1, 100, 2, 1, 7, 3), (1, 65, 1, 1, 64, 8), (1, 95, 1, 1, 32, 64), (1, 97, 2, 1, 128, 32), (1, 127, 2, 2, 128, 128), (2, 128, 1, 1, 100, 72), (1, 129, 2, 2, 48, 80), (1, 256, 1, 1, 128, 128),
     (1, 300, 4, 2, 64, 64), (2, 391, 2, 1, 72, 127), (1, 777, 6, 2, 48, 80),
 ]
 
@@ -496,7 +496,7 @@ def test_decay_attention_of_ragged_batches(T, size, kind):
     sequence's end is NaN."""
     print("decay ragged", size, kind, flush=True)
     Bn, Tn = size[:2]
-    lengths = torch.tensor([0, 1, 128, 129, Tn - 1, Tn + 5, -3][:Bn], dtype=kind)
+    lengths = torch.tensor([0, 1, 64, 129, Tn - 1, Tn + 5, -3][:Bn], dtype=kind)
     v = decay_values(*size, seed=5)
     ref = decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], lengths, 0.2, v["dout"], v["dstate"])
     for b in range(Bn):

@@ -79,9 +79,9 @@ def test_decay_attention_refuses_bad_arguments():
     def ref(h):
         return ctypes.byref(h) if h is not None else None
 
-    # one sequence of 2 x 128 tokens: two segments
+    # one sequence of several chunks: segments
     need = lib.xdna_decay_workspace_bytes(1, 256, 2, 8, 8)
-    assert need > 0 and lib.xdna_decay_workspace_bytes(1, 128, 2, 8, 8) == 0 and lib.xdna_decay_workspace_bytes(0, 256, 2, 8, 8) == 0
+    assert need > 0 and lib.xdna_decay_workspace_bytes(1, 64, 2, 8, 8) == 0 and lib.xdna_decay_workspace_bytes(0, 256, 2, 8, 8) == 0
     assert lib.xdna_decay_workspace_bytes(512, 256, 2, 8, 8) == 0
 
     def fwd(q=ok, k=ok, v=ok, Bn=1, T=256, H=2, G=1, dk=8, dv=8, g=A, n=A, ib=8, scale=1.0, s=A, o=A, so=A, ws=A, have=need):
