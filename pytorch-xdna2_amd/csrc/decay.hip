@@ -16,7 +16,7 @@
 // not decayed before its first token, and ends at the first state's gradient: there the powers of a
 // that q and k take are a^i and a^(n-j) in place of a^(i+1) and a^(n-1-j) (`lead` 0 for 1).
 //
-// A workgroup of four waves walks one sequence, head and 64 columns of v, the state in its registers
+// A workgroup walks one sequence, head and 64 columns of v, the state in its registers
 // in fp32.  Rounded to bf16 are the weighted scores and the state as an operand of q S (one rounding
 // each beside the result's own: error against 64 bits 1.4 times that of the result's rounding);
 // the weighted v of the state's own sum is carried in three bf16 (24 bits), since the state is fp32
@@ -32,7 +32,6 @@ namespace {
 constexpr int kC = 64;        // tokens of a chunk
 constexpr int kVB = 64;       // columns of v of a workgroup
 constexpr int kMaxHead = 128;
-constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Heads {
@@ -78,7 +77,8 @@ __device__ inline float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A value that the compiler takes for a new one: comparisons with it stay where they are written (hoisted
 // out of the chunks' loop, the rare paths' lane masks took every scalar register and more).
-__device__ inline int here(int v) {
+template <class T>
+__device__ inline T here(T v) {
   asm volatile("" : "+v"(v));
   return v;
 }
@@ -145,29 +145,29 @@ struct Stream {
 };
 
 // Rows sh .. 63 of a chunk (tokens c0 .. of the segment) into a tile, zeros in the rows before and behind d: by
-// 16-byte LDS DMA, W / 32 instructions a wave.  The caller waits.
-template <int W>
+// 16-byte LDS DMA, by WAVES waves.  The caller waits.
+template <int W, int WAVES>
 __device__ inline void stage_dma(const Stream& x, int c0, int sh, const uint16_t* tile, int lane, int wave) {
-  constexpr int P = W / 8, ROWS = 64 / P;  // pieces of a row, rows of an instruction
+  constexpr int P = W / 8, ROWS = 64 / P, N = W / 8 / WAVES;  // pieces of a row, rows of an instruction, instructions a wave
   // the base is the lowest address: the chunk's first token, or backwards its last
   const bool down = x.step < 0;
   const uint16_t* base = x.first + (c0 + (down ? kC - 1 - sh : 0)) * x.step;
   const i32x4_t rs = uniform_rsrc(lds_dma_rsrc(base, 0x7FFFFFE0));
   const uint32_t bytes = uint32_t(down ? -x.step : x.step) * 2u;
-  const uint32_t to = lds_addr(tile) + uint32_t(wave * (W / 32)) * 1024u;
+  const uint32_t to = lds_addr(tile) + uint32_t(wave * N) * 1024u;
 #pragma unroll
-  for (int i = 0; i < W / 32; ++i) {
-    const int r = (wave * (W / 32) + i) * ROWS + lane / P, p = (lane % P) ^ swizzle<W>(r);
+  for (int i = 0; i < N; ++i) {
+    const int r = (wave * N + i) * ROWS + lane / P, p = (lane % P) ^ swizzle<W>(r);
     const uint32_t at = uint32_t(down ? kC - 1 - r : r - sh) * bytes + uint32_t(p) * 16u;
     lds_dma16_m0(rs, to + uint32_t(i) * 1024u, r >= sh && p * 8 < x.d ? int(at) : 0x7FFFFFF0);
   }
 }
 
 // The same for rows of any length, stride and alignment, through registers.
-template <int W>
+template <int W, int THREADS>
 __device__ inline void stage_any(const Stream& x, int c0, int sh, uint16_t* tile, int tid) {
 #pragma unroll 2
-  for (int i = tid; i < kC * (W / 8); i += kThreads) {
+  for (int i = tid; i < kC * (W / 8); i += THREADS) {
     const int r = i / (W / 8), p = i % (W / 8);
     Pix8 v = {{0u, 0u, 0u, 0u}};
     if (r >= sh && p * 8 < x.d) v = row_vec(x.first + (c0 + r - sh) * x.step + p * 8, x.d - p * 8);
@@ -189,21 +189,23 @@ struct Lds {  // two buffers each
 
 // STATE: the state of a segment by itself, from zero, and no outputs.
 //
-// Wave (tt, vt) has the outputs of tokens 32 tt .. of a chunk and columns 32 vt .. of v, as [dv][token] so that a
-// lane has one token, and of the state the same columns and half of the rows.  K and V of the next chunk are
-// loaded while one is worked on, and the state before a chunk is in LDS twice, so that a chunk has one barrier.  A
-// chunk of n < 64 tokens takes the tile's last n rows, its first ones are zeros: the weights inside a chunk, which
-// go by differences and by the distance to its end, are those of every other.
+// Four waves have the outputs: wave (tt, vt) tokens 32 tt .. of a chunk and columns 32 vt .. of v, as [dv][token] so that
+// a lane has one token.  Four more have the state, wave (tt, vt) half of its rows and the same columns: while the outputs
+// of a chunk are made they make the state behind it.  (All by four waves in turn, a chunk took 3.7 us with one workgroup a
+// CU: a third of it the waits of one wave a SIMD, the rest scores, weights and the state's products one after the
+// other.)  K and V of the next chunk are loaded while one is worked on, and the state before a chunk is in LDS twice, so
+// that a chunk has one barrier.  A chunk of n < 64 tokens takes the tile's last n rows, its first ones are zeros: the
+// weights inside a chunk, which go by differences and by the distance to its end, are those of every other.
 template <int KT, bool STATE>
-__global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
+__global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a) {
   using L = Lds<KT>;
+  constexpr int WAVES = STATE ? 4 : 8, THREADS = 64 * WAVES;
   constexpr int NS = KT / 64;  // a wave's 32 x 32 tiles of the state
   constexpr int KK = KT / 16;
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   uint16_t* const ks = smem;            // [buffer][token][dk]
   uint16_t* const vs = ks + 2 * L::k;   // [buffer][token][dv]
-  uint16_t* const ss = vs + 2 * L::v;   // [buffer][dv][dk]
-  static_assert(L::s == L::k, "a row's place in K and in the state's tile differ by a constant");
+  static_assert(L::s == L::k, "a row's place in K and in the state's tile ([buffer][dv][dk]) differ by a constant");
   constexpr uint32_t kBuf = 2 * L::k, vBuf = 2 * L::v, kS = 2 * (2 * L::k + 2 * L::v);  // bytes
 
   // workgroups of one sequence and head next to each other on one XCD (each has its own L2)
@@ -220,7 +222,7 @@ __global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
-  const int vt = wave & 1, tt = wave >> 1;
+  const int vt = wave & 1, tt = (wave >> 1) & 1;
   const int len = int(length_of(a, batch));
   const int seg_len = a.chunks * kC, begin = seg * seg_len;
   const int todo = max(0, min(len - begin, seg_len));  // tokens of this segment
@@ -232,15 +234,13 @@ __global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
   // place i of the segment is token t0 + i or, backwards, t0 - i
   const int64_t t0 = w.reverse ? len - 1 - begin : begin;
   const auto step = [&](int64_t st) { return w.reverse ? -st : st; };
-  const uint16_t* const qp = w.q.p + batch * w.q.sb + int64_t(head / w.q.share) * w.q.sh + t0 * w.q.st;
-  const int64_t q_step = step(w.q.st), o_step = step(int64_t(a.H) * w.dv);
   const Stream kx = {w.k.p + batch * w.k.sb + int64_t(head / w.k.share) * w.k.sh + t0 * w.k.st, step(w.k.st), dk};
   const Stream vx = {w.v.p + batch * w.v.sb + int64_t(head / w.v.share) * w.v.sh + t0 * w.v.st + d0, step(w.v.st), dv};
 
   // ---- tokens behind the sequence: zeros
   if constexpr (!STATE) {
     const int from = max(begin, len), to = min(begin + seg_len, a.T);
-    for (int64_t i = tid; i < int64_t(to - from) * kVB; i += kThreads) {
+    for (int64_t i = tid; i < int64_t(to - from) * kVB; i += THREADS) {
       const int64_t t = from + i / kVB;
       const int c = int(i % kVB);
       if (c < dv) {
@@ -257,126 +257,183 @@ __global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
   const auto stage = [&](int c0, int b) {
     const int sh = max(0, kC - (todo - c0));
     if (w.dma) {
-      stage_dma<KT>(kx, c0, sh, ks + b * L::k, lane, wave);
-      stage_dma<kVB>(vx, c0, sh, vs + b * L::v, lane, wave);
+      const int l = here(lane);
+      stage_dma<KT, WAVES>(kx, c0, sh, ks + b * L::k, l, wave);
+      stage_dma<kVB, WAVES>(vx, c0, sh, vs + b * L::v, l, wave);
     } else {
-      stage_any<KT>(kx, c0, sh, ks + b * L::k, tid);
-      stage_any<kVB>(vx, c0, sh, vs + b * L::v, tid);
+      const int t = here(tid);
+      stage_any<KT, THREADS>(kx, c0, sh, ks + b * L::k, t);
+      stage_any<kVB, THREADS>(vx, c0, sh, vs + b * L::v, t);
     }
   };
-  // q of the wave's 32 tokens: lane's token, k 16 kk + 8 half .. (those of no token are not stored; columns past the
-  // head meet zeros of k and of the state)
-  Pix8 qf[KK];
-  const auto load_q = [&](int c0) {
-    const int sh = max(0, kC - (todo - c0));
-    const uint16_t* row = qp + (c0 + max(32 * tt + l32 - sh, 0)) * q_step;
-    const int d = here(dk);
-    if (dk == KT) {
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(row + 16 * kk + 8 * half);
-    } else if (dk % 8 == 0) {
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(row + min(16 * kk + 8 * half, d - 8));
-    } else {
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const int c = 16 * kk + 8 * half;
-        qf[kk] = row_vec(row + min(c, d), max(d - c, 0));
-      }
-    }
+  // The next chunk's barrier: this wave's loads and LDS writes of it have landed; the barrier publishes everyone's, and
+  // everyone has left the other buffers, which the chunk after it takes.
+  const auto next_chunk = [&](int c0, int b) {
+    lds_dma_wait<0>();
+    __syncthreads();
+    if (c0 + kC < todo) stage(c0 + kC, b ^ 1);
   };
-  const auto frag = [](const Pix8& v) { return as_bf16x8(u32x4_t{v.v[0], v.v[1], v.v[2], v.v[3]}); };
-  if (todo > 0) {
-    stage(0, 0);
-    if constexpr (!STATE) load_q(0);
-  }
-
-  // ---- the state: tile x of this wave is dk 32 (tt NS + x) .., dv 32 vt ..
-  f32x16_t S[NS];
-#pragma unroll
-  for (int x = 0; x < NS; ++x) S[x] = zero_acc();
-  const auto dk_of = [&](int x, int i) { return 32 * (tt * NS + x) + mfma_row(i, lane); };
-  const int dv_of = 32 * vt + l32;
+  const auto uniform = [](float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); };
   const uint32_t smem_at = lds_addr(smem);
-  const LaneAt<KT> k_at(lane, 32 * tt * NS);
-  const LaneAt<kVB> v_at(lane, 32 * vt);
-  const uint32_t s_to = smem_at + kS + uint32_t(place<KT>(dv_of, 4 * tt * NS)) * 2u + uint32_t(half) * 8u;
-  const auto store_state = [&](int b) {
-    const uint32_t to = s_to + uint32_t(b) * kBuf;
+  if (todo > 0) stage(0, 0);
+
+  if (STATE || wave >= 4) {
+    // ---- the state: tile x of this wave is dk 32 (tt NS + x) .., dv 32 vt ..
+    f32x16_t S[NS];
 #pragma unroll
-    for (int x = 0; x < NS; ++x)
+    for (int x = 0; x < NS; ++x) S[x] = zero_acc();
+    const auto dk_of = [&](int x, int i) { return 32 * (tt * NS + x) + mfma_row(i, lane); };
+    const int dv_of = 32 * vt + l32;
+    const LaneAt<KT> k_at(lane, 32 * tt * NS);
+    const LaneAt<kVB> v_at(lane, 32 * vt);
+    const uint32_t s_to = smem_at + kS + uint32_t(place<KT>(dv_of, 4 * tt * NS)) * 2u + uint32_t(half) * 8u;
+    const auto store_state = [&](int b) {
+      const uint32_t to = s_to + uint32_t(b) * kBuf;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(to ^ uint32_t((4 * x + q) * 16)) =
-            u32x2_t{pack2(S[x][4 * q], S[x][4 * q + 1]), pack2(S[x][4 * q + 2], S[x][4 * q + 3])};
-  };
-  if constexpr (!STATE) {
-    const auto add = [&](const float* s, int sk, int sv) {  // (a state's places fit 32 bits: one base for all loads)
-      const int rows = here(dk);
-      const uint32_t column = uint32_t((d0 + min(dv_of, dv - 1)) * sv);
+      for (int x = 0; x < NS; ++x)
 #pragma unroll
-      for (int x = 0; x < NS; ++x) {
-        float v[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = s[column + uint32_t(min(dk_of(x, i), rows - 1) * sk)];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) S[x][i] += dk_of(x, i) < rows && dv_of < dv ? v[i] : 0.0f;
-      }
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(to ^ uint32_t((4 * x + q) * 16)) =
+              u32x2_t{pack2(S[x][4 * q], S[x][4 * q + 1]), pack2(S[x][4 * q + 2], S[x][4 * q + 3])};
     };
-    const int64_t per = int64_t(w.dk) * w.dv;
-    if (w.s0 && !(seg > 0 && a.scanned)) add(w.s0 + bh * per, w.s0_k, w.s0_v);
-    // the segments before this one: summed up by scan_kernel, or few
-    if (seg > 0 && a.scanned) add(w.local + (bh * (a.segments - 1) + seg - 1) * per, w.local_k, w.local_v);
-    for (int j = 0; j < seg && !a.scanned; ++j) {
-      const float f = pow2(g2 * float(max(0, min(len - j * seg_len, seg_len))));
+    if constexpr (!STATE) {
+      const auto add = [&](const float* s, int sk, int sv) {  // (a state's places fit 32 bits: one base for all loads)
+        const int rows = here(dk);
+        const uint32_t column = uint32_t((d0 + min(dv_of, dv - 1)) * sv);
+#pragma unroll
+        for (int x = 0; x < NS; ++x) {
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = s[column + uint32_t(min(dk_of(x, i), rows - 1) * sk)];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) S[x][i] += dk_of(x, i) < rows && dv_of < dv ? v[i] : 0.0f;
+        }
+      };
+      const int64_t per = int64_t(w.dk) * w.dv;
+      if (w.s0 && !(seg > 0 && a.scanned)) add(w.s0 + bh * per, w.s0_k, w.s0_v);
+      // the segments before this one: summed up by scan_kernel, or few
+      if (seg > 0 && a.scanned) add(w.local + (bh * (a.segments - 1) + seg - 1) * per, w.local_k, w.local_v);
+      for (int j = 0; j < seg && !a.scanned; ++j) {
+        const float f = pow2(g2 * float(max(0, min(len - j * seg_len, seg_len))));
+#pragma unroll
+        for (int x = 0; x < NS; ++x)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) S[x][i] *= f;
+        add(w.local + (bh * (a.segments - 1) + j) * per, w.local_k, w.local_v);
+      }
+      if (todo > 0) store_state(0);
+    }
+    // weights of v for token e of the lane's 8 of the last 16: tail times far[e], the same in all lanes (no exponent is
+    // negative)
+    float far[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) far[e] = uniform(pow2(g2 * float(8 - lead - e)));
+    const float tail = w.kv_scale * pow2(g2 * float(8 - 8 * half)), a16 = pow2(g2 * 16.0f);
+    int b = 0;
+    for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
+      next_chunk(c0, b);
+      const uint32_t kb = smem_at + uint32_t(b) * kBuf, vbuf = smem_at + 2 * kBuf + uint32_t(b) * vBuf;
+      const float f = pow2(g2 * float(min(todo - c0, kC)));
 #pragma unroll
       for (int x = 0; x < NS; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i) S[x][i] *= f;
-      add(w.local + (bh * (a.segments - 1) + j) * per, w.local_k, w.local_v);
+      float ahead = tail;  // times a^(16 (3 - s))
+      const uint32_t k_lo = here(int(k_at.tr_lo + kb)), k_hi = here(int(k_at.tr_hi + kb));
+      const uint32_t v_lo = v_at.tr_lo + vbuf, v_hi = v_at.tr_hi + vbuf;
+#pragma unroll 2
+      for (int s = 3; s >= 0; --s) {
+        const u32x4_t vu = frag_tr(v_lo + s * 16 * 128, v_hi + s * 16 * 128);
+        bf16x8_t k[NS];
+#pragma unroll
+        for (int x = 0; x < NS; ++x)
+          k[x] = as_bf16x8(frag_tr((k_lo ^ (64 * x)) + s * 16 * LaneAt<KT>::kRow, (k_hi ^ (64 * x)) + s * 16 * LaneAt<KT>::kRow));
+        u32x4_t part[3];  // v weighted, in three bf16
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x0 = __uint_as_float(vu[e] << 16) * (far[2 * e] * ahead);
+          float x1 = __uint_as_float(vu[e] & 0xFFFF0000u) * (far[2 * e + 1] * ahead);
+#pragma unroll
+          for (int y = 0; y < 3; ++y) {
+            part[y][e] = pack2(x0, x1);
+            x0 -= __uint_as_float(part[y][e] << 16);
+            x1 -= __uint_as_float(part[y][e] & 0xFFFF0000u);
+          }
+        }
+        ahead *= a16;
+#pragma unroll
+        for (int y = 2; y >= 0; --y)
+#pragma unroll
+          for (int x = 0; x < NS; ++x) S[x] = mfma_32x32x16(k[x], as_bf16x8(part[y]), S[x]);
+      }
+      if (!STATE && c0 + kC < todo) store_state(b ^ 1);
     }
-    if (todo > 0) store_state(0);
-  }
-
-  // ---- weights.  Of this lane's token (32 tt + l32) against the 16 tokens of its score registers, in its own 32
-  // (diag) and in the 32 before them (off[i / 4] times near[i % 4]); of v in the state's sum, for token e of the lane's
-  // 8 in the last 16: tail times far[e].  The factors' exponents are not negative, near and far the same in all lanes.
-  float diag[16], off[4], near[4], far[8];
-  const auto uniform = [](float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); };
+    if (STATE || last) {
+      const int64_t per = int64_t(w.dk) * w.dv;
+      float* to = STATE ? w.local + (bh * n_seg + seg) * per : w.s1 + bh * per;
+      const int rows = here(dk);
+      if (dv_of < dv) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int apart = l32 - mfma_row(i, lane);
-    diag[i] = apart >= 0 ? w.p_scale * pow2(g2 * float(apart)) : 0.0f;
-  }
+        for (int x = 0; x < NS; ++x)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    off[i] = w.p_scale * pow2(g2 * float(32 + l32 - mfma_row(4 * i + 3, lane)));
-    near[i] = uniform(pow2(g2 * float(3 - i)));
-  }
+          for (int i = 0; i < 16; ++i)
+            if (dk_of(x, i) < rows) to[uint32_t(dk_of(x, i) * w.dv + d0 + dv_of)] = S[x][i];
+      }
+    }
+  } else if constexpr (!STATE) {
+    // ---- the outputs
+    const uint16_t* const qp = w.q.p + batch * w.q.sb + int64_t(head / w.q.share) * w.q.sh + t0 * w.q.st;
+    const int64_t q_step = step(w.q.st), o_step = step(int64_t(a.H) * w.dv);
+    const int64_t o_at = (int64_t(batch) * a.T + t0) * a.H * w.dv + int64_t(head) * w.dv + d0 + 32 * vt;
+    // q of the wave's 32 tokens: lane's token, k 16 kk + 8 half .. (those of no token are not stored; columns past the
+    // head meet zeros of k and of the state)
+    Pix8 qf[KK];
+    const auto load_q = [&](int c0) {
+      const int sh = max(0, kC - (todo - c0));
+      const uint16_t* row = qp + (c0 + max(32 * tt + l32 - sh, 0)) * q_step;
+      const int d = here(dk);
+      if (dk == KT) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) far[e] = uniform(pow2(g2 * float(8 - lead - e)));
-  const float tail = w.kv_scale * pow2(g2 * float(8 - 8 * half));
-  const float a16 = pow2(g2 * 16.0f);
-
-  const int64_t o_at = (int64_t(batch) * a.T + t0) * a.H * w.dv + int64_t(head) * w.dv + d0;
-  int b = 0;
-  for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
-    // this wave's loads and LDS writes of the chunk have landed; the barrier publishes everyone's, and everyone has
-    // left the other buffers
-    lds_dma_wait<0>();
-    __syncthreads();
-    const bool more = c0 + kC < todo;
-    if (more) stage(c0 + kC, b ^ 1);
-    const uint32_t kb = smem_at + uint32_t(b) * kBuf, vbuf = smem_at + 2 * kBuf + uint32_t(b) * vBuf;
-    const int sh = max(0, kC - (todo - c0));
-    if constexpr (!STATE) {
-      const int row = 32 * tt + l32;
+        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(row + 16 * kk + 8 * half);
+      } else if (dk % 8 == 0) {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(row + min(16 * kk + 8 * half, d - 8));
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const int c = 16 * kk + 8 * half;
+          qf[kk] = row_vec(row + min(c, d), max(d - c, 0));
+        }
+      }
+    };
+    const auto frag = [](const Pix8& v) { return as_bf16x8(u32x4_t{v.v[0], v.v[1], v.v[2], v.v[3]}); };
+    if (todo > 0) load_q(0);
+    // weights of this lane's token (32 tt + l32) against the 16 tokens of its score registers, in its own 32 (diag) and
+    // in the 32 before them (off[i / 4] times near[i % 4], the same in all lanes; no exponent is negative)
+    float diag[16], off[4], near[4];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int apart = l32 - mfma_row(i, lane);
+      diag[i] = apart >= 0 ? w.p_scale * pow2(g2 * float(apart)) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      off[i] = w.p_scale * pow2(g2 * float(32 + l32 - mfma_row(4 * i + 3, lane)));
+      near[i] = uniform(pow2(g2 * float(3 - i)));
+    }
+    const LaneAt<KT> k_at(lane, 0);
+    const LaneAt<kVB> v_at(lane, 32 * vt);
+    constexpr uint32_t k32 = 32 * LaneAt<KT>::kRow;  // bytes of 32 rows
+    const int row = 32 * tt + l32;
+    int b = 0;
+    for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
+      next_chunk(c0, b);
+      const uint32_t kb = smem_at + uint32_t(b) * kBuf, vbuf = smem_at + 2 * kBuf + uint32_t(b) * vBuf;
+      const int sh = max(0, kC - (todo - c0));
       f32x16_t o = zero_acc();  // [dv][token]
       if (32 * tt + 32 > sh) {
-        constexpr uint32_t k32 = 32 * LaneAt<KT>::kRow;  // bytes of 32 rows
         const uint32_t k_row = here(int(k_at.row + kb)), s_row = k_row + kS + uint32_t(vt) * k32;
         const uint32_t v_pairs = v_at.pairs + vbuf;
-        f32x16_t p = zero_acc();  // [key token][token]
         uint32_t pw[8];
         const auto times_v = [&](uint32_t at) {
 #pragma unroll
@@ -385,39 +442,34 @@ __global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
                               as_bf16x8(u32x4_t{pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]}), o);
         };
         const float row_weight = w.q_scale * pow2(g2 * float(max(row - sh, 0) + lead));
-        if (tt == 0) {
+        f32x16_t p = zero_acc();  // [key token][token]
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            o = mfma_32x32x16(frag_row(s_row ^ (32 * kk)), frag(qf[kk]), o);
-            p = mfma_32x32x16(frag_row(k_row ^ (32 * kk)), frag(qf[kk]), p);
-          }
-#pragma unroll
-          for (int x = 0; x < 16; ++x) o[x] *= row_weight;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pw[i] = pack2(p[2 * i] * diag[2 * i], p[2 * i + 1] * diag[2 * i + 1]);
-          times_v(v_pairs);
-        } else {
-          f32x16_t before = zero_acc();
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            before = mfma_32x32x16(frag_row(k_row ^ (32 * kk)), frag(qf[kk]), before);
-            o = mfma_32x32x16(frag_row(s_row ^ (32 * kk)), frag(qf[kk]), o);
-            p = mfma_32x32x16(frag_row((k_row ^ (32 * kk)) + k32), frag(qf[kk]), p);
-          }
-#pragma unroll
-          for (int x = 0; x < 16; ++x) o[x] *= row_weight;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            pw[i] = pack2(before[2 * i] * (off[i / 2] * near[2 * i % 4]), before[2 * i + 1] * (off[i / 2] * near[(2 * i + 1) % 4]));
-          times_v(v_pairs);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pw[i] = pack2(p[2 * i] * diag[2 * i], p[2 * i + 1] * diag[2 * i + 1]);
-          times_v(v_pairs + 32 * 128);
+        for (int kk = 0; kk < KK; ++kk) {
+          o = mfma_32x32x16(frag_row(s_row ^ (32 * kk)), frag(qf[kk]), o);
+          p = mfma_32x32x16(frag_row(k_row ^ (32 * kk)), frag(qf[kk]), p);
         }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[x] *= row_weight;
+        if (tt == 1) {  // those were the first 32 keys'
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float f = here(off[q]);
+#pragma unroll
+            for (int i = 2 * q; i < 2 * q + 2; ++i)
+              pw[i] = pack2(p[2 * i] * (f * near[2 * i % 4]), p[2 * i + 1] * (f * near[(2 * i + 1) % 4]));
+          }
+          p = zero_acc();
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) p = mfma_32x32x16(frag_row((k_row ^ (32 * kk)) + k32), frag(qf[kk]), p);
+          times_v(v_pairs);
+        }
+        if (c0 + kC < todo) load_q(c0 + kC);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pw[i] = pack2(p[2 * i] * diag[2 * i], p[2 * i + 1] * diag[2 * i + 1]);
+        times_v(v_pairs + uint32_t(tt) * (32 * 128));
       }
-      if (more) load_q(c0 + kC);
       if (row >= sh) {
-        const int64_t at = o_at + (c0 + row - sh) * o_step + 32 * vt;
+        const int64_t at = o_at + (c0 + row - sh) * o_step;
         const int d = here(dv) - 32 * vt;
         if (w.wide) {
 #pragma unroll
@@ -435,53 +487,6 @@ __global__ __launch_bounds__(kThreads, 2) void walk_kernel(DecayArgs a) {
           }
         }
       }
-    }
-    // ---- the state behind the chunk: v weighted, in three bf16
-    const float f = pow2(g2 * float(kC - sh));
-#pragma unroll
-    for (int x = 0; x < NS; ++x)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) S[x][i] *= f;
-    float ahead = tail;  // times a^(16 (3 - s))
-    const uint32_t k_lo = here(int(k_at.tr_lo + kb)), k_hi = here(int(k_at.tr_hi + kb));
-    const uint32_t v_lo = v_at.tr_lo + vbuf, v_hi = v_at.tr_hi + vbuf;
-#pragma unroll 2  // (four at once spill registers, whose reloads wait for the DMA in flight)
-    for (int s = 3; s >= 0; --s) {
-      const u32x4_t vu = frag_tr(v_lo + s * 16 * 128, v_hi + s * 16 * 128);
-      bf16x8_t k[NS];
-#pragma unroll
-      for (int x = 0; x < NS; ++x)
-        k[x] = as_bf16x8(frag_tr((k_lo ^ (64 * x)) + s * 16 * LaneAt<KT>::kRow, (k_hi ^ (64 * x)) + s * 16 * LaneAt<KT>::kRow));
-      u32x4_t part[3];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x0 = __uint_as_float(vu[e] << 16) * (far[2 * e] * ahead);
-        float x1 = __uint_as_float(vu[e] & 0xFFFF0000u) * (far[2 * e + 1] * ahead);
-#pragma unroll
-        for (int y = 0; y < 3; ++y) {
-          part[y][e] = pack2(x0, x1);
-          x0 -= __uint_as_float(part[y][e] << 16);
-          x1 -= __uint_as_float(part[y][e] & 0xFFFF0000u);
-        }
-      }
-      ahead *= a16;
-#pragma unroll
-      for (int y = 2; y >= 0; --y)
-#pragma unroll
-        for (int x = 0; x < NS; ++x) S[x] = mfma_32x32x16(k[x], as_bf16x8(part[y]), S[x]);
-    }
-    if (!STATE && more) store_state(b ^ 1);
-  }
-  if (STATE || last) {
-    const int64_t per = int64_t(w.dk) * w.dv;
-    float* to = STATE ? w.local + (bh * n_seg + seg) * per : w.s1 + bh * per;
-    const int rows = here(dk);
-    if (dv_of < dv) {
-#pragma unroll
-      for (int x = 0; x < NS; ++x)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (dk_of(x, i) < rows) to[uint32_t(dk_of(x, i) * w.dv + d0 + dv_of)] = S[x][i];
     }
   }
 }
@@ -716,7 +721,7 @@ bool launch_walks(DecayArgs& a, hipStream_t st) {
     w.dma = w.dk % 8 == 0 && w.dv % 8 == 0 && dma_rows(w.k) && dma_rows(w.v) ? 1 : 0;
     n += int64_t(a.B) * a.H * w.vb * (STATE ? a.segments - 1 : a.segments);
   }
-  f<<<unsigned(n), kThreads, Lds<KT>::bytes, st>>>(a);
+  f<<<unsigned(n), STATE ? 256 : 512, Lds<KT>::bytes, st>>>(a);
   return true;
 }
 
