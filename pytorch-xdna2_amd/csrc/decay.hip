@@ -24,6 +24,8 @@
 #include "common.h"
 #include "mfma.h"
 
+#include <type_traits>
+
 #include "../../include/xdna_hip.h"
 
 namespace xdna {
@@ -267,9 +269,12 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
     }
   };
   // The next chunk's barrier: this wave's loads and LDS writes of it have landed; the barrier publishes everyone's, and
-  // everyone has left the other buffers, which the chunk after it takes.
-  const auto next_chunk = [&](int c0, int b) {
-    lds_dma_wait<0>();
+  // everyone has left the other buffers, which the chunk after it takes.  `behind`: memory instructions that the wave has
+  // issued since, which may be under way still (they complete in order): an output wave's two stores, behind its loads of q.
+  // (Waiting for them too, a chunk ended with a store's way to memory and back.)
+  const auto next_chunk = [&](int c0, int b, auto behind) {
+    lds_reads_wait();  // (its LDS writes too; stated here, since the compiler leaves the barrier's own wait out beside the next line's)
+    lds_dma_wait<decltype(behind)::value>();
     __syncthreads();
     if (c0 + kC < todo) stage(c0 + kC, b ^ 1);
   };
@@ -331,7 +336,7 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
     const float tail = w.kv_scale * pow2(g2 * float(8 - 8 * half)), a16 = pow2(g2 * 16.0f);
     int b = 0;
     for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
-      next_chunk(c0, b);
+      next_chunk(c0, b, std::integral_constant<int, 0>{});
       const uint32_t kb = smem_at + uint32_t(b) * kBuf, vbuf = smem_at + 2 * kBuf + uint32_t(b) * vBuf;
       const float f = pow2(g2 * float(min(todo - c0, kC)));
 #pragma unroll
@@ -427,7 +432,7 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
     const int row = 32 * tt + l32;
     int b = 0;
     for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
-      next_chunk(c0, b);
+      next_chunk(c0, b, std::integral_constant<int, 2>{});
       const uint32_t kb = smem_at + uint32_t(b) * kBuf, vbuf = smem_at + 2 * kBuf + uint32_t(b) * vBuf;
       const int sh = max(0, kC - (todo - c0));
       f32x16_t o = zero_acc();  // [dv][token]
