@@ -92,34 +92,31 @@ __device__ inline void put4(float* row, int c, int d, float x, float y, float z,
     if (c + e < d) row[c + e] = v[e];
 }
 
-// Tiles in LDS: rows of W elements (64 or 128), in pieces of 8.  Piece p of row r is at p ^ swizzle(r): row
-// reads (32 rows, one piece each) and transposing reads (4 rows, two pieces) then fall on distinct banks.
+// Tiles in LDS: rows of W elements (64 or 128), in pieces of 8.  Piece p of row r is at p ^ swizzle(r): 16 lanes of a
+// row read (16 rows x 4 pieces) and 32 of a transposing read (8 rows x 2 pieces) then fall on distinct banks.
 template <int W>
 __device__ inline int swizzle(int r) {
-  return W == 128 ? 2 * (r & 3) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
+  return W == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
 }
 template <int W>
 __device__ inline int place(int r, int p) {
   return r * W + ((p ^ swizzle<W>(r)) * 8);
 }
 
-// A lane's byte offsets of the MFMA operands in a tile, of which every other read differs by an XOR or an
-// addition with constants (addresses formed one by one, hoisted out of the chunks' loop, spilled a hundred registers).
-//   row: row lane % 32, piece `half`; element 16 kk on: row ^ 32 kk.  Rows 32 on: + 32 rows.
-//   tr_lo / tr_hi: columns lane % 32 of rows 8 half + 0 .. 3 and + 4 .. 7, transposed; column tile x: ^ 64 x.
-//   pairs: the same of rows 4 half + 0 .. 3; + 8 rows: the next four.
+// A lane's byte offsets of the operands of 16x16x32 MFMAs in a tile, of which every other read differs by an XOR or
+// an addition with constants (addresses formed one by one, hoisted out of the chunks' loop, spilled a hundred registers).
+// With l = lane % 16, g = lane / 16:
+//   row: row l, elements 8 g ..; elements 32 kk on: row ^ 64 kk; rows 16 on: + 16 rows.
+//   tr: column l of rows 4 g .. +3, transposed; columns 16 x on: tr ^ 32 x; rows 16 on: + 16 rows.  An operand's eight k
+//     are these four rows and those 16 further on (both operands of a product have the same order).
 template <int W>
 struct LaneAt {
-  static constexpr int kRow = 2 * W;  // bytes
-  uint32_t row, tr_lo, tr_hi, pairs;
-  __device__ inline LaneAt(int lane, int c0) {  // c0: first column of the transposed reads, a multiple of 32
-    const int l32 = lane & 31, half = lane >> 5, g = lane >> 4, j = lane & 15;
-    const int c = c0 + 16 * (g & 1) + 4 * (j & 3);
-    const auto at = [&](int r) { return uint32_t(place<W>(r, c >> 3) + (c & 7)) * 2u; };
-    row = uint32_t(place<W>(l32, half)) * 2u;
-    tr_lo = at(8 * half + (j >> 2));
-    tr_hi = at(8 * half + 4 + (j >> 2));
-    pairs = at(4 * half + (j >> 2));
+  static constexpr uint32_t k16 = 16 * 2 * W;  // bytes of 16 rows
+  uint32_t row, tr;
+  __device__ inline explicit LaneAt(int lane) {
+    const int l = lane & 15, g = lane >> 4;
+    row = uint32_t(place<W>(l, g)) * 2u;
+    tr = uint32_t(place<W>(4 * g + (l >> 2), (l & 3) >> 1) + 4 * (l & 1)) * 2u;
   }
 };
 
@@ -137,6 +134,11 @@ __device__ inline u32x4_t frag_tr(uint32_t lo, uint32_t hi) {
       u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) i16x4_t*>(hi)));
   return u32x4_t{a[0], a[1], b[0], b[1]};
 }
+
+__device__ inline f32x4_t mfma(const bf16x8_t& a, const bf16x8_t& b, const f32x4_t& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x4_t zero4() { return f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}; }
 
 // One of the two operands that go to LDS by chunks: rows of d elements, `step` from one token of the walk to
 // the next (negative backwards).
@@ -191,19 +193,19 @@ struct Lds {  // two buffers each
 
 // STATE: the state of a segment by itself, from zero, and no outputs.
 //
-// Four waves have the outputs: wave (tt, vt) tokens 32 tt .. of a chunk and columns 32 vt .. of v, as [dv][token] so that
-// a lane has one token.  Four more have the state, wave (tt, vt) half of its rows and the same columns: while the outputs
-// of a chunk are made they make the state behind it.  (All by four waves in turn, a chunk took 3.7 us with one workgroup a
-// CU: a third of it the waits of one wave a SIMD, the rest scores, weights and the state's products one after the
-// other.)  K and V of the next chunk are loaded while one is worked on, and the state before a chunk is in LDS twice, so
-// that a chunk has one barrier.  A chunk of n < 64 tokens takes the tile's last n rows, its first ones are zeros: the
-// weights inside a chunk, which go by differences and by the distance to its end, are those of every other.
+// Four waves have the outputs, 16 tokens of a chunk each, as [dv][token] so that a lane has one token.  Four more have
+// the state, 16 columns of v each: while the outputs of a chunk are made they make the state behind it.  (All by four
+// waves in turn, a chunk took 3.7 us with one workgroup a CU: a third of it the waits of one wave a SIMD, the rest
+// scores, weights and the state's products one after the other.)  K and V of the next chunk are loaded while one is
+// worked on, and the state before a chunk is in LDS twice, so that a chunk has one barrier.  A chunk of n < 64 tokens
+// takes the tile's last n rows, its first ones are zeros: the weights inside a chunk, which go by differences and by the
+// distance to its end, are those of every other.
 template <int KT, bool STATE>
 __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a) {
   using L = Lds<KT>;
   constexpr int WAVES = STATE ? 4 : 8, THREADS = 64 * WAVES;
-  constexpr int NS = KT / 64;  // a wave's 32 x 32 tiles of the state
-  constexpr int KK = KT / 16;
+  constexpr int NS = KT / 16;  // a wave's 16 x 16 tiles of the state
+  constexpr int KK = KT / 32;  // k-steps along a head
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   uint16_t* const ks = smem;            // [buffer][token][dk]
   uint16_t* const vs = ks + 2 * L::k;   // [buffer][token][dv]
@@ -223,8 +225,7 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
   const int64_t bh = int64_t(batch) * a.H + head;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l32 = lane & 31, half = lane >> 5;
-  const int vt = wave & 1, tt = (wave >> 1) & 1;
+  const int l16 = lane & 15, g = lane >> 4;
   const int len = int(length_of(a, batch));
   const int seg_len = a.chunks * kC, begin = seg * seg_len;
   const int todo = max(0, min(len - begin, seg_len));  // tokens of this segment
@@ -283,36 +284,35 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
   if (todo > 0) stage(0, 0);
 
   if (STATE || wave >= 4) {
-    // ---- the state: tile x of this wave is dk 32 (tt NS + x) .., dv 32 vt ..
-    f32x16_t S[NS];
+    // ---- the state: register i of tile x of this wave is dk 16 x + 4 g + i, dv 16 vt + l16
+    const int vt = STATE ? wave : wave - 4;
+    f32x4_t S[NS];
 #pragma unroll
-    for (int x = 0; x < NS; ++x) S[x] = zero_acc();
-    const auto dk_of = [&](int x, int i) { return 32 * (tt * NS + x) + mfma_row(i, lane); };
-    const int dv_of = 32 * vt + l32;
-    const LaneAt<KT> k_at(lane, 32 * tt * NS);
-    const LaneAt<kVB> v_at(lane, 32 * vt);
-    const uint32_t s_to = smem_at + kS + uint32_t(place<KT>(dv_of, 4 * tt * NS)) * 2u + uint32_t(half) * 8u;
+    for (int x = 0; x < NS; ++x) S[x] = zero4();
+    const int dv_of = 16 * vt + l16;
+    const LaneAt<KT> k_at(lane);
+    const LaneAt<kVB> v_at(lane);
+    const uint32_t s_to = smem_at + kS + uint32_t(place<KT>(dv_of, g >> 1)) * 2u + uint32_t(g & 1) * 8u;
     const auto store_state = [&](int b) {
-      const uint32_t to = s_to + uint32_t(b) * kBuf;
+      const uint32_t to = here(s_to + uint32_t(b) * kBuf);
 #pragma unroll
       for (int x = 0; x < NS; ++x)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(to ^ uint32_t((4 * x + q) * 16)) =
-              u32x2_t{pack2(S[x][4 * q], S[x][4 * q + 1]), pack2(S[x][4 * q + 2], S[x][4 * q + 3])};
+        *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(to ^ uint32_t(32 * x)) =
+            u32x2_t{pack2(S[x][0], S[x][1]), pack2(S[x][2], S[x][3])};
     };
     if constexpr (!STATE) {
       const auto add = [&](const float* s, int sk, int sv) {  // (a state's places fit 32 bits: one base for all loads)
         const int rows = here(dk);
         const uint32_t column = uint32_t((d0 + min(dv_of, dv - 1)) * sv);
+        f32x4_t v[NS];
 #pragma unroll
-        for (int x = 0; x < NS; ++x) {
-          float v[16];
+        for (int x = 0; x < NS; ++x)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = s[column + uint32_t(min(dk_of(x, i), rows - 1) * sk)];
+          for (int i = 0; i < 4; ++i) v[x][i] = s[column + uint32_t(min(16 * x + 4 * g + i, rows - 1) * sk)];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) S[x][i] += dk_of(x, i) < rows && dv_of < dv ? v[i] : 0.0f;
-        }
+        for (int x = 0; x < NS; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) S[x][i] += 16 * x + 4 * g + i < rows && dv_of < dv ? v[x][i] : 0.0f;
       };
       const int64_t per = int64_t(w.dk) * w.dv;
       if (w.s0 && !(seg > 0 && a.scanned)) add(w.s0 + bh * per, w.s0_k, w.s0_v);
@@ -321,43 +321,34 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
       for (int j = 0; j < seg && !a.scanned; ++j) {
         const float f = pow2(g2 * float(max(0, min(len - j * seg_len, seg_len))));
 #pragma unroll
-        for (int x = 0; x < NS; ++x)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) S[x][i] *= f;
+        for (int x = 0; x < NS; ++x) S[x] *= f;
         add(w.local + (bh * (a.segments - 1) + j) * per, w.local_k, w.local_v);
       }
       if (todo > 0) store_state(0);
     }
-    // weights of v for token e of the lane's 8 of the last 16: tail times far[e], the same in all lanes (no exponent is
-    // negative)
-    float far[8];
+    // weights of v for the lane's tokens 32 s + 16 y + 4 g + e of a chunk (no exponent is negative)
+    float weight[2][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) far[e] = uniform(pow2(g2 * float(8 - lead - e)));
-    const float tail = w.kv_scale * pow2(g2 * float(8 - 8 * half)), a16 = pow2(g2 * 16.0f);
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) weight[s][e] = w.kv_scale * pow2(g2 * float(kC - lead - 32 * s - 16 * (e >> 2) - 4 * g - (e & 3)));
     int b = 0;
     for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
       next_chunk(c0, b, std::integral_constant<int, 0>{});
-      const uint32_t kb = smem_at + uint32_t(b) * kBuf, vbuf = smem_at + 2 * kBuf + uint32_t(b) * vBuf;
+      const uint32_t k_tr = here(k_at.tr + smem_at + uint32_t(b) * kBuf);
+      const uint32_t v_tr = (v_at.tr ^ uint32_t(32 * vt)) + smem_at + 2 * kBuf + uint32_t(b) * vBuf;
+      constexpr uint32_t k16 = LaneAt<KT>::k16, v16 = LaneAt<kVB>::k16;
       const float f = pow2(g2 * float(min(todo - c0, kC)));
 #pragma unroll
-      for (int x = 0; x < NS; ++x)
+      for (int x = 0; x < NS; ++x) S[x] *= f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[x][i] *= f;
-      float ahead = tail;  // times a^(16 (3 - s))
-      const uint32_t k_lo = here(int(k_at.tr_lo + kb)), k_hi = here(int(k_at.tr_hi + kb));
-      const uint32_t v_lo = v_at.tr_lo + vbuf, v_hi = v_at.tr_hi + vbuf;
-#pragma unroll 2
-      for (int s = 3; s >= 0; --s) {
-        const u32x4_t vu = frag_tr(v_lo + s * 16 * 128, v_hi + s * 16 * 128);
-        bf16x8_t k[NS];
-#pragma unroll
-        for (int x = 0; x < NS; ++x)
-          k[x] = as_bf16x8(frag_tr((k_lo ^ (64 * x)) + s * 16 * LaneAt<KT>::kRow, (k_hi ^ (64 * x)) + s * 16 * LaneAt<KT>::kRow));
+      for (int s = 0; s < 2; ++s) {
+        const u32x4_t vu = frag_tr(v_tr + 2 * s * v16, v_tr + (2 * s + 1) * v16);
         u32x4_t part[3];  // v weighted, in three bf16
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float x0 = __uint_as_float(vu[e] << 16) * (far[2 * e] * ahead);
-          float x1 = __uint_as_float(vu[e] & 0xFFFF0000u) * (far[2 * e + 1] * ahead);
+          float x0 = __uint_as_float(vu[e] << 16) * weight[s][2 * e];
+          float x1 = __uint_as_float(vu[e] & 0xFFFF0000u) * weight[s][2 * e + 1];
 #pragma unroll
           for (int y = 0; y < 3; ++y) {
             part[y][e] = pack2(x0, x1);
@@ -365,11 +356,19 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
             x1 -= __uint_as_float(part[y][e] & 0xFFFF0000u);
           }
         }
-        ahead *= a16;
 #pragma unroll
-        for (int y = 2; y >= 0; --y)
+        for (int x0 = 0; x0 < NS; x0 += 4) {
+          bf16x8_t k[4];
 #pragma unroll
-          for (int x = 0; x < NS; ++x) S[x] = mfma_32x32x16(k[x], as_bf16x8(part[y]), S[x]);
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t at = k_tr ^ uint32_t(32 * (x0 + x));
+            k[x] = as_bf16x8(frag_tr(at + 2 * s * k16, at + (2 * s + 1) * k16));
+          }
+#pragma unroll
+          for (int y = 2; y >= 0; --y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) S[x0 + x] = mfma(k[x], as_bf16x8(part[y]), S[x0 + x]);
+        }
       }
       if (!STATE && c0 + kC < todo) store_state(b ^ 1);
     }
@@ -381,114 +380,119 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
 #pragma unroll
         for (int x = 0; x < NS; ++x)
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (dk_of(x, i) < rows) to[uint32_t(dk_of(x, i) * w.dv + d0 + dv_of)] = S[x][i];
+          for (int i = 0; i < 4; ++i)
+            if (16 * x + 4 * g + i < rows) to[uint32_t((16 * x + 4 * g + i) * w.dv + d0 + dv_of)] = S[x][i];
       }
     }
   } else if constexpr (!STATE) {
-    // ---- the outputs
+    // ---- the outputs of tokens 16 wave .. of a chunk
     const uint16_t* const qp = w.q.p + batch * w.q.sb + int64_t(head / w.q.share) * w.q.sh + t0 * w.q.st;
     const int64_t q_step = step(w.q.st), o_step = step(int64_t(a.H) * w.dv);
-    const int64_t o_at = (int64_t(batch) * a.T + t0) * a.H * w.dv + int64_t(head) * w.dv + d0 + 32 * vt;
-    // q of the wave's 32 tokens: lane's token, k 16 kk + 8 half .. (those of no token are not stored; columns past the
-    // head meet zeros of k and of the state)
+    const int64_t o_at = (int64_t(batch) * a.T + t0) * a.H * w.dv + int64_t(head) * w.dv + d0;
+    const int row = 16 * wave + l16;
+    // q: the lane's token, k 32 kk + 8 g .. (those of no token are not stored; columns past the head meet zeros of k and of
+    // the state)
     Pix8 qf[KK];
     const auto load_q = [&](int c0) {
       const int sh = max(0, kC - (todo - c0));
-      const uint16_t* row = qp + (c0 + max(32 * tt + l32 - sh, 0)) * q_step;
+      const uint16_t* from = qp + (c0 + max(row - sh, 0)) * q_step;
       const int d = here(dk);
       if (dk == KT) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(row + 16 * kk + 8 * half);
+        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(from + 32 * kk + 8 * g);
       } else if (dk % 8 == 0) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(row + min(16 * kk + 8 * half, d - 8));
+        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(from + min(32 * kk + 8 * g, d - 8));
       } else {
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-          const int c = 16 * kk + 8 * half;
-          qf[kk] = row_vec(row + min(c, d), max(d - c, 0));
+          const int c = 32 * kk + 8 * g;
+          qf[kk] = row_vec(from + min(c, d), max(d - c, 0));
         }
       }
     };
     const auto frag = [](const Pix8& v) { return as_bf16x8(u32x4_t{v.v[0], v.v[1], v.v[2], v.v[3]}); };
     if (todo > 0) load_q(0);
-    // weights of this lane's token (32 tt + l32) against the 16 tokens of its score registers, in its own 32 (diag) and
-    // in the 32 before them (off[i / 4] times near[i % 4], the same in all lanes; no exponent is negative)
-    float diag[16], off[4], near[4];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int apart = l32 - mfma_row(i, lane);
-      diag[i] = apart >= 0 ? w.p_scale * pow2(g2 * float(apart)) : 0.0f;
-    }
+    // weights of this lane's token against the 4 keys of its score registers: of its own 16 tokens, and of the 16
+    // before them (d tiles before: times a^(16 (d - 1)); no exponent is negative)
+    float diag[4], off[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      off[i] = w.p_scale * pow2(g2 * float(32 + l32 - mfma_row(4 * i + 3, lane)));
-      near[i] = uniform(pow2(g2 * float(3 - i)));
+      const int apart = l16 - 4 * g - i;
+      diag[i] = apart >= 0 ? w.p_scale * pow2(g2 * float(apart)) : 0.0f;
+      off[i] = w.p_scale * pow2(g2 * float(16 + apart));
     }
-    const LaneAt<KT> k_at(lane, 0);
-    const LaneAt<kVB> v_at(lane, 32 * vt);
-    constexpr uint32_t k32 = 32 * LaneAt<KT>::kRow;  // bytes of 32 rows
-    const int row = 32 * tt + l32;
+    const float a16 = uniform(pow2(g2 * 16.0f)), a32 = uniform(pow2(g2 * 32.0f));
+    const LaneAt<KT> k_at(lane);
+    const LaneAt<kVB> v_at(lane);
+    constexpr uint32_t k16 = LaneAt<KT>::k16, v16 = LaneAt<kVB>::k16;
     int b = 0;
     for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
       next_chunk(c0, b, std::integral_constant<int, 2>{});
-      const uint32_t kb = smem_at + uint32_t(b) * kBuf, vbuf = smem_at + 2 * kBuf + uint32_t(b) * vBuf;
       const int sh = max(0, kC - (todo - c0));
-      f32x16_t o = zero_acc();  // [dv][token]
-      if (32 * tt + 32 > sh) {
-        const uint32_t k_row = here(int(k_at.row + kb)), s_row = k_row + kS + uint32_t(vt) * k32;
-        const uint32_t v_pairs = v_at.pairs + vbuf;
-        uint32_t pw[8];
-        const auto times_v = [&](uint32_t at) {
+      f32x4_t o[4];  // [dv][token], four tiles of 16 columns
 #pragma unroll
-          for (int s = 0; s < 2; ++s)
-            o = mfma_32x32x16(as_bf16x8(frag_tr(at + (16 * s) * 128, at + (16 * s + 8) * 128)),
-                              as_bf16x8(u32x4_t{pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]}), o);
-        };
+      for (int j = 0; j < 4; ++j) o[j] = zero4();
+      if (16 * wave + 16 > sh) {
+        const uint32_t k_row = here(k_at.row + smem_at + uint32_t(b) * kBuf), s_row = k_row + kS;
+        const uint32_t v_tr = here(v_at.tr + smem_at + 2 * kBuf + uint32_t(b) * vBuf);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = mfma(frag_row((s_row ^ uint32_t(64 * kk)) + j * k16), frag(qf[kk]), o[j]);
         const float row_weight = w.q_scale * pow2(g2 * float(max(row - sh, 0) + lead));
-        f32x16_t p = zero_acc();  // [key token][token]
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          o = mfma_32x32x16(frag_row(s_row ^ (32 * kk)), frag(qf[kk]), o);
-          p = mfma_32x32x16(frag_row(k_row ^ (32 * kk)), frag(qf[kk]), p);
-        }
+        for (int j = 0; j < 4; ++j) o[j] *= row_weight;
+        for (int s = 0; 2 * s <= wave; ++s) {  // keys 32 s .. +31
+          const bool two = 2 * s < wave;       // (their second 16 are not all behind)
+          f32x4_t p[2] = {zero4(), zero4()};   // [key][token]
+          const uint32_t k_s = k_row + uint32_t(s) * (2 * k16);
 #pragma unroll
-        for (int x = 0; x < 16; ++x) o[x] *= row_weight;
-        if (tt == 1) {  // those were the first 32 keys'
+          for (int kk = 0; kk < KK; ++kk) p[0] = mfma(frag_row(k_s ^ uint32_t(64 * kk)), frag(qf[kk]), p[0]);
+          if (two) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float f = here(off[q]);
-#pragma unroll
-            for (int i = 2 * q; i < 2 * q + 2; ++i)
-              pw[i] = pack2(p[2 * i] * (f * near[2 * i % 4]), p[2 * i + 1] * (f * near[(2 * i + 1) % 4]));
+            for (int kk = 0; kk < KK; ++kk) p[1] = mfma(frag_row((k_s ^ uint32_t(64 * kk)) + k16), frag(qf[kk]), p[1]);
           }
-          p = zero_acc();
+          uint32_t pw[4] = {0u, 0u, 0u, 0u};
+          const auto scores = [&](int y, int apart) {  // `apart` tiles before the wave's own
+            const float f = apart == 3 ? a32 : apart == 2 ? a16 : 1.0f;
+            float x[4];
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) p = mfma_32x32x16(frag_row((k_row ^ (32 * kk)) + k32), frag(qf[kk]), p);
-          times_v(v_pairs);
+            for (int i = 0; i < 4; ++i) x[i] = p[y][i] * (apart == 0 ? diag[i] : off[i] * f);
+            pw[2 * y] = pack2(x[0], x[1]);
+            pw[2 * y + 1] = pack2(x[2], x[3]);
+          };
+          scores(0, wave - 2 * s);
+          if (two) scores(1, wave - 2 * s - 1);
+          const bf16x8_t pf = as_bf16x8(u32x4_t{pw[0], pw[1], pw[2], pw[3]});
+          const uint32_t v_s = v_tr + uint32_t(s) * (2 * v16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[j] = mfma(as_bf16x8(frag_tr(v_s ^ uint32_t(32 * j), (v_s ^ uint32_t(32 * j)) + v16)), pf, o[j]);
         }
         if (c0 + kC < todo) load_q(c0 + kC);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pw[i] = pack2(p[2 * i] * diag[2 * i], p[2 * i + 1] * diag[2 * i + 1]);
-        times_v(v_pairs + uint32_t(tt) * (32 * 128));
       }
       if (row >= sh) {
         const int64_t at = o_at + (c0 + row - sh) * o_step;
-        const int d = here(dv) - 32 * vt;
+        const int d = here(dv);
         if (w.wide) {
 #pragma unroll
-          for (int x = 0; x < 16; x += 4)
-            put4(static_cast<float*>(w.out) + at, mfma_row(x, lane), d, o[x], o[x + 1], o[x + 2], o[x + 3]);
+          for (int j = 0; j < 4; ++j)
+            put4(static_cast<float*>(w.out) + at, 16 * j + 4 * g, d, o[j][0], o[j][1], o[j][2], o[j][3]);
         } else {
-          // quads of 4 columns to 8 a lane: the halves of a wave (of the same 32 tokens) trade their second and first quads
+          // a lane's quads of columns 4 g .. of two tiles to columns 8 g .. of 32: a 64-byte run of a token's row a store
           uint16_t* to = static_cast<uint16_t*>(w.out) + at;
 #pragma unroll
-          for (int x = 0; x < 16; x += 8) {
-            const auto lo = __builtin_amdgcn_permlane32_swap(pack2(o[x], o[x + 1]), pack2(o[x + 4], o[x + 5]), false, false);
-            const auto hi = __builtin_amdgcn_permlane32_swap(pack2(o[x + 2], o[x + 3]), pack2(o[x + 6], o[x + 7]), false, false);
-            const int c = 2 * x + 8 * half;
-            put_vec(to + c, {{lo[0], hi[0], lo[1], hi[1]}}, d - c);
+          for (int j = 0; j < 4; j += 2) {
+            uint32_t q[2][2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const auto m = __builtin_amdgcn_permlane32_swap(pack2(o[j][2 * x], o[j][2 * x + 1]),
+                                                              pack2(o[j + 1][2 * x], o[j + 1][2 * x + 1]), false, false);
+              const auto n = __builtin_amdgcn_permlane16_swap(m[0], m[1], false, false);
+              q[0][x] = n[0], q[1][x] = n[1];
+            }
+            put_vec(to + 16 * j + 8 * g, {{q[0][0], q[0][1], q[1][0], q[1][1]}}, d - 16 * j - 8 * g);
           }
         }
       }
