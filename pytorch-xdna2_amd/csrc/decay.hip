@@ -24,8 +24,6 @@
 #include "common.h"
 #include "mfma.h"
 
-#include <type_traits>
-
 #include "../../include/xdna_hip.h"
 
 namespace xdna {
@@ -149,10 +147,10 @@ struct Stream {
 };
 
 // Rows sh .. 63 of a chunk (tokens c0 .. of the segment) into a tile, zeros in the rows before and behind d: by
-// 16-byte LDS DMA, by WAVES waves.  The caller waits.
-template <int W, int WAVES>
+// 16-byte LDS DMA, by four waves.  The caller waits.
+template <int W>
 __device__ inline void stage_dma(const Stream& x, int c0, int sh, const uint16_t* tile, int lane, int wave) {
-  constexpr int P = W / 8, ROWS = 64 / P, N = W / 8 / WAVES;  // pieces of a row, rows of an instruction, instructions a wave
+  constexpr int P = W / 8, ROWS = 64 / P, N = W / 32;  // pieces of a row, rows of an instruction, instructions a wave
   // the base is the lowest address: the chunk's first token, or backwards its last
   const bool down = x.step < 0;
   const uint16_t* base = x.first + (c0 + (down ? kC - 1 - sh : 0)) * x.step;
@@ -168,10 +166,10 @@ __device__ inline void stage_dma(const Stream& x, int c0, int sh, const uint16_t
 }
 
 // The same for rows of any length, stride and alignment, through registers.
-template <int W, int THREADS>
+template <int W>
 __device__ inline void stage_any(const Stream& x, int c0, int sh, uint16_t* tile, int tid) {
 #pragma unroll 2
-  for (int i = tid; i < kC * (W / 8); i += THREADS) {
+  for (int i = tid; i < kC * (W / 8); i += 256) {
     const int r = i / (W / 8), p = i % (W / 8);
     Pix8 v = {{0u, 0u, 0u, 0u}};
     if (r >= sh && p * 8 < x.d) v = row_vec(x.first + (c0 + r - sh) * x.step + p * 8, x.d - p * 8);
@@ -203,7 +201,7 @@ struct Lds {  // two buffers each
 template <int KT, bool STATE>
 __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a) {
   using L = Lds<KT>;
-  constexpr int WAVES = STATE ? 4 : 8, THREADS = 64 * WAVES;
+  constexpr int THREADS = STATE ? 256 : 512;
   constexpr int NS = KT / 16;  // a wave's 16 x 16 tiles of the state
   constexpr int KK = KT / 32;  // k-steps along a head
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
@@ -256,36 +254,25 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
   const bool last = !STATE && w.s1 && seg == max(0, (len + seg_len - 1) / seg_len - 1);
   if (todo == 0 && !last && !STATE) return;
 
-  // chunk c0 .. into buffer b
-  const auto stage = [&](int c0, int b) {
-    const int sh = max(0, kC - (todo - c0));
-    if (w.dma) {
-      const int l = here(lane);
-      stage_dma<KT, WAVES>(kx, c0, sh, ks + b * L::k, l, wave);
-      stage_dma<kVB, WAVES>(vx, c0, sh, vs + b * L::v, l, wave);
-    } else {
-      const int t = here(tid);
-      stage_any<KT, THREADS>(kx, c0, sh, ks + b * L::k, t);
-      stage_any<kVB, THREADS>(vx, c0, sh, vs + b * L::v, t);
-    }
-  };
-  // The next chunk's barrier: this wave's loads and LDS writes of it have landed; the barrier publishes everyone's, and
-  // everyone has left the other buffers, which the chunk after it takes.  `behind`: memory instructions that the wave has
-  // issued since, which may be under way still (they complete in order): an output wave's two stores, behind its loads of q.
-  // (Waiting for them too, a chunk ended with a store's way to memory and back.)
-  const auto next_chunk = [&](int c0, int b, auto behind) {
-    lds_reads_wait();  // (its LDS writes too; stated here, since the compiler leaves the barrier's own wait out beside the next line's)
-    lds_dma_wait<decltype(behind)::value>();
-    __syncthreads();
-    if (c0 + kC < todo) stage(c0 + kC, b ^ 1);
-  };
   const auto uniform = [](float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); };
   const uint32_t smem_at = lds_addr(smem);
-  if (todo > 0) stage(0, 0);
-
   if (STATE || wave >= 4) {
-    // ---- the state: register i of tile x of this wave is dk 16 x + 4 g + i, dv 16 vt + l16
+    // ---- the state: register i of tile x of this wave is dk 16 x + 4 g + i, dv 16 vt + l16.  These waves load K and V too
+    // (the others have the longer way through a chunk, and eight waves' loads at its start took a sixth of it).
     const int vt = STATE ? wave : wave - 4;
+    const auto stage = [&](int c0, int b) {  // chunk c0 .. into buffer b
+      const int sh = max(0, kC - (todo - c0));
+      if (w.dma) {
+        const int l = here(lane);
+        stage_dma<KT>(kx, c0, sh, ks + b * L::k, l, vt);
+        stage_dma<kVB>(vx, c0, sh, vs + b * L::v, l, vt);
+      } else {
+        const int t = here(64 * vt + lane);
+        stage_any<KT>(kx, c0, sh, ks + b * L::k, t);
+        stage_any<kVB>(vx, c0, sh, vs + b * L::v, t);
+      }
+    };
+    if (todo > 0) stage(0, 0);
     f32x4_t S[NS];
 #pragma unroll
     for (int x = 0; x < NS; ++x) S[x] = zero4();
@@ -334,7 +321,12 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
       for (int e = 0; e < 8; ++e) weight[s][e] = w.kv_scale * pow2(g2 * float(kC - lead - 32 * s - 16 * (e >> 2) - 4 * g - (e & 3)));
     int b = 0;
     for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
-      next_chunk(c0, b, std::integral_constant<int, 0>{});
+      // this wave's loads and LDS writes of the chunk have landed; the barrier publishes everyone's, and everyone has left
+      // the other buffers, which the chunk after it takes
+      lds_reads_wait();  // (its LDS writes; stated here, since the compiler leaves the barrier's own wait out beside the next line's)
+      lds_dma_wait<0>();
+      __syncthreads();
+      if (c0 + kC < todo) stage(c0 + kC, b ^ 1);
       const uint32_t k_tr = here(k_at.tr + smem_at + uint32_t(b) * kBuf);
       const uint32_t v_tr = (v_at.tr ^ uint32_t(32 * vt)) + smem_at + 2 * kBuf + uint32_t(b) * vBuf;
       constexpr uint32_t k16 = LaneAt<KT>::k16, v16 = LaneAt<kVB>::k16;
@@ -392,22 +384,22 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
     const int row = 16 * wave + l16;
     // q: the lane's token, k 32 kk + 8 g .. (those of no token are not stored; columns past the head meet zeros of k and of
     // the state)
-    Pix8 qf[KK];
+    Pix8 qn[KK];  // of the next chunk
     const auto load_q = [&](int c0) {
       const int sh = max(0, kC - (todo - c0));
       const uint16_t* from = qp + (c0 + max(row - sh, 0)) * q_step;
       const int d = here(dk);
       if (dk == KT) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(from + 32 * kk + 8 * g);
+        for (int kk = 0; kk < KK; ++kk) qn[kk] = *reinterpret_cast<const Pix8*>(from + 32 * kk + 8 * g);
       } else if (dk % 8 == 0) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(from + min(32 * kk + 8 * g, d - 8));
+        for (int kk = 0; kk < KK; ++kk) qn[kk] = *reinterpret_cast<const Pix8*>(from + min(32 * kk + 8 * g, d - 8));
       } else {
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           const int c = 32 * kk + 8 * g;
-          qf[kk] = row_vec(from + min(c, d), max(d - c, 0));
+          qn[kk] = row_vec(from + min(c, d), max(d - c, 0));
         }
       }
     };
@@ -428,8 +420,13 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
     constexpr uint32_t k16 = LaneAt<KT>::k16, v16 = LaneAt<kVB>::k16;
     int b = 0;
     for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
-      next_chunk(c0, b, std::integral_constant<int, 2>{});
+      lds_reads_wait();
+      __syncthreads();
       const int sh = max(0, kC - (todo - c0));
+      Pix8 qf[KK];
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) qf[kk] = qn[kk];
+      if (c0 + kC < todo) load_q(c0 + kC);
       f32x4_t o[4];  // [dv][token], four tiles of 16 columns
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = zero4();
@@ -470,7 +467,6 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
           for (int j = 0; j < 4; ++j)
             o[j] = mfma(as_bf16x8(frag_tr(v_s ^ uint32_t(32 * j), (v_s ^ uint32_t(32 * j)) + v16)), pf, o[j]);
         }
-        if (c0 + kC < todo) load_q(c0 + kC);
       }
       if (row >= sh) {
         const int64_t at = o_at + (c0 + row - sh) * o_step;
