@@ -147,23 +147,45 @@ struct Stream {
 };
 
 // Rows sh .. 63 of a chunk (tokens c0 .. of the segment) into a tile, zeros in the rows before and behind d: by
-// 16-byte LDS DMA, by four waves.  The caller waits.
+// 16-byte LDS DMA, W / 32 instructions of each of four waves.  The caller waits.
+//   A whole chunk of whole rows takes one instruction each and little else: the lane's offset in a block of rows is one of
+// two (lane_at[i % 2]), the blocks' and the chunks' are scalar.
 template <int W>
-__device__ inline void stage_dma(const Stream& x, int c0, int sh, const uint16_t* tile, int lane, int wave) {
-  constexpr int P = W / 8, ROWS = 64 / P, N = W / 32;  // pieces of a row, rows of an instruction, instructions a wave
-  // the base is the lowest address: the chunk's first token, or backwards its last
-  const bool down = x.step < 0;
-  const uint16_t* base = x.first + (c0 + (down ? kC - 1 - sh : 0)) * x.step;
-  const i32x4_t rs = uniform_rsrc(lds_dma_rsrc(base, 0x7FFFFFE0));
-  const uint32_t bytes = uint32_t(down ? -x.step : x.step) * 2u;
-  const uint32_t to = lds_addr(tile) + uint32_t(wave * N) * 1024u;
+struct Dma {
+  static constexpr int P = W / 8, ROWS = 64 / P, N = W / 32;  // pieces of a row, rows of an instruction, instructions a wave
+  uint32_t lane_at[2];
+  uint32_t bytes;  // from row to row
+  bool down;       // backwards: the chunk's last token has the lowest address
+
+  __device__ inline Dma(const Stream& x, int lane) : bytes(uint32_t(x.step < 0 ? -x.step : x.step) * 2u), down(x.step < 0) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int r = (wave * N + i) * ROWS + lane / P, p = (lane % P) ^ swizzle<W>(r);
-    const uint32_t at = uint32_t(down ? kC - 1 - r : r - sh) * bytes + uint32_t(p) * 16u;
-    lds_dma16_m0(rs, to + uint32_t(i) * 1024u, r >= sh && p * 8 < x.d ? int(at) : 0x7FFFFFF0);
+    for (int i = 0; i < 2; ++i) {
+      const int r = i * ROWS + lane / P, p = (lane % P) ^ swizzle<W>(r);
+      lane_at[i] = uint32_t(down ? ROWS - 1 - lane / P : lane / P) * bytes + uint32_t(p) * 16u;
+    }
   }
-}
+
+  __device__ inline i32x4_t rows(const Stream& x, int c0, int sh) const {
+    return uniform_rsrc(lds_dma_rsrc(x.first + (c0 + (down ? kC - 1 - sh : 0)) * x.step, 0x7FFFFFE0));
+  }
+
+  // instruction i of wave `wave`, of a whole chunk
+  __device__ inline void load(const i32x4_t& rs, const uint16_t* tile, int wave, int i) const {
+    const int block = wave * N + i;
+    const uint32_t at = uint32_t(down ? kC - (block + 1) * ROWS : block * ROWS) * bytes;
+    lds_dma16_m0(rs, lds_addr(tile) + uint32_t(block) * 1024u, int(lane_at[i % 2]), at);
+  }
+
+  __device__ inline void load_some(const Stream& x, int c0, int sh, const uint16_t* tile, int lane, int wave) const {
+    const i32x4_t rs = rows(x, c0, sh);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = (wave * N + i) * ROWS + lane / P, p = (lane % P) ^ swizzle<W>(r);
+      const uint32_t at = uint32_t(down ? kC - 1 - r : r - sh) * bytes + uint32_t(p) * 16u;
+      lds_dma16_m0(rs, lds_addr(tile) + uint32_t(wave * N + i) * 1024u, r >= sh && p * 8 < x.d ? int(at) : 0x7FFFFFF0);
+    }
+  }
+};
 
 // The same for rows of any length, stride and alignment, through registers.
 template <int W>
@@ -260,12 +282,15 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
     // ---- the state: register i of tile x of this wave is dk 16 x + 4 g + i, dv 16 vt + l16.  These waves load K and V too
     // (the others have the longer way through a chunk, and eight waves' loads at its start took a sixth of it).
     const int vt = STATE ? wave : wave - 4;
+    const Dma<KT> k_dma(kx, lane);
+    const Dma<kVB> v_dma(vx, lane);
+    const bool whole = w.dma && dk == KT && dv == kVB;
     const auto stage = [&](int c0, int b) {  // chunk c0 .. into buffer b
       const int sh = max(0, kC - (todo - c0));
       if (w.dma) {
         const int l = here(lane);
-        stage_dma<KT>(kx, c0, sh, ks + b * L::k, l, vt);
-        stage_dma<kVB>(vx, c0, sh, vs + b * L::v, l, vt);
+        k_dma.load_some(kx, c0, sh, ks + b * L::k, l, vt);
+        v_dma.load_some(vx, c0, sh, vs + b * L::v, l, vt);
       } else {
         const int t = here(64 * vt + lane);
         stage_any<KT>(kx, c0, sh, ks + b * L::k, t);
@@ -326,7 +351,10 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
       lds_reads_wait();  // (its LDS writes; stated here, since the compiler leaves the barrier's own wait out beside the next line's)
       lds_dma_wait<0>();
       __syncthreads();
-      if (c0 + kC < todo) stage(c0 + kC, b ^ 1);
+      const bool ahead = whole && c0 + 2 * kC <= todo;  // a whole chunk follows: its loads go between the products
+      if (!ahead && c0 + kC < todo) stage(c0 + kC, b ^ 1);
+      i32x4_t k_rows, v_rows;
+      if (ahead) k_rows = k_dma.rows(kx, c0 + kC, 0), v_rows = v_dma.rows(vx, c0 + kC, 0);
       const uint32_t k_tr = here(k_at.tr + smem_at + uint32_t(b) * kBuf);
       const uint32_t v_tr = (v_at.tr ^ uint32_t(32 * vt)) + smem_at + 2 * kBuf + uint32_t(b) * vBuf;
       constexpr uint32_t k16 = LaneAt<KT>::k16, v16 = LaneAt<kVB>::k16;
@@ -356,6 +384,12 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
             const uint32_t at = k_tr ^ uint32_t(32 * (x0 + x));
             k[x] = as_bf16x8(frag_tr(at + 2 * s * k16, at + (2 * s + 1) * k16));
           }
+          if (ahead) {
+            constexpr int N = Dma<KT>::N;  // (2 N products' groups: a load of k each two, of v in the first two)
+            const int at = s * (NS / 4) + x0 / 4;
+            if (NS == 8 || at < N) k_dma.load(k_rows, ks + (b ^ 1) * L::k, vt, at);
+            if (at < Dma<kVB>::N) v_dma.load(v_rows, vs + (b ^ 1) * L::v, vt, at);
+          }
 #pragma unroll
           for (int y = 2; y >= 0; --y)
 #pragma unroll
@@ -384,22 +418,22 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
     const int row = 16 * wave + l16;
     // q: the lane's token, k 32 kk + 8 g .. (those of no token are not stored; columns past the head meet zeros of k and of
     // the state)
-    Pix8 qn[KK];  // of the next chunk
+    Pix8 qf[KK];
     const auto load_q = [&](int c0) {
       const int sh = max(0, kC - (todo - c0));
       const uint16_t* from = qp + (c0 + max(row - sh, 0)) * q_step;
       const int d = here(dk);
       if (dk == KT) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qn[kk] = *reinterpret_cast<const Pix8*>(from + 32 * kk + 8 * g);
+        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(from + 32 * kk + 8 * g);
       } else if (dk % 8 == 0) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qn[kk] = *reinterpret_cast<const Pix8*>(from + min(32 * kk + 8 * g, d - 8));
+        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(from + min(32 * kk + 8 * g, d - 8));
       } else {
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           const int c = 32 * kk + 8 * g;
-          qn[kk] = row_vec(from + min(c, d), max(d - c, 0));
+          qf[kk] = row_vec(from + min(c, d), max(d - c, 0));
         }
       }
     };
@@ -423,10 +457,6 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
       lds_reads_wait();
       __syncthreads();
       const int sh = max(0, kC - (todo - c0));
-      Pix8 qf[KK];
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) qf[kk] = qn[kk];
-      if (c0 + kC < todo) load_q(c0 + kC);
       f32x4_t o[4];  // [dv][token], four tiles of 16 columns
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = zero4();
@@ -468,6 +498,7 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
             o[j] = mfma(as_bf16x8(frag_tr(v_s ^ uint32_t(32 * j), (v_s ^ uint32_t(32 * j)) + v16)), pf, o[j]);
         }
       }
+      if (c0 + kC < todo) load_q(c0 + kC);
       if (row >= sh) {
         const int64_t at = o_at + (c0 + row - sh) * o_step;
         const int d = here(dv);

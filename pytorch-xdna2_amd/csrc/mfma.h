@@ -117,6 +117,14 @@ __device__ inline void lds_dma16_m0(const i32x4_t& rs, uint32_t m0, int voff) {
                : "m0");
 }
 
+// the same with a wave-uniform offset added by the instruction (no VALU work for it)
+__device__ inline void lds_dma16_m0(const i32x4_t& rs, uint32_t m0, int voff, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(m0), "v"(voff), "s"(rs), "s"(soff)
+               : "m0");
+}
+
 // a resource descriptor made wave-uniform
 __device__ inline i32x4_t uniform_rsrc(const i32x4_t& r) {
   return i32x4_t{__builtin_amdgcn_readfirstlane(r[0]), __builtin_amdgcn_readfirstlane(r[1]),
