@@ -491,6 +491,7 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
           };
           scores(0, wave - 2 * s);
           if (two) scores(1, wave - 2 * s - 1);
+          if (2 * s + 2 > wave && c0 + kC < todo) load_q(c0 + kC);  // (after q's last use: the next chunk's into its registers)
           const bf16x8_t pf = as_bf16x8(u32x4_t{pw[0], pw[1], pw[2], pw[3]});
           const uint32_t v_s = v_tr + uint32_t(s) * (2 * v16);
 #pragma unroll
@@ -498,7 +499,6 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
             o[j] = mfma(as_bf16x8(frag_tr(v_s ^ uint32_t(32 * j), (v_s ^ uint32_t(32 * j)) + v16)), pf, o[j]);
         }
       }
-      if (c0 + kC < todo) load_q(c0 + kC);
       if (row >= sh) {
         const int64_t at = o_at + (c0 + row - sh) * o_step;
         const int d = here(dv);
