@@ -206,9 +206,9 @@ __device__ inline int64_t length_of(const DecayArgs& a, int b) {
 }
 
 template <int KT>
-struct Lds {  // two buffers each
+struct Lds {  // two buffers each; of a segment's state by itself three, and none for the state's operand form
   static constexpr int k = kC * KT, v = kC * kVB, s = kVB * KT;
-  static constexpr size_t bytes = size_t(2) * (k + v + s) * 2;
+  static constexpr size_t bytes = size_t(2) * (k + v + s) * 2, state_bytes = size_t(3) * (k + v) * 2;
 };
 
 // STATE: the state of a segment by itself, from zero, and no outputs.
@@ -227,8 +227,9 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
   constexpr int NS = KT / 16;  // a wave's 16 x 16 tiles of the state
   constexpr int KK = KT / 32;  // k-steps along a head
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
-  uint16_t* const ks = smem;            // [buffer][token][dk]
-  uint16_t* const vs = ks + 2 * L::k;   // [buffer][token][dv]
+  constexpr int BUFS = STATE ? 3 : 2;
+  uint16_t* const ks = smem;              // [buffer][token][dk]
+  uint16_t* const vs = ks + BUFS * L::k;  // [buffer][token][dv]
   static_assert(L::s == L::k, "a row's place in K and in the state's tile ([buffer][dv][dk]) differ by a constant");
   constexpr uint32_t kBuf = 2 * L::k, vBuf = 2 * L::v, kS = 2 * (2 * L::k + 2 * L::v);  // bytes
 
@@ -298,6 +299,7 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
       }
     };
     if (todo > 0) stage(0, 0);
+    if (STATE && todo > kC) stage(kC, 1);
     f32x4_t S[NS];
 #pragma unroll
     for (int x = 0; x < NS; ++x) S[x] = zero4();
@@ -345,18 +347,21 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
 #pragma unroll
       for (int e = 0; e < 8; ++e) weight[s][e] = w.kv_scale * pow2(g2 * float(kC - lead - 32 * s - 16 * (e >> 2) - 4 * g - (e & 3)));
     int b = 0;
-    for (int c0 = 0; c0 < todo; c0 += kC, b ^= 1) {
+    for (int c0 = 0; c0 < todo; c0 += kC, b = STATE ? (b == 2 ? 0 : b + 1) : b ^ 1) {
       // this wave's loads and LDS writes of the chunk have landed; the barrier publishes everyone's, and everyone has left
-      // the other buffers, which the chunk after it takes
+      // the buffers that the next loads take.  A segment's state by itself has the loads of two chunks under way (one
+      // ahead, it took 2.6 us a chunk, twice its work).
       lds_reads_wait();  // (its LDS writes; stated here, since the compiler leaves the barrier's own wait out beside the next line's)
-      lds_dma_wait<0>();
+      if (STATE && c0 + kC < todo) lds_dma_wait<Dma<KT>::N + Dma<kVB>::N>();
+      else lds_dma_wait<0>();
       __syncthreads();
-      const bool ahead = whole && c0 + 2 * kC <= todo;  // a whole chunk follows: its loads go between the products
-      if (!ahead && c0 + kC < todo) stage(c0 + kC, b ^ 1);
+      const int coming = c0 + (STATE ? 2 : 1) * kC, to = STATE ? (b == 0 ? 2 : b - 1) : b ^ 1;
+      const bool ahead = whole && coming + kC <= todo;  // a whole chunk: its loads go between the products
+      if (!ahead && coming < todo) stage(coming, to);
       i32x4_t k_rows, v_rows;
-      if (ahead) k_rows = k_dma.rows(kx, c0 + kC, 0), v_rows = v_dma.rows(vx, c0 + kC, 0);
+      if (ahead) k_rows = k_dma.rows(kx, coming, 0), v_rows = v_dma.rows(vx, coming, 0);
       const uint32_t k_tr = here(k_at.tr + smem_at + uint32_t(b) * kBuf);
-      const uint32_t v_tr = (v_at.tr ^ uint32_t(32 * vt)) + smem_at + 2 * kBuf + uint32_t(b) * vBuf;
+      const uint32_t v_tr = (v_at.tr ^ uint32_t(32 * vt)) + smem_at + BUFS * kBuf + uint32_t(b) * vBuf;
       constexpr uint32_t k16 = LaneAt<KT>::k16, v16 = LaneAt<kVB>::k16;
       const float f = pow2(g2 * float(min(todo - c0, kC)));
 #pragma unroll
@@ -387,8 +392,8 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
           if (ahead) {
             constexpr int N = Dma<KT>::N;  // (2 N products' groups: a load of k each two, of v in the first two)
             const int at = s * (NS / 4) + x0 / 4;
-            if (NS == 8 || at < N) k_dma.load(k_rows, ks + (b ^ 1) * L::k, vt, at);
-            if (at < Dma<kVB>::N) v_dma.load(v_rows, vs + (b ^ 1) * L::v, vt, at);
+            if (NS == 8 || at < N) k_dma.load(k_rows, ks + to * L::k, vt, at);
+            if (at < Dma<kVB>::N) v_dma.load(v_rows, vs + to * L::v, vt, at);
           }
 #pragma unroll
           for (int y = 2; y >= 0; --y)
@@ -528,7 +533,7 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
 }
 
 // The segments' own states to the states before segments 1, 2, ..: in place, a thread four elements, the
-// segments' loads four ahead.  s0: the state before the first (dense [B][H][dk][dv], or null).
+// segments' loads eight ahead.  s0: the state before the first (dense [B][H][dk][dv], or null).
 struct ScanArgs {
   float* local;
   const float* s0;
@@ -559,12 +564,13 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanArgs x, ScanArgs y, Decay
 #pragma unroll
     for (int e = 0; e < 4; ++e) S[e] = e < n ? s.s0[int64_t(bh) * s.per + i + e] : 0.0f;
   }
-  for (int j0 = 0; j0 < s.count; j0 += 4) {
-    float v[4][4];
+  constexpr int A = 8;
+  for (int j0 = 0; j0 < s.count; j0 += A) {
+    float v[A][4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) get(p + int64_t(min(j0 + u, s.count - 1)) * s.per, v[u]);
+    for (int u = 0; u < A; ++u) get(p + int64_t(min(j0 + u, s.count - 1)) * s.per, v[u]);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < A; ++u) {
       const int j = j0 + u;
       if (j >= s.count) break;
       const float f = pow2(g2 * float(max(0, min(len - j * seg_len, seg_len))));
@@ -745,9 +751,10 @@ bool dma_rows(const Heads& h) {
 
 template <int KT, bool STATE>
 bool launch_walks(DecayArgs& a, hipStream_t st) {
+  constexpr size_t bytes = STATE ? Lds<KT>::state_bytes : Lds<KT>::bytes;
   void (*f)(DecayArgs) = walk_kernel<KT, STATE>;
   static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             int(Lds<KT>::bytes)) == hipSuccess;
+                                             int(bytes)) == hipSuccess;
   if (!ok) return false;
   int64_t n = 0;
   for (int i = 0; i < a.n; ++i) {
@@ -757,7 +764,7 @@ bool launch_walks(DecayArgs& a, hipStream_t st) {
     w.dma = w.dk % 8 == 0 && w.dv % 8 == 0 && dma_rows(w.k) && dma_rows(w.v) ? 1 : 0;
     n += int64_t(a.B) * a.H * w.vb * (STATE ? a.segments - 1 : a.segments);
   }
-  f<<<unsigned(n), STATE ? 256 : 512, Lds<KT>::bytes, st>>>(a);
+  f<<<unsigned(n), STATE ? 256 : 512, bytes, st>>>(a);
   return true;
 }
 
