@@ -589,14 +589,23 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanArgs x, ScanArgs y, Decay
 }
 
 // Gradients of shared heads: out[.., g, d] = the sum over the group's heads in order, rounded once.
-__global__ __launch_bounds__(256) void group_kernel(const float* from, uint16_t* to, int64_t rows, int group, int d) {
-  const int64_t n = rows * d;
+struct GroupArgs {
+  const float* from[2];  // of k and v
+  uint16_t* to[2];
+  int d[2];
+  int64_t rows;
+  int group;
+};
+
+__global__ __launch_bounds__(256) void group_kernel(GroupArgs a) {
+  const int d = a.d[blockIdx.y];
+  const int64_t n = a.rows * d;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
     const int64_t r = i / d;
-    const float* p = from + r * group * d + (i - r * d);
+    const float* p = a.from[blockIdx.y] + r * a.group * d + (i - r * d);
     float s = 0.0f;
-    for (int j = 0; j < group; ++j) s += p[int64_t(j) * d];
-    to[i] = f32_to_bf16(s);
+    for (int j = 0; j < a.group; ++j) s += p[int64_t(j) * d];
+    a.to[blockIdx.y][i] = f32_to_bf16(s);
   }
 }
 
@@ -721,23 +730,48 @@ const char* heads_fault(const xdna_heads_bf16* h) {
 
 Heads heads_of(const xdna_heads_bf16* h, int64_t share) { return {h->data, h->batch, h->token, h->head, int(share)}; }
 
-// Segments of a sequence: where the sequences and heads alone leave CUs without a workgroup.
+constexpr int kScanFrom = 5;  // segments from which on their states are summed up by a launch
+
+// Segments of a sequence, by what a call takes in us.  Fitted to 11 shapes (1 to 6 sequences of 200 to 32768 tokens, 4 to
+// 16 heads of 64 or 128, both directions, 1 to 64 segments; 10 % off in the mean): a chunk takes 1.55 with few
+// workgroups, 2.2 with one on each CU and 3.3 with two; of the segments' own states 1.05 a workgroup on a CU; heads up to 64
+// three quarters of that.  1 x 8192 tokens, 16 heads of 128, forward: 201 us whole, 62 in 8 segments, 59 in 16, 104 in 64;
+// 6 x 1024 tokens 33 whole, 43 in 2; backward of 1 x 8192 203 whole, 117 in 5, 137 in 16.
 struct Plan {
   int segments, chunks;
 };
 
-Plan plan_segments(int64_t workgroups, int64_t T) {
+float walk_cost(int64_t workgroups, int64_t chunks) {
+  const auto round = [](float n) { return n <= 256.0f ? 1.55f + 0.65f * n / 256.0f : 2.2f + 1.1f * (n - 256.0f) / 256.0f; };
+  const int64_t rest = workgroups % 512;
+  return 5.0f + float(chunks) * (3.3f * float(workgroups / 512) + (rest ? round(float(rest)) : 0.0f));
+}
+
+// `walks`, `states`: workgroups of a segment's walks and of its states; `state_mb`: bytes of all heads' states
+Plan plan_segments(int64_t walks, int64_t states, float state_mb, int64_t T, bool big) {
   const int64_t chunks = ceil_div(T, int64_t(kC));
-  if (workgroups >= 256 || chunks < 2) return {1, int(std::max<int64_t>(chunks, 1))};
-  const int64_t per = std::max<int64_t>(1, chunks / std::max<int64_t>(1, 512 / workgroups));
-  return {int(ceil_div(chunks, per)), int(per)};
+  const float size = big ? 1.0f : 0.75f;
+  Plan best = {1, int(std::max<int64_t>(chunks, 1))};
+  float least = walk_cost(walks, chunks) * size;
+  for (int64_t n = 2; n <= std::min<int64_t>(chunks, 256); n += n < 64 ? 1 : 32) {
+    const int64_t per = ceil_div(chunks, n), segments = ceil_div(chunks, per);
+    const float own = 6.0f + float(per) * std::max(1.0f, 1.05f * float(states * (segments - 1)) / 256.0f);
+    const float join = segments >= kScanFrom ? 4.0f + 0.34f * state_mb * float(segments - 1) : float(segments - 1);
+    const float cost = (walk_cost(walks * segments, per) + 3.0f + own) * size + join;
+    if (cost < least) least = cost, best = {int(segments), int(per)};
+  }
+  return best;
 }
 
 int blocks64(int64_t d) { return int(ceil_div(d, int64_t(kVB))); }
 
-Plan fwd_plan(int64_t B, int64_t T, int64_t H, int64_t dv) { return plan_segments(B * H * blocks64(dv), T); }
+Plan fwd_plan(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv) {
+  const int64_t n = B * H * blocks64(dv);
+  return plan_segments(n, n, float(B * H * dk * dv) * 4e-6f, T, dk > 64);
+}
 Plan bwd_plan(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv) {
-  return plan_segments(B * H * (2 * blocks64(dk) + blocks64(dv)), T);
+  return plan_segments(B * H * (2 * blocks64(dk) + blocks64(dv)), 2 * B * H * blocks64(dv), float(B * H * dk * dv) * 8e-6f, T,
+                       dk > 64 || dv > 64);
 }
 
 size_t local_floats(const Plan& p, int64_t B, int64_t H, int64_t dk, int64_t dv) {
@@ -768,20 +802,18 @@ bool launch_walks(DecayArgs& a, hipStream_t st) {
   return true;
 }
 
-// The walks of one launch each where their keys' sizes are on the same side of 64.
+// All walks in one launch, on tiles for the largest of their keys' heads (walks of sizes on both sides of 64 in a launch
+// each took 26 us where one takes 16: 3 x 777 tokens, 6 heads of 48 and 80).
 template <bool STATE>
-bool launch(const DecayArgs& a, const Walk* walks, int n, hipStream_t st) {
-  for (const bool big : {true, false}) {
-    DecayArgs b = a;
-    b.n = 0;
-    for (int i = 0; i < n; ++i)
-      if ((walks[i].dk > 64) == big) b.walk[b.n++] = walks[i];
-    if (b.n && !(big ? launch_walks<128, STATE>(b, st) : launch_walks<64, STATE>(b, st))) return false;
+bool launch(DecayArgs a, const Walk* walks, int n, hipStream_t st) {
+  bool big = false;
+  a.n = n;
+  for (int i = 0; i < n; ++i) {
+    a.walk[i] = walks[i];
+    big |= walks[i].dk > 64;
   }
-  return true;
+  return big ? launch_walks<128, STATE>(a, st) : launch_walks<64, STATE>(a, st);
 }
-
-constexpr int kScanFrom = 5;  // segments
 
 // the segments' own states, and where they are many the states before them
 template <int N>
@@ -819,7 +851,7 @@ extern "C" {
 
 size_t xdna_decay_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv) {
   if (sizes_fault(B, T, H, H, dk, dv) || B == 0 || T == 0) return 0;
-  return local_floats(fwd_plan(B, T, H, dv), B, H, dk, dv) * sizeof(float);
+  return local_floats(fwd_plan(B, T, H, dk, dv), B, H, dk, dv) * sizeof(float);
 }
 
 int xdna_decay_attention(const xdna_heads_bf16* q, const xdna_heads_bf16* k, const xdna_heads_bf16* v, int64_t B, int64_t T,
@@ -843,7 +875,7 @@ int xdna_decay_attention(const xdna_heads_bf16* q, const xdna_heads_bf16* k, con
   a.log_decay = log_decay;
   a.lengths = lengths;
   a.index_bytes = index_bytes;
-  const Plan p = fwd_plan(B, T, H, dv);
+  const Plan p = fwd_plan(B, T, H, dk, dv);
   a.segments = p.segments, a.chunks = p.chunks;
   Walk w = {};
   w.q = heads_of(q, 1), w.k = heads_of(k, H / G), w.v = heads_of(v, H / G);
@@ -937,12 +969,9 @@ int xdna_decay_attention_bwd(const xdna_heads_bf16* dout, const float* d_state_o
   s[0].dk = int(dk), s[0].dv = int(dv);
   if (!launch_segments<2>(a, s, {state, d_state_out}, st) || !launch<false>(a, w, 3, st)) return refuse(what, "the kernel's LDS size cannot be had");
   if (group > 1) {
-    const auto sum = [&](const float* from, uint16_t* to, int64_t d) {
-      const unsigned grid = unsigned(std::min<int64_t>(ceil_div(B * T * G * d, int64_t(256)), 16384));
-      group_kernel<<<grid, 256, 0, st>>>(from, to, B * T * G, int(group), int(d));
-    };
-    sum(wide_k, d_k, dk);
-    sum(wide_v, d_v, dv);
+    const GroupArgs g = {{wide_k, wide_v}, {d_k, d_v}, {int(dk), int(dv)}, B * T * G, int(group)};
+    const unsigned grid = unsigned(std::min<int64_t>(ceil_div(B * T * G * std::max(dk, dv), int64_t(256)), 16384));
+    group_kernel<<<dim3(grid, 2), 256, 0, st>>>(g);
   }
   return check_launch(what);
 }

@@ -510,12 +510,30 @@ def test_decay_attention_of_ragged_batches(T, size, kind):
             assert not got[name][b, max(0, min(Tn, int(lengths[b]))):].cpu().any(), (name, b)
 
 
-@pytest.mark.parametrize("size", [(1, 1500, 1, 1, 64, 64), (1, 1025, 64, 32, 8, 16), (2, 1400, 33, 33, 16, 8)])
-def test_decay_attention_of_long_sequences_in_segments(T, size):
-    """Sequences cut into segments of one chunk and of several, ragged among them."""
-    print("decay segments", size, flush=True)
+def segments(hip, size, backward):
+    """Segments of a sequence, from the workspace that holds all but one of their states."""
+    Bn, Tn, H, G, dk, dv = size
+    state = 4 * Bn * H * dk * dv
+    if not backward:
+        return 1 + hip.xdna_decay_workspace_bytes(Bn, Tn, H, dk, dv) // state
+    shared = 4 * Bn * Tn * H * (dk + dv) if G < H else 0
+    return 1 + (hip.xdna_decay_bwd_workspace_bytes(Bn, Tn, H, G, dk, dv) - shared) // (2 * state)
+
+
+SEGMENTED = [  # size, segments of the forward's and the backward's sequences: whole, few (read one by one) or many (summed first)
+    ((1, 1500, 1, 1, 64, 64), "many", "many"), ((2, 1100, 20, 20, 128, 128), "few", "whole"), ((1, 2000, 14, 14, 72, 72), "many", "few"),
+    ((1, 2500, 30, 15, 16, 128), "many", "few"), ((2, 2000, 9, 3, 128, 24), "many", "many"), ((3, 777, 6, 2, 48, 80), "many", "whole"),
+]
+
+
+@pytest.mark.parametrize("ragged", [False, True], ids=["whole", "ragged"])
+@pytest.mark.parametrize("size,forward,backward", SEGMENTED)
+def test_decay_attention_in_segments(T, hip, size, forward, backward, ragged):
+    n = [segments(hip, size, b) for b in (False, True)]
+    print("decay segments", size, ragged, n, flush=True)
+    assert [("whole" if x == 1 else "few" if x < 5 else "many") for x in n] == [forward, backward], n
     v = decay_values(*size, seed=7)
-    lengths = None if size[0] == 1 else torch.tensor([size[1], 300])
+    lengths = torch.tensor([300, size[1] - 1, 65][: size[0]]) if ragged else None
     got = run_decay(T, v, lengths)
     check_decay(got, decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], lengths, size[4] ** -0.5, v["dout"], v["dstate"]))
 

@@ -79,12 +79,12 @@ def test_decay_attention_refuses_bad_arguments():
     def ref(h):
         return ctypes.byref(h) if h is not None else None
 
-    # one sequence of several chunks: segments
-    need = lib.xdna_decay_workspace_bytes(1, 256, 2, 8, 8)
-    assert need > 0 and lib.xdna_decay_workspace_bytes(1, 64, 2, 8, 8) == 0 and lib.xdna_decay_workspace_bytes(0, 256, 2, 8, 8) == 0
-    assert lib.xdna_decay_workspace_bytes(512, 256, 2, 8, 8) == 0
+    # few long sequences: segments
+    need = lib.xdna_decay_workspace_bytes(1, 8192, 2, 8, 8)
+    assert need > 0 and lib.xdna_decay_workspace_bytes(1, 64, 2, 8, 8) == 0 and lib.xdna_decay_workspace_bytes(0, 8192, 2, 8, 8) == 0
+    assert lib.xdna_decay_workspace_bytes(512, 8192, 2, 8, 8) == 0
 
-    def fwd(q=ok, k=ok, v=ok, Bn=1, T=256, H=2, G=1, dk=8, dv=8, g=A, n=A, ib=8, scale=1.0, s=A, o=A, so=A, ws=A, have=need):
+    def fwd(q=ok, k=ok, v=ok, Bn=1, T=8192, H=2, G=1, dk=8, dv=8, g=A, n=A, ib=8, scale=1.0, s=A, o=A, so=A, ws=A, have=need):
         return lib.xdna_decay_attention(ref(q), ref(k), ref(v), Bn, T, H, G, dk, dv, g, n, ib, scale, s, o, so, ws, have, None)
 
     bad = [({"q": None}, "null"), ({"k": hip_abi.Heads(None, 1, 1, 1)}, "null"), ({"v": hip_abi.Heads(A + 1, 1, 1, 1)}, "misaligned"),
@@ -96,10 +96,10 @@ def test_decay_attention_refuses_bad_arguments():
                           ({"ws": None}, "workspace"), ({"ws": A + 8}, "workspace"), ({"have": need - 1}, "workspace")]:
         assert refused(fwd(**kw), why), (kw, hip_abi.last_error())
     assert fwd(Bn=0, q=None) == 0
-    need_b = lib.xdna_decay_bwd_workspace_bytes(1, 256, 2, 1, 8, 8)
-    assert need_b > lib.xdna_decay_bwd_workspace_bytes(1, 256, 2, 2, 8, 8) > 0
+    need_b = lib.xdna_decay_bwd_workspace_bytes(1, 8192, 2, 1, 8, 8)
+    assert need_b > lib.xdna_decay_bwd_workspace_bytes(1, 8192, 2, 2, 8, 8) > 0
 
-    def bwd(do=ok, ds=A, q=ok, k=ok, v=ok, Bn=1, T=256, H=2, G=1, dk=8, dv=8, g=A, n=A, ib=8, scale=1.0, s=A, dq=A, dkk=A, dvv=A, d0=A, ws=A, have=need_b):
+    def bwd(do=ok, ds=A, q=ok, k=ok, v=ok, Bn=1, T=8192, H=2, G=1, dk=8, dv=8, g=A, n=A, ib=8, scale=1.0, s=A, dq=A, dkk=A, dvv=A, d0=A, ws=A, have=need_b):
         return lib.xdna_decay_attention_bwd(ref(do), ds, ref(q), ref(k), ref(v), Bn, T, H, G, dk, dv, g, n, ib, scale, s, dq, dkk, dvv, d0, ws, have, None)
 
     for kw, why in bad + [({"do": None}, "null"), ({"dq": None}, "null"), ({"dkk": None}, "null"), ({"dvv": None}, "null"), ({"dq": A + 1}, "misaligned"),
