@@ -15,7 +15,8 @@
 // The linear layer y = act(x W^T + b) + r runs on the same tiles with an epilogue of its own.  For
 // training it keeps the slope act'(v) as an fp16 times 2^15 (2 bytes a unit, 11 bits of mantissa
 // down to 1.9e-9): what the backward multiplies dy by, without the activation again and within 2^-12,
-// where a slope in bf16 would be a second rounding as large as that of dy act'(v) itself.
+// where a slope in bf16 would be a second rounding as large as that of dy act'(v) itself.  ReLU's slopes are bits, four
+// units a byte: the layer's traffic beside its products is a fifth less.
 #include "common.h"
 #include "gemm_dma.h"
 #include "mfma.h"
@@ -120,7 +121,7 @@ struct TileArgs {
   const uint16_t* bias;  // [p] or null
   const uint16_t* res;   // [q][p], row stride ldr, or null
   int64_t ldr;
-  uint16_t* slope;       // [q][p], written where not null
+  void* kept;            // the slopes, written where not null (xdna_linear_kept_bytes)
 };
 
 // A workgroup's tile.  Workgroups go to the XCDs (each with its own L2) in turn: XCD c takes the
@@ -361,32 +362,40 @@ __device__ inline void store_kept(const TileArgs& a, int q, int at, int n, const
 
 constexpr float kSlopeScale = 32768.0f;  // slopes are up to 1.13 in size: 37000 of fp16's 65504
 
-// act(v) and act'(v) where the activation is a value of the launch: an epilogue's few instructions
-// are cheaper than four copies of every tile kernel
-__device__ inline float2 act_pair(int act, float v) {
-  if (act == kNone) return make_float2(v, 1.0f);
-  if (act == kSilu) return act_pair<kSilu>(v);
-  if (act == kGelu) return act_pair<kGelu>(v);
-  return act_pair<kRelu>(v);
-}
+// (The linear layer's activation is a value of the launch: an epilogue's few instructions are cheaper than four copies
+// of every tile kernel.)
 
-// N outputs of row q from column `at` on (n of them in range): the product's sums d to the layer's
-// outputs, and their slopes
+// N values v (the product's sums and the bias) to the layer's outputs, residual r added, and what is kept of their
+// slopes: relu's as bits, the others' as fp16
 template <int N>
-__device__ inline void linear_values(const TileArgs& a, int q, int at, int n, float (&d)[N], uint16_t (&slope)[N]) {
-  if (a.bias) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) d[e] += e < n ? bf16_to_f32(a.bias[at + e]) : 0.0f;
-  }
-  if (a.act != kNone) {
+struct LinearOut {
+  float y[N];
+  uint16_t slope[N];
+  uint32_t bits;
+};
+
+template <int N>
+__device__ inline LinearOut<N> linear_out(int act, const float (&v)[N], const float (&r)[N]) {
+  LinearOut<N> o;
+  o.bits = 0;
+  if (act == kNone || act == kRelu) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float2 t = act_pair(a.act, d[e]);
-      d[e] = t.x;
-      slope[e] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(t.y * kSlopeScale));
+      o.bits |= v[e] > 0.0f ? 1u << e : 0u;
+      o.y[e] = (act == kRelu ? act_of<kRelu>(v[e]) : v[e]) + r[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float2 t = act == kSilu ? act_pair<kSilu>(v[e]) : act_pair<kGelu>(v[e]);
+      o.y[e] = t.x + r[e];
+      o.slope[e] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(t.y * kSlopeScale));
     }
   }
+  return o;
 }
+
+__host__ __device__ inline int64_t bit_bytes(int64_t units) { return (units + 3) / 4; }  // a row of relu's slopes
 
 // 4 consecutive outputs: d0 (and for the gated forward the up projection d1) of row q, from
 // column `at` on
@@ -396,18 +405,20 @@ __device__ inline void put_quad(const TileArgs& a, int q, int at, const float (&
     put4(a.out + int64_t(q) * a.ldc + at, d0, a.p.rows - at, a.vec);
   } else if constexpr (EPI == kLinear) {
     const int n = min(a.p.rows - at, 4);
-    float y[4] = {d0[0], d0[1], d0[2], d0[3]};
-    uint16_t slope[4] = {};
-    linear_values(a, q, at, n, y, slope);
-    if (a.res) {
+    float v[4], r[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += e < n ? bf16_to_f32(a.res[int64_t(q) * a.ldr + at + e]) : 0.0f;
+    for (int e = 0; e < 4; ++e) {
+      v[e] = d0[e] + (a.bias && e < n ? bf16_to_f32(a.bias[at + e]) : 0.0f);
+      r[e] = a.res && e < n ? bf16_to_f32(a.res[int64_t(q) * a.ldr + at + e]) : 0.0f;
     }
-    put4(a.out + int64_t(q) * a.ldc + at, y, n, a.vec);
-    if (a.slope) {
+    const LinearOut<4> o = linear_out(a.act, v, r);
+    put4(a.out + int64_t(q) * a.ldc + at, o.y, n, a.vec);
+    if (a.kept && a.act == kRelu) {
+      static_cast<uint8_t*>(a.kept)[q * bit_bytes(a.p.rows) + at / 4] = uint8_t(o.bits);
+    } else if (a.kept) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (e < n) a.slope[int64_t(q) * a.p.rows + at + e] = slope[e];
+        if (e < n) static_cast<uint16_t*>(a.kept)[int64_t(q) * a.p.rows + at + e] = o.slope[e];
     }
   } else if constexpr (EPI == kGatedGrad) {
     const int n = a.F - at;
@@ -501,25 +512,39 @@ __device__ inline void grad8(const float (&d)[8], const Pix8& g, const Pix8& u, 
   }
 }
 
+__device__ inline void unpack8(const Pix8& p, float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(e & 1 ? p.v[e >> 1] & 0xFFFF0000u : p.v[e >> 1] << 16);
+}
+
+// the linear layer's bias at 8 columns (n in range), and a row's residual there
+__device__ inline void load_bias8(const TileArgs& a, int at, int n, float (&bias)[8]) {
+  const Pix8 none = {{0u, 0u, 0u, 0u}};
+  unpack8(a.bias && n > 0 ? row_vec(a.bias + at, n) : none, bias);
+}
+__device__ inline Pix8 load_res8(const TileArgs& a, int q, int at, int n) {
+  const Pix8 none = {{0u, 0u, 0u, 0u}};
+  return a.res && n > 0 ? row_vec(a.res + int64_t(q) * a.ldr + at, n) : none;
+}
+
 // 8 outputs of the linear layer
-__device__ inline void put_linear8(const TileArgs& a, int q, int at, int n, const float (&d)[8]) {
-  Pix8 r = {{0u, 0u, 0u, 0u}};
-  if (a.res) r = row_vec(a.res + int64_t(q) * a.ldr + at, n);  // (in flight beside the activation)
-  float y[8];
+__device__ inline void put_linear8(const TileArgs& a, int q, int at, int n, const float (&d)[8], const float (&bias)[8],
+                                   const Pix8& res) {
+  float v[8], r[8];
+  unpack8(res, r);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = d[e];
-  uint16_t slope[8] = {};
-  linear_values(a, q, at, n, y, slope);
-  if (a.res) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] += __uint_as_float(e & 1 ? r.v[e >> 1] & 0xFFFF0000u : r.v[e >> 1] << 16);
-  }
-  put_vec(a.out + int64_t(q) * a.ldc + at, pack_vec(y), n);
-  if (a.slope) {
+  for (int e = 0; e < 8; ++e) v[e] = d[e] + bias[e];
+  const LinearOut<8> o = linear_out(a.act, v, r);
+  put_vec(a.out + int64_t(q) * a.ldc + at, pack_vec(o.y), n);
+  if (a.kept && a.act == kRelu) {
+    uint8_t* to = static_cast<uint8_t*>(a.kept) + q * bit_bytes(a.p.rows) + at / 4;
+    to[0] = uint8_t(o.bits & 15u);
+    if (n > 4) to[1] = uint8_t(o.bits >> 4);
+  } else if (a.kept) {
     Pix8 s;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s.v[e] = uint32_t(slope[2 * e]) | uint32_t(slope[2 * e + 1]) << 16;
-    put_vec(a.slope + int64_t(q) * a.p.rows + at, s, n);
+    for (int e = 0; e < 4; ++e) s.v[e] = uint32_t(o.slope[2 * e]) | uint32_t(o.slope[2 * e + 1]) << 16;
+    put_vec(static_cast<uint16_t*>(a.kept) + int64_t(q) * a.p.rows + at, s, n);
   }
 }
 
@@ -540,8 +565,7 @@ __device__ inline void put_row8(const TileArgs& a, int q, int at, int n, const f
         if (e < n) to[e] = d0[e];
       return;
     }
-    if constexpr (EPI == kLinear) put_linear8(a, q, at, n, d0);
-    else put_vec(a.out + int64_t(q) * a.ldc + at, pack_vec(d0), n);
+    put_vec(a.out + int64_t(q) * a.ldc + at, pack_vec(d0), n);
   } else if constexpr (EPI == kGatedGrad) {
     Pix8 g, u;
     Bytes8 low;
@@ -557,6 +581,30 @@ __device__ inline void put_row8(const TileArgs& a, int q, int at, int n, const f
     for (int e = 0; e < 8; ++e) h[e] = act_of<ACT>(d0[e]) * d1[e];
     put_vec(a.out + int64_t(q) * a.F + at, pack_vec(h), n);
     if constexpr (EPI == kGatedKeep) store_kept8(a, q, at, n, d0, d1);
+  }
+}
+
+// The linear layer's outputs of 8 columns from `at` on (n of them in range), rows r0, r0 + STEP, .. of ROWS: row(r) is
+// row r's place in the output, sum(r, e) its product.  The bias is loaded once, the residual of four rows at a time from
+// clamped places (row by row, each waited for its own: the epilogue of 8192 x 1024 -> 4096 took twice the k-loop).
+template <int ROWS, int STEP, class Row, class Sum>
+__device__ inline void put_linear_rows(const TileArgs& a, int r0, const Row& row, int at, int n, const Sum& sum) {
+  constexpr int B = ROWS / STEP < 4 ? ROWS / STEP : 4;
+  float bias[8];
+  load_bias8(a, at, n, bias);
+#pragma unroll 1
+  for (int r = r0; r < ROWS; r += B * STEP) {
+    Pix8 res[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) res[u] = load_res8(a, min(row(r + u * STEP), a.q.rows - 1), at, n);
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const int q = row(r + u * STEP);
+      float d[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = sum(r + u * STEP, e);
+      if (q < a.q.rows) put_linear8(a, q, at, n, d, bias, res[u]);
+    }
   }
 }
 
@@ -699,6 +747,13 @@ __device__ inline void tile_block(const TileArgs& a, const TileAt tile) {
   const int at = (GATED ? p0 / 2 : p0) + 8 * o, n = (own_rows(EPI) ? a.p.rows : a.F) - at;
   const float* from = block + (GATED ? (o >> 2) * 64 + (o & 3) * 8 : 8 * o);
   if (n <= 0) return;
+  if constexpr (EPI == kLinear) {
+    if (!a.part) {
+      put_linear_rows<C::T, C::NT / kAcross>(a, tid / kAcross, [&](int r) { return q0 + r; }, at, n,
+                                             [&](int r, int e) { return from[r * EP + e]; });
+      return;
+    }
+  }
 #pragma unroll 2
   for (int r = tid / kAcross; r < C::T; r += C::NT / kAcross) {
     if (q0 + r >= a.q.rows) break;
@@ -799,7 +854,9 @@ __global__ __launch_bounds__(256) void linear_join_kernel(TileArgs a, int splits
           for (int e = 0; e < 8; ++e) d[e] += v[u][e >> 2].v[e & 3];
         }
     }
-    put_linear8(a, q, at, n, d);
+    float bias[8];
+    load_bias8(a, at, n, bias);
+    put_linear8(a, q, at, n, d, bias, load_res8(a, q, at, n));
   }
 }
 
@@ -809,7 +866,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(TileArgs a, int splits
 struct LinearBwdArgs {
   const uint16_t* dy;     // [M][N], row stride ld
   int64_t ld;
-  const uint16_t* slope;  // dense
+  const void* kept;       // as the forward wrote them
+  int bits;               // relu's
   uint16_t* dp;           // dense, or null
   float* part;            // or null
   int M, N;
@@ -819,28 +877,40 @@ __global__ __launch_bounds__(256) void linear_bwd_kernel(LinearBwdArgs a) {
   __shared__ float red[8][256];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
   const int at = blockIdx.x * 256 + lane * 8, n = min(a.N - at, 8);
+  const int64_t bit_ld = bit_bytes(a.N);
   float sum[8] = {};
   if (n > 0) {
     const int step = gridDim.y * 8;
     for (int64_t q0 = int64_t(blockIdx.y) * 8 + row; q0 < a.M; q0 += 4 * int64_t(step)) {
       Pix8 d[4], k[4];
+      uint32_t bits[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {  // (rows past the end: the last one again, unused)
         const int64_t q = min(q0 + int64_t(u) * step, int64_t(a.M - 1));
         d[u] = row_vec(a.dy + q * a.ld + at, n);
-        if (a.slope) k[u] = row_vec(a.slope + q * a.N + at, n);
+        if (a.bits) {
+          const uint8_t* p = static_cast<const uint8_t*>(a.kept) + q * bit_ld + at / 4;
+          bits[u] = p[0] | uint32_t(p[n > 4 ? 1 : 0]) << 4;
+        } else if (a.kept) {
+          k[u] = row_vec(static_cast<const uint16_t*>(a.kept) + q * a.N + at, n);
+        }
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int64_t q = q0 + int64_t(u) * step;
         if (q >= a.M) break;
         float g[8];
+        unpack8(d[u], g);
+        if (a.bits) {  // (a product with the slope 0, as the others': NaN and infinities stay)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          g[e] = __uint_as_float(e & 1 ? d[u].v[e >> 1] & 0xFFFF0000u : d[u].v[e >> 1] << 16);
-          if (a.slope) g[e] *= float(__builtin_bit_cast(_Float16, uint16_t(k[u].v[e >> 1] >> (16 * (e & 1))))) * (1.0f / kSlopeScale);
-          sum[e] += g[e];
+          for (int e = 0; e < 8; ++e) g[e] *= (bits[u] >> e) & 1u ? 1.0f : 0.0f;
+        } else if (a.kept) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            g[e] *= float(__builtin_bit_cast(_Float16, uint16_t(k[u].v[e >> 1] >> (16 * (e & 1))))) * (1.0f / kSlopeScale);
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += g[e];
         if (a.dp) put_vec(a.dp + q * a.N + at, pack_vec(g), n);
       }
     }
@@ -1060,13 +1130,9 @@ void gated_large_kernel(TileArgs a) {
         if (row(r) < a.q.rows && f < a.F) put_row8<EPI, ACT>(a, row(r), f, 8, g, u, 0);
       }
     } else if constexpr (EPI == kLinear) {
-#pragma unroll 2
-      for (int r = rr; r < kEpiRows; r += kRound) {
-        float d[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = epi[r * kEpiPitch + 8 * o + e];
-        if (row(r) < a.q.rows && f < units) put_linear8(a, row(r), f, min(units - f, 8), d);
-      }
+      if (f < units)
+        put_linear_rows<kEpiRows, kRound>(a, rr, row, f, min(units - f, 8),
+                                          [&](int r, int e) { return epi[r * kEpiPitch + 8 * o + e]; });
     } else {
       // four rows' [g u] in flight: clamped addresses, no branch around the loads
 #pragma unroll 1
@@ -1476,15 +1542,15 @@ int xdna_gated_grads_bf16(const uint16_t* dgu, const uint16_t* x, int64_t ldx, c
 }
 
 int xdna_linear_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t M, int64_t K, int64_t N, int act,
-                     const uint16_t* bias, const uint16_t* residual, int64_t ldr, uint16_t* y, uint16_t* slope, void* stream) {
+                     const uint16_t* bias, const uint16_t* residual, int64_t ldr, uint16_t* y, void* kept, void* stream) {
   const char* what = "xdna_linear_bf16";
   if (const char* why = linear_fault(M, K, N)) return refuse(what, why);
   if (act < 0 || act > 3) return refuse(what, "activation must be 0 (silu), 1 (gelu), 2 (relu) or 3 (none)");
   if ((M > 1 && (ldx < K || (residual && ldr < N))) || (ldw < K && N > 1)) return refuse(what, "rows overlap");
   if (M == 0) return 0;
   if (!x || !w || !y) return refuse(what, "null operand");
-  if (slope && act == 3) return refuse(what, "no activation has no slopes");
-  if (odd(x) || odd(w) || odd(bias) || odd(residual) || odd(y) || odd(slope)) return refuse(what, "misaligned operand");
+  if (kept && act == kNone) return refuse(what, "no activation has no slopes");
+  if (odd(x) || odd(w) || odd(bias) || odd(residual) || odd(y) || odd(kept)) return refuse(what, "misaligned operand");
   if (!admit_launch(what)) return -1;
   TileArgs a = {};
   a.p = {w, N > 1 ? ldw : K, int(N)};
@@ -1497,27 +1563,33 @@ int xdna_linear_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t 
   a.bias = bias;
   a.res = residual;
   a.ldr = M > 1 ? ldr : N;
-  a.slope = slope;
+  a.kept = kept;
   return launched(what, launch_sized<kLinear, false, kSilu>(a, as_stream(stream)));
+}
+
+size_t xdna_linear_kept_bytes(int64_t M, int64_t N, int act) {
+  if (linear_fault(M, 1, N) || M == 0) return 0;
+  return act == kSilu || act == kGelu ? size_t(M) * size_t(N) * 2 : act == kRelu ? size_t(M) * size_t(bit_bytes(N)) : 0;
 }
 
 size_t xdna_linear_bwd_workspace_bytes(int64_t M, int64_t N) {
   return linear_fault(M, 1, N) ? 0 : size_t(linear_parts(M, N)) * size_t(N) * sizeof(float);
 }
 
-int xdna_linear_bwd_bf16(const uint16_t* dy, int64_t ld, const uint16_t* slope, int64_t M, int64_t N, uint16_t* dp,
+int xdna_linear_bwd_bf16(const uint16_t* dy, int64_t ld, const void* kept, int act, int64_t M, int64_t N, uint16_t* dp,
                          uint16_t* d_bias, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "xdna_linear_bwd_bf16";
   if (const char* why = linear_fault(M, 1, N)) return refuse(what, why);
   if (ld < N && M > 1) return refuse(what, "rows overlap");
-  if (M > 0 && !dy) return refuse(what, "null operand");
-  if (odd(dy) || odd(slope) || odd(dp) || odd(d_bias)) return refuse(what, "misaligned operand");
+  if (act < 0 || act > 3) return refuse(what, "activation must be 0 (silu), 1 (gelu), 2 (relu) or 3 (none)");
+  if (M > 0 && (!dy || (act != kNone && !kept))) return refuse(what, "null operand");
+  if (odd(dy) || odd(kept) || odd(dp) || odd(d_bias)) return refuse(what, "misaligned operand");
   if (d_bias && M > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < xdna_linear_bwd_workspace_bytes(M, N)))
     return refuse(what, "workspace missing, misaligned or too small");
   if ((M == 0 || !dp) && !d_bias) return 0;
   if (!admit_launch(what)) return -1;
   hipStream_t st = as_stream(stream);
-  LinearBwdArgs a = {dy, M > 1 ? ld : N, slope, dp, d_bias ? static_cast<float*>(workspace) : nullptr, int(M), int(N)};
+  LinearBwdArgs a = {dy, M > 1 ? ld : N, act == kNone ? nullptr : kept, act == kRelu, dp, d_bias ? static_cast<float*>(workspace) : nullptr, int(M), int(N)};
   const int64_t parts = linear_parts(M, N);
   if (M > 0) linear_bwd_kernel<<<dim3(unsigned(ceil_div(N, int64_t(256))), unsigned(parts)), 256, 0, st>>>(a);
   if (d_bias) linear_bias_kernel<<<unsigned(ceil_div(N, int64_t(64))), 1024, 0, st>>>(a.part, int(parts), int(N), d_bias);

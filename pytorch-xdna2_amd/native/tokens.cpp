@@ -545,7 +545,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
 constexpr int64_t kNoActivation = 3;
 
 struct LinearForward {
-  at::Tensor y, slope;  // slope: undefined where not kept
+  at::Tensor y, kept;  // kept: undefined where no slopes are
 };
 
 LinearForward linear_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, const at::Tensor& residual,
@@ -556,11 +556,11 @@ LinearForward linear_forward(const at::Tensor& x, const at::Tensor& weight, cons
   const at::Tensor rr = residual.defined() ? as_rows(residual) : residual;
   const int64_t M = xr.size(0), K = xr.size(1), N = w.size(0);
   r.y = empty_xdna(with_last(x, N), at::kBFloat16);
-  if (keep && act != kNoActivation) r.slope = empty_xdna({M, N}, at::kShort);
+  if (keep && act != kNoActivation) r.kept = workspace(xdna_linear_kept_bytes(M, N, int(act)));
   check_abi(xdna_linear_bf16(p16(xr), row_stride(xr), p16(w), row_stride(w), M, K, N, int(act),
                              static_cast<const uint16_t*>(cptr(b)), static_cast<const uint16_t*>(cptr(rr)),
                              rr.defined() ? row_stride(rr) : 0, static_cast<uint16_t*>(ptr_or_null(r.y)),
-                             static_cast<uint16_t*>(ptr_or_null(r.slope)), current_stream()),
+                             ptr_or_null(r.kept), current_stream()),
             "linear");
   return r;
 }
@@ -572,7 +572,8 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     // only the gradient of what comes before the activation takes its slopes
     const auto wants = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
     const LinearForward f = linear_forward(x, weight, bias, residual, act, wants(x) || wants(weight) || wants(bias));
-    ctx->save_for_backward({x, weight, f.slope});
+    ctx->save_for_backward({x, weight, f.kept});
+    ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = bias.defined();
     ctx->saved_data["residual"] = residual.defined();
     return f.y;
@@ -588,16 +589,17 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     if (!want_x && !want_w && !want_b) return out;
     ScopedCount sc("hip_tokens.linear.bwd.run");
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor x = as_rows(saved[0]), w = as_rows(saved[1]), dy = as_rows(grads[0]), &slope = saved[2];
+    const at::Tensor x = as_rows(saved[0]), w = as_rows(saved[1]), dy = as_rows(grads[0]), &kept = saved[2];
     const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
     at::Tensor dp = dy, db, ws;
-    if (slope.defined() && (want_x || want_w)) dp = empty_xdna({M, N}, at::kBFloat16);
+    const bool slopes = kept.defined(), own_dp = slopes && (want_x || want_w);
+    if (own_dp) dp = empty_xdna({M, N}, at::kBFloat16);
     if (want_b) db = empty_xdna({N}, at::kBFloat16);
-    if (slope.defined() || want_b) {
+    if (slopes || want_b) {
       const size_t bytes = want_b ? xdna_linear_bwd_workspace_bytes(M, N) : 0;
       if (bytes) ws = workspace(bytes);
-      check_abi(xdna_linear_bwd_bf16(p16(dy), row_stride(dy), static_cast<const uint16_t*>(ptr_or_null(slope)), M, N,
-                                     slope.defined() && (want_x || want_w) ? static_cast<uint16_t*>(ptr_or_null(dp)) : nullptr,
+      check_abi(xdna_linear_bwd_bf16(p16(dy), row_stride(dy), ptr_or_null(kept), int(ctx->saved_data["act"].toInt()), M, N,
+                                     own_dp ? static_cast<uint16_t*>(ptr_or_null(dp)) : nullptr,
                                      static_cast<uint16_t*>(ptr_or_null(db)), ptr_or_null(ws), bytes, current_stream()),
                 "linear backward");
       out[2] = db;

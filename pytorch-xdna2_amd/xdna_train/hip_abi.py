@@ -171,7 +171,8 @@ SIGNATURES = {
     "xdna_layer_norm_bwd": (I, [P, L, P, L, P, L, I, L, L, P, I, P, P, P, P, P, Z, P]),
     "xdna_linear_bf16": (I, [P, L, P, L, L, L, L, I, P, P, L, P, P, P]),
     "xdna_linear_bwd_workspace_bytes": (Z, [L, L]),
-    "xdna_linear_bwd_bf16": (I, [P, L, P, L, L, P, P, P, Z, P]),
+    "xdna_linear_kept_bytes": (Z, [L, L, I]),
+    "xdna_linear_bwd_bf16": (I, [P, L, P, I, L, L, P, P, P, Z, P]),
     "xdna_linear_grads_pick": (I, [L, L, L]),
     "xdna_linear_grads_bf16": (I, [P, L, P, L, P, L, L, L, L, P, P, P]),
     "xdna_decay_workspace_bytes": (Z, [L] * 5),

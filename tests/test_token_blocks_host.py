@@ -55,10 +55,12 @@ def test_linear_refuses_bad_arguments():
     need = lib.xdna_linear_bwd_workspace_bytes(2, 4)
     assert need > 0 and lib.xdna_linear_bwd_workspace_bytes(0, 4) == 0
 
-    def bwd(dy=A, ld=4, s=A, M=2, N=4, dp=A, db=A, ws=A, have=need):
-        return lib.xdna_linear_bwd_bf16(dy, ld, s, M, N, dp, db, ws, have, None)
+    assert [lib.xdna_linear_kept_bytes(3, 10, act) for act in range(4)] == [60, 60, 9, 0] and lib.xdna_linear_kept_bytes(0, 10, 0) == 0
 
-    for kw, why in [({"dy": None}, "null"), ({"ld": 3}, "overlap"), ({"ws": None}, "workspace"), ({"ws": A + 8}, "workspace"),
+    def bwd(dy=A, ld=4, s=A, act=0, M=2, N=4, dp=A, db=A, ws=A, have=need):
+        return lib.xdna_linear_bwd_bf16(dy, ld, s, act, M, N, dp, db, ws, have, None)
+
+    for kw, why in [({"dy": None}, "null"), ({"s": None}, "null"), ({"act": 4}, "activation"), ({"ld": 3}, "overlap"), ({"ws": None}, "workspace"), ({"ws": A + 8}, "workspace"),
                     ({"have": need - 1}, "workspace"), ({"dp": A + 1}, "misaligned"), ({"N": 0}, "sizes")]:
         assert refused(bwd(**kw), why), (kw, hip_abi.last_error())
     assert bwd(dp=None, db=None) == 0 and bwd(M=0, db=None) == 0
