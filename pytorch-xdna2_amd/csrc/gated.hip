@@ -1427,10 +1427,10 @@ const char* linear_fault(int64_t M, int64_t K, int64_t N) {
   return M * N > kMaxOutputs ? "too many outputs" : nullptr;
 }
 
-// Row slices of the column sums: enough workgroups for the chip (four a CU), 32 rows a slice at least.
+// Row slices of the column sums: enough workgroups for the chip (four a CU), a row of each thread at least.
 int64_t linear_parts(int64_t M, int64_t N) {
   if (M <= 0) return 0;
-  return std::max<int64_t>(1, std::min(ceil_div(int64_t(1024), ceil_div(N, int64_t(256))), ceil_div(M, int64_t(32))));
+  return std::max<int64_t>(1, std::min(ceil_div(int64_t(1024), ceil_div(N, int64_t(256))), ceil_div(M, int64_t(8))));
 }
 
 int launched(const char* what, bool ok) {

@@ -131,10 +131,22 @@ __device__ inline bool counts(const Window& w, int e) {
   return EVEN ? w.from == 0 : e >= w.from && e < w.n;
 }
 
+// The sum over the wave, in every lane: quads, halves of 8 and rows of 16 by DPP, rows by gfx950's swaps: no LDS and
+// no waits (six shuffles through LDS took 0.6 us of a row's 2).
+template <int CTRL>
+__device__ inline float dpp(float v) {
+  return __uint_as_float(uint32_t(__builtin_amdgcn_update_dpp(0, int(__float_as_uint(v)), CTRL, 0xF, 0xF, true)));
+}
+
 __device__ inline float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  v += dpp<0xB1>(v);   // quad_perm 1 0 3 2
+  v += dpp<0x4E>(v);   // quad_perm 2 3 0 1
+  v += dpp<0x141>(v);  // row_half_mirror
+  v += dpp<0x140>(v);  // row_mirror
+  auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
 // The sums of N values over the WAVES waves that share a row, the same in every thread; `red` holds
@@ -259,14 +271,25 @@ __global__ __launch_bounds__(64 * WAVES * GROUP) void bwd_kernel(NormArgs a) {
   }
   int phase = 0;
   const float scale = 1.0f / float(a.dim);
-  for (int64_t r = int64_t(blockIdx.x) * GROUP + group; r < a.rows; r += int64_t(gridDim.x) * GROUP) {
-    typename Elem<DT>::Vec qx[V], qd[V];
+  // A row's loads fly beside the row before it where that costs no occupancy (at two waves a SIMD: 65536 x 2048 in bf16
+  // 196 -> 187 us; with two vectors a thread it takes the fourth wave: 8192 x 1024 16.5 -> 20).
+  constexpr bool kAhead = DT == kBf16 && WAVES < 16 && V == 4;
+  typename Elem<DT>::Vec qx[V], qd[V];
+  float2 stat;
+  const auto load = [&](int64_t r) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       qx[j] = load8<DT, EVEN>(static_cast<const T*>(a.x) + r * a.ldx, win[j]);
       qd[j] = load8<DT, EVEN>(static_cast<const T*>(a.dy) + r * a.lddy, win[j]);
     }
-    const float mean = a.stats[2 * r], inv = a.stats[2 * r + 1];
+    stat = make_float2(a.stats[2 * r], a.stats[2 * r + 1]);
+  };
+  const int64_t step = int64_t(gridDim.x) * GROUP;
+  int64_t r = int64_t(blockIdx.x) * GROUP + group;
+  if (kAhead && r < a.rows) load(r);
+  for (; r < a.rows; r += step) {
+    if (!kAhead) load(r);
+    const float mean = stat.x, inv = stat.y;
     float sums[2] = {0.0f, 0.0f};
     float h[V][8], g[V][8];
 #pragma unroll
@@ -286,6 +309,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUP) void bwd_kernel(NormArgs a) {
         sums[1] += in ? g[j][e] * h[j][e] : 0.0f;
       }
     }
+    if (kAhead && r + step < a.rows) load(r + step);
     if (!a.out) continue;
     row_sums<WAVES>(sums, lds, phase);
     const float ma = sums[0] * scale, mh = sums[1] * scale;
@@ -420,22 +444,20 @@ __global__ __launch_bounds__(256) void long_part_kernel(NormArgs a) {
   a.part[(int64_t(blockIdx.y) * 2 + 1) * a.dim + c] = db;
 }
 
-// dw and db from the workgroups' partials: 64 columns a workgroup, its 16 waves every 16th partial,
-// then the waves in order.
+// dw and db from the workgroups' partials: 16 columns a workgroup, its 64 parts of 16 lanes every 64th partial, then the
+// parts in order.
 template <int PT>
 __global__ __launch_bounds__(1024) void finish_kernel(const float* part, int parts, int dim, void* dweight, void* dbias) {
   typedef typename Elem<PT>::T P;
-  __shared__ float red[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t i = int64_t(blockIdx.x) * 64 + lane, n = 2 * int64_t(dim);
-  float s = 0.0f;
-  if (i < n) s = sum_strided8(0.0f, part + i, n, wave, 16, parts);
-  red[wave][lane] = s;
+  __shared__ float red[64][17];
+  const int column = threadIdx.x & 15, slice = threadIdx.x >> 4;
+  const int64_t i = int64_t(blockIdx.x) * 16 + column, n = 2 * int64_t(dim);
+  red[slice][column] = i < n ? sum_strided8(0.0f, part + i, n, slice, 64, parts) : 0.0f;
   __syncthreads();
-  if (wave != 0 || i >= n) return;
-  s = 0.0f;
+  if (slice != 0 || i >= n) return;
+  float s = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) s += red[w][lane];
+  for (int w = 0; w < 64; ++w) s += red[w][column];
   if (i < dim) {
     if (dweight) put(static_cast<P*>(dweight) + i, s);
   } else if (dbias) {
@@ -458,7 +480,10 @@ constexpr int kBwdGroup = 8;                     // waves of a backward workgrou
 // longer rows; few rows, fewer.
 int64_t bwd_groups(int64_t rows, int64_t dim) {
   if (rows <= 0) return 0;
-  if (dim <= kWaveDim) return std::min<int64_t>(ceil_div(rows, int64_t(kBwdGroup)), 512);
+  if (dim <= kWaveDim) {  // (as many rows for every wave)
+    const int64_t each = ceil_div(rows, int64_t(512) * kBwdGroup);
+    return ceil_div(rows, each * kBwdGroup);
+  }
   if (dim <= kRegDim) return std::min<int64_t>(rows, dim <= 8192 ? 512 : 256);
   return std::min<int64_t>(rows, 64);
 }
@@ -604,7 +629,7 @@ int xdna_layer_norm_bwd(const void* dy, int64_t lddy, const void* dsum, int64_t 
     if (!ok) return refuse(what, "the kernel's LDS size cannot be had");
   }
   if (params) {
-    const unsigned grid = unsigned(ceil_div(2 * dim, int64_t(64)));
+    const unsigned grid = unsigned(ceil_div(2 * dim, int64_t(16)));
     const int parts = int(bwd_groups(rows, dim));
     if (param_dtype == kF32) finish_kernel<kF32><<<grid, 1024, 0, st>>>(a.part, parts, a.dim, dweight, dbias);
     else finish_kernel<kBf16><<<grid, 1024, 0, st>>>(a.part, parts, a.dim, dweight, dbias);
