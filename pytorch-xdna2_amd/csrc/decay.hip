@@ -708,13 +708,15 @@ int refuse(const char* what, const char* why) {
   return -1;
 }
 
-constexpr int64_t kMaxTokens = int64_t(1) << 30, kMaxGrid = (int64_t(1) << 31) - 1;
+constexpr int64_t kMaxTokens = int64_t(1) << 30;
+constexpr int64_t kMaxWalks = (int64_t(1) << 23) - 1;  // workgroups of a launch (512 threads: under 2^32 of them)
+constexpr int64_t kSplitWalks = 4096;                  // most workgroups whose sequences are cut into segments
 
 const char* sizes_fault(int64_t B, int64_t T, int64_t H, int64_t G, int64_t dk, int64_t dv) {
   if (B < 0 || B > (1 << 20) || T < 0 || T > kMaxTokens || H < 1 || H > (1 << 16)) return "batch, tokens or heads out of range";
   if (G < 1 || G > H || H % G) return "the heads of k and v must divide those of q";
   if (dk < 1 || dk > kMaxHead || dv < 1 || dv > kMaxHead) return "head sizes outside 1 .. 128";
-  if (B * H * ceil_div(T, int64_t(kC)) * 6 > kMaxGrid) return "too many chunks";
+  if (B * H * 6 > kMaxWalks) return "too many sequences and heads";  // (three walks of two blocks of columns)
   return nullptr;
 }
 
@@ -752,6 +754,7 @@ Plan plan_segments(int64_t walks, int64_t states, float state_mb, int64_t T, boo
   const int64_t chunks = ceil_div(T, int64_t(kC));
   const float size = big ? 1.0f : 0.75f;
   Plan best = {1, int(std::max<int64_t>(chunks, 1))};
+  if (walks > kSplitWalks) return best;  // (the last round's gap is an eighth of the time at most, the states' pass a quarter)
   float least = walk_cost(walks, chunks) * size;
   for (int64_t n = 2; n <= std::min<int64_t>(chunks, 256); n += n < 64 ? 1 : 32) {
     const int64_t per = ceil_div(chunks, n), segments = ceil_div(chunks, per);

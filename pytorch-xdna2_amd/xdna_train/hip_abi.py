@@ -22,7 +22,6 @@ PP = ctypes.POINTER(ctypes.c_void_p)
 PL = ctypes.POINTER(ctypes.c_int64)
 
 
-
 class Heads(ctypes.Structure):
     """``xdna_heads_bf16``: device pointer and element strides of a [B, T, H, D] operand."""
 

@@ -93,7 +93,7 @@ def test_decay_attention_refuses_bad_arguments():
            ({"q": hip_abi.Heads(A, -1, 1, 1)}, "negative"), ({"Bn": -1}, "range"), ({"T": -1}, "range"), ({"T": 0}, "no tokens"), ({"H": 0}, "range"),
            ({"G": 0}, "divide"), ({"H": 3, "G": 2}, "divide"), ({"G": 4}, "divide"), ({"dk": 0}, "1 .. 128"), ({"dv": 129}, "1 .. 128"), ({"g": None}, "null"),
            ({"g": A + 2}, "misaligned"), ({"ib": 2}, "4 or 8"), ({"n": A + 4}, "misaligned"), ({"scale": math.inf}, "scale"), ({"scale": math.nan}, "scale"),
-           ({"Bn": 1 << 20, "H": 1 << 12}, "chunks")]
+           ({"Bn": 1 << 20, "H": 1 << 12}, "too many"), ({"Bn": 1398102, "H": 1}, "out of range"), ({"Bn": 699051, "H": 2}, "too many")]
     for kw, why in bad + [({"o": None}, "null"), ({"o": A + 1}, "misaligned"), ({"s": A + 2}, "misaligned"), ({"so": A + 2}, "misaligned"),
                           ({"ws": None}, "workspace"), ({"ws": A + 8}, "workspace"), ({"have": need - 1}, "workspace")]:
         assert refused(fwd(**kw), why), (kw, hip_abi.last_error())
@@ -114,7 +114,7 @@ def test_decay_attention_refuses_bad_arguments():
 
     for kw, why in [({"q": None}, "null"), ({"g": None}, "null"), ({"s": None}, "null"), ({"o": None}, "null"), ({"slots": 2}, "fewer states"),
                     ({"slots": -1, "i": A}, "fewer states"), ({"i": A, "ib": 1}, "4 or 8"), ({"s": A + 2}, "misaligned"), ({"H": 3, "G": 2}, "divide"),
-                    ({"dk": 129}, "1 .. 128"), ({"scale": math.nan}, "scale")]:
+                    ({"dk": 129}, "1 .. 128"), ({"scale": math.nan}, "scale"), ({"Bn": 699051, "slots": 699051}, "too many")]:
         assert refused(step(**kw), why), (kw, hip_abi.last_error())
     assert step(Bn=0, q=None, slots=0) == 0
 
