@@ -45,7 +45,6 @@ struct Heads {
 struct Walk {
   Heads q, k, v;
   int dk, dv;       // head sizes of k and q, and of v
-  int dma;          // rows of k and v can be loaded by the LDS DMA
   int vb;           // workgroups along dv
   int reverse;
   float p_scale, q_scale, kv_scale;
@@ -151,6 +150,7 @@ struct Stream {
   const uint16_t* first;  // the segment's first token
   int64_t step;
   int d;
+  bool narrow;  // no 8 elements up to the end of d in a row
 };
 
 // Rows sh .. 63 of a chunk (tokens c0 .. of the segment) into a tile, zeros in the rows before and behind d: by
@@ -194,17 +194,42 @@ struct Dma {
   }
 };
 
-// The same for rows of any length, stride and alignment, through registers.
-template <int W>
-__device__ inline void stage_any(const Stream& x, int c0, int sh, uint16_t* tile, int tid) {
-#pragma unroll 2
-  for (int i = tid; i < kC * (W / 8); i += 256) {
-    const int r = i / (W / 8), p = i % (W / 8);
-    Pix8 v = {{0u, 0u, 0u, 0u}};
-    if (r >= sh && p * 8 < x.d) v = row_vec(x.first + (c0 + r - sh) * x.step + p * 8, x.d - p * 8);
-    *reinterpret_cast<uint4*>(tile + place<W>(r, p)) = make_uint4(v.v[0], v.v[1], v.v[2], v.v[3]);
-  }
+// 8 elements of a row of d from column c on (a multiple of 8 below d + 8 k): a row's last ones in a window that ends with
+// it, so that every load is whole and hangs on no branch; `to_place` puts them where they belong.  Rows shorter than a
+// window, which does not start before the tensor's row, are read one by one.
+__device__ inline Pix8 window8(const uint16_t* row, int c, int d, bool narrow) {
+  if (!narrow) return *reinterpret_cast<const Pix8*>(row + min(c, d - 8));
+  return row_vec(row + min(c, d), max(d - c, 0));
 }
+__device__ inline Pix8 to_place(const Pix8& v, int c, int d, bool narrow) {
+  if (c >= d) return {{0u, 0u, 0u, 0u}};
+  return narrow ? v : shifted(v, max(c + 8 - d, 0));
+}
+
+// The same as Dma for rows of any length, stride and alignment, through registers: loaded before a chunk's work, written to
+// LDS behind it (one behind the other, the loads' way was in every chunk: heads of 127 took 271 us where 128 take 74).
+template <int W>
+struct Staged {
+  static constexpr int P = W / 8, N = W / 32;
+  Pix8 v[N];
+
+  __device__ inline void load(const Stream& x, int c0, int sh, int t) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = (t + 256 * i) / P, p = (t + 256 * i) % P;
+      v[i] = window8(x.first + (c0 + max(r - sh, 0)) * x.step, p * 8, x.d, x.narrow);
+    }
+  }
+  __device__ inline void store(const Stream& x, int sh, uint16_t* tile, int t) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = (t + 256 * i) / P, p = (t + 256 * i) % P;
+      Pix8 q = to_place(v[i], p * 8, x.d, x.narrow);
+      if (r < sh) q = {{0u, 0u, 0u, 0u}};
+      *reinterpret_cast<uint4*>(tile + place<W>(r, p)) = make_uint4(q.v[0], q.v[1], q.v[2], q.v[3]);
+    }
+  }
+};
 
 __device__ inline int64_t length_of(const DecayArgs& a, int b) {
   if (!a.lengths) return a.T;
@@ -227,7 +252,8 @@ struct Lds {  // two buffers each; of a segment's state by itself three, and non
 // worked on, and the state before a chunk is in LDS twice, so that a chunk has one barrier.  A chunk of n < 64 tokens
 // takes the tile's last n rows, its first ones are zeros: the weights inside a chunk, which go by differences and by the
 // distance to its end, are those of every other.
-template <int KT, bool STATE>
+//   DMA: rows of k and v are whole 16-byte pieces.
+template <int KT, bool STATE, bool DMA>
 __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a) {
   using L = Lds<KT>;
   constexpr int THREADS = STATE ? 256 : 512;
@@ -267,8 +293,8 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
   // place i of the segment is token t0 + i or, backwards, t0 - i
   const int64_t t0 = w.reverse ? len - 1 - begin : begin;
   const auto step = [&](int64_t st) { return w.reverse ? -st : st; };
-  const Stream kx = {w.k.p + batch * w.k.sb + int64_t(head / w.k.share) * w.k.sh + t0 * w.k.st, step(w.k.st), dk};
-  const Stream vx = {w.v.p + batch * w.v.sb + int64_t(head / w.v.share) * w.v.sh + t0 * w.v.st + d0, step(w.v.st), dv};
+  const Stream kx = {w.k.p + batch * w.k.sb + int64_t(head / w.k.share) * w.k.sh + t0 * w.k.st, step(w.k.st), dk, dk < 8};
+  const Stream vx = {w.v.p + batch * w.v.sb + int64_t(head / w.v.share) * w.v.sh + t0 * w.v.st + d0, step(w.v.st), dv, w.dv < 8};
 
   // ---- tokens behind the sequence: zeros
   if constexpr (!STATE) {
@@ -294,21 +320,30 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
     const int vt = STATE ? wave : wave - 4;
     const Dma<KT> k_dma(kx, lane);
     const Dma<kVB> v_dma(vx, lane);
-    const bool whole = w.dma && dk == KT && dv == kVB;
-    const auto stage = [&](int c0, int b) {  // chunk c0 .. into buffer b
+    const bool whole = DMA && dk == KT && dv == kVB;
+    Staged<KT> k_staged;
+    Staged<kVB> v_staged;
+    const auto load = [&](int c0, int b) {  // chunk c0 .. into buffer b, or the registers that go there
       const int sh = max(0, kC - (todo - c0));
-      if (w.dma) {
+      if constexpr (DMA) {
         const int l = here(lane);
         k_dma.load_some(kx, c0, sh, ks + b * L::k, l, vt);
         v_dma.load_some(vx, c0, sh, vs + b * L::v, l, vt);
       } else {
         const int t = here(64 * vt + lane);
-        stage_any<KT>(kx, c0, sh, ks + b * L::k, t);
-        stage_any<kVB>(vx, c0, sh, vs + b * L::v, t);
+        k_staged.load(kx, c0, sh, t);
+        v_staged.load(vx, c0, sh, t);
       }
     };
-    if (todo > 0) stage(0, 0);
-    if (STATE && todo > kC) stage(kC, 1);
+    const auto write = [&](int c0, int b) {
+      if constexpr (!DMA) {
+        const int sh = max(0, kC - (todo - c0)), t = here(64 * vt + lane);
+        k_staged.store(kx, sh, ks + b * L::k, t);
+        v_staged.store(vx, sh, vs + b * L::v, t);
+      }
+    };
+    if (todo > 0) load(0, 0), write(0, 0);
+    if (STATE && todo > kC) load(kC, 1), write(kC, 1);
     f32x4_t S[NS];
 #pragma unroll
     for (int x = 0; x < NS; ++x) S[x] = zero4();
@@ -361,12 +396,14 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
       // the buffers that the next loads take.  A segment's state by itself has the loads of two chunks under way (one
       // ahead, it took 2.6 us a chunk, twice its work).
       lds_reads_wait();  // (its LDS writes; stated here, since the compiler leaves the barrier's own wait out beside the next line's)
-      if (STATE && c0 + kC < todo) lds_dma_wait<Dma<KT>::N + Dma<kVB>::N>();
-      else lds_dma_wait<0>();
+      if constexpr (DMA) {
+        if (STATE && c0 + kC < todo) lds_dma_wait<Dma<KT>::N + Dma<kVB>::N>();
+        else lds_dma_wait<0>();
+      }
       __syncthreads();
       const int coming = c0 + (STATE ? 2 : 1) * kC, to = STATE ? (b == 0 ? 2 : b - 1) : b ^ 1;
       const bool ahead = whole && coming + kC <= todo;  // a whole chunk: its loads go between the products
-      if (!ahead && coming < todo) stage(coming, to);
+      if (!ahead && coming < todo) load(coming, to);
       i32x4_t k_rows, v_rows;
       if (ahead) k_rows = k_dma.rows(kx, coming, 0), v_rows = v_dma.rows(vx, coming, 0);
       const uint32_t k_tr = here(k_at.tr + smem_at + uint32_t(b) * kBuf);
@@ -410,6 +447,7 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
             for (int x = 0; x < 4; ++x) S[x0 + x] = mfma(k[x], as_bf16x8(part[y]), S[x0 + x]);
         }
       }
+      if (coming < todo) write(coming, to);
       if (!STATE && c0 + kC < todo) store_state(b ^ 1);
     }
     if (STATE || last) {
@@ -447,7 +485,7 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           const int c = 32 * kk + 8 * g;
-          qf[kk] = row_vec(from + min(c, d), max(d - c, 0));
+          qf[kk] = to_place(window8(from, c, d, d < 8), c, d, d < 8);
         }
       }
     };
@@ -797,20 +835,13 @@ bool dma_rows(const Heads& h) {
   return (reinterpret_cast<uintptr_t>(h.p) & 15) == 0 && h.sb % 8 == 0 && h.st % 8 == 0 && h.sh % 8 == 0 && h.st < (int64_t(1) << 23);
 }
 
-template <int KT, bool STATE>
-bool launch_walks(DecayArgs& a, hipStream_t st) {
+template <int KT, bool STATE, bool DMA>
+bool launch_walks(const DecayArgs& a, hipStream_t st) {
   constexpr size_t bytes = STATE ? Lds<KT>::state_bytes : Lds<KT>::bytes;
-  void (*f)(DecayArgs) = walk_kernel<KT, STATE>;
+  void (*f)(DecayArgs) = walk_kernel<KT, STATE, DMA>;
   static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize,
                                              int(bytes)) == hipSuccess;
   if (!ok) return false;
-  a.blocks = 0;
-  for (int i = 0; i < a.n; ++i) {
-    Walk& w = a.walk[i];
-    w.vb = blocks64(w.dv);
-    w.dma = w.dk % 8 == 0 && w.dv % 8 == 0 && dma_rows(w.k) && dma_rows(w.v) ? 1 : 0;
-    a.blocks += w.vb;
-  }
   const int64_t n = int64_t(a.B) * a.H * a.blocks * (STATE ? a.segments - 1 : a.segments);
   f<<<unsigned(n), STATE ? 256 : 512, bytes, st>>>(a);
   return true;
@@ -820,13 +851,18 @@ bool launch_walks(DecayArgs& a, hipStream_t st) {
 // each took 26 us where one takes 16: 3 x 777 tokens, 6 heads of 48 and 80).
 template <bool STATE>
 bool launch(DecayArgs a, const Walk* walks, int n, hipStream_t st) {
-  bool big = false;
+  bool big = false, dma = true;
   a.n = n;
+  a.blocks = 0;
   for (int i = 0; i < n; ++i) {
-    a.walk[i] = walks[i];
-    big |= walks[i].dk > 64;
+    Walk& w = a.walk[i] = walks[i];
+    w.vb = blocks64(w.dv);
+    a.blocks += w.vb;
+    big |= w.dk > 64;
+    dma = dma && w.dk % 8 == 0 && w.dv % 8 == 0 && dma_rows(w.k) && dma_rows(w.v);
   }
-  return big ? launch_walks<128, STATE>(a, st) : launch_walks<64, STATE>(a, st);
+  if (dma) return big ? launch_walks<128, STATE, true>(a, st) : launch_walks<64, STATE, true>(a, st);
+  return big ? launch_walks<128, STATE, false>(a, st) : launch_walks<64, STATE, false>(a, st);
 }
 
 // the segments' own states, and where they are many the states before them
