@@ -194,17 +194,10 @@ struct Dma {
   }
 };
 
-// 8 elements of a row of d from column c on (a multiple of 8 below d + 8 k): a row's last ones in a window that ends with
-// it, so that every load is whole and hangs on no branch; `to_place` puts them where they belong.  Rows shorter than a
-// window, which does not start before the tensor's row, are read one by one.
-__device__ inline Pix8 window8(const uint16_t* row, int c, int d, bool narrow) {
-  if (!narrow) return *reinterpret_cast<const Pix8*>(row + min(c, d - 8));
-  return row_vec(row + min(c, d), max(d - c, 0));
-}
-__device__ inline Pix8 to_place(const Pix8& v, int c, int d, bool narrow) {
-  if (c >= d) return {{0u, 0u, 0u, 0u}};
-  return narrow ? v : shifted(v, max(c + 8 - d, 0));
-}
+// 8 elements of a row of d (at least 8) from column c on: a row's last ones in a window that ends with it, so that every
+// load is whole and hangs on no branch; `to_place` then puts them where they belong, zeros behind them.
+__device__ inline Pix8 window8(const uint16_t* row, int c, int d) { return *reinterpret_cast<const Pix8*>(row + min(c, d - 8)); }
+__device__ inline Pix8 to_place(const Pix8& v, int c, int d) { return c < d ? shifted(v, max(c + 8 - d, 0)) : Pix8{{0u, 0u, 0u, 0u}}; }
 
 // The same as Dma for rows of any length, stride and alignment, through registers: loaded before a chunk's work, written to
 // LDS behind it (one behind the other, the loads' way was in every chunk: heads of 127 took 271 us where 128 take 74).
@@ -214,20 +207,25 @@ struct Staged {
   Pix8 v[N];
 
   __device__ inline void load(const Stream& x, int c0, int sh, int t) {
+    if (x.narrow) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = window8(x.first + (c0 + max(t / P + i * (256 / P) - sh, 0)) * x.step, t % P * 8, x.d);
+  }
+  __device__ inline void store(const Stream& x, int c0, int sh, uint16_t* tile, int t) const {
+    if (x.narrow) {  // (rows of under 8: element by element, here)
+#pragma unroll 1
+      for (int r = t / P; r < kC; r += 256 / P) put(tile, r, t % P, row_vec(x.first + (c0 + max(r - sh, 0)) * x.step, r >= sh && t % P == 0 ? x.d : 0));
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int r = (t + 256 * i) / P, p = (t + 256 * i) % P;
-      v[i] = window8(x.first + (c0 + max(r - sh, 0)) * x.step, p * 8, x.d, x.narrow);
+      const int r = t / P + i * (256 / P);
+      put(tile, r, t % P, r >= sh ? to_place(v[i], t % P * 8, x.d) : Pix8{{0u, 0u, 0u, 0u}});
     }
   }
-  __device__ inline void store(const Stream& x, int sh, uint16_t* tile, int t) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = (t + 256 * i) / P, p = (t + 256 * i) % P;
-      Pix8 q = to_place(v[i], p * 8, x.d, x.narrow);
-      if (r < sh) q = {{0u, 0u, 0u, 0u}};
-      *reinterpret_cast<uint4*>(tile + place<W>(r, p)) = make_uint4(q.v[0], q.v[1], q.v[2], q.v[3]);
-    }
+  __device__ static inline void put(uint16_t* tile, int r, int p, const Pix8& q) {
+    *reinterpret_cast<uint4*>(tile + place<W>(r, p)) = make_uint4(q.v[0], q.v[1], q.v[2], q.v[3]);
   }
 };
 
@@ -338,8 +336,8 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
     const auto write = [&](int c0, int b) {
       if constexpr (!DMA) {
         const int sh = max(0, kC - (todo - c0)), t = here(64 * vt + lane);
-        k_staged.store(kx, sh, ks + b * L::k, t);
-        v_staged.store(vx, sh, vs + b * L::v, t);
+        k_staged.store(kx, c0, sh, ks + b * L::k, t);
+        v_staged.store(vx, c0, sh, vs + b * L::v, t);
       }
     };
     if (todo > 0) load(0, 0), write(0, 0);
@@ -475,17 +473,23 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
       const int sh = max(0, kC - (todo - c0));
       const uint16_t* from = qp + (c0 + max(row - sh, 0)) * q_step;
       const int d = here(dk);
-      if (dk == KT) {
+      if (DMA && dk == KT) {
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(from + 32 * kk + 8 * g);
-      } else if (dk % 8 == 0) {
+      } else if (DMA || d >= 8) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const Pix8*>(from + min(32 * kk + 8 * g, d - 8));
+        for (int kk = 0; kk < KK; ++kk) qf[kk] = window8(from, 32 * kk + 8 * g, d);
       } else {
+        qf[0] = row_vec(from, d);
+      }
+    };
+    const auto place_q = [&] {  // (with DMA a row is whole pieces: they are in place, and those past it meet zeros)
+      if constexpr (!DMA) {
+        const int d = here(dk);
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           const int c = 32 * kk + 8 * g;
-          qf[kk] = to_place(window8(from, c, d, d < 8), c, d, d < 8);
+          qf[kk] = d >= 8 ? to_place(qf[kk], c, d) : c == 0 ? qf[0] : Pix8{{0u, 0u, 0u, 0u}};
         }
       }
     };
@@ -513,6 +517,7 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = zero4();
       if (16 * wave + 16 > sh) {
+        place_q();
         const uint32_t k_row = here(k_at.row + smem_at + uint32_t(b) * kBuf), s_row = k_row + kS;
         const uint32_t v_tr = here(v_at.tr + smem_at + 2 * kBuf + uint32_t(b) * vBuf);
 #pragma unroll
