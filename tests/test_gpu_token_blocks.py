@@ -538,6 +538,22 @@ def test_decay_attention_in_segments(T, hip, size, forward, backward, ragged):
     check_decay(got, decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], lengths, size[4] ** -0.5, v["dout"], v["dstate"]))
 
 
+@pytest.mark.parametrize("ragged", [False, True], ids=["whole", "ragged"])
+@pytest.mark.parametrize("size", [(1, 1500, 2, 1, 33, 65), (2, 1300, 5, 5, 100, 71), (1, 1100, 6, 3, 127, 5), (2, 900, 3, 3, 6, 126), (1, 2000, 14, 14, 90, 66)])
+def test_decay_attention_of_odd_heads_in_segments(T, hip, size, ragged):
+    """Rows that are no whole vectors, shorter than one, or whose last block of columns is."""
+    n = [segments(hip, size, b) for b in (False, True)]
+    print("decay odd segments", size, ragged, n, flush=True)
+    assert max(n) > 1, n
+    v = decay_values(*size, seed=17)
+    lengths = torch.tensor([700, 65][: size[0]]) if ragged else None
+    ref = decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], lengths, size[4] ** -0.5, v["dout"], v["dstate"])
+    for b in range(size[0] if ragged else 0):
+        for name in ("q", "k", "v", "dout"):
+            v[name][b, int(lengths[b]):] = math.nan
+    check_decay(run_decay(T, v, lengths), ref)
+
+
 def test_decay_attention_of_many_heads_in_one_walk(T):
     """As many workgroups as the chip takes: no segments, several chunks each."""
     size = (1, 400, 260, 260, 9, 70)
