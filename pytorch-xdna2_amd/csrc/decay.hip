@@ -229,6 +229,12 @@ struct Staged {
   }
 };
 
+// This workgroup's place in an order whose neighbours are on one XCD (workgroups go to the 8 XCDs in turn).
+__device__ inline int xcd_block() {
+  const int n = int(gridDim.x), xcd = int(blockIdx.x) % 8;
+  return xcd * (n / 8) + min(xcd, n % 8) + int(blockIdx.x) / 8;
+}
+
 __device__ inline int64_t length_of(const DecayArgs& a, int b) {
   if (!a.lengths) return a.T;
   const int64_t n = a.index_bytes == 8 ? static_cast<const int64_t*>(a.lengths)[b] : static_cast<const int32_t*>(a.lengths)[b];
@@ -267,15 +273,13 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
   // workgroups of one sequence and head, all walks', next to each other on one XCD: they read the same rows, and each XCD
   // has its own L2 (walk after walk, the backward of 8 x 2048 tokens, 16 heads of 128 took 177 us for 169, of 16 x 2048
   // with heads of 64 165 for 150)
-  const int n_all = int(gridDim.x), xcd = int(blockIdx.x) % 8;
-  int64_t id = int64_t(xcd) * (n_all / 8) + min(xcd, n_all % 8) + int(blockIdx.x) / 8;
-  int vb = int(id % a.blocks), wi = 0;
+  int id = xcd_block();
+  int vb = id % a.blocks, wi = 0;
   id /= a.blocks;
   while (vb >= a.walk[wi].vb) vb -= a.walk[wi++].vb;
   const Walk& w = a.walk[wi];
   const int n_seg = STATE ? a.segments - 1 : a.segments;
-  const int seg = int(id % n_seg);
-  const int head = int(id / n_seg % a.H), batch = int(id / n_seg / a.H);
+  const int seg = id % n_seg, head = id / n_seg % a.H, batch = id / n_seg / a.H;
   const int64_t bh = int64_t(batch) * a.H + head;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -665,7 +669,9 @@ __global__ __launch_bounds__(256) void group_kernel(GroupArgs a) {
 
 // ---- single tokens --------------------------------------------------------------------------------
 // S = a S + k^T v in place, o = scale q S.  Bound by the state's bytes, read and written once: a
-// workgroup takes a head and 32 columns of v, a thread four columns of every 32nd row.
+// workgroup takes a head and 32 columns of v, a thread four columns of every 32nd row.  64 x 16 heads of 128: 26 us, 5.1
+// TB/s.  Where tiles share lines of memory, those of a head are on one XCD, whose L2 puts the lines together (heads of 127
+// 49 -> 34 us, of 100 32 -> 21; heads of 128 are 1 us faster spread out).
 struct StepArgs {
   Heads q, k, v;
   int B, H, dk, dv;
@@ -678,6 +684,7 @@ struct StepArgs {
   uint16_t* out;  // dense [B][H][dv]
   int tiles;      // of 32 columns
   int vec;        // rows of whole 16-byte vectors
+  int lines;      // and a tile's rows whole lines of memory
 };
 
 __device__ inline int64_t slot_of(const StepArgs& a, int b) {
@@ -687,7 +694,7 @@ __device__ inline int64_t slot_of(const StepArgs& a, int b) {
 
 __global__ __launch_bounds__(256) void step_kernel(StepArgs a) {
   __shared__ float red[4][32];
-  const int tile = int(blockIdx.x) % a.tiles, head = int(blockIdx.x) / a.tiles % a.H, b = int(blockIdx.x) / a.tiles / a.H;
+  const int id = a.lines ? int(blockIdx.x) : xcd_block(), tile = id % a.tiles, head = id / a.tiles % a.H, b = id / a.tiles / a.H;
   const int tid = threadIdx.x, c = tile * 32 + (tid & 7) * 4, r0 = tid >> 3;
   const int64_t slot = slot_of(a, b);
   uint16_t* out = a.out + (int64_t(b) * a.H + head) * a.dv;
@@ -718,6 +725,10 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs a) {
         if (a.vec) {
           const float4 x = *reinterpret_cast<const float4*>(S + int64_t(r) * a.dv);
           s[i][0] = x.x, s[i][1] = x.y, s[i][2] = x.z, s[i][3] = x.w;
+        } else if (n == 4) {
+          const Floats4 x = *reinterpret_cast<const Floats4*>(S + int64_t(r) * a.dv);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] = x.v[e];
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[i][e] = e < n ? S[int64_t(r) * a.dv + e] : 0.0f;
@@ -736,6 +747,8 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs a) {
         }
         if (a.vec) {
           *reinterpret_cast<float4*>(S + int64_t(r) * a.dv) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+        } else if (n == 4) {
+          *reinterpret_cast<Floats4*>(S + int64_t(r) * a.dv) = {{s[i][0], s[i][1], s[i][2], s[i][3]}};
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -1058,6 +1071,7 @@ int xdna_decay_step(const xdna_heads_bf16* q, const xdna_heads_bf16* k, const xd
   a.out = out;
   a.tiles = int(ceil_div(dv, int64_t(32)));
   a.vec = dv % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15) == 0 ? 1 : 0;
+  a.lines = dv % 32 == 0 && (reinterpret_cast<uintptr_t>(state) & 127) == 0 ? 1 : 0;
   step_kernel<<<unsigned(B * H * a.tiles), 256, 0, as_stream(stream)>>>(a);
   return check_launch(what);
 }
