@@ -909,8 +909,8 @@ int xdna_distill_bwd(const void* logits, int dtype, int64_t rows, int64_t vocab,
 /* Layer norm of rows of dim elements: y = (s - m) / sqrt(var + eps) * weight + bias, s = x, or with a
  * residual s = x + residual, stored (rounded once) in `sum`; the norm is that of the stored sum.
  * weight / bias: NULL (1 / 0) or dim values of param_dtype (fp32, or the rows' dtype).  stats (NULL, or
- * two floats a row): mean and 1 / sqrt(var + eps), for the gradient.  sum and y are dense.  dim up to
- * 2^24.  eps >= 0. */
+ * two floats a row): mean and 1 / sqrt(var + eps), for the gradient.  sum and y are dense, and no operand's
+ * memory.  dim up to 2^24.  eps >= 0. */
 int xdna_layer_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, int dtype, int64_t rows, int64_t dim,
                     const void* weight, const void* bias, int param_dtype, float eps, void* sum, void* y, float* stats,
                     void* stream);

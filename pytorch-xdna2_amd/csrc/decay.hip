@@ -256,6 +256,10 @@ struct Lds {  // two buffers each; of a segment's state by itself three, and non
 // worked on, and the state before a chunk is in LDS twice, so that a chunk has one barrier.  A chunk of n < 64 tokens
 // takes the tile's last n rows, its first ones are zeros: the weights inside a chunk, which go by differences and by the
 // distance to its end, are those of every other.
+//   A chunk takes 2.2 us with one workgroup a CU and 3.3 with two: MFMAs a third of it and LDS reads under a half, a wave's
+// products, scores and weights one after the other.  8 x 2048 tokens, 16 heads of 128: forward 75 us (256 workgroups, one a
+// CU; 268 MB, 3.6 TB/s), backward 169 (three walks, 805 MB, 4.8 TB/s: bound by memory); 1 x 8192 tokens: the segments'
+// states 21, their sums 6, the outputs 33.
 //   DMA: rows of k and v are whole 16-byte pieces.
 template <int KT, bool STATE, bool DMA>
 __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a) {
@@ -801,33 +805,36 @@ Heads heads_of(const xdna_heads_bf16* h, int64_t share) { return {h->data, h->ba
 
 constexpr int kScanFrom = 5;  // segments from which on their states are summed up by a launch
 
-// Segments of a sequence, by what a call takes in us.  Fitted to 11 shapes (1 to 6 sequences of 200 to 32768 tokens, 4 to
-// 16 heads of 64 or 128, both directions, 1 to 64 segments; 10 % off in the mean): a chunk takes 1.55 with few
-// workgroups, 2.2 with one on each CU and 3.3 with two; of the segments' own states 1.05 a workgroup on a CU; heads up to 64
-// three quarters of that.  1 x 8192 tokens, 16 heads of 128, forward: 201 us whole, 62 in 8 segments, 59 in 16, 104 in 64;
-// 6 x 1024 tokens 33 whole, 43 in 2; backward of 1 x 8192 203 whole, 117 in 5, 137 in 16.
+// Segments of a sequence, by what a call takes in us.  Fitted to 21 shapes (1 to 8 sequences of 300 to 32768 tokens, 2 to
+// 32 heads of 32, 64 or 128, both directions, whole and in 2 to 64 segments; 8 % off in the mean, the choice under 2 % slower
+// than the best in the mean and 15 % at most): a chunk takes 1.4 with few workgroups, 1.7 with one on each CU, and with two
+// 2.8 forward and 3.2 backward (three walks' rows from memory); of the segments' own states 0.43 a workgroup on a CU, at
+// least 1.1; heads up to 64 three quarters of that; the states' sums 0.94 a MB.  1 x 8192 tokens, 16 heads of 128, forward:
+// 193 us whole, 60 in 8 segments, 56 in 16, 97 in 64; 4 x 5000, 4 heads of 64: 99, 32, 24 and 32; backward of 1 x 8192 199
+// whole, 113 in 8, 129 in 16.
 struct Plan {
   int segments, chunks;
 };
 
-float walk_cost(int64_t workgroups, int64_t chunks) {
-  const auto round = [](float n) { return n <= 256.0f ? 1.55f + 0.65f * n / 256.0f : 2.2f + 1.1f * (n - 256.0f) / 256.0f; };
+// `chunk`: a chunk's time against that of heads of 128, `two`: that with two workgroups on each CU
+float walk_cost(int64_t workgroups, int64_t chunks, float chunk, float two) {
+  const auto round = [&](float n) { return n <= 256.0f ? 1.4f + 0.3f * n / 256.0f : 1.7f + (two - 1.7f) * (n - 256.0f) / 256.0f; };
   const int64_t rest = workgroups % 512;
-  return 5.0f + float(chunks) * (3.3f * float(workgroups / 512) + (rest ? round(float(rest)) : 0.0f));
+  return 5.4f + float(chunks) * chunk * (two * float(workgroups / 512) + (rest ? round(float(rest)) : 0.0f));
 }
 
 // `walks`, `states`: workgroups of a segment's walks and of its states; `state_mb`: bytes of all heads' states
-Plan plan_segments(int64_t walks, int64_t states, float state_mb, int64_t T, bool big) {
+Plan plan_segments(int64_t walks, int64_t states, float state_mb, int64_t T, bool big, float two) {
   const int64_t chunks = ceil_div(T, int64_t(kC));
   const float size = big ? 1.0f : 0.75f;
   Plan best = {1, int(std::max<int64_t>(chunks, 1))};
   if (walks > kSplitWalks) return best;  // (the last round's gap is an eighth of the time at most, the states' pass a quarter)
-  float least = walk_cost(walks, chunks) * size;
+  float least = 0.95f * walk_cost(walks, chunks, size, two);  // (cut for a gain beyond the fit's errors)
   for (int64_t n = 2; n <= std::min<int64_t>(chunks, 256); n += n < 64 ? 1 : 32) {
     const int64_t per = ceil_div(chunks, n), segments = ceil_div(chunks, per);
-    const float own = 6.0f + float(per) * std::max(1.0f, 1.05f * float(states * (segments - 1)) / 256.0f);
-    const float join = segments >= kScanFrom ? 4.0f + 0.34f * state_mb * float(segments - 1) : float(segments - 1);
-    const float cost = (walk_cost(walks * segments, per) + 3.0f + own) * size + join;
+    const float own = 3.4f + float(per) * size * std::max(1.1f, 0.43f * float(states * (segments - 1)) / 256.0f);
+    const float join = segments >= kScanFrom ? 2.9f + (0.94f * state_mb + 0.08f) * float(segments - 1) : 1.25f * float(segments - 1);
+    const float cost = walk_cost(walks * segments, per, size, two) + own + join;
     if (cost < least) least = cost, best = {int(segments), int(per)};
   }
   return best;
@@ -837,11 +844,11 @@ int blocks64(int64_t d) { return int(ceil_div(d, int64_t(kVB))); }
 
 Plan fwd_plan(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv) {
   const int64_t n = B * H * blocks64(dv);
-  return plan_segments(n, n, float(B * H * dk * dv) * 4e-6f, T, dk > 64);
+  return plan_segments(n, n, float(B * H * dk * dv) * 4e-6f, T, dk > 64, 2.8f);
 }
 Plan bwd_plan(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv) {
   return plan_segments(B * H * (2 * blocks64(dk) + blocks64(dv)), 2 * B * H * blocks64(dv), float(B * H * dk * dv) * 8e-6f, T,
-                       dk > 64 || dv > 64);
+                       dk > 64 || dv > 64, 3.2f);
 }
 
 size_t local_floats(const Plan& p, int64_t B, int64_t H, int64_t dk, int64_t dv) {

