@@ -97,7 +97,9 @@ __device__ inline void put4(float* row, int c, int d, bool vec, const f32x4_t& v
 }
 
 // Tiles in LDS: rows of W elements (64 or 128), in pieces of 8.  Piece p of row r is at p ^ swizzle(r): 16 lanes of a
-// row read (16 rows x 4 pieces) and 32 of a transposing read (8 rows x 2 pieces) then fall on distinct banks.
+// row read (16 rows x 4 pieces) and 32 of a transposing read (8 rows x 2 pieces) then fall on distinct banks.  (The writes
+// of the state's operand form do meet on banks, 29 % of the LDS's cycles; in whole pieces or with rows 8 apart on other
+// banks they meet less, and no call gets faster by more than the 2 % that others lose.)
 template <int W>
 __device__ inline int swizzle(int r) {
   return W == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
@@ -256,10 +258,10 @@ struct Lds {  // two buffers each; of a segment's state by itself three, and non
 // worked on, and the state before a chunk is in LDS twice, so that a chunk has one barrier.  A chunk of n < 64 tokens
 // takes the tile's last n rows, its first ones are zeros: the weights inside a chunk, which go by differences and by the
 // distance to its end, are those of every other.
-//   A chunk takes 2.2 us with one workgroup a CU and 3.3 with two: MFMAs a third of it and LDS reads under a half, a wave's
-// products, scores and weights one after the other.  8 x 2048 tokens, 16 heads of 128: forward 75 us (256 workgroups, one a
-// CU; 268 MB, 3.6 TB/s), backward 169 (three walks, 805 MB, 4.8 TB/s: bound by memory); 1 x 8192 tokens: the segments'
-// states 21, their sums 6, the outputs 33.
+//   A chunk takes 2.2 us with one workgroup a CU and 3.3 with two: VALU and MFMA a third of it each, LDS reads about as
+// much, a wave's products, scores and weights one after the other.  8 x 2048 tokens, 16 heads of 128: forward 75 us (256
+// workgroups, one a CU; 268 MB, 3.6 TB/s), backward 169 (three walks, 805 MB of rows, of which 647 come from memory: 3.8
+// TB/s); 1 x 8192 tokens: the segments' states 21, their sums 6, the outputs 33.
 //   DMA: rows of k and v are whole 16-byte pieces.
 template <int KT, bool STATE, bool DMA>
 __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a) {
