@@ -932,6 +932,71 @@ def test_captured_blocks_follow_their_inputs(T, leaves):
         gr.reset()
 
 
+def test_one_tensor_in_several_places(T):
+    """A tensor that a call has twice or three times gets the sum of what separate ones get."""
+    x, w = torch.randn(40, 64, generator=gen(1)).to(BF16), (torch.randn(64, 64, generator=gen(2)) / 8).to(BF16)
+    dy = torch.randn(40, 64, generator=gen(3)).to(BF16).to("xdna")
+
+    def grads(call, n, shape):
+        one = x.view(shape).to("xdna").requires_grad_()
+        several = [x.view(shape).to("xdna").requires_grad_() for _ in range(n)]
+        y1, y = call(*[one] * n), call(*several)
+        assert same(y1, y)
+        g = torch.autograd.grad(y, several, dy.view(y.shape))
+        return torch.autograd.grad(y1, one, dy.view(y1.shape))[0], [t.cpu().double() for t in g]
+
+    log_decay = torch.tensor([-0.1, -0.5], device="xdna")
+    for call, n, shape in [(lambda a, b: T.add_layer_norm(a, b).norm, 2, (40, 64)), (lambda a, b: T.linear(a, w.to("xdna"), None, "silu", b), 2, (40, 64)),
+                           (lambda a, b, c: T.decay_attention(a, b, c, log_decay).out, 3, (2, 20, 2, 32))]:
+        got, parts = grads(call, n, shape)
+        size = sum(p.abs() for p in parts)
+        assert ((got.cpu().double() - sum(parts)).abs() <= (n - 1) * B * size).all()  # (a rounding of each sum of two)
+
+
+def test_a_result_written_before_its_backward_raises(T):
+    x, r = (torch.randn(5, 16, generator=gen(i)).to("xdna").requires_grad_() for i in (1, 2))
+    out = T.add_layer_norm(x, r)
+    with torch.no_grad():
+        out.sum.detach().add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.norm.sum().backward()
+    q = torch.randn(1, 9, 1, 8, generator=gen(3)).to(BF16).to("xdna").requires_grad_()
+    g, state = torch.tensor([-0.1], device="xdna"), torch.zeros(1, 1, 8, 8, device="xdna")
+    a = T.decay_attention(q, q, q, g, state)
+    with torch.no_grad():
+        T.decay_attention_step(*[q[:, 0].detach()] * 3, g, state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        a.out.sum().backward()
+
+
+def test_captured_attention_follows_lengths_and_slots(T):
+    """Lengths and slots are device data of a replay: rewritten between replays, they give the eager results."""
+    v = {n: t.to("xdna") for n, t in decay_values(3, 200, 2, 2, 16, 24, seed=6).items()}
+    lengths, slots = torch.tensor([200, 3, 64], device="xdna"), torch.tensor([0, 1, 2], device="xdna")
+    pool = torch.zeros(4, 2, 16, 24, device="xdna")
+
+    def run():
+        a = T.decay_attention(v["q"], v["k"], v["v"], v["g"], v["state"], lengths)
+        pool.zero_()
+        pool[:3].copy_(a.state)
+        return a.out, a.state, T.decay_attention_step(v["q"][:, 0], v["k"][:, 0], v["v"][:, 0], v["g"], pool, slots), pool.clone()
+
+    run()
+    graph = torch.xdna.Graph()
+    with torch.xdna.graph(graph):
+        out = run()
+    for n, s in [([0, 200, 65], [3, 2, 0]), ([7, 128, 500], [-1, 0, 1]), ([200, 3, 64], [2, 1, 0]), ([63, 1, -2], [3, 1, 2])]:
+        lengths.copy_(torch.tensor(n))
+        slots.copy_(torch.tensor(s))
+        torch.xdna.synchronize()
+        graph.replay()
+        torch.xdna.synchronize()
+        got = [t.cpu() for t in out]
+        for i, (a, b) in enumerate(zip(got, run())):
+            assert same(a, b), (n, s, i)
+    graph.reset()
+
+
 def test_refusals_on_the_device(T):
     x, w = torch.randn(3, 8, device="xdna"), torch.ones(8, device="xdna")
     for call, why in [
