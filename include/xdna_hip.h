@@ -934,11 +934,13 @@ int xdna_linear_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t 
 
 /* dp = dy act'(v) (M x N, dense, or NULL) from the kept slopes (not read with act 3), and d_bias (N, or NULL) = its
  * column sums before that rounding, fp32 in a fixed order.  dx = dp w and dw = dp^T x are plain products,
- * or one launch, where _pick says 1 (a few hundred rows). */
+ * or one launch: _pick says 1 for tiles of 64 or 128 (a few hundred rows), 2 for tiles of 256 (thousands; it then is the
+ * faster way at any rate), 0 for products apart. */
 size_t xdna_linear_bwd_workspace_bytes(int64_t M, int64_t N);
 int xdna_linear_bwd_bf16(const uint16_t* dy, int64_t ld, const void* kept, int act, int64_t M, int64_t N, uint16_t* dp,
                          uint16_t* d_bias, void* workspace, size_t workspace_bytes, void* stream);
-int xdna_linear_grads_pick(int64_t M, int64_t K, int64_t N);
+int xdna_linear_grads_pick(const uint16_t* dp, int64_t lddp, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw,
+                           int64_t M, int64_t K, int64_t N);
 int xdna_linear_grads_bf16(const uint16_t* dp, int64_t lddp, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw,
                            int64_t M, int64_t K, int64_t N, uint16_t* dx, uint16_t* dw, void* stream);
 

@@ -1162,6 +1162,59 @@ void gated_large_kernel(TileArgs a) {
   }
 }
 
+// ---- dx and dw of a large linear layer in one launch -----------------------------------------
+// The two products' 256 x 256 tiles, k split so that all of them are at work at once and end together: one by one, each
+// is split to fill the CUs by itself, and both have their partials to write and add.
+struct LargeGradsArgs {
+  TileArgs dx, dw;
+  int n_dx, n_dw;  // workgroups of each
+};
+
+template <bool QROWS>
+__device__ __forceinline__ void large_plain(const TileArgs& a, const TileAt tile, uint16_t* smem) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = wave & 1, wn = wave >> 1;
+  const int p0 = tile.x * kT4, q0 = tile.y * kT4, kbeg = tile.z * a.k_split;
+  f32x4_t acc[8][8];
+  {
+    const G5Operand op = g5_operand<kAlongRow, true>(a.p.src, 1, a.p.ld, p0, a.p.rows, a.K, tid);
+    G5Operand oq;
+    if constexpr (QROWS) oq = g5_operand<kAlongRow, true>(a.q.src, 1, a.q.ld, q0, a.q.rows, a.K, tid);
+    else oq = g5_operand<kAlongK, true>(a.q.src, a.q.ld, 1, q0, a.q.rows, a.K, tid);
+    gemm6_loop<kAlongRow, kDmaMode<QROWS>>(acc, op, oq, smem, kbeg, min(a.K, kbeg + a.k_split), tid);
+  }
+  mfma16_fence(acc);
+  float* epi = reinterpret_cast<float*>(smem);
+  const int o = tid & 31, at = p0 + 8 * o;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<f32x4_t*>(epi + (wn * 64 + j * 16 + (lane & 15)) * kEpiPitch + wm * 128 + i * 16 + 4 * (lane >> 4)) =
+            acc[i][half * 4 + j];
+    __syncthreads();
+#pragma unroll 4
+    for (int r = tid >> 5; r < kEpiRows; r += 8) {
+      const int q = q0 + 128 * (r >> 6) + 64 * half + (r & 63);
+      float d[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = epi[r * kEpiPitch + 8 * o + e];
+      if (q < a.q.rows && at < a.p.rows) put_row8<kPlain, kSilu>(a, q, at, a.p.rows - at, d, d, tile.z);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void linear_grads_large_kernel(LargeGradsArgs g) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
+  const int i = int(blockIdx.x);
+  if (i < g.n_dx) large_plain<false>(g.dx, tile_at(g.dx, i, g.n_dx), smem);
+  else large_plain<true>(g.dw, tile_at(g.dw, i - g.n_dx, g.n_dw), smem);
+}
+
 // ---- backward, elementwise: [dg du] from dh and the kept [g u] ------------------------------
 // Bound by its bytes: 8192 x 4096 units, 370 MB, take 65 us (5.7 TB/s).
 struct GatedBwdArgs {
@@ -1373,6 +1426,57 @@ bool launch_large(TileArgs a, dim3 tiles, hipStream_t st) {
   return true;
 }
 
+// dx and dw on large tiles in one launch: their splits, such that all workgroups are at work at once, by the launch's cost
+// in us.  Fitted to 8 sizes (3 % off at most): 0.87 a k-tile of the longest workgroup, and the split products' partials.
+// Measured, this launch, the tiles' best and the GEMM for each product: 8192 x 1024 -> 4096 132, 166 and 168; 8192 x 1024 -> 1024
+// 49, 65 and 175; 8192 x 512 -> 4096 91, 111 and 311; but 4096 x 1024 -> 4096 96, 83 and 107, 2048 x 1024 -> 2048 51, 31 and 131.
+struct LargeGrads {
+  int64_t s_dx, s_dw;
+  float cost;  // infinite: the tiles alone are more than the CUs
+};
+
+float large_join(int64_t splits, int64_t outputs) { return splits > 1 ? 4.0f + float(outputs) * float(splits) * 1.6e-6f : 0.0f; }
+
+LargeGrads plan_large_grads(int64_t M, int64_t K, int64_t N) {
+  const int64_t t = kT4, n_dx = ceil_div(K, t) * ceil_div(M, t), n_dw = ceil_div(K, t) * ceil_div(N, t);
+  const int64_t k_dx = ceil_div(N, int64_t(kK5)), k_dw = ceil_div(M, int64_t(kK5));
+  LargeGrads best = {1, 1, INFINITY};
+  for (int64_t a = 1; a <= 16; ++a)
+    for (int64_t b = 1; b <= 16 && n_dx * a + n_dw * b <= 256; ++b) {
+      const float cost = 4.0f + 0.87f * float(std::max(ceil_div(k_dx, a), ceil_div(k_dw, b))) + large_join(a, M * K) + large_join(b, N * K);
+      if (cost < best.cost) best = {a, b, cost};
+    }
+  return best;
+}
+
+bool launch_grads_large(GradsArgs g, hipStream_t st) {
+  static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(linear_grads_large_kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, int(kLargeLds)) == hipSuccess;
+  if (!ok) return false;
+  const LargeGrads p = plan_large_grads(g.dx.q.rows, g.dx.p.rows, g.dw_in.q.rows);
+  const auto plan = [](TileArgs& a, int64_t splits) {
+    a.k_split = int(ceil_div(ceil_div(a.K, kK5), splits)) * kK5;
+    splits = ceil_div(a.K, a.k_split);
+    if (splits > 1) {
+      a.part = static_cast<float*>(xdna_hip_cache_alloc(size_t(splits) * size_t(a.p.rows) * size_t(a.q.rows) * sizeof(float)));
+      if (!a.part) return int64_t(0);
+    }
+    return plan_tiles(a, ceil_div(a.p.rows, kT4), ceil_div(a.q.rows, kT4), splits, 32);
+  };
+  LargeGradsArgs l = {g.dx, g.dw_in, 0, 0};
+  l.n_dx = int(plan(l.dx, p.s_dx));
+  l.n_dw = l.n_dx ? int(plan(l.dw, p.s_dw)) : 0;
+  const bool have = l.n_dx && l.n_dw;
+  if (have) linear_grads_large_kernel<<<unsigned(l.n_dx + l.n_dw), 256, kLargeLds, st>>>(l);
+  for (TileArgs* a : {&l.dx, &l.dw}) {
+    if (!a->part) continue;
+    const int64_t n = int64_t(a->p.rows) * a->q.rows;
+    if (have) tile_join_kernel<<<unsigned(std::min<int64_t>(ceil_div(n, int64_t(1024)), 4096)), 256, 0, st>>>(*a, int(ceil_div(a->K, a->k_split)));
+    xdna_hip_cache_free(a->part);  // stream-ordered reuse: the block's next user runs after the join
+  }
+  return have;
+}
+
 // Large tiles where they give every CU one and fill the rounds that they take.  Measured, large
 // and wide tiles in us: 8192 x 512 -> 1024 units (256 tiles) 27 and 34, 8192 x 1024 -> 4096 158 and
 // 192; but 8192 x 512 -> 1024's gradient (128 tiles) 37 and 27, 4800 x 1024 -> 2048 (1.2 rounds) 64
@@ -1433,6 +1537,17 @@ const char* linear_fault(int64_t M, int64_t K, int64_t N) {
 int64_t linear_parts(int64_t M, int64_t N) {
   if (M <= 0) return 0;
   return std::max<int64_t>(1, std::min(ceil_div(int64_t(1024), ceil_div(N, int64_t(256))), ceil_div(M, int64_t(8))));
+}
+
+// How dx and dw are best made: 0 apart, 1 together on small tiles, 2 together on large ones.
+int grads_how(const GradsArgs& g) {
+  const int64_t M = g.dx.q.rows, K = g.dx.p.rows, N = g.dx.K;
+  const bool dma = K % 8 == 0 && N % 8 == 0 && dma_ok(g.dx.p, K, N, true) && dma_ok(g.dx.q, M, N, false) && dma_ok(g.dw_in.p, K, M, true) &&
+                   dma_ok(g.dw_in.q, N, M, true);
+  const float together = std::min(grads_cost(false, M, K, N, 0, 0), grads_cost(true, M, K, N, 0, 0));
+  const float apart = choose_tiles(K, M, N, true).cost + choose_tiles(K, N, M, true).cost;
+  if (dma && plan_large_grads(M, K, N).cost < std::min(together, apart)) return 2;
+  return together < apart ? 1 : 0;
 }
 
 int launched(const char* what, bool ok) {
@@ -1598,10 +1713,10 @@ int xdna_linear_bwd_bf16(const uint16_t* dy, int64_t ld, const void* kept, int a
   return check_launch(what);
 }
 
-int xdna_linear_grads_pick(int64_t M, int64_t K, int64_t N) {
-  if (linear_fault(M, K, N) || M == 0 || N > kMaxRows) return 0;
-  const float apart = choose_tiles(K, M, N, true).cost + choose_tiles(K, N, M, true).cost;
-  return std::min(grads_cost(false, M, K, N, 0, 0), grads_cost(true, M, K, N, 0, 0)) < apart ? 1 : 0;
+int xdna_linear_grads_pick(const uint16_t* dp, int64_t lddp, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw,
+                           int64_t M, int64_t K, int64_t N) {
+  if (linear_fault(M, K, N) || M == 0 || N > kMaxRows || N * K > kMaxOutputs || M * K > kMaxOutputs) return 0;
+  return grads_how(input_grads(dp, M > 1 ? lddp : N, x, ldx, w, N > 1 ? ldw : K, M, K, N, nullptr, nullptr));
 }
 
 int xdna_linear_grads_bf16(const uint16_t* dp, int64_t lddp, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw,
@@ -1617,6 +1732,7 @@ int xdna_linear_grads_bf16(const uint16_t* dp, int64_t lddp, const uint16_t* x, 
   const GradsArgs g = input_grads(dp, M > 1 ? lddp : N, x, ldx, w, N > 1 ? ldw : K, M, K, N, dx, dw);
   const bool wide = grads_cost(true, M, K, N, 0, 0) < grads_cost(false, M, K, N, 0, 0);
   hipStream_t st = as_stream(stream);
+  if (grads_how(g) == 2) return launched(what, launch_grads_large(g, st));
   return launched(what, wide ? launch_grads<true>(g, st) : launch_grads<false>(g, st));
 }
 

@@ -604,8 +604,10 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
                 "linear backward");
       out[2] = db;
     }
-    if (want_x && want_w && M > 0 && xdna_linear_grads_pick(M, K, N) &&
-        (short_block(M, K, N, 0) || !(on_gemm(dp, w) || on_gemm(dp.t(), x)))) {
+    const int how = want_x && want_w && M > 0
+                        ? xdna_linear_grads_pick(p16(dp), row_stride(dp), p16(x), row_stride(x), p16(w), row_stride(w), M, K, N)
+                        : 0;
+    if (how == 2 || (how == 1 && (short_block(M, K, N, 0) || !(on_gemm(dp, w) || on_gemm(dp.t(), x))))) {
       at::Tensor dx = empty_xdna({M, K}, at::kBFloat16), dw = empty_xdna({N, K}, at::kBFloat16);
       check_abi(xdna_linear_grads_bf16(p16(dp), row_stride(dp), p16(x), row_stride(x), p16(w), row_stride(w), M, K, N, m16(dx),
                                        m16(dw), current_stream()),

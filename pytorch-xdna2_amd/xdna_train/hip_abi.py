@@ -172,7 +172,7 @@ SIGNATURES = {
     "xdna_linear_bwd_workspace_bytes": (Z, [L, L]),
     "xdna_linear_kept_bytes": (Z, [L, L, I]),
     "xdna_linear_bwd_bf16": (I, [P, L, P, I, L, L, P, P, P, Z, P]),
-    "xdna_linear_grads_pick": (I, [L, L, L]),
+    "xdna_linear_grads_pick": (I, [P, L, P, L, P, L, L, L, L]),
     "xdna_linear_grads_bf16": (I, [P, L, P, L, P, L, L, L, L, P, P, P]),
     "xdna_decay_workspace_bytes": (Z, [L] * 5),
     "xdna_decay_attention": (I, [PH, PH, PH] + [L] * 6 + [P, P, I, F, P, P, P, P, Z, P]),

@@ -296,6 +296,27 @@ def test_linear_large(T, M, K, N, act):
         close(got, *ref[name], name)
 
 
+@pytest.mark.parametrize("M,K,N,off,how", [(8191, 520, 1032, 0, 2), (5056, 1024, 448, 0, 2), (5056, 1024, 448, 8, 2), (5056, 1024, 448, 1, 0),
+                                           (2500, 2048, 2048, 0, 1), (6001, 768, 1536, 0, 2), (6001, 1024, 1536, 0, 2)])
+def test_linear_gradients_in_one_launch_of_large_tiles(T, hip, M, K, N, off, how):
+    """Both products' 256 x 256 tiles together, whole or with either's k in splits; operands that are slices (``off``),
+    of which those off the 16-byte grid go elsewhere."""
+    print("linear large gradients", M, K, N, off, flush=True)
+    g = gen(M + off)
+    x, w = torch.randn(M, K, generator=g).to(BF16), (torch.randn(N, K, generator=g) / math.sqrt(K)).to(BF16)
+    dy = torch.randn(M, N, generator=g).to(BF16)
+    cut = lambda t: torch.nn.functional.pad(t, (off, 8)).to("xdna")[:, off:off + t.shape[1]] if off else t.to("xdna")  # noqa: E731
+    lv = [cut(x).detach().requires_grad_(), cut(w).detach().requires_grad_()]
+    d = cut(dy)
+    assert (hip.xdna_linear_grads_pick(d.data_ptr(), d.stride(0), lv[0].data_ptr(), lv[0].stride(0), lv[1].data_ptr(), lv[1].stride(0), M, K, N) == 2) == (how == 2)
+    dx, dw = torch.autograd.grad(T.linear(*lv), lv, d)
+    ref = linear_reference(x, w, None, None, dy, "none")
+    close(dx, *ref["dx"], "dx")
+    close(dw, *ref["dw"], "dw")
+    again = torch.autograd.grad(T.linear(*lv), lv, d)
+    assert same(again[0], dx) and same(again[1], dw)
+
+
 @pytest.mark.parametrize("M,K,N", [(3, 40, 24), (70, 129, 65), (700, 264, 512)])
 def test_linear_strides_and_parts_of_the_gradient(T, M, K, N):
     print("linear strides", M, K, N, flush=True)

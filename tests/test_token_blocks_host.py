@@ -71,7 +71,13 @@ def test_linear_refuses_bad_arguments():
     for kw, why in [({"dp": None}, "null"), ({"dx": None}, "null"), ({"dw": None}, "null"), ({"M": 0}, "no rows"), ({"lddp": 3}, "overlap"),
                     ({"ldx": 7}, "overlap"), ({"ldw": 7}, "overlap"), ({"K": 0}, "sizes"), ({"dw": A + 1}, "misaligned")]:
         assert refused(grads(**kw), why), (kw, hip_abi.last_error())
-    assert lib.xdna_linear_grads_pick(0, 8, 8) == 0 and lib.xdna_linear_grads_pick(333, 1000, 1367) == 1
+
+    def pick(M, K, N, at=A, ld=0):
+        return lib.xdna_linear_grads_pick(at, ld or N, at, ld or K, at, ld or K, M, K, N)
+
+    assert pick(0, 8, 8) == 0 and pick(333, 1000, 1367) == 1 and pick(8192, 1024, 4096) == 2
+    assert pick(8192, 1024, 4096, at=A + 2) != 2 and pick(8192, 1024, 4096, ld=4097) != 2  # (no whole vectors)
+    assert pick(8192, 1024, 4096, ld=1 << 20) != 2  # (offsets past 32 bits)
 
 
 def test_decay_attention_refuses_bad_arguments():
