@@ -792,17 +792,18 @@ __global__ __launch_bounds__(Tile<WIDE>::NT, WIDE ? 2 : 4) void grads_kernel(Gra
   }
 }
 
-// out[q][p] = the partials of the k splits, added in order, four outputs a thread (eight splits'
+// out[q][p] = the partials of the k splits, added in order, four outputs a thread (Z splits'
 // loads in flight)
+template <int Z>
 __global__ __launch_bounds__(256) void tile_join_kernel(TileArgs a, int splits) {
   const int64_t n = int64_t(a.q.rows) * a.p.rows;
   for (int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4; i < n; i += int64_t(gridDim.x) * 1024) {
     float d[4] = {};
     const int m = int(n - i < 4 ? n - i : 4);
-    for (int z = 0; z < splits; z += 8) {
-      Floats4 v[8];
+    for (int z = 0; z < splits; z += Z) {
+      Floats4 v[Z];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+      for (int u = 0; u < Z; ++u) {
         const float* p = a.part + int64_t(min(z + u, splits - 1)) * n + i;
         if (m == 4) {
           v[u] = *reinterpret_cast<const Floats4*>(p);
@@ -812,7 +813,7 @@ __global__ __launch_bounds__(256) void tile_join_kernel(TileArgs a, int splits) 
         }
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < Z; ++u)
         if (z + u < splits) d[0] += v[u].v[0], d[1] += v[u].v[1], d[2] += v[u].v[2], d[3] += v[u].v[3];
     }
     if (a.ldc == a.p.rows && m == 4) {
@@ -1289,6 +1290,14 @@ bool launch_few(TileArgs a, hipStream_t st) {
   return true;
 }
 
+void launch_join(const TileArgs& a, int splits, hipStream_t st) {
+  const int64_t n = int64_t(a.q.rows) * a.p.rows;
+  const unsigned grid = unsigned(std::min<int64_t>(ceil_div(n, int64_t(1024)), 4096));
+  if (splits <= 2) tile_join_kernel<2><<<grid, 256, 0, st>>>(a, splits);
+  else if (splits <= 4) tile_join_kernel<4><<<grid, 256, 0, st>>>(a, splits);
+  else tile_join_kernel<8><<<grid, 256, 0, st>>>(a, splits);
+}
+
 // k split over the grid into `splits` parts, joined by a second launch
 template <bool WIDE, bool PROWS, bool QROWS, int EPI>
 bool launch_split(TileArgs a, dim3 tiles, int64_t splits, hipStream_t st) {
@@ -1302,7 +1311,7 @@ bool launch_split(TileArgs a, dim3 tiles, int64_t splits, hipStream_t st) {
   if (ok && EPI == kLinear)
     linear_join_kernel<<<unsigned(std::min<int64_t>(ceil_div(int64_t(a.q.rows) * ceil_div(a.p.rows, 8), int64_t(256)), 4096)), 256, 0, st>>>(
         a, int(tiles.z));
-  else if (ok) tile_join_kernel<<<unsigned(std::min<int64_t>(ceil_div(n, int64_t(1024)), 4096)), 256, 0, st>>>(a, int(tiles.z));
+  else if (ok) launch_join(a, int(tiles.z), st);
   xdna_hip_cache_free(a.part);  // stream-ordered reuse: the block's next user runs after the join
   return ok;
 }
@@ -1470,8 +1479,7 @@ bool launch_grads_large(GradsArgs g, hipStream_t st) {
   if (have) linear_grads_large_kernel<<<unsigned(l.n_dx + l.n_dw), 256, kLargeLds, st>>>(l);
   for (TileArgs* a : {&l.dx, &l.dw}) {
     if (!a->part) continue;
-    const int64_t n = int64_t(a->p.rows) * a->q.rows;
-    if (have) tile_join_kernel<<<unsigned(std::min<int64_t>(ceil_div(n, int64_t(1024)), 4096)), 256, 0, st>>>(*a, int(ceil_div(a->K, a->k_split)));
+    if (have) launch_join(*a, int(ceil_div(a->K, a->k_split)), st);
     xdna_hip_cache_free(a->part);  // stream-ordered reuse: the block's next user runs after the join
   }
   return have;
