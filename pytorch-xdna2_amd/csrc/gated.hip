@@ -17,8 +17,8 @@
 // down to 1.9e-9): what the backward multiplies dy by, without the activation again and within 2^-12,
 // where a slope in bf16 would be a second rounding as large as that of dy act'(v) itself.  ReLU's slopes are bits, four
 // units a byte: the layer's traffic beside its products is a fifth less.  8192 x 1024 -> 4096 with bias, ReLU and residual:
-// 104 us (0.66 PFLOP/s: two rounds of tiles, each its k-loop and then its 128 KB of outputs, residual and slopes), dy and
-// slopes to dp 27 (143 MB, 5.3 TB/s); 1 x 4096 -> 1024: 4.6.
+// 102 us (0.67 PFLOP/s: two rounds of tiles, each its k-loop and then its 128 KB of outputs, residual and slopes; 84 without
+// residual and slopes), dy and slopes to dp 26 (143 MB, 5.5 TB/s); 1 x 4096 -> 1024: 4.6.
 #include "common.h"
 #include "gemm_dma.h"
 #include "mfma.h"
@@ -1437,8 +1437,8 @@ bool launch_large(TileArgs a, dim3 tiles, hipStream_t st) {
 
 // dx and dw on large tiles in one launch: their splits, such that all workgroups are at work at once, by the launch's cost
 // in us.  Fitted to 8 sizes (3 % off at most): 0.87 a k-tile of the longest workgroup, and the split products' partials.
-// Measured, this launch, the tiles' best and the GEMM for each product: 8192 x 1024 -> 4096 132, 166 and 168; 8192 x 1024 -> 1024
-// 49, 65 and 175; 8192 x 512 -> 4096 91, 111 and 311; but 4096 x 1024 -> 4096 96, 83 and 107, 2048 x 1024 -> 2048 51, 31 and 131.
+// Measured, this launch, the tiles' best and the GEMM for each product: 8192 x 1024 -> 4096 126, 166 and 168; 8192 x 1024 -> 1024
+// 49, 64 and 174; 8192 x 512 -> 4096 85, 108 and 310; but 4096 x 1024 -> 4096 96, 83 and 107, 2048 x 1024 -> 2048 51, 31 and 131.
 struct LargeGrads {
   int64_t s_dx, s_dw;
   float cost;  // infinite: the tiles alone are more than the CUs
