@@ -157,8 +157,8 @@ struct Stream {
 
 // Rows sh .. 63 of a chunk (tokens c0 .. of the segment) into a tile, zeros in the rows before and behind d: by
 // 16-byte LDS DMA, W / 32 instructions of each of four waves.  The caller waits.
-//   A whole chunk of whole rows takes one instruction each and little else: the lane's offset in a block of rows is one of
-// two (lane_at[i % 2]), the blocks' and the chunks' are scalar.
+//   A whole chunk takes one instruction each and little else: the lane's offset in a block of rows is one of two (lane_at[i
+// % 2], out of range behind d), the blocks' and the chunks' are scalar.
 template <int W>
 struct Dma {
   static constexpr int P = W / 8, ROWS = 64 / P, N = W / 32;  // pieces of a row, rows of an instruction, instructions a wave
@@ -170,7 +170,7 @@ struct Dma {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = i * ROWS + lane / P, p = (lane % P) ^ swizzle<W>(r);
-      lane_at[i] = uint32_t(down ? ROWS - 1 - lane / P : lane / P) * bytes + uint32_t(p) * 16u;
+      lane_at[i] = p * 8 < x.d ? uint32_t(down ? ROWS - 1 - lane / P : lane / P) * bytes + uint32_t(p) * 16u : 0x7FFFFFF0u;
     }
   }
 
@@ -178,11 +178,14 @@ struct Dma {
     return uniform_rsrc(lds_dma_rsrc(x.first + (c0 + (down ? kC - 1 - sh : 0)) * x.step, 0x7FFFFFE0));
   }
 
-  // instruction i of wave `wave`, of a whole chunk
-  __device__ inline void load(const i32x4_t& rs, const uint16_t* tile, int wave, int i) const {
-    const int block = wave * N + i;
-    const uint32_t at = uint32_t(down ? kC - (block + 1) * ROWS : block * ROWS) * bytes;
-    lds_dma16_m0(rs, lds_addr(tile) + uint32_t(block) * 1024u, int(lane_at[i % 2]), at);
+  __device__ inline void load_whole(const Stream& x, int c0, const uint16_t* tile, int wave) const {
+    const i32x4_t rs = rows(x, c0, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int block = wave * N + i;
+      const uint32_t at = uint32_t(down ? kC - (block + 1) * ROWS : block * ROWS) * bytes;
+      lds_dma16_m0(rs, lds_addr(tile) + uint32_t(block) * 1024u, int(lane_at[i % 2]), at);
+    }
   }
 
   __device__ inline void load_some(const Stream& x, int c0, int sh, const uint16_t* tile, int lane, int wave) const {
@@ -258,9 +261,9 @@ struct Lds {  // two buffers each; of a segment's state by itself three, and non
 // worked on, and the state before a chunk is in LDS twice, so that a chunk has one barrier.  A chunk of n < 64 tokens
 // takes the tile's last n rows, its first ones are zeros: the weights inside a chunk, which go by differences and by the
 // distance to its end, are those of every other.
-//   A chunk takes 2.2 us with one workgroup a CU and 3.3 with two: VALU and MFMA a third of it each, LDS reads about as
-// much, a wave's products, scores and weights one after the other.  8 x 2048 tokens, 16 heads of 128: forward 75 us (256
-// workgroups, one a CU; 268 MB, 3.6 TB/s), backward 169 (three walks, 805 MB of rows, of which 647 come from memory: 3.8
+//   A chunk takes 2.0 us with one workgroup a CU and 3.2 with two: VALU and MFMA a third of it each, LDS reads about as
+// much, a wave's products, scores and weights one after the other.  8 x 2048 tokens, 16 heads of 128: forward 69 us (256
+// workgroups, one a CU; 268 MB, 3.9 TB/s), backward 165 (three walks, 805 MB of rows, of which 647 come from memory: 3.9
 // TB/s); 1 x 8192 tokens: the segments' states 21, their sums 6, the outputs 33.
 //   DMA: rows of k and v are whole 16-byte pieces.
 template <int KT, bool STATE, bool DMA>
@@ -328,12 +331,14 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
     const int vt = STATE ? wave : wave - 4;
     const Dma<KT> k_dma(kx, lane);
     const Dma<kVB> v_dma(vx, lane);
-    const bool whole = DMA && dk == KT && dv == kVB;
     Staged<KT> k_staged;
     Staged<kVB> v_staged;
     const auto load = [&](int c0, int b) {  // chunk c0 .. into buffer b, or the registers that go there
       const int sh = max(0, kC - (todo - c0));
-      if constexpr (DMA) {
+      if (DMA && sh == 0) {
+        k_dma.load_whole(kx, c0, ks + b * L::k, vt);
+        v_dma.load_whole(vx, c0, vs + b * L::v, vt);
+      } else if constexpr (DMA) {
         const int l = here(lane);
         k_dma.load_some(kx, c0, sh, ks + b * L::k, l, vt);
         v_dma.load_some(vx, c0, sh, vs + b * L::v, l, vt);
@@ -410,10 +415,9 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
       }
       __syncthreads();
       const int coming = c0 + (STATE ? 2 : 1) * kC, to = STATE ? (b == 0 ? 2 : b - 1) : b ^ 1;
-      const bool ahead = whole && coming + kC <= todo;  // a whole chunk: its loads go between the products
-      if (!ahead && coming < todo) load(coming, to);
-      i32x4_t k_rows, v_rows;
-      if (ahead) k_rows = k_dma.rows(kx, coming, 0), v_rows = v_dma.rows(vx, coming, 0);
+      // (at once: among the state's products they came later, and the forward of 8 x 2048 tokens, 16 heads of 128, took 76 us
+      // for 69, the backward 169 for 165)
+      if (coming < todo) load(coming, to);
       const uint32_t k_tr = here(k_at.tr + smem_at + uint32_t(b) * kBuf);
       const uint32_t v_tr = (v_at.tr ^ uint32_t(32 * vt)) + smem_at + BUFS * kBuf + uint32_t(b) * vBuf;
       constexpr uint32_t k16 = LaneAt<KT>::k16, v16 = LaneAt<kVB>::k16;
@@ -442,12 +446,6 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
           for (int x = 0; x < 4; ++x) {
             const uint32_t at = k_tr ^ uint32_t(32 * (x0 + x));
             k[x] = as_bf16x8(frag_tr(at + 2 * s * k16, at + (2 * s + 1) * k16));
-          }
-          if (ahead) {
-            constexpr int N = Dma<KT>::N;  // (2 N products' groups: a load of k each two, of v in the first two)
-            const int at = s * (NS / 4) + x0 / 4;
-            if (NS == 8 || at < N) k_dma.load(k_rows, ks + to * L::k, vt, at);
-            if (at < Dma<kVB>::N) v_dma.load(v_rows, vs + to * L::v, vt, at);
           }
 #pragma unroll
           for (int y = 2; y >= 0; --y)
