@@ -205,7 +205,7 @@ __device__ inline Pix8 window8(const uint16_t* row, int c, int d) { return *rein
 __device__ inline Pix8 to_place(const Pix8& v, int c, int d) { return c < d ? shifted(v, max(c + 8 - d, 0)) : Pix8{{0u, 0u, 0u, 0u}}; }
 
 // The same as Dma for rows of any length, stride and alignment, through registers: loaded before a chunk's work, written to
-// LDS behind it (one behind the other, the loads' way was in every chunk: heads of 127 took 271 us where 128 take 74).
+// LDS behind it (one behind the other, the loads' way was in every chunk: heads of 127 took 271 us for 135).
 template <int W>
 struct Staged {
   static constexpr int P = W / 8, N = W / 32;
@@ -261,10 +261,10 @@ struct Lds {  // two buffers each; of a segment's state by itself three, and non
 // worked on, and the state before a chunk is in LDS twice, so that a chunk has one barrier.  A chunk of n < 64 tokens
 // takes the tile's last n rows, its first ones are zeros: the weights inside a chunk, which go by differences and by the
 // distance to its end, are those of every other.
-//   A chunk takes 2.0 us with one workgroup a CU and 3.2 with two: VALU and MFMA a third of it each, LDS reads about as
+//   A chunk takes 2.0 us with one workgroup a CU and 3.2 with two: MFMA a quarter of it and VALU a third, LDS reads about as
 // much, a wave's products, scores and weights one after the other.  8 x 2048 tokens, 16 heads of 128: forward 69 us (256
-// workgroups, one a CU; 268 MB, 3.9 TB/s), backward 165 (three walks, 805 MB of rows, of which 647 come from memory: 3.9
-// TB/s); 1 x 8192 tokens: the segments' states 21, their sums 6, the outputs 33.
+// workgroups, one a CU; 268 MB, 3.9 TB/s), backward 165 (three walks, 805 MB of rows, of which 687 come from memory: 4.2
+// TB/s); 1 x 8192 tokens: the segments' states 20, their sums 6, the outputs 33.
 //   DMA: rows of k and v are whole 16-byte pieces.
 template <int KT, bool STATE, bool DMA>
 __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a) {
