@@ -781,7 +781,7 @@ int refuse(const char* what, const char* why) {
 
 constexpr int64_t kMaxTokens = int64_t(1) << 30;
 constexpr int64_t kMaxWalks = (int64_t(1) << 23) - 1;  // workgroups of a launch (512 threads: under 2^32 of them)
-constexpr int64_t kSplitWalks = 4096;                  // most workgroups whose sequences are cut into segments
+constexpr int64_t kSplitWalks = 256;                   // most workgroups whose sequences are cut into segments
 
 const char* sizes_fault(int64_t B, int64_t T, int64_t H, int64_t G, int64_t dk, int64_t dv) {
   if (B < 0 || B > (1 << 20) || T < 0 || T > kMaxTokens || H < 1 || H > (1 << 16)) return "batch, tokens or heads out of range";
@@ -805,7 +805,7 @@ Heads heads_of(const xdna_heads_bf16* h, int64_t share) { return {h->data, h->ba
 
 constexpr int kScanFrom = 5;  // segments from which on their states are summed up by a launch
 
-// Segments of a sequence, by what a call takes in us.  Fitted to 21 shapes (1 to 8 sequences of 300 to 32768 tokens, 2 to
+// Segments of a sequence, by what a call takes in us, where its workgroups are at most one a CU.  Fitted to 21 shapes (1 to 8 sequences of 300 to 32768 tokens, 2 to
 // 32 heads of 32, 64 or 128, both directions, whole and in 2 to 64 segments; 8 % off in the mean, the choice under 2 % slower
 // than the best in the mean and 15 % at most): a chunk takes 1.4 with few workgroups, 1.7 with one on each CU, and with two
 // 2.8 forward and 3.2 backward (three walks' rows from memory); of the segments' own states 0.43 a workgroup on a CU, at
@@ -828,7 +828,9 @@ Plan plan_segments(int64_t walks, int64_t states, float state_mb, int64_t T, boo
   const int64_t chunks = ceil_div(T, int64_t(kC));
   const float size = big ? 1.0f : 0.75f;
   Plan best = {1, int(std::max<int64_t>(chunks, 1))};
-  if (walks > kSplitWalks) return best;  // (the last round's gap is an eighth of the time at most, the states' pass a quarter)
+// (every CU has one: backward of 6 x 2048 tokens, 16 heads of 128, 130 us whole, 149 in 2 segments, 182 in 4; of 3 x 4096, 157,
+  // 169 and 170)
+  if (walks > kSplitWalks) return best;
   float least = 0.95f * walk_cost(walks, chunks, size, two);  // (cut for a gain beyond the fit's errors)
   for (int64_t n = 2; n <= std::min<int64_t>(chunks, 256); n += n < 64 ? 1 : 32) {
     const int64_t per = ceil_div(chunks, n), segments = ceil_div(chunks, per);

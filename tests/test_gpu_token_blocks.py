@@ -583,6 +583,25 @@ def test_decay_attention_of_many_heads_in_one_walk(T):
     check_decay(run_decay(T, v), decay_reference(v["q"], v["k"], v["v"], v["g"], v["state"], None, size[4] ** -0.5, v["dout"], v["dstate"]))
 
 
+def test_decay_attention_of_a_large_batch(T):
+    """2000 sequences, more rounds of workgroups than the chip holds at once: the bits of its parts' calls."""
+    Bn, Tn, H, dk, dv = 2000, 100, 4, 48, 44
+    g = gen(4)
+    part = {n: torch.randn(100, Tn, H, d, generator=g).to(BF16).to("xdna") for n, d in (("q", dk), ("k", dk), ("v", dv), ("dout", dv))}
+    log_decay = torch.tensor([-0.5, -0.1, -0.02, -0.004], device="xdna")
+
+    def run(v):
+        lv = [v[n].requires_grad_() for n in ("q", "k", "v")]
+        r = T.decay_attention(*lv, log_decay)
+        return [r.out.detach(), r.state.detach(), *torch.autograd.grad(r.out, lv, v["dout"])]
+
+    one = [t.cpu() for t in run({n: t.clone() for n, t in part.items()})]
+    whole = run({n: t.repeat(Bn // 100, 1, 1, 1) for n, t in part.items()})
+    for i, (a, b) in enumerate(zip(whole, one)):
+        for j in (0, 1, 10, Bn // 100 - 1):
+            assert same(a[100 * j:100 * j + 100], b), (i, j)
+
+
 def test_decay_attention_at_the_ends_of_the_decays(T):
     """Nothing forgotten (0), everything (-inf), and decays that underflow within a chunk."""
     v = decay_values(2, 200, 4, 4, 16, 24, seed=9)
