@@ -805,13 +805,13 @@ Heads heads_of(const xdna_heads_bf16* h, int64_t share) { return {h->data, h->ba
 
 constexpr int kScanFrom = 5;  // segments from which on their states are summed up by a launch
 
-// Segments of a sequence, by what a call takes in us, where its workgroups are at most one a CU.  Fitted to 21 shapes (1 to 8 sequences of 300 to 32768 tokens, 2 to
-// 32 heads of 32, 64 or 128, both directions, whole and in 2 to 64 segments; 8 % off in the mean, the choice under 2 % slower
-// than the best in the mean and 15 % at most): a chunk takes 1.4 with few workgroups, 1.7 with one on each CU, and with two
-// 2.8 forward and 3.2 backward (three walks' rows from memory); of the segments' own states 0.43 a workgroup on a CU, at
-// least 1.1; heads up to 64 three quarters of that; the states' sums 0.94 a MB.  1 x 8192 tokens, 16 heads of 128, forward:
-// 193 us whole, 60 in 8 segments, 56 in 16, 97 in 64; 4 x 5000, 4 heads of 64: 99, 32, 24 and 32; backward of 1 x 8192 199
-// whole, 113 in 8, 129 in 16.
+// Segments of a sequence, where its call has no workgroup for every CU, by what it takes in us.  Fitted to 21 shapes (1 to
+// 8 sequences of 300 to 32768 tokens, 2 to 32 heads of 32, 64 or 128, both directions, whole and in 2 to 64 segments; 8 % off
+// in the mean, the choice under 2 % slower than the best in the mean and 15 % at most): a chunk takes 1.4 with few
+// workgroups, 1.7 with one on each CU, and with two 2.8 forward and 3.2 backward (three walks' rows from memory); of the
+// segments' own states 0.43 a workgroup on a CU, at least 1.1; heads up to 64 three quarters of that; the states' sums 0.94 a
+// MB.  1 x 8192 tokens, 16 heads of 128, forward: 193 us whole, 60 in 8 segments, 56 in 16, 97 in 64; 4 x 5000, 4 heads of
+// 64: 99, 32, 24 and 32; backward of 1 x 8192 199 whole, 113 in 8, 129 in 16.
 struct Plan {
   int segments, chunks;
 };
@@ -828,8 +828,8 @@ Plan plan_segments(int64_t walks, int64_t states, float state_mb, int64_t T, boo
   const int64_t chunks = ceil_div(T, int64_t(kC));
   const float size = big ? 1.0f : 0.75f;
   Plan best = {1, int(std::max<int64_t>(chunks, 1))};
-// (every CU has one: backward of 6 x 2048 tokens, 16 heads of 128, 130 us whole, 149 in 2 segments, 182 in 4; of 3 x 4096, 157,
-  // 169 and 170)
+  // (every CU has one: backward of 6 x 2048 tokens, 16 heads of 128, 130 us whole, 149 in 2 segments, 182 in 4; of 3 x
+  // 4096, 157, 169 and 170)
   if (walks > kSplitWalks) return best;
   float least = 0.95f * walk_cost(walks, chunks, size, two);  // (cut for a gain beyond the fit's errors)
   for (int64_t n = 2; n <= std::min<int64_t>(chunks, 256); n += n < 64 ? 1 : 32) {
