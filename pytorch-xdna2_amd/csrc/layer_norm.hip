@@ -10,7 +10,11 @@
 // The norm is that of the sum as it is stored, so that the fused form gives the bits of an add
 // followed by a norm, and the backward pass has the same h.  Everything is fp32 between one load
 // and one rounding; the variance is summed from the differences to the mean (a row is in registers,
-// so the second pass costs no memory).  The gradients of w and b: a wave's rows add up in its
+// so the second pass costs no memory).  In the same pass the differences' own mean c is summed: what the
+// mean, a rounded sum and quotient, is off by (an ulp of a row far from zero is a large part of its
+// deviation, and a constant row's is all of it: rows of 1000 gave -0.02 at width 1000, of 1e6 -1).  The
+// differences are then s - m - c and the variance their squares' mean less c^2; what is kept for the
+// gradient is m + c, rounded.  The gradients of w and b: a wave's rows add up in its
 // lanes' registers, a workgroup's waves through LDS in wave order, the workgroups' partials by a
 // second launch in order: no atomics, equal inputs give equal bits.
 //
@@ -175,6 +179,12 @@ __device__ inline void row_sums(float (&v)[N], float* red, int& phase) {
   }
 }
 
+// 1 / sqrt(var + eps) from the mean square of differences that are all `off` too large
+__device__ inline float inverse_deviation(float square, float off, float eps) {
+  const float var = square - off * off;
+  return 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);  // (NaN stays NaN)
+}
+
 constexpr int kRowWaves = 4;  // waves of a workgroup where each has rows of its own
 
 // Forward.  WAVES waves share a row (1: each of a workgroup's four waves has its own rows), V
@@ -219,19 +229,20 @@ __global__ __launch_bounds__(64 * (WAVES == 1 ? kRowWaves : WAVES)) void fwd_ker
       for (int e = 0; e < 8; ++e) sums[0] += counts<EVEN>(win[j], e) ? v[j][e] : 0.0f;
     }
     row_sums<WAVES>(sums, red, phase);
-    const float mean = sums[0] * scale;
-    sums[0] = 0.0f;
+    const float mean = sums[0] / float(a.dim);
+    float dev[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[j][e] -= mean;
-        sums[0] += counts<EVEN>(win[j], e) ? v[j][e] * v[j][e] : 0.0f;
+        dev[0] += counts<EVEN>(win[j], e) ? v[j][e] : 0.0f;
+        dev[1] += counts<EVEN>(win[j], e) ? v[j][e] * v[j][e] : 0.0f;
       }
-    row_sums<WAVES>(sums, red, phase);
-    const float inv = 1.0f / sqrtf(sums[0] * scale + a.eps);
+    row_sums<WAVES>(dev, red, phase);
+    const float off = dev[0] * scale, inv = inverse_deviation(dev[1] * scale, off, a.eps);
     if (a.stats && lane == 0) {
-      a.stats[2 * r] = mean;
+      a.stats[2 * r] = mean + off;
       a.stats[2 * r + 1] = inv;
     }
 #pragma unroll
@@ -240,10 +251,10 @@ __global__ __launch_bounds__(64 * (WAVES == 1 ? kRowWaves : WAVES)) void fwd_ker
       if (a.weight) {
         unpack(load8<PT, EVEN>(a.weight, win[j]), w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] *= inv * w[e];
+        for (int e = 0; e < 8; ++e) v[j][e] = (v[j][e] - off) * (inv * w[e]);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] *= inv;
+        for (int e = 0; e < 8; ++e) v[j][e] = (v[j][e] - off) * inv;
       }
       if (a.bias) {
         unpack(load8<PT, EVEN>(a.bias, win[j]), b);
@@ -381,20 +392,21 @@ __global__ __launch_bounds__(1024) void long_fwd_kernel(NormArgs a) {
     }
     if (a.other) x = s;
     row_sums<16>(sums, red, phase);
-    const float mean = sums[0] * scale;
-    sums[0] = 0.0f;
+    const float mean = sums[0] / float(a.dim);
+    float dev[2] = {0.0f, 0.0f};
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
       const float v = to_f32(x[c]) - mean;
-      sums[0] += v * v;
+      dev[0] += v;
+      dev[1] += v * v;
     }
-    row_sums<16>(sums, red, phase);
-    const float inv = 1.0f / sqrtf(sums[0] * scale + a.eps);
+    row_sums<16>(dev, red, phase);
+    const float off = dev[0] * scale, inv = inverse_deviation(dev[1] * scale, off, a.eps);
     if (a.stats && threadIdx.x == 0) {
-      a.stats[2 * r] = mean;
+      a.stats[2 * r] = mean + off;
       a.stats[2 * r + 1] = inv;
     }
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
-      float v = (to_f32(x[c]) - mean) * inv;
+      float v = (to_f32(x[c]) - mean - off) * inv;
       if (a.weight) v *= to_f32(static_cast<const P*>(a.weight)[c]);
       if (a.bias) v += to_f32(static_cast<const P*>(a.bias)[c]);
       put(static_cast<T*>(a.out) + r * a.dim + c, v);

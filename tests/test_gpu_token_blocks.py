@@ -187,6 +187,54 @@ def test_layer_norm_of_special_rows(T):
     close(y[3:], *ref, "rows beside them")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("D", [7, 64, 515, 1000, 1160, 2047, 3000, 10000, 20011])
+def test_layer_norm_of_constant_rows(T, D, dtype):
+    """A constant row is zeros before the bias, whatever 1 / width rounds to, and gives the weight no gradient.  The mean is
+    off by n = 66 u of itself at most before it is corrected by the deviations' own mean, which is as exact of them: what is left
+    is (66 u)^2 of the row's value, over sqrt(eps)."""
+    print("layer norm of constant rows", D, dtype, flush=True)
+    at = torch.tensor([3.0, 1000.0, 1e6, -0.1, 1000.1, 0.0])[:, None].to(dtype)
+    x, dy = at.expand(6, D).contiguous(), torch.ones(6, D).to(dtype)
+    lv = [t.to("xdna").requires_grad_() for t in (x, torch.ones(D, dtype=dtype))]
+    y = T.layer_norm(*lv, torch.full((D,), 0.5, dtype=dtype, device="xdna"))
+    left = (66 * U) ** 2 * at.to(F64).abs() / math.sqrt(1e-5)
+    close(y, torch.full((6, D), 0.5, dtype=F64), (left + rounding(dtype)).expand(6, D), "y")
+    dx, dw = torch.autograd.grad(y, lv, dy.to("xdna"))
+    close(dw, torch.zeros(D, dtype=F64), float(left.sum()) + 1e-30, "dw")
+    # dx = inv (1 - mean(1) - h mean(h)): the mean of ones is within 66 u of one
+    close(dx, torch.zeros(6, D, dtype=F64), ((66 * U + left * left) / math.sqrt(1e-5)).expand(6, D), "dx")
+
+
+@pytest.mark.parametrize("at,spread", [(1000.0, 0.01), (-1e4, 1.0), (1e6, 30.0)])
+@pytest.mark.parametrize("D", [7, 515, 1000, 2047, 3000, 10000, 20011])
+def test_layer_norm_of_rows_far_from_zero(T, D, at, spread):
+    """fp32 rows whose spread is small against their mean.  x - mean is exact (within a factor of two); the correction leaves
+    it off by e = 66 u (mean |x - m| + 66 u |m|).  The squares' mean less the correction's square is off by 68 u of both, and
+    e adds its square.  The gradient takes the mean as it is kept, rounded: half an ulp, 2 u of it, more."""
+    print("layer norm far from zero", D, at, spread, flush=True)
+    g = gen(D)
+    x = (at + spread * torch.randn(4, D, generator=g)).to(F32)
+    dy = torch.randn(4, D, generator=g)
+    lv = [t.to("xdna").requires_grad_() for t in (x, torch.ones(D))]
+    y = T.layer_norm(*lv)
+    dx, dw = torch.autograd.grad(y, lv, dy.to("xdna"))
+    m, dy = x.to(F64).mean(1, keepdim=True), dy.to(F64)
+    d = x.to(F64) - m
+    inv = 1 / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-5)
+    h = d * inv
+    first = 66 * U * m.abs()
+    e = 66 * U * (d.abs().mean(1, keepdim=True) + first)
+    ei = 40 * U + 68 * U * (first * inv) ** 2 + (e * inv) ** 2
+    close(y, h, inv * (e + U * d.abs()) + (ei + 4 * U) * h.abs() + 1e-30, "y")
+    eh = inv * (e + 2 * U * m.abs() + U * d.abs()) + (ei + 2 * U) * h.abs()
+    mg, mh = dy.mean(1, keepdim=True), (dy * h).mean(1, keepdim=True)
+    emg, emh = 66 * U * dy.abs().mean(1, keepdim=True), 67 * U * (dy * h).abs().mean(1, keepdim=True) + (dy.abs() * eh).mean(1, keepdim=True)
+    want = inv * (dy - mg - h * mh)
+    close(dx, want, inv * (4 * U * (dy.abs() + mg.abs() + (h * mh).abs()) + emg + eh * mh.abs() + (h.abs() + eh) * emh) + (ei + 4 * U) * want.abs(), "dx")
+    close(dw, (dy * h).sum(0), (dy.abs() * eh).sum(0) + 6 * U * (dy * h).abs().sum(0) + 1e-30, "dw")
+
+
 def test_layer_norm_gradient_against_differences(T):
     g = gen(11)
     x, w, dy = torch.randn(3, 40, generator=g), 1 + 0.1 * torch.randn(40, generator=g), torch.randn(3, 40, generator=g)
