@@ -370,7 +370,17 @@ __global__ __launch_bounds__(64 * WAVES * GROUP) void bwd_kernel(NormArgs a) {
   }
 }
 
-// Rows past the register forms: a workgroup of 1024 threads a row, which it reads again for each pass.
+// Rows past the register forms: a workgroup of 1024 threads a row, which it reads again for each pass.  A thread adds up to
+// 16384 elements: compensated (Kahan), or squares that are alike put the variance 2e-4 off.
+struct Compensated {
+  float s = 0.0f, c = 0.0f;
+  __device__ inline void add(float v) {
+    const float y = v - c, t = s + y;
+    c = (t - s) - y;
+    s = t;
+  }
+};
+
 template <int DT, int PT>
 __global__ __launch_bounds__(1024) void long_fwd_kernel(NormArgs a) {
   typedef typename Elem<DT>::T T;
@@ -381,24 +391,25 @@ __global__ __launch_bounds__(1024) void long_fwd_kernel(NormArgs a) {
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + r * a.ldx;
     T* s = static_cast<T*>(a.sum) + r * a.dim;
-    float sums[1] = {0.0f};
+    Compensated sum, first, second;
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
       float v = to_f32(x[c]);
       if (a.other) {
         put(s + c, v + to_f32(static_cast<const T*>(a.other)[r * a.ldo + c]));  // (read again by this thread alone)
         v = to_f32(s[c]);
       }
-      sums[0] += v;
+      sum.add(v);
     }
     if (a.other) x = s;
+    float sums[1] = {sum.s};
     row_sums<16>(sums, red, phase);
     const float mean = sums[0] / float(a.dim);
-    float dev[2] = {0.0f, 0.0f};
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
       const float v = to_f32(x[c]) - mean;
-      dev[0] += v;
-      dev[1] += v * v;
+      first.add(v);
+      second.add(v * v);
     }
+    float dev[2] = {first.s, second.s};
     row_sums<16>(dev, red, phase);
     const float off = dev[0] * scale, inv = inverse_deviation(dev[1] * scale, off, a.eps);
     if (a.stats && threadIdx.x == 0) {
@@ -426,12 +437,13 @@ __global__ __launch_bounds__(1024) void long_dx_kernel(NormArgs a) {
     const T* dy = static_cast<const T*>(a.dy) + r * a.lddy;
     const float mean = a.stats[2 * r], inv = a.stats[2 * r + 1];
     const auto grad = [&](int c) { return to_f32(dy[c]) * (a.weight ? to_f32(static_cast<const P*>(a.weight)[c]) : 1.0f); };
-    float sums[2] = {0.0f, 0.0f};
+    Compensated first, second;
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
       const float g = grad(c);
-      sums[0] += g;
-      sums[1] += g * ((to_f32(x[c]) - mean) * inv);
+      first.add(g);
+      second.add(g * ((to_f32(x[c]) - mean) * inv));
     }
+    float sums[2] = {first.s, second.s};
     row_sums<16>(sums, red, phase);
     const float ma = sums[0] * scale, mh = sums[1] * scale;
     for (int c = threadIdx.x; c < a.dim; c += 1024) {

@@ -235,6 +235,23 @@ def test_layer_norm_of_rows_far_from_zero(T, D, at, spread):
     close(dw, (dy * h).sum(0), (dy.abs() * eh).sum(0) + 6 * U * (dy * h).abs().sum(0) + 1e-30, "dw")
 
 
+@pytest.mark.parametrize("add", [False, True], ids=["norm", "add"])
+@pytest.mark.parametrize("D", [(1 << 22) + 5, 1 << 24])
+def test_layer_norm_of_the_longest_rows(T, D, add):
+    """Squares and gradients that are alike: a thread's plain sum of 4096 or 16384 of them would round most additions the same
+    way.  The tolerance is that of every other row (norm_reference)."""
+    print("layer norm of the longest rows", D, add, flush=True)
+    g = gen(D)
+    x = torch.where(torch.rand(1, D, generator=g) < 0.5, 0.7, -0.7)
+    r, dy = torch.full((1, D), 0.125), torch.full((1, D), 0.7)
+    leaves = [t.to("xdna").requires_grad_() for t in ((x, r) if add else (x,))]
+    y, stored = (T.add_layer_norm(*leaves).norm, x + r) if add else (T.layer_norm(*leaves), x)
+    (dx,) = torch.autograd.grad(y, leaves[:1], dy.to("xdna"))
+    ref = norm_reference(stored, None, None, dy, None, 1e-5, F32, F32)
+    close(y, *ref["y"], "y")
+    close(dx, *ref["dx"], "dx")
+
+
 def test_layer_norm_gradient_against_differences(T):
     g = gen(11)
     x, w, dy = torch.randn(3, 40, generator=g), 1 + 0.1 * torch.randn(40, generator=g), torch.randn(3, 40, generator=g)
