@@ -252,6 +252,31 @@ def test_layer_norm_of_the_longest_rows(T, D, add):
     close(dx, *ref["dx"], "dx")
 
 
+MANY = [  # rows, width: more rows than the backward's launch has places for, in each of its forms
+    (9001, 1160), (4200, 2047), (600, 2049), (1100, 4099), (1030, 8192), (520, 16384), (130, 16400),
+]
+
+
+@pytest.mark.parametrize("types,add", [((BF16, BF16), True), ((BF16, F32), False), ((F32, F32), True)], ids=["bf16-add", "bf16-f32-norm", "f32-add"])
+@pytest.mark.parametrize("R,D", MANY)
+def test_layer_norm_of_several_rows_a_place(T, R, D, types, add):
+    """A wave or workgroup that takes one row after another: rows loaded ahead, sums in LDS in turn, the parameters' sums
+    over rows."""
+    test_layer_norm(T, R, D, add, types)
+
+
+@pytest.mark.parametrize("R,D", [(263001, 64), (65537 + 400, 2050), (65537 + 400, 9000), (65537 + 400, 16392)])
+def test_layer_norm_of_more_rows_than_a_launch(T, R, D):
+    """Rows past the grid's bound: those of the second turn have the bits of a small call."""
+    print("layer norm of many rows", R, D, flush=True)
+    part = torch.randn(331, D, generator=gen(D)).to(BF16).to("xdna")
+    with torch.no_grad():
+        y = T.layer_norm(part.repeat(R // 331 + 1, 1)[:R])
+        one = T.layer_norm(part).cpu()
+    for r0 in (0, R // 331 // 2 * 331, (R // 331 - 1) * 331):
+        assert same(y[r0:r0 + 331], one), r0
+
+
 def test_layer_norm_gradient_against_differences(T):
     g = gen(11)
     x, w, dy = torch.randn(3, 40, generator=g), 1 + 0.1 * torch.randn(40, generator=g), torch.randn(3, 40, generator=g)
