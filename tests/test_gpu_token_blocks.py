@@ -386,6 +386,27 @@ def test_linear_large(T, M, K, N, act):
         close(got, *ref[name], name)
 
 
+@pytest.mark.parametrize("M,K,N,act", [(8192, 72, 3001, "relu"), (8200, 64, 3002, "silu"), (8192, 136, 4093, "relu"), (8193, 64, 4093, "gelu"), (8192, 64, 3002, "relu"),
+                                       (8192, 72, 3001, "none"), (8192, 64, 4099, "gelu")])
+def test_linear_large_of_odd_units(T, M, K, N, act):
+    """256 x 256 tiles whose units are no whole vectors: outputs, slopes and ReLU's rows of bits at odd places, parts of
+    vectors at the rows' ends, bias and residual at any alignment."""
+    print("linear large, odd units", M, K, N, act, flush=True)
+    tiles = -(-M // 256) * -(-N // 256)
+    assert tiles >= 256 and 100 * tiles >= 65 * 256 * -(-tiles // 256) and K % 8 == 0
+    g = gen(M + N)
+    x, w = torch.randn(M, K, generator=g).to(BF16), (torch.randn(N, K, generator=g) / math.sqrt(K)).to(BF16)
+    b, r, dy = torch.randn(N, generator=g).to(BF16), torch.randn(M, N, generator=g).to(BF16), torch.randn(M, N, generator=g).to(BF16)
+    bx = padded(b[None], 0, 3)[0]
+    lv = [x.to("xdna").requires_grad_(), w.to("xdna").requires_grad_(), bx.requires_grad_()]
+    ref = linear_reference(x, w, b, r, dy, act)
+    y = T.linear(*lv, act, padded(r, 4, 5))
+    for got, name in zip((y, *torch.autograd.grad(y, lv, padded(dy, 1, 1))), ("y", "dx", "dw", "db")):
+        close(got, *ref[name], name)
+    with torch.no_grad():
+        assert same(T.linear(*lv, act, padded(r, 0, 1)), y)
+
+
 @pytest.mark.parametrize("M,K,N,off,how", [(8191, 520, 1032, 0, 2), (5056, 1024, 448, 0, 2), (5056, 1024, 448, 8, 2), (5056, 1024, 448, 1, 0),
                                            (2500, 2048, 2048, 0, 1), (6001, 768, 1536, 0, 2), (6001, 1024, 1536, 0, 2)])
 def test_linear_gradients_in_one_launch_of_large_tiles(T, hip, M, K, N, off, how):
