@@ -741,6 +741,33 @@ def test_decay_attention_of_a_token_that_is_not_finite(T, name, bad):
     assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("size", [(1, 2, 3, 3, 64, 64), (2, 5, 3, 1, 128, 128), (1, 64, 3, 3, 33, 70), (1, 1000, 3, 3, 128, 64)])
+def test_decay_attention_keeps_states_in_24_bits(T, size):
+    """The weighted v of the state's sum has 24 bits.  Each sequence has one token that counts, so that every element of the
+    state is one product: exp(g n) is off by (2 |g n| + 2) u, its product with v by u, the three parts' sum by 4 u, and what
+    carries it to the end by 2 u a chunk: 16 u with |g n| at most 1 and two chunks.  (Parts of 16 bits would be off by up to 128
+    u, over 16 u in half of the elements.)  The gradient's sum for the state is the same walk."""
+    print("decay state's bits", size, flush=True)
+    Bn, Tn, H, G, dk, dv = size
+    v = decay_values(*size, seed=40)
+    v["g"] = -torch.tensor([0.05, 0.3, 0.9])
+    counts = max(0, Tn - 2)  # the forward's: a token before the last
+    far = torch.arange(Tn) != counts
+    kk, state = v["k"].clone(), torch.zeros(Bn, H, dk, dv)
+    kk[:, far] = 0.0
+    leaf = state.to("xdna").requires_grad_()
+    r = T.decay_attention(v["q"].to("xdna"), kk.to("xdna"), v["v"].to("xdna"), v["g"].to("xdna"), leaf, scale=1.0)
+    heads = lambda t: t.to(F64).repeat_interleave(H // t.shape[1], 1)  # noqa: E731
+    a = torch.exp(v["g"].to(F64) * (Tn - 1 - counts))[:, None, None]
+    want = a * heads(kk[:, counts])[..., :, None] * heads(v["v"][:, counts])[..., None, :]
+    close(r.state, want, 16 * U * want.abs() + 1e-30, "state")
+    dout = v["dout"].clone()
+    dout[:, 1:] = 0.0  # the backward's: the first token, decayed once
+    (d,) = torch.autograd.grad(r.out, [leaf], dout.to("xdna"))
+    want = torch.exp(v["g"].to(F64))[:, None, None] * v["q"][:, 0].to(F64)[..., :, None] * dout[:, 0].to(F64)[..., None, :]
+    close(d, want, 16 * U * want.abs() + 1e-30, "dstate")
+
+
 def test_decay_attention_of_slices_and_broadcast_heads(T):
     Bn, Tn, H, G, dk, dv = 2, 150, 4, 2, 24, 40
     v = decay_values(Bn, Tn, H, G, dk, dv, seed=10)
