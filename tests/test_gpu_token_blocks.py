@@ -1175,6 +1175,45 @@ def test_captured_attention_follows_lengths_and_slots(T):
     graph.reset()
 
 
+def test_captured_steps_leave_the_pool_like_eager_ones(T):
+    """A decoding step as a graph, after a prompt whose states it goes on with: the pool behind each replay has the bits of as
+    many eager steps, in the slots that are named and in the others."""
+    Bn, heads, head = 3, 2, 32
+    v = {n: t.to("xdna") for n, t in decay_values(Bn, 200, heads, heads, head, head, seed=41).items()}
+    start = torch.randn(5, heads, head, head, generator=gen(42))
+    pool, slots = start.to("xdna"), torch.tensor([4, 0, 2], device="xdna")
+    qkv = [v[n][:, 0].clone() for n in ("q", "k", "v")]
+
+    def step():
+        return T.decay_attention_step(*qkv, v["g"], pool, slots)
+
+    def begin():
+        pool.copy_(start)
+        pool[:2].copy_(T.decay_attention(v["q"], v["k"], v["v"], v["g"], v["state"]).state[:2])
+
+    with torch.no_grad():
+        begin()
+        eager = []
+        for i in range(4):
+            for t, n in zip(qkv, ("q", "k", "v")):
+                t.copy_(v[n][:, i])
+            eager.append((step().cpu(), pool.cpu()))
+        graph = torch.xdna.Graph()
+        with torch.xdna.graph(graph):
+            out = step()
+        for _ in range(2):
+            begin()
+            for i in range(4):
+                for t, n in zip(qkv, ("q", "k", "v")):
+                    t.copy_(v[n][:, i])
+                torch.xdna.synchronize()
+                graph.replay()
+                torch.xdna.synchronize()
+                assert same(out, eager[i][0]) and same(pool, eager[i][1]), i
+                assert same(pool[1], eager[0][1][1]) and same(pool[3], start[3])
+    graph.reset()
+
+
 def test_refusals_on_the_device(T):
     x, w = torch.randn(3, 8, device="xdna"), torch.ones(8, device="xdna")
     for call, why in [
