@@ -59,7 +59,6 @@ struct Walk {
 
 struct DecayArgs {
   Walk walk[3];
-  int n;       // walks
   int blocks;  // workgroups of all walks along their dv
   int B, T, H;
   const float* log_decay;
@@ -879,7 +878,6 @@ bool launch_walks(const DecayArgs& a, hipStream_t st) {
 template <bool STATE>
 bool launch(DecayArgs a, const Walk* walks, int n, hipStream_t st) {
   bool big = false, dma = true;
-  a.n = n;
   a.blocks = 0;
   for (int i = 0; i < n; ++i) {
     Walk& w = a.walk[i] = walks[i];
