@@ -932,9 +932,9 @@ size_t xdna_linear_kept_bytes(int64_t M, int64_t N, int act);
 int xdna_linear_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t M, int64_t K, int64_t N, int act,
                      const uint16_t* bias, const uint16_t* residual, int64_t ldr, uint16_t* y, void* kept, void* stream);
 
-/* dp = dy act'(v) (M x N, dense, or NULL) from the kept slopes (not read with act 3), and d_bias (N, or NULL) = its
- * column sums before that rounding, fp32 in a fixed order.  dx = dp w and dw = dp^T x are plain products,
- * or one launch: _pick says 1 for tiles of 64 or 128 (a few hundred rows), 2 for tiles of 256 (thousands; it then is the
+/* dp = dy act'(v) (M x N, dense, or NULL) from the kept slopes (not read with act 3; relu's select: 0 where the
+ * unit is off, whatever dy is), and d_bias (N, or NULL) = its column sums before that rounding, fp32 in a fixed
+ * order.  dx = dp w and dw = dp^T x are plain products, or one launch: _pick says 1 for tiles of 64 or 128 (a few hundred rows), 2 for tiles of 256 (thousands; it then is the
  * faster way at any rate), 0 for products apart. */
 size_t xdna_linear_bwd_workspace_bytes(int64_t M, int64_t N);
 int xdna_linear_bwd_bf16(const uint16_t* dy, int64_t ld, const void* kept, int act, int64_t M, int64_t N, uint16_t* dp,

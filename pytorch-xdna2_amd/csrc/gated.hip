@@ -16,7 +16,7 @@
 // training it keeps the slope act'(v) as an fp16 times 2^15 (2 bytes a unit, 11 bits of mantissa
 // down to 1.9e-9): what the backward multiplies dy by, without the activation again and within 2^-12,
 // where a slope in bf16 would be a second rounding as large as that of dy act'(v) itself.  ReLU's slopes are bits, four
-// units a byte: the layer's traffic beside its products is a fifth less.  8192 x 1024 -> 4096 with bias, ReLU and residual:
+// units a byte, by which its gradient is selected (0 at a unit that is off, whatever comes in): the layer's traffic beside its products is a fifth less.  8192 x 1024 -> 4096 with bias, ReLU and residual:
 // 102 us (0.67 PFLOP/s: two rounds of tiles, each its k-loop and then its 128 KB of outputs, residual and slopes; 84 without
 // residual and slopes), dy and slopes to dp 26 (143 MB, 5.5 TB/s); 1 x 4096 -> 1024: 4.6.
 #include "common.h"
@@ -383,8 +383,9 @@ __device__ inline LinearOut<N> linear_out(int act, const float (&v)[N], const fl
   if (act == kNone || act == kRelu) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      o.bits |= v[e] > 0.0f ? 1u << e : 0u;
-      o.y[e] = (act == kRelu ? act_of<kRelu>(v[e]) : v[e]) + r[e];
+      const bool off = v[e] <= 0.0f;  // (a NaN is not: it passes value and gradient, as through the other fused ReLUs)
+      o.bits |= off ? 0u : 1u << e;
+      o.y[e] = (act == kRelu && off ? 0.0f : v[e]) + r[e];
     }
   } else {
 #pragma unroll
@@ -904,9 +905,9 @@ __global__ __launch_bounds__(256) void linear_bwd_kernel(LinearBwdArgs a) {
         if (q >= a.M) break;
         float g[8];
         unpack8(d[u], g);
-        if (a.bits) {  // (a product with the slope 0, as the others': NaN and infinities stay)
+        if (a.bits) {  // (selected: a unit that is off has gradient 0, whatever dy is there)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) g[e] *= (bits[u] >> e) & 1u ? 1.0f : 0.0f;
+          for (int e = 0; e < 8; ++e) g[e] = (bits[u] >> e) & 1u ? g[e] : 0.0f;
         } else if (a.kept) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)

@@ -123,7 +123,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     """``act(x @ weight.T + bias) + residual`` in one kernel: ``x`` [..., K], ``weight`` [N, K],
     ``bias`` [N], ``residual`` [..., N], all bf16 (rows of any stride); ``activation`` "none",
     "silu", "gelu" (with erf) or "relu".  fp32 from the product to the one rounding.  For the backward
-    the activation's slopes are kept in 16 bits (11 of mantissa), ReLU's as bits."""
+    the activation's slopes are kept in 16 bits (11 of mantissa), ReLU's as bits: its gradient is 0 where
+    a unit is off, whatever comes in, and passes a NaN, as ``torch.relu``'s."""
     return _dev.native().token_linear(x, weight, bias, residual, _choice(_LINEAR_ACTIVATIONS, activation, "activation"))
 
 

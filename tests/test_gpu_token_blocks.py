@@ -482,6 +482,30 @@ def test_linear_slopes_keep_the_lower_tail(T):
         assert abs(float(dw[0, 1]) - M * s) <= (2 * B + 2.0 ** -10) * abs(M * s)
 
 
+@pytest.mark.parametrize("M,K,N", [(3, 8, 24), (70, 129, 65), (700, 264, 512), (8192, 72, 3001)])
+def test_linear_relu_selects_its_gradient(T, M, K, N):
+    """As torch.relu's: a unit that is off has gradient 0 whatever comes in, infinities and NaN too, and a unit whose sum is
+    NaN passes it.  Whole numbers: every sum is exact, the results are the reference's roundings."""
+    print("linear relu selects", M, K, N, flush=True)
+    g = gen(M)
+    x, w = torch.zeros(M, K), torch.zeros(N, K)
+    x[:, 0], w[:, 0] = torch.where(torch.rand(M, generator=g) < 0.5, 1.0, -1.0), 1.0
+    x[0, 0], x[1, 0], x[M - 1, 0] = 1.0, -1.0, math.nan
+    on = ~(x[:, :1] <= 0)
+    dy = torch.randint(-8, 9, (M, N), generator=g).float()
+    p = torch.where(on, dy, 0.0)
+    bad = torch.tensor([math.inf, -math.inf, math.nan])[torch.randint(0, 3, (M, N), generator=g)]
+    dy = torch.where(~on & (torch.rand(M, N, generator=g) < 0.5), bad, dy)
+    assert not dy.isfinite().all()
+    lv = [t.to(BF16).to("xdna").requires_grad_() for t in (x, w, torch.zeros(N))]
+    y = T.linear(*lv, "relu")
+    assert (y[:-1].cpu() == on[:-1]).all() and y[-1].cpu().isnan().all()
+    dx, dw, db = (t.cpu() for t in torch.autograd.grad(y, lv, dy.to(BF16).to("xdna")))
+    assert torch.equal(db, p.sum(0).to(BF16))
+    assert torch.equal(dx, (p @ w).to(BF16))
+    assert not dw[:, 1:].any() and dw[:, 0].isnan().all()
+
+
 def test_linear_gradient_against_differences(T):
     g = gen(5)
     x, w, b, dy = (torch.randn(*s, generator=g).to(BF16) for s in ((6, 24), (10, 24), (10,), (6, 10)))
