@@ -151,7 +151,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     (each as large an error as that of ``out``'s own rounding).  ``q``, ``k``, ``v`` and ``state`` have
     gradients; those of shared heads are summed in fp32 before their one rounding.  A token whose ``k`` or
     ``v`` is not finite makes its own and the later outputs of its sequence so, and may make those of up to 63 tokens
-    before it NaN (chunks of 64 tokens are multiplied whole, the later tokens with weights of 0)."""
+    before it NaN (chunks of 64 tokens are multiplied whole, the later tokens with weights of 0); the gradient of ``q`` likewise.
+    A ``q`` or gradient of ``out`` that is not finite makes the gradients of ``k`` and ``v`` of its own and the earlier tokens
+    so, and may make those of up to 63 tokens behind it NaN."""
     return DecayAttention(*_dev.native().token_decay(q, k, v, log_decay, state, lengths, _scale(q, scale)))
 
 

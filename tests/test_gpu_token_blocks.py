@@ -765,6 +765,33 @@ def test_decay_attention_of_a_token_that_is_not_finite(T, name, bad):
     assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("name", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_decay_gradients_of_a_token_that_is_not_finite(T, name, bad):
+    """k and v go forwards (out and dq of their own and the later tokens), q and out's gradient backwards (dk and dv of their
+    own and the earlier ones, and the first state's): those are not finite, and of the tokens on the other side at most 63.  What
+    a token's own row alone enters is bad there alone, and everything else keeps its bits."""
+    size, s = (2, 300, 3, 3, 32, 40), 170
+    v = decay_values(*size, seed=3)
+    v["g"] = torch.tensor([-0.01, -0.1, -0.02])
+    call = lambda: {n: t.detach().cpu() for n, t in run_decay(T, v).items()}  # noqa: E731
+    clean = call()
+    v[name][1, s, 1] = bad
+    got = call()
+    forwards, backwards = (slice(s, None), slice(s - 63, None)), (slice(None, s + 1), slice(None, s + 64))
+    own = (slice(s, s + 1), slice(s, s + 1))
+    reach = {"q": {"out": own, "dk": backwards, "dv": backwards}, "k": {"out": forwards, "dq": forwards, "dv": own},
+             "v": {"out": forwards, "dq": forwards, "dk": own}, "dout": {"dq": own, "dk": backwards, "dv": backwards}}[name]
+    for n, (must, may) in reach.items():
+        assert not got[n][1, must, 1].isfinite().any(), n
+        got[n][1, may, 1] = clean[n][1, may, 1]
+    for n in (["state"] if name in "kv" else ["dstate"]):
+        assert not got[n][1, 1].isfinite().any(), n
+        got[n][1, 1] = clean[n][1, 1]
+    for n in got:
+        assert torch.equal(got[n], clean[n]), n
+
+
 @pytest.mark.parametrize("size", [(1, 2, 3, 3, 64, 64), (2, 5, 3, 1, 128, 128), (1, 64, 3, 3, 33, 70), (1, 1000, 3, 3, 128, 64)])
 def test_decay_attention_keeps_states_in_24_bits(T, size):
     """The weighted v of the state's sum has 24 bits.  Each sequence has one token that counts, so that every element of the
