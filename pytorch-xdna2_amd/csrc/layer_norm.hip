@@ -19,9 +19,9 @@
 // second launch in order: no atomics, equal inputs give equal bits.
 //
 // Bound by HBM.  A row is held in registers: by one wave up to 2048 elements, by four waves up to
-// 8192, by sixteen up to 16384; longer rows are read again for each pass.  65536 rows of 2048 in bf16: forward 112 us
-// (537 MB, 4.8 TB/s), backward 173 (805 MB, 4.7) and 5.5 for the partials' sums; 8192 x 1024 with the residual sum: 15, 17
-// and 4; one row of 1024: 3.
+// 8192, by sixteen up to 16384; longer rows are read again for each pass.  65536 rows of 2048 in bf16: forward 106 us
+// (537 MB, 5.1 TB/s), backward 165 (805 MB, 4.9) and 5 for the partials' sums; 8192 x 1024 with the residual sum: 15, 16
+// and 4; one row of 1024: 3.1; 4099 x 515 in fp32: 7.8 (2.2 TB/s), 10.4 (2.4) and 3.9.
 #include "common.h"
 
 #include "../../include/xdna_hip.h"
