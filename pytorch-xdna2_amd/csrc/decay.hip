@@ -17,10 +17,11 @@
 // that q and k take are a^i and a^(n-j) in place of a^(i+1) and a^(n-1-j) (`lead` 0 for 1).
 //
 // A workgroup walks one sequence, head and 64 columns of v, the state in its registers
-// in fp32.  Rounded to bf16 are the weighted scores and the state as an operand of q S (one rounding
-// each beside the result's own: error against 64 bits 1.4 times that of the result's rounding);
-// the weighted v of the state's own sum is carried in three bf16 (24 bits), since the state is fp32
-// (two leave it 2.8e-6 off).
+// in fp32.  Rounded to bf16 is the state as an operand of q S (one rounding beside the result's own:
+// error against 64 bits 1.25 times that of the result's rounding in training batches, 1.4 where nearly all
+// comes from the state); the weighted scores go in two bf16 parts (one put sequences of a few tokens, whose rows share
+// a few roundings, up to 1.8 times as far off; the second's products cost 1.5 % of a training batch), and the weighted v of
+// the state's own sum in three (24 bits), since the state is fp32 (two leave it 2.8e-6 off).
 #include "common.h"
 #include "mfma.h"
 
@@ -261,9 +262,9 @@ struct Lds {  // two buffers each; of a segment's state by itself three, and non
 // takes the tile's last n rows, its first ones are zeros: the weights inside a chunk, which go by differences and by the
 // distance to its end, are those of every other.
 //   A chunk takes 2.0 us with one workgroup a CU and 3.2 with two: MFMA a quarter of it and VALU a third, LDS reads about as
-// much, a wave's products, scores and weights one after the other.  8 x 2048 tokens, 16 heads of 128: forward 72 us (256
-// workgroups, one a CU; 268 MB, 3.7 TB/s), backward 162 (three walks, 805 MB of rows, 490 MB read from memory and 197
-// written: 4.2 TB/s); 1 x 8192 tokens: the segments' states 20, their sums 7, the outputs 32.
+// much, a wave's products, scores and weights one after the other.  8 x 2048 tokens, 16 heads of 128: forward 73 us (256
+// workgroups, one a CU; 268 MB, 3.7 TB/s), backward 166 (three walks, 805 MB of rows, 490 MB read from memory and 197
+// written: 4.1 TB/s); 1 x 8192 tokens: the segments' states 20, their sums 7, the outputs 33.
 //   DMA: rows of k and v are whole 16-byte pieces.
 template <int KT, bool STATE, bool DMA>
 __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a) {
@@ -544,23 +545,32 @@ __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a)
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) p[1] = mfma(frag_row((k_s ^ uint32_t(64 * kk)) + k16), frag(qf[kk]), p[1]);
           }
-          uint32_t pw[4] = {0u, 0u, 0u, 0u};
+          uint32_t pw[2][4] = {};  // the weighted scores and what their rounding to bf16 left
           const auto scores = [&](int y, int apart) {  // `apart` tiles before the wave's own
             const float f = apart == 3 ? a32 : apart == 2 ? a16 : 1.0f;
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = p[y][i] * (apart == 0 ? diag[i] : off[i] * f);
-            pw[2 * y] = pack2(x[0], x[1]);
-            pw[2 * y + 1] = pack2(x[2], x[3]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t hi = pack2(x[2 * i], x[2 * i + 1]);
+              pw[0][2 * y + i] = hi;
+              pw[1][2 * y + i] = pack2(x[2 * i] - __uint_as_float(hi << 16), x[2 * i + 1] - __uint_as_float(hi & 0xFFFF0000u));
+            }
           };
           scores(0, wave - 2 * s);
           if (two) scores(1, wave - 2 * s - 1);
           if (2 * s + 2 > wave && c0 + kC < todo) load_q(c0 + kC);  // (after q's last use: the next chunk's into its registers)
-          const bf16x8_t pf = as_bf16x8(u32x4_t{pw[0], pw[1], pw[2], pw[3]});
           const uint32_t v_s = v_tr + uint32_t(s) * (2 * v16);
+          bf16x8_t vf[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            o[j] = mfma(as_bf16x8(frag_tr(v_s ^ uint32_t(32 * j), (v_s ^ uint32_t(32 * j)) + v16)), pf, o[j]);
+          for (int j = 0; j < 4; ++j) vf[j] = as_bf16x8(frag_tr(v_s ^ uint32_t(32 * j), (v_s ^ uint32_t(32 * j)) + v16));
+#pragma unroll
+          for (int y = 1; y >= 0; --y) {
+            const bf16x8_t pf = as_bf16x8(u32x4_t{pw[y][0], pw[y][1], pw[y][2], pw[y][3]});
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = mfma(vf[j], pf, o[j]);
+          }
         }
       }
       if (row >= sh) {

@@ -150,8 +150,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     tokens: what lies behind a sequence's end is not read, its ``out`` and gradients are 0.  ``scale`` defaults
     to ``dk ** -0.5``.
 
-    The state is fp32; the weighted scores, and the state where ``q`` multiplies it, are rounded to bf16
-    (each as large an error as that of ``out``'s own rounding).  ``q``, ``k``, ``v`` and ``state`` have
+    The state is fp32; where ``q`` multiplies it, it is rounded to bf16 (at most as large an error as that of
+    ``out``'s own rounding); the weighted scores have 16 bits.  ``q``, ``k``, ``v`` and ``state`` have
     gradients; those of shared heads are summed in fp32 before their one rounding.  A token whose ``k`` or
     ``v`` is not finite makes its own and the later outputs of its sequence so, and may make those of up to 63 tokens
     before it NaN (chunks of 64 tokens are multiplied whole, the later tokens with weights of 0); the gradient of ``q`` likewise.

@@ -819,6 +819,32 @@ def test_decay_attention_keeps_states_in_24_bits(T, size):
     close(d, want, 16 * U * want.abs() + 1e-30, "dstate")
 
 
+@pytest.mark.parametrize("size", [(1, 1, 2, 2, 32, 32), (3, 2, 4, 4, 128, 128), (2, 4, 2, 1, 32, 32), (1, 20, 2, 2, 7, 3), (3, 22, 1, 1, 32, 64), (1, 40, 2, 2, 100, 72),
+                                  (2, 64, 3, 3, 128, 128)])
+def test_decay_attention_keeps_scores_in_16_bits(T, size):
+    """A chunk alone, without a state before it: nothing but the weighted scores is rounded before the result, and they have
+    two bf16: 2^-18 of each.  (One rounding to 8 bits, b, put sequences of a few tokens 1.8 times as far off as the result's own.)"""
+    print("decay score's bits", size, flush=True)
+    Bn, Tn, H, G, dk, dv = size
+    v = decay_values(*size, seed=50, state=False)
+    got = run_decay(T, v, scale=0.4)
+    want = {n: (torch.zeros(v[m].shape, dtype=F64), torch.zeros(v[m].shape, dtype=F64)) for n, m in (("out", "dout"), ("dq", "q"), ("dk", "k"), ("dv", "v"))}
+    zero, rev, u = torch.zeros(dk, dv, dtype=F64), lambda t: t.flip(0), (Tn + 640) * U + 2.0 ** -18
+    for b in range(Bn):
+        for h in range(H):
+            j = h // (H // G)
+            qh, kh, vh, do = (v[n][b, :, i].to(F64) for n, i in (("q", h), ("k", j), ("v", j), ("dout", h)))
+            for n, (x, y, z), s, i, turn in (("out", (qh, kh, vh), zero, h, False), ("dq", (do, vh, kh), zero.t(), h, False), ("dv", (kh, qh, do), zero, j, True),
+                                             ("dk", (vh, do, qh), zero.t(), j, True)):
+                x, y, z = (rev(t) if turn else t for t in (x, y, z))
+                (o, _), _ = walk(x, y, z, v["g"][h].to(F64), s, 0 if turn else 1, 0.4, 0.4, 1.0)
+                (mag, _), _ = walk(x.abs(), y.abs(), z.abs(), v["g"][h].to(F64), s, 0 if turn else 1, 0.4, 0.4, 1.0)
+                want[n][0][b, :, i] += rev(o) if turn else o
+                want[n][1][b, :, i] += u * (rev(mag) if turn else mag)
+    for n, (o, e) in want.items():
+        close(got[n], o, e + B * o.abs() + 1e-30, n)
+
+
 def test_decay_attention_of_slices_and_broadcast_heads(T):
     Bn, Tn, H, G, dk, dv = 2, 150, 4, 2, 24, 40
     v = decay_values(Bn, Tn, H, G, dk, dv, seed=10)
