@@ -927,15 +927,18 @@ int xdna_layer_norm_bwd(const void* dy, int64_t lddy, const void* dsum, int64_t 
  * erf, 2 relu, 3 none; bias (N values) and residual (rows of N) may be NULL.  fp32 to the one rounding.
  * kept (xdna_linear_kept_bytes, or NULL; not with act 3): the slopes act'(v), for the gradient: 2^15 times them
  * as fp16 (M x N), of relu as bits (M rows of (N + 3) / 4 bytes, four units a byte).  Where k is split, the fp32
- * partials come from the library's caching allocator.  M up to 2^22. */
+ * partials come from the library's caching allocator, whose blocks are reused in the order of the calls: calls on
+ * streams that can overlap race for them.  M up to 2^22. */
 size_t xdna_linear_kept_bytes(int64_t M, int64_t N, int act);
 int xdna_linear_bf16(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t M, int64_t K, int64_t N, int act,
                      const uint16_t* bias, const uint16_t* residual, int64_t ldr, uint16_t* y, void* kept, void* stream);
 
 /* dp = dy act'(v) (M x N, dense, or NULL) from the kept slopes (not read with act 3; relu's select: 0 where the
  * unit is off, whatever dy is), and d_bias (N, or NULL) = its column sums before that rounding, fp32 in a fixed
- * order.  dx = dp w and dw = dp^T x are plain products, or one launch: _pick says 1 for tiles of 64 or 128 (a few hundred rows), 2 for tiles of 256 (thousands; it then is the
- * faster way at any rate), 0 for products apart. */
+ * order.  dx = dp w and dw = dp^T x are plain products, or one launch: _pick says 1 for tiles of 64 or 128 (a few
+ * hundred rows), 2 for tiles of 256 (thousands; it then is the faster way at any rate), 0 for products apart.
+ * _grads' split products' partials come from the library's caching allocator too: calls on streams that can
+ * overlap race for them. */
 size_t xdna_linear_bwd_workspace_bytes(int64_t M, int64_t N);
 int xdna_linear_bwd_bf16(const uint16_t* dy, int64_t ld, const void* kept, int act, int64_t M, int64_t N, uint16_t* dp,
                          uint16_t* d_bias, void* workspace, size_t workspace_bytes, void* stream);

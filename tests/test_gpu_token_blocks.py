@@ -1330,6 +1330,22 @@ def test_refusals_on_the_device(T):
         torch.autograd.grad(r.out.sum(), [leaf], create_graph=True)
 
 
+def test_work_on_another_stream_is_refused(T):
+    """The device's allocator orders its blocks on one stream: a call on a stream beside it raises, and writes nothing."""
+    x, w = torch.randn(40, 64, device="xdna").bfloat16(), torch.ones(64, 64, device="xdna", dtype=BF16)
+    q, g = torch.zeros(2, 5, 2, 8, device="xdna", dtype=BF16), torch.zeros(2, device="xdna")
+    state = torch.ones(2, 2, 8, 8, device="xdna")
+    before = T.linear(x, w)
+    torch.xdna.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for call in (lambda: T.layer_norm(x), lambda: T.add_layer_norm(x, x), lambda: T.linear(x, w), lambda: T.decay_attention(q, q, q, g, state),
+                     lambda: T.decay_attention_step(q[:, 0], q[:, 0], q[:, 0], g, state)):
+            with pytest.raises(RuntimeError, match="default one is not supported"):
+                call()
+    torch.cuda.synchronize()
+    assert same(T.linear(x, w), before) and (state.cpu() == 1).all()
+
+
 def test_forward_mode_is_refused(T):
     import torch.autograd.forward_ad as fw
 
