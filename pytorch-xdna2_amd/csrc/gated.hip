@@ -14,11 +14,12 @@
 //
 // The linear layer y = act(x W^T + b) + r runs on the same tiles with an epilogue of its own.  For
 // training it keeps the slope act'(v) as an fp16 times 2^15 (2 bytes a unit, 11 bits of mantissa
-// down to 1.9e-9): what the backward multiplies dy by, without the activation again and within 2^-12,
+// down to 1.9e-9): what the backward multiplies dy by, without the activation again and within 2^-11,
 // where a slope in bf16 would be a second rounding as large as that of dy act'(v) itself.  ReLU's slopes are bits, four
-// units a byte, by which its gradient is selected (0 at a unit that is off, whatever comes in): the layer's traffic beside its products is a fifth less.  8192 x 1024 -> 4096 with bias, ReLU and residual:
-// 102 us (0.67 PFLOP/s: two rounds of tiles, each its k-loop and then its 128 KB of outputs, residual and slopes; 84 without
-// residual and slopes), dy and slopes to dp 26 (143 MB, 5.5 TB/s); 1 x 4096 -> 1024: 4.6.
+// units a byte, by which its gradient is selected (0 at a unit that is off, whatever comes in): the layer's traffic beside its
+// products is a fifth less.  8192 x 1024 -> 4096 with bias, ReLU and residual: 96 us in a training pass (0.72 PFLOP/s: two
+// rounds of tiles, each its k-loop and then its 128 KB of outputs, residual and slopes), 90 in a loop of its own and 84
+// there without residual and slopes; dy and slopes to dp 25 (143 MB, 5.6 TB/s); 1 x 4096 -> 1024: 4.6.
 #include "common.h"
 #include "gemm_dma.h"
 #include "mfma.h"

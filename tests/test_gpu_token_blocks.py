@@ -506,6 +506,29 @@ def test_linear_relu_selects_its_gradient(T, M, K, N):
     assert not dw[:, 1:].any() and dw[:, 0].isnan().all()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,K,N", [(2, 1, 700), (4, 5, 453)])
+def test_linear_bias_gradient_that_cancels(T, M, K, N, act):
+    """Few rows whose terms of d_bias nearly cancel: what is left shows the kept slopes' rounding, half a step of fp16: 2^-11 of a
+    slope.  Beside it the sum's error times act'' (at most 0.8), the activation's own arithmetic (32 u) and the sums over rows."""
+    print("linear bias gradient that cancels", M, K, N, act, flush=True)
+    g = gen(M * K * N)
+    x, w = torch.randn(M, K, generator=g).to(BF16), (torch.randn(N, K, generator=g) / math.sqrt(K)).to(BF16)
+    b = torch.randn(N, generator=g).to(BF16)
+    v = x.to(F64) @ w.to(F64).t() + b.to(F64)
+    ev = (K + 8) * U * (x.to(F64).abs() @ w.to(F64).abs().t() + b.to(F64).abs())
+    s = act64(act, v)[1]
+    dy = torch.ones(M, N)
+    dy[-1] = -(s[:-1].sum(0) / s[-1]).clamp(-8, 8)  # the last row takes the others' terms away
+    dy = dy.to(BF16)
+    bx = b.to("xdna").requires_grad_()
+    (db,) = torch.autograd.grad(T.linear(x.to("xdna"), w.to("xdna"), bx, act), [bx], dy.to("xdna"))
+    p = dy.to(F64) * s
+    ep = dy.to(F64).abs() * (0.8 * ev + 32 * U * (1 + v.abs()) + 2.0 ** -11 * s.abs() + 2.0 ** -40) + 2 * U * p.abs()
+    want = p.sum(0)
+    close(db, want, (ep + (M + 8) * U * p.abs()).sum(0) + B * want.abs(), "db")
+
+
 def test_linear_gradient_against_differences(T):
     g = gen(5)
     x, w, b, dy = (torch.randn(*s, generator=g).to(BF16) for s in ((6, 24), (10, 24), (10,), (6, 10)))
