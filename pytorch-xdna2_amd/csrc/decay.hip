@@ -261,10 +261,10 @@ struct Lds {  // two buffers each; of a segment's state by itself three, and non
 // worked on, and the state before a chunk is in LDS twice, so that a chunk has one barrier.  A chunk of n < 64 tokens
 // takes the tile's last n rows, its first ones are zeros: the weights inside a chunk, which go by differences and by the
 // distance to its end, are those of every other.
-//   A chunk takes 2.0 us with one workgroup a CU and 3.2 with two: MFMA a quarter to a third of it and VALU a third to two fifths, LDS reads about as
-// much, a wave's products, scores and weights one after the other.  8 x 2048 tokens, 16 heads of 128: forward 73 us (256
-// workgroups, one a CU; 268 MB, 3.7 TB/s), backward 166 (three walks, 805 MB of rows, 480 MB read from memory and 197
-// written: 4.1 TB/s); 1 x 8192 tokens: the segments' states 20, their sums 7, the outputs 33.
+//   A chunk takes 2.1 us with one workgroup a CU and 3.2 with two: MFMA a quarter to a third of it and VALU a third to two
+// fifths, LDS reads about as much, a wave's products, scores and weights one after the other.  8 x 2048 tokens, 16 heads of
+// 128: forward 73 us (256 workgroups, one a CU; 268 MB, 3.7 TB/s), backward 166 (three walks, 805 MB of rows, 480 MB read
+// from memory and 197 written: 4.1 TB/s); 1 x 8192 tokens: the segments' states 20, their sums 7, the outputs 33.
 //   DMA: rows of k and v are whole 16-byte pieces.
 template <int KT, bool STATE, bool DMA>
 __global__ __launch_bounds__(STATE ? 256 : 512, 4) void walk_kernel(DecayArgs a) {
